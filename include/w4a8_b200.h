@@ -245,6 +245,99 @@ W4A8_API int w4a8_linear_prepared_allreduce(const void* x, int64_t M, int64_t K,
                                             int32_t has_zero, int32_t act, void* y, void* workspace,
                                             size_t workspace_bytes, w4a8_ar* ar, void* stream);
 
+/* ---- residual addition + root-mean-square norm ----
+ *   h = x + residual (fp32; residual NULL: h = x), residual_out = bf16(h)
+ *   y = h / sqrt(sum(h^2) / K + eps) * weight    (fp32, rounded once to bf16)
+ * The step between a decoder layer's linears, which the reference leaves to its
+ * host framework; no counterpart in its operator surface.
+ *   x, residual, residual_out, y   bf16 [M, ld] (ld >= K); residual_out may be
+ *                                  NULL, and may be x or residual itself
+ *   weight                         [K] bf16 or f32 (weight_dtype)
+ * 1 <= K <= W4A8_NORM_MAX_K. */
+#define W4A8_NORM_MAX_K 32768
+W4A8_API int w4a8_rms_norm(const void* x, int64_t M, int64_t K, int64_t ldx, const void* residual, int64_t ldr,
+                           void* residual_out, int64_t ldro, const void* weight, int32_t weight_dtype, float eps,
+                           void* y, int64_t ldy, void* stream);
+/* The same norm with the output quantised by the activation quantiser's rule
+ * (w4a8_quant_act) from its fp32 values, without a rounding to bf16 between:
+ * a_q int8 [M, K], a_scale [G, M] bf16 or f32. */
+W4A8_API int w4a8_rms_norm_quant(const void* x, int64_t M, int64_t K, int64_t ldx, const void* residual, int64_t ldr,
+                                 void* residual_out, int64_t ldro, const void* weight, int32_t weight_dtype, float eps,
+                                 int32_t group_size, int8_t* a_q, void* a_scale, int32_t scale_dtype, void* stream);
+/* w4a8_linear_prepared on the norm's quantised output: the norm kernel writes
+ * codes and scales straight into the GEMM's operand tiles in the workspace
+ * (those of w4a8_rms_norm_quant), in place of the activation quantiser. */
+W4A8_API int w4a8_linear_prepared_rms_norm(const void* x, int64_t M, int64_t K, int64_t ldx, const void* residual,
+                                           int64_t ldr, void* residual_out, int64_t ldro, const void* weight,
+                                           int32_t weight_dtype, float eps, int64_t N, int32_t group_size,
+                                           const void* prepared, int32_t w_scale_dtype, int32_t has_zero, void* y,
+                                           int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- paged 8-bit key / value cache ----
+ * No counterpart in the reference (its serving stack keeps a bf16 cache).  One
+ * layer's cache: int8 codes [pages, kv_heads, page_size, head_dim] and one fp32
+ * scale per (page, kv head), for k and v each; value = code * scale.
+ * page_size 16, 32, 64 or 128; head_dim 64 or 128; codes 16-byte aligned.
+ *
+ * The batch arguments of the calls below:
+ *   page_table  int32 [batch, ld_table], table_cols columns in use: the page that
+ *               holds tokens [c * page_size, (c + 1) * page_size) of a sequence
+ *   kv_lens     int32 [batch]: tokens of each sequence in the cache, the call's
+ *               own included (at most table_cols * page_size count)
+ *   cu          int32 [batch + 1]: the call's tokens of sequence s are rows
+ *               [cu[s], cu[s + 1]), its LAST cu[s + 1] - cu[s] tokens
+ * They are read on the device, so a captured graph follows their contents.  A
+ * page id outside [0, pages) means "no page": its tokens are not written, not
+ * attended to and read as zeros.  Distinct sequences written by one call must
+ * not share a page that the call writes. */
+typedef struct w4a8_kv_cache {
+    void* k;
+    void* v;
+    void* k_scale;
+    void* v_scale;
+    int64_t pages;
+    int32_t kv_heads, page_size, head_dim, reserved;
+} w4a8_kv_cache;
+
+/* Writes k, v (bf16 [tokens, ld], kv_heads * head_dim used) of the call's tokens.
+ * A page's scale is max(its scale if it holds earlier tokens, max|new| / 127);
+ * where it grows, earlier codes become rint(code * (old / new)); new codes are
+ * rint(x / scale).  With cos_sin (f32 [table_rows, rot]: rot / 2 cosines, then
+ * rot / 2 sines for each position; rot a multiple of 16, at most head_dim) the
+ * first rot elements of every k head, and of every q head into q_out, are turned
+ * by the token's position (the first and second half of them pairwise, or
+ * neighbours with interleaved != 0); positions past the table use its last row.
+ * q (bf16 [tokens, ldq], q_heads * head_dim used) may be NULL, q_out may be q.
+ * Rows 16-byte aligned, leading dimensions multiples of 8. */
+W4A8_API int w4a8_kv_write(const w4a8_kv_cache* cache, const int32_t* page_table, int64_t ld_table,
+                           int64_t table_cols, const int32_t* kv_lens, const int32_t* cu_q, int64_t batch,
+                           int64_t tokens, const void* k, int64_t ldk, const void* v, int64_t ldv, const void* q,
+                           int64_t ldq, int32_t q_heads, void* q_out, int64_t ldqo, const float* cos_sin,
+                           int64_t table_rows, int32_t rot, int32_t interleaved, void* stream);
+/* Reads each sequence's last cu_out[s + 1] - cu_out[s] tokens back:
+ * k, v bf16 [tokens, kv_heads, head_dim] dense. */
+W4A8_API int w4a8_kv_read(const w4a8_kv_cache* cache, const int32_t* page_table, int64_t ld_table,
+                          int64_t table_cols, const int32_t* kv_lens, const int32_t* cu_out, int64_t batch,
+                          int64_t tokens, void* k, void* v, void* stream);
+
+/* ---- causal attention over the cache ----
+ * out[t, h] = sum_j softmax_j(softmax_scale * q[t, h] . k_j) v_j over the cached
+ * tokens j at or before query token t's position, k and v of kv head
+ * h / (q_heads / kv_heads); a row that sees no token is zero.  q, out bf16
+ * [tokens, ld] (q_heads * head_dim used; rows 16-byte aligned, ld a multiple of
+ * 8).  max_q_len: no sequence has more query tokens than that (rows past it
+ * are not computed).  batch <= W4A8_ATTENTION_MAX_BATCH.  Workspace as for the
+ * linear calls (w4a8_attention_workspace_size bytes, 1024-byte aligned, zeroed
+ * before first use, may be shared with them in stream order). */
+#define W4A8_ATTENTION_MAX_BATCH 2048
+W4A8_API size_t w4a8_attention_workspace_size(int64_t batch, int64_t tokens, int32_t q_heads, int32_t kv_heads,
+                                              int32_t head_dim, int32_t max_q_len);
+W4A8_API int w4a8_attention(const w4a8_kv_cache* cache, const int32_t* page_table, int64_t ld_table,
+                            int64_t table_cols, const int32_t* kv_lens, const int32_t* cu_q, int64_t batch,
+                            int64_t tokens, const void* q, int64_t ldq, int32_t q_heads, int32_t max_q_len,
+                            float softmax_scale, void* out, int64_t ldo, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
 /* ---- status ---- */
 /* Synchronises `stream` and returns the device status word of `workspace`
  * (0 = no kernel reported a failure; otherwise 0x100 + the id of the wait

@@ -1,0 +1,807 @@
+// w4a8_attention.cu -- causal attention over the paged 8-bit cache.
+//
+// For query token i of a sequence with n query tokens and L tokens in the
+// cache (these included), position p = L - n + i, and one kv head:
+//
+//   s_j = scale * ks(page of j) * (q . kc_j)        j <= p
+//   o   = sum_j exp(s_j - max s) * vs(page of j) * vc_j / sum_j exp(s_j - max s)
+//
+// kc, vc are the cache's int8 codes, ks, vs the page scales.  Codes enter the
+// tensor core as fp16, exactly; the page scales multiply scores and
+// probabilities in fp32, so a page costs one product per score and none per
+// element.  fp16 rather than bf16 for both products: a code takes three
+// instructions a pair instead of four to convert, and probabilities keep 11
+// bits instead of 8.  Its range is kept by powers of two, which are exact:
+//   * a query row is divided by 2^e with its largest element in [2^13, 2^14)
+//     before it becomes fp16 (8 significand bits fit; what falls below fp16's
+//     range is under 2^-28 of the row's largest element), and scores are
+//     multiplied by 2^e;
+//   * a probability enters as p * vs / vr * 2^14 with p <= 1 and vr a power of
+//     two, at least every vs so far (raised together with the running maximum),
+//     so weights down to 2^-28 of the largest possible keep all 11 bits.
+// Scores, running maximum and sum, and the output accumulate in fp32; the sum
+// is taken before the weights are rounded.  A row that sees no token is zero.
+//
+// Few query rows (kernel below): one pass over the cache, bound by HBM.
+//   * Work is cut in units of 16 tokens of one (sequence, kv head, row tile);
+//     a row tile is R = 8 * NT packed rows (query token x query head of the
+//     group).  All units of the call form one list; every warp of the grid
+//     takes an equal contiguous share, whatever the lengths are.  Lengths are
+//     read on the device, so a captured graph follows them.
+//   * A warp computes S^T = K Q^T and O^T += V^T P^T with m16n8k16: the cache
+//     is the 16-row operand, so 8 query rows fill an instruction and a single
+//     token's group of 5 or 8 heads wastes little.  It keeps O^T (D x R), the
+//     running maximum and its lanes' part of the sum in registers.
+//   * Units arrive by 16-byte asynchronous copies in a ring of its own, three
+//     deep: with 16 warps up to 128 KB are on the way to an SM.  Shared memory holds codes with
+//     16-byte chunks permuted by token, so fragment reads do not collide.
+//   * A warp's share begins and ends inside (sequence, head) segments.  Pieces
+//     of one segment are joined in the CTA, and across CTAs by a second small
+//     kernel, in unit order: no atomics, the same bits on every run.
+#include <cuda_fp16.h>
+
+#include "w4a8_common.cuh"
+#include "w4a8_kernels.h"
+
+namespace w4a8 {
+
+namespace {
+
+constexpr int kBlkTok = 16;        // tokens per unit
+constexpr int kStages = 3;         // units in a warp's ring
+constexpr int kMaxBatch = 2048;
+constexpr float kNegInf = -INFINITY;
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool ok)
+{
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(ok ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ uint4 lds128(uint32_t a)
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a)
+{
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ float lds32f(uint32_t a)
+{
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
+    return v;
+}
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x)
+{
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+// Two int8 codes in bytes 0 and 2 of w (bytes 1 and 3: anything) -> fp16 pair,
+// exactly: the bits 0x6400 | (code + 128) are the fp16 number 1024 + code + 128.
+__device__ __forceinline__ uint32_t codes_to_f16x2(uint32_t w)
+{
+    const uint32_t m = (w & 0x00FF00FFu) ^ 0x64806480u;
+    const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&m), __half2half2(__ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t*>(&d);
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi)
+{
+    const __half2 b = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&b);
+}
+
+// 2^-e for a row whose largest magnitude is m, m * 2^-e in [2^13, 2^14); 1 for a
+// zero or non-finite m.  e is held within what fp32 can scale by.
+__device__ __forceinline__ float row_shrink(float m)
+{
+    if (!(m > 0.0f) || m == INFINITY) return 1.0f;
+    const int e = static_cast<int>((__float_as_uint(m) >> 23) & 0xFFu) - 127 - 13;
+    return __uint_as_float(static_cast<uint32_t>(127 - min(max(e, -126), 126)) << 23);
+}
+
+// The smallest power of two at or above a positive finite v (at least 2^-100);
+// 1 for a non-finite v.
+__device__ __forceinline__ float pow2_above(float v)
+{
+    if (!(v < INFINITY)) return 1.0f;
+    const uint32_t b = __float_as_uint(fmaxf(v, 7.888609052210118e-31f));
+    return __uint_as_float((b & 0x7F800000u) + ((b & 0x007FFFFFu) ? 0x00800000u : 0u));
+}
+constexpr float kVrMin = 7.888609052210118e-31f;   // 2^-100
+constexpr float kWeightOne = 16384.0f;             // 2^14
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi)
+{
+    const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&b);
+}
+
+// ------------------------------------------------------------------ the batch
+
+// A sequence as the kernels see it, every value held within the tensors.
+struct Seq {
+    int q0, n;       // first query token and their number
+    int len;         // tokens in the cache
+};
+
+__device__ __forceinline__ Seq load_seq(const CacheView& c, int s)
+{
+    Seq r;
+    const int64_t a = min(static_cast<int64_t>(max(c.cu[s], 0)), c.tokens);
+    const int64_t b = min(static_cast<int64_t>(max(c.cu[s + 1], 0)), c.tokens);
+    r.q0 = static_cast<int>(a);
+    r.n = static_cast<int>(max(b - a, static_cast<int64_t>(0)));
+    r.len = static_cast<int>(min(static_cast<int64_t>(max(c.kv_lens[s], 0)),
+                                 static_cast<int64_t>(c.table_cols) << c.page_log2));
+    return r;
+}
+
+// Row tiles of a sequence, and 16-token blocks of each (at least one, so that
+// rows which see nothing are written too).
+__device__ __forceinline__ int seq_tiles(const Seq& s, int group, int rows) { return (s.n * group + rows - 1) / rows; }
+__device__ __forceinline__ int seq_blocks(const Seq& s) { return max(1, (s.len + kBlkTok - 1) / kBlkTok); }
+
+// ------------------------------------------------------------------ few rows
+
+template <int D_, int NT_>
+struct DecCfg {
+    static constexpr int D = D_, NT = NT_, R = 8 * NT_;
+    static constexpr int WARPS = NT_ == 1 ? 16 : 8;
+    static constexpr int THREADS = WARPS * 32;
+    static constexpr int KV_BYTES = kBlkTok * D_;                  // codes of K (or V) in a unit
+    static constexpr int STAGE = 2 * KV_BYTES + 16;                // + the page's two scales
+    static constexpr int RING = kStages * STAGE;                   // one warp's
+    static constexpr int PIECE = R * D_ * 4;                       // fp32 O of one piece
+    static constexpr int SLOT = RING > PIECE ? RING : PIECE;       // the ring's memory holds the last piece
+    static constexpr int SMEM = WARPS * SLOT;
+    static constexpr int CHUNKS = D_ / 16;                         // 16-byte chunks of a token's row
+};
+
+// Where chunk ch of token t is in shared memory: permuted so that the reads of
+// K (two neighbouring tokens x four chunks) and of V (tokens 2c x chunk) by the
+// eight lanes of a phase fall in different banks.
+template <int D>
+__device__ __forceinline__ uint32_t chunk_off(int t, int ch)
+{
+    if (D == 128) return t * 128 + ((ch ^ (t & 7)) << 4);
+    return t * 64 + ((ch ^ ((t >> 1) & 3)) << 4);
+}
+
+// One piece of a segment kept for the join: unit range and softmax state.
+struct PieceInfo {
+    long long seg;      // first unit of the segment; -1: none
+    int seq, head, tile, complete_lo, complete_hi;   // the piece reaches the segment's first / last unit
+};
+
+struct Partial {        // one per CTA and slot, in the workspace
+    long long seg;
+    int seq, head, tile, pad;
+};
+
+template <class C>
+struct Layout {
+    // workspace: [grid][2] Partial, then [grid][2] (m, l)[R], then [grid][2] O, then [grid * WARPS] stash (O, m, l)
+    static __host__ __device__ size_t info() { return 0; }
+    static __host__ __device__ size_t ml(int grid) { return static_cast<size_t>(grid) * 2 * sizeof(Partial); }
+    static __host__ __device__ size_t o(int grid) { return ml(grid) + static_cast<size_t>(grid) * 2 * 2 * C::R * 4; }
+    static __host__ __device__ size_t stash(int grid) { return o(grid) + static_cast<size_t>(grid) * 2 * C::PIECE; }
+    static __host__ __device__ size_t total(int grid)
+    {
+        return stash(grid) + static_cast<size_t>(grid) * C::WARPS * C::PIECE;
+    }
+};
+
+// The position of a warp in the unit list.
+template <class C>
+struct Cursor {
+    int seq, head, tile, blk, blocks;
+    Seq s;
+    __device__ __forceinline__ void set(const CacheView& c, int group, int sq, long long off)
+    {
+        seq = sq;
+        s = load_seq(c, sq);
+        blocks = seq_blocks(s);
+        const int tiles = seq_tiles(s, group, C::R);
+        const long long per_head = static_cast<long long>(tiles) * blocks;
+        head = static_cast<int>(off / per_head);
+        const long long r = off - head * per_head;
+        tile = static_cast<int>(r / blocks);
+        blk = static_cast<int>(r - static_cast<long long>(tile) * blocks);
+    }
+    // Next unit; false past the end of the list.
+    __device__ __forceinline__ bool next(const CacheView& c, int group)
+    {
+        if (++blk < blocks) return true;
+        blk = 0;
+        if (++tile < seq_tiles(s, group, C::R)) return true;
+        tile = 0;
+        if (++head < c.kv_heads) return true;
+        head = 0;
+        do {
+            if (++seq >= c.batch) return false;
+            s = load_seq(c, seq);
+        } while (s.n == 0);
+        blocks = seq_blocks(s);
+        return true;
+    }
+};
+
+// Writes rows of O^T that a warp holds: out[row] = acc / l for the valid rows.
+template <class C>
+__device__ __forceinline__ void store_rows(const AttentionParams& p, const Seq& s, int head, int tile,
+                                           const float (&acc)[C::NT][C::D / 16][4], const float (&l)[C::NT][2])
+{
+    const int r = lane_id() >> 2, c = lane_id() & 3;
+#pragma unroll
+    for (int nt = 0; nt < C::NT; ++nt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int row = tile * C::R + nt * 8 + 2 * c + h;
+            if (row >= s.n * p.group) continue;
+            const int tok = row / p.group, g = row - tok * p.group;
+            const float inv = l[nt][h] > 0.0f ? __fdiv_rn(1.0f, l[nt][h]) : (l[nt][h] == 0.0f ? 0.0f : l[nt][h]);
+            uint16_t* o = p.out + static_cast<int64_t>(s.q0 + tok) * p.ldo +
+                          static_cast<int64_t>(head * p.group + g) * C::D + r * (C::D / 8);
+            uint32_t w[C::D / 16];
+#pragma unroll
+            for (int i = 0; i < C::D / 16; ++i) w[i] = pack_bf16(acc[nt][i][h] * inv, acc[nt][i][2 + h] * inv);
+#pragma unroll
+            for (int i = 0; i < C::D / 16; i += 4)
+                *reinterpret_cast<uint4*>(o + 2 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+        }
+}
+
+template <class C>
+__global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const AttentionParams p)
+{
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ PieceInfo pieces[2 * C::WARPS];
+    __shared__ float piece_m[2 * C::WARPS][C::R], piece_l[2 * C::WARPS][C::R];
+    __shared__ long long warp_sum[C::WARPS];
+    __shared__ long long running;
+    long long* prefix = reinterpret_cast<long long*>(smem + C::SMEM);   // [batch + 1] units before each sequence
+
+    const int tid = threadIdx.x, warp = warp_id(), lane = lane_id();
+    const CacheView& cv = p.c;
+    if (tid < 2 * C::WARPS) pieces[tid].seg = -1;
+    if (tid == 0) running = 0;
+    pdl_wait();
+
+    // ---- units before each sequence ----
+    __syncthreads();
+    for (int base = 0; base < cv.batch; base += C::THREADS) {
+        const int s = base + tid;
+        long long u = 0;
+        if (s < cv.batch) {
+            const Seq q = load_seq(cv, s);
+            u = static_cast<long long>(cv.kv_heads) * seq_tiles(q, p.group, C::R) * seq_blocks(q);
+        }
+        long long x = u;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) warp_sum[warp] = x;
+        __syncthreads();
+        long long before = running;
+        for (int w = 0; w < warp; ++w) before += warp_sum[w];
+        if (s < cv.batch) prefix[s] = before + x - u;
+        __syncthreads();
+        if (tid == C::THREADS - 1) running = before + x;
+        __syncthreads();
+    }
+    const long long total = running;
+    // equal contiguous shares, at least one unit each: a list shorter than the
+    // grid leaves the last CTAs without work, none between working ones
+    const long long W = min(static_cast<long long>(gridDim.x) * C::WARPS, total);
+    const long long wk = static_cast<long long>(blockIdx.x) * C::WARPS + warp;
+    const long long u0 = wk < W ? total * wk / W : total, u1 = wk < W ? total * (wk + 1) / W : total;
+
+    float acc[C::NT][C::D / 16][4];
+    float m[C::NT][2], l[C::NT][2];
+    const int r = lane >> 2, c = lane & 3;
+    const uint32_t ring = smem_u32(smem + warp * C::SLOT);
+
+    if (u0 < u1) {
+        // last sequence whose first unit is at or before u0
+        int lo = 0, hi = cv.batch - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (prefix[mid] <= u0) lo = mid;
+            else hi = mid - 1;
+        }
+        Cursor<C> cur, pre;
+        cur.set(cv, p.group, lo, u0 - prefix[lo]);
+        pre = cur;
+        bool pre_ok = true;
+        long long pre_u = u0;
+
+        // Brings the unit under `pre` into ring stage st and moves on.
+        auto fetch = [&](int st) {
+            if (pre_u < u1 && pre_ok) {
+                const int tok = pre.blk * kBlkTok;
+                const int pg = tok >> cv.page_log2;
+                const int id = pg < cv.table_cols ? cv.table[static_cast<int64_t>(pre.seq) * cv.ld_table + pg] : -1;
+                const bool ok = id >= 0 && id < cv.pages && tok < pre.s.len;
+                const int64_t ph = ok ? static_cast<int64_t>(id) * cv.kv_heads + pre.head : 0;
+                const int64_t base = (ph << cv.page_log2) * C::D + static_cast<int64_t>(ok ? tok & (cv.page - 1) : 0) * C::D;
+                const uint32_t d = ring + st * C::STAGE;
+#pragma unroll
+                for (int i = 0; i < C::KV_BYTES / 512; ++i) {
+                    const int ch = i * 32 + lane;
+                    const uint32_t off = chunk_off<C::D>(ch / C::CHUNKS, ch % C::CHUNKS);
+                    cp_async16(d + off, cv.k + base + ch * 16, ok);
+                    cp_async16(d + C::KV_BYTES + off, cv.v + base + ch * 16, ok);
+                }
+                // a page that is not there has no tokens: its scale is marked with -1
+                if (lane < 2) {
+                    if (ok) cp_async4(d + 2 * C::KV_BYTES + lane * 4, (lane ? cv.v_scale : cv.k_scale) + ph, true);
+                    else asm volatile("st.shared.f32 [%0], %1;" ::"r"(d + 2 * C::KV_BYTES + lane * 4), "f"(-1.0f));
+                }
+                ++pre_u;
+                pre_ok = pre.next(cv, p.group);
+            }
+            cp_commit();
+        };
+
+#pragma unroll
+        for (int i = 0; i < kStages - 1; ++i) fetch(i);
+
+        uint32_t qf[C::NT][C::D / 16][2];
+        int limit[C::NT][2];
+        float qs[C::NT][2];
+        float vr = kVrMin;                        // power of two at or above every vs of the segment so far
+        float vr_inv = kWeightOne / kVrMin;       // 2^14 / vr
+        int min_limit = 0;
+        // Query rows of the segment under `cur`, and a fresh softmax state.
+        auto begin_segment = [&]() {
+            min_limit = 0x7FFFFFFF;
+            vr = kVrMin;
+            vr_inv = kWeightOne / kVrMin;
+#pragma unroll
+            for (int nt = 0; nt < C::NT; ++nt) {
+                const int row = cur.tile * C::R + nt * 8 + r;
+                const bool ok = row < cur.s.n * p.group;
+                const int tok = ok ? row / p.group : 0, g = ok ? row - tok * p.group : 0;
+                const uint16_t* q = p.q + static_cast<int64_t>(cur.s.q0 + tok) * p.ldq +
+                                    static_cast<int64_t>(cur.head * p.group + g) * C::D + c * (C::D / 4);
+                uint32_t big = 0;
+#pragma unroll
+                for (int i = 0; i < C::D / 32; ++i) {
+                    const uint4 v = ok ? *reinterpret_cast<const uint4*>(q + 8 * i) : make_uint4(0, 0, 0, 0);
+                    qf[nt][2 * i][0] = v.x;
+                    qf[nt][2 * i][1] = v.y;
+                    qf[nt][2 * i + 1][0] = v.z;
+                    qf[nt][2 * i + 1][1] = v.w;
+                }
+                // the row's largest magnitude, as bits: its elements are in the four lanes of r
+#pragma unroll
+                for (int i = 0; i < C::D / 16; ++i)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        big = max(big, max((qf[nt][i][e] << 16) & 0x7FFFFFFFu, qf[nt][i][e] & 0x7FFF0000u));
+                big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+                big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+                const float shrink = row_shrink(__uint_as_float(big));
+#pragma unroll
+                for (int i = 0; i < C::D / 16; ++i)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        qf[nt][i][e] = pack_f16(__uint_as_float(qf[nt][i][e] << 16) * shrink,
+                                                __uint_as_float(qf[nt][i][e] & 0xFFFF0000u) * shrink);
+                // scores of columns 2c, 2c + 1: their rows' factor lies with lanes r = 2c, 2c + 1
+                const float grow_back = __fdiv_rn(p.scale_log2, shrink);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) qs[nt][h] = __shfl_sync(0xffffffffu, grow_back, (2 * c + h) * 4);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int qr = cur.tile * C::R + nt * 8 + 2 * c + h;
+                    // rows past the sequence's last are computed on zero queries and not stored
+                    limit[nt][h] = qr < cur.s.n * p.group ? cur.s.len - cur.s.n + qr / p.group : 0x7FFFFFFF;
+                    min_limit = min(min_limit, limit[nt][h]);
+                    m[nt][h] = kNegInf;
+                    l[nt][h] = 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < C::D / 16; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[nt][i][e] = 0.0f;
+            }
+            min_limit = __reduce_min_sync(0xffffffffu, min_limit);
+        };
+
+        begin_segment();
+        long long seg_lo = u0 - cur.blk;          // first unit of the segment under `cur`
+        int piece_blk = cur.blk;                  // the piece's first block
+        int st = 0;
+        for (long long u = u0; u < u1; ++u) {
+            cp_wait<kStages - 2>();
+            __syncwarp();
+            fetch(st == 0 ? kStages - 1 : st - 1);     // the stage consumed in the previous pass
+            const uint32_t kb = ring + st * C::STAGE, vb = kb + C::KV_BYTES;
+            const float ks = lds32f(kb + 2 * C::KV_BYTES), vs = lds32f(kb + 2 * C::KV_BYTES + 4);
+            const int t0 = cur.blk * kBlkTok;
+            const bool there = ks >= 0.0f || ks != ks;   // NaN scales pass on; -1: no page
+
+            // ---- S^T = K Q^T ----
+            float sc[C::NT][4];
+#pragma unroll
+            for (int nt = 0; nt < C::NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[nt][e] = 0.0f;
+            uint32_t kw[2][C::D / 16];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < C::D / 64; ++i) {
+                    const uint4 v = lds128(kb + chunk_off<C::D>(r + 8 * t, c * (C::D / 64) + i));
+                    kw[t][4 * i] = v.x;
+                    kw[t][4 * i + 1] = v.y;
+                    kw[t][4 * i + 2] = v.z;
+                    kw[t][4 * i + 3] = v.w;
+                }
+#pragma unroll
+            for (int ks_ = 0; ks_ < C::D / 16; ++ks_) {
+                uint32_t a[4];
+                a[0] = codes_to_f16x2(__byte_perm(kw[0][ks_], 0, 0x4140));
+                a[1] = codes_to_f16x2(__byte_perm(kw[1][ks_], 0, 0x4140));
+                a[2] = codes_to_f16x2(__byte_perm(kw[0][ks_], 0, 0x4342));
+                a[3] = codes_to_f16x2(__byte_perm(kw[1][ks_], 0, 0x4342));
+#pragma unroll
+                for (int nt = 0; nt < C::NT; ++nt) mma_f16(sc[nt], a, qf[nt][ks_][0], qf[nt][ks_][1]);
+            }
+
+            // ---- running maximum ----
+            const bool edge = t0 + kBlkTok - 1 > min_limit || !there;
+            bool grow = vs > vr;
+#pragma unroll
+            for (int nt = 0; nt < C::NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    sc[nt][e] *= ks * qs[nt][e & 1];
+                    if (edge && (!there || t0 + r + (e >> 1) * 8 > limit[nt][e & 1])) sc[nt][e] = kNegInf;
+                    grow = grow || sc[nt][e] > m[nt][e & 1];
+                }
+            if (__any_sync(0xffffffffu, grow)) {
+                const float vn = fmaxf(vr, pow2_above(vs));
+                const float va = __fdiv_rn(vr, vn);
+                vr = vn;
+                vr_inv = __fdiv_rn(kWeightOne, vr);
+#pragma unroll
+                for (int nt = 0; nt < C::NT; ++nt)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float x = fmaxf(sc[nt][h], sc[nt][2 + h]);
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                        const float mn = fmaxf(m[nt][h], x);
+                        const float a = mn == kNegInf ? 1.0f : exp2f(m[nt][h] - mn);
+                        m[nt][h] = mn;
+                        l[nt][h] *= a;
+                        const float av = a * va;
+#pragma unroll
+                        for (int i = 0; i < C::D / 16; ++i) {
+                            acc[nt][i][h] *= av;
+                            acc[nt][i][2 + h] *= av;
+                        }
+                    }
+            }
+
+            // ---- P, its sum, and the weights P * vs / vr * 2^14 as the second product's operand ----
+            uint32_t pb[C::NT][2];
+            const float vw_ = vs * vr_inv;
+#pragma unroll
+            for (int nt = 0; nt < C::NT; ++nt) {
+                float e4[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float mm = m[nt][e & 1] == kNegInf ? 0.0f : m[nt][e & 1];
+                    const float x = exp2f(sc[nt][e] - mm);
+                    l[nt][e & 1] += x;
+                    e4[e] = edge && sc[nt][e] == kNegInf ? 0.0f : x * vw_;
+                }
+                pb[nt][0] = movmatrix_trans(pack_f16(e4[0], e4[1]));
+                pb[nt][1] = movmatrix_trans(pack_f16(e4[2], e4[3]));
+            }
+
+            // ---- O^T += V^T P^T ----
+            uint32_t vw[4][C::D / 32];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int tok = 2 * c + (t & 1) + (t >> 1) * 8;
+                if (C::D == 128) {
+                    const uint4 v = lds128(vb + chunk_off<C::D>(tok, r));
+                    vw[t][0] = v.x;
+                    vw[t][1] = v.y;
+                    vw[t][2 % (C::D / 32)] = v.z;
+                    vw[t][3 % (C::D / 32)] = v.w;
+                } else {
+                    const uint2 v = lds64(vb + chunk_off<C::D>(tok, r >> 1) + (r & 1) * 8);
+                    vw[t][0] = v.x;
+                    vw[t][1] = v.y;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < C::D / 16; ++i) {
+                const int w = i >> 1;
+                const uint32_t s0 = (i & 1) ? 0x0602 : 0x0400, s1 = (i & 1) ? 0x0703 : 0x0501;
+                uint32_t a[4];
+                a[0] = codes_to_f16x2(__byte_perm(vw[0][w], vw[1][w], s0));
+                a[1] = codes_to_f16x2(__byte_perm(vw[0][w], vw[1][w], s1));
+                a[2] = codes_to_f16x2(__byte_perm(vw[2][w], vw[3][w], s0));
+                a[3] = codes_to_f16x2(__byte_perm(vw[2][w], vw[3][w], s1));
+#pragma unroll
+                for (int nt = 0; nt < C::NT; ++nt) mma_f16(acc[nt][i], a, pb[nt][0], pb[nt][1]);
+            }
+            st = st == kStages - 1 ? 0 : st + 1;
+
+            // ---- end of a piece ----
+            const bool seg_end = cur.blk == cur.blocks - 1;
+            if (seg_end || u + 1 == u1) {
+#pragma unroll
+                for (int nt = 0; nt < C::NT; ++nt)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float x = l[nt][h];
+                        x += __shfl_xor_sync(0xffffffffu, x, 4);
+                        x += __shfl_xor_sync(0xffffffffu, x, 8);
+                        x += __shfl_xor_sync(0xffffffffu, x, 16);
+                        l[nt][h] = x;
+                    }
+                const float back = vr * (1.0f / kWeightOne);
+#pragma unroll
+                for (int nt = 0; nt < C::NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < C::D / 16; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[nt][i][e] *= back;
+                if (seg_end && piece_blk == 0) {
+                    store_rows<C>(p, cur.s, cur.head, cur.tile, acc, l);
+                } else {
+                    const bool last = u + 1 == u1;
+                    const int pi = 2 * warp + (last ? 1 : 0);
+                    float* dst;
+                    if (last) {
+                        cp_wait<0>();
+                        __syncwarp();
+                        dst = reinterpret_cast<float*>(smem + warp * C::SLOT);
+                    } else {
+                        dst = reinterpret_cast<float*>(p.ws + Layout<C>::stash(gridDim.x) + wk * C::PIECE);
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < C::NT; ++nt)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int row = nt * 8 + 2 * c + h;
+#pragma unroll
+                            for (int i = 0; i < C::D / 16; i += 2)
+                                *reinterpret_cast<float4*>(dst + row * C::D + r * (C::D / 8) + 2 * i) =
+                                    make_float4(acc[nt][i][h], acc[nt][i][2 + h], acc[nt][i + 1][h], acc[nt][i + 1][2 + h]);
+                            if (r == 0) {
+                                piece_m[pi][row] = m[nt][h];
+                                piece_l[pi][row] = l[nt][h];
+                            }
+                        }
+                    if (lane == 0) {
+                        PieceInfo& q = pieces[pi];
+                        q.seg = seg_lo;
+                        q.seq = cur.seq;
+                        q.head = cur.head;
+                        q.tile = cur.tile;
+                        q.complete_lo = piece_blk == 0;
+                        q.complete_hi = seg_end;
+                    }
+                }
+            }
+            if (u + 1 < u1) {
+                cur.next(cv, p.group);
+                if (seg_end) {
+                    seg_lo = u + 1;
+                    piece_blk = 0;
+                    begin_segment();
+                }
+            }
+        }
+        cp_wait<0>();
+    }
+    pdl_launch_dependents();
+    __syncthreads();
+
+    // ---- join the CTA's pieces, in unit order ----
+    Partial* info = reinterpret_cast<Partial*>(p.ws + Layout<C>::info()) + 2 * blockIdx.x;
+    float* ml = reinterpret_cast<float*>(p.ws + Layout<C>::ml(gridDim.x)) + static_cast<size_t>(blockIdx.x) * 2 * 2 * C::R;
+    float* po = reinterpret_cast<float*>(p.ws + Layout<C>::o(gridDim.x) + static_cast<size_t>(blockIdx.x) * 2 * C::PIECE);
+    bool have[2] = {false, false};
+    int i = 0;
+    while (i < 2 * C::WARPS) {
+        if (pieces[i].seg < 0) {
+            ++i;
+            continue;
+        }
+        int e = i;                                  // [i, e]: the segment's pieces in this CTA
+        for (int k = i + 1; k < 2 * C::WARPS; ++k) {
+            if (pieces[k].seg < 0) continue;
+            if (pieces[k].seg != pieces[i].seg) break;
+            e = k;
+        }
+        const bool from_start = pieces[i].complete_lo, to_end = pieces[e].complete_hi;
+        const bool whole = from_start && to_end;
+        const int slot = from_start ? 1 : 0;
+        const Seq s = load_seq(cv, pieces[i].seq);
+        for (int idx = tid; idx < C::R * C::D / 4; idx += C::THREADS) {
+            const int row = idx / (C::D / 4), d4 = idx % (C::D / 4);
+            float mx = kNegInf;
+            for (int k = i; k <= e; ++k)
+                if (pieces[k].seg >= 0) mx = fmaxf(mx, piece_m[k][row]);
+            float ls = 0.0f;
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int k = i; k <= e; ++k) {
+                if (pieces[k].seg < 0) continue;
+                const float* src = (k & 1) ? reinterpret_cast<const float*>(smem + (k >> 1) * C::SLOT)
+                                           : reinterpret_cast<const float*>(
+                                                 p.ws + Layout<C>::stash(gridDim.x) +
+                                                 (static_cast<size_t>(blockIdx.x) * C::WARPS + (k >> 1)) * C::PIECE);
+                const float a = mx == kNegInf ? 1.0f : exp2f(piece_m[k][row] - mx);
+                const float4 x = *reinterpret_cast<const float4*>(src + row * C::D + d4 * 4);
+                ls += a * piece_l[k][row];
+                o.x += a * x.x;
+                o.y += a * x.y;
+                o.z += a * x.z;
+                o.w += a * x.w;
+            }
+            if (whole) {
+                const int rr = pieces[i].tile * C::R + row;
+                if (rr < s.n * p.group) {
+                    const int tok = rr / p.group, g = rr - tok * p.group;
+                    const float inv = ls > 0.0f ? __fdiv_rn(1.0f, ls) : (ls == 0.0f ? 0.0f : ls);
+                    uint16_t* dst = p.out + static_cast<int64_t>(s.q0 + tok) * p.ldo +
+                                    static_cast<int64_t>(pieces[i].head * p.group + g) * C::D + d4 * 4;
+                    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+                }
+            } else {
+                *reinterpret_cast<float4*>(po + slot * (C::R * C::D) + row * C::D + d4 * 4) = o;
+                if (d4 == 0) {
+                    ml[slot * 2 * C::R + row] = mx;
+                    ml[slot * 2 * C::R + C::R + row] = ls;
+                }
+            }
+        }
+        if (!whole) {
+            have[slot] = true;
+            if (tid == 0) info[slot] = Partial{pieces[i].seg, pieces[i].seq, pieces[i].head, pieces[i].tile, 0};
+        }
+        i = e + 1;
+    }
+    if (tid < 2 && !have[tid]) info[tid] = Partial{-1, 0, 0, 0, 0};
+}
+
+// Joins the parts of segments that span CTAs: block b leads the segment that
+// begins in CTA b and goes on, and adds the parts of b + 1, b + 2, ... in order.
+template <class C>
+__global__ void __launch_bounds__(256) attend_join_kernel(const AttentionParams p, const int nctas)
+{
+    pdl_launch_dependents();
+    pdl_wait();
+    const Partial* info = reinterpret_cast<const Partial*>(p.ws + Layout<C>::info());
+    const float* ml = reinterpret_cast<const float*>(p.ws + Layout<C>::ml(nctas));
+    const float* po = reinterpret_cast<const float*>(p.ws + Layout<C>::o(nctas));
+    const Partial lead = info[2 * blockIdx.x + 1];
+    if (lead.seg < 0) return;
+    const Seq s = load_seq(p.c, lead.seq);
+    int last = blockIdx.x;
+    while (last + 1 < nctas && info[2 * (last + 1)].seg == lead.seg) ++last;
+    for (int idx = threadIdx.x; idx < C::R * C::D / 4; idx += blockDim.x) {
+        const int row = idx / (C::D / 4), d4 = idx % (C::D / 4);
+        float mx = kNegInf;
+        for (int k = blockIdx.x; k <= last; ++k)
+            mx = fmaxf(mx, ml[(2 * k + (k == static_cast<int>(blockIdx.x))) * 2 * C::R + row]);
+        float ls = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int k = blockIdx.x; k <= last; ++k) {
+            const int sl = 2 * k + (k == static_cast<int>(blockIdx.x));
+            const float a = mx == kNegInf ? 1.0f : exp2f(ml[sl * 2 * C::R + row] - mx);
+            const float4 x = *reinterpret_cast<const float4*>(po + static_cast<size_t>(sl) * C::R * C::D + row * C::D + d4 * 4);
+            ls += a * ml[sl * 2 * C::R + C::R + row];
+            o.x += a * x.x;
+            o.y += a * x.y;
+            o.z += a * x.z;
+            o.w += a * x.w;
+        }
+        const int rr = lead.tile * C::R + row;
+        if (rr >= s.n * p.group) continue;
+        const int tok = rr / p.group, g = rr - tok * p.group;
+        const float inv = ls > 0.0f ? __fdiv_rn(1.0f, ls) : (ls == 0.0f ? 0.0f : ls);
+        uint16_t* dst = p.out + static_cast<int64_t>(s.q0 + tok) * p.ldo +
+                        static_cast<int64_t>(lead.head * p.group + g) * C::D + d4 * 4;
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+    }
+}
+
+template <class C>
+cudaError_t launch_few(const AttentionParams& p, int sms, cudaStream_t stream)
+{
+    const int smem = C::SMEM + (p.c.batch + 1) * 8;
+    cudaError_t e = cudaFuncSetAttribute(attend_few_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         C::SMEM + (kMaxBatch + 1) * 8);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(sms);
+    cfg.blockDim = dim3(C::THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, attend_few_kernel<C>, p);
+    if (e != cudaSuccess) return e;
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 0;
+    return cudaLaunchKernelEx(&cfg, attend_join_kernel<C>, p, sms);
+}
+
+// Row tile of 8 * NT packed rows: the smallest that holds the longest
+// sequence's rows, at most 32.
+int few_nt(int max_q, int group)
+{
+    const int64_t rows = static_cast<int64_t>(max_q) * group;
+    return rows <= 8 ? 1 : (rows <= 16 ? 2 : 4);
+}
+
+}  // namespace
+
+size_t attention_ws_bytes(int batch, int64_t tokens, int q_heads, int kv_heads, int D, int max_q, int sms)
+{
+    (void)batch;
+    (void)tokens;
+    const int nt = few_nt(max_q, q_heads / kv_heads);
+    if (D == 128) {
+        if (nt == 1) return Layout<DecCfg<128, 1>>::total(sms);
+        if (nt == 2) return Layout<DecCfg<128, 2>>::total(sms);
+        return Layout<DecCfg<128, 4>>::total(sms);
+    }
+    if (nt == 1) return Layout<DecCfg<64, 1>>::total(sms);
+    if (nt == 2) return Layout<DecCfg<64, 2>>::total(sms);
+    return Layout<DecCfg<64, 4>>::total(sms);
+}
+
+cudaError_t launch_attention(const AttentionParams& p, int sms, cudaStream_t stream)
+{
+    const int nt = few_nt(p.max_q, p.group);
+    if (p.c.D == 128) {
+        if (nt == 1) return launch_few<DecCfg<128, 1>>(p, sms, stream);
+        if (nt == 2) return launch_few<DecCfg<128, 2>>(p, sms, stream);
+        return launch_few<DecCfg<128, 4>>(p, sms, stream);
+    }
+    if (nt == 1) return launch_few<DecCfg<64, 1>>(p, sms, stream);
+    if (nt == 2) return launch_few<DecCfg<64, 2>>(p, sms, stream);
+    return launch_few<DecCfg<64, 4>>(p, sms, stream);
+}
+
+}  // namespace w4a8

@@ -533,7 +533,50 @@ int linear_prepared_impl(const void* x, int64_t M, int64_t K, int64_t ldx, int64
                       swiglu);
 }
 
+// The norm's arguments into a parameter block: rows of x (and of the residual in
+// and out, where given), the weight, eps.
+int make_norm(const void* x, int64_t M, int64_t K, int64_t ldx, const void* residual, int64_t ldr, void* residual_out,
+              int64_t ldro, const void* weight, int32_t weight_dtype, float eps, NormParams* out)
+{
+    if (M < 0 || K <= 0 || M > (int64_t(1) << 30)) return W4A8_ERR_INVALID;
+    if (K > W4A8_NORM_MAX_K) return W4A8_ERR_UNSUPPORTED;
+    if (weight_dtype != W4A8_DTYPE_BF16 && weight_dtype != W4A8_DTYPE_F32) return W4A8_ERR_UNSUPPORTED;
+    if (!(eps >= 0.0f)) return W4A8_ERR_INVALID;
+    NormParams p{};
+    p.M = static_cast<int>(M);
+    p.K = static_cast<int>(K);
+    p.rows = p.M;
+    *out = p;
+    if (M == 0) return W4A8_OK;
+    if (!x || ldx < K || !aligned(x, 2) || !weight || !aligned(weight, weight_dtype == W4A8_DTYPE_F32 ? 4 : 2))
+        return W4A8_ERR_INVALID;
+    if (residual && (ldr < K || !aligned(residual, 2))) return W4A8_ERR_INVALID;
+    if (residual_out && (ldro < K || !aligned(residual_out, 2))) return W4A8_ERR_INVALID;
+    p.x = static_cast<const uint16_t*>(x);
+    p.res = static_cast<const uint16_t*>(residual);
+    p.weight = weight;
+    p.res_out = static_cast<uint16_t*>(residual_out);
+    p.ldx = ldx;
+    p.ldr = ldr;
+    p.ldro = ldro;
+    p.eps = eps;
+    p.weight_f32 = weight_dtype == W4A8_DTYPE_F32;
+    p.vec_x = aligned(x, 16) && ldx % 8 == 0;
+    p.vec_r = aligned(residual, 16) && ldr % 8 == 0;
+    p.vec_ro = aligned(residual_out, 16) && ldro % 8 == 0;
+    p.vec_w = aligned(weight, 16);
+    *out = p;
+    return W4A8_OK;
+}
+
 }  // namespace
+
+namespace w4a8 {
+
+int capi_device_sms(int* sms) { return device_info(sms); }
+int capi_fail_cuda(cudaError_t e) { return fail_cuda(e); }
+
+}  // namespace w4a8
 
 extern "C" {
 
@@ -803,6 +846,81 @@ int w4a8_linear_prepared_swiglu(const void* gu, int64_t M, int64_t K, int64_t ld
 {
     return linear_prepared_impl(gu, M, K, ldx, N, gk, prepared, ws_dtype, has_zero, y, ldy, workspace,
                                 workspace_bytes, stream, true);
+}
+
+int w4a8_rms_norm(const void* x, int64_t M, int64_t K, int64_t ldx, const void* residual, int64_t ldr,
+                  void* residual_out, int64_t ldro, const void* weight, int32_t weight_dtype, float eps, void* y,
+                  int64_t ldy, void* stream)
+{
+    NormParams p;
+    int rc = make_norm(x, M, K, ldx, residual, ldr, residual_out, ldro, weight, weight_dtype, eps, &p);
+    if (rc != W4A8_OK) return rc;
+    if (M == 0) return W4A8_OK;
+    if (!y || ldy < K || !aligned(y, 2)) return W4A8_ERR_INVALID;
+    int sms = 0;
+    if ((rc = device_info(&sms)) != W4A8_OK) return rc;
+    p.y = static_cast<uint16_t*>(y);
+    p.ldy = ldy;
+    p.vec_y = aligned(y, 16) && ldy % 8 == 0;
+    const cudaError_t e = launch_rms_norm(p, kNormBf16, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? W4A8_OK : fail_cuda(e);
+}
+
+int w4a8_rms_norm_quant(const void* x, int64_t M, int64_t K, int64_t ldx, const void* residual, int64_t ldr,
+                        void* residual_out, int64_t ldro, const void* weight, int32_t weight_dtype, float eps,
+                        int32_t gk, int8_t* a_q, void* a_scale, int32_t scale_dtype, void* stream)
+{
+    NormParams p;
+    int rc = make_norm(x, M, K, ldx, residual, ldr, residual_out, ldro, weight, weight_dtype, eps, &p);
+    if (rc != W4A8_OK) return rc;
+    if (!group_ok(gk)) return W4A8_ERR_UNSUPPORTED;
+    if (scale_dtype != W4A8_DTYPE_BF16 && scale_dtype != W4A8_DTYPE_F32) return W4A8_ERR_UNSUPPORTED;
+    if (M == 0) return W4A8_OK;
+    if (!a_q || !a_scale || !aligned(a_scale, scale_dtype == W4A8_DTYPE_F32 ? 4 : 2)) return W4A8_ERR_INVALID;
+    int sms = 0;
+    if ((rc = device_info(&sms)) != W4A8_OK) return rc;
+    p.gk = gk;
+    p.G = static_cast<int>(cdiv(K, gk));
+    p.q = a_q;
+    p.scale = a_scale;
+    p.scale_f32 = scale_dtype == W4A8_DTYPE_F32;
+    p.vec_q = aligned(a_q, 8) && K % 8 == 0;
+    const cudaError_t e = launch_rms_norm(p, kNormCodes, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? W4A8_OK : fail_cuda(e);
+}
+
+int w4a8_linear_prepared_rms_norm(const void* x, int64_t M, int64_t K, int64_t ldx, const void* residual, int64_t ldr,
+                                  void* residual_out, int64_t ldro, const void* weight, int32_t weight_dtype,
+                                  float eps, int64_t N, int32_t gk, const void* prepared, int32_t ws_dtype,
+                                  int32_t has_zero, void* y, int64_t ldy, void* workspace, size_t workspace_bytes,
+                                  void* stream)
+{
+    int rc = check_common(M, N, K, gk);
+    if (rc != W4A8_OK) return rc;
+    NormParams p;
+    if ((rc = make_norm(x, M, K, ldx, residual, ldr, residual_out, ldro, weight, weight_dtype, eps, &p)) != W4A8_OK)
+        return rc;
+    if (M == 0) return W4A8_OK;
+    if (!prepared || !aligned(prepared, 256)) return W4A8_ERR_INVALID;
+    if (ws_dtype != W4A8_DTYPE_BF16 && ws_dtype != W4A8_DTYPE_F32) return W4A8_ERR_UNSUPPORTED;
+    if (!y || ldy < N || !aligned(y, 2)) return W4A8_ERR_INVALID;
+    int sms = 0;
+    if ((rc = device_info(&sms)) != W4A8_OK) return rc;
+    const Plan pl = make_plan(M, N, K, gk, sms);
+    if (!workspace || !aligned(workspace, 1024) || workspace_bytes < pl.total) return W4A8_ERR_WORKSPACE;
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    p.rows = pl.n_tt * pl.tt;
+    p.gk = gk;
+    p.G = static_cast<int>(pl.G);
+    p.aq = reinterpret_cast<int8_t*>(ws + pl.off_aq);
+    p.as = reinterpret_cast<float*>(ws + pl.off_as);
+    p.tt = pl.tt;
+    p.kb_total = pl.kb_total;
+    const cudaError_t e = launch_rms_norm(p, kNormTiles, st);
+    if (e != cudaSuccess) return fail_cuda(e);
+    const Weights w{nullptr, nullptr, nullptr, static_cast<const uint8_t*>(prepared), has_zero != 0, ws_dtype};
+    return run_gemm(pl, w, y, ldy, false, ws, st);
 }
 
 int w4a8_linear_prepared_allreduce(const void* x, int64_t M, int64_t K, int64_t ldx, int64_t N, int32_t gk,

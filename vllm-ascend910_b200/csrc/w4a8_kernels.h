@@ -148,6 +148,91 @@ size_t gemm_smem_bytes(const GemmConfig& cfg);
 // dependent of the GEMM launched with the same parameters and grid).
 cudaError_t launch_splitk_reduce(const GemmParams& p, int tt, int grid, cudaStream_t stream);
 
+
+// ---- residual addition + root-mean-square norm (w4a8_norm.cu) ----
+enum NormOutKind { kNormBf16 = 0, kNormCodes = 1, kNormTiles = 2 };
+
+struct NormParams {
+    const uint16_t* x;        // bf16 [M, ldx]
+    const uint16_t* res;      // bf16 [M, ldr], or null
+    const void* weight;       // [K] bf16 or fp32
+    uint16_t* res_out;        // bf16 [M, ldro]: bf16(x + res), or null
+    int64_t ldx, ldr, ldro;
+    float eps;
+    int weight_f32;
+    int M, K;
+    int rows;                 // rows to emit: M, or whole token tiles (kNormTiles)
+    int vec_x, vec_r, vec_ro, vec_w, vec_y, vec_q;   // 16-byte (codes: 8-byte) accesses are legal
+    // kNormBf16
+    uint16_t* y;              // bf16 [M, ldy]
+    int64_t ldy;
+    // kNormCodes
+    int gk, G;
+    int8_t* q;                // [M, K]
+    void* scale;              // [G, M] bf16 bits or fp32
+    int scale_f32;
+    // kNormTiles: as QuantParams' kOutKernel form
+    int8_t* aq;
+    float* as;
+    int tt, kb_total;
+};
+
+cudaError_t launch_rms_norm(const NormParams& p, int out_kind, cudaStream_t stream);
+
+// ---- paged 8-bit cache (w4a8_kvcache.cu) and attention over it (w4a8_attention.cu) ----
+
+// One layer's cache and the batch of sequences that a call works on.
+struct CacheView {
+    int8_t* k;                // [pages][kv_heads][page][D]
+    int8_t* v;
+    float* k_scale;           // [pages][kv_heads]
+    float* v_scale;
+    const int32_t* table;     // page ids [batch][ld_table]
+    const int32_t* kv_lens;   // [batch] tokens in the cache, this call's included
+    const int32_t* cu;        // [batch + 1] offsets of each sequence's tokens in this call
+    int64_t ld_table, pages, tokens;
+    int table_cols, batch, kv_heads, page, page_log2, D;
+};
+
+struct KvWriteParams {
+    CacheView c;
+    const uint16_t* q;        // bf16 [tokens, ldq] of q_heads * D, or null
+    const uint16_t* k;        // bf16 [tokens, ldk] of kv_heads * D
+    const uint16_t* v;
+    uint16_t* q_out;          // bf16 [tokens, ldqo]
+    const float* cos_sin;     // [table_rows, rot]: cos of rot / 2 angles, then sin; null: no rotation
+    int64_t ldq, ldk, ldv, ldqo, table_rows;
+    int q_heads, rot, interleaved;
+};
+
+struct KvReadParams {
+    CacheView c;              // cu: offsets of the tokens to read (each sequence's last ones)
+    uint16_t* k;              // bf16 [tokens, kv_heads, D]
+    uint16_t* v;
+};
+
+struct AttentionParams {
+    CacheView c;
+    const uint16_t* q;        // bf16 [tokens, ldq] of q_heads * D
+    uint16_t* out;            // bf16 [tokens, ldo]
+    int64_t ldq, ldo;
+    int q_heads, group;       // group: query heads per kv head
+    int max_q;                // no sequence has more query tokens (host's knowledge)
+    float scale_log2;         // softmax scale * log2(e)
+    int* status;              // workspace: status word
+    uint8_t* ws;              // workspace past the status block
+};
+
+cudaError_t launch_kv_write(const KvWriteParams& p, cudaStream_t stream);
+cudaError_t launch_kv_read(const KvReadParams& p, cudaStream_t stream);
+// Bytes of p.ws that a call of these sizes needs.
+size_t attention_ws_bytes(int batch, int64_t tokens, int q_heads, int kv_heads, int D, int max_q, int sms);
+cudaError_t launch_attention(const AttentionParams& p, int sms, cudaStream_t stream);
+
+// Host helpers of the C entry points (w4a8_capi.cu).
+int capi_device_sms(int* sms);
+int capi_fail_cuda(cudaError_t e);
+
 // The one-shot all-reduce's side of the fused row-parallel linear
 // (w4a8_allreduce.cu): where a GEMM must push a message of `bytes`, and the
 // reduction that follows the pushes (flags, bounded waits, rank-order sum).

@@ -26,12 +26,15 @@ OPT_FUSED_QUANT = 1              # W4A8_OPT_FUSED_QUANT
 OPT_AR_PUSH = 2                  # W4A8_OPT_AR_PUSH
 ACT_NONE = 0                     # W4A8_ACT_NONE
 ACT_SWIGLU = 1                   # W4A8_ACT_SWIGLU
+NORM_MAX_K = 32768               # W4A8_NORM_MAX_K
+ATTENTION_MAX_BATCH = 2048       # W4A8_ATTENTION_MAX_BATCH
 
 _L = None
 
 _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int32
+_f32 = ctypes.c_float
 _sz = ctypes.c_size_t
 
 # (name, restype, argtypes) of every exported symbol, in header order.
@@ -76,12 +79,31 @@ SIGNATURES = [
     ("w4a8_ar_destroy", ctypes.c_int, [_p]),
     ("w4a8_linear_prepared_allreduce", ctypes.c_int,
      [_p, _i64, _i64, _i64, _i64, _i32, _p, _i32, _i32, _i32, _p, _p, _sz, _p, _p]),
+    ("w4a8_rms_norm", ctypes.c_int,
+     [_p, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _i32, _f32, _p, _i64, _p]),
+    ("w4a8_rms_norm_quant", ctypes.c_int,
+     [_p, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _i32, _f32, _i32, _p, _p, _i32, _p]),
+    ("w4a8_linear_prepared_rms_norm", ctypes.c_int,
+     [_p, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _i32, _f32, _i64, _i32, _p, _i32, _i32, _p, _i64, _p, _sz, _p]),
+    ("w4a8_kv_write", ctypes.c_int,
+     [_p, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _i32, _p, _i64, _p, _i64, _i32, _i32,
+      _p]),
+    ("w4a8_kv_read", ctypes.c_int, [_p, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _p]),
+    ("w4a8_attention_workspace_size", _sz, [_i64, _i64, _i32, _i32, _i32, _i32]),
+    ("w4a8_attention", ctypes.c_int,
+     [_p, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _i32, _i32, _f32, _p, _i64, _p, _sz, _p]),
     ("w4a8_workspace_status", ctypes.c_int, [_p, _i32, _p]),
     ("w4a8_status_string", ctypes.c_char_p, [ctypes.c_int]),
     ("w4a8_last_cuda_error", ctypes.c_int, []),
     ("w4a8_build_arch", ctypes.c_int, []),
     ("w4a8_set_options", ctypes.c_int, [_i32]),
 ]
+
+
+class KvCacheDesc(ctypes.Structure):
+    """w4a8_kv_cache."""
+    _fields_ = [("k", _p), ("v", _p), ("k_scale", _p), ("v_scale", _p), ("pages", _i64), ("kv_heads", _i32),
+                ("page_size", _i32), ("head_dim", _i32), ("reserved", _i32)]
 
 
 def lib_path() -> str:

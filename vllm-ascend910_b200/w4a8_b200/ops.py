@@ -389,6 +389,128 @@ def group_partials(x: torch.Tensor, w_packed: torch.Tensor, w_zero: Optional[tor
     return P
 
 
+# ---------------------------------------------------------------- residual addition + RMS norm
+
+def _norm_args(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor],
+               residual_out: Optional[torch.Tensor], what: str):
+    """Checked (x2 [M, K], residual2, residual_out2, weight dtype code) of a norm call."""
+    if x.dtype != torch.bfloat16:
+        raise RuntimeError(f"{what}: x must be bfloat16")
+    if not x.is_cuda or weight.device != x.device:
+        raise RuntimeError(f"{what}: needs CUDA tensors on one device (there is no CPU implementation)")
+    K = x.shape[-1] if x.dim() else 0
+    _check(0 < K <= _lib.NORM_MAX_K, f"{what}: the last dimension must be 1..{_lib.NORM_MAX_K}")
+    if weight.dim() != 1 or weight.shape[0] != K or weight.stride(0) != 1:
+        raise RuntimeError(f"{what}: weight must be a dense [{K}]")
+    if weight.dtype == torch.bfloat16:
+        wd = _lib.DTYPE_BF16
+    else:
+        _check(weight.dtype == torch.float32, f"{what}: weight must be bfloat16 or float32")
+        wd = _lib.DTYPE_F32
+    x2 = x if x.dim() == 2 else x.reshape(-1, K)
+    if x2.stride(1) != 1:
+        x2 = x2.contiguous()
+    if residual is None:
+        _check(residual_out is None, f"{what}: residual_out without residual")
+        return x2, None, None, wd
+    if residual.dtype != torch.bfloat16 or residual.shape != x.shape or residual.device != x.device:
+        raise RuntimeError(f"{what}: residual must be bfloat16, of x's shape and on its device")
+    r2 = residual if residual.dim() == 2 else residual.reshape(-1, K)
+    if r2.stride(1) != 1:
+        r2 = r2.contiguous()
+    if residual_out is None:
+        ro = torch.empty(x2.shape, dtype=torch.bfloat16, device=x.device)
+    else:
+        ro = residual_out
+        _check(ro.dtype == torch.bfloat16 and ro.shape == x.shape and ro.device == x.device,
+               f"{what}: residual_out must be bfloat16, of x's shape and on its device")
+        if ro.dim() != 2:
+            _check(ro.is_contiguous(), f"{what}: residual_out must be dense unless it is 2-D")
+            ro = ro.view(-1, K)
+        _check(ro.stride(1) == 1, f"{what}: residual_out's rows must be dense")
+    return x2, r2, ro, wd
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: Optional[torch.Tensor] = None,
+             residual_out: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None):
+    """y = h / sqrt(mean(h^2) + eps) * weight over the last dimension, h = x (+ residual).
+
+    Without a residual returns y.  With one returns (y, bf16(h)), the latter
+    into ``residual_out`` when given (it may be the residual itself).  fp32
+    inside, each output rounded once."""
+    x2, r2, ro, wd = _norm_args(x, weight, residual, residual_out, "rms_norm")
+    M, K = x2.shape
+    if out is None:
+        y = torch.empty((M, K), dtype=torch.bfloat16, device=x.device)
+    else:
+        _check(out.dtype == torch.bfloat16 and out.shape == x.shape and out.device == x.device and
+               (out.is_contiguous() or (out.dim() == 2 and out.stride(1) == 1)),
+               "rms_norm: out must be bfloat16, of x's shape, on its device, with dense rows")
+        y = out if out.dim() == 2 else out.view(-1, K)
+    rc = _lib.lib().w4a8_rms_norm(x2.data_ptr(), M, K, x2.stride(0), None if r2 is None else r2.data_ptr(),
+                                  0 if r2 is None else r2.stride(0), None if ro is None else ro.data_ptr(),
+                                  0 if ro is None else ro.stride(0), weight.data_ptr(), wd, eps, y.data_ptr(),
+                                  y.stride(0), _stream_of(x2))
+    if rc != 0:
+        _lib.check(rc, "w4a8_rms_norm")
+    if x.dim() != 2:
+        y = y.view(x.shape)
+    if r2 is None:
+        return y
+    return y, (ro if x.dim() == 2 else ro.view(x.shape))
+
+
+def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, group_size: int, eps: float = 1e-6,
+                   residual: Optional[torch.Tensor] = None, residual_out: Optional[torch.Tensor] = None,
+                   scale_dtype: torch.dtype = torch.bfloat16):
+    """``rms_norm`` with its fp32 result quantised per (token, group) by ``quant_act``'s rule:
+    x [M, K] -> (q int8 [M, K], scale [G, M], bf16(x + residual) or None)."""
+    _check(x.dim() == 2, "rms_norm_quant: x must be [M, K]")
+    _check(scale_dtype in (torch.float32, torch.bfloat16), "rms_norm_quant: scale dtype must be bf16 or f32")
+    x2, r2, ro, wd = _norm_args(x, weight, residual, residual_out, "rms_norm_quant")
+    M, K = x2.shape
+    q = torch.empty((M, K), dtype=torch.int8, device=x.device)
+    s = torch.empty((num_groups(K, max(group_size, 1)), M), dtype=scale_dtype, device=x.device)
+    rc = _lib.lib().w4a8_rms_norm_quant(x2.data_ptr(), M, K, x2.stride(0), None if r2 is None else r2.data_ptr(),
+                                        0 if r2 is None else r2.stride(0), None if ro is None else ro.data_ptr(),
+                                        0 if ro is None else ro.stride(0), weight.data_ptr(), wd, eps, group_size,
+                                        q.data_ptr(), s.data_ptr(),
+                                        _lib.DTYPE_F32 if scale_dtype == torch.float32 else _lib.DTYPE_BF16,
+                                        _stream_of(x2))
+    if rc != 0:
+        _lib.check(rc, "w4a8_rms_norm_quant")
+    return q, s, ro
+
+
+def linear_prepared_rms_norm(x: torch.Tensor, weight: torch.Tensor, pw: PreparedWeight, eps: float = 1e-6,
+                             residual: Optional[torch.Tensor] = None, residual_out: Optional[torch.Tensor] = None,
+                             out: Optional[torch.Tensor] = None):
+    """``linear_prepared`` on the norm of x (+ residual): the norm kernel quantises straight into the
+    GEMM's operand tiles (``rms_norm_quant``'s codes).  Returns y, or (y, bf16(x + residual))."""
+    x2, r2, ro, wd = _norm_args(x, weight, residual, residual_out, "linear_prepared_rms_norm")
+    M, K = x2.shape
+    _check(x.device == pw.buf.device, "linear_prepared_rms_norm: x must be on the weights' device")
+    _check(K == pw.K, f"linear_prepared_rms_norm: x has last dimension {K}, weights were prepared for K={pw.K}")
+    N = pw.N
+    if out is not None:
+        _check(out.dtype == torch.bfloat16 and tuple(out.shape) == (M, N) and out.stride(1) == 1 and
+               out.device == x.device, f"linear_prepared_rms_norm: out must be bfloat16 [{M}, {N}] with dense rows")
+    y = out if out is not None else torch.empty((M, N), dtype=torch.bfloat16, device=x.device)
+    if M > 0:
+        ws, wsb = workspace(_ws_bytes(M, N, K, pw.group_size), x.device)
+        rc = _lib.lib().w4a8_linear_prepared_rms_norm(
+            x2.data_ptr(), M, K, x2.stride(0), None if r2 is None else r2.data_ptr(),
+            0 if r2 is None else r2.stride(0), None if ro is None else ro.data_ptr(),
+            0 if ro is None else ro.stride(0), weight.data_ptr(), wd, eps, N, pw.group_size, pw.ptr(), pw.ws_dtype,
+            1 if pw.has_zero else 0, y.data_ptr(), y.stride(0), ws, wsb, _stream_of(x2))
+        if rc != 0:
+            _lib.check(rc, "w4a8_linear_prepared_rms_norm")
+    y = y if x.dim() == 2 else y.reshape(*x.shape[:-1], N)
+    if r2 is None:
+        return y
+    return y, (ro if x.dim() == 2 else ro.view(x.shape))
+
+
 # ---------------------------------------------------------------- weight packing (device-agnostic torch)
 
 def pack_int4(v: torch.Tensor) -> torch.Tensor:
