@@ -38,10 +38,9 @@
 //   * A warp's share begins and ends inside (sequence, head) segments.  Pieces
 //     of one segment are joined in the CTA, and across CTAs by a second small
 //     kernel, in unit order: no atomics, the same bits on every run.
-#include <cuda_fp16.h>
+#include <algorithm>
 
-#include "w4a8_common.cuh"
-#include "w4a8_kernels.h"
+#include "w4a8_attention.cuh"
 
 namespace w4a8 {
 
@@ -49,8 +48,6 @@ namespace {
 
 constexpr int kBlkTok = 16;        // tokens per unit
 constexpr int kStages = 3;         // units in a warp's ring
-constexpr int kMaxBatch = 2048;
-constexpr float kNegInf = -INFINITY;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok)
 {
@@ -98,70 +95,12 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x)
     return y;
 }
 
-// Two int8 codes in bytes 0 and 2 of w (bytes 1 and 3: anything) -> fp16 pair,
-// exactly: the bits 0x6400 | (code + 128) are the fp16 number 1024 + code + 128.
-__device__ __forceinline__ uint32_t codes_to_f16x2(uint32_t w)
-{
-    const uint32_t m = (w & 0x00FF00FFu) ^ 0x64806480u;
-    const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&m), __half2half2(__ushort_as_half(0x6480)));
-    return *reinterpret_cast<const uint32_t*>(&d);
-}
-
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi)
-{
-    const __half2 b = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&b);
-}
-
-// 2^-e for a row whose largest magnitude is m, m * 2^-e in [2^13, 2^14); 1 for a
-// zero or non-finite m.  e is held within what fp32 can scale by.
-__device__ __forceinline__ float row_shrink(float m)
-{
-    if (!(m > 0.0f) || m == INFINITY) return 1.0f;
-    const int e = static_cast<int>((__float_as_uint(m) >> 23) & 0xFFu) - 127 - 13;
-    return __uint_as_float(static_cast<uint32_t>(127 - min(max(e, -126), 126)) << 23);
-}
-
-// The smallest power of two at or above a positive finite v (at least 2^-100);
-// 1 for a non-finite v.
-__device__ __forceinline__ float pow2_above(float v)
-{
-    if (!(v < INFINITY)) return 1.0f;
-    const uint32_t b = __float_as_uint(fmaxf(v, 7.888609052210118e-31f));
-    return __uint_as_float((b & 0x7F800000u) + ((b & 0x007FFFFFu) ? 0x00800000u : 0u));
-}
-constexpr float kVrMin = 7.888609052210118e-31f;   // 2^-100
-constexpr float kWeightOne = 16384.0f;             // 2^14
-
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi)
-{
-    const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&b);
-}
-
-// ------------------------------------------------------------------ the batch
-
-// A sequence as the kernels see it, every value held within the tensors.
-struct Seq {
-    int q0, n;       // first query token and their number
-    int len;         // tokens in the cache
-};
-
-__device__ __forceinline__ Seq load_seq(const CacheView& c, int s)
-{
-    Seq r;
-    const int64_t a = min(static_cast<int64_t>(max(c.cu[s], 0)), c.tokens);
-    const int64_t b = min(static_cast<int64_t>(max(c.cu[s + 1], 0)), c.tokens);
-    r.q0 = static_cast<int>(a);
-    r.n = static_cast<int>(max(b - a, static_cast<int64_t>(0)));
-    r.len = static_cast<int>(min(static_cast<int64_t>(max(c.kv_lens[s], 0)),
-                                 static_cast<int64_t>(c.table_cols) << c.page_log2));
-    return r;
-}
-
 // Row tiles of a sequence, and 16-token blocks of each (at least one, so that
 // rows which see nothing are written too).
-__device__ __forceinline__ int seq_tiles(const Seq& s, int group, int rows) { return (s.n * group + rows - 1) / rows; }
+__device__ __forceinline__ int seq_tiles(const Seq& s, int group, int rows, int most)
+{
+    return s.n * group <= most ? (s.n * group + rows - 1) / rows : 0;
+}
 __device__ __forceinline__ int seq_blocks(const Seq& s) { return max(1, (s.len + kBlkTok - 1) / kBlkTok); }
 
 // ------------------------------------------------------------------ few rows
@@ -196,11 +135,6 @@ struct PieceInfo {
     int seq, head, tile, complete_lo, complete_hi;   // the piece reaches the segment's first / last unit
 };
 
-struct Partial {        // one per CTA and slot, in the workspace
-    long long seg;
-    int seq, head, tile, pad;
-};
-
 template <class C>
 struct Layout {
     // workspace: [grid][2] Partial, then [grid][2] (m, l)[R], then [grid][2] O, then [grid * WARPS] stash (O, m, l)
@@ -219,12 +153,12 @@ template <class C>
 struct Cursor {
     int seq, head, tile, blk, blocks;
     Seq s;
-    __device__ __forceinline__ void set(const CacheView& c, int group, int sq, long long off)
+    __device__ __forceinline__ void set(const CacheView& c, int group, int most, int sq, long long off)
     {
         seq = sq;
         s = load_seq(c, sq);
         blocks = seq_blocks(s);
-        const int tiles = seq_tiles(s, group, C::R);
+        const int tiles = seq_tiles(s, group, C::R, most);
         const long long per_head = static_cast<long long>(tiles) * blocks;
         head = static_cast<int>(off / per_head);
         const long long r = off - head * per_head;
@@ -232,18 +166,18 @@ struct Cursor {
         blk = static_cast<int>(r - static_cast<long long>(tile) * blocks);
     }
     // Next unit; false past the end of the list.
-    __device__ __forceinline__ bool next(const CacheView& c, int group)
+    __device__ __forceinline__ bool next(const CacheView& c, int group, int most)
     {
         if (++blk < blocks) return true;
         blk = 0;
-        if (++tile < seq_tiles(s, group, C::R)) return true;
+        if (++tile < seq_tiles(s, group, C::R, most)) return true;
         tile = 0;
         if (++head < c.kv_heads) return true;
         head = 0;
         do {
             if (++seq >= c.batch) return false;
             s = load_seq(c, seq);
-        } while (s.n == 0);
+        } while (seq_tiles(s, group, C::R, most) == 0);
         blocks = seq_blocks(s);
         return true;
     }
@@ -261,10 +195,8 @@ __device__ __forceinline__ void store_rows(const AttentionParams& p, const Seq& 
         for (int h = 0; h < 2; ++h) {
             const int row = tile * C::R + nt * 8 + 2 * c + h;
             if (row >= s.n * p.group) continue;
-            const int tok = row / p.group, g = row - tok * p.group;
-            const float inv = l[nt][h] > 0.0f ? __fdiv_rn(1.0f, l[nt][h]) : (l[nt][h] == 0.0f ? 0.0f : l[nt][h]);
-            uint16_t* o = p.out + static_cast<int64_t>(s.q0 + tok) * p.ldo +
-                          static_cast<int64_t>(head * p.group + g) * C::D + r * (C::D / 8);
+            const float inv = inv_sum(l[nt][h]);
+            uint16_t* o = out_row(p, s, head, row) + r * (C::D / 8);
             uint32_t w[C::D / 16];
 #pragma unroll
             for (int i = 0; i < C::D / 16; ++i) w[i] = pack_bf16(acc[nt][i][h] * inv, acc[nt][i][2 + h] * inv);
@@ -297,7 +229,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
         long long u = 0;
         if (s < cv.batch) {
             const Seq q = load_seq(cv, s);
-            u = static_cast<long long>(cv.kv_heads) * seq_tiles(q, p.group, C::R) * seq_blocks(q);
+            u = static_cast<long long>(cv.kv_heads) * seq_tiles(q, p.group, C::R, p.few_most) * seq_blocks(q);
         }
         long long x = u;
 #pragma unroll
@@ -335,7 +267,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
             else hi = mid - 1;
         }
         Cursor<C> cur, pre;
-        cur.set(cv, p.group, lo, u0 - prefix[lo]);
+        cur.set(cv, p.group, p.few_most, lo, u0 - prefix[lo]);
         pre = cur;
         bool pre_ok = true;
         long long pre_u = u0;
@@ -363,7 +295,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
                     else asm volatile("st.shared.f32 [%0], %1;" ::"r"(d + 2 * C::KV_BYTES + lane * 4), "f"(-1.0f));
                 }
                 ++pre_u;
-                pre_ok = pre.next(cv, p.group);
+                pre_ok = pre.next(cv, p.group, p.few_most);
             }
             cp_commit();
         };
@@ -500,7 +432,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
                         const float mn = fmaxf(m[nt][h], x);
-                        const float a = mn == kNegInf ? 1.0f : exp2f(m[nt][h] - mn);
+                        const float a = mn == kNegInf ? 1.0f : ex2(m[nt][h] - mn);
                         m[nt][h] = mn;
                         l[nt][h] *= a;
                         const float av = a * va;
@@ -521,7 +453,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float mm = m[nt][e & 1] == kNegInf ? 0.0f : m[nt][e & 1];
-                    const float x = exp2f(sc[nt][e] - mm);
+                    const float x = ex2(sc[nt][e] - mm);
                     l[nt][e & 1] += x;
                     e4[e] = edge && sc[nt][e] == kNegInf ? 0.0f : x * vw_;
                 }
@@ -619,7 +551,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
                 }
             }
             if (u + 1 < u1) {
-                cur.next(cv, p.group);
+                cur.next(cv, p.group, p.few_most);
                 if (seg_end) {
                     seg_lo = u + 1;
                     piece_blk = 0;
@@ -677,10 +609,8 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
             if (whole) {
                 const int rr = pieces[i].tile * C::R + row;
                 if (rr < s.n * p.group) {
-                    const int tok = rr / p.group, g = rr - tok * p.group;
-                    const float inv = ls > 0.0f ? __fdiv_rn(1.0f, ls) : (ls == 0.0f ? 0.0f : ls);
-                    uint16_t* dst = p.out + static_cast<int64_t>(s.q0 + tok) * p.ldo +
-                                    static_cast<int64_t>(pieces[i].head * p.group + g) * C::D + d4 * 4;
+                    const float inv = inv_sum(ls);
+                    uint16_t* dst = out_row(p, s, pieces[i].head, rr) + d4 * 4;
                     *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
                 }
             } else {
@@ -734,10 +664,8 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttentionParams 
         }
         const int rr = lead.tile * C::R + row;
         if (rr >= s.n * p.group) continue;
-        const int tok = rr / p.group, g = rr - tok * p.group;
-        const float inv = ls > 0.0f ? __fdiv_rn(1.0f, ls) : (ls == 0.0f ? 0.0f : ls);
-        uint16_t* dst = p.out + static_cast<int64_t>(s.q0 + tok) * p.ldo +
-                        static_cast<int64_t>(lead.head * p.group + g) * C::D + d4 * 4;
+        const float inv = inv_sum(ls);
+        uint16_t* dst = out_row(p, s, lead.head, rr) + d4 * 4;
         *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
     }
 }
@@ -746,9 +674,16 @@ template <class C>
 cudaError_t launch_few(const AttentionParams& p, int sms, cudaStream_t stream)
 {
     const int smem = C::SMEM + (p.c.batch + 1) * 8;
-    cudaError_t e = cudaFuncSetAttribute(attend_few_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         C::SMEM + (kMaxBatch + 1) * 8);
+    static bool ready[64] = {};          // per device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64 || !ready[dev]) {
+        e = cudaFuncSetAttribute(attend_few_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 C::SMEM + (kMaxBatch + 1) * 8);
+        if (e != cudaSuccess) return e;
+        if (dev >= 0 && dev < 64) ready[dev] = true;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(sms);
     cfg.blockDim = dim3(C::THREADS);
@@ -766,12 +701,21 @@ cudaError_t launch_few(const AttentionParams& p, int sms, cudaStream_t stream)
     return cudaLaunchKernelEx(&cfg, attend_join_kernel<C>, p, sms);
 }
 
-// Row tile of 8 * NT packed rows: the smallest that holds the longest
-// sequence's rows, at most 32.
-int few_nt(int max_q, int group)
+// Row tile of 8 * NT packed rows: the smallest that holds the rows of any
+// sequence the kernel takes, at most 32.
+int few_nt(int64_t rows) { return rows <= 8 ? 1 : (rows <= 16 ? 2 : 4); }
+
+template <class F>
+auto with_few(int D, int nt, const F& f)
 {
-    const int64_t rows = static_cast<int64_t>(max_q) * group;
-    return rows <= 8 ? 1 : (rows <= 16 ? 2 : 4);
+    if (D == 128) {
+        if (nt == 1) return f(DecCfg<128, 1>{});
+        if (nt == 2) return f(DecCfg<128, 2>{});
+        return f(DecCfg<128, 4>{});
+    }
+    if (nt == 1) return f(DecCfg<64, 1>{});
+    if (nt == 2) return f(DecCfg<64, 2>{});
+    return f(DecCfg<64, 4>{});
 }
 
 }  // namespace
@@ -780,28 +724,23 @@ size_t attention_ws_bytes(int batch, int64_t tokens, int q_heads, int kv_heads, 
 {
     (void)batch;
     (void)tokens;
-    const int nt = few_nt(max_q, q_heads / kv_heads);
-    if (D == 128) {
-        if (nt == 1) return Layout<DecCfg<128, 1>>::total(sms);
-        if (nt == 2) return Layout<DecCfg<128, 2>>::total(sms);
-        return Layout<DecCfg<128, 4>>::total(sms);
-    }
-    if (nt == 1) return Layout<DecCfg<64, 1>>::total(sms);
-    if (nt == 2) return Layout<DecCfg<64, 2>>::total(sms);
-    return Layout<DecCfg<64, 4>>::total(sms);
+    const int64_t rows = static_cast<int64_t>(max_q) * (q_heads / kv_heads);
+    const size_t few = with_few(D, few_nt(rows), [&](auto c) { return Layout<decltype(c)>::total(sms); });
+    return rows <= kFewRows ? few : std::max(few, attend_many_ws_bytes(D, sms));
 }
 
-cudaError_t launch_attention(const AttentionParams& p, int sms, cudaStream_t stream)
+cudaError_t launch_attention(const AttentionParams& p0, int sms, cudaStream_t stream)
 {
-    const int nt = few_nt(p.max_q, p.group);
-    if (p.c.D == 128) {
-        if (nt == 1) return launch_few<DecCfg<128, 1>>(p, sms, stream);
-        if (nt == 2) return launch_few<DecCfg<128, 2>>(p, sms, stream);
-        return launch_few<DecCfg<128, 4>>(p, sms, stream);
+    AttentionParams p = p0;
+    const int64_t rows = static_cast<int64_t>(p.max_q) * p.group;
+    p.few_most = 0x7FFFFFFF;
+    if (rows > kFewRows) {
+        // one sequence at least has more rows: attend_many_kernel takes those
+        const cudaError_t e = launch_attend_many(p, sms, stream);
+        if (e != cudaSuccess || p.c.batch == 1) return e;   // (alone, it takes any sequence)
+        p.few_most = kFewRows;
     }
-    if (nt == 1) return launch_few<DecCfg<64, 1>>(p, sms, stream);
-    if (nt == 2) return launch_few<DecCfg<64, 2>>(p, sms, stream);
-    return launch_few<DecCfg<64, 4>>(p, sms, stream);
+    return with_few(p.c.D, few_nt(rows), [&](auto c) { return launch_few<decltype(c)>(p, sms, stream); });
 }
 
 }  // namespace w4a8

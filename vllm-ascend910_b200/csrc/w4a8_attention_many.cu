@@ -1,0 +1,890 @@
+// w4a8_attention_many.cu -- attention over the paged 8-bit cache for sequences
+// with many query rows (prompts, chunks), on the 5th-generation tensor core.
+// The mathematics and the fp16 operand ranges are those of w4a8_attention.cu.
+//
+// Rows of one kv head are packed (query token x query head of the group) into
+// tiles of 256: two halves A and B of 128 rows, one TMEM lane each.  The cache
+// is walked in blocks of 64 tokens:
+//
+//   S_X = Q_X K^T          tcgen05.mma f16, M 128, N 64, both operands in smem
+//   P_X = exp2(...)        softmax warps, a thread per row, from and to TMEM
+//   O_X += P_X V           A operand = P_X in TMEM, N = D, V K-row-major in smem
+//
+// Roles (one CTA per SM):
+//   warps 0-3, 4-7   softmax of half A, B: row maximum, exponentials, weights, sum;
+//                    their rows' queries to fp16 in smem, and the output rows
+//   warps 8-11       converters: cache codes by 16-byte loads (one block ahead in
+//                    registers), exact fp16 into the swizzled operand layout
+//   warp 12          issues every MMA (warps 13-15 fill its warpgroup)
+// Scores are double buffered (TMEM: 2 x 2 x 64 columns of S, P over its S, 2 x D
+// of O), so Q K^T of block j + 1 runs while the softmax of block j works, and
+// the tensor core, the exponential unit and the converters overlap.
+//
+// The reference maximum of a row moves only when a block exceeds it by more than
+// 2^1.5 (weights stay below 2^15.5, inside fp16): a rescale of O in TMEM is then
+// rare instead of once a block.
+//
+// Work: units of (row tile, 64-token block), causally pruned, in one list; every
+// CTA takes an equal contiguous share, so chunks over long contexts and mixed
+// batches fill the machine alike.  Tiles split between CTAs leave fp32 parts that
+// attend_many_join_kernel adds in order.
+//
+// Bounds per 256 x 64 step at D = 128: 1024 tensor cycles, 1024 cycles of the
+// exponential unit (16 / clock / SM), about 760 issue slots per scheduler.
+#include <algorithm>
+
+#include "w4a8_attention.cuh"
+
+namespace w4a8 {
+
+namespace {
+
+constexpr int kBlk = 64;                   // tokens per step
+constexpr int kRows = 256;                 // packed rows per tile
+constexpr int kNS = 4;                     // K and V stages
+constexpr int kScaleRing = 16;             // blocks whose page scales are kept
+constexpr int kManyThreads = 16 * 32;      // whole warpgroups: setmaxnreg moves registers between them
+constexpr int kConvWarp = 8, kMmaWarp = 12;
+constexpr int kRegsSoft = 176, kRegsConv = 88, kRegsMma = 64;      // 2, 1 and 1 warpgroups of them
+static_assert(2 * kRegsSoft + kRegsConv + kRegsMma <= 4 * 128, "the launch allocates 128 registers a thread");
+constexpr int kMinUnits = 4;               // a CTA's share is not cut below this
+constexpr float kSlack = 1.5f;             // log2 by which scores may exceed the reference maximum
+
+// wait-site ids for the status word
+enum { kAMmaK = 0x41, kAMmaV, kAMmaQ, kAMmaO, kAMmaP, kAMmaS, kASoftS, kASoftPv, kASoftEnd, kAConvK, kAConvV, kADrain };
+
+template <int D_>
+struct ManyCfg {
+    static constexpr int D = D_;
+    static constexpr int CH = D_ / 64;                       // 128-byte column chunks of a row
+    static constexpr int Q_CHUNK = 128 * 128;                // one half's rows x 128 B
+    static constexpr int Q_HALF = CH * Q_CHUNK;
+    static constexpr int KV_CHUNK = kBlk * 128;
+    static constexpr int KV_STAGE = CH * KV_CHUNK;
+    static constexpr int OFF_K = 2 * Q_HALF;
+    static constexpr int OFF_V = OFF_K + kNS * KV_STAGE;
+    static constexpr int OFF_PREFIX = OFF_V + kNS * KV_STAGE;
+    static constexpr int TM_S = 0;                           // [half][buffer] of 64 columns
+    static constexpr int TM_O = 256;                         // [half] of D columns
+    static constexpr int TM_COLS = 512;
+    static constexpr int PIECE = kRows * D_ * 4;
+    static constexpr int UNITS_PER_THREAD = kBlk * D_ / 16 / 128;   // 16-byte code vectors a converter thread moves
+};
+
+// S, P and PV phases have a barrier for each of the two buffers: every wait is
+// for a phase whose predecessor on the same barrier (two blocks back) is known to
+// be complete and whose successor cannot have completed, so parity tells.
+struct ManyBars {
+    uint64_t kfull[kNS], kempty[kNS], vfull[kNS], vempty[kNS];
+    uint64_t sfull[2][2], pready[2][2], pvdone[2][2], qfull[2], ofree[2], drain;
+    uint32_t tmem_base;
+    int abort;
+};
+
+// mbar_wait for a whole warp, with one answer for all of its lanes.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int where)
+{
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, where));
+}
+
+struct Start {           // where the CTA's share begins
+    int seq, head, tile, blk;
+    long long units;
+};
+
+__device__ __forceinline__ int many_tiles(const Seq& s, int group, int least)
+{
+    const long long rows = static_cast<long long>(s.n) * group;
+    return rows > least ? static_cast<int>((rows + kRows - 1) / kRows) : 0;
+}
+
+// 64-token blocks that some row of tile t sees (at least one: rows that see
+// nothing are written too).
+__device__ __forceinline__ int many_blocks(const Seq& s, int group, int t)
+{
+    const int last = min(s.n - 1, static_cast<int>(((static_cast<long long>(t) + 1) * kRows - 1) / group));
+    const int lim = s.len - s.n + last;
+    return lim < 0 ? 1 : lim / kBlk + 1;
+}
+
+// A piece: blocks [b0, b1) of a tile that has nb of them.
+struct Walk {
+    int seq, head, tile, b0, b1, nb;
+    Seq s;
+    long long left;
+    __device__ __forceinline__ void begin(const AttentionParams& p, const Start& st)
+    {
+        seq = st.seq;
+        head = st.head;
+        tile = st.tile;
+        b0 = st.blk;
+        left = st.units;
+        if (left > 0) {
+            s = load_seq(p.c, seq);
+            cut(p);
+        }
+    }
+    __device__ __forceinline__ void cut(const AttentionParams& p)
+    {
+        nb = many_blocks(s, p.group, tile);
+        b1 = static_cast<int>(min(static_cast<long long>(nb), b0 + left));
+    }
+    // Moves to the next piece; false when the share is done.
+    __device__ __forceinline__ bool next(const AttentionParams& p, int least)
+    {
+        left -= b1 - b0;
+        if (left <= 0) return false;
+        b0 = 0;
+        if (++tile >= many_tiles(s, p.group, least)) {
+            tile = 0;
+            if (++head >= p.c.kv_heads) {
+                head = 0;
+                do {
+                    if (++seq >= p.c.batch) return false;
+                    s = load_seq(p.c, seq);
+                } while (many_tiles(s, p.group, least) == 0);
+            }
+        }
+        cut(p);
+        return true;
+    }
+    __device__ __forceinline__ bool has_b(int group) const
+    {
+        return static_cast<long long>(s.n) * group - static_cast<long long>(tile) * kRows > 128;
+    }
+};
+
+// Shared-memory descriptor of a row-major operand whose rows are tokens and
+// whose contiguous direction is the MMA's M / N direction (128-byte swizzle):
+// 64-element chunks `chunk` bytes apart, 8-row groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t saddr, uint32_t chunk)
+{
+    uint64_t d = smem_desc_sw128(saddr);
+    d &= ~(static_cast<uint64_t>(0x3FFF) << 16);
+    d |= static_cast<uint64_t>((chunk >> 4) & 0x3FFFu) << 16;
+    return d;
+}
+
+// f16 x f16 -> f32; b_mn: B is contiguous along N.
+__host__ __device__ constexpr uint32_t idesc_f16(uint32_t M, uint32_t N, bool b_mn)
+{
+    return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((N >> 3) << 17) | ((M >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+
+// 32 lanes x 32 columns, a lane per thread of the warp.
+__device__ __forceinline__ void tm_ld32(uint32_t t, uint32_t* r)
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(t));
+}
+__device__ __forceinline__ void tm_st32(uint32_t t, const uint32_t* r)
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(t),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+// Keeps uses of r behind the wait that precedes this call (see reg_fence16).
+__device__ __forceinline__ void reg_fence32(uint32_t* r)
+{
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) reg_fence4(r + i);
+}
+
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b)
+{
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ void unpair2(uint64_t v, float& lo, float& hi)
+{
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint32_t cvt_f16x2(float lo, float hi)
+{
+    uint32_t d;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+}
+__device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w)
+{
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
+// Workspace: [grid][2] Partial, [grid][2][2][256] (m, l), [grid][2] O as [D / 4][256] float4.
+template <class C>
+struct ManyLayout {
+    static __host__ __device__ size_t ml(int grid) { return static_cast<size_t>(grid) * 2 * sizeof(Partial); }
+    static __host__ __device__ size_t o(int grid) { return ml(grid) + static_cast<size_t>(grid) * 2 * 2 * kRows * 4; }
+    static __host__ __device__ size_t total(int grid) { return o(grid) + static_cast<size_t>(grid) * 2 * C::PIECE; }
+};
+
+// ------------------------------------------------------------------ converters
+
+// One 16-byte vector of codes -> 16 fp16 values in two 16-byte units of the
+// swizzled row.
+template <class C>
+__device__ __forceinline__ void put_codes(uint32_t stage, int tok, int c, const uint4& v)
+{
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t h[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        h[2 * i] = codes_to_f16x2(__byte_perm(w[i], 0, 0x4140));
+        h[2 * i + 1] = codes_to_f16x2(__byte_perm(w[i], 0, 0x4342));
+    }
+    const uint32_t row = stage + (c >> 2) * C::KV_CHUNK + tok * 128;
+    const uint32_t u = (c & 3) * 2, x = tok & 7;
+    sts128(row + ((u ^ x) << 4), h[0], h[1], h[2], h[3]);
+    sts128(row + (((u + 1) ^ x) << 4), h[4], h[5], h[6], h[7]);
+}
+
+template <class C>
+__device__ __forceinline__ void converter_role(const AttentionParams& p, ManyBars* bars, uint32_t sm, float (*ring)[8],
+                                               const Start& st, int least, volatile int* abort_flag)
+{
+    constexpr int N = C::UNITS_PER_THREAD, PER_ROW = C::D / 16;     // vectors of a token's row
+    const int i = threadIdx.x - kConvWarp * 32;
+    const CacheView& cv = p.c;
+    // The thread's vectors of a block: token tok0 + k * 16 * (8 / PER_ROW)..., one 16-token
+    // granule (or two) per step of k.  Lanes are dealt so that the eight lanes of a
+    // store phase hit distinct banks: two tokens x four vectors.
+    const int lane = lane_id(), w = i >> 5;
+    int tok0, c;
+    if (PER_ROW == 8) {
+        tok0 = w * 4 + (lane >> 4) * 2 + ((lane >> 2) & 1);
+        c = (lane & 3) + ((lane >> 3) & 1) * 4;
+    } else {
+        tok0 = w * 8 + (lane >> 2);
+        c = lane & 3;
+    }
+    constexpr int TSTEP = 128 / PER_ROW;                            // tokens between a thread's vectors
+
+    Walk a;                      // the block being loaded
+    a.begin(p, st);
+    bool more = a.left > 0;
+    int ab = a.b0;
+    uint4 kr[N], vr[N];
+    float sc[2] = {-1.0f, -1.0f};
+    auto load = [&]() {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int tok = ab * kBlk + tok0 + k * TSTEP;
+            const int pg = tok >> cv.page_log2;
+            const int id = tok < a.s.len ? cv.table[static_cast<int64_t>(a.seq) * cv.ld_table + pg] : -1;
+            const bool ok = id >= 0 && id < cv.pages;
+            kr[k] = make_uint4(0, 0, 0, 0);
+            vr[k] = kr[k];
+            if (ok) {
+                const int64_t at = (((static_cast<int64_t>(id) * cv.kv_heads + a.head) << cv.page_log2) +
+                                    (tok & (cv.page - 1))) * C::D + c * 16;
+                kr[k] = *reinterpret_cast<const uint4*>(cv.k + at);
+                vr[k] = *reinterpret_cast<const uint4*>(cv.v + at);
+            }
+        }
+        // page scales of the block's four 16-token granules, -1 where there is no page
+        if (i < 4) {
+            const int tok = ab * kBlk + i * 16;
+            const int id = tok < a.s.len ? cv.table[static_cast<int64_t>(a.seq) * cv.ld_table + (tok >> cv.page_log2)] : -1;
+            sc[0] = sc[1] = -1.0f;
+            if (id >= 0 && id < cv.pages) {
+                const int64_t ph = static_cast<int64_t>(id) * cv.kv_heads + a.head;
+                sc[0] = cv.k_scale[ph];
+                sc[1] = cv.v_scale[ph];
+            }
+        }
+    };
+    auto step = [&]() {
+        if (++ab < a.b1) return true;
+        if (!a.next(p, least)) return false;
+        ab = a.b0;
+        return true;
+    };
+    if (more) load();
+    for (uint32_t g = 0; more; ++g) {
+        const uint32_t sg = g % kNS, ph = (g / kNS) & 1;
+        const uint32_t ks = sm + C::OFF_K + sg * C::KV_STAGE, vs = sm + C::OFF_V + sg * C::KV_STAGE;
+        uint4 kc[N], vc[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            kc[k] = kr[k];
+            vc[k] = vr[k];
+        }
+        const float s0 = sc[0], s1 = sc[1];
+        more = step();
+        if (more) load();                        // in flight while this block is converted
+        if (!warp_wait(&bars->kempty[sg], ph ^ 1, abort_flag, p.status, kAConvK)) return;
+        if (i < 4) {
+            ring[g % kScaleRing][i] = s0;
+            ring[g % kScaleRing][4 + i] = s1;
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k) put_codes<C>(ks, tok0 + k * TSTEP, c, kc[k]);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->kfull[sg]);
+        if (!warp_wait(&bars->vempty[sg], ph ^ 1, abort_flag, p.status, kAConvV)) return;
+#pragma unroll
+        for (int k = 0; k < N; ++k) put_codes<C>(vs, tok0 + k * TSTEP, c, vc[k]);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->vfull[sg]);
+    }
+}
+
+// ------------------------------------------------------------------ MMA issuer
+
+template <class C>
+__device__ __forceinline__ void mma_role(const AttentionParams& p, ManyBars* bars, uint32_t sm, uint32_t tbase,
+                                         const Start& st, int least, volatile int* abort_flag)
+{
+    constexpr uint32_t idqk = idesc_f16(128, kBlk, false), idpv = idesc_f16(128, C::D, true);
+    Walk a;
+    a.begin(p, st);
+    bool more = a.left > 0, ok = true;
+    uint32_t g = 0;                 // blocks issued (K, V stages)
+    uint32_t n[2] = {0, 0};         // blocks issued of each half
+    uint32_t seg[2] = {0, 0};       // pieces of each half
+    auto wait = [&](uint64_t* b, uint32_t parity, int where) {
+        ok = ok && mbar_wait(b, parity, abort_flag, p.status, where);
+        return ok;
+    };
+    // PV of the half's block number m (stage sg), the piece's first with acc = 0
+    auto pv = [&](int x, uint32_t m, uint32_t sg, bool first) {
+        if (!wait(&bars->pready[x][m & 1], (m >> 1) & 1, kAMmaP)) return;
+        tc_fence_after();
+        const uint32_t d = tbase + C::TM_O + x * C::D, ap = tbase + C::TM_S + (x * 2 + (m & 1)) * kBlk;
+        const uint32_t v = sm + C::OFF_V + sg * C::KV_STAGE;
+#pragma unroll
+        for (int k = 0; k < kBlk / 16; ++k)
+            mma_ts(d, ap + k * 8, smem_desc_mn(v + k * 2048, C::KV_CHUNK), idpv, first && k == 0 ? 0u : 1u);
+        tc_commit(&bars->pvdone[x][m & 1]);
+    };
+    while (more && ok) {
+        const int halves = a.has_b(p.group) ? 2 : 1;
+        for (int x = 0; x < halves && ok; ++x) wait(&bars->qfull[x], seg[x] & 1, kAMmaQ);
+        const int steps = a.b1 - a.b0;
+        for (int j = 0; j <= steps && ok; ++j) {
+            if (j < steps) {
+                const uint32_t sg = g % kNS;
+                if (!wait(&bars->kfull[sg], (g / kNS) & 1, kAMmaK)) break;
+                tc_fence_after();
+                for (int x = 0; x < halves && ok; ++x) {
+                    // the S buffer is free once the PV that read its P, two blocks back, is done
+                    if (n[x] >= 2 && !wait(&bars->pvdone[x][n[x] & 1], ((n[x] - 2) >> 1) & 1, kAMmaS)) break;
+                    tc_fence_after();
+                    const uint32_t d = tbase + C::TM_S + (x * 2 + (n[x] & 1)) * kBlk;
+#pragma unroll
+                    for (int k = 0; k < C::D / 16; ++k)
+                        mma_ss(d, smem_desc_sw128(sm + x * C::Q_HALF + (k >> 2) * C::Q_CHUNK + (k & 3) * 32),
+                               smem_desc_sw128(sm + C::OFF_K + sg * C::KV_STAGE + (k >> 2) * C::KV_CHUNK + (k & 3) * 32),
+                               idqk, k == 0 ? 0u : 1u);
+                    tc_commit(&bars->sfull[x][n[x] & 1]);
+                    ++n[x];
+                }
+                if (!ok) break;
+                tc_commit(&bars->kempty[sg]);
+                ++g;
+            }
+            if (j > 0) {
+                const uint32_t gv = j < steps ? g - 2 : g - 1;       // the block before the one just issued
+                const uint32_t sg = gv % kNS;
+                if (!wait(&bars->vfull[sg], (gv / kNS) & 1, kAMmaV)) break;
+                for (int x = 0; x < halves && ok; ++x) {
+                    // the piece's first PV overwrites O: the half's previous output must have been read
+                    if (j == 1 && seg[x] > 0 && !wait(&bars->ofree[x], (seg[x] - 1) & 1, kAMmaO)) break;
+                    pv(x, j < steps ? n[x] - 2 : n[x] - 1, sg, j == 1);
+                }
+                if (!ok) break;
+                tc_commit(&bars->vempty[sg]);
+            }
+        }
+        for (int x = 0; x < halves; ++x) ++seg[x];
+        if (ok) more = a.next(p, least);
+    }
+    // nothing of this thread's is in flight when TMEM is freed
+    tc_commit(&bars->drain);
+    mbar_wait(&bars->drain, 0, abort_flag, p.status, kADrain);
+}
+
+// ------------------------------------------------------------------ softmax
+
+template <class C>
+__device__ __forceinline__ void softmax_role(const AttentionParams& p, ManyBars* bars, uint32_t sm, uint32_t tbase,
+                                             float (*ring)[8], const Start& st, int least, volatile int* abort_flag)
+{
+    const int x = warp_id() >> 2;                               // half
+    const int row = threadIdx.x & 127;                          // row within it, and TMEM lane
+    const int lane = lane_id();
+    const uint32_t lane_off = static_cast<uint32_t>(row & 96) << 16;
+    const uint32_t t_o = tbase + lane_off + C::TM_O + x * C::D;
+    const uint32_t q_sm = sm + x * C::Q_HALF + row * 128;
+    Partial* info = reinterpret_cast<Partial*>(p.ws) + 2 * blockIdx.x;
+    float* ml = reinterpret_cast<float*>(p.ws + ManyLayout<C>::ml(gridDim.x)) + static_cast<size_t>(blockIdx.x) * 4 * kRows;
+    float* po = reinterpret_cast<float*>(p.ws + ManyLayout<C>::o(gridDim.x) + static_cast<size_t>(blockIdx.x) * 2 * C::PIECE);
+    if (threadIdx.x < 2) info[threadIdx.x] = Partial{-1, 0, 0, 0, 0};
+    __syncwarp();
+
+    Walk a;
+    a.begin(p, st);
+    bool more = a.left > 0;
+    uint32_t g = 0, n = 0;           // blocks of the CTA, of this half
+    while (more) {
+        const int steps = a.b1 - a.b0;
+        if (x == 1 && !a.has_b(p.group)) {
+            g += steps;
+            more = a.next(p, least);
+            continue;
+        }
+        const int pr = a.tile * kRows + x * 128 + row;          // packed row
+        const bool valid = pr < a.s.n * p.group;
+        const bool live = __any_sync(0xffffffffu, valid);
+
+        // ---- this row's query: largest element to [2^13, 2^14), fp16, into the operand ----
+        float qs = 0.0f;                                        // what turns a raw score into log2 units
+        int limit = 0x7FFFFFFF;                                 // last token the row sees
+        {
+            uint4 v[C::D / 8];
+            const int tok = valid ? pr / p.group : 0;
+            const uint16_t* src = p.q + static_cast<int64_t>(a.s.q0 + tok) * p.ldq +
+                                  static_cast<int64_t>(a.head * p.group + (valid ? pr - tok * p.group : 0)) * C::D;
+#pragma unroll
+            for (int i = 0; i < C::D / 8; ++i) v[i] = valid ? *reinterpret_cast<const uint4*>(src + 8 * i) : make_uint4(0, 0, 0, 0);
+            uint32_t big = 0;
+#pragma unroll
+            for (int i = 0; i < C::D / 8; ++i) {
+                const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) big = max(big, max((w[e] << 16) & 0x7FFFFFFFu, w[e] & 0x7FFF0000u));
+            }
+            const float shrink = row_shrink(__uint_as_float(big));
+            qs = __fdiv_rn(p.scale_log2, shrink);
+            if (valid) limit = a.s.len - a.s.n + tok;
+#pragma unroll
+            for (int i = 0; i < C::D / 8; ++i) {
+                const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+                uint32_t h[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    h[e] = cvt_f16x2(__uint_as_float(w[e] << 16) * shrink, __uint_as_float(w[e] & 0xFFFF0000u) * shrink);
+                sts128(q_sm + (i >> 3) * C::Q_CHUNK + (((i & 7) ^ (row & 7)) << 4), h[0], h[1], h[2], h[3]);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->qfull[x]);
+        }
+        const int min_limit = __reduce_min_sync(0xffffffffu, limit);
+
+        float m = kNegInf, l = 0.0f, vr = kVrMin, vr_inv = kWeightOne / kVrMin;
+        for (int j = 0; j < steps; ++j, ++g, ++n) {
+            if (!warp_wait(&bars->sfull[x][n & 1], (n >> 1) & 1, abort_flag, p.status, kASoftS)) return;
+            if (live) {
+                tc_fence_after();
+                const uint32_t t_s = tbase + lane_off + C::TM_S + (x * 2 + (n & 1)) * kBlk;
+                uint32_t s[kBlk];
+                tm_ld32(t_s, s);
+                tm_ld32(t_s + 32, s + 32);
+                tc_wait_ld();
+                reg_fence32(s);
+                reg_fence32(s + 32);
+                const float* rg = ring[g % kScaleRing];
+                float f[4], vs[4];
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    f[b] = rg[b] * qs;
+                    vs[b] = rg[4 + b];
+                }
+                const int t0 = (a.b0 + j) * kBlk;
+                // (a page scale below 0 marks tokens without a page; NaN scales pass on)
+                const bool gone = rg[0] < 0.0f || rg[1] < 0.0f || rg[2] < 0.0f || rg[3] < 0.0f;
+                const bool edge = gone || t0 + kBlk - 1 > min_limit;
+                if (edge) {
+                    // masked scores become -inf before their granule's factor (a positive
+                    // one: zero, NaN and infinite scales must not touch them)
+#pragma unroll
+                    for (int i = 0; i < kBlk; ++i)
+                        if (t0 + i > limit || rg[i >> 4] < 0.0f) s[i] = 0xFF800000u;
+                }
+                // ---- reference maximum ----
+                float mx = kNegInf;
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    float r = __uint_as_float(s[16 * b]);
+#pragma unroll
+                    for (int i = 1; i < 16; ++i) r = fmaxf(r, __uint_as_float(s[16 * b + i]));
+                    if (r > kNegInf) mx = fmaxf(mx, r * f[b]);
+                }
+                const float vmax = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
+                const bool grow = mx > m + kSlack || (m == kNegInf && mx > m) || vmax > vr;
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float mn = fmaxf(m, mx), vn = fmaxf(vr, pow2_above(vmax));
+                    const float al = mn == kNegInf ? 1.0f : ex2(m - mn), av = al * __fdiv_rn(vr, vn);
+                    m = mn;
+                    l *= al;
+                    vr = vn;
+                    vr_inv = __fdiv_rn(kWeightOne, vr);
+                    if (j > 0) {
+                        if (!warp_wait(&bars->pvdone[x][(n - 1) & 1], ((n - 1) >> 1) & 1, abort_flag, p.status, kASoftPv)) return;
+                        tc_fence_after();
+                        // O is scaled 32 columns at a time
+#pragma unroll
+                        for (int c = 0; c < C::D; c += 32) {
+                            uint32_t o[32];
+                            tm_ld32(t_o + c, o);
+                            tc_wait_ld();
+                            reg_fence32(o);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * av);
+                            tm_st32(t_o + c, o);
+                        }
+                        tc_wait_st();
+                    }
+                }
+                // ---- weights ----
+                const float neg_m = m == kNegInf ? 0.0f : -m;
+                uint32_t pk[kBlk / 2];
+                uint64_t sum = 0;
+                if (!edge) {
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        const uint64_t f2 = pair2(f[b], f[b]), m2 = pair2(neg_m, neg_m);
+                        const float wv = vs[b] * vr_inv;
+                        const uint64_t w2 = pair2(wv, wv);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int e = 16 * b + 2 * i;
+                            float lo, hi;
+                            unpair2(f2_fma(pair2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), f2, m2), lo, hi);
+                            const uint64_t pp = pair2(ex2(lo), ex2(hi));
+                            sum = f2_add(sum, pp);
+                            unpair2(f2_mul(pp, w2), lo, hi);
+                            pk[8 * b + i] = cvt_f16x2(lo, hi);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        const float wv = vs[b] * vr_inv;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int e = 16 * b + 2 * i;
+                            float pp[2], ww[2];
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const bool hidden = t0 + e + h > limit || rg[b] < 0.0f;
+                                pp[h] = hidden ? 0.0f : ex2(fmaf(__uint_as_float(s[e + h]), f[b], neg_m));
+                                ww[h] = hidden ? 0.0f : pp[h] * wv;
+                            }
+                            sum = f2_add(sum, pair2(pp[0], pp[1]));
+                            pk[8 * b + i] = cvt_f16x2(ww[0], ww[1]);
+                        }
+                    }
+                }
+                float lo, hi;
+                unpair2(sum, lo, hi);
+                l += lo + hi;
+                tm_st32(t_s, pk);
+                tc_wait_st();
+                tc_fence_before();
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->pready[x][n & 1]);
+        }
+
+        // ---- the piece's output ----
+        if (!warp_wait(&bars->pvdone[x][(n - 1) & 1], ((n - 1) >> 1) & 1, abort_flag, p.status, kASoftEnd)) return;
+        if (live) {
+            tc_fence_after();
+            const float back = vr * (1.0f / kWeightOne);
+            const bool whole = a.b0 == 0 && a.b1 == a.nb;
+            const int slot = a.b0 == 0 ? 1 : 0;
+            const float inv = whole ? inv_sum(l) * back : back;
+            uint16_t* dst = whole && valid ? out_row(p, a.s, a.head, pr) : nullptr;
+            float4* part = reinterpret_cast<float4*>(po + static_cast<size_t>(slot) * kRows * C::D) + x * 128 + row;
+#pragma unroll
+            for (int c = 0; c < C::D; c += 32) {
+                uint32_t o[32];
+                tm_ld32(t_o + c, o);
+                tc_wait_ld();
+                reg_fence32(o);
+                float v[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(o[i]) * inv;
+                if (whole) {
+                    if (valid)
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8)
+                            *reinterpret_cast<uint4*>(dst + c + i) =
+                                make_uint4(pack_bf16(v[i], v[i + 1]), pack_bf16(v[i + 2], v[i + 3]),
+                                           pack_bf16(v[i + 4], v[i + 5]), pack_bf16(v[i + 6], v[i + 7]));
+                } else if (valid) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        part[static_cast<size_t>((c + i) / 4) * kRows] = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                }
+            }
+            if (!whole) {
+                ml[slot * 2 * kRows + x * 128 + row] = m;
+                ml[slot * 2 * kRows + kRows + x * 128 + row] = l;
+                if (x == 0 && row == 0)
+                    info[slot] = Partial{(static_cast<long long>(a.seq) * p.c.kv_heads + a.head) * 0x1000000LL + a.tile, a.seq,
+                                         a.head, a.tile, 0};
+            }
+            tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->ofree[x]);
+        more = a.next(p, least);
+    }
+}
+
+// ------------------------------------------------------------------ kernel
+
+template <class C>
+__global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const AttentionParams p, const int least)
+{
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ ManyBars bars_;
+    __shared__ float ring[kScaleRing][8];
+    __shared__ Start start;
+    ManyBars* bars = &bars_;
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    long long* prefix = reinterpret_cast<long long*>(smem + C::OFF_PREFIX);
+    const int warp = warp_id(), lane = lane_id();
+    const CacheView& cv = p.c;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kNS; ++i) {
+            mbar_init(&bars->kfull[i], 4);
+            mbar_init(&bars->kempty[i], 1);
+            mbar_init(&bars->vfull[i], 4);
+            mbar_init(&bars->vempty[i], 1);
+        }
+        for (int x = 0; x < 2; ++x) {
+            for (int b = 0; b < 2; ++b) {
+                mbar_init(&bars->sfull[x][b], 1);
+                mbar_init(&bars->pready[x][b], 4);
+                mbar_init(&bars->pvdone[x][b], 1);
+            }
+            mbar_init(&bars->qfull[x], 4);
+            mbar_init(&bars->ofree[x], 4);
+        }
+        mbar_init(&bars->drain, 1);
+        bars->abort = 0;
+        fence_mbar_init();
+    }
+    if (warp == kMmaWarp) {
+        tmem_alloc(&bars->tmem_base, C::TM_COLS);
+        tmem_relinquish();
+    }
+    pdl_wait();
+
+    // ---- units of each sequence: a warp sums its tiles' blocks ----
+    for (int s = warp; s < cv.batch; s += kManyThreads / 32) {
+        const Seq q = load_seq(cv, s);
+        const int tiles = many_tiles(q, p.group, least);
+        long long u = 0;
+        for (int t = lane; t < tiles; t += 32) u += many_blocks(q, p.group, t);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+        if (lane == 0) prefix[s] = u * cv.kv_heads;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        long long run = 0;
+        for (int base = 0; base < cv.batch; base += 32) {
+            const int s = base + lane;
+            const long long u = s < cv.batch ? prefix[s] : 0;
+            long long v = u;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long y = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v += y;
+            }
+            if (s < cv.batch) prefix[s] = run + v - u;
+            run += __shfl_sync(0xffffffffu, v, 31);
+        }
+        __syncwarp();
+        const long long W = min(static_cast<long long>(gridDim.x), (run + kMinUnits - 1) / kMinUnits);
+        const long long c = blockIdx.x;
+        const long long u0 = c < W ? run * c / W : run, u1 = c < W ? run * (c + 1) / W : run;
+        Start st{0, 0, 0, 0, u1 - u0};
+        if (u0 < u1) {
+            int lo = 0, hi = cv.batch - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (prefix[mid] <= u0) lo = mid;
+                else hi = mid - 1;
+            }
+            const Seq q = load_seq(cv, lo);
+            const long long per_head = ((lo + 1 < cv.batch ? prefix[lo + 1] : run) - prefix[lo]) / cv.kv_heads;
+            const long long off = u0 - prefix[lo];
+            st.seq = lo;
+            st.head = static_cast<int>(off / per_head);
+            long long r = off - st.head * per_head;
+            // the tile that holds block r of the head
+            const int tiles = many_tiles(q, p.group, least);
+            for (int base = 0; base < tiles; base += 32) {
+                const int t = base + lane;
+                const long long u = t < tiles ? many_blocks(q, p.group, t) : 0;
+                long long v = u;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const long long y = __shfl_up_sync(0xffffffffu, v, o);
+                    if (lane >= o) v += y;
+                }
+                const unsigned hit = __ballot_sync(0xffffffffu, v > r);
+                if (hit) {
+                    const int w = __ffs(hit) - 1;
+                    st.tile = base + w;
+                    st.blk = static_cast<int>(r - __shfl_sync(0xffffffffu, v - u, w));
+                    break;
+                }
+                r -= __shfl_sync(0xffffffffu, v, 31);
+            }
+        }
+        if (lane == 0) start = st;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tbase = bars->tmem_base, sm = smem_u32(smem);
+    volatile int* abort_flag = &bars->abort;
+    const Start st = start;
+
+    if (warp < kConvWarp) {
+        regs_inc<kRegsSoft>();
+        softmax_role<C>(p, bars, sm, tbase, ring, st, least, abort_flag);
+    } else if (warp < kMmaWarp) {
+        regs_dec<kRegsConv>();
+        converter_role<C>(p, bars, sm, ring, st, least, abort_flag);
+    } else {
+        regs_dec<kRegsMma>();
+        if (warp == kMmaWarp && elect_one()) mma_role<C>(p, bars, sm, tbase, st, least, abort_flag);
+    }
+    pdl_launch_dependents();
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tc_fence_after();
+        tmem_dealloc(tbase, C::TM_COLS);
+    }
+}
+
+// Joins the parts of tiles that span CTAs: blockIdx.x leads the tile that begins
+// in CTA blockIdx.x and goes on; blockIdx.y takes 16 of its rows.
+constexpr int kJoinRows = 16;
+
+template <class C>
+__global__ void __launch_bounds__(256) attend_many_join_kernel(const AttentionParams p, const int nctas)
+{
+    pdl_launch_dependents();
+    pdl_wait();
+    const Partial* info = reinterpret_cast<const Partial*>(p.ws);
+    const float* ml = reinterpret_cast<const float*>(p.ws + ManyLayout<C>::ml(nctas));
+    const float4* po = reinterpret_cast<const float4*>(p.ws + ManyLayout<C>::o(nctas));
+    const int lead_cta = blockIdx.x;
+    const Partial lead = info[2 * lead_cta + 1];
+    if (lead.seg < 0) return;
+    const Seq s = load_seq(p.c, lead.seq);
+    int last = lead_cta;
+    while (last + 1 < nctas && info[2 * (last + 1)].seg == lead.seg) ++last;
+    for (int idx = threadIdx.x; idx < kJoinRows * C::D / 4; idx += 256) {
+        const int row = blockIdx.y * kJoinRows + idx % kJoinRows, d4 = idx / kJoinRows;
+        const int pr = lead.tile * kRows + row;
+        if (pr >= s.n * p.group) continue;
+        float mx = kNegInf;
+        for (int k = lead_cta; k <= last; ++k) mx = fmaxf(mx, ml[(2 * k + (k == lead_cta)) * 2 * kRows + row]);
+        float ls = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int k = lead_cta; k <= last; ++k) {
+            const size_t sl = 2 * k + (k == lead_cta);
+            const float a = mx == kNegInf ? 1.0f : ex2(ml[sl * 2 * kRows + row] - mx);
+            const float4 v = po[sl * (kRows * C::D / 4) + static_cast<size_t>(d4) * kRows + row];
+            ls += a * ml[sl * 2 * kRows + kRows + row];
+            o.x += a * v.x;
+            o.y += a * v.y;
+            o.z += a * v.z;
+            o.w += a * v.w;
+        }
+        const float inv = inv_sum(ls);
+        *reinterpret_cast<uint2*>(out_row(p, s, lead.head, pr) + d4 * 4) =
+            make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+    }
+}
+
+template <class C>
+cudaError_t launch_many(const AttentionParams& p, int sms, cudaStream_t stream)
+{
+    const int fixed = C::OFF_PREFIX + 1024;
+    static bool ready[64] = {};          // per device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64 || !ready[dev]) {
+        e = cudaFuncSetAttribute(attend_many_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, fixed + kMaxBatch * 8);
+        if (e != cudaSuccess) return e;
+        // setmaxnreg draws on the launch's registers: a build with fewer than the split needs must not start
+        cudaFuncAttributes fa{};
+        if ((e = cudaFuncGetAttributes(&fa, attend_many_kernel<C>)) != cudaSuccess) return e;
+        if (fa.numRegs * 4 < 2 * kRegsSoft + kRegsConv + kRegsMma) return cudaErrorInvalidConfiguration;
+        if (dev >= 0 && dev < 64) ready[dev] = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(sms);
+    cfg.blockDim = dim3(kManyThreads);
+    cfg.dynamicSmemBytes = fixed + p.c.batch * 8;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, attend_many_kernel<C>, p, p.c.batch == 1 ? 0 : kFewRows);
+    if (e != cudaSuccess) return e;
+    cfg.gridDim = dim3(sms, kRows / kJoinRows);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 0;
+    return cudaLaunchKernelEx(&cfg, attend_many_join_kernel<C>, p, sms);
+}
+
+}  // namespace
+
+size_t attend_many_ws_bytes(int D, int sms)
+{
+    return D == 128 ? ManyLayout<ManyCfg<128>>::total(sms) : ManyLayout<ManyCfg<64>>::total(sms);
+}
+
+cudaError_t launch_attend_many(const AttentionParams& p, int sms, cudaStream_t stream)
+{
+    return p.c.D == 128 ? launch_many<ManyCfg<128>>(p, sms, stream) : launch_many<ManyCfg<64>>(p, sms, stream);
+}
+
+}  // namespace w4a8

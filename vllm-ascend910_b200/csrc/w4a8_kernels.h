@@ -219,6 +219,7 @@ struct AttentionParams {
     int q_heads, group;       // group: query heads per kv head
     int max_q;                // no sequence has more query tokens (host's knowledge)
     float scale_log2;         // softmax scale * log2(e)
+    int few_most;             // attend_few_kernel takes sequences of at most this many packed rows
     int* status;              // workspace: status word
     uint8_t* ws;              // workspace past the status block
 };
