@@ -325,7 +325,7 @@ W4A8_API int w4a8_kv_read(const w4a8_kv_cache* cache, const int32_t* page_table,
  * tokens j at or before query token t's position, k and v of kv head
  * h / (q_heads / kv_heads); a row that sees no token is zero.  q, out bf16
  * [tokens, ld] (q_heads * head_dim used; rows 16-byte aligned, ld a multiple of
- * 8).  max_q_len: no sequence has more query tokens than that (rows past it
+ * 8).  softmax_scale >= 0.  max_q_len: no sequence has more query tokens than that (rows past it
  * are not computed).  batch <= W4A8_ATTENTION_MAX_BATCH.  Workspace as for the
  * linear calls (w4a8_attention_workspace_size bytes, 1024-byte aligned, zeroed
  * before first use, may be shared with them in stream order). */

@@ -129,7 +129,7 @@ def test_cache_argument_contract():
                                 None)
 
     assert attend(T=0) == _lib.OK and attend(hq=3) == inv and attend(hq=0) == inv and attend(mq=0) == inv
-    assert attend(scale=float("nan")) == inv and attend(B=_lib.ATTENTION_MAX_BATCH + 1) == uns
+    assert attend(scale=float("nan")) == inv and attend(scale=-0.1) == inv and attend(B=_lib.ATTENTION_MAX_BATCH + 1) == uns
     assert attend(q=None) == inv and attend(ldo=255) == inv and attend(out=9 * A + 2) == inv
     assert attend() in (_lib.ERR_CUDA, _lib.ERR_DEVICE, _lib.ERR_WORKSPACE)
     assert L.w4a8_attention_workspace_size(2, 6, 4, 2, 64, 3) > 0

@@ -21,12 +21,13 @@
 // the tensor core, the exponential unit and the converters overlap.
 //
 // The reference maximum of a row moves only when a block exceeds it by more than
-// 2^1.5 (weights stay below 2^15.5, inside fp16): a rescale of O in TMEM is then
-// rare instead of once a block.
+// 2^1.9 (weights stay below 2^15.9, inside fp16), and then to 2^2 above what was
+// seen: a rescale of O in TMEM is rare instead of once a block, at the price of
+// two of the 28 binades below the largest weight that keep all 11 bits.
 //
-// Work: units of (row tile, 64-token block), causally pruned, in one list; every
-// CTA takes an equal contiguous share, so chunks over long contexts and mixed
-// batches fill the machine alike.  Tiles split between CTAs leave fp32 parts that
+// Work: units of (row tile, 64-token block), causally pruned, and a few for each
+// tile's beginning and end, in one list; every CTA takes an equal contiguous
+// share, so chunks over long contexts and mixed batches fill the machine alike.  Tiles split between CTAs leave fp32 parts that
 // attend_many_join_kernel adds in order.
 //
 // Bounds per 256 x 64 step at D = 128: 1024 tensor cycles, 1024 cycles of the
@@ -47,8 +48,10 @@ constexpr int kManyThreads = 16 * 32;      // whole warpgroups: setmaxnreg moves
 constexpr int kConvWarp = 8, kMmaWarp = 12;
 constexpr int kRegsSoft = 176, kRegsConv = 88, kRegsMma = 64;      // 2, 1 and 1 warpgroups of them
 static_assert(2 * kRegsSoft + kRegsConv + kRegsMma <= 4 * 128, "the launch allocates 128 registers a thread");
+constexpr int kTileUnits = 4;              // what beginning and ending a tile costs, in blocks (work shares)
 constexpr int kMinUnits = 4;               // a CTA's share is not cut below this
-constexpr float kSlack = 1.5f;             // log2 by which scores may exceed the reference maximum
+constexpr float kSlack = 1.9f;             // log2 by which scores may exceed the reference maximum
+constexpr float kMargin = 2.0f;            // log2 by which a new reference exceeds the scores seen
 
 // wait-site ids for the status word
 enum { kAMmaK = 0x41, kAMmaV, kAMmaQ, kAMmaO, kAMmaP, kAMmaS, kASoftS, kASoftPv, kASoftEnd, kAConvK, kAConvV, kADrain };
@@ -87,8 +90,8 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, where));
 }
 
-struct Start {           // where the CTA's share begins
-    int seq, head, tile, blk;
+struct Start {           // where the CTA's share begins: unit `unit` of a tile
+    int seq, head, tile, unit;
     long long units;
 };
 
@@ -107,34 +110,40 @@ __device__ __forceinline__ int many_blocks(const Seq& s, int group, int t)
     return lim < 0 ? 1 : lim / kBlk + 1;
 }
 
+// Units of a tile in the work list: kTileUnits for its queries and output, then
+// its blocks.
+__device__ __forceinline__ int many_units(const Seq& s, int group, int t) { return kTileUnits + many_blocks(s, group, t); }
+
 // A piece: blocks [b0, b1) of a tile that has nb of them.
 struct Walk {
     int seq, head, tile, b0, b1, nb;
     Seq s;
     long long left;
-    __device__ __forceinline__ void begin(const AttentionParams& p, const Start& st)
+    // False when the share has no block.
+    __device__ __forceinline__ bool begin(const AttentionParams& p, const Start& st, int least)
     {
         seq = st.seq;
         head = st.head;
         tile = st.tile;
-        b0 = st.blk;
         left = st.units;
-        if (left > 0) {
-            s = load_seq(p.c, seq);
-            cut(p);
-        }
+        if (left <= 0) return false;
+        s = load_seq(p.c, seq);
+        return cut(p, st.unit) || next(p, least);
     }
-    __device__ __forceinline__ void cut(const AttentionParams& p)
+    // The blocks of the current tile from its unit u0 on that are within the share.
+    __device__ __forceinline__ bool cut(const AttentionParams& p, int u0)
     {
         nb = many_blocks(s, p.group, tile);
-        b1 = static_cast<int>(min(static_cast<long long>(nb), b0 + left));
+        const int u1 = static_cast<int>(min(static_cast<long long>(kTileUnits + nb), u0 + left));
+        left -= u1 - u0;
+        b0 = max(u0 - kTileUnits, 0);
+        b1 = max(u1 - kTileUnits, 0);
+        return b1 > b0;
     }
     // Moves to the next piece; false when the share is done.
     __device__ __forceinline__ bool next(const AttentionParams& p, int least)
     {
-        left -= b1 - b0;
         if (left <= 0) return false;
-        b0 = 0;
         if (++tile >= many_tiles(s, p.group, least)) {
             tile = 0;
             if (++head >= p.c.kv_heads) {
@@ -145,8 +154,7 @@ struct Walk {
                 } while (many_tiles(s, p.group, least) == 0);
             }
         }
-        cut(p);
-        return true;
+        return cut(p, 0);     // (without a block it is the share's last tile)
     }
     __device__ __forceinline__ bool has_b(int group) const
     {
@@ -286,23 +294,33 @@ __device__ __forceinline__ void converter_role(const AttentionParams& p, ManyBar
     }
     constexpr int TSTEP = 128 / PER_ROW;                            // tokens between a thread's vectors
 
-    Walk a;                      // the block being loaded
-    a.begin(p, st);
-    bool more = a.left > 0;
+    // Three blocks are on their way: page ids of the one after next (a), codes of
+    // the next (kr, vr, in registers), and the block being converted.
+    Walk a;
+    bool have_id = a.begin(p, st, least);
     int ab = a.b0;
+    int id[N], sid = -1, head = 0, base = 0;
     uint4 kr[N], vr[N];
     float sc[2] = {-1.0f, -1.0f};
-    auto load = [&]() {
+    auto load_ids = [&]() {
+        const int32_t* row = cv.table + static_cast<int64_t>(a.seq) * cv.ld_table;
+        head = a.head;
+        base = ab * kBlk;
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            const int tok = ab * kBlk + tok0 + k * TSTEP;
-            const int pg = tok >> cv.page_log2;
-            const int id = tok < a.s.len ? cv.table[static_cast<int64_t>(a.seq) * cv.ld_table + pg] : -1;
-            const bool ok = id >= 0 && id < cv.pages;
+            const int tok = base + tok0 + k * TSTEP;
+            id[k] = tok < a.s.len ? row[tok >> cv.page_log2] : -1;
+        }
+        if (i < 4) sid = base + i * 16 < a.s.len ? row[(base + i * 16) >> cv.page_log2] : -1;
+    };
+    auto load_codes = [&]() {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
             kr[k] = make_uint4(0, 0, 0, 0);
             vr[k] = kr[k];
-            if (ok) {
-                const int64_t at = (((static_cast<int64_t>(id) * cv.kv_heads + a.head) << cv.page_log2) +
+            if (id[k] >= 0 && id[k] < cv.pages) {
+                const int tok = base + tok0 + k * TSTEP;
+                const int64_t at = (((static_cast<int64_t>(id[k]) * cv.kv_heads + head) << cv.page_log2) +
                                     (tok & (cv.page - 1))) * C::D + c * 16;
                 kr[k] = *reinterpret_cast<const uint4*>(cv.k + at);
                 vr[k] = *reinterpret_cast<const uint4*>(cv.v + at);
@@ -310,48 +328,48 @@ __device__ __forceinline__ void converter_role(const AttentionParams& p, ManyBar
         }
         // page scales of the block's four 16-token granules, -1 where there is no page
         if (i < 4) {
-            const int tok = ab * kBlk + i * 16;
-            const int id = tok < a.s.len ? cv.table[static_cast<int64_t>(a.seq) * cv.ld_table + (tok >> cv.page_log2)] : -1;
             sc[0] = sc[1] = -1.0f;
-            if (id >= 0 && id < cv.pages) {
-                const int64_t ph = static_cast<int64_t>(id) * cv.kv_heads + a.head;
+            if (sid >= 0 && sid < cv.pages) {
+                const int64_t ph = static_cast<int64_t>(sid) * cv.kv_heads + head;
                 sc[0] = cv.k_scale[ph];
                 sc[1] = cv.v_scale[ph];
             }
         }
     };
-    auto step = [&]() {
-        if (++ab < a.b1) return true;
-        if (!a.next(p, least)) return false;
-        ab = a.b0;
-        return true;
+    auto step_ids = [&]() {
+        if (++ab >= a.b1) {
+            have_id = a.next(p, least);
+            ab = a.b0;
+        }
+        if (have_id) load_ids();
     };
-    if (more) load();
+    bool more = have_id;
+    if (have_id) {
+        load_ids();
+        load_codes();
+        step_ids();
+    }
     for (uint32_t g = 0; more; ++g) {
         const uint32_t sg = g % kNS, ph = (g / kNS) & 1;
         const uint32_t ks = sm + C::OFF_K + sg * C::KV_STAGE, vs = sm + C::OFF_V + sg * C::KV_STAGE;
-        uint4 kc[N], vc[N];
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            kc[k] = kr[k];
-            vc[k] = vr[k];
-        }
-        const float s0 = sc[0], s1 = sc[1];
-        more = step();
-        if (more) load();                        // in flight while this block is converted
         if (!warp_wait(&bars->kempty[sg], ph ^ 1, abort_flag, p.status, kAConvK)) return;
         if (i < 4) {
-            ring[g % kScaleRing][i] = s0;
-            ring[g % kScaleRing][4 + i] = s1;
+            ring[g % kScaleRing][i] = sc[0];
+            ring[g % kScaleRing][4 + i] = sc[1];
         }
 #pragma unroll
-        for (int k = 0; k < N; ++k) put_codes<C>(ks, tok0 + k * TSTEP, c, kc[k]);
+        for (int k = 0; k < N; ++k) put_codes<C>(ks, tok0 + k * TSTEP, c, kr[k]);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->kfull[sg]);
         if (!warp_wait(&bars->vempty[sg], ph ^ 1, abort_flag, p.status, kAConvV)) return;
 #pragma unroll
-        for (int k = 0; k < N; ++k) put_codes<C>(vs, tok0 + k * TSTEP, c, vc[k]);
+        for (int k = 0; k < N; ++k) put_codes<C>(vs, tok0 + k * TSTEP, c, vr[k]);
+        more = have_id;
+        if (more) {
+            load_codes();
+            step_ids();
+        }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->vfull[sg]);
@@ -365,67 +383,72 @@ __device__ __forceinline__ void mma_role(const AttentionParams& p, ManyBars* bar
                                          const Start& st, int least, volatile int* abort_flag)
 {
     constexpr uint32_t idqk = idesc_f16(128, kBlk, false), idpv = idesc_f16(128, C::D, true);
+    const uint64_t q_desc = smem_desc_sw128(sm), k_desc = smem_desc_sw128(sm + C::OFF_K);
+    const uint64_t v_desc = smem_desc_mn(sm + C::OFF_V, C::KV_CHUNK);
     Walk a;
-    a.begin(p, st);
-    bool more = a.left > 0, ok = true;
+    bool more = a.begin(p, st, least), ok = true;
     uint32_t g = 0;                 // blocks issued (K, V stages)
-    uint32_t n[2] = {0, 0};         // blocks issued of each half
-    uint32_t seg[2] = {0, 0};       // pieces of each half
+    uint32_t na = 0, nb = 0;        // blocks issued of each half
+    uint32_t sa = 0, sb = 0;        // pieces of each half
     auto wait = [&](uint64_t* b, uint32_t parity, int where) {
         ok = ok && mbar_wait(b, parity, abort_flag, p.status, where);
         return ok;
     };
-    // PV of the half's block number m (stage sg), the piece's first with acc = 0
-    auto pv = [&](int x, uint32_t m, uint32_t sg, bool first) {
-        if (!wait(&bars->pready[x][m & 1], (m >> 1) & 1, kAMmaP)) return;
+    // Descriptors count 16-byte units.
+    auto qk = [&](int x, uint32_t n, uint32_t sg) {
+        // the S buffer is free once the PV that read its P, two blocks back, is done
+        if (n >= 2 && !wait(&bars->pvdone[x][n & 1], ((n - 2) >> 1) & 1, kAMmaS)) return;
         tc_fence_after();
-        const uint32_t d = tbase + C::TM_O + x * C::D, ap = tbase + C::TM_S + (x * 2 + (m & 1)) * kBlk;
-        const uint32_t v = sm + C::OFF_V + sg * C::KV_STAGE;
+        const uint32_t d = tbase + C::TM_S + (x * 2 + (n & 1)) * kBlk;
+        const uint64_t qd = q_desc + x * (C::Q_HALF / 16), kd = k_desc + sg * (C::KV_STAGE / 16);
 #pragma unroll
-        for (int k = 0; k < kBlk / 16; ++k)
-            mma_ts(d, ap + k * 8, smem_desc_mn(v + k * 2048, C::KV_CHUNK), idpv, first && k == 0 ? 0u : 1u);
-        tc_commit(&bars->pvdone[x][m & 1]);
+        for (int k = 0; k < C::D / 16; ++k)
+            mma_ss(d, qd + ((k >> 2) * C::Q_CHUNK + (k & 3) * 32) / 16, kd + ((k >> 2) * C::KV_CHUNK + (k & 3) * 32) / 16,
+                   idqk, k == 0 ? 0u : 1u);
+        tc_commit(&bars->sfull[x][n & 1]);
+    };
+    // PV of the half's block n (stage sg); the piece's first overwrites O, whose
+    // previous output must then have been read.
+    auto pv = [&](int x, uint32_t n, uint32_t sg, bool first, uint32_t piece) {
+        if (first && piece > 0 && !wait(&bars->ofree[x], (piece - 1) & 1, kAMmaO)) return;
+        if (!wait(&bars->pready[x][n & 1], (n >> 1) & 1, kAMmaP)) return;
+        tc_fence_after();
+        const uint32_t d = tbase + C::TM_O + x * C::D, ap = tbase + C::TM_S + (x * 2 + (n & 1)) * kBlk;
+        const uint64_t vd = v_desc + sg * (C::KV_STAGE / 16);
+#pragma unroll
+        for (int k = 0; k < kBlk / 16; ++k) mma_ts(d, ap + k * 8, vd + k * 128, idpv, first && k == 0 ? 0u : 1u);
+        tc_commit(&bars->pvdone[x][n & 1]);
     };
     while (more && ok) {
-        const int halves = a.has_b(p.group) ? 2 : 1;
-        for (int x = 0; x < halves && ok; ++x) wait(&bars->qfull[x], seg[x] & 1, kAMmaQ);
+        const bool two = a.has_b(p.group);
+        if (!wait(&bars->qfull[0], sa & 1, kAMmaQ)) break;
+        if (two && !wait(&bars->qfull[1], sb & 1, kAMmaQ)) break;
         const int steps = a.b1 - a.b0;
         for (int j = 0; j <= steps && ok; ++j) {
             if (j < steps) {
-                const uint32_t sg = g % kNS;
-                if (!wait(&bars->kfull[sg], (g / kNS) & 1, kAMmaK)) break;
-                tc_fence_after();
-                for (int x = 0; x < halves && ok; ++x) {
-                    // the S buffer is free once the PV that read its P, two blocks back, is done
-                    if (n[x] >= 2 && !wait(&bars->pvdone[x][n[x] & 1], ((n[x] - 2) >> 1) & 1, kAMmaS)) break;
-                    tc_fence_after();
-                    const uint32_t d = tbase + C::TM_S + (x * 2 + (n[x] & 1)) * kBlk;
-#pragma unroll
-                    for (int k = 0; k < C::D / 16; ++k)
-                        mma_ss(d, smem_desc_sw128(sm + x * C::Q_HALF + (k >> 2) * C::Q_CHUNK + (k & 3) * 32),
-                               smem_desc_sw128(sm + C::OFF_K + sg * C::KV_STAGE + (k >> 2) * C::KV_CHUNK + (k & 3) * 32),
-                               idqk, k == 0 ? 0u : 1u);
-                    tc_commit(&bars->sfull[x][n[x] & 1]);
-                    ++n[x];
-                }
+                const uint32_t sg = (g + j) % kNS;
+                if (!wait(&bars->kfull[sg], ((g + j) / kNS) & 1, kAMmaK)) break;
+                qk(0, na + j, sg);
+                if (two && ok) qk(1, nb + j, sg);
                 if (!ok) break;
                 tc_commit(&bars->kempty[sg]);
-                ++g;
             }
             if (j > 0) {
-                const uint32_t gv = j < steps ? g - 2 : g - 1;       // the block before the one just issued
-                const uint32_t sg = gv % kNS;
-                if (!wait(&bars->vfull[sg], (gv / kNS) & 1, kAMmaV)) break;
-                for (int x = 0; x < halves && ok; ++x) {
-                    // the piece's first PV overwrites O: the half's previous output must have been read
-                    if (j == 1 && seg[x] > 0 && !wait(&bars->ofree[x], (seg[x] - 1) & 1, kAMmaO)) break;
-                    pv(x, j < steps ? n[x] - 2 : n[x] - 1, sg, j == 1);
-                }
+                const uint32_t sg = (g + j - 1) % kNS;
+                if (!wait(&bars->vfull[sg], ((g + j - 1) / kNS) & 1, kAMmaV)) break;
+                pv(0, na + j - 1, sg, j == 1, sa);
+                if (two && ok) pv(1, nb + j - 1, sg, j == 1, sb);
                 if (!ok) break;
                 tc_commit(&bars->vempty[sg]);
             }
         }
-        for (int x = 0; x < halves; ++x) ++seg[x];
+        g += steps;
+        na += steps;
+        ++sa;
+        if (two) {
+            nb += steps;
+            ++sb;
+        }
         if (ok) more = a.next(p, least);
     }
     // nothing of this thread's is in flight when TMEM is freed
@@ -444,7 +467,8 @@ __device__ __forceinline__ void softmax_role(const AttentionParams& p, ManyBars*
     const int lane = lane_id();
     const uint32_t lane_off = static_cast<uint32_t>(row & 96) << 16;
     const uint32_t t_o = tbase + lane_off + C::TM_O + x * C::D;
-    const uint32_t q_sm = sm + x * C::Q_HALF + row * 128;
+    const uint32_t half_sm = sm + x * C::Q_HALF;                // its queries; afterwards its output rows on their way
+    constexpr int LPR = C::D / 8, RPI = 32 / LPR;               // lanes of a row's 16-byte vectors, rows per access
     Partial* info = reinterpret_cast<Partial*>(p.ws) + 2 * blockIdx.x;
     float* ml = reinterpret_cast<float*>(p.ws + ManyLayout<C>::ml(gridDim.x)) + static_cast<size_t>(blockIdx.x) * 4 * kRows;
     float* po = reinterpret_cast<float*>(p.ws + ManyLayout<C>::o(gridDim.x) + static_cast<size_t>(blockIdx.x) * 2 * C::PIECE);
@@ -452,8 +476,7 @@ __device__ __forceinline__ void softmax_role(const AttentionParams& p, ManyBars*
     __syncwarp();
 
     Walk a;
-    a.begin(p, st);
-    bool more = a.left > 0;
+    bool more = a.begin(p, st, least);
     uint32_t g = 0, n = 0;           // blocks of the CTA, of this half
     while (more) {
         const int steps = a.b1 - a.b0;
@@ -466,35 +489,43 @@ __device__ __forceinline__ void softmax_role(const AttentionParams& p, ManyBars*
         const bool valid = pr < a.s.n * p.group;
         const bool live = __any_sync(0xffffffffu, valid);
 
-        // ---- this row's query: largest element to [2^13, 2^14), fp16, into the operand ----
+        // ---- this warp's 32 queries: largest element to [2^13, 2^14), fp16, into the
+        // operand.  RPI rows a load, a lane per 16 bytes; a lane is a row from here on ----
         float qs = 0.0f;                                        // what turns a raw score into log2 units
-        int limit = 0x7FFFFFFF;                                 // last token the row sees
+        const int limit = valid ? a.s.len - a.s.n + pr / p.group : 0x7FFFFFFF;   // last token the row sees
         {
-            uint4 v[C::D / 8];
-            const int tok = valid ? pr / p.group : 0;
-            const uint16_t* src = p.q + static_cast<int64_t>(a.s.q0 + tok) * p.ldq +
-                                  static_cast<int64_t>(a.head * p.group + (valid ? pr - tok * p.group : 0)) * C::D;
+            const int sub = lane / LPR, ch = lane % LPR;
+            uint4 v[32 / RPI];
 #pragma unroll
-            for (int i = 0; i < C::D / 8; ++i) v[i] = valid ? *reinterpret_cast<const uint4*>(src + 8 * i) : make_uint4(0, 0, 0, 0);
-            uint32_t big = 0;
+            for (int i = 0; i < 32 / RPI; ++i) {
+                const int r = pr - lane + i * RPI + sub;
+                v[i] = make_uint4(0, 0, 0, 0);
+                if (r < a.s.n * p.group) {
+                    const int tok = r / p.group;
+                    v[i] = *reinterpret_cast<const uint4*>(p.q + static_cast<int64_t>(a.s.q0 + tok) * p.ldq +
+                                                           static_cast<int64_t>(a.head * p.group + (r - tok * p.group)) * C::D +
+                                                           ch * 8);
+                }
+            }
 #pragma unroll
-            for (int i = 0; i < C::D / 8; ++i) {
+            for (int i = 0; i < 32 / RPI; ++i) {
                 const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+                uint32_t big = 0;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) big = max(big, max((w[e] << 16) & 0x7FFFFFFFu, w[e] & 0x7FFF0000u));
-            }
-            const float shrink = row_shrink(__uint_as_float(big));
-            qs = __fdiv_rn(p.scale_log2, shrink);
-            if (valid) limit = a.s.len - a.s.n + tok;
 #pragma unroll
-            for (int i = 0; i < C::D / 8; ++i) {
-                const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+                for (int o = LPR / 2; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
+                const float shrink = row_shrink(__uint_as_float(big));
+                const float mine = __shfl_sync(0xffffffffu, shrink, (lane % RPI) * LPR);
+                if (lane / RPI == i) qs = mine;
                 uint32_t h[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     h[e] = cvt_f16x2(__uint_as_float(w[e] << 16) * shrink, __uint_as_float(w[e] & 0xFFFF0000u) * shrink);
-                sts128(q_sm + (i >> 3) * C::Q_CHUNK + (((i & 7) ^ (row & 7)) << 4), h[0], h[1], h[2], h[3]);
+                const int rr = (row & 96) + i * RPI + sub;
+                sts128(half_sm + rr * 128 + (ch >> 3) * C::Q_CHUNK + (((ch & 7) ^ (rr & 7)) << 4), h[0], h[1], h[2], h[3]);
             }
+            qs = __fdiv_rn(p.scale_log2, qs);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars->qfull[x]);
@@ -514,19 +545,24 @@ __device__ __forceinline__ void softmax_role(const AttentionParams& p, ManyBars*
                 reg_fence32(s);
                 reg_fence32(s + 32);
                 const float* rg = ring[g % kScaleRing];
-                float f[4], vs[4];
+                const int t0 = (a.b0 + j) * kBlk;
+                float f[4], wv[4];       // a granule's factors of scores and of weights
+                float vmax = 0.0f;
+                bool gone = false;       // (a scale below 0 marks tokens without a page; NaN scales pass on)
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
-                    f[b] = rg[b] * qs;
-                    vs[b] = rg[4 + b];
+                    const float ks = rg[b], vs = rg[4 + b];
+                    // A granule that this row does not see at all takes factors that
+                    // cannot touch it, whatever its scales are.  A zero factor would turn
+                    // a masked score into NaN: the smallest one changes no visible score.
+                    const bool none = ks < 0.0f || t0 + 16 * b > limit;
+                    gone = gone || ks < 0.0f;
+                    f[b] = none ? 1.0f : fmaxf(ks * qs, 1e-37f);
+                    if (ks != ks) f[b] = none ? 1.0f : ks;
+                    wv[b] = none ? 0.0f : vs;
+                    vmax = fmaxf(vmax, wv[b]);
                 }
-                const int t0 = (a.b0 + j) * kBlk;
-                // (a page scale below 0 marks tokens without a page; NaN scales pass on)
-                const bool gone = rg[0] < 0.0f || rg[1] < 0.0f || rg[2] < 0.0f || rg[3] < 0.0f;
-                const bool edge = gone || t0 + kBlk - 1 > min_limit;
-                if (edge) {
-                    // masked scores become -inf before their granule's factor (a positive
-                    // one: zero, NaN and infinite scales must not touch them)
+                if (gone || t0 + kBlk - 1 > min_limit) {
 #pragma unroll
                     for (int i = 0; i < kBlk; ++i)
                         if (t0 + i > limit || rg[i >> 4] < 0.0f) s[i] = 0xFF800000u;
@@ -535,15 +571,15 @@ __device__ __forceinline__ void softmax_role(const AttentionParams& p, ManyBars*
                 float mx = kNegInf;
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
-                    float r = __uint_as_float(s[16 * b]);
+                    float r[4];
 #pragma unroll
-                    for (int i = 1; i < 16; ++i) r = fmaxf(r, __uint_as_float(s[16 * b + i]));
-                    if (r > kNegInf) mx = fmaxf(mx, r * f[b]);
+                    for (int k = 0; k < 4; ++k)
+                        r[k] = fmaxf(fmaxf(__uint_as_float(s[16 * b + 4 * k]), __uint_as_float(s[16 * b + 4 * k + 1])),
+                                     fmaxf(__uint_as_float(s[16 * b + 4 * k + 2]), __uint_as_float(s[16 * b + 4 * k + 3])));
+                    mx = fmaxf(mx, fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3])) * f[b]);
                 }
-                const float vmax = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
-                const bool grow = mx > m + kSlack || (m == kNegInf && mx > m) || vmax > vr;
-                if (__any_sync(0xffffffffu, grow)) {
-                    const float mn = fmaxf(m, mx), vn = fmaxf(vr, pow2_above(vmax));
+                if (__any_sync(0xffffffffu, mx > m + kSlack || vmax > vr)) {
+                    const float mn = fmaxf(m, mx + kMargin), vn = fmaxf(vr, pow2_above(vmax));
                     const float al = mn == kNegInf ? 1.0f : ex2(m - mn), av = al * __fdiv_rn(vr, vn);
                     m = mn;
                     l *= al;
@@ -552,16 +588,18 @@ __device__ __forceinline__ void softmax_role(const AttentionParams& p, ManyBars*
                     if (j > 0) {
                         if (!warp_wait(&bars->pvdone[x][(n - 1) & 1], ((n - 1) >> 1) & 1, abort_flag, p.status, kASoftPv)) return;
                         tc_fence_after();
-                        // O is scaled 32 columns at a time
-#pragma unroll
-                        for (int c = 0; c < C::D; c += 32) {
-                            uint32_t o[32];
+#pragma unroll 1
+                        for (int c = 0; c < C::D; c += 64) {
+                            uint32_t o[64];
                             tm_ld32(t_o + c, o);
+                            tm_ld32(t_o + c + 32, o + 32);
                             tc_wait_ld();
                             reg_fence32(o);
+                            reg_fence32(o + 32);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * av);
+                            for (int i = 0; i < 64; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * av);
                             tm_st32(t_o + c, o);
+                            tm_st32(t_o + c + 32, o + 32);
                         }
                         tc_wait_st();
                     }
@@ -570,40 +608,20 @@ __device__ __forceinline__ void softmax_role(const AttentionParams& p, ManyBars*
                 const float neg_m = m == kNegInf ? 0.0f : -m;
                 uint32_t pk[kBlk / 2];
                 uint64_t sum = 0;
-                if (!edge) {
 #pragma unroll
-                    for (int b = 0; b < 4; ++b) {
-                        const uint64_t f2 = pair2(f[b], f[b]), m2 = pair2(neg_m, neg_m);
-                        const float wv = vs[b] * vr_inv;
-                        const uint64_t w2 = pair2(wv, wv);
+                for (int b = 0; b < 4; ++b) {
+                    const uint64_t f2 = pair2(f[b], f[b]), m2 = pair2(neg_m, neg_m);
+                    const float w = wv[b] * vr_inv;
+                    const uint64_t w2 = pair2(w, w);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const int e = 16 * b + 2 * i;
-                            float lo, hi;
-                            unpair2(f2_fma(pair2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), f2, m2), lo, hi);
-                            const uint64_t pp = pair2(ex2(lo), ex2(hi));
-                            sum = f2_add(sum, pp);
-                            unpair2(f2_mul(pp, w2), lo, hi);
-                            pk[8 * b + i] = cvt_f16x2(lo, hi);
-                        }
-                    }
-                } else {
-#pragma unroll
-                    for (int b = 0; b < 4; ++b) {
-                        const float wv = vs[b] * vr_inv;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const int e = 16 * b + 2 * i;
-                            float pp[2], ww[2];
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const bool hidden = t0 + e + h > limit || rg[b] < 0.0f;
-                                pp[h] = hidden ? 0.0f : ex2(fmaf(__uint_as_float(s[e + h]), f[b], neg_m));
-                                ww[h] = hidden ? 0.0f : pp[h] * wv;
-                            }
-                            sum = f2_add(sum, pair2(pp[0], pp[1]));
-                            pk[8 * b + i] = cvt_f16x2(ww[0], ww[1]);
-                        }
+                    for (int i = 0; i < 8; ++i) {
+                        const int e = 16 * b + 2 * i;
+                        float lo, hi;
+                        unpair2(f2_fma(pair2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), f2, m2), lo, hi);
+                        const uint64_t pp = pair2(ex2(lo), ex2(hi));
+                        sum = f2_add(sum, pp);
+                        unpair2(f2_mul(pp, w2), lo, hi);
+                        pk[8 * b + i] = cvt_f16x2(lo, hi);
                     }
                 }
                 float lo, hi;
@@ -625,9 +643,8 @@ __device__ __forceinline__ void softmax_role(const AttentionParams& p, ManyBars*
             const bool whole = a.b0 == 0 && a.b1 == a.nb;
             const int slot = a.b0 == 0 ? 1 : 0;
             const float inv = whole ? inv_sum(l) * back : back;
-            uint16_t* dst = whole && valid ? out_row(p, a.s, a.head, pr) : nullptr;
             float4* part = reinterpret_cast<float4*>(po + static_cast<size_t>(slot) * kRows * C::D) + x * 128 + row;
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < C::D; c += 32) {
                 uint32_t o[32];
                 tm_ld32(t_o + c, o);
@@ -637,17 +654,33 @@ __device__ __forceinline__ void softmax_role(const AttentionParams& p, ManyBars*
 #pragma unroll
                 for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(o[i]) * inv;
                 if (whole) {
-                    if (valid)
+                    // through shared memory (its queries are done with), so that rows leave whole
 #pragma unroll
-                        for (int i = 0; i < 32; i += 8)
-                            *reinterpret_cast<uint4*>(dst + c + i) =
-                                make_uint4(pack_bf16(v[i], v[i + 1]), pack_bf16(v[i + 2], v[i + 3]),
-                                           pack_bf16(v[i + 4], v[i + 5]), pack_bf16(v[i + 6], v[i + 7]));
+                    for (int i = 0; i < 32; i += 8) {
+                        const int u = (c + i) / 8;
+                        sts128(half_sm + row * 128 + (u >> 3) * C::Q_CHUNK + (((u & 7) ^ (row & 7)) << 4),
+                               pack_bf16(v[i], v[i + 1]), pack_bf16(v[i + 2], v[i + 3]), pack_bf16(v[i + 4], v[i + 5]),
+                               pack_bf16(v[i + 6], v[i + 7]));
+                    }
                 } else if (valid) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 4)
                         part[static_cast<size_t>((c + i) / 4) * kRows] = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
                 }
+            }
+            if (whole) {
+                __syncwarp();
+                const int sub = lane / LPR, ch = lane % LPR;
+#pragma unroll 4
+                for (int i = 0; i < 32 / RPI; ++i) {
+                    const int rr = (row & 96) + i * RPI + sub, r = pr - lane + i * RPI + sub;
+                    uint4 v;
+                    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                                 : "r"(half_sm + rr * 128 + (ch >> 3) * C::Q_CHUNK + (((ch & 7) ^ (rr & 7)) << 4)));
+                    if (r < a.s.n * p.group) *reinterpret_cast<uint4*>(out_row(p, a.s, a.head, r) + ch * 8) = v;
+                }
+                __syncwarp();
             }
             if (!whole) {
                 ml[slot * 2 * kRows + x * 128 + row] = m;
@@ -710,7 +743,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Atte
         const Seq q = load_seq(cv, s);
         const int tiles = many_tiles(q, p.group, least);
         long long u = 0;
-        for (int t = lane; t < tiles; t += 32) u += many_blocks(q, p.group, t);
+        for (int t = lane; t < tiles; t += 32) u += many_units(q, p.group, t);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
         if (lane == 0) prefix[s] = u * cv.kv_heads;
@@ -748,11 +781,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Atte
             st.seq = lo;
             st.head = static_cast<int>(off / per_head);
             long long r = off - st.head * per_head;
-            // the tile that holds block r of the head
+            // the tile that holds unit r of the head
             const int tiles = many_tiles(q, p.group, least);
             for (int base = 0; base < tiles; base += 32) {
                 const int t = base + lane;
-                const long long u = t < tiles ? many_blocks(q, p.group, t) : 0;
+                const long long u = t < tiles ? many_units(q, p.group, t) : 0;
                 long long v = u;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -763,7 +796,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Atte
                 if (hit) {
                     const int w = __ffs(hit) - 1;
                     st.tile = base + w;
-                    st.blk = static_cast<int>(r - __shfl_sync(0xffffffffu, v - u, w));
+                    st.unit = static_cast<int>(r - __shfl_sync(0xffffffffu, v - u, w));
                     break;
                 }
                 r -= __shfl_sync(0xffffffffu, v, 31);

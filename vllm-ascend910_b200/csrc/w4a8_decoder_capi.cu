@@ -132,7 +132,7 @@ int w4a8_attention(const w4a8_kv_cache* cache, const int32_t* page_table, int64_
     int rc = make_view(cache, page_table, ld_table, table_cols, kv_lens, cu_q, batch, tokens, &p.c);
     if (rc != W4A8_OK) return rc;
     if (q_heads <= 0 || q_heads > 65536 || q_heads % cache->kv_heads != 0) return W4A8_ERR_INVALID;
-    if (max_q_len < 0 || !(softmax_scale == softmax_scale)) return W4A8_ERR_INVALID;
+    if (max_q_len < 0 || !(softmax_scale >= 0.0f)) return W4A8_ERR_INVALID;
     if (batch > W4A8_ATTENTION_MAX_BATCH) return W4A8_ERR_UNSUPPORTED;
     if (tokens * (q_heads / cache->kv_heads) > 0x7FFF0000) return W4A8_ERR_UNSUPPORTED;   // packed rows are 32-bit
     if (p.c.batch == 0) return W4A8_OK;
