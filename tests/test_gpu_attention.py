@@ -98,6 +98,9 @@ CASES = [
     (8, 1, 64, 32, [300], [300]),
     (3, 3, 64, 16, [200, 1, 131], [333, 40, 131]),
     (6, 1, 128, 16, [64, 300, 1], [64, 1000, 17]),
+    (5, 1, 128, 16, [1] * 30 + [40, 2, 0, 60], [100] * 30 + [90, 300, 5, 61]),   # single tokens beside two chunks
+    (16, 2, 64, 32, [2, 1, 1, 50, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1],
+     [33, 70, 64, 120] + [50] * 24),
 ]
 
 

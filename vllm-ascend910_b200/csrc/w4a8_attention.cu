@@ -36,8 +36,9 @@
 //     deep: with 16 warps up to 128 KB are on the way to an SM.  Shared memory holds codes with
 //     16-byte chunks permuted by token, so fragment reads do not collide.
 //   * A warp's share begins and ends inside (sequence, head) segments.  Pieces
-//     of one segment are joined in the CTA, and across CTAs by a second small
-//     kernel, in unit order: no atomics, the same bits on every run.
+//     of one segment are joined in the CTA; parts of CTAs by the last of them to
+//     finish (a counter tells which), always in unit order, so the bits do not
+//     depend on who is last.  Nothing waits for another CTA.
 #include <algorithm>
 
 #include "w4a8_attention.cuh"
@@ -61,12 +62,6 @@ __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_grou
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-__device__ __forceinline__ uint4 lds128(uint32_t a)
-{
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-    return v;
-}
 __device__ __forceinline__ uint2 lds64(uint32_t a)
 {
     uint2 v;
@@ -131,20 +126,47 @@ __device__ __forceinline__ uint32_t chunk_off(int t, int ch)
 
 // One piece of a segment kept for the join: unit range and softmax state.
 struct PieceInfo {
-    long long seg;      // first unit of the segment; -1: none
-    int seq, head, tile, complete_lo, complete_hi;   // the piece reaches the segment's first / last unit
+    long long seg, seg_end;          // the segment's units; seg -1: no piece
+    int q0, rows, head, tile;        // its sequence's first query token and packed rows, kv head, row tile
+    int complete_lo, complete_hi;    // the piece reaches the segment's first / last unit
 };
 
 template <class C>
 struct Layout {
-    // workspace: [grid][2] Partial, then [grid][2] (m, l)[R], then [grid][2] O, then [grid * WARPS] stash (O, m, l)
-    static __host__ __device__ size_t info() { return 0; }
-    static __host__ __device__ size_t ml(int grid) { return static_cast<size_t>(grid) * 2 * sizeof(Partial); }
-    static __host__ __device__ size_t o(int grid) { return ml(grid) + static_cast<size_t>(grid) * 2 * 2 * C::R * 4; }
+    // workspace: [grid][2] (m, l)[R], then [grid][2] O, then [grid * WARPS] O of stashed pieces
+    static __host__ __device__ size_t ml() { return 0; }
+    static __host__ __device__ size_t o(int grid) { return static_cast<size_t>(grid) * 2 * 2 * C::R * 4; }
     static __host__ __device__ size_t stash(int grid) { return o(grid) + static_cast<size_t>(grid) * 2 * C::PIECE; }
     static __host__ __device__ size_t total(int grid)
     {
         return stash(grid) + static_cast<size_t>(grid) * C::WARPS * C::PIECE;
+    }
+};
+
+// The unit list cut in `workers` contiguous shares: the first `more` of them have
+// `each` + 1 units, the others `each`.
+struct Shares {
+    long long total, each;
+    int workers, more;
+    __device__ __forceinline__ Shares(long long t, int w) : total(t), workers(w)
+    {
+        if (t < 0x7FFFFFFF) {                       // (32-bit division is several times shorter)
+            each = static_cast<uint32_t>(t) / static_cast<uint32_t>(w);
+        } else {
+            each = t / w;
+        }
+        more = static_cast<int>(t - each * w);
+    }
+    __device__ __forceinline__ long long begin(int w) const { return w >= workers ? total : each * w + min(w, more); }
+    // The worker whose share holds unit u.
+    __device__ __forceinline__ int of(long long u) const
+    {
+        const long long first = (each + 1) * more;  // units of the longer shares
+        if (u < first) return u < 0x7FFFFFFF ? static_cast<int>(static_cast<uint32_t>(u) / static_cast<uint32_t>(each + 1))
+                                             : static_cast<int>(u / (each + 1));
+        u -= first;
+        return more + (u < 0x7FFFFFFF ? static_cast<int>(static_cast<uint32_t>(u) / static_cast<uint32_t>(each))
+                                      : static_cast<int>(u / each));
     }
 };
 
@@ -159,11 +181,17 @@ struct Cursor {
         s = load_seq(c, sq);
         blocks = seq_blocks(s);
         const int tiles = seq_tiles(s, group, C::R, most);
-        const long long per_head = static_cast<long long>(tiles) * blocks;
-        head = static_cast<int>(off / per_head);
-        const long long r = off - head * per_head;
-        tile = static_cast<int>(r / blocks);
-        blk = static_cast<int>(r - static_cast<long long>(tile) * blocks);
+        if (off < 0x7FFFFFFF) {
+            const int t = static_cast<int>(static_cast<uint32_t>(off) / static_cast<uint32_t>(blocks));
+            blk = static_cast<int>(off) - t * blocks;
+            head = t / tiles;
+            tile = t - head * tiles;
+        } else {
+            const long long t = off / blocks;
+            blk = static_cast<int>(off - t * blocks);
+            head = static_cast<int>(t / tiles);
+            tile = static_cast<int>(t - static_cast<long long>(head) * tiles);
+        }
     }
     // Next unit; false past the end of the list.
     __device__ __forceinline__ bool next(const CacheView& c, int group, int most)
@@ -196,7 +224,7 @@ __device__ __forceinline__ void store_rows(const AttentionParams& p, const Seq& 
             const int row = tile * C::R + nt * 8 + 2 * c + h;
             if (row >= s.n * p.group) continue;
             const float inv = inv_sum(l[nt][h]);
-            uint16_t* o = out_row(p, s, head, row) + r * (C::D / 8);
+            uint16_t* o = out_row(p, s.q0, head, row) + r * (C::D / 8);
             uint32_t w[C::D / 16];
 #pragma unroll
             for (int i = 0; i < C::D / 16; ++i) w[i] = pack_bf16(acc[nt][i][h] * inv, acc[nt][i][2 + h] * inv);
@@ -212,8 +240,10 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ PieceInfo pieces[2 * C::WARPS];
     __shared__ float piece_m[2 * C::WARPS][C::R], piece_l[2 * C::WARPS][C::R];
+    __shared__ float factor[2 * C::WARPS][C::R], row_l[C::R];
     __shared__ long long warp_sum[C::WARPS];
     __shared__ long long running;
+    __shared__ bool is_last;
     long long* prefix = reinterpret_cast<long long*>(smem + C::SMEM);   // [batch + 1] units before each sequence
 
     const int tid = threadIdx.x, warp = warp_id(), lane = lane_id();
@@ -249,12 +279,12 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
     const long long total = running;
     // equal contiguous shares, at least one unit each: a list shorter than the
     // grid leaves the last CTAs without work, none between working ones
-    const long long W = min(static_cast<long long>(gridDim.x) * C::WARPS, total);
-    const long long wk = static_cast<long long>(blockIdx.x) * C::WARPS + warp;
-    const long long u0 = wk < W ? total * wk / W : total, u1 = wk < W ? total * (wk + 1) / W : total;
+    const int wk = static_cast<int>(blockIdx.x) * C::WARPS + warp;
+    const Shares sh(total, static_cast<int>(gridDim.x) * C::WARPS);
+    const long long u0 = sh.begin(wk), u1 = sh.begin(wk + 1);
 
     float acc[C::NT][C::D / 16][4];
-    float m[C::NT][2], l[C::NT][2];
+    float m[C::NT][2], negm[C::NT][2], l[C::NT][2];
     const int r = lane >> 2, c = lane & 3;
     const uint32_t ring = smem_u32(smem + warp * C::SLOT);
 
@@ -269,33 +299,40 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
         Cursor<C> cur, pre;
         cur.set(cv, p.group, p.few_most, lo, u0 - prefix[lo]);
         pre = cur;
-        bool pre_ok = true;
-        long long pre_u = u0;
+
+        // Where this lane's copies and fragment reads lie in a stage.  chunk_off swizzles
+        // by the token's low bits, so offsets of further copies and tokens are constants:
+        // tokens 8 apart keep their swizzle, and a copy's neighbour 4 tokens on flips one bit.
+        const uint32_t cp0 = chunk_off<C::D>(lane / C::CHUNKS, lane % C::CHUNKS);
+        const uint32_t cp1 = chunk_off<C::D>(lane / C::CHUNKS + 32 / C::CHUNKS, lane % C::CHUNKS) - 512;
+        const uint32_t k0 = chunk_off<C::D>(r, c * (C::D / 64)), k1 = chunk_off<C::D>(r, c * (C::D / 64) + (C::D / 64 - 1));
+        const uint32_t v0 = C::D == 128 ? chunk_off<C::D>(2 * c, r) : chunk_off<C::D>(2 * c, r >> 1) + (r & 1) * 8;
+        const uint32_t v1 = C::D == 128 ? chunk_off<C::D>(2 * c + 1, r) : chunk_off<C::D>(2 * c + 1, r >> 1) + (r & 1) * 8;
+        const int pages = static_cast<int>(cv.pages);
+        int ahead = static_cast<int>(u1 - u0);    // units of the share still to be fetched
 
         // Brings the unit under `pre` into ring stage st and moves on.
         auto fetch = [&](int st) {
-            if (pre_u < u1 && pre_ok) {
+            if (ahead > 0) {
                 const int tok = pre.blk * kBlkTok;
-                const int pg = tok >> cv.page_log2;
-                const int id = pg < cv.table_cols ? cv.table[static_cast<int64_t>(pre.seq) * cv.ld_table + pg] : -1;
-                const bool ok = id >= 0 && id < cv.pages && tok < pre.s.len;
+                const int id = tok < pre.s.len ? cv.table[pre.seq * cv.ld_table + (tok >> cv.page_log2)] : -1;
+                const bool ok = static_cast<unsigned>(id) < static_cast<unsigned>(pages);
                 const int64_t ph = ok ? static_cast<int64_t>(id) * cv.kv_heads + pre.head : 0;
-                const int64_t base = (ph << cv.page_log2) * C::D + static_cast<int64_t>(ok ? tok & (cv.page - 1) : 0) * C::D;
+                const int64_t at = ((ph << cv.page_log2) + (ok ? tok & (cv.page - 1) : 0)) * C::D + lane * 16;
+                const int8_t *kp = cv.k + at, *vp = cv.v + at;
                 const uint32_t d = ring + st * C::STAGE;
 #pragma unroll
                 for (int i = 0; i < C::KV_BYTES / 512; ++i) {
-                    const int ch = i * 32 + lane;
-                    const uint32_t off = chunk_off<C::D>(ch / C::CHUNKS, ch % C::CHUNKS);
-                    cp_async16(d + off, cv.k + base + ch * 16, ok);
-                    cp_async16(d + C::KV_BYTES + off, cv.v + base + ch * 16, ok);
+                    const uint32_t off = d + ((i & 1) ? cp1 : cp0) + i * 512;
+                    cp_async16(off, kp + i * 512, ok);
+                    cp_async16(off + C::KV_BYTES, vp + i * 512, ok);
                 }
                 // a page that is not there has no tokens: its scale is marked with -1
                 if (lane < 2) {
                     if (ok) cp_async4(d + 2 * C::KV_BYTES + lane * 4, (lane ? cv.v_scale : cv.k_scale) + ph, true);
                     else asm volatile("st.shared.f32 [%0], %1;" ::"r"(d + 2 * C::KV_BYTES + lane * 4), "f"(-1.0f));
                 }
-                ++pre_u;
-                pre_ok = pre.next(cv, p.group, p.few_most);
+                if (--ahead > 0) pre.next(cv, p.group, p.few_most);
             }
             cp_commit();
         };
@@ -318,7 +355,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
             for (int nt = 0; nt < C::NT; ++nt) {
                 const int row = cur.tile * C::R + nt * 8 + r;
                 const bool ok = row < cur.s.n * p.group;
-                const int tok = ok ? row / p.group : 0, g = ok ? row - tok * p.group : 0;
+                const int tok = ok ? row_token(p, row) : 0, g = ok ? row - tok * p.group : 0;
                 const uint16_t* q = p.q + static_cast<int64_t>(cur.s.q0 + tok) * p.ldq +
                                     static_cast<int64_t>(cur.head * p.group + g) * C::D + c * (C::D / 4);
                 uint32_t big = 0;
@@ -353,9 +390,10 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
                 for (int h = 0; h < 2; ++h) {
                     const int qr = cur.tile * C::R + nt * 8 + 2 * c + h;
                     // rows past the sequence's last are computed on zero queries and not stored
-                    limit[nt][h] = qr < cur.s.n * p.group ? cur.s.len - cur.s.n + qr / p.group : 0x7FFFFFFF;
+                    limit[nt][h] = qr < cur.s.n * p.group ? cur.s.len - cur.s.n + row_token(p, qr) : 0x7FFFFFFF;
                     min_limit = min(min_limit, limit[nt][h]);
                     m[nt][h] = kNegInf;
+                    negm[nt][h] = first_reference(kNegInf);
                     l[nt][h] = 0.0f;
                 }
 #pragma unroll
@@ -370,14 +408,12 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
         long long seg_lo = u0 - cur.blk;          // first unit of the segment under `cur`
         int piece_blk = cur.blk;                  // the piece's first block
         int st = 0;
-        for (long long u = u0; u < u1; ++u) {
+        for (int left = static_cast<int>(u1 - u0); left > 0; --left) {
             cp_wait<kStages - 2>();
             __syncwarp();
             fetch(st == 0 ? kStages - 1 : st - 1);     // the stage consumed in the previous pass
             const uint32_t kb = ring + st * C::STAGE, vb = kb + C::KV_BYTES;
             const float ks = lds32f(kb + 2 * C::KV_BYTES), vs = lds32f(kb + 2 * C::KV_BYTES + 4);
-            const int t0 = cur.blk * kBlkTok;
-            const bool there = ks >= 0.0f || ks != ks;   // NaN scales pass on; -1: no page
 
             // ---- S^T = K Q^T ----
             float sc[C::NT][4];
@@ -390,36 +426,65 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int i = 0; i < C::D / 64; ++i) {
-                    const uint4 v = lds128(kb + chunk_off<C::D>(r + 8 * t, c * (C::D / 64) + i));
-                    kw[t][4 * i] = v.x;
-                    kw[t][4 * i + 1] = v.y;
-                    kw[t][4 * i + 2] = v.z;
-                    kw[t][4 * i + 3] = v.w;
+                    const uint4 v = lds128(kb + (i ? k1 : k0) + t * (8 * C::D));
+                    kw[t][4 * i] = v.x ^ 0x80808080u;
+                    kw[t][4 * i + 1] = v.y ^ 0x80808080u;
+                    kw[t][4 * i + 2] = v.z ^ 0x80808080u;
+                    kw[t][4 * i + 3] = v.w ^ 0x80808080u;
                 }
 #pragma unroll
             for (int ks_ = 0; ks_ < C::D / 16; ++ks_) {
                 uint32_t a[4];
-                a[0] = codes_to_f16x2(__byte_perm(kw[0][ks_], 0, 0x4140));
-                a[1] = codes_to_f16x2(__byte_perm(kw[1][ks_], 0, 0x4140));
-                a[2] = codes_to_f16x2(__byte_perm(kw[0][ks_], 0, 0x4342));
-                a[3] = codes_to_f16x2(__byte_perm(kw[1][ks_], 0, 0x4342));
+                a[0] = biased_lo(kw[0][ks_]);
+                a[1] = biased_lo(kw[1][ks_]);
+                a[2] = biased_hi(kw[0][ks_]);
+                a[3] = biased_hi(kw[1][ks_]);
 #pragma unroll
                 for (int nt = 0; nt < C::NT; ++nt) mma_f16(sc[nt], a, qf[nt][ks_][0], qf[nt][ks_][1]);
             }
 
-            // ---- running maximum ----
-            const bool edge = t0 + kBlkTok - 1 > min_limit || !there;
-            bool grow = vs > vr;
+            // ---- scores less the reference, in log2 units ----
+            float f[C::NT][2], wv[C::NT][2];
+            const float vsr = vs * vr_inv;
+#pragma unroll
+            for (int nt = 0; nt < C::NT; ++nt)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    f[nt][h] = ks * qs[nt][h];
+                    wv[nt][h] = vsr;
+                }
+            const int t0 = cur.blk * kBlkTok;
+            const bool there = !(ks < 0.0f);             // (a NaN scale passes on; -1: no page)
+            float vsu = there ? vs : 0.0f;               // what vr has to cover
+            if (t0 + kBlkTok - 1 > min_limit || !there) {
+                // Masked scores become -inf; a row that sees nothing of the unit takes
+                // factors that cannot touch it, and no factor is 0 (0 * inf).
+                bool seen = false;
+#pragma unroll
+                for (int nt = 0; nt < C::NT; ++nt)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const bool none = !there || t0 > limit[nt][h];
+                        f[nt][h] = none ? 1.0f : (ks != ks ? ks : fmaxf(f[nt][h], 1e-37f));
+                        if (none) wv[nt][h] = 0.0f;
+                        seen = seen || !none;
+                        if (none || t0 + r > limit[nt][h]) sc[nt][h] = kNegInf;
+                        if (none || t0 + r + 8 > limit[nt][h]) sc[nt][2 + h] = kNegInf;
+                    }
+                if (!__any_sync(0xffffffffu, seen)) vsu = 0.0f;
+            }
+            float raise = vsu > vr ? INFINITY : 0.0f;
+            float d[C::NT][4];
 #pragma unroll
             for (int nt = 0; nt < C::NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    sc[nt][e] *= ks * qs[nt][e & 1];
-                    if (edge && (!there || t0 + r + (e >> 1) * 8 > limit[nt][e & 1])) sc[nt][e] = kNegInf;
-                    grow = grow || sc[nt][e] > m[nt][e & 1];
+                    d[nt][e] = fmaf(sc[nt][e], f[nt][e & 1], negm[nt][e & 1]);
+                    raise = fmaxf(raise, d[nt][e]);
                 }
-            if (__any_sync(0xffffffffu, grow)) {
-                const float vn = fmaxf(vr, pow2_above(vs));
+            if (__any_sync(0xffffffffu, raise > kSlack)) {
+                // ---- the references move: m to the scores' maximum, vr over vs ----
+                const float vn = fmaxf(vr, pow2_above(vsu));
                 const float va = __fdiv_rn(vr, vn);
                 vr = vn;
                 vr_inv = __fdiv_rn(kWeightOne, vr);
@@ -427,13 +492,14 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
                 for (int nt = 0; nt < C::NT; ++nt)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        float x = fmaxf(sc[nt][h], sc[nt][2 + h]);
+                        float x = fmaxf(sc[nt][h], sc[nt][2 + h]) * f[nt][h];
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
                         const float mn = fmaxf(m[nt][h], x);
                         const float a = mn == kNegInf ? 1.0f : ex2(m[nt][h] - mn);
                         m[nt][h] = mn;
+                        negm[nt][h] = first_reference(mn);
                         l[nt][h] *= a;
                         const float av = a * va;
 #pragma unroll
@@ -441,39 +507,36 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
                             acc[nt][i][h] *= av;
                             acc[nt][i][2 + h] *= av;
                         }
+                        d[nt][h] = fmaf(sc[nt][h], f[nt][h], negm[nt][h]);
+                        d[nt][2 + h] = fmaf(sc[nt][2 + h], f[nt][h], negm[nt][h]);
+                        if (wv[nt][h] != 0.0f) wv[nt][h] = vs * vr_inv;
                     }
             }
 
             // ---- P, its sum, and the weights P * vs / vr * 2^14 as the second product's operand ----
             uint32_t pb[C::NT][2];
-            const float vw_ = vs * vr_inv;
 #pragma unroll
             for (int nt = 0; nt < C::NT; ++nt) {
-                float e4[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float mm = m[nt][e & 1] == kNegInf ? 0.0f : m[nt][e & 1];
-                    const float x = ex2(sc[nt][e] - mm);
-                    l[nt][e & 1] += x;
-                    e4[e] = edge && sc[nt][e] == kNegInf ? 0.0f : x * vw_;
-                }
-                pb[nt][0] = movmatrix_trans(pack_f16(e4[0], e4[1]));
-                pb[nt][1] = movmatrix_trans(pack_f16(e4[2], e4[3]));
+                const float x0 = ex2(d[nt][0]), x1 = ex2(d[nt][1]), x2 = ex2(d[nt][2]), x3 = ex2(d[nt][3]);
+                l[nt][0] += x0 + x2;
+                l[nt][1] += x1 + x3;
+                pb[nt][0] = movmatrix_trans(pack_f16(x0 * wv[nt][0], x1 * wv[nt][1]));
+                pb[nt][1] = movmatrix_trans(pack_f16(x2 * wv[nt][0], x3 * wv[nt][1]));
             }
 
             // ---- O^T += V^T P^T ----
             uint32_t vw[4][C::D / 32];
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                const int tok = 2 * c + (t & 1) + (t >> 1) * 8;
+                const uint32_t at = vb + ((t & 1) ? v1 : v0) + (t >> 1) * (8 * C::D);
                 if (C::D == 128) {
-                    const uint4 v = lds128(vb + chunk_off<C::D>(tok, r));
+                    const uint4 v = lds128(at);
                     vw[t][0] = v.x;
                     vw[t][1] = v.y;
                     vw[t][2 % (C::D / 32)] = v.z;
                     vw[t][3 % (C::D / 32)] = v.w;
                 } else {
-                    const uint2 v = lds64(vb + chunk_off<C::D>(tok, r >> 1) + (r & 1) * 8);
+                    const uint2 v = lds64(at);
                     vw[t][0] = v.x;
                     vw[t][1] = v.y;
                 }
@@ -494,7 +557,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
 
             // ---- end of a piece ----
             const bool seg_end = cur.blk == cur.blocks - 1;
-            if (seg_end || u + 1 == u1) {
+            if (seg_end || left == 1) {
 #pragma unroll
                 for (int nt = 0; nt < C::NT; ++nt)
 #pragma unroll
@@ -515,7 +578,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
                 if (seg_end && piece_blk == 0) {
                     store_rows<C>(p, cur.s, cur.head, cur.tile, acc, l);
                 } else {
-                    const bool last = u + 1 == u1;
+                    const bool last = left == 1;
                     const int pi = 2 * warp + (last ? 1 : 0);
                     float* dst;
                     if (last) {
@@ -542,7 +605,9 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
                     if (lane == 0) {
                         PieceInfo& q = pieces[pi];
                         q.seg = seg_lo;
-                        q.seq = cur.seq;
+                        q.seg_end = seg_lo + cur.blocks;
+                        q.q0 = cur.s.q0;
+                        q.rows = cur.s.n * p.group;
                         q.head = cur.head;
                         q.tile = cur.tile;
                         q.complete_lo = piece_blk == 0;
@@ -550,10 +615,10 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
                     }
                 }
             }
-            if (u + 1 < u1) {
+            if (left > 1) {
                 cur.next(cv, p.group, p.few_most);
                 if (seg_end) {
-                    seg_lo = u + 1;
+                    seg_lo = u1 - left + 1;
                     piece_blk = 0;
                     begin_segment();
                 }
@@ -565,108 +630,98 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
     __syncthreads();
 
     // ---- join the CTA's pieces, in unit order ----
-    Partial* info = reinterpret_cast<Partial*>(p.ws + Layout<C>::info()) + 2 * blockIdx.x;
-    float* ml = reinterpret_cast<float*>(p.ws + Layout<C>::ml(gridDim.x)) + static_cast<size_t>(blockIdx.x) * 2 * 2 * C::R;
-    float* po = reinterpret_cast<float*>(p.ws + Layout<C>::o(gridDim.x) + static_cast<size_t>(blockIdx.x) * 2 * C::PIECE);
-    bool have[2] = {false, false};
-    int i = 0;
-    while (i < 2 * C::WARPS) {
-        if (pieces[i].seg < 0) {
-            ++i;
-            continue;
+    float* all_ml = reinterpret_cast<float*>(p.ws + Layout<C>::ml());
+    float* all_o = reinterpret_cast<float*>(p.ws + Layout<C>::o(gridDim.x));
+    float* ml = all_ml + static_cast<size_t>(blockIdx.x) * 2 * 2 * C::R;
+    float* po = all_o + static_cast<size_t>(blockIdx.x) * 2 * C::R * C::D;
+    const long long my_seg = lane < 2 * C::WARPS ? pieces[lane].seg : -1;
+    unsigned todo = __ballot_sync(0xffffffffu, my_seg >= 0);
+    while (todo) {
+        // the pieces of one segment, a bit each
+        const int i = __ffs(todo) - 1;
+        const unsigned mask = __ballot_sync(0xffffffffu, my_seg == __shfl_sync(0xffffffffu, my_seg, i));
+        const int e = 31 - __clz(mask);
+        todo &= ~mask;
+        const PieceInfo first = pieces[i];
+        const bool whole = first.complete_lo && pieces[e].complete_hi;
+        const int slot = first.complete_lo ? 1 : 0;
+        __syncthreads();                            // the previous segment's factors have been read
+        for (int row = warp; row < C::R; row += C::WARPS) {      // a lane per piece
+            const bool in = (mask >> lane) & 1;
+            const float pm = in ? piece_m[lane][row] : kNegInf;
+            float mx = pm;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            const float a = in ? (mx == kNegInf ? 1.0f : ex2(pm - mx)) : 0.0f;
+            float ls = in ? a * piece_l[lane][row] : 0.0f;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, o);
+            if (lane < 2 * C::WARPS) factor[lane][row] = a;
+            if (lane == 0) {
+                row_l[row] = ls;
+                if (!whole) {
+                    ml[slot * 2 * C::R + row] = mx;
+                    ml[slot * 2 * C::R + C::R + row] = ls;
+                }
+            }
         }
-        int e = i;                                  // [i, e]: the segment's pieces in this CTA
-        for (int k = i + 1; k < 2 * C::WARPS; ++k) {
-            if (pieces[k].seg < 0) continue;
-            if (pieces[k].seg != pieces[i].seg) break;
-            e = k;
-        }
-        const bool from_start = pieces[i].complete_lo, to_end = pieces[e].complete_hi;
-        const bool whole = from_start && to_end;
-        const int slot = from_start ? 1 : 0;
-        const Seq s = load_seq(cv, pieces[i].seq);
+        __syncthreads();
         for (int idx = tid; idx < C::R * C::D / 4; idx += C::THREADS) {
             const int row = idx / (C::D / 4), d4 = idx % (C::D / 4);
-            float mx = kNegInf;
-            for (int k = i; k <= e; ++k)
-                if (pieces[k].seg >= 0) mx = fmaxf(mx, piece_m[k][row]);
-            float ls = 0.0f;
             float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            for (int k = i; k <= e; ++k) {
-                if (pieces[k].seg < 0) continue;
+            for (unsigned left = mask; left; left &= left - 1) {
+                const int k = __ffs(left) - 1;
                 const float* src = (k & 1) ? reinterpret_cast<const float*>(smem + (k >> 1) * C::SLOT)
                                            : reinterpret_cast<const float*>(
                                                  p.ws + Layout<C>::stash(gridDim.x) +
                                                  (static_cast<size_t>(blockIdx.x) * C::WARPS + (k >> 1)) * C::PIECE);
-                const float a = mx == kNegInf ? 1.0f : exp2f(piece_m[k][row] - mx);
+                const float a = factor[k][row];
                 const float4 x = *reinterpret_cast<const float4*>(src + row * C::D + d4 * 4);
-                ls += a * piece_l[k][row];
                 o.x += a * x.x;
                 o.y += a * x.y;
                 o.z += a * x.z;
                 o.w += a * x.w;
             }
             if (whole) {
-                const int rr = pieces[i].tile * C::R + row;
-                if (rr < s.n * p.group) {
-                    const float inv = inv_sum(ls);
-                    uint16_t* dst = out_row(p, s, pieces[i].head, rr) + d4 * 4;
+                if (first.tile * C::R + row < first.rows) {
+                    const float inv = inv_sum(row_l[row]);
+                    uint16_t* dst = out_row(p, first.q0, first.head, first.tile * C::R + row) + d4 * 4;
                     *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
                 }
             } else {
                 *reinterpret_cast<float4*>(po + slot * (C::R * C::D) + row * C::D + d4 * 4) = o;
-                if (d4 == 0) {
-                    ml[slot * 2 * C::R + row] = mx;
-                    ml[slot * 2 * C::R + C::R + row] = ls;
-                }
             }
         }
-        if (!whole) {
-            have[slot] = true;
-            if (tid == 0) info[slot] = Partial{pieces[i].seg, pieces[i].seq, pieces[i].head, pieces[i].tile, 0};
+        if (whole) continue;
+        // ---- the last of the segment's CTAs to come here joins their parts ----
+        const int cta0 = sh.of(first.seg) / C::WARPS, n = sh.of(first.seg_end - 1) / C::WARPS - cta0 + 1;
+        __syncthreads();                            // the whole part has been written
+        if (tid == 0) {
+            __threadfence();
+            const uint32_t t = atomicAdd(p.tickets + cta0, 1u);
+            is_last = t == static_cast<uint32_t>(n - 1);
+            if (is_last) {
+                p.tickets[cta0] = 0;
+                __threadfence();
+            }
         }
-        i = e + 1;
-    }
-    if (tid < 2 && !have[tid]) info[tid] = Partial{-1, 0, 0, 0, 0};
-}
-
-// Joins the parts of segments that span CTAs: block b leads the segment that
-// begins in CTA b and goes on, and adds the parts of b + 1, b + 2, ... in order.
-template <class C>
-__global__ void __launch_bounds__(256) attend_join_kernel(const AttentionParams p, const int nctas)
-{
-    pdl_launch_dependents();
-    pdl_wait();
-    const Partial* info = reinterpret_cast<const Partial*>(p.ws + Layout<C>::info());
-    const float* ml = reinterpret_cast<const float*>(p.ws + Layout<C>::ml(nctas));
-    const float* po = reinterpret_cast<const float*>(p.ws + Layout<C>::o(nctas));
-    const Partial lead = info[2 * blockIdx.x + 1];
-    if (lead.seg < 0) return;
-    const Seq s = load_seq(p.c, lead.seq);
-    int last = blockIdx.x;
-    while (last + 1 < nctas && info[2 * (last + 1)].seg == lead.seg) ++last;
-    for (int idx = threadIdx.x; idx < C::R * C::D / 4; idx += blockDim.x) {
-        const int row = idx / (C::D / 4), d4 = idx % (C::D / 4);
-        float mx = kNegInf;
-        for (int k = blockIdx.x; k <= last; ++k)
-            mx = fmaxf(mx, ml[(2 * k + (k == static_cast<int>(blockIdx.x))) * 2 * C::R + row]);
-        float ls = 0.0f;
-        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int k = blockIdx.x; k <= last; ++k) {
-            const int sl = 2 * k + (k == static_cast<int>(blockIdx.x));
-            const float a = mx == kNegInf ? 1.0f : exp2f(ml[sl * 2 * C::R + row] - mx);
-            const float4 x = *reinterpret_cast<const float4*>(po + static_cast<size_t>(sl) * C::R * C::D + row * C::D + d4 * 4);
-            ls += a * ml[sl * 2 * C::R + C::R + row];
-            o.x += a * x.x;
-            o.y += a * x.y;
-            o.z += a * x.z;
-            o.w += a * x.w;
+        __syncthreads();
+        if (!is_last) continue;
+        for (int idx = tid; idx < C::R * C::D / 4; idx += C::THREADS) {
+            const int row = idx / (C::D / 4), d4 = idx % (C::D / 4);
+            if (first.tile * C::R + row >= first.rows) continue;
+            // part k is slot 1 of the segment's first CTA, slot 0 of the others
+            const auto at = [&](int k) { return static_cast<size_t>(2 * (cta0 + k) + (k == 0)); };
+            const float4 o = join_parts(
+                n,
+                [&](int k) {
+                    const float* v = all_ml + at(k) * 2 * C::R + row;
+                    return make_float2(__ldcg(v), __ldcg(v + C::R));
+                },
+                [&](int k) { return __ldcg(reinterpret_cast<const float4*>(all_o + at(k) * C::R * C::D + row * C::D + d4 * 4)); });
+            uint16_t* dst = out_row(p, first.q0, first.head, first.tile * C::R + row) + d4 * 4;
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
         }
-        const int rr = lead.tile * C::R + row;
-        if (rr >= s.n * p.group) continue;
-        const float inv = inv_sum(ls);
-        uint16_t* dst = out_row(p, s, lead.head, rr) + d4 * 4;
-        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
     }
 }
 
@@ -694,28 +749,22 @@ cudaError_t launch_few(const AttentionParams& p, int sms, cudaStream_t stream)
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, attend_few_kernel<C>, p);
-    if (e != cudaSuccess) return e;
-    cfg.blockDim = dim3(256);
-    cfg.dynamicSmemBytes = 0;
-    return cudaLaunchKernelEx(&cfg, attend_join_kernel<C>, p, sms);
+    return cudaLaunchKernelEx(&cfg, attend_few_kernel<C>, p);
 }
 
 // Row tile of 8 * NT packed rows: the smallest that holds the rows of any
-// sequence the kernel takes, at most 32.
-int few_nt(int64_t rows) { return rows <= 8 ? 1 : (rows <= 16 ? 2 : 4); }
+// sequence the kernel takes, at most 16.
+int few_nt(int64_t rows) { return rows <= 8 ? 1 : 2; }
 
 template <class F>
 auto with_few(int D, int nt, const F& f)
 {
     if (D == 128) {
         if (nt == 1) return f(DecCfg<128, 1>{});
-        if (nt == 2) return f(DecCfg<128, 2>{});
-        return f(DecCfg<128, 4>{});
+        return f(DecCfg<128, 2>{});
     }
     if (nt == 1) return f(DecCfg<64, 1>{});
-    if (nt == 2) return f(DecCfg<64, 2>{});
-    return f(DecCfg<64, 4>{});
+    return f(DecCfg<64, 2>{});
 }
 
 }  // namespace
@@ -735,9 +784,12 @@ cudaError_t launch_attention(const AttentionParams& p0, int sms, cudaStream_t st
     const int64_t rows = static_cast<int64_t>(p.max_q) * p.group;
     p.few_most = 0x7FFFFFFF;
     if (rows > kFewRows) {
-        // one sequence at least has more rows: attend_many_kernel takes those
-        const cudaError_t e = launch_attend_many(p, sms, stream);
-        if (e != cudaSuccess || p.c.batch == 1) return e;   // (alone, it takes any sequence)
+        // A sequence has more rows than attend_few_kernel is made for.  Where most
+        // may have fewer (the batch's average is within its limit) each kernel takes
+        // its kind; else attend_many_kernel takes all, and one launch is saved.
+        const bool mixed = p.c.tokens * p.group <= static_cast<int64_t>(p.c.batch) * kFewRows;
+        const cudaError_t e = launch_attend_many(p, mixed ? kFewRows : 0, sms, stream);
+        if (e != cudaSuccess || !mixed) return e;
         p.few_most = kFewRows;
     }
     return with_few(p.c.D, few_nt(rows), [&](auto c) { return launch_few<decltype(c)>(p, sms, stream); });

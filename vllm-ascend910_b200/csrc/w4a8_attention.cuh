@@ -12,8 +12,14 @@ namespace w4a8 {
 
 constexpr int kMaxBatch = 2048;            // W4A8_ATTENTION_MAX_BATCH
 constexpr float kNegInf = -INFINITY;
-constexpr int kFewRows = 32;               // packed query rows of a sequence that attend_few_kernel takes beside attend_many_kernel
+constexpr int kFewRows = 16;               // sequences of more packed query rows go to attend_many_kernel
 
+__device__ __forceinline__ uint4 lds128(uint32_t a)
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+    return v;
+}
 // Two int8 codes in bytes 0 and 2 of w (bytes 1 and 3: anything) -> fp16 pair,
 // exactly: the bits 0x6400 | (code + 128) are the fp16 number 1024 + code + 128.
 __device__ __forceinline__ uint32_t codes_to_f16x2(uint32_t w)
@@ -22,6 +28,15 @@ __device__ __forceinline__ uint32_t codes_to_f16x2(uint32_t w)
     const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&m), __half2half2(__ushort_as_half(0x6480)));
     return *reinterpret_cast<const uint32_t*>(&d);
 }
+
+// The same from codes already biased (code ^ 0x80): bytes 0 and 1, or 2 and 3, of w.
+__device__ __forceinline__ uint32_t biased_f16x2(uint32_t m)
+{
+    const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&m), __half2half2(__ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t*>(&d);
+}
+__device__ __forceinline__ uint32_t biased_lo(uint32_t w) { return biased_f16x2(__byte_perm(w, 0x64646464u, 0x4140)); }
+__device__ __forceinline__ uint32_t biased_hi(uint32_t w) { return biased_f16x2(__byte_perm(w, 0x64646464u, 0x4342)); }
 
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi)
 {
@@ -48,12 +63,17 @@ __device__ __forceinline__ float pow2_above(float v)
 }
 constexpr float kVrMin = 7.888609052210118e-31f;   // 2^-100
 constexpr float kWeightOne = 16384.0f;             // 2^14
+constexpr float kSlack = 1.9f;                     // log2 by which scores may exceed the reference maximum: weights stay below 2^15.9
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi)
 {
     const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&b);
 }
+
+// What is added to a row's scaled scores: minus its reference maximum.  Before the
+// first score it is so large that any finite score exceeds the slack.
+__device__ __forceinline__ float first_reference(float m) { return m == kNegInf ? 1e38f : -m; }
 
 // 2^x (one MUFU instruction; results below 2^-126 are 0).
 __device__ __forceinline__ float ex2(float x)
@@ -83,22 +103,98 @@ __device__ __forceinline__ Seq load_seq(const CacheView& c, int s)
     return r;
 }
 
-struct Partial {        // one per CTA and slot, in the workspace
-    long long seg;
-    int seq, head, tile, pad;
+// One per CTA and slot, in the workspace: which segment the part belongs to, and
+// where its rows go.
+struct Partial {
+    long long seg;      // -1: none
+    int q0, rows;       // the sequence's first query token, its packed rows
+    int head, row0;     // kv head, the segment's first packed row
 };
 
-// Output row `row` of a sequence's packed rows for one kv head.
-__device__ __forceinline__ uint16_t* out_row(const AttentionParams& p, const Seq& s, int head, int row)
+// Adds one segment's n parts for 4 elements of one row: parts are the leader's
+// slot 1 and slot 0 of the CTAs behind it.  Loads of 8 parts (maximum, sum, values)
+// are in flight together.
+template <class M, class V>
+__device__ __forceinline__ float4 join_parts(int n, const M& ml, const V& value)
 {
-    const int tok = row / p.group, g = row - tok * p.group;
-    return p.out + static_cast<int64_t>(s.q0 + tok) * p.ldo + static_cast<int64_t>(head * p.group + g) * p.c.D;
+    float mx = kNegInf, ls = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int base = 0; base < n; base += 8) {
+        float m[8], l[8];
+        float4 x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const bool in = base + i < n;
+            const int k = in ? base + i : 0;
+            const float2 v = ml(k);
+            m[i] = in ? v.x : kNegInf;
+            l[i] = in ? v.y : 0.0f;
+            x[i] = value(k);
+        }
+        float mn = mx;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mn = fmaxf(mn, m[i]);
+        const float keep = mx == kNegInf ? (mn == kNegInf ? 1.0f : 0.0f) : exp2f(mx - mn);
+        ls *= keep;
+        o.x *= keep;
+        o.y *= keep;
+        o.z *= keep;
+        o.w *= keep;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (base + i >= n) break;
+            // (a part without a visible token has m = -inf, l = 0 and zeros)
+            const float a = m[i] == kNegInf ? 1.0f : exp2f(m[i] - mn);
+            ls += a * l[i];
+            o.x += a * x[i].x;
+            o.y += a * x[i].y;
+            o.z += a * x[i].z;
+            o.w += a * x[i].w;
+        }
+        mx = mn;
+    }
+    const float inv = ls > 0.0f ? __fdiv_rn(1.0f, ls) : (ls == 0.0f ? 0.0f : ls);
+    return make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+}
+
+// row / group: the query token of a packed row.  With M = floor(2^64 / g) + 1 the
+// high word of row * M is the quotient for every 32-bit row (row * (M g - 2^64)
+// stays below 2^64).
+__device__ __forceinline__ int row_token(const AttentionParams& p, int row)
+{
+    return p.group_magic == 0 ? row : static_cast<int>(__umul64hi(static_cast<uint64_t>(static_cast<uint32_t>(row)), p.group_magic));
+}
+
+// Output row `row` of the packed rows, for one kv head, of the sequence whose first
+// query token is q0.
+__device__ __forceinline__ uint16_t* out_row(const AttentionParams& p, int q0, int head, int row)
+{
+    const int tok = row_token(p, row), g = row - tok * p.group;
+    return p.out + static_cast<int64_t>(q0 + tok) * p.ldo + static_cast<int64_t>(head * p.group + g) * p.c.D;
+}
+
+// The segment that begins in CTA `lead` and goes on: its record and number of
+// parts (0: there is none).  A whole block calls it.
+__device__ __forceinline__ int find_parts(const Partial* info, int lead, int nctas, Partial& rec)
+{
+    int n = 0;
+    for (int base = lead + 1; base <= nctas; base += blockDim.x) {
+        const int k = base + threadIdx.x;
+        const long long seg = k < nctas ? info[2 * k].seg : -1;
+        rec = info[2 * lead + 1];
+        const int more = __syncthreads_count(seg >= 0 && seg == rec.seg);
+        if (rec.seg < 0) return 0;
+        n += more;
+        if (more < static_cast<int>(blockDim.x)) break;
+    }
+    return n + 1;
 }
 
 // 1 / l; 0 for a row that saw no token, NaN for a NaN.
 __device__ __forceinline__ float inv_sum(float l) { return l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l); }
 
 size_t attend_many_ws_bytes(int D, int sms);
-cudaError_t launch_attend_many(const AttentionParams& p, int sms, cudaStream_t stream);
+// Sequences of more than `least` packed rows.
+cudaError_t launch_attend_many(const AttentionParams& p, int least, int sms, cudaStream_t stream);
 
 }  // namespace w4a8

@@ -50,7 +50,6 @@ constexpr int kRegsSoft = 176, kRegsConv = 88, kRegsMma = 64;      // 2, 1 and 1
 static_assert(2 * kRegsSoft + kRegsConv + kRegsMma <= 4 * 128, "the launch allocates 128 registers a thread");
 constexpr int kTileUnits = 4;              // what beginning and ending a tile costs, in blocks (work shares)
 constexpr int kMinUnits = 4;               // a CTA's share is not cut below this
-constexpr float kSlack = 1.9f;             // log2 by which scores may exceed the reference maximum
 constexpr float kMargin = 2.0f;            // log2 by which a new reference exceeds the scores seen
 
 // wait-site ids for the status word
@@ -260,12 +259,12 @@ struct ManyLayout {
 template <class C>
 __device__ __forceinline__ void put_codes(uint32_t stage, int tok, int c, const uint4& v)
 {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    const uint32_t w[4] = {v.x ^ 0x80808080u, v.y ^ 0x80808080u, v.z ^ 0x80808080u, v.w ^ 0x80808080u};
     uint32_t h[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        h[2 * i] = codes_to_f16x2(__byte_perm(w[i], 0, 0x4140));
-        h[2 * i + 1] = codes_to_f16x2(__byte_perm(w[i], 0, 0x4342));
+        h[2 * i] = biased_lo(w[i]);
+        h[2 * i + 1] = biased_hi(w[i]);
     }
     const uint32_t row = stage + (c >> 2) * C::KV_CHUNK + tok * 128;
     const uint32_t u = (c & 3) * 2, x = tok & 7;
@@ -469,6 +468,7 @@ __device__ __forceinline__ void softmax_role(const AttentionParams& p, ManyBars*
     const uint32_t t_o = tbase + lane_off + C::TM_O + x * C::D;
     const uint32_t half_sm = sm + x * C::Q_HALF;                // its queries; afterwards its output rows on their way
     constexpr int LPR = C::D / 8, RPI = 32 / LPR;               // lanes of a row's 16-byte vectors, rows per access
+    const auto q_unit = [&](int r, int u) { return half_sm + (u >> 3) * C::Q_CHUNK + r * 128 + (((u & 7) ^ (r & 7)) << 4); };
     Partial* info = reinterpret_cast<Partial*>(p.ws) + 2 * blockIdx.x;
     float* ml = reinterpret_cast<float*>(p.ws + ManyLayout<C>::ml(gridDim.x)) + static_cast<size_t>(blockIdx.x) * 4 * kRows;
     float* po = reinterpret_cast<float*>(p.ws + ManyLayout<C>::o(gridDim.x) + static_cast<size_t>(blockIdx.x) * 2 * C::PIECE);
@@ -489,43 +489,45 @@ __device__ __forceinline__ void softmax_role(const AttentionParams& p, ManyBars*
         const bool valid = pr < a.s.n * p.group;
         const bool live = __any_sync(0xffffffffu, valid);
 
-        // ---- this warp's 32 queries: largest element to [2^13, 2^14), fp16, into the
-        // operand.  RPI rows a load, a lane per 16 bytes; a lane is a row from here on ----
+        // ---- this warp's 32 queries into the operand: rows come by asynchronous copies
+        // (RPI rows a turn, a lane per 16 bytes), then a lane is a row: its largest
+        // element to [2^13, 2^14), fp16, in place.  Short loops: a tile passes here once ----
         float qs = 0.0f;                                        // what turns a raw score into log2 units
-        const int limit = valid ? a.s.len - a.s.n + pr / p.group : 0x7FFFFFFF;   // last token the row sees
+        const int limit = valid ? a.s.len - a.s.n + row_token(p, pr) : 0x7FFFFFFF;   // last token the row sees
         {
             const int sub = lane / LPR, ch = lane % LPR;
-            uint4 v[32 / RPI];
-#pragma unroll
+#pragma unroll 2
             for (int i = 0; i < 32 / RPI; ++i) {
-                const int r = pr - lane + i * RPI + sub;
-                v[i] = make_uint4(0, 0, 0, 0);
-                if (r < a.s.n * p.group) {
-                    const int tok = r / p.group;
-                    v[i] = *reinterpret_cast<const uint4*>(p.q + static_cast<int64_t>(a.s.q0 + tok) * p.ldq +
-                                                           static_cast<int64_t>(a.head * p.group + (r - tok * p.group)) * C::D +
-                                                           ch * 8);
-                }
+                const int rr = (row & 96) + i * RPI + sub, r = pr - lane + i * RPI + sub;
+                const bool ok = r < a.s.n * p.group;
+                const int tok = ok ? row_token(p, r) : 0;
+                const uint16_t* src = p.q + static_cast<int64_t>(a.s.q0 + tok) * p.ldq +
+                                      static_cast<int64_t>(a.head * p.group + (ok ? r - tok * p.group : 0)) * C::D + ch * 8;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(q_unit(rr, ch)), "l"(src), "r"(ok ? 16 : 0)
+                             : "memory");
             }
-#pragma unroll
-            for (int i = 0; i < 32 / RPI; ++i) {
-                const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-                uint32_t big = 0;
+            asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+            __syncwarp();
+            uint32_t big = 0;
+#pragma unroll 4
+            for (int u = 0; u < LPR; ++u) {
+                const uint4 v = lds128(q_unit(row, u));
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) big = max(big, max((w[e] << 16) & 0x7FFFFFFFu, w[e] & 0x7FFF0000u));
-#pragma unroll
-                for (int o = LPR / 2; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
-                const float shrink = row_shrink(__uint_as_float(big));
-                const float mine = __shfl_sync(0xffffffffu, shrink, (lane % RPI) * LPR);
-                if (lane / RPI == i) qs = mine;
+            }
+            const float shrink = row_shrink(__uint_as_float(big));
+#pragma unroll 4
+            for (int u = 0; u < LPR; ++u) {
+                const uint4 v = lds128(q_unit(row, u));
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
                 uint32_t h[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     h[e] = cvt_f16x2(__uint_as_float(w[e] << 16) * shrink, __uint_as_float(w[e] & 0xFFFF0000u) * shrink);
-                const int rr = (row & 96) + i * RPI + sub;
-                sts128(half_sm + rr * 128 + (ch >> 3) * C::Q_CHUNK + (((ch & 7) ^ (rr & 7)) << 4), h[0], h[1], h[2], h[3]);
+                sts128(q_unit(row, u), h[0], h[1], h[2], h[3]);
             }
-            qs = __fdiv_rn(p.scale_log2, qs);
+            qs = __fdiv_rn(p.scale_log2, shrink);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars->qfull[x]);
@@ -657,9 +659,7 @@ __device__ __forceinline__ void softmax_role(const AttentionParams& p, ManyBars*
                     // through shared memory (its queries are done with), so that rows leave whole
 #pragma unroll
                     for (int i = 0; i < 32; i += 8) {
-                        const int u = (c + i) / 8;
-                        sts128(half_sm + row * 128 + (u >> 3) * C::Q_CHUNK + (((u & 7) ^ (row & 7)) << 4),
-                               pack_bf16(v[i], v[i + 1]), pack_bf16(v[i + 2], v[i + 3]), pack_bf16(v[i + 4], v[i + 5]),
+                        sts128(q_unit(row, (c + i) / 8), pack_bf16(v[i], v[i + 1]), pack_bf16(v[i + 2], v[i + 3]), pack_bf16(v[i + 4], v[i + 5]),
                                pack_bf16(v[i + 6], v[i + 7]));
                     }
                 } else if (valid) {
@@ -674,11 +674,8 @@ __device__ __forceinline__ void softmax_role(const AttentionParams& p, ManyBars*
 #pragma unroll 4
                 for (int i = 0; i < 32 / RPI; ++i) {
                     const int rr = (row & 96) + i * RPI + sub, r = pr - lane + i * RPI + sub;
-                    uint4 v;
-                    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                                 : "r"(half_sm + rr * 128 + (ch >> 3) * C::Q_CHUNK + (((ch & 7) ^ (rr & 7)) << 4)));
-                    if (r < a.s.n * p.group) *reinterpret_cast<uint4*>(out_row(p, a.s, a.head, r) + ch * 8) = v;
+                    const uint4 v = lds128(q_unit(rr, ch));
+                    if (r < a.s.n * p.group) *reinterpret_cast<uint4*>(out_row(p, a.s.q0, a.head, r) + ch * 8) = v;
                 }
                 __syncwarp();
             }
@@ -686,8 +683,8 @@ __device__ __forceinline__ void softmax_role(const AttentionParams& p, ManyBars*
                 ml[slot * 2 * kRows + x * 128 + row] = m;
                 ml[slot * 2 * kRows + kRows + x * 128 + row] = l;
                 if (x == 0 && row == 0)
-                    info[slot] = Partial{(static_cast<long long>(a.seq) * p.c.kv_heads + a.head) * 0x1000000LL + a.tile, a.seq,
-                                         a.head, a.tile, 0};
+                    info[slot] = Partial{(static_cast<long long>(a.seq) * p.c.kv_heads + a.head) * 0x1000000LL + a.tile, a.s.q0,
+                                         a.s.n * p.group, a.head, a.tile * kRows};
             }
             tc_fence_before();
         }
@@ -832,49 +829,31 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Atte
 }
 
 // Joins the parts of tiles that span CTAs: blockIdx.x leads the tile that begins
-// in CTA blockIdx.x and goes on; blockIdx.y takes 16 of its rows.
+// in CTA blockIdx.x and goes on; blockIdx.y takes kJoinRows of its rows.
 constexpr int kJoinRows = 16;
 
 template <class C>
-__global__ void __launch_bounds__(256) attend_many_join_kernel(const AttentionParams p, const int nctas)
+__global__ void __launch_bounds__(kJoinRows * C::D / 4) attend_many_join_kernel(const AttentionParams p, const int nctas)
 {
     pdl_launch_dependents();
     pdl_wait();
-    const Partial* info = reinterpret_cast<const Partial*>(p.ws);
     const float* ml = reinterpret_cast<const float*>(p.ws + ManyLayout<C>::ml(nctas));
     const float4* po = reinterpret_cast<const float4*>(p.ws + ManyLayout<C>::o(nctas));
-    const int lead_cta = blockIdx.x;
-    const Partial lead = info[2 * lead_cta + 1];
-    if (lead.seg < 0) return;
-    const Seq s = load_seq(p.c, lead.seq);
-    int last = lead_cta;
-    while (last + 1 < nctas && info[2 * (last + 1)].seg == lead.seg) ++last;
-    for (int idx = threadIdx.x; idx < kJoinRows * C::D / 4; idx += 256) {
-        const int row = blockIdx.y * kJoinRows + idx % kJoinRows, d4 = idx / kJoinRows;
-        const int pr = lead.tile * kRows + row;
-        if (pr >= s.n * p.group) continue;
-        float mx = kNegInf;
-        for (int k = lead_cta; k <= last; ++k) mx = fmaxf(mx, ml[(2 * k + (k == lead_cta)) * 2 * kRows + row]);
-        float ls = 0.0f;
-        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int k = lead_cta; k <= last; ++k) {
-            const size_t sl = 2 * k + (k == lead_cta);
-            const float a = mx == kNegInf ? 1.0f : ex2(ml[sl * 2 * kRows + row] - mx);
-            const float4 v = po[sl * (kRows * C::D / 4) + static_cast<size_t>(d4) * kRows + row];
-            ls += a * ml[sl * 2 * kRows + kRows + row];
-            o.x += a * v.x;
-            o.y += a * v.y;
-            o.z += a * v.z;
-            o.w += a * v.w;
-        }
-        const float inv = inv_sum(ls);
-        *reinterpret_cast<uint2*>(out_row(p, s, lead.head, pr) + d4 * 4) =
-            make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
-    }
+    const int lead = blockIdx.x;
+    Partial rec;
+    const int n = find_parts(reinterpret_cast<const Partial*>(p.ws), lead, nctas, rec);
+    const int row = blockIdx.y * kJoinRows + threadIdx.x % kJoinRows, d4 = threadIdx.x / kJoinRows;
+    if (n == 0 || rec.row0 + row >= rec.rows) return;
+    const auto slot = [&](int i) { return 2 * (lead + i) + (i == 0); };
+    const float4 o = join_parts(
+        n, [&](int i) { const float* v = ml + slot(i) * 2 * kRows + row; return make_float2(v[0], v[kRows]); },
+        [&](int i) { return po[static_cast<size_t>(slot(i)) * (kRows * C::D / 4) + static_cast<size_t>(d4) * kRows + row]; });
+    *reinterpret_cast<uint2*>(out_row(p, rec.q0, rec.head, rec.row0 + row) + d4 * 4) =
+        make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
 }
 
 template <class C>
-cudaError_t launch_many(const AttentionParams& p, int sms, cudaStream_t stream)
+cudaError_t launch_many(const AttentionParams& p, int least, int sms, cudaStream_t stream)
 {
     const int fixed = C::OFF_PREFIX + 1024;
     static bool ready[64] = {};          // per device
@@ -900,10 +879,10 @@ cudaError_t launch_many(const AttentionParams& p, int sms, cudaStream_t stream)
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, attend_many_kernel<C>, p, p.c.batch == 1 ? 0 : kFewRows);
+    e = cudaLaunchKernelEx(&cfg, attend_many_kernel<C>, p, least);
     if (e != cudaSuccess) return e;
     cfg.gridDim = dim3(sms, kRows / kJoinRows);
-    cfg.blockDim = dim3(256);
+    cfg.blockDim = dim3(kJoinRows * C::D / 4);
     cfg.dynamicSmemBytes = 0;
     return cudaLaunchKernelEx(&cfg, attend_many_join_kernel<C>, p, sms);
 }
@@ -915,9 +894,9 @@ size_t attend_many_ws_bytes(int D, int sms)
     return D == 128 ? ManyLayout<ManyCfg<128>>::total(sms) : ManyLayout<ManyCfg<64>>::total(sms);
 }
 
-cudaError_t launch_attend_many(const AttentionParams& p, int sms, cudaStream_t stream)
+cudaError_t launch_attend_many(const AttentionParams& p, int least, int sms, cudaStream_t stream)
 {
-    return p.c.D == 128 ? launch_many<ManyCfg<128>>(p, sms, stream) : launch_many<ManyCfg<64>>(p, sms, stream);
+    return p.c.D == 128 ? launch_many<ManyCfg<128>>(p, least, sms, stream) : launch_many<ManyCfg<64>>(p, least, sms, stream);
 }
 
 }  // namespace w4a8

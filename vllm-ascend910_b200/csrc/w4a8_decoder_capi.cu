@@ -10,6 +10,7 @@ using namespace w4a8;
 namespace {
 
 constexpr size_t kStatusBytes = 1024;      // status word block at the start of a workspace
+constexpr int kTicketWord = 16;            // first ticket word within it
 constexpr int64_t kMaxTokens = int64_t(1) << 30;
 
 bool aligned(const void* ptr, uintptr_t a) { return (reinterpret_cast<uintptr_t>(ptr) & (a - 1)) == 0; }
@@ -150,9 +151,12 @@ int w4a8_attention(const w4a8_kv_cache* cache, const int32_t* page_table, int64_
     p.ldo = ldo;
     p.q_heads = q_heads;
     p.group = q_heads / cache->kv_heads;
+    p.group_magic = p.group == 1 ? 0 : ~static_cast<uint64_t>(0) / static_cast<uint64_t>(p.group) + 1;
     p.max_q = max_q_len;
     p.scale_log2 = softmax_scale * 1.4426950408889634f;
     p.status = static_cast<int*>(workspace);
+    p.tickets = static_cast<uint32_t*>(workspace) + kTicketWord;
+    if (sms > static_cast<int>(kStatusBytes / 4) - kTicketWord) return W4A8_ERR_DEVICE;
     p.ws = static_cast<uint8_t*>(workspace) + kStatusBytes;
     const cudaError_t e = launch_attention(p, sms, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? W4A8_OK : capi_fail_cuda(e);

@@ -217,10 +217,12 @@ struct AttentionParams {
     uint16_t* out;            // bf16 [tokens, ldo]
     int64_t ldq, ldo;
     int q_heads, group;       // group: query heads per kv head
+    uint64_t group_magic;     // floor(2^64 / group) + 1 (0 for group 1): see row_token
     int max_q;                // no sequence has more query tokens (host's knowledge)
     float scale_log2;         // softmax scale * log2(e)
     int few_most;             // attend_few_kernel takes sequences of at most this many packed rows
     int* status;              // workspace: status word
+    uint32_t* tickets;        // workspace: zeroed counters beside it, one per CTA (attend_few_kernel leaves them zero)
     uint8_t* ws;              // workspace past the status block
 };
 
