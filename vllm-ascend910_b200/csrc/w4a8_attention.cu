@@ -240,10 +240,10 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ PieceInfo pieces[2 * C::WARPS];
     __shared__ float piece_m[2 * C::WARPS][C::R], piece_l[2 * C::WARPS][C::R];
-    __shared__ float factor[2 * C::WARPS][C::R], row_l[C::R];
     __shared__ long long warp_sum[C::WARPS];
     __shared__ long long running;
-    __shared__ bool is_last;
+    __shared__ bool is_last[2];
+    __shared__ int seg_cta0[2], seg_parts[2];
     long long* prefix = reinterpret_cast<long long*>(smem + C::SMEM);   // [batch + 1] units before each sequence
 
     const int tid = threadIdx.x, warp = warp_id(), lane = lane_id();
@@ -310,12 +310,19 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
         const uint32_t v1 = C::D == 128 ? chunk_off<C::D>(2 * c + 1, r) : chunk_off<C::D>(2 * c + 1, r >> 1) + (r & 1) * 8;
         const int pages = static_cast<int>(cv.pages);
         int ahead = static_cast<int>(u1 - u0);    // units of the share still to be fetched
+        // Page ids of a sequence, 32 at a time: lane i holds that of page id_page + i.
+        int ids = -1, id_seq = -1, id_page = 0;
 
         // Brings the unit under `pre` into ring stage st and moves on.
         auto fetch = [&](int st) {
             if (ahead > 0) {
-                const int tok = pre.blk * kBlkTok;
-                const int id = tok < pre.s.len ? cv.table[pre.seq * cv.ld_table + (tok >> cv.page_log2)] : -1;
+                const int tok = pre.blk * kBlkTok, pg = tok >> cv.page_log2;
+                if (pre.seq != id_seq || pg < id_page || pg >= id_page + 32) {
+                    id_seq = pre.seq;
+                    id_page = pg;
+                    ids = pg + lane <= (pre.s.len - 1) >> cv.page_log2 ? cv.table[pre.seq * cv.ld_table + pg + lane] : -1;
+                }
+                const int id = __shfl_sync(0xffffffffu, ids, pg - id_page);
                 const bool ok = static_cast<unsigned>(id) < static_cast<unsigned>(pages);
                 const int64_t ph = ok ? static_cast<int64_t>(id) * cv.kv_heads + pre.head : 0;
                 const int64_t at = ((ph << cv.page_log2) + (ok ? tok & (cv.page - 1) : 0)) * C::D + lane * 16;
@@ -337,20 +344,14 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
             cp_commit();
         };
 
-#pragma unroll
-        for (int i = 0; i < kStages - 1; ++i) fetch(i);
-
         uint32_t qf[C::NT][C::D / 16][2];
         int limit[C::NT][2];
         float qs[C::NT][2];
         float vr = kVrMin;                        // power of two at or above every vs of the segment so far
         float vr_inv = kWeightOne / kVrMin;       // 2^14 / vr
         int min_limit = 0;
-        // Query rows of the segment under `cur`, and a fresh softmax state.
-        auto begin_segment = [&]() {
-            min_limit = 0x7FFFFFFF;
-            vr = kVrMin;
-            vr_inv = kWeightOne / kVrMin;
+        // The segment's query rows as they are, this lane's elements of row r.
+        auto load_queries = [&]() {
 #pragma unroll
             for (int nt = 0; nt < C::NT; ++nt) {
                 const int row = cur.tile * C::R + nt * 8 + r;
@@ -358,7 +359,6 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
                 const int tok = ok ? row_token(p, row) : 0, g = ok ? row - tok * p.group : 0;
                 const uint16_t* q = p.q + static_cast<int64_t>(cur.s.q0 + tok) * p.ldq +
                                     static_cast<int64_t>(cur.head * p.group + g) * C::D + c * (C::D / 4);
-                uint32_t big = 0;
 #pragma unroll
                 for (int i = 0; i < C::D / 32; ++i) {
                     const uint4 v = ok ? *reinterpret_cast<const uint4*>(q + 8 * i) : make_uint4(0, 0, 0, 0);
@@ -367,7 +367,17 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
                     qf[nt][2 * i + 1][0] = v.z;
                     qf[nt][2 * i + 1][1] = v.w;
                 }
+            }
+        };
+        // The rows in fp16, and a fresh softmax state.
+        auto begin_segment = [&]() {
+            min_limit = 0x7FFFFFFF;
+            vr = kVrMin;
+            vr_inv = kWeightOne / kVrMin;
+#pragma unroll
+            for (int nt = 0; nt < C::NT; ++nt) {
                 // the row's largest magnitude, as bits: its elements are in the four lanes of r
+                uint32_t big = 0;
 #pragma unroll
                 for (int i = 0; i < C::D / 16; ++i)
 #pragma unroll
@@ -404,6 +414,9 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
             min_limit = __reduce_min_sync(0xffffffffu, min_limit);
         };
 
+        load_queries();
+#pragma unroll
+        for (int i = 0; i < kStages - 1; ++i) fetch(i);
         begin_segment();
         long long seg_lo = u0 - cur.blk;          // first unit of the segment under `cur`
         int piece_blk = cur.blk;                  // the piece's first block
@@ -620,6 +633,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
                 if (seg_end) {
                     seg_lo = u1 - left + 1;
                     piece_blk = 0;
+                    load_queries();
                     begin_segment();
                 }
             }
@@ -635,48 +649,39 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
     float* ml = all_ml + static_cast<size_t>(blockIdx.x) * 2 * 2 * C::R;
     float* po = all_o + static_cast<size_t>(blockIdx.x) * 2 * C::R * C::D;
     const long long my_seg = lane < 2 * C::WARPS ? pieces[lane].seg : -1;
-    unsigned todo = __ballot_sync(0xffffffffu, my_seg >= 0);
-    while (todo) {
+    constexpr int ITEMS = C::R * C::D / 4;          // a segment's rows, 4 elements each
+    int open[2] = {-1, -1};                         // first pieces of the segments that other CTAs have parts of
+    int turn = 0;
+    for (unsigned todo = __ballot_sync(0xffffffffu, my_seg >= 0); todo; ++turn) {
         // the pieces of one segment, a bit each
         const int i = __ffs(todo) - 1;
         const unsigned mask = __ballot_sync(0xffffffffu, my_seg == __shfl_sync(0xffffffffu, my_seg, i));
-        const int e = 31 - __clz(mask);
+        const int e = 31 - __clz(mask), n = __popc(mask);
         todo &= ~mask;
         const PieceInfo first = pieces[i];
         const bool whole = first.complete_lo && pieces[e].complete_hi;
         const int slot = first.complete_lo ? 1 : 0;
-        __syncthreads();                            // the previous segment's factors have been read
-        for (int row = warp; row < C::R; row += C::WARPS) {      // a lane per piece
-            const bool in = (mask >> lane) & 1;
-            const float pm = in ? piece_m[lane][row] : kNegInf;
-            float mx = pm;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            const float a = in ? (mx == kNegInf ? 1.0f : ex2(pm - mx)) : 0.0f;
-            float ls = in ? a * piece_l[lane][row] : 0.0f;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, o);
-            if (lane < 2 * C::WARPS) factor[lane][row] = a;
-            if (lane == 0) {
-                row_l[row] = ls;
-                if (!whole) {
-                    ml[slot * 2 * C::R + row] = mx;
-                    ml[slot * 2 * C::R + C::R + row] = ls;
-                }
-            }
-        }
-        __syncthreads();
-        for (int idx = tid; idx < C::R * C::D / 4; idx += C::THREADS) {
+        if (!whole) open[slot] = i;
+        // segments go round the thread groups that hold one each
+        constexpr int GROUPS = C::THREADS >= ITEMS ? C::THREADS / ITEMS : 1;
+        if (GROUPS > 1 && tid / ITEMS != turn % GROUPS) continue;
+        for (int idx = GROUPS > 1 ? tid % ITEMS : tid; idx < ITEMS; idx += GROUPS > 1 ? ITEMS : C::THREADS) {
             const int row = idx / (C::D / 4), d4 = idx % (C::D / 4);
+            float mx = kNegInf;
+            for (unsigned left = mask; left; left &= left - 1) mx = fmaxf(mx, piece_m[__ffs(left) - 1][row]);
+            float ls = 0.0f;
             float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            for (unsigned left = mask; left; left &= left - 1) {
+            unsigned left = mask;
+#pragma unroll 4
+            for (int j = 0; j < n; ++j, left &= left - 1) {
                 const int k = __ffs(left) - 1;
                 const float* src = (k & 1) ? reinterpret_cast<const float*>(smem + (k >> 1) * C::SLOT)
                                            : reinterpret_cast<const float*>(
                                                  p.ws + Layout<C>::stash(gridDim.x) +
                                                  (static_cast<size_t>(blockIdx.x) * C::WARPS + (k >> 1)) * C::PIECE);
-                const float a = factor[k][row];
+                const float a = mx == kNegInf ? 1.0f : ex2(piece_m[k][row] - mx);
                 const float4 x = *reinterpret_cast<const float4*>(src + row * C::D + d4 * 4);
+                ls += a * piece_l[k][row];
                 o.x += a * x.x;
                 o.y += a * x.y;
                 o.z += a * x.z;
@@ -684,30 +689,41 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
             }
             if (whole) {
                 if (first.tile * C::R + row < first.rows) {
-                    const float inv = inv_sum(row_l[row]);
+                    const float inv = inv_sum(ls);
                     uint16_t* dst = out_row(p, first.q0, first.head, first.tile * C::R + row) + d4 * 4;
                     *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
                 }
             } else {
                 *reinterpret_cast<float4*>(po + slot * (C::R * C::D) + row * C::D + d4 * 4) = o;
+                if (d4 == 0) {
+                    ml[slot * 2 * C::R + row] = mx;
+                    ml[slot * 2 * C::R + C::R + row] = ls;
+                }
             }
         }
-        if (whole) continue;
-        // ---- the last of the segment's CTAs to come here joins their parts ----
+    }
+    if (open[0] < 0 && open[1] < 0) return;
+    // ---- the last of a segment's CTAs to come here joins their parts ----
+    __syncthreads();                                // the CTA's parts have been written
+    if (warp < 2 && lane == 0) is_last[warp] = false;
+    if (warp < 2 && lane == 0 && open[warp] >= 0) {
+        const PieceInfo& first = pieces[open[warp]];
         const int cta0 = sh.of(first.seg) / C::WARPS, n = sh.of(first.seg_end - 1) / C::WARPS - cta0 + 1;
-        __syncthreads();                            // the whole part has been written
-        if (tid == 0) {
+        seg_cta0[warp] = cta0;
+        seg_parts[warp] = n;
+        __threadfence();
+        if (atomicAdd(p.tickets + cta0, 1u) == static_cast<uint32_t>(n - 1)) {
+            is_last[warp] = true;
+            p.tickets[cta0] = 0;
             __threadfence();
-            const uint32_t t = atomicAdd(p.tickets + cta0, 1u);
-            is_last = t == static_cast<uint32_t>(n - 1);
-            if (is_last) {
-                p.tickets[cta0] = 0;
-                __threadfence();
-            }
         }
-        __syncthreads();
-        if (!is_last) continue;
-        for (int idx = tid; idx < C::R * C::D / 4; idx += C::THREADS) {
+    }
+    __syncthreads();
+    for (int sl = 0; sl < 2; ++sl) {
+        if (open[sl] < 0 || !is_last[sl]) continue;
+        const PieceInfo first = pieces[open[sl]];
+        const int cta0 = seg_cta0[sl], n = seg_parts[sl];
+        for (int idx = tid; idx < ITEMS; idx += C::THREADS) {
             const int row = idx / (C::D / 4), d4 = idx % (C::D / 4);
             if (first.tile * C::R + row >= first.rows) continue;
             // part k is slot 1 of the segment's first CTA, slot 0 of the others

@@ -12,7 +12,7 @@ namespace w4a8 {
 
 constexpr int kMaxBatch = 2048;            // W4A8_ATTENTION_MAX_BATCH
 constexpr float kNegInf = -INFINITY;
-constexpr int kFewRows = 16;               // sequences of more packed query rows go to attend_many_kernel
+constexpr int kFewRows = 32;               // sequences of more packed query rows go to attend_many_kernel
 
 __device__ __forceinline__ uint4 lds128(uint32_t a)
 {
