@@ -124,6 +124,16 @@ __device__ __forceinline__ uint32_t chunk_off(int t, int ch)
     return t * 64 + ((ch ^ ((t >> 1) & 3)) << 4);
 }
 
+// Where 16-byte unit u of row `row` of a piece lies: permuted so that the eight
+// lanes of a store phase (four rows 2c + h, two neighbouring r) and of a read
+// phase (eight units of one row) hit different banks.
+template <int D>
+__device__ __forceinline__ int piece_off(int row, int u)
+{
+    const int c = (row >> 1) & 3;
+    return row * D * 4 + ((u ^ (D == 128 ? c : (c & 1) | ((c & 2) << 1))) << 4);
+}
+
 // One piece of a segment kept for the join: unit range and softmax state.
 struct PieceInfo {
     long long seg, seg_end;          // the segment's units; seg -1: no piece
@@ -593,13 +603,13 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
                 } else {
                     const bool last = left == 1;
                     const int pi = 2 * warp + (last ? 1 : 0);
-                    float* dst;
+                    uint8_t* dst;
                     if (last) {
                         cp_wait<0>();
                         __syncwarp();
-                        dst = reinterpret_cast<float*>(smem + warp * C::SLOT);
+                        dst = smem + warp * C::SLOT;
                     } else {
-                        dst = reinterpret_cast<float*>(p.ws + Layout<C>::stash(gridDim.x) + wk * C::PIECE);
+                        dst = p.ws + Layout<C>::stash(gridDim.x) + static_cast<size_t>(wk) * C::PIECE;
                     }
 #pragma unroll
                     for (int nt = 0; nt < C::NT; ++nt)
@@ -608,7 +618,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
                             const int row = nt * 8 + 2 * c + h;
 #pragma unroll
                             for (int i = 0; i < C::D / 16; i += 2)
-                                *reinterpret_cast<float4*>(dst + row * C::D + r * (C::D / 8) + 2 * i) =
+                                *reinterpret_cast<float4*>(dst + piece_off<C::D>(row, r * (C::D / 32) + i / 2)) =
                                     make_float4(acc[nt][i][h], acc[nt][i][2 + h], acc[nt][i + 1][h], acc[nt][i + 1][2 + h]);
                             if (r == 0) {
                                 piece_m[pi][row] = m[nt][h];
@@ -656,7 +666,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
         // the pieces of one segment, a bit each
         const int i = __ffs(todo) - 1;
         const unsigned mask = __ballot_sync(0xffffffffu, my_seg == __shfl_sync(0xffffffffu, my_seg, i));
-        const int e = 31 - __clz(mask), n = __popc(mask);
+        const int e = 31 - __clz(mask);
         todo &= ~mask;
         const PieceInfo first = pieces[i];
         const bool whole = first.complete_lo && pieces[e].complete_hi;
@@ -666,38 +676,56 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
         constexpr int GROUPS = C::THREADS >= ITEMS ? C::THREADS / ITEMS : 1;
         if (GROUPS > 1 && tid / ITEMS != turn % GROUPS) continue;
         for (int idx = GROUPS > 1 ? tid % ITEMS : tid; idx < ITEMS; idx += GROUPS > 1 ? ITEMS : C::THREADS) {
-            const int row = idx / (C::D / 4), d4 = idx % (C::D / 4);
-            float mx = kNegInf;
-            for (unsigned left = mask; left; left &= left - 1) mx = fmaxf(mx, piece_m[__ffs(left) - 1][row]);
-            float ls = 0.0f;
-            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            unsigned left = mask;
-#pragma unroll 4
-            for (int j = 0; j < n; ++j, left &= left - 1) {
-                const int k = __ffs(left) - 1;
-                const float* src = (k & 1) ? reinterpret_cast<const float*>(smem + (k >> 1) * C::SLOT)
-                                           : reinterpret_cast<const float*>(
-                                                 p.ws + Layout<C>::stash(gridDim.x) +
-                                                 (static_cast<size_t>(blockIdx.x) * C::WARPS + (k >> 1)) * C::PIECE);
-                const float a = mx == kNegInf ? 1.0f : ex2(piece_m[k][row] - mx);
-                const float4 x = *reinterpret_cast<const float4*>(src + row * C::D + d4 * 4);
-                ls += a * piece_l[k][row];
-                o.x += a * x.x;
-                o.y += a * x.y;
-                o.z += a * x.z;
-                o.w += a * x.w;
+            // a warp has one row (or two): lane k finds the factor of piece k
+            constexpr int RPW = 128 / C::D;
+            const int row = idx / (C::D / 4), d4 = idx % (C::D / 4), row0 = row & ~(RPW - 1);
+            const bool in = (mask >> lane) & 1;
+            float a[RPW], mx[RPW], ls[RPW];
+#pragma unroll
+            for (int k = 0; k < RPW; ++k) {
+                const float pm = in ? piece_m[lane][row0 + k] : kNegInf;
+                mx[k] = pm;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], o));
+                a[k] = in ? (mx[k] == kNegInf ? 1.0f : ex2(pm - mx[k])) : 0.0f;
+                ls[k] = in ? a[k] * piece_l[lane][row0 + k] : 0.0f;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) ls[k] += __shfl_xor_sync(0xffffffffu, ls[k], o);
             }
+            const int mine = RPW > 1 ? row - row0 : 0;
+            const int off = piece_off<C::D>(row, d4);
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            const auto add = [&](int k, const float4& x) {
+                float f = __shfl_sync(0xffffffffu, a[0], k);
+                if (RPW > 1) {
+                    const float f1 = __shfl_sync(0xffffffffu, a[RPW - 1], k);
+                    f = mine ? f1 : f;
+                }
+                o.x += f * x.x;
+                o.y += f * x.y;
+                o.z += f * x.z;
+                o.w += f * x.w;
+            };
+            const uint8_t* stash = p.ws + Layout<C>::stash(gridDim.x) + static_cast<size_t>(blockIdx.x) * C::WARPS * C::PIECE + off;
+            // in unit order: the only stashed piece of a segment is its last one's warp's
+            // first, all others are in shared memory
+#pragma unroll 4
+            for (unsigned left = mask & 0xAAAAAAAAu; left; left &= left - 1) {
+                const int k = __ffs(left) - 1;
+                add(k, *reinterpret_cast<const float4*>(smem + (k >> 1) * C::SLOT + off));
+            }
+            if (mask & 0x55555555u) add(e, __ldcg(reinterpret_cast<const float4*>(stash + static_cast<size_t>(e >> 1) * C::PIECE)));
             if (whole) {
                 if (first.tile * C::R + row < first.rows) {
-                    const float inv = inv_sum(ls);
+                    const float inv = inv_sum(ls[mine]);
                     uint16_t* dst = out_row(p, first.q0, first.head, first.tile * C::R + row) + d4 * 4;
                     *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
                 }
             } else {
                 *reinterpret_cast<float4*>(po + slot * (C::R * C::D) + row * C::D + d4 * 4) = o;
                 if (d4 == 0) {
-                    ml[slot * 2 * C::R + row] = mx;
-                    ml[slot * 2 * C::R + C::R + row] = ls;
+                    ml[slot * 2 * C::R + row] = mx[mine];
+                    ml[slot * 2 * C::R + C::R + row] = ls[mine];
                 }
             }
         }
@@ -711,11 +739,14 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
         const int cta0 = sh.of(first.seg) / C::WARPS, n = sh.of(first.seg_end - 1) / C::WARPS - cta0 + 1;
         seg_cta0[warp] = cta0;
         seg_parts[warp] = n;
-        __threadfence();
-        if (atomicAdd(p.tickets + cta0, 1u) == static_cast<uint32_t>(n - 1)) {
+        uint32_t ticket;
+        asm volatile("fence.acq_rel.gpu;\n\tatom.relaxed.gpu.global.add.u32 %0, [%1], 1;\n\tfence.acq_rel.gpu;"
+                     : "=r"(ticket)
+                     : "l"(p.tickets + cta0)
+                     : "memory");
+        if (ticket == static_cast<uint32_t>(n - 1)) {
             is_last[warp] = true;
             p.tickets[cta0] = 0;
-            __threadfence();
         }
     }
     __syncthreads();
