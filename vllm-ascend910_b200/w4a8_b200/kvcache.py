@@ -125,35 +125,60 @@ def rotary_table(rot: int, positions: int, base: float = 1e6, scaling: Optional[
 
 # ---------------------------------------------------------------- the step's arguments
 
+_I32, _BF16 = torch.int32, torch.bfloat16
+
+
 def _batch(what: str, cache: KVCache, page_table, kv_lens, cu):
-    """Checks the batch tensors; (batch, table pointer, row stride, columns)."""
+    """Checks the batch tensors; (batch, table pointer, row stride, columns).  A decode step makes many
+    small calls, so the checks read each attribute once."""
     dev = cache.device
-    if (page_table.dtype != torch.int32 or kv_lens.dtype != torch.int32 or cu.dtype != torch.int32 or
-            page_table.device != dev or kv_lens.device != dev or cu.device != dev):
+    if not (page_table.dtype is _I32 and kv_lens.dtype is _I32 and cu.dtype is _I32 and page_table.device == dev and
+            kv_lens.device == dev and cu.device == dev):
         raise RuntimeError(f"{what}: page_table, kv_lens and cu must be int32 on the cache's device")
-    B = kv_lens.shape[0] if kv_lens.dim() == 1 else -1
-    if B < 0 or page_table.dim() != 2 or page_table.shape[0] != B or cu.dim() != 1 or cu.shape[0] != B + 1:
+    try:
+        rows, cols = page_table.shape
+        B, = kv_lens.shape
+        ok = rows == B and cu.shape == (B + 1,)
+    except ValueError:
+        ok = False
+    if not ok:
         raise RuntimeError(f"{what}: page_table [batch, columns], kv_lens [batch] and cu [batch + 1] do not agree")
-    if B > 0 and ((page_table.shape[1] > 1 and page_table.stride(1) != 1) or (B > 1 and kv_lens.stride(0) != 1) or
-                  cu.stride(0) != 1):
-        raise RuntimeError(f"{what}: page_table's rows, kv_lens and cu must be dense")
-    cols = page_table.shape[1]
-    return B, page_table.data_ptr(), (page_table.stride(0) if B > 1 else cols), cols
+    if not (kv_lens.is_contiguous() and cu.is_contiguous()):
+        raise RuntimeError(f"{what}: kv_lens and cu must be dense")
+    if page_table.is_contiguous():
+        return B, page_table.data_ptr(), cols, cols
+    ld, step = page_table.stride()
+    if step != 1 and cols > 1 or ld < cols and B > 1:
+        raise RuntimeError(f"{what}: page_table's rows must be dense")
+    return B, page_table.data_ptr(), max(ld, cols), cols
 
 
 def _heads(what: str, name: str, t: torch.Tensor, cache: KVCache):
     """t as [tokens, heads, head_dim] whose heads are dense within a token and whose rows suit 16-byte
-    accesses (copied if they are not); its row stride."""
-    if t.dtype != torch.bfloat16 or t.device != cache.device or t.dim() != 3 or t.shape[2] != cache.head_dim:
-        raise RuntimeError(f"{what}: {name} must be bfloat16 [tokens, heads, {cache.head_dim}] on the cache's device")
-    D = t.shape[2]
-    s = t.stride()
-    if s[2] != 1 or (s[1] != D and t.shape[1] > 1) or s[0] % 8 or s[0] < t.shape[1] * D or t.data_ptr() % 16:
-        t = t.contiguous()
-        if t.data_ptr() % 16 or t.stride(0) < t.shape[1] * D:
-            t = t.clone(memory_format=torch.contiguous_format)
-        return t, t.shape[1] * D
-    return t, s[0]
+    accesses (copied if they are not); tokens, heads, row stride, pointer."""
+    D = cache.head_dim
+    if t.dtype is not _BF16 or t.dim() != 3 or t.shape[2] != D or t.device != cache.device:
+        raise RuntimeError(f"{what}: {name} must be bfloat16 [tokens, heads, {D}] on the cache's device")
+    T, H, _ = t.shape
+    s0, s1, s2 = t.stride()
+    ptr = t.data_ptr()
+    if s2 != 1 or (s1 != D and H > 1) or s0 % 8 or s0 < H * D or ptr % 16:
+        t = torch.empty((T, H, D), dtype=_BF16, device=t.device).copy_(t)
+        return t, T, H, H * D, t.data_ptr()
+    return t, T, H, s0, ptr
+
+
+def _out_like(what: str, name: str, out: Optional[torch.Tensor], t: torch.Tensor, T: int, H: int, cache: KVCache):
+    """The output of t's shape: a new dense tensor, or the caller's after the checks; its row stride and pointer."""
+    if out is None:
+        out = torch.empty_like(t) if t.is_contiguous() else torch.empty((T, H, cache.head_dim), dtype=_BF16, device=t.device)
+        return out, H * cache.head_dim, out.data_ptr()
+    if out.shape != t.shape:
+        raise RuntimeError(f"{what}: {name} must have q's shape")
+    dense, _, _, ld, ptr = _heads(what, name, out, cache)
+    if dense is not out:
+        raise RuntimeError(f"{what}: {name}'s heads must be dense and its rows 16-byte aligned")
+    return out, ld, ptr
 
 
 def kv_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
@@ -166,41 +191,31 @@ def kv_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, page_table: torch
     are turned by the token's position in its sequence: first and second half pairwise, or
     neighbours with ``interleaved``.  q, k and v may be strided views of one [q | k | v] tensor."""
     B, tp, ld, cols = _batch("kv_write", cache, page_table, kv_lens, cu_q)
-    k, ldk = _heads("kv_write", "k", k, cache)
-    v, ldv = _heads("kv_write", "v", v, cache)
-    T = k.shape[0]
-    if k.shape[1] != cache.kv_heads or v.shape != k.shape:
+    k, T, H, ldk, kp = _heads("kv_write", "k", k, cache)
+    v, Tv, Hv, ldv, vp = _heads("kv_write", "v", v, cache)
+    if H != cache.kv_heads or Hv != H or Tv != T:
         raise RuntimeError(f"kv_write: k and v must both be [tokens, {cache.kv_heads}, {cache.head_dim}]")
     qp, ldq, hq, op, ldo, out = None, 0, 0, None, 0, None
     if q is not None:
-        q, ldq = _heads("kv_write", "q", q, cache)
-        hq = q.shape[1]
-        if q.shape[0] != T or hq == 0:
+        q, Tq, hq, ldq, qp = _heads("kv_write", "q", q, cache)
+        if Tq != T or hq == 0:
             raise RuntimeError("kv_write: q must have k's tokens and at least one head")
-        if q_out is None:
-            out = torch.empty((T, hq, cache.head_dim), dtype=torch.bfloat16, device=q.device)
-        else:
-            out = q_out
-            _check(out.shape == q.shape, "kv_write: q_out must have q's shape")
-            dense, _ = _heads("kv_write", "q_out", out, cache)
-            _check(dense is out, "kv_write: q_out's heads must be dense and its rows 16-byte aligned")
-        qp, op, ldo = q.data_ptr(), out.data_ptr(), out.stride(0) if T > 1 else hq * cache.head_dim
-    else:
-        _check(q_out is None, "kv_write: q_out without q")
+        out, ldo, op = _out_like("kv_write", "q_out", q_out, q, T, hq, cache)
+    elif q_out is not None:
+        raise RuntimeError("kv_write: q_out without q")
     cs, rows, rot = None, 0, 0
     if cos_sin is not None:
-        if (cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or not cos_sin.is_contiguous() or
+        if (cos_sin.dtype is not torch.float32 or cos_sin.dim() != 2 or not cos_sin.is_contiguous() or
                 cos_sin.device != cache.device):
             raise RuntimeError("kv_write: cos_sin must be a dense float32 [positions, rot] on the cache's device")
         rows, rot = cos_sin.shape
-        _check(0 < rot <= cache.head_dim and rot % 16 == 0 and rows > 0,
-               "kv_write: rot must be a multiple of 16, at most head_dim")
+        if not (0 < rot <= cache.head_dim and rot % 16 == 0 and rows > 0):
+            raise RuntimeError("kv_write: rot must be a multiple of 16, at most head_dim")
         cs = cos_sin.data_ptr()
     if T == 0 or B == 0:
         return out
-    rc = _lib.lib().w4a8_kv_write(cache._ref, tp, ld, cols, kv_lens.data_ptr(), cu_q.data_ptr(), B, T, k.data_ptr(),
-                                  ldk, v.data_ptr(), ldv, qp, ldq, hq, op, ldo, cs, rows, rot,
-                                  1 if interleaved else 0, _stream_of(k))
+    rc = _lib.lib().w4a8_kv_write(cache._ref, tp, ld, cols, kv_lens.data_ptr(), cu_q.data_ptr(), B, T, kp, ldk, vp, ldv,
+                                  qp, ldq, hq, op, ldo, cs, rows, rot, 1 if interleaved else 0, _stream_of(k))
     if rc != 0:
         _lib.check(rc, "w4a8_kv_write")
     return out
@@ -211,8 +226,9 @@ def kv_read(cache: KVCache, page_table: torch.Tensor, kv_lens: torch.Tensor, cu_
     """The last ``cu_out[s + 1] - cu_out[s]`` cached tokens of each sequence (``tokens`` =
     cu_out's last value, known to the caller): k, v bf16 [tokens, kv_heads, head_dim]."""
     B, tp, ld, cols = _batch("kv_read", cache, page_table, kv_lens, cu_out)
-    _check(tokens >= 0, "kv_read: tokens must not be negative")
-    k = torch.empty((tokens, cache.kv_heads, cache.head_dim), dtype=torch.bfloat16, device=cache.device)
+    if tokens < 0:
+        raise RuntimeError("kv_read: tokens must not be negative")
+    k = torch.empty((tokens, cache.kv_heads, cache.head_dim), dtype=_BF16, device=cache.device)
     v = torch.empty_like(k)
     if tokens == 0:
         return k, v
@@ -235,34 +251,29 @@ def attention(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor, kv_lens
     cache's kv_heads; ``max_q_len`` is the longest cu_q[s + 1] - cu_q[s]; ``scale`` defaults to
     head_dim ** -0.5.  A row that sees no token is zero."""
     B, tp, ld, cols = _batch("attention", cache, page_table, kv_lens, cu_q)
-    q, ldq = _heads("attention", "q", q, cache)
-    T, hq, D = q.shape
-    if hq == 0 or hq % cache.kv_heads:
-        raise RuntimeError(f"attention: q heads must be a multiple of the cache's {cache.kv_heads}; got {hq}")
+    q, T, hq, ldq, qp = _heads("attention", "q", q, cache)
+    H, D = cache.kv_heads, cache.head_dim
+    if hq == 0 or hq % H:
+        raise RuntimeError(f"attention: q heads must be a multiple of the cache's {H}; got {hq}")
     if B > _lib.ATTENTION_MAX_BATCH:
         raise RuntimeError(f"attention: at most {_lib.ATTENTION_MAX_BATCH} sequences; got {B}")
-    _check(T == 0 or max_q_len > 0, "attention: max_q_len must be positive")
-    if out is None:
-        out = torch.empty((T, hq, D), dtype=torch.bfloat16, device=q.device)
-        ldo = hq * D
-    else:
-        _check(out.shape == q.shape, "attention: out must have q's shape")
-        dense, ldo = _heads("attention", "out", out, cache)
-        _check(dense is out, "attention: out's heads must be dense and its rows 16-byte aligned")
+    if max_q_len <= 0 and T > 0:
+        raise RuntimeError("attention: max_q_len must be positive")
+    out, ldo, op = _out_like("attention", "out", out, q, T, hq, cache)
     if T == 0:
         return out
-    _check(B > 0, "attention: tokens of no sequence")
+    if B == 0:
+        raise RuntimeError("attention: tokens of no sequence")
     L = _lib.lib()
-    key = (B, T, hq, cache.kv_heads, D, max_q_len)
+    key = (B, T, hq, H, D, max_q_len)
     need = _WS_BYTES.get(key)
     if need is None:
         if len(_WS_BYTES) > 4096:
             _WS_BYTES.clear()
         need = _WS_BYTES[key] = L.w4a8_attention_workspace_size(*key)
-    ws, wsb = workspace(need, q.device)
-    rc = L.w4a8_attention(cache._ref, tp, ld, cols, kv_lens.data_ptr(), cu_q.data_ptr(), B, T, q.data_ptr(), ldq, hq,
-                          max_q_len, D ** -0.5 if scale is None else scale, out.data_ptr(), ldo, ws, wsb,
-                          _stream_of(q))
+    ws, wsb = workspace(need, cache.device)
+    rc = L.w4a8_attention(cache._ref, tp, ld, cols, kv_lens.data_ptr(), cu_q.data_ptr(), B, T, qp, ldq, hq, max_q_len,
+                          D ** -0.5 if scale is None else scale, op, ldo, ws, wsb, _stream_of(q))
     if rc != 0:
         _lib.check(rc, "w4a8_attention")
     return out

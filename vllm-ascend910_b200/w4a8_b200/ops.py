@@ -391,44 +391,68 @@ def group_partials(x: torch.Tensor, w_packed: torch.Tensor, w_zero: Optional[tor
 
 # ---------------------------------------------------------------- residual addition + RMS norm
 
+_BF16 = torch.bfloat16
+
+
 def _norm_args(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor],
                residual_out: Optional[torch.Tensor], what: str):
-    """Checked (x2 [M, K], residual2, residual_out2, weight dtype code) of a norm call."""
-    if x.dtype != torch.bfloat16:
+    """Checked arguments of a norm call: x as [M, K] and its M, K, row stride; the weight's dtype code; the
+    residual's and its output's tensor, pointer and row stride (None, None, 0 without).  Few attribute
+    reads: a decode step makes many small calls."""
+    if x.dtype is not _BF16:
         raise RuntimeError(f"{what}: x must be bfloat16")
-    if not x.is_cuda or weight.device != x.device:
+    dev = x.device
+    if not x.is_cuda or weight.device != dev:
         raise RuntimeError(f"{what}: needs CUDA tensors on one device (there is no CPU implementation)")
-    K = x.shape[-1] if x.dim() else 0
-    _check(0 < K <= _lib.NORM_MAX_K, f"{what}: the last dimension must be 1..{_lib.NORM_MAX_K}")
-    if weight.dim() != 1 or weight.shape[0] != K or weight.stride(0) != 1:
+    shape = x.shape
+    K = shape[-1] if shape else 0
+    if not 0 < K <= _lib.NORM_MAX_K:
+        raise RuntimeError(f"{what}: the last dimension must be 1..{_lib.NORM_MAX_K}")
+    if weight.shape != (K,) or not weight.is_contiguous():
         raise RuntimeError(f"{what}: weight must be a dense [{K}]")
-    if weight.dtype == torch.bfloat16:
+    if weight.dtype is _BF16:
         wd = _lib.DTYPE_BF16
-    else:
-        _check(weight.dtype == torch.float32, f"{what}: weight must be bfloat16 or float32")
+    elif weight.dtype is torch.float32:
         wd = _lib.DTYPE_F32
-    x2 = x if x.dim() == 2 else x.reshape(-1, K)
-    if x2.stride(1) != 1:
-        x2 = x2.contiguous()
-    if residual is None:
-        _check(residual_out is None, f"{what}: residual_out without residual")
-        return x2, None, None, wd
-    if residual.dtype != torch.bfloat16 or residual.shape != x.shape or residual.device != x.device:
-        raise RuntimeError(f"{what}: residual must be bfloat16, of x's shape and on its device")
-    r2 = residual if residual.dim() == 2 else residual.reshape(-1, K)
-    if r2.stride(1) != 1:
-        r2 = r2.contiguous()
-    if residual_out is None:
-        ro = torch.empty(x2.shape, dtype=torch.bfloat16, device=x.device)
     else:
-        ro = residual_out
-        _check(ro.dtype == torch.bfloat16 and ro.shape == x.shape and ro.device == x.device,
-               f"{what}: residual_out must be bfloat16, of x's shape and on its device")
-        if ro.dim() != 2:
-            _check(ro.is_contiguous(), f"{what}: residual_out must be dense unless it is 2-D")
-            ro = ro.view(-1, K)
-        _check(ro.stride(1) == 1, f"{what}: residual_out's rows must be dense")
-    return x2, r2, ro, wd
+        raise RuntimeError(f"{what}: weight must be bfloat16 or float32")
+    x2, M, ldx = _rows(x, K)
+    if residual is None:
+        if residual_out is not None:
+            raise RuntimeError(f"{what}: residual_out without residual")
+        return x2, M, K, ldx, wd, None, None, 0, None, None, 0
+    if residual.dtype is not _BF16 or residual.shape != shape or residual.device != dev:
+        raise RuntimeError(f"{what}: residual must be bfloat16, of x's shape and on its device")
+    r2, _, ldr = _rows(residual, K)
+    if residual_out is None:
+        ro = torch.empty_like(x2) if x2.is_contiguous() else torch.empty((M, K), dtype=_BF16, device=dev)
+        ldro = K
+    else:
+        ro, ldro = _dense_rows(residual_out, shape, K, dev, what, "residual_out")
+    return x2, M, K, ldx, wd, r2, r2.data_ptr(), ldr, ro, ro.data_ptr(), ldro
+
+
+def _rows(t: torch.Tensor, K: int):
+    """t as rows of K dense elements (copied if they are not): tensor, number of rows, row stride."""
+    if t.dim() != 2:
+        t = t.reshape(-1, K)
+    if t.is_contiguous():
+        return t, t.shape[0], K
+    ld, step = t.stride()
+    if step != 1 and K > 1 or ld < K and t.shape[0] > 1:
+        t = t.contiguous()
+        ld = K
+    return t, t.shape[0], max(ld, K)
+
+
+def _dense_rows(t: torch.Tensor, shape, K: int, dev, what: str, name: str):
+    """A caller's output of the given shape with dense rows, as [M, K], and its row stride."""
+    if t.dtype is _BF16 and t.shape == shape and t.device == dev:
+        if t.is_contiguous():
+            return (t if t.dim() == 2 else t.view(-1, K)), K
+        if t.dim() == 2 and (t.stride(1) == 1 or K == 1) and (t.stride(0) >= K or t.shape[0] <= 1):
+            return t, max(t.stride(0), K)
+    raise RuntimeError(f"{what}: {name} must be bfloat16, of x's shape, on its device, with dense rows")
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: Optional[torch.Tensor] = None,
@@ -438,26 +462,20 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
     Without a residual returns y.  With one returns (y, bf16(h)), the latter
     into ``residual_out`` when given (it may be the residual itself).  fp32
     inside, each output rounded once."""
-    x2, r2, ro, wd = _norm_args(x, weight, residual, residual_out, "rms_norm")
-    M, K = x2.shape
+    x2, M, K, ldx, wd, r2, rp, ldr, ro, rop, ldro = _norm_args(x, weight, residual, residual_out, "rms_norm")
     if out is None:
-        y = torch.empty((M, K), dtype=torch.bfloat16, device=x.device)
+        y = torch.empty_like(x2) if ldx == K else torch.empty((M, K), dtype=_BF16, device=x.device)
+        ldy = K
     else:
-        _check(out.dtype == torch.bfloat16 and out.shape == x.shape and out.device == x.device and
-               (out.is_contiguous() or (out.dim() == 2 and out.stride(1) == 1)),
-               "rms_norm: out must be bfloat16, of x's shape, on its device, with dense rows")
-        y = out if out.dim() == 2 else out.view(-1, K)
-    rc = _lib.lib().w4a8_rms_norm(x2.data_ptr(), M, K, x2.stride(0), None if r2 is None else r2.data_ptr(),
-                                  0 if r2 is None else r2.stride(0), None if ro is None else ro.data_ptr(),
-                                  0 if ro is None else ro.stride(0), weight.data_ptr(), wd, eps, y.data_ptr(),
-                                  y.stride(0), _stream_of(x2))
+        y, ldy = _dense_rows(out, x.shape, K, x.device, "rms_norm", "out")
+    rc = _lib.lib().w4a8_rms_norm(x2.data_ptr(), M, K, ldx, rp, ldr, rop, ldro, weight.data_ptr(), wd, eps, y.data_ptr(),
+                                  ldy, _stream_of(x2))
     if rc != 0:
         _lib.check(rc, "w4a8_rms_norm")
     if x.dim() != 2:
         y = y.view(x.shape)
-    if r2 is None:
-        return y
-    return y, (ro if x.dim() == 2 else ro.view(x.shape))
+        ro = None if ro is None else ro.view(x.shape)
+    return y if r2 is None else (y, ro)
 
 
 def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, group_size: int, eps: float = 1e-6,
@@ -467,15 +485,12 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, group_size: int, eps: 
     x [M, K] -> (q int8 [M, K], scale [G, M], bf16(x + residual) or None)."""
     _check(x.dim() == 2, "rms_norm_quant: x must be [M, K]")
     _check(scale_dtype in (torch.float32, torch.bfloat16), "rms_norm_quant: scale dtype must be bf16 or f32")
-    x2, r2, ro, wd = _norm_args(x, weight, residual, residual_out, "rms_norm_quant")
-    M, K = x2.shape
+    x2, M, K, ldx, wd, r2, rp, ldr, ro, rop, ldro = _norm_args(x, weight, residual, residual_out, "rms_norm_quant")
     q = torch.empty((M, K), dtype=torch.int8, device=x.device)
     s = torch.empty((num_groups(K, max(group_size, 1)), M), dtype=scale_dtype, device=x.device)
-    rc = _lib.lib().w4a8_rms_norm_quant(x2.data_ptr(), M, K, x2.stride(0), None if r2 is None else r2.data_ptr(),
-                                        0 if r2 is None else r2.stride(0), None if ro is None else ro.data_ptr(),
-                                        0 if ro is None else ro.stride(0), weight.data_ptr(), wd, eps, group_size,
-                                        q.data_ptr(), s.data_ptr(),
-                                        _lib.DTYPE_F32 if scale_dtype == torch.float32 else _lib.DTYPE_BF16,
+    rc = _lib.lib().w4a8_rms_norm_quant(x2.data_ptr(), M, K, ldx, rp, ldr, rop, ldro, weight.data_ptr(), wd, eps,
+                                        group_size, q.data_ptr(), s.data_ptr(),
+                                        _lib.DTYPE_F32 if scale_dtype is torch.float32 else _lib.DTYPE_BF16,
                                         _stream_of(x2))
     if rc != 0:
         _lib.check(rc, "w4a8_rms_norm_quant")
@@ -487,28 +502,29 @@ def linear_prepared_rms_norm(x: torch.Tensor, weight: torch.Tensor, pw: Prepared
                              out: Optional[torch.Tensor] = None):
     """``linear_prepared`` on the norm of x (+ residual): the norm kernel quantises straight into the
     GEMM's operand tiles (``rms_norm_quant``'s codes).  Returns y, or (y, bf16(x + residual))."""
-    x2, r2, ro, wd = _norm_args(x, weight, residual, residual_out, "linear_prepared_rms_norm")
-    M, K = x2.shape
-    _check(x.device == pw.buf.device, "linear_prepared_rms_norm: x must be on the weights' device")
-    _check(K == pw.K, f"linear_prepared_rms_norm: x has last dimension {K}, weights were prepared for K={pw.K}")
+    what = "linear_prepared_rms_norm"
+    x2, M, K, ldx, wd, r2, rp, ldr, ro, rop, ldro = _norm_args(x, weight, residual, residual_out, what)
+    if x.device != pw.buf.device:
+        raise RuntimeError(f"{what}: x must be on the weights' device")
+    if K != pw.K:
+        raise RuntimeError(f"{what}: x has last dimension {K}, weights were prepared for K={pw.K}")
     N = pw.N
-    if out is not None:
-        _check(out.dtype == torch.bfloat16 and tuple(out.shape) == (M, N) and out.stride(1) == 1 and
-               out.device == x.device, f"linear_prepared_rms_norm: out must be bfloat16 [{M}, {N}] with dense rows")
-    y = out if out is not None else torch.empty((M, N), dtype=torch.bfloat16, device=x.device)
+    if out is None:
+        y, ldy = torch.empty((M, N), dtype=_BF16, device=x.device), N
+    else:
+        y, ldy = _dense_rows(out, (M, N), N, x.device, what, f"out [{M}, {N}]")
     if M > 0:
         ws, wsb = workspace(_ws_bytes(M, N, K, pw.group_size), x.device)
-        rc = _lib.lib().w4a8_linear_prepared_rms_norm(
-            x2.data_ptr(), M, K, x2.stride(0), None if r2 is None else r2.data_ptr(),
-            0 if r2 is None else r2.stride(0), None if ro is None else ro.data_ptr(),
-            0 if ro is None else ro.stride(0), weight.data_ptr(), wd, eps, N, pw.group_size, pw.ptr(), pw.ws_dtype,
-            1 if pw.has_zero else 0, y.data_ptr(), y.stride(0), ws, wsb, _stream_of(x2))
+        rc = _lib.lib().w4a8_linear_prepared_rms_norm(x2.data_ptr(), M, K, ldx, rp, ldr, rop, ldro, weight.data_ptr(), wd,
+                                                      eps, N, pw.group_size, pw.ptr(), pw.ws_dtype,
+                                                      1 if pw.has_zero else 0, y.data_ptr(), ldy, ws, wsb,
+                                                      _stream_of(x2))
         if rc != 0:
             _lib.check(rc, "w4a8_linear_prepared_rms_norm")
-    y = y if x.dim() == 2 else y.reshape(*x.shape[:-1], N)
-    if r2 is None:
-        return y
-    return y, (ro if x.dim() == 2 else ro.view(x.shape))
+    if x.dim() != 2:
+        y = y.view(*x.shape[:-1], N)
+        ro = None if ro is None else ro.view(x.shape)
+    return y if r2 is None else (y, ro)
 
 
 # ---------------------------------------------------------------- weight packing (device-agnostic torch)
