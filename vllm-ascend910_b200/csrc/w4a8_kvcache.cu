@@ -18,10 +18,16 @@
 // codes.)  A page of zeros has s' = 0 and codes 0; a non-finite value makes the
 // page's scale non-finite and the page reads back as NaN.
 //
-// The write is one launch: some blocks turn the query heads of a few tokens
-// each, the others each own one touched page (so no two blocks write one
-// scale), a warp per (kv head, K or V).  Bound by HBM for prompts: q is read and
-// written, k and v read, a byte per element written.
+// The write is one launch.  Some blocks turn query heads: a thread stays with
+// its token and its elements of a head, so it reads the table once for all the
+// heads it turns.  The other blocks own eight warps' worth of one touched page's
+// (kv head, K or V) items: a warp holds 4 rows of 128 elements in registers (a page
+// of 32 rows is eight warps), so k and v are read once -- rotated, their maximum found, and
+// written as codes.  All loads of a warp are in flight together; short chains of
+// dependent loads, not bandwidth, set the time until thousands of blocks run.  Dividing by the scale is a product with its reciprocal
+// except next to half-integers, where the true division decides (the activation
+// quantiser's rule).  Bound by HBM for prompts: q is read and written, k and v
+// read, a byte per element written.
 #include <algorithm>
 
 #include "w4a8_common.cuh"
@@ -32,7 +38,8 @@ namespace w4a8 {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kQTok = 4;           // tokens of one query block
+constexpr int kWarps = kThreads / 32;
+__host__ __device__ constexpr int chunk_rows(int D) { return 512 / D; }   // rows that a warp holds: 16 elements a lane
 
 __device__ __forceinline__ void rotate_pair(float& a, float& b, float c, float s)
 {
@@ -51,15 +58,20 @@ __device__ __forceinline__ void seq_bounds(const CacheView& c, int s, int64_t& t
     len = static_cast<int>(min(static_cast<int64_t>(max(c.kv_lens[s], 0)), static_cast<int64_t>(c.table_cols) << c.page_log2));
 }
 
-// The sequence that token t belongs to: the last s with cu[s] <= t (t >= cu[0]).
-__device__ __forceinline__ int seq_of(const int32_t* cu, int batch, int64_t t)
+// The sequence that token t belongs to: the last s with cu[s] <= t.  The whole
+// warp searches for its first token t0 (32 probes a step, so two dependent loads
+// for 1024 sequences), then each lane moves on to its own t >= t0.
+__device__ __forceinline__ int seq_of(const int32_t* cu, int batch, int64_t t0, int64_t t)
 {
-    int lo = 0, hi = batch - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (cu[mid] <= t) lo = mid;
-        else hi = mid - 1;
+    int lo = 0;
+    for (int n = batch; n > 1;) {
+        const int step = (n + 31) / 32, at = static_cast<int>(lane_id()) * step;
+        const unsigned hit = __ballot_sync(0xffffffffu, at < n && cu[lo + at] <= t0) | 1u;
+        const int k = (31 - __clz(hit)) * step;
+        lo += k;
+        n = min(step, n - k);
     }
+    while (lo + 1 < batch && cu[lo + 1] <= t) ++lo;
     return lo;
 }
 
@@ -77,14 +89,21 @@ __device__ __forceinline__ void item_cols(int j, int rot, int interleaved, int& 
     }
 }
 
-__device__ __forceinline__ void rotate_item(int j, int rot, int interleaved, const float* cs, float (&a)[8], float (&b)[8])
+// Cosines and sines of item j's 8 pairs, from a table row.
+__device__ __forceinline__ void load_angles(const float* row, int j, int rot, float4 (&cs)[4])
 {
-    if (j >= rot / 16) return;
-    const float4* cp = reinterpret_cast<const float4*>(cs + 8 * j);
-    const float4* sp = reinterpret_cast<const float4*>(cs + rot / 2 + 8 * j);
-    const float4 c0 = cp[0], c1 = cp[1], s0 = sp[0], s1 = sp[1];
-    const float c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-    const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+    const float4* cp = reinterpret_cast<const float4*>(row + 8 * j);
+    const float4* sp = reinterpret_cast<const float4*>(row + rot / 2 + 8 * j);
+    cs[0] = cp[0];
+    cs[1] = cp[1];
+    cs[2] = sp[0];
+    cs[3] = sp[1];
+}
+
+__device__ __forceinline__ void rotate_item(int interleaved, const float4 (&cs)[4], float (&a)[8], float (&b)[8])
+{
+    const float c[8] = {cs[0].x, cs[0].y, cs[0].z, cs[0].w, cs[1].x, cs[1].y, cs[1].z, cs[1].w};
+    const float s[8] = {cs[2].x, cs[2].y, cs[2].z, cs[2].w, cs[3].x, cs[3].y, cs[3].z, cs[3].w};
     if (!interleaved) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) rotate_pair(a[i], b[i], c[i], s[i]);
@@ -112,176 +131,256 @@ __device__ __forceinline__ int64_t clamp_row(int64_t pos, int64_t rows)
     return pos < 0 ? 0 : (pos >= rows ? rows - 1 : pos);
 }
 
-// One code: rint(x / s) within +-127; 0 for a zero or non-finite scale.
-__device__ __forceinline__ uint32_t code_of(float x, float s)
+// Codes of 4 values: rint(x / s) within +-127, a byte each.  y = x * (1 / s) is
+// within 2^-15 of x / s, so rint(y) is the code unless y is within 2^-14 of a
+// half-integer; there the IEEE division decides.  Adding 1.5 * 2^23 rounds y to
+// nearest even and leaves the code in the low byte.  |x| <= 127 s here, up to the
+// scale's own rounding, so nothing needs clamping.
+__device__ __forceinline__ uint32_t codes4(const float* x, float s, float rcp)
 {
-    const float q = fminf(fmaxf(rintf(__fdiv_rn(x, s)), -127.0f), 127.0f);
-    return s > 0.0f && s < INFINITY ? static_cast<uint32_t>(static_cast<int>(q)) & 0xFFu : 0u;
+    constexpr float kMagic = 12582912.0f;
+    uint32_t q[4];
+    bool tie = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float y = __fmul_rn(x[i], rcp), t = __fadd_rn(y, kMagic);
+        q[i] = __float_as_uint(t);
+        tie = tie || fabsf(__fsub_rn(y, __fsub_rn(t, kMagic))) > 0.49993896484375f;
+    }
+    if (tie) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[i] = __float_as_uint(__fadd_rn(__fdiv_rn(x[i], s), kMagic));
+    }
+    return __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
 }
 
-__device__ __forceinline__ uint2 codes8(const float (&v)[8], float s)
+// The same by the division alone, for scales whose reciprocal fp32 cannot hold;
+// 0 for a zero or non-finite scale.
+__device__ __forceinline__ uint32_t codes4_slow(const float* x, float s)
 {
-    uint2 w;
-    w.x = code_of(v[0], s) | (code_of(v[1], s) << 8) | (code_of(v[2], s) << 16) | (code_of(v[3], s) << 24);
-    w.y = code_of(v[4], s) | (code_of(v[5], s) << 8) | (code_of(v[6], s) << 16) | (code_of(v[7], s) << 24);
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float q = fminf(fmaxf(rintf(__fdiv_rn(x[i], s)), -127.0f), 127.0f);
+        if (s > 0.0f && s < INFINITY) w |= (static_cast<uint32_t>(static_cast<int>(q)) & 0xFFu) << (8 * i);
+    }
     return w;
 }
 
-__global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvWriteParams p, const int q_blocks)
+// Number of pages of sequence s that the call writes; 0 past the last sequence
+// (the loads do not wait for that test).
+__device__ __forceinline__ int touched_pages(const CacheView& cv, int s)
 {
-    __shared__ int64_t sh_pos[kQTok];
-    __shared__ int64_t sh_warp[kThreads / 32];
-    __shared__ int64_t sh_run;
-    __shared__ int sh_found, sh_local;
+    int64_t t0;
+    int n, len;
+    seq_bounds(cv, min(s, cv.batch - 1), t0, n, len);
+    const int lo = max(len - n, 0);          // tokens before position 0 are not written
+    return s < cv.batch && len > lo ? ((len - 1) >> cv.page_log2) - (lo >> cv.page_log2) + 1 : 0;
+}
 
+// The larger magnitude; a NaN of either wins.
+__device__ __forceinline__ float max_abs_nan(float m, float x)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(x)));
+    return r;
+}
+
+// Query heads of QT tokens.
+template <int D, int QT>
+__device__ __forceinline__ void rotate_queries(const KvWriteParams& p, int64_t t0)
+{
+    constexpr int LPH = D / 16;                          // threads of a head
     const CacheView& cv = p.c;
-    const int tid = threadIdx.x;
-    pdl_launch_dependents();
-    pdl_wait();
-
-    if (static_cast<int>(blockIdx.x) < q_blocks) {
-        // ---- query heads of kQTok tokens ----
-        const int64_t t0 = static_cast<int64_t>(blockIdx.x) * kQTok;
-        if (tid < kQTok && t0 + tid < cv.tokens) {
-            const int s = seq_of(cv.cu, cv.batch, t0 + tid);
+    const int j = threadIdx.x % LPH, slot = threadIdx.x / LPH;
+    const int64_t t = t0 + slot % QT;
+    const int s = p.rot ? seq_of(cv.cu, cv.batch, t0, min(t, cv.tokens - 1)) : 0;
+    if (t >= cv.tokens) return;
+    int c0, c1;
+    item_cols(j, p.rot, p.interleaved, c0, c1);
+    // the first heads' elements are on their way while the token's angles are found
+    constexpr int STEP = kThreads / LPH / QT, AHEAD = 4;
+    const uint16_t* src = p.q + t * p.ldq;
+    uint16_t* dst = p.q_out + t * p.ldqo;
+    const bool turn = j < p.rot / 16;
+    float4 cs[4] = {};
+    for (int h0 = slot / QT; h0 < p.q_heads; h0 += AHEAD * STEP) {
+        uint4 w[AHEAD][2];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            const int64_t h = min(h0 + k * STEP, p.q_heads - 1);
+            w[k][0] = *reinterpret_cast<const uint4*>(src + h * D + c0);
+            w[k][1] = *reinterpret_cast<const uint4*>(src + h * D + c1);
+        }
+        if (turn && h0 == slot / QT) {
             int64_t first;
             int n, len;
             seq_bounds(cv, s, first, n, len);
-            sh_pos[tid] = clamp_row(static_cast<int64_t>(len) - n + (t0 + tid - first), p.table_rows);
+            load_angles(p.cos_sin + clamp_row(static_cast<int64_t>(len) - n + (t - first), p.table_rows) * p.rot, j, p.rot, cs);
         }
-        __syncthreads();
-        const int per_head = cv.D / 16, per_tok = p.q_heads * per_head;
-        for (int i = tid; i < kQTok * per_tok; i += kThreads) {
-            const int k = i / per_tok, rest = i - k * per_tok;
-            const int64_t t = t0 + k;
-            if (t >= cv.tokens) break;
-            const int h = rest / per_head, j = rest - h * per_head;
-            int c0, c1;
-            item_cols(j, p.rot, p.interleaved, c0, c1);
-            const uint16_t* src = p.q + t * p.ldq + static_cast<int64_t>(h) * cv.D;
-            uint16_t* dst = p.q_out + t * p.ldqo + static_cast<int64_t>(h) * cv.D;
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            const int64_t h = h0 + k * STEP;
+            if (h >= p.q_heads) break;
             float a[8], b[8];
-            unpack8_bf16(*reinterpret_cast<const uint4*>(src + c0), a);
-            unpack8_bf16(*reinterpret_cast<const uint4*>(src + c1), b);
-            if (p.cos_sin) rotate_item(j, p.rot, p.interleaved, p.cos_sin + sh_pos[k] * p.rot, a, b);
-            *reinterpret_cast<uint4*>(dst + c0) = pack8(a);
-            *reinterpret_cast<uint4*>(dst + c1) = pack8(b);
+            unpack8_bf16(w[k][0], a);
+            unpack8_bf16(w[k][1], b);
+            if (turn) rotate_item(p.interleaved, cs, a, b);
+            *reinterpret_cast<uint4*>(dst + h * D + c0) = pack8(a);
+            *reinterpret_cast<uint4*>(dst + h * D + c1) = pack8(b);
         }
+    }
+}
+
+template <int D, int QT>
+__global__ void __launch_bounds__(kThreads, 4) kv_write_kernel(const KvWriteParams p, const int q_blocks, const int groups)
+{
+    __shared__ uint32_t sh_max[kWarps];
+
+    const CacheView& cv = p.c;
+    const int lane = lane_id(), warp = warp_id();
+    pdl_wait();
+
+    // Query blocks (bound by bandwidth) and page blocks (by latency) alternate in
+    // proportion, so that both kinds are resident together.
+    const int64_t qi = static_cast<int64_t>(blockIdx.x) * q_blocks / gridDim.x;
+    if ((static_cast<int64_t>(blockIdx.x) + 1) * q_blocks / gridDim.x > qi) {
+        rotate_queries<D, QT>(p, qi * QT);
         return;
     }
 
-    // ---- one touched page: find (sequence, page) number `job` ----
-    const int64_t job = blockIdx.x - q_blocks;
-    if (tid == 0) {
-        sh_run = 0;
-        sh_found = -1;
-    }
-    __syncthreads();
-    for (int base = 0; base < cv.batch; base += kThreads) {
-        const int s = base + tid;
-        int64_t np = 0;
-        if (s < cv.batch) {
-            int64_t t0;
-            int n, len;
-            seq_bounds(cv, s, t0, n, len);
-            const int lo = max(len - n, 0);          // tokens before position 0 are not written
-            if (len > lo) np = ((len - 1) >> cv.page_log2) - (lo >> cv.page_log2) + 1;
+    // ---- one touched page: every warp finds (sequence, page) number `job`, four
+    // sequences a lane ----
+    const uint32_t bid = blockIdx.x - static_cast<uint32_t>(qi);
+    const int64_t job = bid / static_cast<uint32_t>(groups);
+    const int group = static_cast<int>(bid - static_cast<uint32_t>(job) * groups);
+    int s = -1, local = 0;
+    int64_t run = 0;                                         // touched pages before the current 128 sequences
+    for (int base = 0; base < cv.batch && s < 0; base += 128) {
+        int np[4];
+        int64_t sum = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int q = base + lane * 4 + k;
+            np[k] = touched_pages(cv, q);
+            sum += np[k];
         }
-        int64_t x = np;
+        int64_t x = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-            if (static_cast<int>(lane_id()) >= o) x += y;
+            if (lane >= o) x += y;
         }
-        if (lane_id() == 31) sh_warp[warp_id()] = x;
-        __syncthreads();
-        int64_t before = sh_run;
-        for (int w = 0; w < static_cast<int>(warp_id()); ++w) before += sh_warp[w];
-        if (job >= before + x - np && job < before + x) {
-            sh_found = s;
-            sh_local = static_cast<int>(job - (before + x - np));
+        const unsigned hit = __ballot_sync(0xffffffffu, run + x > job);
+        if (hit) {
+            int64_t r = job - (run + x - sum);               // the page's number among the lane's sequences
+            int k = 0;
+            while (k < 3 && r >= np[k]) r -= np[k++];
+            const int w = __ffs(hit) - 1;
+            s = base + w * 4 + __shfl_sync(0xffffffffu, k, w);
+            local = __shfl_sync(0xffffffffu, static_cast<int>(r), w);
         }
-        __syncthreads();
-        if (tid == kThreads - 1) sh_run = before + x;
-        __syncthreads();
-        if (sh_found >= 0) break;
+        run += __shfl_sync(0xffffffffu, x, 31);
     }
-    if (sh_found < 0) return;
-    const int s = sh_found;
+    if (s < 0) return;
     int64_t t0;
     int n, len;
     seq_bounds(cv, s, t0, n, len);
     const int start = len - n;                               // position of the call's first token (may be < 0)
-    const int pg = (max(start, 0) >> cv.page_log2) + sh_local;
+    const int pg = (max(start, 0) >> cv.page_log2) + local;
     const int page_at = pg << cv.page_log2;
     const int lo = max(start - page_at, 0);                  // rows [0, lo): earlier tokens
-    const int hi = min(len - page_at, cv.page);              // rows [max(lo, -start), hi): this call's
-    const int first = max(lo, max(-page_at, 0));
+    const int hi = min(len - page_at, cv.page);              // rows [lo, hi): this call's
     const int id = cv.table[static_cast<int64_t>(s) * cv.ld_table + pg];
     if (id < 0 || id >= cv.pages) return;
 
-    const int per_row = cv.D / 16, rows = hi - first;
-    for (int it = warp_id(); it < 2 * cv.kv_heads; it += kThreads / 32) {
-        const int h = it >> 1;
-        const bool is_v = it & 1;
-        const int64_t ph = static_cast<int64_t>(id) * cv.kv_heads + h;
-        int8_t* codes = (is_v ? cv.v : cv.k) + (ph << cv.page_log2) * cv.D;
-        float* scale = (is_v ? cv.v_scale : cv.k_scale) + ph;
-        const int64_t ld = is_v ? p.ldv : p.ldk;
-        const uint16_t* src = (is_v ? p.v : p.k) + (t0 + (page_at + first - start)) * ld + static_cast<int64_t>(h) * cv.D;
-        const bool turn = !is_v && p.cos_sin != nullptr;
-        const int rot = is_v ? 0 : p.rot;
-
-        // this call's largest magnitude, as bits (a NaN wins)
-        uint32_t amax = 0;
-        for (int i = lane_id(); i < rows * per_row; i += 32) {
-            const int rw = i / per_row, j = i - rw * per_row;
-            int c0, c1;
-            item_cols(j, rot, p.interleaved, c0, c1);
-            float a[8], b[8];
-            unpack8_bf16(*reinterpret_cast<const uint4*>(src + rw * ld + c0), a);
-            unpack8_bf16(*reinterpret_cast<const uint4*>(src + rw * ld + c1), b);
-            if (turn)
-                rotate_item(j, rot, p.interleaved, p.cos_sin + clamp_row(page_at + first + rw, p.table_rows) * rot, a, b);
+    // This warp's item (kv head, K or V) and its chunks of the page's rows: chunk
+    // `part`, part + 8, ... where a page has more than eight.
+    constexpr int CHUNK = chunk_rows(D), LPR = D / 16, RPI = 32 / LPR;     // lanes of a row, rows at a time
+    static_assert(CHUNK == RPI, "a lane holds 16 elements of one row");
+    const int wpi = min(cv.page / CHUNK, kWarps), part = warp % wpi, sub = lane / LPR, j = lane % LPR;
+    const int item = group * (kWarps / wpi) + warp / wpi;
+    const bool on = item < 2 * cv.kv_heads;
+    const bool is_v = on && item >= cv.kv_heads;
+    const int h = !on ? 0 : is_v ? item - cv.kv_heads : item;
+    const int64_t ph = static_cast<int64_t>(id) * cv.kv_heads + h;
+    int8_t* codes = (is_v ? cv.v : cv.k) + (ph << cv.page_log2) * D;
+    float* scale = (is_v ? cv.v_scale : cv.k_scale) + ph;
+    const int64_t ld = is_v ? p.ldv : p.ldk;
+    const uint16_t* src = (is_v ? p.v : p.k) + (t0 - start + page_at) * ld + static_cast<int64_t>(h) * D;   // of row 0
+    const int rot = is_v ? 0 : p.rot;
+    int c0, c1;
+    item_cols(j, rot, p.interleaved, c0, c1);
+    float v[16];
+    auto load = [&](int chunk) {
+        const int row = chunk * CHUNK + sub;
+        const int64_t from = min(max(row, lo), hi - 1);                // a row that is there
+        const uint4 w0 = *reinterpret_cast<const uint4*>(src + from * ld + c0);
+        const uint4 w1 = *reinterpret_cast<const uint4*>(src + from * ld + c1);
+        float4 cs[4];
+        if (rot) load_angles(p.cos_sin + clamp_row(page_at + row, p.table_rows) * rot, min(j, rot / 16 - 1), rot, cs);
+        float a[8], b[8];
+        unpack8_bf16(w0, a);
+        unpack8_bf16(w1, b);
+        if (j < rot / 16) rotate_item(p.interleaved, cs, a, b);
+        const bool there = row >= lo && row < hi;
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                amax = max(amax, max(__float_as_uint(a[e]) & 0x7FFFFFFFu, __float_as_uint(b[e]) & 0x7FFFFFFFu));
+        for (int e = 0; e < 8; ++e) {
+            v[e] = there ? a[e] : 0.0f;
+            v[8 + e] = there ? b[e] : 0.0f;
         }
-        amax = __reduce_max_sync(0xffffffffu, amax);
-        const float mine = __fdiv_rn(__uint_as_float(amax), 127.0f);
-        const float was = lo > 0 ? *scale : 0.0f;
-        __syncwarp();
-        // the larger of the two; a NaN of either stays
-        const float now = was >= mine || was != was ? was : mine;
+    };
 
-        if (lo > 0 && now != was) {
-            const float ratio = __fdiv_rn(was, now);
-            for (int i = lane_id(); i < lo * cv.D / 4; i += 32) {
-                uint32_t w = reinterpret_cast<const uint32_t*>(codes)[i], o = 0;
+    // this call's largest magnitude
+    float big = 0.0f;
+    const int chunks = cv.page / CHUNK;
+    int held = part;
+    for (int c = part; c < chunks; c += wpi) {
+        load(c);
+        held = c;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float c = static_cast<float>(static_cast<int8_t>(w >> (8 * e)));
-                    const float q = rintf(__fmul_rn(c, ratio));
-                    o |= (static_cast<uint32_t>(static_cast<int>(q)) & 0xFFu) << (8 * e);
-                }
-                reinterpret_cast<uint32_t*>(codes)[i] = o;
-            }
-        }
-        for (int i = lane_id(); i < rows * per_row; i += 32) {
-            const int rw = i / per_row, j = i - rw * per_row;
-            int c0, c1;
-            item_cols(j, rot, p.interleaved, c0, c1);
-            float a[8], b[8];
-            unpack8_bf16(*reinterpret_cast<const uint4*>(src + rw * ld + c0), a);
-            unpack8_bf16(*reinterpret_cast<const uint4*>(src + rw * ld + c1), b);
-            if (turn)
-                rotate_item(j, rot, p.interleaved, p.cos_sin + clamp_row(page_at + first + rw, p.table_rows) * rot, a, b);
-            int8_t* d = codes + (first + rw) * cv.D;
-            *reinterpret_cast<uint2*>(d + c0) = codes8(a, now);
-            *reinterpret_cast<uint2*>(d + c1) = codes8(b, now);
-        }
-        if (lane_id() == 0) *scale = now;
+        for (int e = 0; e < 16; ++e) big = max_abs_nan(big, v[e]);
     }
+    uint32_t amax = __reduce_max_sync(0xffffffffu, __float_as_uint(big));   // (as bits, a NaN is the largest)
+    const float was = lo > 0 ? *scale : 0.0f;
+    if (wpi > 1) {
+        if (lane == 0) sh_max[warp] = amax;
+        __syncthreads();
+        for (int w = warp - part; w < warp - part + wpi; ++w) amax = max(amax, sh_max[w]);
+    }
+    if (!on) return;
+    const float mine = __fdiv_rn(__uint_as_float(amax), 127.0f);
+    // the larger of the two; a NaN of either stays
+    const float now = was >= mine || was != was ? was : mine;
+
+    if (lo > 0 && now != was) {
+        const float ratio = __fdiv_rn(was, now);
+        for (int i = part * 32 + lane; i < lo * D / 4; i += wpi * 32) {
+            uint32_t w = reinterpret_cast<const uint32_t*>(codes)[i], o = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float c = static_cast<float>(static_cast<int8_t>(w >> (8 * e)));
+                const float q = rintf(__fmul_rn(c, ratio));
+                o |= (static_cast<uint32_t>(static_cast<int>(q)) & 0xFFu) << (8 * e);
+            }
+            reinterpret_cast<uint32_t*>(codes)[i] = o;
+        }
+    }
+    const bool fast = now >= 1.1754943508222875e-38f && now < INFINITY;
+    const float rcp = fast ? __frcp_rn(now) : 0.0f;
+    for (int c = held; c >= 0; c -= wpi) {
+        if (c != held) load(c);
+        const int row = c * CHUNK + sub;
+        if (row < lo || row >= hi) continue;
+        int8_t* d = codes + row * D;
+        uint32_t w[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) w[q] = fast ? codes4(v + 4 * q, now, rcp) : codes4_slow(v + 4 * q, now);
+        *reinterpret_cast<uint2*>(d + c0) = make_uint2(w[0], w[1]);
+        *reinterpret_cast<uint2*>(d + c1) = make_uint2(w[2], w[3]);
+    }
+    __syncwarp();
+    if (lane == 0 && part == 0) *scale = now;
 }
 
 // ------------------------------------------------------------------ reading back
@@ -295,12 +394,11 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvReadParams p)
     __shared__ int64_t sh_ph[kRTok];       // page * kv_heads, or -1
     __shared__ int sh_row[kRTok];
     const CacheView& cv = p.c;
-    pdl_launch_dependents();
     pdl_wait();
     const int64_t t0 = static_cast<int64_t>(blockIdx.x) * kRTok;
     const int tid = threadIdx.x;
+    const int s = tid < 32 ? seq_of(cv.cu, cv.batch, t0, min(t0 + min(tid, kRTok - 1), cv.tokens - 1)) : 0;
     if (tid < kRTok && t0 + tid < cv.tokens) {
-        const int s = seq_of(cv.cu, cv.batch, t0 + tid);
         int64_t first;
         int n, len;
         seq_bounds(cv, s, first, n, len);
@@ -361,11 +459,23 @@ cudaError_t launch(Kern kern, int64_t blocks, cudaStream_t stream, const Args&..
 
 cudaError_t launch_kv_write(const KvWriteParams& p, cudaStream_t stream)
 {
-    const int64_t q_blocks = p.q ? (p.c.tokens + kQTok - 1) / kQTok : 0;
+    // One token a block while there are few (a decode step), four when blocks are
+    // plenty: B200, 8.2k tokens of 40 heads, four is faster than one.
+    const bool few = p.c.tokens <= 1024;
+    const int qt = few ? 1 : 4;
+    const int64_t q_blocks = p.q ? (p.c.tokens + qt - 1) / qt : 0;
     // n tokens of a sequence touch at most n pages, and at most (n - 1) / page + 2
-    const int64_t jobs = p.k ? std::min<int64_t>(p.c.tokens, p.c.tokens / p.c.page + 2 * static_cast<int64_t>(p.c.batch)) : 0;
-    if (q_blocks + jobs == 0) return cudaSuccess;
-    return launch(kv_write_kernel, q_blocks + jobs, stream, p, static_cast<int>(q_blocks));
+    const int64_t jobs = std::min<int64_t>(p.c.tokens, p.c.tokens / p.c.page + 2 * static_cast<int64_t>(p.c.batch));
+    const int per_block = kWarps / std::min(p.c.page / chunk_rows(p.c.D), kWarps);       // items
+    const int groups = (2 * p.c.kv_heads + per_block - 1) / per_block;
+    const int64_t blocks = q_blocks + jobs * groups;
+    if (blocks > 0x7FFFFFFF) return cudaErrorInvalidValue;
+    const int qb = static_cast<int>(q_blocks);
+    if (p.c.D == 128)
+        return few ? launch(kv_write_kernel<128, 1>, blocks, stream, p, qb, groups)
+                   : launch(kv_write_kernel<128, 4>, blocks, stream, p, qb, groups);
+    return few ? launch(kv_write_kernel<64, 1>, blocks, stream, p, qb, groups)
+               : launch(kv_write_kernel<64, 4>, blocks, stream, p, qb, groups);
 }
 
 cudaError_t launch_kv_read(const KvReadParams& p, cudaStream_t stream)
