@@ -390,6 +390,36 @@ __device__ __forceinline__ int quant_fast(float xv, float s, float rcp)
 
 __device__ __forceinline__ bool act_scale_fast(uint16_t sb) { return (sb & 0x7F80u) != 0; }
 
+// The larger magnitude; a NaN of either wins.
+__device__ __forceinline__ float max_abs_nan(float m, float x)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(x)));
+    return r;
+}
+
+// Codes of 4 fp32 values, a byte each: rint(x / s) for |x / s| < 127.5 and a normal
+// s.  y = x * (1 / s) is within 2^-15 of x / s, so rint(y) is the code unless y is
+// within 2^-14 of a half-integer; there the IEEE division decides.  Adding
+// 1.5 * 2^23 rounds y to nearest even and leaves the code in the low byte.
+__device__ __forceinline__ uint32_t codes4(const float* x, float s, float rcp)
+{
+    constexpr float kMagic = 12582912.0f;
+    uint32_t q[4];
+    bool tie = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float y = __fmul_rn(x[i], rcp), t = __fadd_rn(y, kMagic);
+        q[i] = __float_as_uint(t);
+        tie = tie || fabsf(__fsub_rn(y, __fsub_rn(t, kMagic))) > 0.49993896484375f;
+    }
+    if (tie) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[i] = __float_as_uint(__fadd_rn(__fdiv_rn(x[i], s), kMagic));
+    }
+    return __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+}
+
 // 8 codes k0..k7 -> two words in the GEMM's operand order: k0 k2 k4 k6 | k1 k3 k5 k7.
 __device__ __forceinline__ uint2 pack_operand_order(const int (&q)[8])
 {

@@ -131,31 +131,8 @@ __device__ __forceinline__ int64_t clamp_row(int64_t pos, int64_t rows)
     return pos < 0 ? 0 : (pos >= rows ? rows - 1 : pos);
 }
 
-// Codes of 4 values: rint(x / s) within +-127, a byte each.  y = x * (1 / s) is
-// within 2^-15 of x / s, so rint(y) is the code unless y is within 2^-14 of a
-// half-integer; there the IEEE division decides.  Adding 1.5 * 2^23 rounds y to
-// nearest even and leaves the code in the low byte.  |x| <= 127 s here, up to the
-// scale's own rounding, so nothing needs clamping.
-__device__ __forceinline__ uint32_t codes4(const float* x, float s, float rcp)
-{
-    constexpr float kMagic = 12582912.0f;
-    uint32_t q[4];
-    bool tie = false;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float y = __fmul_rn(x[i], rcp), t = __fadd_rn(y, kMagic);
-        q[i] = __float_as_uint(t);
-        tie = tie || fabsf(__fsub_rn(y, __fsub_rn(t, kMagic))) > 0.49993896484375f;
-    }
-    if (tie) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) q[i] = __float_as_uint(__fadd_rn(__fdiv_rn(x[i], s), kMagic));
-    }
-    return __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
-}
-
-// The same by the division alone, for scales whose reciprocal fp32 cannot hold;
-// 0 for a zero or non-finite scale.
+// codes4 by the division alone, within +-127, for scales whose reciprocal fp32
+// cannot hold; 0 for a zero or non-finite scale.
 __device__ __forceinline__ uint32_t codes4_slow(const float* x, float s)
 {
     uint32_t w = 0;
@@ -176,14 +153,6 @@ __device__ __forceinline__ int touched_pages(const CacheView& cv, int s)
     seq_bounds(cv, min(s, cv.batch - 1), t0, n, len);
     const int lo = max(len - n, 0);          // tokens before position 0 are not written
     return s < cv.batch && len > lo ? ((len - 1) >> cv.page_log2) - (lo >> cv.page_log2) + 1 : 0;
-}
-
-// The larger magnitude; a NaN of either wins.
-__device__ __forceinline__ float max_abs_nan(float m, float x)
-{
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(x)));
-    return r;
 }
 
 // Query heads of QT tokens.

@@ -12,12 +12,16 @@
 //   kNormTiles   the same codes and scales in the GEMM's operand order, straight
 //                into a linear call's workspace (QuantParams' kOutKernel form)
 //
-// One block holds one row in registers: a thread owns VPT vectors of 8
-// consecutive elements (16-byte loads), so x and r are read once and y, r' are
-// written once.  The sum of squares takes one warp reduction and one barrier;
-// the fp32 parts are added in a fixed order, so repeated calls give the same
-// bits.  A group's amax stays within GK / 8 neighbouring threads.  Bound by HBM
-// for many rows and by the launch and two dependent load latencies for few.
+// A block holds one row in registers: a thread owns VPT vectors of 8 consecutive
+// elements (16-byte loads), so x and r are read once and y, r' are written once.
+// Blocks stay for several rows when there are many: the weight is read once, and
+// the next row's loads are on their way while this one is reduced.  The sum of
+// squares takes one warp reduction and one barrier; the fp32 parts are added in a
+// fixed order, so repeated calls give the same bits.  A group's amax stays within
+// GK / 8 neighbouring threads.  Bound by HBM for many rows and by the launch and
+// one load latency for few.
+#include <algorithm>
+
 #include "w4a8_common.cuh"
 #include "w4a8_kernels.h"
 
@@ -26,15 +30,20 @@ namespace w4a8 {
 namespace {
 
 constexpr int kMaxNormThreads = 1024;
+constexpr int kManyRows = 296;             // rows past which a block takes two vectors a thread
+constexpr int kResident = 1024;            // threads per SM that the kernels' 64 registers allow
 
-__device__ __forceinline__ void load_row8(const uint16_t* row, int pos, int K, bool vec, float (&v)[8])
+// 8 bf16 elements from position pos of a row (zeros past K), as they are.
+__device__ __forceinline__ uint4 load_row8(const uint16_t* row, int pos, int K, bool vec)
 {
-    if (vec && pos + 8 <= K) {
-        unpack8_bf16(*reinterpret_cast<const uint4*>(row + pos), v);
-    } else {
+    if (vec && pos + 8 <= K) return *reinterpret_cast<const uint4*>(row + pos);
+    uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = pos + i < K ? bf16_bits_to_f32(row[pos + i]) : 0.0f;
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = pos + 2 * i < K ? row[pos + 2 * i] : 0u, hi = pos + 2 * i + 1 < K ? row[pos + 2 * i + 1] : 0u;
+        w[i] = lo | (hi << 16);
     }
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 __device__ __forceinline__ uint4 pack8_bf16(const float (&v)[8])
@@ -59,151 +68,182 @@ __device__ __forceinline__ void store_row8(uint16_t* row, int pos, int K, bool v
     }
 }
 
-template <int OUT, int VPT>
-__global__ void __launch_bounds__(kMaxNormThreads) rms_norm_kernel(const NormParams p)
+// The weight's 8 elements from position pos.
+__device__ __forceinline__ void load_weight8(const NormParams& p, int pos, float (&w)[8])
 {
-    __shared__ float red[kMaxNormThreads / 32];
-    __shared__ uint32_t red_max[VPT][kMaxNormThreads / 32];
+    if (p.weight_f32) {
+        const float* wf = static_cast<const float*>(p.weight);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = pos + i < p.K ? wf[pos + i] : 0.0f;
+    } else {
+        unpack8_bf16(load_row8(static_cast<const uint16_t*>(p.weight), pos, p.K, p.vec_w), w);
+    }
+}
 
-    pdl_launch_dependents();
-    const int row = blockIdx.x, tid = threadIdx.x, T = blockDim.x;
-    const bool real_row = OUT != kNormTiles || row < p.M;
+template <int OUT, int VPT>
+__global__ void __launch_bounds__(VPT == 2 ? 512 : kMaxNormThreads, VPT == 2 ? 2 : 1) rms_norm_kernel(const NormParams p)
+{
+    __shared__ float red[2][kMaxNormThreads / 32];
+    __shared__ uint32_t red_max[2][VPT][kMaxNormThreads / 32];
+
+    // the next kernel may come early where this one leaves room for it
+    if (gridDim.x <= 148) pdl_launch_dependents();
+    const int tid = threadIdx.x, T = blockDim.x, nw = T >> 5;
     pdl_wait();
 
-    float h[VPT][8];
-    float ss = 0.0f;
-#pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-        const int pos = (j * T + tid) * 8;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) h[j][i] = 0.0f;
-        if (real_row && pos < p.K) {
-            load_row8(p.x + static_cast<int64_t>(row) * p.ldx, pos, p.K, p.vec_x, h[j]);
-            if (p.res) {
-                float r[8];
-                load_row8(p.res + static_cast<int64_t>(row) * p.ldr, pos, p.K, p.vec_r, r);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) h[j][i] = __fadd_rn(h[j][i], r[i]);
-            }
-        }
-    }
-    // the weight's loads go out with the row's: they do not depend on the sum
-    float w[VPT][8];
-#pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-        const int pos = (j * T + tid) * 8;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[j][i] = 0.0f;
-        if (pos < p.K) {
-            if (p.weight_f32) {
-                const float* wf = static_cast<const float*>(p.weight);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) w[j][i] = pos + i < p.K ? wf[pos + i] : 0.0f;
-            } else {
-                load_row8(static_cast<const uint16_t*>(p.weight), pos, p.K, p.vec_w, w[j]);
-            }
-        }
-    }
-#pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(h[j][i], h[j][i], ss);
-        const int pos = (j * T + tid) * 8;
-        if (p.res_out && real_row && pos < p.K)
-            store_row8(p.res_out + static_cast<int64_t>(row) * p.ldro, pos, p.K, p.vec_ro, h[j]);
-    }
-
-    // ---- sum of squares over the block ----
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const int nw = T >> 5;
-    if (lane_id() == 0) red[warp_id()] = ss;
-    __syncthreads();
-    ss = static_cast<int>(lane_id()) < nw ? red[lane_id()] : 0.0f;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const float n = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(ss, static_cast<float>(p.K)) + p.eps));
-
-#pragma unroll
-    for (int j = 0; j < VPT; ++j)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) h[j][i] = __fmul_rn(__fmul_rn(h[j][i], n), w[j][i]);
-
-    if (OUT == kNormBf16) {
+    uint4 xn[VPT], rn[VPT];                        // a row's elements, loaded one row ahead
+    auto load = [&](int row) {
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             const int pos = (j * T + tid) * 8;
-            if (pos < p.K) store_row8(p.y + static_cast<int64_t>(row) * p.ldy, pos, p.K, p.vec_y, h[j]);
+            xn[j] = make_uint4(0, 0, 0, 0);
+            rn[j] = xn[j];
+            if (row < p.M && pos < p.K) {          // (the tile form has rows past M: zeros)
+                xn[j] = load_row8(p.x + static_cast<int64_t>(row) * p.ldx, pos, p.K, p.vec_x);
+                if (p.res) rn[j] = load_row8(p.res + static_cast<int64_t>(row) * p.ldr, pos, p.K, p.vec_r);
+            }
         }
-        return;
-    }
+    };
+    load(blockIdx.x);
+    constexpr bool kKeep = VPT <= 2;               // the weight stays in registers
+    float w[kKeep ? VPT : 1][8];
+    if (kKeep)
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) load_weight8(p, (j * T + tid) * 8, w[kKeep ? j : 0]);
 
-    // ---- group amax (as bits of |y|: a NaN wins over every number) ----
-    const int tpg = p.gk >> 3;
-    uint32_t amax[VPT];
-#pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-        uint32_t a = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) a = max(a, __float_as_uint(h[j][i]) & 0x7FFFFFFFu);
-        for (int o = (tpg < 32 ? tpg : 32) >> 1; o > 0; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
-        if (tpg > 32 && lane_id() == 0) red_max[j][warp_id()] = a;
-        amax[j] = a;
-    }
-    if (tpg > 32) {
-        __syncthreads();
-        const int w0 = (warp_id() / (tpg >> 5)) * (tpg >> 5);
+    int flip = 0;
+    for (int row = blockIdx.x; row < p.rows; row += gridDim.x, flip ^= 1) {
+        const bool real_row = OUT != kNormTiles || row < p.M;
+        float h[VPT][8];
+        float ss = 0.0f;
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
-            uint32_t a = 0;
-            for (int k = 0; k < (tpg >> 5); ++k) a = max(a, red_max[j][w0 + k]);
-            amax[j] = a;
+            float r[8];
+            unpack8_bf16(xn[j], h[j]);
+            unpack8_bf16(rn[j], r);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h[j][i] = __fadd_rn(h[j][i], r[i]);      // (without a residual, + 0)
         }
-    }
+        if (row + static_cast<int>(gridDim.x) < p.rows) load(row + gridDim.x);
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss = fmaf(h[j][i], h[j][i], ss);
+            const int pos = (j * T + tid) * 8;
+            if (p.res_out && real_row && pos < p.K)
+                store_row8(p.res_out + static_cast<int64_t>(row) * p.ldro, pos, p.K, p.vec_ro, h[j]);
+        }
+
+        // ---- sum of squares over the block; group maxima of |h w| on the way ----
+        // max|y| is max|h w| * n up to fp32 rounding, so the maxima need not wait for
+        // the sum.  The 2^40 keeps tiny products normal; large ones are out of range
+        // only where the sum of squares is too.
+        uint32_t amax[VPT];
+        const int tpg = p.gk >> 3;
+        if (OUT != kNormBf16) {
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) {
+                if (!kKeep) load_weight8(p, (j * T + tid) * 8, w[0]);
+                float a = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) a = max_abs_nan(a, (h[j][i] * 0x1p40f) * w[kKeep ? j : 0][i]);
+                amax[j] = __float_as_uint(a);          // (as bits, a NaN is the largest)
+            }
+            for (int o = (tpg < 32 ? tpg : 32) >> 1; o > 0; o >>= 1)
+#pragma unroll
+                for (int j = 0; j < VPT; ++j) amax[j] = max(amax[j], __shfl_xor_sync(0xffffffffu, amax[j], o));
+            if (tpg > 32 && lane_id() == 0)
+#pragma unroll
+                for (int j = 0; j < VPT; ++j) red_max[flip][j][warp_id()] = amax[j];
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (lane_id() == 0) red[flip][warp_id()] = ss;
+        __syncthreads();
+        ss = static_cast<int>(lane_id()) < nw ? red[flip][lane_id()] : 0.0f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float n = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(ss, static_cast<float>(p.K)) + p.eps));
 
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-        const int pos = (j * T + tid) * 8;
-        const int g = pos / p.gk;
-        const uint16_t sb = act_scale_bits(__uint_as_float(amax[j]));
-        const float s = bf16_bits_to_f32(sb);
-        int q[8];
-        if (act_scale_fast(sb)) {
-            const float rcp = __frcp_rn(s);
+        for (int j = 0; j < VPT; ++j) {
+            if (!kKeep) load_weight8(p, (j * T + tid) * 8, w[0]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) q[i] = quant_fast(h[j][i], s, rcp);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) q[i] = quant_exact(h[j][i], s);
+            for (int i = 0; i < 8; ++i) h[j][i] = __fmul_rn(__fmul_rn(h[j][i], n), w[kKeep ? j : 0][i]);
         }
-        const bool leader = pos % p.gk == 0;
-        if (OUT == kNormTiles) {
-            if (pos < p.kb_total * 256) {
-                *reinterpret_cast<uint2*>(p.aq + gemm_act_tile_offset(row, pos, p.tt, p.kb_total)) =
-                    pack_operand_order(q);
-                if (leader && g < p.G)
-                    p.as[(static_cast<int64_t>(row / p.tt) * p.G + g) * p.tt + row % p.tt] = real_row ? s : 0.0f;
-            }
-        } else if (pos < p.K) {
-            int8_t* qr = p.q + static_cast<int64_t>(row) * p.K;
-            if (pos + 8 <= p.K && p.vec_q) {
-                const uint32_t w0 = (q[0] & 0xFF) | ((q[1] & 0xFF) << 8) | ((q[2] & 0xFF) << 16) |
-                                    (static_cast<uint32_t>(q[3] & 0xFF) << 24);
-                const uint32_t w1 = (q[4] & 0xFF) | ((q[5] & 0xFF) << 8) | ((q[6] & 0xFF) << 16) |
-                                    (static_cast<uint32_t>(q[7] & 0xFF) << 24);
-                *reinterpret_cast<uint2*>(qr + pos) = make_uint2(w0, w1);
-            } else {
+
+        if (OUT == kNormBf16) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (pos + i < p.K) qr[pos + i] = static_cast<int8_t>(q[i]);
+            for (int j = 0; j < VPT; ++j) {
+                const int pos = (j * T + tid) * 8;
+                if (pos < p.K) store_row8(p.y + static_cast<int64_t>(row) * p.ldy, pos, p.K, p.vec_y, h[j]);
             }
-            if (leader) {
-                const int64_t o = static_cast<int64_t>(g) * p.M + row;
-                if (p.scale_f32) reinterpret_cast<float*>(p.scale)[o] = s;
-                else reinterpret_cast<uint16_t*>(p.scale)[o] = sb;
+            continue;
+        }
+
+        if (tpg > 32) {
+            const int w0 = (warp_id() / (tpg >> 5)) * (tpg >> 5);
+#pragma unroll
+            for (int j = 0; j < VPT; ++j)
+                for (int k = 0; k < (tpg >> 5); ++k) amax[j] = max(amax[j], red_max[flip][j][w0 + k]);
+        }
+        const float n40 = n * 0x1p-40f;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const int pos = (j * T + tid) * 8;
+            const int g = pos / p.gk;
+            const uint16_t sb = act_scale_bits(__uint_as_float(amax[j]) * n40);
+            const float s = bf16_bits_to_f32(sb);
+            uint2 q;                                   // 8 codes, a byte each
+            if (act_scale_fast(sb)) {
+                const float rcp = __frcp_rn(s);
+                q = make_uint2(codes4(h[j], s, rcp), codes4(h[j] + 4, s, rcp));
+            } else {
+                uint32_t b[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) b[i] = static_cast<uint32_t>(quant_exact(h[j][i], s)) & 0xFFu;
+                q = make_uint2(b[0] | (b[1] << 8) | (b[2] << 16) | (b[3] << 24), b[4] | (b[5] << 8) | (b[6] << 16) | (b[7] << 24));
+            }
+            const bool leader = pos % p.gk == 0;
+            if (OUT == kNormTiles) {
+                if (pos < p.kb_total * 256) {
+                    *reinterpret_cast<uint2*>(p.aq + gemm_act_tile_offset(row, pos, p.tt, p.kb_total)) =
+                        make_uint2(__byte_perm(q.x, q.y, 0x6420), __byte_perm(q.x, q.y, 0x7531));   // k0 k2 k4 k6 | k1 k3 k5 k7
+                    if (leader && g < p.G)
+                        p.as[(static_cast<int64_t>(row / p.tt) * p.G + g) * p.tt + row % p.tt] = real_row ? s : 0.0f;
+                }
+            } else if (pos < p.K) {
+                int8_t* qr = p.q + static_cast<int64_t>(row) * p.K;
+                if (pos + 8 <= p.K && p.vec_q) {
+                    *reinterpret_cast<uint2*>(qr + pos) = q;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (pos + i < p.K) qr[pos + i] = static_cast<int8_t>((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
+                }
+                if (leader) {
+                    const int64_t o = static_cast<int64_t>(g) * p.M + row;
+                    if (p.scale_f32) reinterpret_cast<float*>(p.scale)[o] = s;
+                    else reinterpret_cast<uint16_t*>(p.scale)[o] = sb;
+                }
             }
         }
     }
+}
+
+template <int OUT, int VPT>
+cudaError_t launch_vpt(const NormParams& p, int threads, cudaStream_t stream)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(std::min(p.rows, 148 * std::max(1, kResident / threads)));
+    cfg.blockDim = dim3(threads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, rms_norm_kernel<OUT, VPT>, p);
 }
 
 template <int OUT>
@@ -214,24 +254,15 @@ cudaError_t launch_out(const NormParams& p, cudaStream_t stream)
     const int nvec = (span + 7) / 8;
     // threads per row: a multiple of a warp, and of a 1024-element group's 128 threads
     const int unit = OUT != kNormBf16 && p.gk > 256 ? p.gk / 8 : 32;
-    int vpt = 1;
-    while (vpt < 4 && (nvec + vpt - 1) / vpt > kMaxNormThreads) vpt *= 2;
-    const int threads = ((nvec + vpt - 1) / vpt + unit - 1) / unit * unit;
-    if (threads > kMaxNormThreads) return cudaErrorInvalidValue;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.rows);
-    cfg.blockDim = dim3(threads);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    switch (vpt) {
-        case 1: return cudaLaunchKernelEx(&cfg, rms_norm_kernel<OUT, 1>, p);
-        case 2: return cudaLaunchKernelEx(&cfg, rms_norm_kernel<OUT, 2>, p);
-        default: return cudaLaunchKernelEx(&cfg, rms_norm_kernel<OUT, 4>, p);
-    }
+    const auto threads = [&](int vpt) { return ((nvec + vpt - 1) / vpt + unit - 1) / unit * unit; };
+    // One vector a thread is quickest for few rows; for many, two vectors keep more
+    // bytes in flight per register (kManyRows below).  Wide rows take what fits.
+    const bool one = threads(1) <= kMaxNormThreads;
+    if (one && (p.rows <= kManyRows || nvec < 64)) return launch_vpt<OUT, 1>(p, threads(1), stream);
+    if (threads(2) <= 512) return launch_vpt<OUT, 2>(p, threads(2), stream);
+    if (one) return launch_vpt<OUT, 1>(p, threads(1), stream);
+    if (threads(4) > kMaxNormThreads) return cudaErrorInvalidValue;
+    return launch_vpt<OUT, 4>(p, threads(4), stream);
 }
 
 }  // namespace
