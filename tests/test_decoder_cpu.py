@@ -113,6 +113,7 @@ def test_cache_argument_contract():
     assert write(B=0) == _lib.OK and write(T=0) == _lib.OK
     assert write(desc(d=80)) == uns and write(desc(page=8)) == uns and write(desc(heads=0)) == inv
     assert write(desc(k=None)) == inv and write(desc(k=A + 8)) == inv and write(desc(pages=-1)) == inv
+    assert write(desc(pages=0)) == inv
     assert write(B=-1) == inv and write(T=-1) == inv and write(ld=3) == inv and write(cols=1 << 30, ld=1 << 30) == inv
     assert write(table=None) == inv and write(kl=None) == inv and write(cu=7 * A + 2) == inv
     assert write(k=None) == inv and write(k=8 * A + 2) == inv and write(ldk=120) == inv and write(ldv=132) == inv

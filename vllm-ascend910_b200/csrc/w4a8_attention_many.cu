@@ -89,6 +89,13 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, where));
 }
 
+// Page scales of a block's four 16-token granules (-1: no page).
+struct __align__(16) BlockScales {
+    float k[4], v[4];
+    int odd;                 // a k scale is missing, zero, infinite or NaN
+    int pad[3];
+};
+
 struct Start {           // where the CTA's share begins: unit `unit` of a tile
     int seq, head, tile, unit;
     long long units;
@@ -273,7 +280,7 @@ __device__ __forceinline__ void put_codes(uint32_t stage, int tok, int c, const 
 }
 
 template <class C>
-__device__ __forceinline__ void converter_role(const AttentionParams& p, ManyBars* bars, uint32_t sm, float (*ring)[8],
+__device__ __forceinline__ void converter_role(const AttentionParams& p, ManyBars* bars, uint32_t sm, BlockScales* ring,
                                                const Start& st, int least, volatile int* abort_flag)
 {
     constexpr int N = C::UNITS_PER_THREAD, PER_ROW = C::D / 16;     // vectors of a token's row
@@ -298,42 +305,42 @@ __device__ __forceinline__ void converter_role(const AttentionParams& p, ManyBar
     Walk a;
     bool have_id = a.begin(p, st, least);
     int ab = a.b0;
+    const int pages = static_cast<int>(cv.pages);
     int id[N], sid = -1, head = 0, base = 0;
     uint4 kr[N], vr[N];
     float sc[2] = {-1.0f, -1.0f};
+    // Loads do not wait for tests: tokens past the length take the last token's page,
+    // and where there is no page codes come from page 0 (what they are does not
+    // matter: their scores are masked and their weights 0).
     auto load_ids = [&]() {
         const int32_t* row = cv.table + static_cast<int64_t>(a.seq) * cv.ld_table;
         head = a.head;
         base = ab * kBlk;
+        const int last = a.s.len - 1;
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            const int tok = base + tok0 + k * TSTEP;
-            id[k] = tok < a.s.len ? row[tok >> cv.page_log2] : -1;
+            id[k] = -1;
+            if (last >= 0) id[k] = row[min(base + tok0 + k * TSTEP, last) >> cv.page_log2];
         }
-        if (i < 4) sid = base + i * 16 < a.s.len ? row[(base + i * 16) >> cv.page_log2] : -1;
+        sid = -1;
+        if (base + (i & 3) * 16 <= last) sid = row[(base + (i & 3) * 16) >> cv.page_log2];
     };
     auto load_codes = [&]() {
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            kr[k] = make_uint4(0, 0, 0, 0);
-            vr[k] = kr[k];
-            if (id[k] >= 0 && id[k] < cv.pages) {
-                const int tok = base + tok0 + k * TSTEP;
-                const int64_t at = (((static_cast<int64_t>(id[k]) * cv.kv_heads + head) << cv.page_log2) +
-                                    (tok & (cv.page - 1))) * C::D + c * 16;
-                kr[k] = *reinterpret_cast<const uint4*>(cv.k + at);
-                vr[k] = *reinterpret_cast<const uint4*>(cv.v + at);
-            }
+            const int from = static_cast<unsigned>(id[k]) < static_cast<unsigned>(pages) ? id[k] : 0;
+            const int64_t at = (((static_cast<int64_t>(from) * cv.kv_heads + head) << cv.page_log2) +
+                                ((base + tok0 + k * TSTEP) & (cv.page - 1))) * C::D + c * 16;
+            kr[k] = *reinterpret_cast<const uint4*>(cv.k + at);
+            vr[k] = *reinterpret_cast<const uint4*>(cv.v + at);
         }
-        // page scales of the block's four 16-token granules, -1 where there is no page
-        if (i < 4) {
-            sc[0] = sc[1] = -1.0f;
-            if (sid >= 0 && sid < cv.pages) {
-                const int64_t ph = static_cast<int64_t>(sid) * cv.kv_heads + head;
-                sc[0] = cv.k_scale[ph];
-                sc[1] = cv.v_scale[ph];
-            }
-        }
+        // page scales of the block's four 16-token granules (lanes hold one each, four
+        // times over), -1 where there is no page
+        const bool there = static_cast<unsigned>(sid) < static_cast<unsigned>(pages);
+        const int64_t ph = there ? static_cast<int64_t>(sid) * cv.kv_heads + head : head;
+        sc[0] = cv.k_scale[ph];
+        sc[1] = cv.v_scale[ph];
+        if (!there) sc[0] = sc[1] = -1.0f;
     };
     auto step_ids = [&]() {
         if (++ab >= a.b1) {
@@ -353,9 +360,12 @@ __device__ __forceinline__ void converter_role(const AttentionParams& p, ManyBar
         const uint32_t ks = sm + C::OFF_K + sg * C::KV_STAGE, vs = sm + C::OFF_V + sg * C::KV_STAGE;
         if (!warp_wait(&bars->kempty[sg], ph ^ 1, abort_flag, p.status, kAConvK)) return;
         if (i < 4) {
-            ring[g % kScaleRing][i] = sc[0];
-            ring[g % kScaleRing][4 + i] = sc[1];
+            ring[g % kScaleRing].k[i] = sc[0];
+            ring[g % kScaleRing].v[i] = sc[1];
         }
+        // a block with a scale that is missing, zero, infinite or NaN takes the careful path
+        const bool odd = __any_sync(0xffffffffu, !(sc[0] >= 1e-30f && sc[0] < 1e30f));
+        if (i == 0) ring[g % kScaleRing].odd = odd;
 #pragma unroll
         for (int k = 0; k < N; ++k) put_codes<C>(ks, tok0 + k * TSTEP, c, kr[k]);
         fence_proxy_async_smem();
@@ -459,7 +469,7 @@ __device__ __forceinline__ void mma_role(const AttentionParams& p, ManyBars* bar
 
 template <class C>
 __device__ __forceinline__ void softmax_role(const AttentionParams& p, ManyBars* bars, uint32_t sm, uint32_t tbase,
-                                             float (*ring)[8], const Start& st, int least, volatile int* abort_flag)
+                                             BlockScales* ring, const Start& st, int least, volatile int* abort_flag)
 {
     const int x = warp_id() >> 2;                               // half
     const int row = threadIdx.x & 127;                          // row within it, and TMEM lane
@@ -546,39 +556,40 @@ __device__ __forceinline__ void softmax_role(const AttentionParams& p, ManyBars*
                 tc_wait_ld();
                 reg_fence32(s);
                 reg_fence32(s + 32);
-                const float* rg = ring[g % kScaleRing];
+                const BlockScales& rg = ring[g % kScaleRing];
+                const float4 rk = *reinterpret_cast<const float4*>(rg.k), rv = *reinterpret_cast<const float4*>(rg.v);
                 const int t0 = (a.b0 + j) * kBlk;
-                float f[4], wv[4];       // a granule's factors of scores and of weights
-                float vmax = 0.0f;
-                bool gone = false;       // (a scale below 0 marks tokens without a page; NaN scales pass on)
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    const float ks = rg[b], vs = rg[4 + b];
+                // a granule's factors of scores and of weights
+                float f[4] = {rk.x * qs, rk.y * qs, rk.z * qs, rk.w * qs}, wv[4] = {rv.x, rv.y, rv.z, rv.w};
+                if (rg.odd || t0 + kBlk - 1 > min_limit) {
                     // A granule that this row does not see at all takes factors that
                     // cannot touch it, whatever its scales are.  A zero factor would turn
                     // a masked score into NaN: the smallest one changes no visible score.
-                    const bool none = ks < 0.0f || t0 + 16 * b > limit;
-                    gone = gone || ks < 0.0f;
-                    f[b] = none ? 1.0f : fmaxf(ks * qs, 1e-37f);
-                    if (ks != ks) f[b] = none ? 1.0f : ks;
-                    wv[b] = none ? 0.0f : vs;
-                    vmax = fmaxf(vmax, wv[b]);
-                }
-                if (gone || t0 + kBlk - 1 > min_limit) {
+                    const float ks[4] = {rk.x, rk.y, rk.z, rk.w};
 #pragma unroll
-                    for (int i = 0; i < kBlk; ++i)
-                        if (t0 + i > limit || rg[i >> 4] < 0.0f) s[i] = 0xFF800000u;
+                    for (int b = 0; b < 4; ++b) {
+                        const bool none = ks[b] < 0.0f || t0 + 16 * b > limit;
+                        f[b] = none ? 1.0f : ks[b] != ks[b] ? ks[b] : fmaxf(f[b], 1e-37f);
+                        if (none) wv[b] = 0.0f;
+                        const int seen = none ? -1 : limit - t0 - 16 * b;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (i > seen) s[16 * b + i] = 0xFF800000u;
+                    }
                 }
+                const float vmax = fmaxf(fmaxf(wv[0], wv[1]), fmaxf(wv[2], wv[3]));
                 // ---- reference maximum ----
                 float mx = kNegInf;
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
-                    float r[4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        r[k] = fmaxf(fmaxf(__uint_as_float(s[16 * b + 4 * k]), __uint_as_float(s[16 * b + 4 * k + 1])),
-                                     fmaxf(__uint_as_float(s[16 * b + 4 * k + 2]), __uint_as_float(s[16 * b + 4 * k + 3])));
-                    mx = fmaxf(mx, fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3])) * f[b]);
+                    const auto x = [&](int i) { return __uint_as_float(s[16 * b + i]); };
+                    float r = fmaxf(fmaxf(x(0), x(1)), x(2)), q = fmaxf(fmaxf(x(3), x(4)), x(5));
+                    r = fmaxf(fmaxf(r, x(6)), x(7));
+                    q = fmaxf(fmaxf(q, x(8)), x(9));
+                    r = fmaxf(fmaxf(r, x(10)), x(11));
+                    q = fmaxf(fmaxf(q, x(12)), x(13));
+                    r = fmaxf(fmaxf(r, x(14)), x(15));
+                    mx = fmaxf(mx, fmaxf(r, q) * f[b]);
                 }
                 if (__any_sync(0xffffffffu, mx > m + kSlack || vmax > vr)) {
                     const float mn = fmaxf(m, mx + kMargin), vn = fmaxf(vr, pow2_above(vmax));
@@ -701,7 +712,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Atte
 {
     extern __shared__ uint8_t smem_raw[];
     __shared__ ManyBars bars_;
-    __shared__ float ring[kScaleRing][8];
+    __shared__ BlockScales ring[kScaleRing];
     __shared__ Start start;
     ManyBars* bars = &bars_;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
