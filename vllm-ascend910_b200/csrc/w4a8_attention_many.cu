@@ -15,10 +15,15 @@
 //                    their rows' queries to fp16 in smem, and the output rows
 //   warps 8-11       converters: cache codes by 16-byte loads (one block ahead in
 //                    registers), exact fp16 into the swizzled operand layout
-//   warp 12          issues every MMA (warps 13-15 fill its warpgroup)
-// Scores are double buffered (TMEM: 2 x 2 x 64 columns of S, P over its S, 2 x D
-// of O), so Q K^T of block j + 1 runs while the softmax of block j works, and
-// the tensor core, the exponential unit and the converters overlap.
+//   warps 12, 13     issue the MMAs of half A, B (warps 14, 15 fill the warpgroup)
+// One issuer for both halves was measured first: its chain of waits and commits
+// (about 100 cycles each) set the pace at 1,900 cycles a block with all other work
+// taken out.
+// TMEM holds S of each half (64 columns), two P of each half (32 columns) and O (D
+// columns).  S is free as soon as the softmax has it in registers, so Q K^T of block
+// j + 1 runs while the softmax of block j works; P of a block is kept until its PV
+// has read it, two blocks deep.  Neither product waits for the other (P over S in
+// two buffers, measured first, made every Q K^T wait for a PV just issued).
 //
 // The reference maximum of a row moves only when a block exceeds it by more than
 // 2^1.9 (weights stay below 2^15.9, inside fp16), and then to 2^2 above what was
@@ -53,7 +58,7 @@ constexpr int kMinUnits = 4;               // a CTA's share is not cut below thi
 constexpr float kMargin = 2.0f;            // log2 by which a new reference exceeds the scores seen
 
 // wait-site ids for the status word
-enum { kAMmaK = 0x41, kAMmaV, kAMmaQ, kAMmaO, kAMmaP, kAMmaS, kASoftS, kASoftPv, kASoftEnd, kAConvK, kAConvV, kADrain };
+enum { kAMmaK = 0x41, kAMmaV, kAMmaQ, kAMmaO, kAMmaP, kAMmaS, kASoftS, kASoftPv, kASoftP, kASoftEnd, kAConvK, kAConvV, kADrain };
 
 template <int D_>
 struct ManyCfg {
@@ -66,19 +71,20 @@ struct ManyCfg {
     static constexpr int OFF_K = 2 * Q_HALF;
     static constexpr int OFF_V = OFF_K + kNS * KV_STAGE;
     static constexpr int OFF_PREFIX = OFF_V + kNS * KV_STAGE;
-    static constexpr int TM_S = 0;                           // [half][buffer] of 64 columns
+    static constexpr int TM_S = 0;                           // [half] of 64 columns
+    static constexpr int TM_P = 128;                         // [half][buffer] of 32 columns
     static constexpr int TM_O = 256;                         // [half] of D columns
     static constexpr int TM_COLS = 512;
     static constexpr int PIECE = kRows * D_ * 4;
     static constexpr int UNITS_PER_THREAD = kBlk * D_ / 16 / 128;   // 16-byte code vectors a converter thread moves
 };
 
-// S, P and PV phases have a barrier for each of the two buffers: every wait is
-// for a phase whose predecessor on the same barrier (two blocks back) is known to
-// be complete and whose successor cannot have completed, so parity tells.
+// P and PV phases have a barrier for each of the two buffers: every wait is for a
+// phase whose predecessor on the same barrier (two blocks back) is known to be
+// complete and whose successor cannot have completed, so parity tells.
 struct ManyBars {
     uint64_t kfull[kNS], kempty[kNS], vfull[kNS], vempty[kNS];
-    uint64_t sfull[2][2], pready[2][2], pvdone[2][2], qfull[2], ofree[2], drain;
+    uint64_t sfull[2], sfree[2], pready[2][2], pvdone[2][2], qfull[2], ofree[2], drain[2];
     uint32_t tmem_base;
     int abort;
 };
@@ -387,82 +393,77 @@ __device__ __forceinline__ void converter_role(const AttentionParams& p, ManyBar
 
 // ------------------------------------------------------------------ MMA issuer
 
+// Half x.  Stages are handed back when both halves' issuers are done with them; in
+// a piece without half B its issuer follows along and hands them back at once.
 template <class C>
-__device__ __forceinline__ void mma_role(const AttentionParams& p, ManyBars* bars, uint32_t sm, uint32_t tbase,
+__device__ __forceinline__ void mma_role(const AttentionParams& p, ManyBars* bars, uint32_t sm, uint32_t tbase, const int x,
                                          const Start& st, int least, volatile int* abort_flag)
 {
     constexpr uint32_t idqk = idesc_f16(128, kBlk, false), idpv = idesc_f16(128, C::D, true);
-    const uint64_t q_desc = smem_desc_sw128(sm), k_desc = smem_desc_sw128(sm + C::OFF_K);
+    // Descriptors count 16-byte units.
+    const uint64_t q_desc = smem_desc_sw128(sm + x * C::Q_HALF), k_desc = smem_desc_sw128(sm + C::OFF_K);
     const uint64_t v_desc = smem_desc_mn(sm + C::OFF_V, C::KV_CHUNK);
+    const uint32_t t_s = tbase + C::TM_S + x * kBlk, t_p = tbase + C::TM_P + x * kBlk, t_o = tbase + C::TM_O + x * C::D;
     Walk a;
     bool more = a.begin(p, st, least), ok = true;
-    uint32_t g = 0;                 // blocks issued (K, V stages)
-    uint32_t na = 0, nb = 0;        // blocks issued of each half
-    uint32_t sa = 0, sb = 0;        // pieces of each half
+    uint32_t g = 0;                 // blocks of the CTA (K, V stages)
+    uint32_t n = 0, piece = 0;      // blocks and pieces of the half
     auto wait = [&](uint64_t* b, uint32_t parity, int where) {
         ok = ok && mbar_wait(b, parity, abort_flag, p.status, where);
         return ok;
     };
-    // Descriptors count 16-byte units.
-    auto qk = [&](int x, uint32_t n, uint32_t sg) {
-        // the S buffer is free once the PV that read its P, two blocks back, is done
-        if (n >= 2 && !wait(&bars->pvdone[x][n & 1], ((n - 2) >> 1) & 1, kAMmaS)) return;
-        tc_fence_after();
-        const uint32_t d = tbase + C::TM_S + (x * 2 + (n & 1)) * kBlk;
-        const uint64_t qd = q_desc + x * (C::Q_HALF / 16), kd = k_desc + sg * (C::KV_STAGE / 16);
-#pragma unroll
-        for (int k = 0; k < C::D / 16; ++k)
-            mma_ss(d, qd + ((k >> 2) * C::Q_CHUNK + (k & 3) * 32) / 16, kd + ((k >> 2) * C::KV_CHUNK + (k & 3) * 32) / 16,
-                   idqk, k == 0 ? 0u : 1u);
-        tc_commit(&bars->sfull[x][n & 1]);
-    };
-    // PV of the half's block n (stage sg); the piece's first overwrites O, whose
-    // previous output must then have been read.
-    auto pv = [&](int x, uint32_t n, uint32_t sg, bool first, uint32_t piece) {
-        if (first && piece > 0 && !wait(&bars->ofree[x], (piece - 1) & 1, kAMmaO)) return;
-        if (!wait(&bars->pready[x][n & 1], (n >> 1) & 1, kAMmaP)) return;
-        tc_fence_after();
-        const uint32_t d = tbase + C::TM_O + x * C::D, ap = tbase + C::TM_S + (x * 2 + (n & 1)) * kBlk;
-        const uint64_t vd = v_desc + sg * (C::KV_STAGE / 16);
-#pragma unroll
-        for (int k = 0; k < kBlk / 16; ++k) mma_ts(d, ap + k * 8, vd + k * 128, idpv, first && k == 0 ? 0u : 1u);
-        tc_commit(&bars->pvdone[x][n & 1]);
-    };
     while (more && ok) {
-        const bool two = a.has_b(p.group);
-        if (!wait(&bars->qfull[0], sa & 1, kAMmaQ)) break;
-        if (two && !wait(&bars->qfull[1], sb & 1, kAMmaQ)) break;
         const int steps = a.b1 - a.b0;
-        for (int j = 0; j <= steps && ok; ++j) {
+        if (x == 1 && !a.has_b(p.group)) {
+            for (int j = 0; j < steps && ok; ++j, ++g) {
+                const uint32_t sg = g % kNS, ph = (g / kNS) & 1;
+                if (!wait(&bars->kfull[sg], ph, kAMmaK)) break;
+                mbar_arrive(&bars->kempty[sg]);
+                if (!wait(&bars->vfull[sg], ph, kAMmaV)) break;
+                mbar_arrive(&bars->vempty[sg]);
+            }
+            if (ok) more = a.next(p, least);
+            continue;
+        }
+        if (!wait(&bars->qfull[x], piece & 1, kAMmaQ)) break;
+        for (int j = 0; j <= steps; ++j) {
             if (j < steps) {
-                const uint32_t sg = (g + j) % kNS;
+                const uint32_t sg = (g + j) % kNS, b = n + j;
                 if (!wait(&bars->kfull[sg], ((g + j) / kNS) & 1, kAMmaK)) break;
-                qk(0, na + j, sg);
-                if (two && ok) qk(1, nb + j, sg);
-                if (!ok) break;
+                if (b >= 1 && !wait(&bars->sfree[x], (b - 1) & 1, kAMmaS)) break;     // the scores before have been read
+                tc_fence_after();
+                const uint64_t kd = k_desc + sg * (C::KV_STAGE / 16);
+#pragma unroll
+                for (int k = 0; k < C::D / 16; ++k)
+                    mma_ss(t_s, q_desc + ((k >> 2) * C::Q_CHUNK + (k & 3) * 32) / 16,
+                           kd + ((k >> 2) * C::KV_CHUNK + (k & 3) * 32) / 16, idqk, k == 0 ? 0u : 1u);
+                tc_commit(&bars->sfull[x]);
                 tc_commit(&bars->kempty[sg]);
             }
             if (j > 0) {
-                const uint32_t sg = (g + j - 1) % kNS;
+                const uint32_t sg = (g + j - 1) % kNS, b = n + j - 1;
                 if (!wait(&bars->vfull[sg], ((g + j - 1) / kNS) & 1, kAMmaV)) break;
-                pv(0, na + j - 1, sg, j == 1, sa);
-                if (two && ok) pv(1, nb + j - 1, sg, j == 1, sb);
-                if (!ok) break;
+                // the piece's first PV overwrites O, whose previous output must have been read
+                if (j == 1 && piece > 0 && !wait(&bars->ofree[x], (piece - 1) & 1, kAMmaO)) break;
+                if (!wait(&bars->pready[x][b & 1], (b >> 1) & 1, kAMmaP)) break;
+                tc_fence_after();
+                const uint32_t ap = t_p + (b & 1) * (kBlk / 2);
+                const uint64_t vd = v_desc + sg * (C::KV_STAGE / 16);
+#pragma unroll
+                for (int k = 0; k < kBlk / 16; ++k) mma_ts(t_o, ap + k * 8, vd + k * 128, idpv, j == 1 && k == 0 ? 0u : 1u);
+                tc_commit(&bars->pvdone[x][b & 1]);
                 tc_commit(&bars->vempty[sg]);
             }
         }
+        if (!ok) break;
         g += steps;
-        na += steps;
-        ++sa;
-        if (two) {
-            nb += steps;
-            ++sb;
-        }
-        if (ok) more = a.next(p, least);
+        n += steps;
+        ++piece;
+        more = a.next(p, least);
     }
     // nothing of this thread's is in flight when TMEM is freed
-    tc_commit(&bars->drain);
-    mbar_wait(&bars->drain, 0, abort_flag, p.status, kADrain);
+    tc_commit(&bars->drain[x]);
+    mbar_wait(&bars->drain[x], 0, abort_flag, p.status, kADrain);
 }
 
 // ------------------------------------------------------------------ softmax
@@ -546,16 +547,21 @@ __device__ __forceinline__ void softmax_role(const AttentionParams& p, ManyBars*
 
         float m = kNegInf, l = 0.0f, vr = kVrMin, vr_inv = kWeightOne / kVrMin;
         for (int j = 0; j < steps; ++j, ++g, ++n) {
-            if (!warp_wait(&bars->sfull[x][n & 1], (n >> 1) & 1, abort_flag, p.status, kASoftS)) return;
+            uint32_t s[kBlk];
+            if (!warp_wait(&bars->sfull[x], n & 1, abort_flag, p.status, kASoftS)) return;
             if (live) {
                 tc_fence_after();
-                const uint32_t t_s = tbase + lane_off + C::TM_S + (x * 2 + (n & 1)) * kBlk;
-                uint32_t s[kBlk];
+                const uint32_t t_s = tbase + lane_off + C::TM_S + x * kBlk;
                 tm_ld32(t_s, s);
                 tm_ld32(t_s + 32, s + 32);
                 tc_wait_ld();
                 reg_fence32(s);
                 reg_fence32(s + 32);
+                tc_fence_before();
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->sfree[x]);
+            if (live) {
                 const BlockScales& rg = ring[g % kScaleRing];
                 const float4 rk = *reinterpret_cast<const float4*>(rg.k), rv = *reinterpret_cast<const float4*>(rg.v);
                 const int t0 = (a.b0 + j) * kBlk;
@@ -640,7 +646,10 @@ __device__ __forceinline__ void softmax_role(const AttentionParams& p, ManyBars*
                 float lo, hi;
                 unpair2(sum, lo, hi);
                 l += lo + hi;
-                tm_st32(t_s, pk);
+                // this P buffer is free once the PV two blocks back has read it
+                if (n >= 2 && !warp_wait(&bars->pvdone[x][n & 1], ((n - 2) >> 1) & 1, abort_flag, p.status, kASoftP)) return;
+                tc_fence_after();
+                tm_st32(tbase + lane_off + C::TM_P + (x * 2 + (n & 1)) * (kBlk / 2), pk);
                 tc_wait_st();
                 tc_fence_before();
             }
@@ -723,20 +732,21 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Atte
     if (threadIdx.x == 0) {
         for (int i = 0; i < kNS; ++i) {
             mbar_init(&bars->kfull[i], 4);
-            mbar_init(&bars->kempty[i], 1);
+            mbar_init(&bars->kempty[i], 2);
             mbar_init(&bars->vfull[i], 4);
-            mbar_init(&bars->vempty[i], 1);
+            mbar_init(&bars->vempty[i], 2);
         }
         for (int x = 0; x < 2; ++x) {
             for (int b = 0; b < 2; ++b) {
-                mbar_init(&bars->sfull[x][b], 1);
                 mbar_init(&bars->pready[x][b], 4);
                 mbar_init(&bars->pvdone[x][b], 1);
             }
+            mbar_init(&bars->sfull[x], 1);
+            mbar_init(&bars->sfree[x], 4);
             mbar_init(&bars->qfull[x], 4);
             mbar_init(&bars->ofree[x], 4);
+            mbar_init(&bars->drain[x], 1);
         }
-        mbar_init(&bars->drain, 1);
         bars->abort = 0;
         fence_mbar_init();
     }
@@ -827,7 +837,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Atte
         converter_role<C>(p, bars, sm, ring, st, least, abort_flag);
     } else {
         regs_dec<kRegsMma>();
-        if (warp == kMmaWarp && elect_one()) mma_role<C>(p, bars, sm, tbase, st, least, abort_flag);
+        if (warp < kMmaWarp + 2 && elect_one()) mma_role<C>(p, bars, sm, tbase, warp - kMmaWarp, st, least, abort_flag);
     }
     pdl_launch_dependents();
     __syncwarp();
