@@ -236,6 +236,15 @@ __device__ __forceinline__ void reg_fence32(uint32_t* r)
     for (int i = 0; i < 32; i += 4) reg_fence4(r + i);
 }
 
+// The largest of three scores (one instruction).
+__device__ __forceinline__ float max3(float a, uint32_t b, uint32_t c)
+{
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
+    return r;
+}
+__device__ __forceinline__ float max3(uint32_t a, uint32_t b, uint32_t c) { return max3(__uint_as_float(a), b, c); }
+
 __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b)
 {
     uint64_t d;
@@ -547,112 +556,114 @@ __device__ __forceinline__ void softmax_role(const AttentionParams& p, ManyBars*
 
         float m = kNegInf, l = 0.0f, vr = kVrMin, vr_inv = kWeightOne / kVrMin;
         for (int j = 0; j < steps; ++j, ++g, ++n) {
-            uint32_t s[kBlk];
             if (!warp_wait(&bars->sfull[x], n & 1, abort_flag, p.status, kASoftS)) return;
-            if (live) {
-                tc_fence_after();
-                const uint32_t t_s = tbase + lane_off + C::TM_S + x * kBlk;
-                tm_ld32(t_s, s);
-                tm_ld32(t_s + 32, s + 32);
-                tc_wait_ld();
-                reg_fence32(s);
-                reg_fence32(s + 32);
-                tc_fence_before();
+            if (!live) {                             // (no row of this warp's: it only keeps step)
+                if (lane == 0) {
+                    mbar_arrive(&bars->sfree[x]);
+                    mbar_arrive(&bars->pready[x][n & 1]);
+                }
+                continue;
             }
+            tc_fence_after();
+            uint32_t s[kBlk];
+            tm_ld32(tbase + lane_off + C::TM_S + x * kBlk, s);
+            tm_ld32(tbase + lane_off + C::TM_S + x * kBlk + 32, s + 32);
+            tc_wait_ld();
+            reg_fence32(s);
+            reg_fence32(s + 32);
+            tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars->sfree[x]);
-            if (live) {
-                const BlockScales& rg = ring[g % kScaleRing];
-                const float4 rk = *reinterpret_cast<const float4*>(rg.k), rv = *reinterpret_cast<const float4*>(rg.v);
-                const int t0 = (a.b0 + j) * kBlk;
-                // a granule's factors of scores and of weights
-                float f[4] = {rk.x * qs, rk.y * qs, rk.z * qs, rk.w * qs}, wv[4] = {rv.x, rv.y, rv.z, rv.w};
-                if (rg.odd || t0 + kBlk - 1 > min_limit) {
-                    // A granule that this row does not see at all takes factors that
-                    // cannot touch it, whatever its scales are.  A zero factor would turn
-                    // a masked score into NaN: the smallest one changes no visible score.
-                    const float ks[4] = {rk.x, rk.y, rk.z, rk.w};
-#pragma unroll
-                    for (int b = 0; b < 4; ++b) {
-                        const bool none = ks[b] < 0.0f || t0 + 16 * b > limit;
-                        f[b] = none ? 1.0f : ks[b] != ks[b] ? ks[b] : fmaxf(f[b], 1e-37f);
-                        if (none) wv[b] = 0.0f;
-                        const int seen = none ? -1 : limit - t0 - 16 * b;
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (i > seen) s[16 * b + i] = 0xFF800000u;
-                    }
-                }
-                const float vmax = fmaxf(fmaxf(wv[0], wv[1]), fmaxf(wv[2], wv[3]));
-                // ---- reference maximum ----
-                float mx = kNegInf;
+            const BlockScales& rg = ring[g % kScaleRing];
+            const float4 rk = *reinterpret_cast<const float4*>(rg.k), rv = *reinterpret_cast<const float4*>(rg.v);
+            const int t0 = (a.b0 + j) * kBlk;
+            // a granule's factors of scores and of weights
+            float f[4] = {rk.x * qs, rk.y * qs, rk.z * qs, rk.w * qs}, wv[4] = {rv.x, rv.y, rv.z, rv.w};
+            if (rg.odd || t0 + kBlk - 1 > min_limit) {
+                // A granule that this row does not see at all takes factors that
+                // cannot touch it, whatever its scales are.  A zero factor would turn
+                // a masked score into NaN: the smallest one changes no visible score.
+                const float ks[4] = {rk.x, rk.y, rk.z, rk.w};
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
-                    const auto x = [&](int i) { return __uint_as_float(s[16 * b + i]); };
-                    float r = fmaxf(fmaxf(x(0), x(1)), x(2)), q = fmaxf(fmaxf(x(3), x(4)), x(5));
-                    r = fmaxf(fmaxf(r, x(6)), x(7));
-                    q = fmaxf(fmaxf(q, x(8)), x(9));
-                    r = fmaxf(fmaxf(r, x(10)), x(11));
-                    q = fmaxf(fmaxf(q, x(12)), x(13));
-                    r = fmaxf(fmaxf(r, x(14)), x(15));
-                    mx = fmaxf(mx, fmaxf(r, q) * f[b]);
-                }
-                if (__any_sync(0xffffffffu, mx > m + kSlack || vmax > vr)) {
-                    const float mn = fmaxf(m, mx + kMargin), vn = fmaxf(vr, pow2_above(vmax));
-                    const float al = mn == kNegInf ? 1.0f : ex2(m - mn), av = al * __fdiv_rn(vr, vn);
-                    m = mn;
-                    l *= al;
-                    vr = vn;
-                    vr_inv = __fdiv_rn(kWeightOne, vr);
-                    if (j > 0) {
-                        if (!warp_wait(&bars->pvdone[x][(n - 1) & 1], ((n - 1) >> 1) & 1, abort_flag, p.status, kASoftPv)) return;
-                        tc_fence_after();
-#pragma unroll 1
-                        for (int c = 0; c < C::D; c += 64) {
-                            uint32_t o[64];
-                            tm_ld32(t_o + c, o);
-                            tm_ld32(t_o + c + 32, o + 32);
-                            tc_wait_ld();
-                            reg_fence32(o);
-                            reg_fence32(o + 32);
+                    const bool none = ks[b] < 0.0f || t0 + 16 * b > limit;
+                    f[b] = none ? 1.0f : ks[b] != ks[b] ? ks[b] : fmaxf(f[b], 1e-37f);
+                    if (none) wv[b] = 0.0f;
+                    const int seen = none ? -1 : limit - t0 - 16 * b;
 #pragma unroll
-                            for (int i = 0; i < 64; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * av);
-                            tm_st32(t_o + c, o);
-                            tm_st32(t_o + c + 32, o + 32);
-                        }
-                        tc_wait_st();
-                    }
+                    for (int i = 0; i < 16; ++i)
+                        if (i > seen) s[16 * b + i] = 0xFF800000u;
                 }
-                // ---- weights ----
-                const float neg_m = m == kNegInf ? 0.0f : -m;
-                uint32_t pk[kBlk / 2];
-                uint64_t sum = 0;
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    const uint64_t f2 = pair2(f[b], f[b]), m2 = pair2(neg_m, neg_m);
-                    const float w = wv[b] * vr_inv;
-                    const uint64_t w2 = pair2(w, w);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int e = 16 * b + 2 * i;
-                        float lo, hi;
-                        unpair2(f2_fma(pair2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), f2, m2), lo, hi);
-                        const uint64_t pp = pair2(ex2(lo), ex2(hi));
-                        sum = f2_add(sum, pp);
-                        unpair2(f2_mul(pp, w2), lo, hi);
-                        pk[8 * b + i] = cvt_f16x2(lo, hi);
-                    }
-                }
-                float lo, hi;
-                unpair2(sum, lo, hi);
-                l += lo + hi;
-                // this P buffer is free once the PV two blocks back has read it
-                if (n >= 2 && !warp_wait(&bars->pvdone[x][n & 1], ((n - 2) >> 1) & 1, abort_flag, p.status, kASoftP)) return;
-                tc_fence_after();
-                tm_st32(tbase + lane_off + C::TM_P + (x * 2 + (n & 1)) * (kBlk / 2), pk);
-                tc_wait_st();
-                tc_fence_before();
             }
+            const float vmax = fmaxf(fmaxf(wv[0], wv[1]), fmaxf(wv[2], wv[3]));
+            // ---- reference maximum ----
+            float mx = kNegInf;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const uint32_t* x = s + 16 * b;
+                float r = max3(x[0], x[1], x[2]), q = max3(x[3], x[4], x[5]);
+                r = max3(r, x[6], x[7]);
+                q = max3(q, x[8], x[9]);
+                r = max3(r, x[10], x[11]);
+                q = max3(q, x[12], x[13]);
+                r = max3(r, x[14], x[15]);
+                mx = fmaxf(mx, fmaxf(r, q) * f[b]);
+            }
+            if (__any_sync(0xffffffffu, mx > m + kSlack || vmax > vr)) {
+                const float mn = fmaxf(m, mx + kMargin), vn = fmaxf(vr, pow2_above(vmax));
+                const float al = mn == kNegInf ? 1.0f : ex2(m - mn), av = al * __fdiv_rn(vr, vn);
+                m = mn;
+                l *= al;
+                vr = vn;
+                vr_inv = __fdiv_rn(kWeightOne, vr);
+                if (j > 0) {
+                    if (!warp_wait(&bars->pvdone[x][(n - 1) & 1], ((n - 1) >> 1) & 1, abort_flag, p.status, kASoftPv)) return;
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < C::D; c += 64) {
+                        uint32_t o[64];
+                        tm_ld32(t_o + c, o);
+                        tm_ld32(t_o + c + 32, o + 32);
+                        tc_wait_ld();
+                        reg_fence32(o);
+                        reg_fence32(o + 32);
+#pragma unroll
+                        for (int i = 0; i < 64; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * av);
+                        tm_st32(t_o + c, o);
+                        tm_st32(t_o + c + 32, o + 32);
+                    }
+                    tc_wait_st();
+                }
+            }
+            // ---- weights ----
+            const float neg_m = m == kNegInf ? 0.0f : -m;
+            uint32_t pk[kBlk / 2];
+            uint64_t sum[2] = {0, 0};
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const uint64_t f2 = pair2(f[b], f[b]), m2 = pair2(neg_m, neg_m);
+                const float w = wv[b] * vr_inv;
+                const uint64_t w2 = pair2(w, w);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int e = 16 * b + 2 * i;
+                    float lo, hi;
+                    unpair2(f2_fma(pair2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), f2, m2), lo, hi);
+                    const uint64_t pp = pair2(ex2(lo), ex2(hi));
+                    sum[i & 1] = f2_add(sum[i & 1], pp);
+                    unpair2(f2_mul(pp, w2), lo, hi);
+                    pk[8 * b + i] = cvt_f16x2(lo, hi);
+                }
+            }
+            float lo, hi;
+            unpair2(f2_add(sum[0], sum[1]), lo, hi);
+            l += lo + hi;
+            // this P buffer is free once the PV two blocks back has read it
+            if (n >= 2 && !warp_wait(&bars->pvdone[x][n & 1], ((n - 2) >> 1) & 1, abort_flag, p.status, kASoftP)) return;
+            tc_fence_after();
+            tm_st32(tbase + lane_off + C::TM_P + (x * 2 + (n & 1)) * (kBlk / 2), pk);
+            tc_wait_st();
+            tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars->pready[x][n & 1]);
         }
