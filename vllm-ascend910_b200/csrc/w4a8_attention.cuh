@@ -124,12 +124,15 @@ __device__ __forceinline__ float4 join_parts(int n, const M& ml, const V& value)
         float4 x[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const bool in = base + i < n;
-            const int k = in ? base + i : 0;
-            const float2 v = ml(k);
-            m[i] = in ? v.x : kNegInf;
-            l[i] = in ? v.y : 0.0f;
-            x[i] = value(k);
+            m[i] = kNegInf;
+            l[i] = 0.0f;
+            x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (base + i < n) {
+                const float2 v = ml(base + i);
+                m[i] = v.x;
+                l[i] = v.y;
+                x[i] = value(base + i);
+            }
         }
         float mn = mx;
 #pragma unroll

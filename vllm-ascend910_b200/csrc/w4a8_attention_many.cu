@@ -53,7 +53,7 @@ constexpr int kManyThreads = 16 * 32;      // whole warpgroups: setmaxnreg moves
 constexpr int kConvWarp = 8, kMmaWarp = 12;
 constexpr int kRegsSoft = 176, kRegsConv = 88, kRegsMma = 64;      // 2, 1 and 1 warpgroups of them
 static_assert(2 * kRegsSoft + kRegsConv + kRegsMma <= 4 * 128, "the launch allocates 128 registers a thread");
-constexpr int kTileUnits = 4;              // what beginning and ending a tile costs, in blocks (work shares)
+constexpr int kTileUnits = 6;              // what beginning and ending a tile costs, in blocks (work shares)
 constexpr int kMinUnits = 4;               // a CTA's share is not cut below this
 constexpr float kMargin = 2.0f;            // log2 by which a new reference exceeds the scores seen
 
@@ -276,22 +276,12 @@ struct ManyLayout {
 
 // ------------------------------------------------------------------ converters
 
-// One 16-byte vector of codes -> 16 fp16 values in two 16-byte units of the
-// swizzled row.
-template <class C>
-__device__ __forceinline__ void put_codes(uint32_t stage, int tok, int c, const uint4& v)
+// One 16-byte vector of codes -> 16 fp16 values, two 16-byte units at a0 and a1.
+__device__ __forceinline__ void put_codes(uint32_t a0, uint32_t a1, const uint4& v)
 {
     const uint32_t w[4] = {v.x ^ 0x80808080u, v.y ^ 0x80808080u, v.z ^ 0x80808080u, v.w ^ 0x80808080u};
-    uint32_t h[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        h[2 * i] = biased_lo(w[i]);
-        h[2 * i + 1] = biased_hi(w[i]);
-    }
-    const uint32_t row = stage + (c >> 2) * C::KV_CHUNK + tok * 128;
-    const uint32_t u = (c & 3) * 2, x = tok & 7;
-    sts128(row + ((u ^ x) << 4), h[0], h[1], h[2], h[3]);
-    sts128(row + (((u + 1) ^ x) << 4), h[4], h[5], h[6], h[7]);
+    sts128(a0, biased_lo(w[0]), biased_hi(w[0]), biased_lo(w[1]), biased_hi(w[1]));
+    sts128(a1, biased_lo(w[2]), biased_hi(w[2]), biased_lo(w[3]), biased_hi(w[3]));
 }
 
 template <class C>
@@ -314,48 +304,42 @@ __device__ __forceinline__ void converter_role(const AttentionParams& p, ManyBar
         c = lane & 3;
     }
     constexpr int TSTEP = 128 / PER_ROW;                            // tokens between a thread's vectors
+    // Offsets of its first vector in a stage (the swizzle is the same for the others)
+    // and, in a 16-token granule of the cache, in bytes.
+    const uint32_t row0 = (c >> 2) * C::KV_CHUNK + tok0 * 128;
+    const uint32_t off0 = row0 + ((((c & 3) * 2) ^ (tok0 & 7)) << 4), off1 = row0 + ((((c & 3) * 2 + 1) ^ (tok0 & 7)) << 4);
+    const int in_granule = (tok0 & 15) * C::D + c * 16;
 
     // Three blocks are on their way: page ids of the one after next (a), codes of
-    // the next (kr, vr, in registers), and the block being converted.
+    // the next (kr, vr, in registers), and the block being converted.  Lane l holds
+    // what concerns granule l % 4 of a block and hands it round.
+    const int gr = lane & 3, pages = static_cast<int>(cv.pages);
     Walk a;
     bool have_id = a.begin(p, st, least);
     int ab = a.b0;
-    const int pages = static_cast<int>(cv.pages);
-    int id[N], sid = -1, head = 0, base = 0;
+    int id = -1, head = 0, base = 0;
     uint4 kr[N], vr[N];
     float sc[2] = {-1.0f, -1.0f};
-    // Loads do not wait for tests: tokens past the length take the last token's page,
-    // and where there is no page codes come from page 0 (what they are does not
-    // matter: their scores are masked and their weights 0).
     auto load_ids = [&]() {
-        const int32_t* row = cv.table + static_cast<int64_t>(a.seq) * cv.ld_table;
         head = a.head;
-        base = ab * kBlk;
-        const int last = a.s.len - 1;
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            id[k] = -1;
-            if (last >= 0) id[k] = row[min(base + tok0 + k * TSTEP, last) >> cv.page_log2];
-        }
-        sid = -1;
-        if (base + (i & 3) * 16 <= last) sid = row[(base + (i & 3) * 16) >> cv.page_log2];
+        base = ab * kBlk + gr * 16;
+        id = base < a.s.len ? cv.table[a.seq * cv.ld_table + (base >> cv.page_log2)] : -1;
     };
+    // Where there is no page, codes come from page 0: what they are does not matter,
+    // their scores are masked and their weights 0.
     auto load_codes = [&]() {
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            const int from = static_cast<unsigned>(id[k]) < static_cast<unsigned>(pages) ? id[k] : 0;
-            const int64_t at = (((static_cast<int64_t>(from) * cv.kv_heads + head) << cv.page_log2) +
-                                ((base + tok0 + k * TSTEP) & (cv.page - 1))) * C::D + c * 16;
-            kr[k] = *reinterpret_cast<const uint4*>(cv.k + at);
-            vr[k] = *reinterpret_cast<const uint4*>(cv.v + at);
-        }
-        // page scales of the block's four 16-token granules (lanes hold one each, four
-        // times over), -1 where there is no page
-        const bool there = static_cast<unsigned>(sid) < static_cast<unsigned>(pages);
-        const int64_t ph = there ? static_cast<int64_t>(sid) * cv.kv_heads + head : head;
+        const bool there = static_cast<unsigned>(id) < static_cast<unsigned>(pages);
+        const int64_t ph = static_cast<int64_t>(there ? id : 0) * cv.kv_heads + head;
+        const int64_t at = ((ph << cv.page_log2) + (base & (cv.page - 1))) * C::D;
         sc[0] = cv.k_scale[ph];
         sc[1] = cv.v_scale[ph];
         if (!there) sc[0] = sc[1] = -1.0f;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int64_t from = __shfl_sync(0xffffffffu, at, (tok0 + k * TSTEP) >> 4) + in_granule;
+            kr[k] = *reinterpret_cast<const uint4*>(cv.k + from);
+            vr[k] = *reinterpret_cast<const uint4*>(cv.v + from);
+        }
     };
     auto step_ids = [&]() {
         if (++ab >= a.b1) {
@@ -382,13 +366,13 @@ __device__ __forceinline__ void converter_role(const AttentionParams& p, ManyBar
         const bool odd = __any_sync(0xffffffffu, !(sc[0] >= 1e-30f && sc[0] < 1e30f));
         if (i == 0) ring[g % kScaleRing].odd = odd;
 #pragma unroll
-        for (int k = 0; k < N; ++k) put_codes<C>(ks, tok0 + k * TSTEP, c, kr[k]);
+        for (int k = 0; k < N; ++k) put_codes(ks + off0 + k * TSTEP * 128, ks + off1 + k * TSTEP * 128, kr[k]);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->kfull[sg]);
         if (!warp_wait(&bars->vempty[sg], ph ^ 1, abort_flag, p.status, kAConvV)) return;
 #pragma unroll
-        for (int k = 0; k < N; ++k) put_codes<C>(vs, tok0 + k * TSTEP, c, vr[k]);
+        for (int k = 0; k < N; ++k) put_codes(vs + off0 + k * TSTEP * 128, vs + off1 + k * TSTEP * 128, vr[k]);
         more = have_id;
         if (more) {
             load_codes();
