@@ -30,6 +30,7 @@ NORM_MAX_K = 32768               # W4A8_NORM_MAX_K
 ATTENTION_MAX_BATCH = 2048       # W4A8_ATTENTION_MAX_BATCH
 
 _L = None
+_N = False                       # the module behind native(), None if absent, False before the first call
 
 _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -126,6 +127,24 @@ def lib() -> ctypes.CDLL:
             fn.argtypes = args
         _L = L
     return _L
+
+
+def native():
+    """The short way into the small operators' entry points (``_native``, csrc/w4a8_native.cpp), bound to
+    the library that ``lib()`` loaded; None where it was not built.  Its functions return
+    NotImplemented for a call that needs the wrappers' own checks, copies or messages."""
+    global _N
+    if _N is False:
+        L = lib()
+        try:
+            from . import _native as N
+        except ImportError:
+            N = None
+        if N is not None:
+            N.bind(*(ctypes.cast(getattr(L, name), _p).value for name in
+                     ("w4a8_rms_norm", "w4a8_rms_norm_quant", "w4a8_kv_write", "w4a8_kv_read", "w4a8_attention")))
+        _N = N
+    return _N
 
 
 class W4A8Error(RuntimeError):

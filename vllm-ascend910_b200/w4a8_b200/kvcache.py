@@ -36,7 +36,7 @@ HEAD_DIMS = (64, 128)
 class KVCache:
     """One layer's cache: four tensors, checked once, and their C descriptor."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "kv_heads", "page_size", "head_dim", "device", "_desc",
+    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "kv_heads", "page_size", "head_dim", "device", "_index", "_desc",
                  "_ref")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
@@ -55,6 +55,7 @@ class KVCache:
         self.device = k.device
         self._desc = _lib.KvCacheDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), P, H, S, D, 0)
         self._ref = ctypes.addressof(self._desc)
+        self._index = k.get_device()
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, page_size: int = 16, head_dim: int = 128, device="cuda") -> "KVCache":
@@ -190,6 +191,11 @@ def kv_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, page_table: torch
     With ``cos_sin`` (``rotary_table``) the first ``cos_sin.shape[1]`` elements of every q and k head
     are turned by the token's position in its sequence: first and second half pairwise, or
     neighbours with ``interleaved``.  q, k and v may be strided views of one [q | k | v] tensor."""
+    N = _lib.native()
+    if N is not None and q_out is None:
+        got = N.kv_write(cache._ref, cache._index, page_table, kv_lens, cu_q, k, v, q, cos_sin, interleaved)
+        if got is not NotImplemented:
+            return got
     B, tp, ld, cols = _batch("kv_write", cache, page_table, kv_lens, cu_q)
     k, T, H, ldk, kp = _heads("kv_write", "k", k, cache)
     v, Tv, Hv, ldv, vp = _heads("kv_write", "v", v, cache)
@@ -225,6 +231,11 @@ def kv_read(cache: KVCache, page_table: torch.Tensor, kv_lens: torch.Tensor, cu_
             tokens: int) -> Tuple[torch.Tensor, torch.Tensor]:
     """The last ``cu_out[s + 1] - cu_out[s]`` cached tokens of each sequence (``tokens`` =
     cu_out's last value, known to the caller): k, v bf16 [tokens, kv_heads, head_dim]."""
+    N = _lib.native()
+    if N is not None:
+        got = N.kv_read(cache._ref, cache._index, page_table, kv_lens, cu_out, tokens)
+        if got is not NotImplemented:
+            return got
     B, tp, ld, cols = _batch("kv_read", cache, page_table, kv_lens, cu_out)
     if tokens < 0:
         raise RuntimeError("kv_read: tokens must not be negative")
@@ -250,6 +261,13 @@ def attention(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor, kv_lens
     (``kv_write`` comes first: ``kv_lens`` counts these tokens).  q_heads is a multiple of the
     cache's kv_heads; ``max_q_len`` is the longest cu_q[s + 1] - cu_q[s]; ``scale`` defaults to
     head_dim ** -0.5.  A row that sees no token is zero."""
+    N = _lib.native()
+    if N is not None and out is None:
+        # a workspace that is too small for the call is refused, and grown below
+        got = N.attention(cache._ref, cache._index, page_table, kv_lens, cu_q, q, max_q_len,
+                          cache.head_dim ** -0.5 if scale is None else scale, *workspace(0, cache.device))
+        if got is not NotImplemented:
+            return got
     B, tp, ld, cols = _batch("attention", cache, page_table, kv_lens, cu_q)
     q, T, hq, ldq, qp = _heads("attention", "q", q, cache)
     H, D = cache.kv_heads, cache.head_dim

@@ -462,6 +462,11 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
     Without a residual returns y.  With one returns (y, bf16(h)), the latter
     into ``residual_out`` when given (it may be the residual itself).  fp32
     inside, each output rounded once."""
+    N = _lib.native()
+    if N is not None and residual_out is None and out is None:
+        got = N.rms_norm(x, weight, residual, eps)
+        if got is not NotImplemented:
+            return got
     x2, M, K, ldx, wd, r2, rp, ldr, ro, rop, ldro = _norm_args(x, weight, residual, residual_out, "rms_norm")
     if out is None:
         y = torch.empty_like(x2) if ldx == K else torch.empty((M, K), dtype=_BF16, device=x.device)
@@ -483,6 +488,11 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, group_size: int, eps: 
                    scale_dtype: torch.dtype = torch.bfloat16):
     """``rms_norm`` with its fp32 result quantised per (token, group) by ``quant_act``'s rule:
     x [M, K] -> (q int8 [M, K], scale [G, M], bf16(x + residual) or None)."""
+    N = _lib.native()
+    if N is not None and residual_out is None:
+        got = N.rms_norm_quant(x, weight, residual, eps, group_size, scale_dtype)
+        if got is not NotImplemented:
+            return got
     _check(x.dim() == 2, "rms_norm_quant: x must be [M, K]")
     _check(scale_dtype in (torch.float32, torch.bfloat16), "rms_norm_quant: scale dtype must be bf16 or f32")
     x2, M, K, ldx, wd, r2, rp, ldr, ro, rop, ldro = _norm_args(x, weight, residual, residual_out, "rms_norm_quant")
