@@ -47,18 +47,20 @@ namespace {
 
 constexpr int kBlk = 64;                   // tokens per step
 constexpr int kRows = 256;                 // packed rows per tile
-constexpr int kNS = 4;                     // K and V stages
+constexpr int kNS = 3;                     // K and V stages
+constexpr int kNR = 3;                     // blocks of codes on their way
+static_assert(kNR <= kNS, "the fetching warp arrives on a K stage's barrier for no block but its next");
 constexpr int kScaleRing = 16;             // blocks whose page scales are kept
 constexpr int kManyThreads = 16 * 32;      // whole warpgroups: setmaxnreg moves registers between them
-constexpr int kConvWarp = 8, kMmaWarp = 12;
-constexpr int kRegsSoft = 176, kRegsConv = 88, kRegsMma = 64;      // 2, 1 and 1 warpgroups of them
-static_assert(2 * kRegsSoft + kRegsConv + kRegsMma <= 4 * 128, "the launch allocates 128 registers a thread");
+constexpr int kConvWarp = 8, kMmaWarp = 12, kFetchWarp = 14;
+constexpr int kRegsSoft = 176, kRegsRest = 80;      // 2 warpgroups of each
+static_assert(2 * kRegsSoft + 2 * kRegsRest <= 4 * 128, "the launch allocates 128 registers a thread");
 constexpr int kTileUnits = 6;              // what beginning and ending a tile costs, in blocks (work shares)
 constexpr int kMinUnits = 4;               // a CTA's share is not cut below this
 constexpr float kMargin = 2.0f;            // log2 by which a new reference exceeds the scores seen
 
 // wait-site ids for the status word
-enum { kAMmaK = 0x41, kAMmaV, kAMmaQ, kAMmaO, kAMmaP, kAMmaS, kASoftS, kASoftPv, kASoftP, kASoftEnd, kAConvK, kAConvV, kADrain };
+enum { kAMmaK = 0x41, kAMmaV, kAMmaQ, kAMmaO, kAMmaP, kAMmaS, kASoftS, kASoftPv, kASoftP, kASoftEnd, kAConvK, kAConvV, kAConvRaw, kAFetch, kADrain };
 
 template <int D_>
 struct ManyCfg {
@@ -70,20 +72,21 @@ struct ManyCfg {
     static constexpr int KV_STAGE = CH * KV_CHUNK;
     static constexpr int OFF_K = 2 * Q_HALF;
     static constexpr int OFF_V = OFF_K + kNS * KV_STAGE;
-    static constexpr int OFF_PREFIX = OFF_V + kNS * KV_STAGE;
+    static constexpr int RAW_STAGE = 2 * kBlk * D_;          // codes of K, then V
+    static constexpr int OFF_RAW = OFF_V + kNS * KV_STAGE;
+    static constexpr int OFF_PREFIX = OFF_RAW + kNR * RAW_STAGE;
     static constexpr int TM_S = 0;                           // [half] of 64 columns
     static constexpr int TM_P = 128;                         // [half][buffer] of 32 columns
     static constexpr int TM_O = 256;                         // [half] of D columns
     static constexpr int TM_COLS = 512;
     static constexpr int PIECE = kRows * D_ * 4;
-    static constexpr int UNITS_PER_THREAD = kBlk * D_ / 16 / 128;   // 16-byte code vectors a converter thread moves
 };
 
 // P and PV phases have a barrier for each of the two buffers: every wait is for a
 // phase whose predecessor on the same barrier (two blocks back) is known to be
 // complete and whose successor cannot have completed, so parity tells.
 struct ManyBars {
-    uint64_t kfull[kNS], kempty[kNS], vfull[kNS], vempty[kNS];
+    uint64_t kfull[kNS], kempty[kNS], vfull[kNS], vempty[kNS], rfull[kNR], rempty[kNR];
     uint64_t sfull[2], sfree[2], pready[2][2], pvdone[2][2], qfull[2], ofree[2], drain[2];
     uint32_t tmem_base;
     int abort;
@@ -284,103 +287,120 @@ __device__ __forceinline__ void put_codes(uint32_t a0, uint32_t a1, const uint4&
     sts128(a1, biased_lo(w[2]), biased_hi(w[2]), biased_lo(w[3]), biased_hi(w[3]));
 }
 
-template <class C>
-__device__ __forceinline__ void converter_role(const AttentionParams& p, ManyBars* bars, uint32_t sm, BlockScales* ring,
-                                               const Start& st, int least, volatile int* abort_flag)
+__device__ __forceinline__ void bulk_to(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar)
 {
-    constexpr int N = C::UNITS_PER_THREAD, PER_ROW = C::D / 16;     // vectors of a token's row
-    const int i = threadIdx.x - kConvWarp * 32;
-    const CacheView& cv = p.c;
-    // The thread's vectors of a block: token tok0 + k * 16 * (8 / PER_ROW)..., one 16-token
-    // granule (or two) per step of k.  Lanes are dealt so that the eight lanes of a
-    // store phase hit distinct banks: two tokens x four vectors.
-    const int lane = lane_id(), w = i >> 5;
-    int tok0, c;
-    if (PER_ROW == 8) {
-        tok0 = w * 4 + (lane >> 4) * 2 + ((lane >> 2) & 1);
-        c = (lane & 3) + ((lane >> 3) & 1) * 4;
-    } else {
-        tok0 = w * 8 + (lane >> 2);
-        c = lane & 3;
-    }
-    constexpr int TSTEP = 128 / PER_ROW;                            // tokens between a thread's vectors
-    // Offsets of its first vector in a stage (the swizzle is the same for the others)
-    // and, in a 16-token granule of the cache, in bytes.
-    const uint32_t row0 = (c >> 2) * C::KV_CHUNK + tok0 * 128;
-    const uint32_t off0 = row0 + ((((c & 3) * 2) ^ (tok0 & 7)) << 4), off1 = row0 + ((((c & 3) * 2 + 1) ^ (tok0 & 7)) << 4);
-    const int in_granule = (tok0 & 15) * C::D + c * 16;
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
 
-    // Three blocks are on their way: page ids of the one after next (a), codes of
-    // the next (kr, vr, in registers), and the block being converted.  Lane l holds
-    // what concerns granule l % 4 of a block and hands it round.
-    const int gr = lane & 3, pages = static_cast<int>(cv.pages);
+// One warp fetches: the codes of a block's four 16-token granules, which lie together in
+// their pages, by bulk copies (lanes 0-3 K's, 4-7 V's), and the page scales.
+template <class C>
+__device__ __forceinline__ void fetch_role(const AttentionParams& p, ManyBars* bars, uint32_t sm, BlockScales* ring,
+                                           const Start& st, int least, volatile int* abort_flag)
+{
+    const CacheView& cv = p.c;
+    const int lane = lane_id(), gr = lane & 3, pages = static_cast<int>(cv.pages);
+    const bool of_v = lane & 4;
+    const int8_t* codes = of_v ? cv.v : cv.k;
+    const float* scales = of_v ? cv.v_scale : cv.k_scale;
+    const uint32_t to = sm + C::OFF_RAW + (of_v ? C::RAW_STAGE / 2 : 0) + gr * 16 * C::D;
     Walk a;
-    bool have_id = a.begin(p, st, least);
-    int ab = a.b0;
-    int id = -1, head = 0, base = 0;
-    uint4 kr[N], vr[N];
-    float sc[2] = {-1.0f, -1.0f};
-    auto load_ids = [&]() {
+    bool more = a.begin(p, st, least);
+    int ab = a.b0, id = -1, head = 0, base = 0;
+    auto load_id = [&]() {               // a block ahead
         head = a.head;
         base = ab * kBlk + gr * 16;
         id = base < a.s.len ? cv.table[a.seq * cv.ld_table + (base >> cv.page_log2)] : -1;
     };
-    // Where there is no page, codes come from page 0: what they are does not matter,
-    // their scores are masked and their weights 0.
-    auto load_codes = [&]() {
+    if (more) load_id();
+    uint32_t g = 0;
+    for (; more; ++g) {
+        const uint32_t sr = g % kNR;
+        if (!warp_wait(&bars->rempty[sr], ((g / kNR) & 1) ^ 1, abort_flag, p.status, kAFetch)) break;
+        // Where there is no page, codes come from page 0: what they are does not matter,
+        // their scores are masked and their weights 0.
         const bool there = static_cast<unsigned>(id) < static_cast<unsigned>(pages);
         const int64_t ph = static_cast<int64_t>(there ? id : 0) * cv.kv_heads + head;
-        const int64_t at = ((ph << cv.page_log2) + (base & (cv.page - 1))) * C::D;
-        sc[0] = cv.k_scale[ph];
-        sc[1] = cv.v_scale[ph];
-        if (!there) sc[0] = sc[1] = -1.0f;
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            const int64_t from = __shfl_sync(0xffffffffu, at, (tok0 + k * TSTEP) >> 4) + in_granule;
-            kr[k] = *reinterpret_cast<const uint4*>(cv.k + from);
-            vr[k] = *reinterpret_cast<const uint4*>(cv.v + from);
-        }
-    };
-    auto step_ids = [&]() {
+        const int8_t* from = codes + ((ph << cv.page_log2) + (base & (cv.page - 1))) * C::D;
+        if (lane == 0) mbar_arrive_expect_tx(&bars->rfull[sr], C::RAW_STAGE);
+        __syncwarp();
+        if (lane < 8) bulk_to(to + sr * C::RAW_STAGE, from, 16 * C::D, &bars->rfull[sr]);
+        const float sc = there ? scales[ph] : -1.0f;
         if (++ab >= a.b1) {
-            have_id = a.next(p, least);
+            more = a.next(p, least);
             ab = a.b0;
         }
-        if (have_id) load_ids();
-    };
-    bool more = have_id;
-    if (have_id) {
-        load_ids();
-        load_codes();
-        step_ids();
-    }
-    for (uint32_t g = 0; more; ++g) {
-        const uint32_t sg = g % kNS, ph = (g / kNS) & 1;
-        const uint32_t ks = sm + C::OFF_K + sg * C::KV_STAGE, vs = sm + C::OFF_V + sg * C::KV_STAGE;
-        if (!warp_wait(&bars->kempty[sg], ph ^ 1, abort_flag, p.status, kAConvK)) return;
-        if (i < 4) {
-            ring[g % kScaleRing].k[i] = sc[0];
-            ring[g % kScaleRing].v[i] = sc[1];
-        }
+        if (more) load_id();
+        BlockScales& rg = ring[g % kScaleRing];
+        if (lane < 8) (of_v ? rg.v : rg.k)[gr] = sc;
         // a block with a scale that is missing, zero, infinite or NaN takes the careful path
-        const bool odd = __any_sync(0xffffffffu, !(sc[0] >= 1e-30f && sc[0] < 1e30f));
-        if (i == 0) ring[g % kScaleRing].odd = odd;
+        const bool odd = __any_sync(0xffffffffu, !of_v && !(sc >= 1e-30f && sc < 1e30f));
+        if (lane == 0) rg.odd = odd;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->kfull[g % kNS]);
+    }
+    // no copy is in flight when the block ends, whatever became of the other warps
+    int own = 0;
+    for (uint32_t i = g < kNR ? 0 : g - kNR; i < g; ++i) mbar_wait(&bars->rfull[i % kNR], (i / kNR) & 1, &own, p.status, kADrain);
+}
+
+template <class C>
+__device__ __forceinline__ void converter_role(const AttentionParams& p, ManyBars* bars, uint32_t sm, const Start& st, int least,
+                                               volatile int* abort_flag)
+{
+    constexpr int PER_ROW = C::D / 16;                              // vectors of a token's row
+    constexpr int N = kBlk * PER_ROW / 128;                         // vectors of a thread
+    constexpr int TSTEP = 128 / PER_ROW;                            // tokens between them
+    static_assert(TSTEP % 8 == 0, "the swizzle is the same for a thread's vectors");
+    // Lanes are dealt so that the eight lanes of a phase hit distinct banks reading and
+    // writing: a token's first half of vectors and the next one's second half, or two
+    // whole rows of four vectors.
+    const int lane = lane_id(), w = warp_id() - kConvWarp;
+    int tok0, c;
+    if (PER_ROW == 8) {
+        tok0 = w * 4 + (lane >> 4) * 2 + (((lane >> 2) ^ (lane >> 3)) & 1);
+        c = lane & 7;
+    } else {
+        tok0 = w * 8 + (lane >> 2);
+        c = lane & 3;
+    }
+    const uint32_t from = sm + C::OFF_RAW + tok0 * C::D + c * 16;
+    const uint32_t row0 = sm + (c >> 2) * C::KV_CHUNK + tok0 * 128;
+    const uint32_t to0 = row0 + ((((c & 3) * 2) ^ (tok0 & 7)) << 4), to1 = row0 + ((((c & 3) * 2 + 1) ^ (tok0 & 7)) << 4);
+    Walk a;
+    bool more = a.begin(p, st, least);
+    int ab = a.b0;
+    for (uint32_t g = 0; more; ++g) {
+        const uint32_t sg = g % kNS, ph = (g / kNS) & 1, sr = g % kNR;
+        uint4 r[N];
+        if (!warp_wait(&bars->rfull[sr], (g / kNR) & 1, abort_flag, p.status, kAConvRaw)) return;
 #pragma unroll
-        for (int k = 0; k < N; ++k) put_codes(ks + off0 + k * TSTEP * 128, ks + off1 + k * TSTEP * 128, kr[k]);
+        for (int k = 0; k < N; ++k) r[k] = lds128(from + sr * C::RAW_STAGE + k * TSTEP * C::D);
+        if (!warp_wait(&bars->kempty[sg], ph ^ 1, abort_flag, p.status, kAConvK)) return;
+        uint32_t at = C::OFF_K + sg * C::KV_STAGE;
+#pragma unroll
+        for (int k = 0; k < N; ++k) put_codes(to0 + at + k * TSTEP * 128, to1 + at + k * TSTEP * 128, r[k]);
+#pragma unroll
+        for (int k = 0; k < N; ++k) r[k] = lds128(from + sr * C::RAW_STAGE + C::RAW_STAGE / 2 + k * TSTEP * C::D);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->kfull[sg]);
         if (!warp_wait(&bars->vempty[sg], ph ^ 1, abort_flag, p.status, kAConvV)) return;
+        at = C::OFF_V + sg * C::KV_STAGE;
 #pragma unroll
-        for (int k = 0; k < N; ++k) put_codes(vs + off0 + k * TSTEP * 128, vs + off1 + k * TSTEP * 128, vr[k]);
-        more = have_id;
-        if (more) {
-            load_codes();
-            step_ids();
-        }
+        for (int k = 0; k < N; ++k) put_codes(to0 + at + k * TSTEP * 128, to1 + at + k * TSTEP * 128, r[k]);
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->vfull[sg]);
+        if (lane == 0) {
+            mbar_arrive(&bars->vfull[sg]);
+            mbar_arrive(&bars->rempty[sr]);
+        }
+        if (++ab >= a.b1) {
+            more = a.next(p, least);
+            ab = a.b0;
+        }
     }
 }
 
@@ -726,10 +746,14 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Atte
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kNS; ++i) {
-            mbar_init(&bars->kfull[i], 4);
+            mbar_init(&bars->kfull[i], 5);
             mbar_init(&bars->kempty[i], 2);
             mbar_init(&bars->vfull[i], 4);
             mbar_init(&bars->vempty[i], 2);
+        }
+        for (int i = 0; i < kNR; ++i) {
+            mbar_init(&bars->rfull[i], 1);
+            mbar_init(&bars->rempty[i], 4);
         }
         for (int x = 0; x < 2; ++x) {
             for (int b = 0; b < 2; ++b) {
@@ -827,12 +851,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Atte
     if (warp < kConvWarp) {
         regs_inc<kRegsSoft>();
         softmax_role<C>(p, bars, sm, tbase, ring, st, least, abort_flag);
-    } else if (warp < kMmaWarp) {
-        regs_dec<kRegsConv>();
-        converter_role<C>(p, bars, sm, ring, st, least, abort_flag);
     } else {
-        regs_dec<kRegsMma>();
-        if (warp < kMmaWarp + 2 && elect_one()) mma_role<C>(p, bars, sm, tbase, warp - kMmaWarp, st, least, abort_flag);
+        regs_dec<kRegsRest>();
+        if (warp < kMmaWarp) converter_role<C>(p, bars, sm, st, least, abort_flag);
+        else if (warp == kFetchWarp) fetch_role<C>(p, bars, sm, ring, st, least, abort_flag);
+        else if (warp < kFetchWarp && elect_one()) mma_role<C>(p, bars, sm, tbase, warp - kMmaWarp, st, least, abort_flag);
     }
     pdl_launch_dependents();
     __syncwarp();
@@ -882,7 +905,7 @@ cudaError_t launch_many(const AttentionParams& p, int least, int sms, cudaStream
         // setmaxnreg draws on the launch's registers: a build with fewer than the split needs must not start
         cudaFuncAttributes fa{};
         if ((e = cudaFuncGetAttributes(&fa, attend_many_kernel<C>)) != cudaSuccess) return e;
-        if (fa.numRegs * 4 < 2 * kRegsSoft + kRegsConv + kRegsMma) return cudaErrorInvalidConfiguration;
+        if (fa.numRegs * 4 < 2 * kRegsSoft + 2 * kRegsRest) return cudaErrorInvalidConfiguration;
         if (dev >= 0 && dev < 64) ready[dev] = true;
     }
     cudaLaunchConfig_t cfg = {};
