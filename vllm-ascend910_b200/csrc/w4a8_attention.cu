@@ -759,15 +759,17 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
             if (first.tile * C::R + row >= first.rows) continue;
             // part k is slot 1 of the segment's first CTA, slot 0 of the others
             const auto at = [&](int k) { return static_cast<size_t>(2 * (cta0 + k) + (k == 0)); };
-            const float4 o = join_parts(
+            float4 o[1];
+            join_parts<8>(
                 n,
                 [&](int k) {
                     const float* v = all_ml + at(k) * 2 * C::R + row;
                     return make_float2(__ldcg(v), __ldcg(v + C::R));
                 },
-                [&](int k) { return __ldcg(reinterpret_cast<const float4*>(all_o + at(k) * C::R * C::D + row * C::D + d4 * 4)); });
+                [&](int k, int) { return __ldcg(reinterpret_cast<const float4*>(all_o + at(k) * C::R * C::D + row * C::D + d4 * 4)); },
+                o);
             uint16_t* dst = out_row(p, first.q0, first.head, first.tile * C::R + row) + d4 * 4;
-            *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(o[0].x, o[0].y), pack_bf16(o[0].z, o[0].w));
         }
     }
 }

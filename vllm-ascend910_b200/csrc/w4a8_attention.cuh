@@ -111,53 +111,58 @@ struct Partial {
     int head, row0;     // kv head, the segment's first packed row
 };
 
-// Adds one segment's n parts for 4 elements of one row: parts are the leader's
-// slot 1 and slot 0 of the CTAs behind it.  Loads of 8 parts (maximum, sum, values)
-// are in flight together.
-template <class M, class V>
-__device__ __forceinline__ float4 join_parts(int n, const M& ml, const V& value)
+// Adds one segment's n parts for NV times 4 elements of one row: parts are the
+// leader's slot 1 and slot 0 of the CTAs behind it.  Loads of NB parts (maximum, sum,
+// values) are in flight together.
+template <int NB, int NV, class M, class V>
+__device__ __forceinline__ void join_parts(int n, const M& ml, const V& value, float4 (&o)[NV])
 {
     float mx = kNegInf, ls = 0.0f;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int base = 0; base < n; base += 8) {
-        float m[8], l[8];
-        float4 x[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+    for (int v = 0; v < NV; ++v) o[v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int base = 0; base < n; base += NB) {
+        float m[NB], l[NB];
+        float4 x[NB][NV];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
             m[i] = kNegInf;
             l[i] = 0.0f;
-            x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int v = 0; v < NV; ++v) x[i][v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (base + i < n) {
-                const float2 v = ml(base + i);
-                m[i] = v.x;
-                l[i] = v.y;
-                x[i] = value(base + i);
+                const float2 t = ml(base + i);
+                m[i] = t.x;
+                l[i] = t.y;
+#pragma unroll
+                for (int v = 0; v < NV; ++v) x[i][v] = value(base + i, v);
             }
         }
         float mn = mx;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) mn = fmaxf(mn, m[i]);
+        for (int i = 0; i < NB; ++i) mn = fmaxf(mn, m[i]);
         const float keep = mx == kNegInf ? (mn == kNegInf ? 1.0f : 0.0f) : exp2f(mx - mn);
         ls *= keep;
-        o.x *= keep;
-        o.y *= keep;
-        o.z *= keep;
-        o.w *= keep;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int v = 0; v < NV; ++v) o[v] = make_float4(o[v].x * keep, o[v].y * keep, o[v].z * keep, o[v].w * keep);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
             if (base + i >= n) break;
             // (a part without a visible token has m = -inf, l = 0 and zeros)
             const float a = m[i] == kNegInf ? 1.0f : exp2f(m[i] - mn);
             ls += a * l[i];
-            o.x += a * x[i].x;
-            o.y += a * x[i].y;
-            o.z += a * x[i].z;
-            o.w += a * x[i].w;
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                o[v].x += a * x[i][v].x;
+                o[v].y += a * x[i][v].y;
+                o[v].z += a * x[i][v].z;
+                o[v].w += a * x[i][v].w;
+            }
         }
         mx = mn;
     }
     const float inv = ls > 0.0f ? __fdiv_rn(1.0f, ls) : (ls == 0.0f ? 0.0f : ls);
-    return make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) o[v] = make_float4(o[v].x * inv, o[v].y * inv, o[v].z * inv, o[v].w * inv);
 }
 
 // row / group: the query token of a packed row.  With M = floor(2^64 / g) + 1 the

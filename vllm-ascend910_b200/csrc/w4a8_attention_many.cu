@@ -60,7 +60,7 @@ constexpr int kMinUnits = 4;               // a CTA's share is not cut below thi
 constexpr float kMargin = 2.0f;            // log2 by which a new reference exceeds the scores seen
 
 // wait-site ids for the status word
-enum { kAMmaK = 0x41, kAMmaV, kAMmaQ, kAMmaO, kAMmaP, kAMmaS, kASoftS, kASoftPv, kASoftP, kASoftEnd, kAConvK, kAConvV, kAConvRaw, kAFetch, kADrain };
+enum { kAMmaK = 0x41, kAMmaV, kAMmaQ, kAMmaO, kAMmaP, kAMmaS, kASoftS, kASoftPv, kASoftEnd, kAConvK, kAConvV, kAConvRaw, kAFetch, kADrain };
 
 template <int D_>
 struct ManyCfg {
@@ -662,9 +662,8 @@ __device__ __forceinline__ void softmax_role(const AttentionParams& p, ManyBars*
             float lo, hi;
             unpair2(f2_add(sum[0], sum[1]), lo, hi);
             l += lo + hi;
-            // this P buffer is free once the PV two blocks back has read it
-            if (n >= 2 && !warp_wait(&bars->pvdone[x][n & 1], ((n - 2) >> 1) & 1, abort_flag, p.status, kASoftP)) return;
-            tc_fence_after();
+            // This P buffer is free: the scores' barrier says that every product issued before
+            // them is done, the PV of two blocks back among them.
             tm_st32(tbase + lane_off + C::TM_P + (x * 2 + (n & 1)) * (kBlk / 2), pk);
             tc_wait_st();
             tc_fence_before();
@@ -868,11 +867,13 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Atte
 }
 
 // Joins the parts of tiles that span CTAs: blockIdx.x leads the tile that begins
-// in CTA blockIdx.x and goes on; blockIdx.y takes kJoinRows of its rows.
-constexpr int kJoinRows = 16;
+// in CTA blockIdx.x and goes on; blockIdx.y takes 32 of its rows, a lane each, and a
+// warp 16 columns, so that a thread's output is one whole sector.  Almost every tile
+// has two parts, whose loads a thread has in flight together.
+constexpr int kJoinRows = 32;
 
 template <class C>
-__global__ void __launch_bounds__(kJoinRows * C::D / 4) attend_many_join_kernel(const AttentionParams p, const int nctas)
+__global__ void __launch_bounds__(kJoinRows * C::D / 16) attend_many_join_kernel(const AttentionParams p, const int nctas)
 {
     pdl_launch_dependents();
     pdl_wait();
@@ -881,14 +882,19 @@ __global__ void __launch_bounds__(kJoinRows * C::D / 4) attend_many_join_kernel(
     const int lead = blockIdx.x;
     Partial rec;
     const int n = find_parts(reinterpret_cast<const Partial*>(p.ws), lead, nctas, rec);
-    const int row = blockIdx.y * kJoinRows + threadIdx.x % kJoinRows, d4 = threadIdx.x / kJoinRows;
+    const int row = blockIdx.y * kJoinRows + lane_id(), d4 = warp_id() * 4;
     if (n == 0 || rec.row0 + row >= rec.rows) return;
     const auto slot = [&](int i) { return 2 * (lead + i) + (i == 0); };
-    const float4 o = join_parts(
+    float4 o[4];
+    join_parts<2>(
         n, [&](int i) { const float* v = ml + slot(i) * 2 * kRows + row; return make_float2(v[0], v[kRows]); },
-        [&](int i) { return po[static_cast<size_t>(slot(i)) * (kRows * C::D / 4) + static_cast<size_t>(d4) * kRows + row]; });
-    *reinterpret_cast<uint2*>(out_row(p, rec.q0, rec.head, rec.row0 + row) + d4 * 4) =
-        make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
+        [&](int i, int v) { return po[static_cast<size_t>(slot(i)) * (kRows * C::D / 4) + static_cast<size_t>(d4 + v) * kRows + row]; },
+        o);
+    uint4* dst = reinterpret_cast<uint4*>(out_row(p, rec.q0, rec.head, rec.row0 + row) + d4 * 4);
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+        dst[v] = make_uint4(pack_bf16(o[2 * v].x, o[2 * v].y), pack_bf16(o[2 * v].z, o[2 * v].w),
+                            pack_bf16(o[2 * v + 1].x, o[2 * v + 1].y), pack_bf16(o[2 * v + 1].z, o[2 * v + 1].w));
 }
 
 template <class C>
@@ -921,7 +927,7 @@ cudaError_t launch_many(const AttentionParams& p, int least, int sms, cudaStream
     e = cudaLaunchKernelEx(&cfg, attend_many_kernel<C>, p, least);
     if (e != cudaSuccess) return e;
     cfg.gridDim = dim3(sms, kRows / kJoinRows);
-    cfg.blockDim = dim3(kJoinRows * C::D / 4);
+    cfg.blockDim = dim3(kJoinRows * C::D / 16);
     cfg.dynamicSmemBytes = 0;
     return cudaLaunchKernelEx(&cfg, attend_many_join_kernel<C>, p, sms);
 }
