@@ -317,6 +317,16 @@ __device__ __forceinline__ uint64_t pair2(float lo, float hi)
     return d;
 }
 
+__device__ __forceinline__ void unpair2(uint64_t v, float& lo, float& hi)
+{
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b)
+{
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 __device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b)
 {
     uint64_t d;
@@ -398,6 +408,14 @@ __device__ __forceinline__ float max_abs_nan(float m, float x)
     return r;
 }
 
+// The largest of m and two magnitudes; a NaN of any wins.
+__device__ __forceinline__ float max_abs_nan(float m, float x, float y)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(fabsf(x)), "f"(fabsf(y)));
+    return r;
+}
+
 // Codes of 4 fp32 values, a byte each: rint(x / s) for |x / s| < 127.5 and a normal
 // s.  y = x * (1 / s) is within 2^-15 of x / s, so rint(y) is the code unless y is
 // within 2^-14 of a half-integer; there the IEEE division decides.  Adding
@@ -405,15 +423,20 @@ __device__ __forceinline__ float max_abs_nan(float m, float x)
 __device__ __forceinline__ uint32_t codes4(const float* x, float s, float rcp)
 {
     constexpr float kMagic = 12582912.0f;
+    const uint64_t magic2 = pair2(kMagic, kMagic), back2 = pair2(-kMagic, -kMagic), minus2 = pair2(-1.0f, -1.0f);
     uint32_t q[4];
-    bool tie = false;
+    float d[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float y = __fmul_rn(x[i], rcp), t = __fadd_rn(y, kMagic);
-        q[i] = __float_as_uint(t);
-        tie = tie || fabsf(__fsub_rn(y, __fsub_rn(t, kMagic))) > 0.49993896484375f;
+    for (int i = 0; i < 4; i += 2) {
+        const uint64_t y = f2_mul(pair2(x[i], x[i + 1]), pair2(rcp, rcp)), t = f2_add(y, magic2);
+        unpair2(f2_fma(f2_add(t, back2), minus2, y), d[i], d[i + 1]);       // y - rint(y), exact
+        float lo, hi;
+        unpair2(t, lo, hi);
+        q[i] = __float_as_uint(lo);
+        q[i + 1] = __float_as_uint(hi);
     }
-    if (tie) {
+    // (a NaN is no tie: its code does not depend on the path)
+    if (fmaxf(fmaxf(fabsf(d[0]), fabsf(d[1])), fmaxf(fabsf(d[2]), fabsf(d[3]))) > 0.49993896484375f) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) q[i] = __float_as_uint(__fadd_rn(__fdiv_rn(x[i], s), kMagic));
     }

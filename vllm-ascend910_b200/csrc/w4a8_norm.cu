@@ -33,10 +33,12 @@ constexpr int kMaxNormThreads = 1024;
 constexpr int kManyRows = 296;             // rows past which a block takes two vectors a thread
 constexpr int kResident = 1024;            // threads per SM that the kernels' 64 registers allow
 
-// 8 bf16 elements from position pos of a row (zeros past K), as they are.
+// 8 bf16 elements from position pos < K of a row (zeros past K), as they are.  WHOLE:
+// rows are 16-byte aligned and K is a multiple of 8.
+template <bool WHOLE>
 __device__ __forceinline__ uint4 load_row8(const uint16_t* row, int pos, int K, bool vec)
 {
-    if (vec && pos + 8 <= K) return *reinterpret_cast<const uint4*>(row + pos);
+    if (WHOLE || (vec && pos + 8 <= K)) return *reinterpret_cast<const uint4*>(row + pos);
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -46,6 +48,18 @@ __device__ __forceinline__ uint4 load_row8(const uint16_t* row, int pos, int K, 
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// Four pairs of fp32 values from 8 bf16 ones, and back.
+__device__ __forceinline__ void unpack_pairs(uint4 v, uint64_t (&x)[4])
+{
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = pair2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+}
+__device__ __forceinline__ void unpair8(const uint64_t (&x)[4], float (&v)[8])
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) unpair2(x[i], v[2 * i], v[2 * i + 1]);
+}
 __device__ __forceinline__ uint4 pack8_bf16(const float (&v)[8])
 {
     uint32_t w[4];
@@ -57,9 +71,12 @@ __device__ __forceinline__ uint4 pack8_bf16(const float (&v)[8])
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-__device__ __forceinline__ void store_row8(uint16_t* row, int pos, int K, bool vec, const float (&v)[8])
+template <bool WHOLE>
+__device__ __forceinline__ void store_row8(uint16_t* row, int pos, int K, bool vec, const uint64_t (&h)[4])
 {
-    if (vec && pos + 8 <= K) {
+    float v[8];
+    unpair8(h, v);
+    if (WHOLE || (vec && pos + 8 <= K)) {
         *reinterpret_cast<uint4*>(row + pos) = pack8_bf16(v);
     } else {
 #pragma unroll
@@ -69,22 +86,22 @@ __device__ __forceinline__ void store_row8(uint16_t* row, int pos, int K, bool v
 }
 
 // The weight's 8 elements from position pos.
-__device__ __forceinline__ void load_weight8(const NormParams& p, int pos, float (&w)[8])
+__device__ __forceinline__ void load_weight8(const NormParams& p, int pos, uint64_t (&w)[4])
 {
     if (p.weight_f32) {
         const float* wf = static_cast<const float*>(p.weight);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = pos + i < p.K ? wf[pos + i] : 0.0f;
+        for (int i = 0; i < 8; i += 2) w[i / 2] = pair2(pos + i < p.K ? wf[pos + i] : 0.0f, pos + i + 1 < p.K ? wf[pos + i + 1] : 0.0f);
     } else {
-        unpack8_bf16(load_row8(static_cast<const uint16_t*>(p.weight), pos, p.K, p.vec_w), w);
+        unpack_pairs(load_row8<false>(static_cast<const uint16_t*>(p.weight), pos, p.K, p.vec_w), w);
     }
 }
 
-template <int OUT, int VPT>
+template <int OUT, int VPT, bool WHOLE>
 __global__ void __launch_bounds__(VPT == 2 ? 512 : kMaxNormThreads, VPT == 2 ? 2 : 1) rms_norm_kernel(const NormParams p)
 {
     __shared__ float red[2][kMaxNormThreads / 32];
-    __shared__ uint32_t red_max[2][VPT][kMaxNormThreads / 32];
+    __shared__ uint32_t red_max[2][VPT * kMaxNormThreads / 32];
 
     // the next kernel may come early where this one leaves room for it
     if (gridDim.x <= 148) pdl_launch_dependents();
@@ -99,39 +116,47 @@ __global__ void __launch_bounds__(VPT == 2 ? 512 : kMaxNormThreads, VPT == 2 ? 2
             xn[j] = make_uint4(0, 0, 0, 0);
             rn[j] = xn[j];
             if (row < p.M && pos < p.K) {          // (the tile form has rows past M: zeros)
-                xn[j] = load_row8(p.x + static_cast<int64_t>(row) * p.ldx, pos, p.K, p.vec_x);
-                if (p.res) rn[j] = load_row8(p.res + static_cast<int64_t>(row) * p.ldr, pos, p.K, p.vec_r);
+                xn[j] = load_row8<WHOLE>(p.x + static_cast<int64_t>(row) * p.ldx, pos, p.K, p.vec_x);
+                if (p.res) rn[j] = load_row8<WHOLE>(p.res + static_cast<int64_t>(row) * p.ldr, pos, p.K, p.vec_r);
             }
         }
     };
     load(blockIdx.x);
     constexpr bool kKeep = VPT <= 2;               // the weight stays in registers
-    float w[kKeep ? VPT : 1][8];
+    uint64_t w[kKeep ? VPT : 1][4];
     if (kKeep)
 #pragma unroll
         for (int j = 0; j < VPT; ++j) load_weight8(p, (j * T + tid) * 8, w[kKeep ? j : 0]);
 
+    // a vector that begins a group: the group, and -1 for the others
+    int leads[VPT];
+    if (OUT != kNormBf16)
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const int pos = (j * T + tid) * 8, g = pos / p.gk;
+            leads[j] = g < p.G && pos - g * p.gk == 0 ? g : -1;
+        }
+
     int flip = 0;
     for (int row = blockIdx.x; row < p.rows; row += gridDim.x, flip ^= 1) {
         const bool real_row = OUT != kNormTiles || row < p.M;
-        float h[VPT][8];
-        float ss = 0.0f;
+        uint64_t h[VPT][4], ss2 = 0;
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
-            float r[8];
-            unpack8_bf16(xn[j], h[j]);
-            unpack8_bf16(rn[j], r);
+            uint64_t r[4];
+            unpack_pairs(xn[j], h[j]);
+            unpack_pairs(rn[j], r);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) h[j][i] = __fadd_rn(h[j][i], r[i]);      // (without a residual, + 0)
+            for (int i = 0; i < 4; ++i) h[j][i] = f2_add(h[j][i], r[i]);         // (without a residual, + 0)
         }
         if (row + static_cast<int>(gridDim.x) < p.rows) load(row + gridDim.x);
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) ss = fmaf(h[j][i], h[j][i], ss);
+            for (int i = 0; i < 4; ++i) ss2 = f2_fma(h[j][i], h[j][i], ss2);
             const int pos = (j * T + tid) * 8;
             if (p.res_out && real_row && pos < p.K)
-                store_row8(p.res_out + static_cast<int64_t>(row) * p.ldro, pos, p.K, p.vec_ro, h[j]);
+                store_row8<WHOLE>(p.res_out + static_cast<int64_t>(row) * p.ldro, pos, p.K, p.vec_ro, h[j]);
         }
 
         // ---- sum of squares over the block; group maxima of |h w| on the way ----
@@ -146,7 +171,11 @@ __global__ void __launch_bounds__(VPT == 2 ? 512 : kMaxNormThreads, VPT == 2 ? 2
                 if (!kKeep) load_weight8(p, (j * T + tid) * 8, w[0]);
                 float a = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) a = max_abs_nan(a, (h[j][i] * 0x1p40f) * w[kKeep ? j : 0][i]);
+                for (int i = 0; i < 4; ++i) {
+                    float lo, hi;
+                    unpair2(f2_mul(f2_mul(h[j][i], pair2(0x1p40f, 0x1p40f)), w[kKeep ? j : 0][i]), lo, hi);
+                    a = max_abs_nan(a, lo, hi);
+                }
                 amax[j] = __float_as_uint(a);          // (as bits, a NaN is the largest)
             }
             for (int o = (tpg < 32 ? tpg : 32) >> 1; o > 0; o >>= 1)
@@ -154,8 +183,11 @@ __global__ void __launch_bounds__(VPT == 2 ? 512 : kMaxNormThreads, VPT == 2 ? 2
                 for (int j = 0; j < VPT; ++j) amax[j] = max(amax[j], __shfl_xor_sync(0xffffffffu, amax[j], o));
             if (tpg > 32 && lane_id() == 0)
 #pragma unroll
-                for (int j = 0; j < VPT; ++j) red_max[flip][j][warp_id()] = amax[j];
+                for (int j = 0; j < VPT; ++j) red_max[flip][j * nw + warp_id()] = amax[j];
         }
+        float ss, ss_odd;
+        unpair2(ss2, ss, ss_odd);
+        ss += ss_odd;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         if (lane_id() == 0) red[flip][warp_id()] = ss;
@@ -169,60 +201,62 @@ __global__ void __launch_bounds__(VPT == 2 ? 512 : kMaxNormThreads, VPT == 2 ? 2
         for (int j = 0; j < VPT; ++j) {
             if (!kKeep) load_weight8(p, (j * T + tid) * 8, w[0]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) h[j][i] = __fmul_rn(__fmul_rn(h[j][i], n), w[kKeep ? j : 0][i]);
+            for (int i = 0; i < 4; ++i) h[j][i] = f2_mul(f2_mul(h[j][i], pair2(n, n)), w[kKeep ? j : 0][i]);
         }
 
         if (OUT == kNormBf16) {
 #pragma unroll
             for (int j = 0; j < VPT; ++j) {
                 const int pos = (j * T + tid) * 8;
-                if (pos < p.K) store_row8(p.y + static_cast<int64_t>(row) * p.ldy, pos, p.K, p.vec_y, h[j]);
+                if (pos < p.K) store_row8<WHOLE>(p.y + static_cast<int64_t>(row) * p.ldy, pos, p.K, p.vec_y, h[j]);
             }
             continue;
         }
 
         if (tpg > 32) {
-            const int w0 = (warp_id() / (tpg >> 5)) * (tpg >> 5);
+            const int wpg = tpg >> 5;                  // warps' worth of vectors in a group
 #pragma unroll
-            for (int j = 0; j < VPT; ++j)
-                for (int k = 0; k < (tpg >> 5); ++k) amax[j] = max(amax[j], red_max[flip][j][w0 + k]);
+            for (int j = 0; j < VPT; ++j) {
+                const int first = static_cast<int>(j * nw + warp_id()) / wpg * wpg, end = min(first + wpg, VPT * nw);
+                for (int k = first; k < end; ++k) amax[j] = max(amax[j], red_max[flip][k]);
+            }
         }
         const float n40 = n * 0x1p-40f;
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             const int pos = (j * T + tid) * 8;
-            const int g = pos / p.gk;
+            float y[8];
+            unpair8(h[j], y);
             const uint16_t sb = act_scale_bits(__uint_as_float(amax[j]) * n40);
             const float s = bf16_bits_to_f32(sb);
             uint2 q;                                   // 8 codes, a byte each
             if (act_scale_fast(sb)) {
                 const float rcp = __frcp_rn(s);
-                q = make_uint2(codes4(h[j], s, rcp), codes4(h[j] + 4, s, rcp));
+                q = make_uint2(codes4(y, s, rcp), codes4(y + 4, s, rcp));
             } else {
                 uint32_t b[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) b[i] = static_cast<uint32_t>(quant_exact(h[j][i], s)) & 0xFFu;
+                for (int i = 0; i < 8; ++i) b[i] = static_cast<uint32_t>(quant_exact(y[i], s)) & 0xFFu;
                 q = make_uint2(b[0] | (b[1] << 8) | (b[2] << 16) | (b[3] << 24), b[4] | (b[5] << 8) | (b[6] << 16) | (b[7] << 24));
             }
-            const bool leader = pos % p.gk == 0;
             if (OUT == kNormTiles) {
                 if (pos < p.kb_total * 256) {
                     *reinterpret_cast<uint2*>(p.aq + gemm_act_tile_offset(row, pos, p.tt, p.kb_total)) =
                         make_uint2(__byte_perm(q.x, q.y, 0x6420), __byte_perm(q.x, q.y, 0x7531));   // k0 k2 k4 k6 | k1 k3 k5 k7
-                    if (leader && g < p.G)
-                        p.as[(static_cast<int64_t>(row / p.tt) * p.G + g) * p.tt + row % p.tt] = real_row ? s : 0.0f;
+                    if (leads[j] >= 0)
+                        p.as[(static_cast<int64_t>(row / p.tt) * p.G + leads[j]) * p.tt + row % p.tt] = real_row ? s : 0.0f;
                 }
             } else if (pos < p.K) {
                 int8_t* qr = p.q + static_cast<int64_t>(row) * p.K;
-                if (pos + 8 <= p.K && p.vec_q) {
+                if (WHOLE || (pos + 8 <= p.K && p.vec_q)) {
                     *reinterpret_cast<uint2*>(qr + pos) = q;
                 } else {
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
                         if (pos + i < p.K) qr[pos + i] = static_cast<int8_t>((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
                 }
-                if (leader) {
-                    const int64_t o = static_cast<int64_t>(g) * p.M + row;
+                if (leads[j] >= 0) {
+                    const int64_t o = static_cast<int64_t>(leads[j]) * p.M + row;
                     if (p.scale_f32) reinterpret_cast<float*>(p.scale)[o] = s;
                     else reinterpret_cast<uint16_t*>(p.scale)[o] = sb;
                 }
@@ -234,6 +268,9 @@ __global__ void __launch_bounds__(VPT == 2 ? 512 : kMaxNormThreads, VPT == 2 ? 2
 template <int OUT, int VPT>
 cudaError_t launch_vpt(const NormParams& p, int threads, cudaStream_t stream)
 {
+    // what the bodies without bounds and alignment tests take
+    const bool whole = p.K % 8 == 0 && p.vec_x && (!p.res || p.vec_r) && (!p.res_out || p.vec_ro) &&
+                       (OUT != kNormBf16 || p.vec_y) && (OUT != kNormCodes || p.vec_q);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(std::min(p.rows, 148 * std::max(1, kResident / threads)));
     cfg.blockDim = dim3(threads);
@@ -243,7 +280,8 @@ cudaError_t launch_vpt(const NormParams& p, int threads, cudaStream_t stream)
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, rms_norm_kernel<OUT, VPT>, p);
+    return whole ? cudaLaunchKernelEx(&cfg, rms_norm_kernel<OUT, VPT, true>, p)
+                 : cudaLaunchKernelEx(&cfg, rms_norm_kernel<OUT, VPT, false>, p);
 }
 
 template <int OUT>
@@ -252,9 +290,7 @@ cudaError_t launch_out(const NormParams& p, cudaStream_t stream)
     // positions to cover: the tile form writes whole k-blocks
     const int span = OUT == kNormTiles ? p.kb_total * 256 : p.K;
     const int nvec = (span + 7) / 8;
-    // threads per row: a multiple of a warp, and of a 1024-element group's 128 threads
-    const int unit = OUT != kNormBf16 && p.gk > 256 ? p.gk / 8 : 32;
-    const auto threads = [&](int vpt) { return ((nvec + vpt - 1) / vpt + unit - 1) / unit * unit; };
+    const auto threads = [&](int vpt) { return ((nvec + vpt - 1) / vpt + 31) / 32 * 32; };
     // One vector a thread is quickest for few rows; for many, two vectors keep more
     // bytes in flight per register (kManyRows below).  Wide rows take what fits.
     const bool one = threads(1) <= kMaxNormThreads;
