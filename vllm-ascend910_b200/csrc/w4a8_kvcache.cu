@@ -201,10 +201,18 @@ __device__ __forceinline__ void rotate_queries(const KvWriteParams& p, int64_t t
     }
 }
 
+// A touched page: the first token, number of tokens and length of its sequence, its
+// number in the sequence and its id (-1: nothing to do).
+struct Job {
+    int64_t t0;
+    int n, len, pg, id;
+};
+
 template <int D, int QT>
 __global__ void __launch_bounds__(kThreads, 4) kv_write_kernel(const KvWriteParams p, const int q_blocks, const int groups)
 {
     __shared__ uint32_t sh_max[kWarps];
+    __shared__ Job sh_job;
 
     const CacheView& cv = p.c;
     const int lane = lane_id(), warp = warp_id();
@@ -218,50 +226,56 @@ __global__ void __launch_bounds__(kThreads, 4) kv_write_kernel(const KvWritePara
         return;
     }
 
-    // ---- one touched page: every warp finds (sequence, page) number `job`, four
+    // ---- one touched page: the first warp finds (sequence, page) number `job`, four
     // sequences a lane ----
     const uint32_t bid = blockIdx.x - static_cast<uint32_t>(qi);
     const int64_t job = bid / static_cast<uint32_t>(groups);
     const int group = static_cast<int>(bid - static_cast<uint32_t>(job) * groups);
-    int s = -1, local = 0;
-    int64_t run = 0;                                         // touched pages before the current 128 sequences
-    for (int base = 0; base < cv.batch && s < 0; base += 128) {
-        int np[4];
-        int64_t sum = 0;
+    if (warp == 0) {
+        int s = -1, local = 0;
+        int64_t run = 0;                                     // touched pages before the current 128 sequences
+        for (int base = 0; base < cv.batch && s < 0; base += 128) {
+            int np[4];
+            int64_t sum = 0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int q = base + lane * 4 + k;
-            np[k] = touched_pages(cv, q);
-            sum += np[k];
-        }
-        int64_t x = sum;
+            for (int k = 0; k < 4; ++k) {
+                const int q = base + lane * 4 + k;
+                np[k] = touched_pages(cv, q);
+                sum += np[k];
+            }
+            int64_t x = sum;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += y;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            const unsigned hit = __ballot_sync(0xffffffffu, run + x > job);
+            if (hit) {
+                int64_t r = job - (run + x - sum);           // the page's number among the lane's sequences
+                int k = 0;
+                while (k < 3 && r >= np[k]) r -= np[k++];
+                const int w = __ffs(hit) - 1;
+                s = base + w * 4 + __shfl_sync(0xffffffffu, k, w);
+                local = __shfl_sync(0xffffffffu, static_cast<int>(r), w);
+            }
+            run += __shfl_sync(0xffffffffu, x, 31);
         }
-        const unsigned hit = __ballot_sync(0xffffffffu, run + x > job);
-        if (hit) {
-            int64_t r = job - (run + x - sum);               // the page's number among the lane's sequences
-            int k = 0;
-            while (k < 3 && r >= np[k]) r -= np[k++];
-            const int w = __ffs(hit) - 1;
-            s = base + w * 4 + __shfl_sync(0xffffffffu, k, w);
-            local = __shfl_sync(0xffffffffu, static_cast<int>(r), w);
+        Job j{0, 0, 0, 0, -1};
+        if (s >= 0) {
+            seq_bounds(cv, s, j.t0, j.n, j.len);
+            j.pg = (max(j.len - j.n, 0) >> cv.page_log2) + local;
+            j.id = cv.table[static_cast<int64_t>(s) * cv.ld_table + j.pg];
         }
-        run += __shfl_sync(0xffffffffu, x, 31);
+        if (lane == 0) sh_job = j;
     }
-    if (s < 0) return;
-    int64_t t0;
-    int n, len;
-    seq_bounds(cv, s, t0, n, len);
+    __syncthreads();
+    const int64_t t0 = sh_job.t0;
+    const int n = sh_job.n, len = sh_job.len, pg = sh_job.pg, id = sh_job.id;
+    if (id < 0 || id >= cv.pages) return;
     const int start = len - n;                               // position of the call's first token (may be < 0)
-    const int pg = (max(start, 0) >> cv.page_log2) + local;
     const int page_at = pg << cv.page_log2;
     const int lo = max(start - page_at, 0);                  // rows [0, lo): earlier tokens
     const int hi = min(len - page_at, cv.page);              // rows [lo, hi): this call's
-    const int id = cv.table[static_cast<int64_t>(s) * cv.ld_table + pg];
-    if (id < 0 || id >= cv.pages) return;
 
     // This warp's item (kv head, K or V) and its chunks of the page's rows: chunk
     // `part`, part + 8, ... where a page has more than eight.
