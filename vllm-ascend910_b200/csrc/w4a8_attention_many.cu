@@ -55,8 +55,13 @@ constexpr int kManyThreads = 16 * 32;      // whole warpgroups: setmaxnreg moves
 constexpr int kConvWarp = 8, kMmaWarp = 12, kFetchWarp = 14;
 constexpr int kRegsSoft = 176, kRegsRest = 80;      // 2 warpgroups of each
 static_assert(2 * kRegsSoft + 2 * kRegsRest <= 4 * 128, "the launch allocates 128 registers a thread");
-constexpr int kTileUnits = 6;              // what beginning and ending a tile costs, in blocks (work shares)
-constexpr int kMinUnits = 4;               // a CTA's share is not cut below this
+// What beginning and ending a tile costs, in blocks (work shares).  Three prompts of 1,200
+// to 2,000 behind 1,300: 264, 235 and 232 us with 3, 6 and 9; one of 2,048: 95, 81 and 82;
+// four times 64 tokens behind 1,000: 30.2, 30.7 and 32.7.
+constexpr int kTileUnits = 6;
+// A CTA's share is not cut below this.  A prompt of 100: 16.3, 16.8, 17.6 and 24.2 us with 1, 2,
+// 4 and 8; 100 tokens behind 400: 21.6, 20.1 and 21.4 with 1, 2 and 4.
+constexpr int kMinUnits = 2;
 constexpr float kMargin = 2.0f;            // log2 by which a new reference exceeds the scores seen
 
 // wait-site ids for the status word

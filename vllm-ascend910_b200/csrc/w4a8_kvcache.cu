@@ -39,6 +39,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+// Tokens whose query heads a block turns.  One a block: 4.3, 7.2 and 37 us for 64, 512 and
+// 4,096 tokens of 40 + 8 + 8 heads of 128; four: 4.2, 5.6 and 30.
+constexpr int kQTok = 4;
 __host__ __device__ constexpr int chunk_rows(int D) { return 512 / D; }   // rows that a warp holds: 16 elements a lane
 
 __device__ __forceinline__ void rotate_pair(float& a, float& b, float c, float s)
@@ -155,25 +158,25 @@ __device__ __forceinline__ int touched_pages(const CacheView& cv, int s)
     return s < cv.batch && len > lo ? ((len - 1) >> cv.page_log2) - (lo >> cv.page_log2) + 1 : 0;
 }
 
-// Query heads of QT tokens.
-template <int D, int QT>
+// Query heads of kQTok tokens.
+template <int D>
 __device__ __forceinline__ void rotate_queries(const KvWriteParams& p, int64_t t0)
 {
     constexpr int LPH = D / 16;                          // threads of a head
     const CacheView& cv = p.c;
     const int j = threadIdx.x % LPH, slot = threadIdx.x / LPH;
-    const int64_t t = t0 + slot % QT;
+    const int64_t t = t0 + slot % kQTok;
     const int s = p.rot ? seq_of(cv.cu, cv.batch, t0, min(t, cv.tokens - 1)) : 0;
     if (t >= cv.tokens) return;
     int c0, c1;
     item_cols(j, p.rot, p.interleaved, c0, c1);
     // the first heads' elements are on their way while the token's angles are found
-    constexpr int STEP = kThreads / LPH / QT, AHEAD = 4;
+    constexpr int STEP = kThreads / LPH / kQTok, AHEAD = 4;
     const uint16_t* src = p.q + t * p.ldq;
     uint16_t* dst = p.q_out + t * p.ldqo;
     const bool turn = j < p.rot / 16;
     float4 cs[4] = {};
-    for (int h0 = slot / QT; h0 < p.q_heads; h0 += AHEAD * STEP) {
+    for (int h0 = slot / kQTok; h0 < p.q_heads; h0 += AHEAD * STEP) {
         uint4 w[AHEAD][2];
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
@@ -181,7 +184,7 @@ __device__ __forceinline__ void rotate_queries(const KvWriteParams& p, int64_t t
             w[k][0] = *reinterpret_cast<const uint4*>(src + h * D + c0);
             w[k][1] = *reinterpret_cast<const uint4*>(src + h * D + c1);
         }
-        if (turn && h0 == slot / QT) {
+        if (turn && h0 == slot / kQTok) {
             int64_t first;
             int n, len;
             seq_bounds(cv, s, first, n, len);
@@ -208,7 +211,7 @@ struct Job {
     int n, len, pg, id;
 };
 
-template <int D, int QT>
+template <int D>
 __global__ void __launch_bounds__(kThreads, 4) kv_write_kernel(const KvWriteParams p, const int q_blocks, const int groups)
 {
     __shared__ uint32_t sh_max[kWarps];
@@ -222,7 +225,7 @@ __global__ void __launch_bounds__(kThreads, 4) kv_write_kernel(const KvWritePara
     // proportion, so that both kinds are resident together.
     const int64_t qi = static_cast<int64_t>(blockIdx.x) * q_blocks / gridDim.x;
     if ((static_cast<int64_t>(blockIdx.x) + 1) * q_blocks / gridDim.x > qi) {
-        rotate_queries<D, QT>(p, qi * QT);
+        rotate_queries<D>(p, qi * kQTok);
         return;
     }
 
@@ -442,11 +445,7 @@ cudaError_t launch(Kern kern, int64_t blocks, cudaStream_t stream, const Args&..
 
 cudaError_t launch_kv_write(const KvWriteParams& p, cudaStream_t stream)
 {
-    // One token a block while there are few (a decode step), four when blocks are
-    // plenty: B200, 8.2k tokens of 40 heads, four is faster than one.
-    const bool few = p.c.tokens <= 1024;
-    const int qt = few ? 1 : 4;
-    const int64_t q_blocks = p.q ? (p.c.tokens + qt - 1) / qt : 0;
+    const int64_t q_blocks = p.q ? (p.c.tokens + kQTok - 1) / kQTok : 0;
     // n tokens of a sequence touch at most n pages, and at most (n - 1) / page + 2
     const int64_t jobs = std::min<int64_t>(p.c.tokens, p.c.tokens / p.c.page + 2 * static_cast<int64_t>(p.c.batch));
     const int per_block = kWarps / std::min(p.c.page / chunk_rows(p.c.D), kWarps);       // items
@@ -454,11 +453,8 @@ cudaError_t launch_kv_write(const KvWriteParams& p, cudaStream_t stream)
     const int64_t blocks = q_blocks + jobs * groups;
     if (blocks > 0x7FFFFFFF) return cudaErrorInvalidValue;
     const int qb = static_cast<int>(q_blocks);
-    if (p.c.D == 128)
-        return few ? launch(kv_write_kernel<128, 1>, blocks, stream, p, qb, groups)
-                   : launch(kv_write_kernel<128, 4>, blocks, stream, p, qb, groups);
-    return few ? launch(kv_write_kernel<64, 1>, blocks, stream, p, qb, groups)
-               : launch(kv_write_kernel<64, 4>, blocks, stream, p, qb, groups);
+    return p.c.D == 128 ? launch(kv_write_kernel<128>, blocks, stream, p, qb, groups)
+                        : launch(kv_write_kernel<64>, blocks, stream, p, qb, groups);
 }
 
 cudaError_t launch_kv_read(const KvReadParams& p, cudaStream_t stream)
