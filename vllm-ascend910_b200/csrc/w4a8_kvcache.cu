@@ -23,11 +23,17 @@
 // heads it turns.  The other blocks own eight warps' worth of one touched page's
 // (kv head, K or V) items: a warp holds 4 rows of 128 elements in registers (a page
 // of 32 rows is eight warps), so k and v are read once -- rotated, their maximum found, and
-// written as codes.  All loads of a warp are in flight together; short chains of
-// dependent loads, not bandwidth, set the time until thousands of blocks run.  Dividing by the scale is a product with its reciprocal
-// except next to half-integers, where the true division decides (the activation
-// quantiser's rule).  Bound by HBM for prompts: q is read and written, k and v
-// read, a byte per element written.
+// written as codes.  All loads of a warp are in flight together, and four blocks an SM
+// (64 registers) hide more than three or five do: 7,584 tokens 53 us against 58 and 69.
+// A loop over several items a block was slower too (68 us).  Dividing by the scale is a
+// product with its reciprocal except next to half-integers, where the true division
+// decides (the activation quantiser's rule).
+//
+// Measured (B200): 7,584 tokens of 40 + 8 + 8 heads of 128, pages of 32: write 53 us, of
+// which the queries' 155 MB alone take 24 at the memory's rate and the pages, by a chain of
+// dependent loads (lengths, page id, rows, scale) in each of 3,800 blocks, 30; read back
+// 11 us (47 MB).  One token of 64 sequences: 5.4 us written, 5.8 us with 4,200 tokens read
+// back: launch and latency.
 #include <algorithm>
 
 #include "w4a8_common.cuh"
@@ -211,7 +217,7 @@ struct Job {
     int n, len, pg, id;
 };
 
-template <int D>
+template <int D, bool ONE>
 __global__ void __launch_bounds__(kThreads, 4) kv_write_kernel(const KvWriteParams p, const int q_blocks, const int groups)
 {
     __shared__ uint32_t sh_max[kWarps];
@@ -321,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, 4) kv_write_kernel(const KvWritePara
     float big = 0.0f;
     const int chunks = cv.page / CHUNK;
     int held = part;
-    for (int c = part; c < chunks; c += wpi) {
+    for (int c = part; c < chunks; c += ONE ? 1 << 20 : wpi) {
         load(c);
         held = c;
 #pragma unroll
@@ -354,8 +360,8 @@ __global__ void __launch_bounds__(kThreads, 4) kv_write_kernel(const KvWritePara
     }
     const bool fast = now >= 1.1754943508222875e-38f && now < INFINITY;
     const float rcp = fast ? __frcp_rn(now) : 0.0f;
-    for (int c = held; c >= 0; c -= wpi) {
-        if (c != held) load(c);
+    for (int c = held; c >= 0; c -= ONE ? 1 << 20 : wpi) {
+        if (!ONE && c != held) load(c);
         const int row = c * CHUNK + sub;
         if (row < lo || row >= hi) continue;
         int8_t* d = codes + row * D;
@@ -453,8 +459,14 @@ cudaError_t launch_kv_write(const KvWriteParams& p, cudaStream_t stream)
     const int64_t blocks = q_blocks + jobs * groups;
     if (blocks > 0x7FFFFFFF) return cudaErrorInvalidValue;
     const int qb = static_cast<int>(q_blocks);
-    return p.c.D == 128 ? launch(kv_write_kernel<128>, blocks, stream, p, qb, groups)
-                        : launch(kv_write_kernel<64>, blocks, stream, p, qb, groups);
+    // Pages that eight warps hold (up to 32 rows of 128 or 64 of 64) need no loop over
+    // chunks: without it 7,584 tokens in pages of 32 take 53 us, with it 57.
+    const bool one = p.c.page / chunk_rows(p.c.D) <= kWarps;
+    if (p.c.D == 128)
+        return one ? launch(kv_write_kernel<128, true>, blocks, stream, p, qb, groups)
+                   : launch(kv_write_kernel<128, false>, blocks, stream, p, qb, groups);
+    return one ? launch(kv_write_kernel<64, true>, blocks, stream, p, qb, groups)
+               : launch(kv_write_kernel<64, false>, blocks, stream, p, qb, groups);
 }
 
 cudaError_t launch_kv_read(const KvReadParams& p, cudaStream_t stream)
