@@ -32,8 +32,8 @@
 // Measured (B200): 7,584 tokens of 40 + 8 + 8 heads of 128, pages of 32: write 53 us, of
 // which the queries' 155 MB alone take 24 at the memory's rate and the pages, by a chain of
 // dependent loads (lengths, page id, rows, scale) in each of 3,800 blocks, 30; read back
-// 11 us (47 MB).  One token of 64 sequences: 5.4 us written, 5.8 us with 4,200 tokens read
-// back: launch and latency.
+// 9 us (47 MB).  One token of 64 sequences written: 5.4 us; 530 tokens read back: 2.9 us:
+// launch and latency.
 #include <algorithm>
 
 #include "w4a8_common.cuh"
@@ -377,20 +377,20 @@ __global__ void __launch_bounds__(kThreads, 4) kv_write_kernel(const KvWritePara
 
 // ------------------------------------------------------------------ reading back
 
-constexpr int kRTok = 16;          // tokens of one block
+constexpr int kRTok = 16;          // most tokens of one block
 
 // bf16(code * scale) of each sequence's last cu[s + 1] - cu[s] tokens.  A token
 // without a page (or before position 0) reads as zeros.
-__global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvReadParams p)
+__global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvReadParams p, const int per)
 {
     __shared__ int64_t sh_ph[kRTok];       // page * kv_heads, or -1
     __shared__ int sh_row[kRTok];
     const CacheView& cv = p.c;
     pdl_wait();
-    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * kRTok;
+    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * per;
     const int tid = threadIdx.x;
-    const int s = tid < 32 ? seq_of(cv.cu, cv.batch, t0, min(t0 + min(tid, kRTok - 1), cv.tokens - 1)) : 0;
-    if (tid < kRTok && t0 + tid < cv.tokens) {
+    const int s = tid < 32 ? seq_of(cv.cu, cv.batch, t0, min(t0 + min(tid, per - 1), cv.tokens - 1)) : 0;
+    if (tid < per && t0 + tid < cv.tokens) {
         int64_t first;
         int n, len;
         seq_bounds(cv, s, first, n, len);
@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvReadParams p)
     }
     __syncthreads();
     const int per_head = cv.D / 16, per_tok = cv.kv_heads * per_head;
-    const int n = static_cast<int>(min(static_cast<int64_t>(kRTok), cv.tokens - t0)) * per_tok;
+    const int n = static_cast<int>(min(static_cast<int64_t>(per), cv.tokens - t0)) * per_tok;
     for (int i = tid; i < n; i += kThreads) {
         const int k = i / per_tok, rest = i - k * per_tok;
         const int h = rest / per_head, j = rest - h * per_head;
@@ -471,7 +471,11 @@ cudaError_t launch_kv_write(const KvWriteParams& p, cudaStream_t stream)
 
 cudaError_t launch_kv_read(const KvReadParams& p, cudaStream_t stream)
 {
-    return launch(kv_read_kernel, (p.c.tokens + kRTok - 1) / kRTok, stream, p);
+    // As many tokens a block as give each thread one vector.  8 heads of 128: 2.9 and 9.1 us
+    // for 530 and 7,584 tokens by four a block, 5.4 and 10.8 by sixteen, 2.8 and 12.4 by one;
+    // one head of 128: 3.0 us for 7,584 by sixteen, 4.3 by four.
+    const int per = std::max(1, std::min(kRTok, kThreads / (p.c.kv_heads * p.c.D / 16)));
+    return launch(kv_read_kernel, (p.c.tokens + per - 1) / per, stream, p, per);
 }
 
 }  // namespace w4a8
