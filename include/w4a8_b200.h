@@ -325,10 +325,13 @@ W4A8_API int w4a8_kv_read(const w4a8_kv_cache* cache, const int32_t* page_table,
  * tokens j at or before query token t's position, k and v of kv head
  * h / (q_heads / kv_heads); a row that sees no token is zero.  q, out bf16
  * [tokens, ld] (q_heads * head_dim used; rows 16-byte aligned, ld a multiple of
- * 8).  softmax_scale >= 0.  max_q_len: no sequence has more query tokens than that (rows past it
- * are not computed).  batch <= W4A8_ATTENTION_MAX_BATCH.  Workspace as for the
- * linear calls (w4a8_attention_workspace_size bytes, 1024-byte aligned, zeroed
- * before first use, may be shared with them in stream order). */
+ * 8); rows of q that cu gives to no sequence are left unwritten in out.
+ * softmax_scale >= 0.  max_q_len is the longest cu[s + 1] - cu[s]: it chooses the
+ * kernel and the workspace's size, and a call whose sequences are longer is slower,
+ * not wrong.  batch <= W4A8_ATTENTION_MAX_BATCH, tokens * (q_heads / kv_heads) <=
+ * 0x7FFF0000, cache->pages > 0.  Workspace as for the linear calls
+ * (w4a8_attention_workspace_size bytes, 1024-byte aligned, zeroed before first use,
+ * may be shared with them in stream order). */
 #define W4A8_ATTENTION_MAX_BATCH 2048
 W4A8_API size_t w4a8_attention_workspace_size(int64_t batch, int64_t tokens, int32_t q_heads, int32_t kv_heads,
                                               int32_t head_dim, int32_t max_q_len);

@@ -13,12 +13,17 @@
 // Roles (one CTA per SM):
 //   warps 0-3, 4-7   softmax of half A, B: row maximum, exponentials, weights, sum;
 //                    their rows' queries to fp16 in smem, and the output rows
-//   warps 8-11       converters: cache codes by 16-byte loads (one block ahead in
-//                    registers), exact fp16 into the swizzled operand layout
-//   warps 12, 13     issue the MMAs of half A, B (warps 14, 15 fill the warpgroup)
+//   warps 8-11       converters: a block's codes from smem, exact fp16 into the
+//                    swizzled operand layout
+//   warps 12, 13     issue the MMAs of half A, B
+//   warp 14          fetches: bulk copies of codes three blocks ahead, page scales
+//                    (warp 15 fills the warpgroup)
 // One issuer for both halves was measured first: its chain of waits and commits
 // (about 100 cycles each) set the pace at 1,900 cycles a block with all other work
-// taken out.
+// taken out.  Converters that loaded codes into registers themselves, one block
+// ahead, were the pace at 3,200 cycles a block of a prompt of 8,192 tokens (latency
+// of loads, addresses and shuffles beside the conversion); fed from smem it is the
+// softmax's, 2,400.
 // TMEM holds S of each half (64 columns), two P of each half (32 columns) and O (D
 // columns).  S is free as soon as the softmax has it in registers, so Q K^T of block
 // j + 1 runs while the softmax of block j works; P of a block is kept until its PV
@@ -27,16 +32,25 @@
 //
 // The reference maximum of a row moves only when a block exceeds it by more than
 // 2^1.9 (weights stay below 2^15.9, inside fp16), and then to 2^2 above what was
-// seen: a rescale of O in TMEM is rare instead of once a block, at the price of
-// two of the 28 binades below the largest weight that keep all 11 bits.
+// seen: a rescale of O in TMEM is rare instead of once a block (35 in 547 blocks of
+// random data), at the price of two of the 28 binades below the largest weight that
+// keep all 11 bits.  Exponentials by the old reference beside the maximum, done again
+// where it has to move, were no faster (227 against 219 us for three prompts).
 //
 // Work: units of (row tile, 64-token block), causally pruned, and a few for each
 // tile's beginning and end, in one list; every CTA takes an equal contiguous
-// share, so chunks over long contexts and mixed batches fill the machine alike.  Tiles split between CTAs leave fp32 parts that
-// attend_many_join_kernel adds in order.
+// share, so chunks over long contexts and mixed batches fill the machine alike.  Tiles
+// split between CTAs leave fp32 parts that attend_many_join_kernel adds in order (a
+// join by the last CTA to finish, as attend_few_kernel does, was slower for long
+// prompts: 733 against 807 TFLOP/s at 8,192 tokens).
 //
 // Bounds per 256 x 64 step at D = 128: 1024 tensor cycles, 1024 cycles of the
-// exponential unit (16 / clock / SM), about 760 issue slots per scheduler.
+// exponential unit (16 / clock / SM), about 1,500 cycles of shared memory (128 KB of
+// operands, 64 KB of codes and their conversion), about 1,200 issue slots per scheduler.
+// Measured (B200, 40 query heads on 8 of 128): 2,400 cycles a step, and 12,000 for a
+// tile's queries and output; three prompts of 900-2,048 tokens behind up to 2,048 193 us,
+// 638 TFLOP/s; one prompt of 2,048, 4,096 and 8,192 tokens 82, 237 and 813 us, 524, 726 and
+// 845 TFLOP/s, the last at 1,810 MHz: it reaches the board's power limit.
 #include <algorithm>
 
 #include "w4a8_attention.cuh"
