@@ -22,8 +22,7 @@
 // fp32 arithmetic runs in pairs, two elements an instruction; each rounds alone.
 //
 // Measured (B200, rows of 5120 with a residual): 4096 rows, bf16 out 27.5 us, 6.1 TB/s, 93 %
-// of a plain copy's rate; 8191 rows with codes 62 us in groups of 128 and 72.5 us in groups
-// of 1024, 4.8 and 4.0 TB/s: about 300 instructions a thread and row bound it, not the
+// of a plain copy's rate; 8191 rows with codes 62 us in groups of 128 or 1024, 4.7 TB/s: about 650 instructions for a thread's 16 elements bound it, not the
 // memory (before the pairs and the bodies without bounds tests 75 and 96 us).  One row: 1.9
 // us, launch and two load latencies.
 #include <algorithm>
@@ -110,7 +109,7 @@ template <int OUT, int VPT, bool WHOLE>
 __global__ void __launch_bounds__(VPT == 2 ? 512 : kMaxNormThreads, VPT == 2 ? 2 : 1) rms_norm_kernel(const NormParams p)
 {
     __shared__ float red[2][kMaxNormThreads / 32];
-    __shared__ uint32_t red_max[2][VPT * kMaxNormThreads / 32];
+    __shared__ __align__(16) uint32_t red_max[2][VPT * kMaxNormThreads / 32];
 
     // the next kernel may come early where this one leaves room for it
     if (gridDim.x <= 148) pdl_launch_dependents();
@@ -136,6 +135,10 @@ __global__ void __launch_bounds__(VPT == 2 ? 512 : kMaxNormThreads, VPT == 2 ? 2
     if (kKeep)
 #pragma unroll
         for (int j = 0; j < VPT; ++j) load_weight8(p, (j * T + tid) * 8, w[kKeep ? j : 0]);
+
+    // (the last group's warps may be fewer than four)
+    if (OUT != kNormBf16 && p.gk == 1024 && tid < 4 && VPT * nw + tid < VPT * kMaxNormThreads / 32)
+        red_max[0][VPT * nw + tid] = red_max[1][VPT * nw + tid] = 0;
 
     // a vector that begins a group: the group, and -1 for the others
     int leads[VPT];
@@ -190,7 +193,7 @@ __global__ void __launch_bounds__(VPT == 2 ? 512 : kMaxNormThreads, VPT == 2 ? 2
             for (int o = (tpg < 32 ? tpg : 32) >> 1; o > 0; o >>= 1)
 #pragma unroll
                 for (int j = 0; j < VPT; ++j) amax[j] = max(amax[j], __shfl_xor_sync(0xffffffffu, amax[j], o));
-            if (tpg > 32 && lane_id() == 0)
+            if (p.gk == 1024 && lane_id() == 0)
 #pragma unroll
                 for (int j = 0; j < VPT; ++j) red_max[flip][j * nw + warp_id()] = amax[j];
         }
@@ -222,12 +225,11 @@ __global__ void __launch_bounds__(VPT == 2 ? 512 : kMaxNormThreads, VPT == 2 ? 2
             continue;
         }
 
-        if (tpg > 32) {
-            const int wpg = tpg >> 5;                  // warps' worth of vectors in a group
+        if (p.gk == 1024) {
 #pragma unroll
-            for (int j = 0; j < VPT; ++j) {
-                const int first = static_cast<int>(j * nw + warp_id()) / wpg * wpg, end = min(first + wpg, VPT * nw);
-                for (int k = first; k < end; ++k) amax[j] = max(amax[j], red_max[flip][k]);
+            for (int j = 0; j < VPT; ++j) {            // a group of 1024 is four warps' vectors
+                const uint4 m = *reinterpret_cast<const uint4*>(&red_max[flip][(j * nw + warp_id()) & ~3u]);
+                amax[j] = max(max(m.x, m.y), max(m.z, m.w));
             }
         }
         const float n40 = n * 0x1p-40f;
