@@ -238,18 +238,19 @@ def test_repeats_streams_and_graphs(qs, lens):
     del g
 
 
-def test_cache_past_32_bits():
+@pytest.mark.parametrize("qs", [[1, 2], [90, 1]])
+def test_cache_past_32_bits(qs):
     """Pages whose byte offset does not fit 32 bits."""
     from w4a8_b200 import kvcache
     dev = _dev()
     P, H, page, D = (1 << 31) // (8 * 16 * 128) + 40, 8, 16, 128
     cache = kvcache.KVCache.empty(P, H, page, D, dev)
-    small = Case(40, 8, 128, 16, [1, 2], [100, 250], seed=11)
+    small = Case(40, 8, 128, 16, qs, [100, 250], seed=11)
     shift = P - small.P
     for dst, src in zip((cache.k, cache.v, cache.k_scale, cache.v_scale), small.codes + small.scales):
         dst[shift:].copy_(src)
     table, kl, cu = small.batch()
-    out = kvcache.attention(small.q.to(dev), cache, table + shift, kl, cu, 2)
+    out = kvcache.attention(small.q.to(dev), cache, table + shift, kl, cu, max(qs))
     small.check(out)
     assert shift * H * page * D > 1 << 31
 

@@ -34,7 +34,7 @@ def _close(got, want, name):
     assert over.max() <= 1e-37, (name, over.max())
 
 
-SHAPES = [(1, 5120), (3, 1), (2, 7), (5, 33), (17, 1057), (64, 5120), (9, 8200), (2, 27648), (1, 32768), (300, 256)]
+SHAPES = [(1, 5120), (3, 1), (2, 7), (5, 33), (17, 1057), (64, 5120), (9, 8200), (2, 27648), (1, 32768), (300, 256), (1000, 5120), (500, 1057)]
 
 
 @pytest.mark.parametrize("M,K", SHAPES)
@@ -53,7 +53,10 @@ def test_bf16_output(M, K, residual, wdtype):
 
 
 @pytest.mark.parametrize("M,K,gk", [(1, 5120, 128), (4, 5120, 1024), (3, 1057, 1024), (65, 256, 64), (2, 33, 64),
-                                    (7, 1000, 256), (2, 27648, 128), (5, 12288, 1024), (1, 20000, 1024)])
+                                    (7, 1000, 256), (2, 27648, 128), (5, 12288, 1024), (1, 20000, 1024),
+                                    # blocks that stay for several rows; groups that end inside a warp's vectors
+                                    (600, 1288, 1024), (900, 5120, 1024), (470, 1057, 1024), (700, 2120, 256),
+                                    (1000, 640, 64), (460, 9000, 1024)])
 @pytest.mark.parametrize("sdt", [torch.bfloat16, torch.float32])
 def test_8_bit_output(M, K, gk, sdt):
     from w4a8_b200 import ops
@@ -125,7 +128,7 @@ def test_in_place_strides_and_leading_dimensions():
 
 
 @pytest.mark.parametrize("M,N,K,gk", [(1, 256, 1024, 128), (16, 512, 640, 64), (33, 256, 5120, 256), (100, 384, 1057, 1024),
-                                      (200, 256, 512, 128)])
+                                      (200, 256, 512, 128), (600, 256, 1288, 1024)])
 def test_linear_on_the_norm(M, N, K, gk):
     """The norm-fed linear equals the GEMM on rms_norm_quant's codes bit for bit (the int4-plane entry
     point takes codes as they are)."""
