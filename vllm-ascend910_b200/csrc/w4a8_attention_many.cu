@@ -524,36 +524,38 @@ __device__ __forceinline__ void softmax_role(const AttentionParams& p, ManyBars*
 
         // ---- this warp's 32 queries into the operand: rows come by asynchronous copies
         // (RPI rows a turn, a lane per 16 bytes), then a lane is a row: its largest
-        // element to [2^13, 2^14), fp16, in place.  Short loops: a tile passes here once ----
+        // element to [2^13, 2^14), fp16, in place ----
         float qs = 0.0f;                                        // what turns a raw score into log2 units
         const int limit = valid ? a.s.len - a.s.n + row_token(p, pr) : 0x7FFFFFFF;   // last token the row sees
         {
+            // (a lane finds its own row's place; the lanes that copy the row are told)
+            const int tok = valid ? row_token(p, pr) : 0;
+            const int64_t place = static_cast<int64_t>(a.s.q0 + tok) * p.ldq +
+                                  static_cast<int64_t>(a.head * p.group + (valid ? pr - tok * p.group : 0)) * C::D;
             const int sub = lane / LPR, ch = lane % LPR;
-#pragma unroll 2
+#pragma unroll 4
             for (int i = 0; i < 32 / RPI; ++i) {
-                const int rr = (row & 96) + i * RPI + sub, r = pr - lane + i * RPI + sub;
-                const bool ok = r < a.s.n * p.group;
-                const int tok = ok ? row_token(p, r) : 0;
-                const uint16_t* src = p.q + static_cast<int64_t>(a.s.q0 + tok) * p.ldq +
-                                      static_cast<int64_t>(a.head * p.group + (ok ? r - tok * p.group : 0)) * C::D + ch * 8;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(q_unit(rr, ch)), "l"(src), "r"(ok ? 16 : 0)
+                const int rr = i * RPI + sub;
+                const uint16_t* src = p.q + __shfl_sync(0xffffffffu, place, rr) + ch * 8;
+                const bool ok = pr - lane + rr < a.s.n * p.group;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(q_unit((row & 96) + rr, ch)), "l"(src), "r"(ok ? 16 : 0)
                              : "memory");
             }
             asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
             __syncwarp();
             uint32_t big = 0;
-#pragma unroll 4
+            uint4 v[LPR];
+#pragma unroll
             for (int u = 0; u < LPR; ++u) {
-                const uint4 v = lds128(q_unit(row, u));
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                v[u] = lds128(q_unit(row, u));
+                const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) big = max(big, max((w[e] << 16) & 0x7FFFFFFFu, w[e] & 0x7FFF0000u));
             }
             const float shrink = row_shrink(__uint_as_float(big));
-#pragma unroll 4
+#pragma unroll
             for (int u = 0; u < LPR; ++u) {
-                const uint4 v = lds128(q_unit(row, u));
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
                 uint32_t h[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
@@ -713,12 +715,15 @@ __device__ __forceinline__ void softmax_role(const AttentionParams& p, ManyBars*
             }
             if (whole) {
                 __syncwarp();
-                const int sub = lane / LPR, ch = lane % LPR;
+                const int sub = lane / LPR, ch = lane % LPR, tok = valid ? row_token(p, pr) : 0;
+                const int64_t place = static_cast<int64_t>(a.s.q0 + tok) * p.ldo +
+                                      static_cast<int64_t>(a.head * p.group + (valid ? pr - tok * p.group : 0)) * C::D;
 #pragma unroll 4
                 for (int i = 0; i < 32 / RPI; ++i) {
-                    const int rr = (row & 96) + i * RPI + sub, r = pr - lane + i * RPI + sub;
-                    const uint4 v = lds128(q_unit(rr, ch));
-                    if (r < a.s.n * p.group) *reinterpret_cast<uint4*>(out_row(p, a.s.q0, a.head, r) + ch * 8) = v;
+                    const int rr = i * RPI + sub;
+                    const int64_t to = __shfl_sync(0xffffffffu, place, rr);
+                    const uint4 v = lds128(q_unit((row & 96) + rr, ch));
+                    if (pr - lane + rr < a.s.n * p.group) *reinterpret_cast<uint4*>(p.out + to + ch * 8) = v;
                 }
                 __syncwarp();
             }
