@@ -67,7 +67,7 @@ static_assert(kNR <= kNS, "the fetching warp arrives on a K stage's barrier for 
 constexpr int kScaleRing = 16;             // blocks whose page scales are kept
 constexpr int kManyThreads = 16 * 32;      // whole warpgroups: setmaxnreg moves registers between them
 constexpr int kConvWarp = 8, kMmaWarp = 12, kFetchWarp = 14;
-constexpr int kRegsSoft = 176, kRegsRest = 80;      // 2 warpgroups of each
+constexpr int kRegsSoft = 184, kRegsRest = 72;      // 2 warpgroups of each
 static_assert(2 * kRegsSoft + 2 * kRegsRest <= 4 * 128, "the launch allocates 128 registers a thread");
 // What beginning and ending a tile costs, in blocks (work shares).  Three prompts of 1,200
 // to 2,000 behind 1,300: 264, 235 and 232 us with 3, 6 and 9; one of 2,048: 95, 81 and 82;

@@ -210,11 +210,11 @@ __device__ __forceinline__ void rotate_queries(const KvWriteParams& p, int64_t t
     }
 }
 
-// A touched page: the first token, number of tokens and length of its sequence, its
-// number in the sequence and its id (-1: nothing to do).
+// A touched page: its sequence (-1: nothing to do), the sequence's first token, number
+// of tokens and length, and the page's number in it.
 struct Job {
     int64_t t0;
-    int n, len, pg, id;
+    int s, n, len, pg;
 };
 
 template <int D, bool ONE>
@@ -269,18 +269,18 @@ __global__ void __launch_bounds__(kThreads, 4) kv_write_kernel(const KvWritePara
             }
             run += __shfl_sync(0xffffffffu, x, 31);
         }
-        Job j{0, 0, 0, 0, -1};
+        Job j{0, s, 0, 0, 0};
         if (s >= 0) {
             seq_bounds(cv, s, j.t0, j.n, j.len);
             j.pg = (max(j.len - j.n, 0) >> cv.page_log2) + local;
-            j.id = cv.table[static_cast<int64_t>(s) * cv.ld_table + j.pg];
         }
         if (lane == 0) sh_job = j;
     }
     __syncthreads();
     const int64_t t0 = sh_job.t0;
-    const int n = sh_job.n, len = sh_job.len, pg = sh_job.pg, id = sh_job.id;
-    if (id < 0 || id >= cv.pages) return;
+    const int n = sh_job.n, len = sh_job.len, pg = sh_job.pg;
+    if (sh_job.s < 0) return;
+    const int id = cv.table[static_cast<int64_t>(sh_job.s) * cv.ld_table + pg];     // (the rows' loads do not wait for it)
     const int start = len - n;                               // position of the call's first token (may be < 0)
     const int page_at = pg << cv.page_log2;
     const int lo = max(start - page_at, 0);                  // rows [0, lo): earlier tokens
@@ -295,9 +295,6 @@ __global__ void __launch_bounds__(kThreads, 4) kv_write_kernel(const KvWritePara
     const bool on = item < 2 * cv.kv_heads;
     const bool is_v = on && item >= cv.kv_heads;
     const int h = !on ? 0 : is_v ? item - cv.kv_heads : item;
-    const int64_t ph = static_cast<int64_t>(id) * cv.kv_heads + h;
-    int8_t* codes = (is_v ? cv.v : cv.k) + (ph << cv.page_log2) * D;
-    float* scale = (is_v ? cv.v_scale : cv.k_scale) + ph;
     const int64_t ld = is_v ? p.ldv : p.ldk;
     const uint16_t* src = (is_v ? p.v : p.k) + (t0 - start + page_at) * ld + static_cast<int64_t>(h) * D;   // of row 0
     const int rot = is_v ? 0 : p.rot;
@@ -333,6 +330,10 @@ __global__ void __launch_bounds__(kThreads, 4) kv_write_kernel(const KvWritePara
 #pragma unroll
         for (int e = 0; e < 16; ++e) big = max_abs_nan(big, v[e]);
     }
+    if (id < 0 || id >= cv.pages) return;                    // (the whole block's page)
+    const int64_t ph = static_cast<int64_t>(id) * cv.kv_heads + h;
+    int8_t* codes = (is_v ? cv.v : cv.k) + (ph << cv.page_log2) * D;
+    float* scale = (is_v ? cv.v_scale : cv.k_scale) + ph;
     uint32_t amax = __reduce_max_sync(0xffffffffu, __float_as_uint(big));   // (as bits, a NaN is the largest)
     const float was = lo > 0 ? *scale : 0.0f;
     if (wpi > 1) {
