@@ -290,8 +290,9 @@ __global__ void __launch_bounds__(kThreads, 4) kv_write_kernel(const KvWritePara
     // `part`, part + 8, ... where a page has more than eight.
     constexpr int CHUNK = chunk_rows(D), LPR = D / 16, RPI = 32 / LPR;     // lanes of a row, rows at a time
     static_assert(CHUNK == RPI, "a lane holds 16 elements of one row");
-    const int wpi = min(cv.page / CHUNK, kWarps), part = warp % wpi, sub = lane / LPR, j = lane % LPR;
-    const int item = group * (kWarps / wpi) + warp / wpi;
+    const int wpi_log2 = min(cv.page_log2 - (D == 128 ? 2 : 3), 3), wpi = 1 << wpi_log2;     // page / CHUNK, at most kWarps
+    const int part = warp & (wpi - 1), sub = lane / LPR, j = lane % LPR;
+    const int item = group * (kWarps >> wpi_log2) + (warp >> wpi_log2);
     const bool on = item < 2 * cv.kv_heads;
     const bool is_v = on && item >= cv.kv_heads;
     const int h = !on ? 0 : is_v ? item - cv.kv_heads : item;
@@ -339,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, 4) kv_write_kernel(const KvWritePara
     if (wpi > 1) {
         if (lane == 0) sh_max[warp] = amax;
         __syncthreads();
-        for (int w = warp - part; w < warp - part + wpi; ++w) amax = max(amax, sh_max[w]);
+        amax = __reduce_max_sync(0xffffffffu, sh_max[warp - part + (lane & (wpi - 1))]);
     }
     if (!on) return;
     const float mine = __fdiv_rn(__uint_as_float(amax), 127.0f);
