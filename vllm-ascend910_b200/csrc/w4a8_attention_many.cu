@@ -47,10 +47,10 @@
 // Bounds per 256 x 64 step at D = 128: 1024 tensor cycles, 1024 cycles of the
 // exponential unit (16 / clock / SM), about 1,500 cycles of shared memory (128 KB of
 // operands, 64 KB of codes and their conversion), about 1,200 issue slots per scheduler.
-// Measured (B200, 40 query heads on 8 of 128): 2,400 cycles a step, and 12,000 for a
-// tile's queries and output; three prompts of 900-2,048 tokens behind up to 2,048 193 us,
-// 638 TFLOP/s; one prompt of 2,048, 4,096 and 8,192 tokens 82, 237 and 813 us, 524, 726 and
-// 845 TFLOP/s, the last at 1,810 MHz: it reaches the board's power limit.
+// Measured (B200, 40 query heads on 8 of 128): 2,400 cycles a step, and 10,000 for a
+// tile's queries and output; three prompts of 1,364-1,668 tokens behind 179-791 184 us, 670
+// TFLOP/s; one prompt of 2,048, 4,096 and 8,192 tokens 77, 228 and 789 us, 556, 753 and 871
+// TFLOP/s, the last at 1,800 MHz: it reaches the board's power limit.
 #include <algorithm>
 
 #include "w4a8_attention.cuh"

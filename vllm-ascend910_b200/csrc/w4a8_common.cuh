@@ -400,14 +400,6 @@ __device__ __forceinline__ int quant_fast(float xv, float s, float rcp)
 
 __device__ __forceinline__ bool act_scale_fast(uint16_t sb) { return (sb & 0x7F80u) != 0; }
 
-// The larger magnitude; a NaN of either wins.
-__device__ __forceinline__ float max_abs_nan(float m, float x)
-{
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(x)));
-    return r;
-}
-
 // The largest of m and two magnitudes; a NaN of any wins.
 __device__ __forceinline__ float max_abs_nan(float m, float x, float y)
 {
@@ -419,7 +411,9 @@ __device__ __forceinline__ float max_abs_nan(float m, float x, float y)
 // Codes of 4 fp32 values, a byte each: rint(x / s) for |x / s| < 127.5 and a normal
 // s.  y = x * (1 / s) is within 2^-15 of x / s, so rint(y) is the code unless y is
 // within 2^-14 of a half-integer; there the IEEE division decides.  Adding
-// 1.5 * 2^23 rounds y to nearest even and leaves the code in the low byte.
+// 1.5 * 2^23 rounds y to nearest even and leaves the code in the low byte.  (Nor does it
+// matter whether the packed product rounds before the packed sum: where that moves the
+// result, y is next to a half-integer.)
 __device__ __forceinline__ uint32_t codes4(const float* x, float s, float rcp)
 {
     constexpr float kMagic = 12582912.0f;

@@ -29,11 +29,11 @@
 // product with its reciprocal except next to half-integers, where the true division
 // decides (the activation quantiser's rule).
 //
-// Measured (B200): 7,584 tokens of 40 + 8 + 8 heads of 128, pages of 32: write 53 us, of
+// Measured (B200): 7,584 tokens of 40 + 8 + 8 heads of 128, pages of 32: write 51 us, of
 // which the queries' 155 MB alone take 24 at the memory's rate and the pages, by a chain of
-// dependent loads (lengths, page id, rows, scale) in each of 3,800 blocks, 30; read back
-// 9 us (47 MB).  One token of 64 sequences written: 5.4 us; 530 tokens read back: 2.9 us:
-// launch and latency.
+// dependent loads (lengths, rows and page id, scale) and some 650 instructions a warp in each
+// of 3,800 blocks, 28; read back 9 us (47 MB).  One token of 64 sequences written: 5.2 us; 530
+// tokens read back: 2.9 us: launch and latency.
 #include <algorithm>
 
 #include "w4a8_common.cuh"
@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, 4) kv_write_kernel(const KvWritePara
         load(c);
         held = c;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) big = max_abs_nan(big, v[e]);
+        for (int e = 0; e < 16; e += 2) big = max_abs_nan(big, v[e], v[e + 1]);
     }
     if (id < 0 || id >= cv.pages) return;                    // (the whole block's page)
     const int64_t ph = static_cast<int64_t>(id) * cv.kv_heads + h;
