@@ -24,12 +24,12 @@
 // (kv head, K or V) items: a warp holds 4 rows of 128 elements in registers (a page
 // of 32 rows is eight warps), so k and v are read once -- rotated, their maximum found, and
 // written as codes.  All loads of a warp are in flight together, and four blocks an SM
-// (64 registers) hide more than three or five do: 7,584 tokens 53 us against 58 and 69.
+// (64 registers) hide more than three or five do: 7,543 tokens 53 us against 58 and 69.
 // A loop over several items a block was slower too (68 us).  Dividing by the scale is a
 // product with its reciprocal except next to half-integers, where the true division
 // decides (the activation quantiser's rule).
 //
-// Measured (B200): 7,584 tokens of 40 + 8 + 8 heads of 128, pages of 32: write 51 us, of
+// Measured (B200): 7,543 tokens of 40 + 8 + 8 heads of 128, pages of 32: write 51 us, of
 // which the queries' 155 MB alone take 24 at the memory's rate and the pages, by a chain of
 // dependent loads (lengths, rows and page id, scale) and some 650 instructions a warp in each
 // of 3,800 blocks, 28; read back 9 us (47 MB).  One token of 64 sequences written: 5.2 us; 530
@@ -462,7 +462,7 @@ cudaError_t launch_kv_write(const KvWriteParams& p, cudaStream_t stream)
     if (blocks > 0x7FFFFFFF) return cudaErrorInvalidValue;
     const int qb = static_cast<int>(q_blocks);
     // Pages that eight warps hold (up to 32 rows of 128 or 64 of 64) need no loop over
-    // chunks: without it 7,584 tokens in pages of 32 take 53 us, with it 57.
+    // chunks: without it 7,543 tokens in pages of 32 take 53 us, with it 57.
     const bool one = p.c.page / chunk_rows(p.c.D) <= kWarps;
     if (p.c.D == 128)
         return one ? launch(kv_write_kernel<128, true>, blocks, stream, p, qb, groups)

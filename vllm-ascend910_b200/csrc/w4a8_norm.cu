@@ -22,9 +22,10 @@
 // fp32 arithmetic runs in pairs, two elements an instruction; each rounds alone.
 //
 // Measured (B200, rows of 5120 with a residual): 4096 rows, bf16 out 27.5 us, 6.1 TB/s, 93 %
-// of a plain copy's rate; 8191 rows with codes 62 us in groups of 128 or 1024, 4.7 TB/s: about 650 instructions for a thread's 16 elements bound it, not the
-// memory (before the pairs and the bodies without bounds tests 75 and 96 us).  One row: 1.9
-// us, launch and two load latencies.
+// of a plain copy's rate; 8191 rows with codes 62 us in groups of 128 or 1024, 4.7 TB/s:
+// about 560 instructions for a thread's 16 elements bound it, not the memory (before the
+// pairs, the bodies without bounds tests and groups by vector order 75 and 96 us).  One
+// row: 1.9 us, launch and two load latencies.
 #include <algorithm>
 
 #include "w4a8_common.cuh"
