@@ -119,6 +119,10 @@ struct DecCfg {
     static constexpr int PIECE = R * D_ * 4;                       // fp32 O of one piece
     static constexpr int SLOT = RING > PIECE ? RING : PIECE;       // the ring's memory holds the last piece
     static constexpr int SMEM = WARPS * SLOT;
+    // What a part costs its segment's join, in units.  One kv head, 1 token at 64,000: 31 us cut
+    // to single units, 25 with 0.15, 30 with 0.6; at 4,000 11.4, 13.2 and 15.3 (so 0.08).  3 tokens
+    // at 16,000: 44, 22 and 24; 3 at 4,000: 17.6, 15.1 and 16.8.
+    static constexpr float PART_UNITS = NT_ == 1 ? 0.08f : 0.2f;
     static constexpr int CHUNKS = D_ / 16;                         // 16-byte chunks of a token's row
 };
 
@@ -295,10 +299,11 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
         __syncthreads();
     }
     const long long total = running;
-    // equal contiguous shares, at least one unit each: a list shorter than the
-    // grid leaves the last CTAs without work, none between working ones
+    // equal contiguous shares, none below the least: a short list leaves the last
+    // CTAs without work, none between working ones
     const int wk = static_cast<int>(blockIdx.x) * C::WARPS + warp;
-    const Shares sh(total, static_cast<int>(gridDim.x) * C::WARPS);
+    const int least = least_share(total, p.segments, C::WARPS, C::PART_UNITS), most = static_cast<int>(gridDim.x) * C::WARPS;
+    const Shares sh(total, total >= static_cast<long long>(most) * least ? most : max(1u, static_cast<uint32_t>(total) / least));
     const long long u0 = sh.begin(wk), u1 = sh.begin(wk + 1);
 
     float acc[C::NT][C::D / 16][4];
@@ -841,6 +846,9 @@ cudaError_t launch_attention(const AttentionParams& p0, int sms, cudaStream_t st
     AttentionParams p = p0;
     const int64_t rows = static_cast<int64_t>(p.max_q) * p.group;
     p.few_most = 0x7FFFFFFF;
+    const int tile = rows <= kFewRows ? 8 * few_nt(rows) : 256;
+    p.segments = static_cast<int>(std::min<int64_t>(
+        0x7FFFFFFF, static_cast<int64_t>(p.c.kv_heads) * std::max<int64_t>(p.c.batch, p.c.tokens * p.group / tile)));
     if (rows > kFewRows) {
         // A sequence has more rows than attend_few_kernel is made for.  Many sequences of
         // uneven lengths are single tokens beside prompts as a rule: each kernel takes its

@@ -201,6 +201,15 @@ __device__ __forceinline__ int find_parts(const Partial* info, int lead, int nct
     return n + 1;
 }
 
+// The least units of a share.  A segment cut in n parts costs n reads in its join, one
+// CTA's; a worker's share costs its units: with `total` units of `segments` segments and
+// `workers` workers to a part, share * 1 + (total / (segments * workers * share)) * ratio
+// is least here, ratio being a part's cost in units.
+__device__ __forceinline__ int least_share(long long total, int segments, int workers, float ratio)
+{
+    return max(1, static_cast<int>(sqrtf(ratio * static_cast<float>(total) / (static_cast<float>(segments) * workers)) + 0.5f));
+}
+
 // 1 / l; 0 for a row that saw no token, NaN for a NaN.
 __device__ __forceinline__ float inv_sum(float l) { return l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l); }
 

@@ -76,6 +76,9 @@ constexpr int kTileUnits = 6;
 // A CTA's share is not cut below this.  A prompt of 100: 16.3, 16.8, 17.6 and 24.2 us with 1, 2,
 // 4 and 8; 100 tokens behind 400: 21.6, 20.1 and 21.4 with 1, 2 and 4.
 constexpr int kMinUnits = 2;
+// What a part costs its tile's join, in blocks.  One kv head, 20 tokens at 16,000: 49 us cut to
+// kMinUnits, 27.5, 27.3 and 28.0 with 0.2, 0.35 and 0.7; 200 tokens there: 40, 38.5, 37.1 and 39.
+constexpr float kPartBlocks = 0.35f;
 constexpr float kMargin = 2.0f;            // log2 by which a new reference exceeds the scores seen
 
 // wait-site ids for the status word
@@ -814,7 +817,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Atte
             run += __shfl_sync(0xffffffffu, v, 31);
         }
         __syncwarp();
-        const long long W = min(static_cast<long long>(gridDim.x), (run + kMinUnits - 1) / kMinUnits);
+        const int share = max(kMinUnits, least_share(run, p.segments, 1, kPartBlocks));
+        const long long W = min(static_cast<long long>(gridDim.x), (run + share - 1) / share);
         const long long c = blockIdx.x;
         const long long u0 = c < W ? run * c / W : run, u1 = c < W ? run * (c + 1) / W : run;
         Start st{0, 0, 0, 0, u1 - u0};

@@ -220,6 +220,7 @@ struct AttentionParams {
     uint64_t group_magic;     // floor(2^64 / group) + 1 (0 for group 1): see row_token
     int max_q;                // no sequence has more query tokens (host's knowledge)
     float scale_log2;         // softmax scale * log2(e)
+    int segments;             // about how many row tiles there are, of all heads and sequences (host's estimate)
     int few_most;             // attend_few_kernel takes sequences of at most this many packed rows
     int* status;              // workspace: status word
     uint32_t* tickets;        // workspace: zeroed counters beside it, one per CTA (attend_few_kernel leaves them zero)
