@@ -134,15 +134,21 @@ struct Start {           // where the CTA's share begins: unit `unit` of a tile
 
 __device__ __forceinline__ int many_tiles(const Seq& s, int group, int least)
 {
-    const long long rows = static_cast<long long>(s.n) * group;
-    return rows > least ? static_cast<int>((rows + kRows - 1) / kRows) : 0;
+    const int rows = s.n * group;            // (at most 0x7FFF0000: checked on the host)
+    return rows > least ? (rows + kRows - 1) / kRows : 0;
+}
+
+// a / b, by the several times shorter 32-bit division where that does.
+__device__ __forceinline__ long long quotient(long long a, long long b)
+{
+    return a < 0x7FFFFFFF && b < 0x7FFFFFFF ? static_cast<uint32_t>(a) / static_cast<uint32_t>(b) : a / b;
 }
 
 // 64-token blocks that some row of tile t sees (at least one: rows that see
 // nothing are written too).
 __device__ __forceinline__ int many_blocks(const Seq& s, int group, int t)
 {
-    const int last = min(s.n - 1, static_cast<int>(((static_cast<long long>(t) + 1) * kRows - 1) / group));
+    const int last = min(s.n - 1, static_cast<int>((static_cast<uint32_t>(t + 1) * kRows - 1) / static_cast<uint32_t>(group)));
     const int lim = s.len - s.n + last;
     return lim < 0 ? 1 : lim / kBlk + 1;
 }
@@ -195,7 +201,7 @@ struct Walk {
     }
     __device__ __forceinline__ bool has_b(int group) const
     {
-        return static_cast<long long>(s.n) * group - static_cast<long long>(tile) * kRows > 128;
+        return s.n * group - tile * kRows > 128;
     }
 };
 
@@ -818,9 +824,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Atte
         }
         __syncwarp();
         const int share = max(kMinUnits, least_share(run, p.segments, 1, kPartBlocks));
-        const long long W = min(static_cast<long long>(gridDim.x), (run + share - 1) / share);
+        const long long W = min(static_cast<long long>(gridDim.x), quotient(run + share - 1, share));
         const long long c = blockIdx.x;
-        const long long u0 = c < W ? run * c / W : run, u1 = c < W ? run * (c + 1) / W : run;
+        const long long u0 = c < W ? quotient(run * c, W) : run, u1 = c < W ? quotient(run * (c + 1), W) : run;
         Start st{0, 0, 0, 0, u1 - u0};
         if (u0 < u1) {
             int lo = 0, hi = cv.batch - 1;
@@ -830,10 +836,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const Atte
                 else hi = mid - 1;
             }
             const Seq q = load_seq(cv, lo);
-            const long long per_head = ((lo + 1 < cv.batch ? prefix[lo + 1] : run) - prefix[lo]) / cv.kv_heads;
+            const long long per_head = quotient((lo + 1 < cv.batch ? prefix[lo + 1] : run) - prefix[lo], cv.kv_heads);
             const long long off = u0 - prefix[lo];
             st.seq = lo;
-            st.head = static_cast<int>(off / per_head);
+            st.head = static_cast<int>(quotient(off, per_head));
             long long r = off - st.head * per_head;
             // the tile that holds unit r of the head
             const int tiles = many_tiles(q, p.group, least);
