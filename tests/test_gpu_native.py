@@ -116,3 +116,98 @@ def test_cache_and_attention(dev, monkeypatch, interleaved):
     assert N.attention(a._ref, a._index, table, kl, cu[:-1], got, 33, 0.2, *ws) is NotImplemented
     assert N.attention(a._ref, a._index, table, kl, cu, got.float(), 33, 0.2, *ws) is NotImplemented
     assert N.attention(a._ref, a._index, table, kl, cu, got, 33, -1.0, *ws) is NotImplemented
+
+
+def test_launches_run_on_the_tensors_device(monkeypatch):
+    """A call whose tensors are not on the current GPU is made with theirs current, and the other is put back."""
+    from w4a8_b200 import ops
+    log = []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            log.append(("in", self.index))
+
+        def __exit__(self, *a):
+            log.append(("out", self.index))
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(ops, "_current_index", lambda: 0)
+    assert ops._launch(1, lambda *a: log.append(a) or 5, 2, 3) == 5
+    assert log == [("in", 1), (2, 3), ("out", 1)]
+    log.clear()
+    assert ops._launch(0, lambda: log.append("here") or 0) == 0 and log == ["here"]
+
+    def fails():
+        raise RuntimeError("fails")
+
+    log.clear()
+    with pytest.raises(RuntimeError, match="fails"):
+        ops._launch(1, fails)
+    assert log == [("in", 1), ("out", 1)]
+
+
+@pytest.mark.gpu
+def test_every_wrapper_switches_to_its_tensors_device(dev, monkeypatch):
+    """With another GPU said to be the current one, each call enters its tensors' device before it reaches the
+    library (whose launches are then made on the only GPU here, as always)."""
+    from w4a8_b200 import _lib, kvcache as kv, ops
+    seen, inside = [], []
+
+    class Device:
+        def __init__(self, index):
+            assert index == 0
+
+        def __enter__(self):
+            inside.append(1)
+
+        def __exit__(self, *a):
+            inside.pop()
+
+    L = _lib.lib()
+
+    class Library:
+        def __getattr__(self, name):
+            fn = getattr(L, name)
+            if name.endswith("_size") or name in ("w4a8_status_string", "w4a8_last_cuda_error"):
+                return fn
+
+            def call(*a):
+                seen.append((name, bool(inside)))
+                return fn(*a)
+            return call
+
+    x = torch.randn(4, 512, device=dev).bfloat16()
+    codes = torch.randint(-8, 8, (64, 512), dtype=torch.int8, device=dev)
+    packed, ws = ops.pack_int4_grouped(codes, 128), torch.ones(4, 64, device=dev)
+    w = torch.ones(512, dtype=torch.bfloat16, device=dev)
+    cache = kv.KVCache.empty(4, 2, 16, 64, dev)
+    i = dict(dtype=torch.int32, device=dev)
+    batch = torch.tensor([[0, 1]], **i), torch.tensor([4], **i), torch.tensor([0, 4], **i)
+    k = x[:, :128].contiguous().view(4, 2, 64)
+    ops.workspace(32 << 20, dev)
+    monkeypatch.setattr(_lib, "_N", None)
+    monkeypatch.setattr(_lib, "_L", Library())
+    monkeypatch.setattr(ops, "_current_index", lambda: 1)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    ops.quant_act(x, 128)
+    ops.midgroup_quant_a(x, 128)
+    ops.linear(x, packed, ws, None, 128)
+    pw = ops.prepare_weights(packed, ws, None, 512, 128)
+    y = ops.linear_prepared(x, pw)
+    ops.linear_quant(x, 64, 128)
+    ops.linear_gemm(4, 512, packed, ws, None, 128, y)
+    ops.linear_gemm_prepared(4, pw, y)
+    ops.group_partials(x, packed, None, 128)
+    ops.rms_norm(x, w)
+    ops.rms_norm_quant(x, w, 128)
+    ops.linear_prepared_rms_norm(x, w, pw)
+    kv.kv_write(cache, k, k, *batch, q=k)
+    kv.kv_read(cache, *batch, 4)
+    kv.attention(k, cache, *batch, 4)
+    assert ops.workspace_status(dev) == 0
+    names = [n for n, _ in seen]
+    assert len(set(names)) >= 14 and {"w4a8_rms_norm", "w4a8_kv_write", "w4a8_kv_read", "w4a8_attention"} <= set(names)
+    assert [n for n, ok in seen if not ok] == []

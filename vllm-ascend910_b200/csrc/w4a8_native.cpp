@@ -4,11 +4,12 @@
 // The Python wrappers (ops.py, kvcache.py) read some thirty tensor attributes a call
 // to check their arguments, which costs more than such a call's kernels run.  These
 // functions do the same checks on the tensors themselves, allocate the outputs and
-// call the C ABI.  They take the well-formed common case only -- exact torch tensors,
-// dense, 16-byte aligned -- and return NotImplemented for everything else, a refusal
+// call the C ABI.  They take the well-formed common case only -- exact torch tensors on
+// the current GPU, dense, 16-byte aligned -- and return NotImplemented for everything else, a refusal
 // by the C entry point included; the wrapper then goes the long way, with its
 // messages, copies and strided forms.  Results are the same either way.
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -38,6 +39,9 @@ bool is(const at::Tensor* t, at::ScalarType type, int dev, int64_t dims)
 {
     return t && t->is_cuda() && t->scalar_type() == type && t->get_device() == dev && t->dim() == dims;
 }
+
+// The library launches on the current GPU; the long way makes the tensors' one current.
+bool current(int dev) { return c10::cuda::current_device() == dev; }
 
 bool dense(const at::Tensor* t, at::ScalarType type, int dev, int64_t dims) { return is(t, type, dev, dims) && t->is_contiguous(); }
 
@@ -90,7 +94,7 @@ bool rows(PyObject* const* a, Rows& n)
         if (!dense(n.r, at::kBFloat16, n.dev, n.x->dim()) || n.r->sizes() != n.x->sizes()) return false;
     }
     n.M = n.x->numel() / n.K;
-    return true;
+    return current(n.dev);
 }
 
 const void* ptr(const at::Tensor* t) { return t ? t->const_data_ptr() : nullptr; }
@@ -165,7 +169,7 @@ bool batch(PyObject* const* a, Batch& b)
         return false;
     b.B = b.lens->size(0);
     b.cols = b.table->size(1);
-    return b.B > 0 && b.table->size(0) == b.B && b.cu->size(0) == b.B + 1;
+    return b.B > 0 && b.table->size(0) == b.B && b.cu->size(0) == b.B + 1 && current(b.dev);
 }
 
 // bf16 [tokens, heads, head_dim] with dense heads and 16-byte rows; its row stride.

@@ -15,7 +15,7 @@ CUDA graph follows their contents; a page id outside the cache means "no
 page" (not written, not attended to, read as zeros).
 
 Argument checks raise ``RuntimeError``; kernels run on the current stream of
-the tensors' device.  The reference has no counterpart (its serving stack keeps a
+the tensors' device, whichever device is current.  The reference has no counterpart (its serving stack keeps a
 bf16 cache); there is no CPU implementation.
 """
 from __future__ import annotations
@@ -27,7 +27,7 @@ from typing import Dict, Optional, Tuple
 import torch
 
 from . import _lib
-from .ops import _check, _stream_of, workspace
+from .ops import _check, _launch, _stream_of, workspace
 
 PAGE_SIZES = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128)
@@ -220,8 +220,8 @@ def kv_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, page_table: torch
         cs = cos_sin.data_ptr()
     if T == 0 or B == 0:
         return out
-    rc = _lib.lib().w4a8_kv_write(cache._ref, tp, ld, cols, kv_lens.data_ptr(), cu_q.data_ptr(), B, T, kp, ldk, vp, ldv,
-                                  qp, ldq, hq, op, ldo, cs, rows, rot, 1 if interleaved else 0, _stream_of(k))
+    rc = _launch(cache._index, _lib.lib().w4a8_kv_write, cache._ref, tp, ld, cols, kv_lens.data_ptr(), cu_q.data_ptr(), B,
+                 T, kp, ldk, vp, ldv, qp, ldq, hq, op, ldo, cs, rows, rot, 1 if interleaved else 0, _stream_of(k))
     if rc != 0:
         _lib.check(rc, "w4a8_kv_write")
     return out
@@ -244,8 +244,8 @@ def kv_read(cache: KVCache, page_table: torch.Tensor, kv_lens: torch.Tensor, cu_
     if tokens == 0:
         return k, v
     _check(B > 0, "kv_read: tokens of no sequence")
-    rc = _lib.lib().w4a8_kv_read(cache._ref, tp, ld, cols, kv_lens.data_ptr(), cu_out.data_ptr(), B, tokens,
-                                 k.data_ptr(), v.data_ptr(), _stream_of(k))
+    rc = _launch(cache._index, _lib.lib().w4a8_kv_read, cache._ref, tp, ld, cols, kv_lens.data_ptr(), cu_out.data_ptr(),
+                 B, tokens, k.data_ptr(), v.data_ptr(), _stream_of(k))
     if rc != 0:
         _lib.check(rc, "w4a8_kv_read")
     return k, v
@@ -290,8 +290,8 @@ def attention(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor, kv_lens
             _WS_BYTES.clear()
         need = _WS_BYTES[key] = L.w4a8_attention_workspace_size(*key)
     ws, wsb = workspace(need, cache.device)
-    rc = L.w4a8_attention(cache._ref, tp, ld, cols, kv_lens.data_ptr(), cu_q.data_ptr(), B, T, qp, ldq, hq, max_q_len,
-                          D ** -0.5 if scale is None else scale, op, ldo, ws, wsb, _stream_of(q))
+    rc = _launch(cache._index, L.w4a8_attention, cache._ref, tp, ld, cols, kv_lens.data_ptr(), cu_q.data_ptr(), B, T, qp,
+                 ldq, hq, max_q_len, D ** -0.5 if scale is None else scale, op, ldo, ws, wsb, _stream_of(q))
     if rc != 0:
         _lib.check(rc, "w4a8_attention")
     return out

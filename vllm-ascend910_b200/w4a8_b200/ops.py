@@ -74,6 +74,21 @@ def _stream_of(t: torch.Tensor) -> int:
     return _stream(t.device)
 
 
+_current_index = torch._C._cuda_getDevice      # (a tenth of torch.cuda.current_device()'s time)
+
+
+def _launch(index: int, fn, *args) -> int:
+    """``fn(*args)``, an entry point that launches on GPU ``index``, with that GPU current.
+
+    The library launches on the current GPU, and the default stream of every GPU is
+    the same null handle: with another one current, kernels would run there, on
+    this one's addresses."""
+    if _current_index() == index:
+        return fn(*args)
+    with torch.cuda.device(index):
+        return fn(*args)
+
+
 # workspace bytes per (M, N, K, group size): a pure function of the shape and
 # the device's SM count (one process drives one kind of GPU)
 _WS_BYTES: Dict[Tuple[int, int, int, int], int] = {}
@@ -131,7 +146,7 @@ def workspace_status(device: Optional[torch.device] = None, reset: bool = True) 
     status = 0
     for buf in _WS_ALL.get(key, []):
         ptr = (buf.data_ptr() + 1023) & ~1023
-        v = _lib.lib().w4a8_workspace_status(ptr, 1 if reset else 0, _stream(device))
+        v = _launch(key, _lib.lib().w4a8_workspace_status, ptr, 1 if reset else 0, _stream(device))
         status = status or v
     return status
 
@@ -167,8 +182,8 @@ def quant_act(x: torch.Tensor, group_size: int, scale_dtype: torch.dtype = torch
     ks = torch.empty((G, M), dtype=torch.int32, device=x.device) if with_ksum else None
     sd = _lib.DTYPE_F32 if scale_dtype == torch.float32 else _lib.DTYPE_BF16
     _check(scale_dtype in (torch.float32, torch.bfloat16), "quant_act: scale dtype must be bf16 or f32")
-    rc = _lib.lib().w4a8_quant_act(x.data_ptr(), M, K, K, group_size, q.data_ptr(), s.data_ptr(), sd,
-                                   _ptr(ks), _stream(x.device))
+    rc = _launch(x.get_device(), _lib.lib().w4a8_quant_act, x.data_ptr(), M, K, K, group_size, q.data_ptr(),
+                 s.data_ptr(), sd, _ptr(ks), _stream(x.device))
     _lib.check(rc, "w4a8_quant_act")
     return q, s, ks
 
@@ -188,9 +203,8 @@ def midgroup_quant_a(x: torch.Tensor, group_size: int = GROUP) -> List[torch.Ten
     a_lo = torch.empty((Mp, Kp // 2), dtype=torch.int8, device=dev)
     a_scale = torch.empty((G, Mp), dtype=torch.bfloat16, device=dev)
     a_ksum = torch.empty((G, Mp), dtype=torch.int32, device=dev)
-    rc = _lib.lib().w4a8_midgroup_quant_a(x.data_ptr(), M, K, group_size, Mp, a_hi.data_ptr(),
-                                          a_lo.data_ptr(), a_scale.data_ptr(), a_ksum.data_ptr(),
-                                          _stream(dev))
+    rc = _launch(x.get_device(), _lib.lib().w4a8_midgroup_quant_a, x.data_ptr(), M, K, group_size, Mp,
+                 a_hi.data_ptr(), a_lo.data_ptr(), a_scale.data_ptr(), a_ksum.data_ptr(), _stream(dev))
     _lib.check(rc, "w4a8_midgroup_quant_a")
     return [a_hi, a_lo, a_scale, a_ksum]
 
@@ -226,9 +240,9 @@ def midgroup_w4a8_gemm(a_hi, a_lo, a_scale, a_ksum, w_q, w_scale, w_ksum, w_zero
     y = torch.empty((M, N), dtype=torch.bfloat16, device=a_hi.device)
     L = _lib.lib()
     ws, wsb = workspace(L.w4a8_midgroup_gemm_workspace_size(M, N, K, group_size), a_hi.device)
-    rc = L.w4a8_midgroup_w4a8_gemm(a_hi.data_ptr(), a_lo.data_ptr(), a_scale.data_ptr(), _ptr(a_ksum), M,
-                                   w_q.data_ptr(), w_scale.data_ptr(), _ptr(w_ksum), _ptr(w_zero), N, K,
-                                   group_size, y.data_ptr(), ws, wsb, _stream(a_hi.device))
+    rc = _launch(a_hi.get_device(), L.w4a8_midgroup_w4a8_gemm, a_hi.data_ptr(), a_lo.data_ptr(), a_scale.data_ptr(),
+                 _ptr(a_ksum), M, w_q.data_ptr(), w_scale.data_ptr(), _ptr(w_ksum), _ptr(w_zero), N, K, group_size,
+                 y.data_ptr(), ws, wsb, _stream(a_hi.device))
     _lib.check(rc, "w4a8_midgroup_w4a8_gemm")
     return y
 
@@ -269,8 +283,8 @@ def linear(x: torch.Tensor, w_packed: torch.Tensor, w_scale: torch.Tensor,
     ws, wsb = workspace(_ws_bytes(M, N, K, group_size), x.device)
     sd = _lib.DTYPE_F32 if w_scale.dtype == torch.float32 else _lib.DTYPE_BF16
     fn = L.w4a8_linear if act is None else L.w4a8_linear_swiglu
-    rc = fn(x2.data_ptr(), M, K, x2.stride(0), N, group_size, w_packed.data_ptr(),
-            w_scale.data_ptr(), sd, _ptr(w_zero), y.data_ptr(), y.stride(0), ws, wsb, _stream_of(x2))
+    rc = _launch(x2.get_device(), fn, x2.data_ptr(), M, K, x2.stride(0), N, group_size, w_packed.data_ptr(),
+                 w_scale.data_ptr(), sd, _ptr(w_zero), y.data_ptr(), y.stride(0), ws, wsb, _stream_of(x2))
     _lib.check(rc, "w4a8_linear" if act is None else "w4a8_linear_swiglu")
     return y.reshape(*lead, N)
 
@@ -280,7 +294,8 @@ def linear_quant(x2: torch.Tensor, N: int, group_size: int) -> None:
     M, K = x2.shape
     L = _lib.lib()
     ws, wsb = workspace(_ws_bytes(M, N, K, group_size), x2.device)
-    rc = L.w4a8_linear_quant(x2.data_ptr(), M, K, x2.stride(0), N, group_size, ws, wsb, _stream(x2.device))
+    rc = _launch(x2.get_device(), L.w4a8_linear_quant, x2.data_ptr(), M, K, x2.stride(0), N, group_size, ws, wsb,
+                 _stream(x2.device))
     _lib.check(rc, "w4a8_linear_quant")
 
 
@@ -290,8 +305,8 @@ def linear_gemm(M: int, K: int, w_packed, w_scale, w_zero, group_size: int, y: t
     L = _lib.lib()
     ws, wsb = workspace(L.w4a8_linear_workspace_size(M, N, K, group_size), y.device)
     sd = _lib.DTYPE_F32 if w_scale.dtype == torch.float32 else _lib.DTYPE_BF16
-    rc = L.w4a8_linear_gemm(M, K, N, group_size, w_packed.data_ptr(), w_scale.data_ptr(), sd, _ptr(w_zero),
-                            y.data_ptr(), y.stride(0), ws, wsb, _stream(y.device))
+    rc = _launch(y.get_device(), L.w4a8_linear_gemm, M, K, N, group_size, w_packed.data_ptr(), w_scale.data_ptr(), sd,
+                 _ptr(w_zero), y.data_ptr(), y.stride(0), ws, wsb, _stream(y.device))
     _lib.check(rc, "w4a8_linear_gemm")
 
 
@@ -324,8 +339,8 @@ def prepare_weights(w_packed: torch.Tensor, w_scale: torch.Tensor, w_zero: Optio
     _check(nbytes > 0, "prepare_weights: unsupported shape")
     buf = torch.empty(nbytes + 256, dtype=torch.uint8, device=w_packed.device)
     pw = PreparedWeight(buf, N, K, group_size, sd, w_zero is not None)
-    rc = L.w4a8_prepare_weights(w_packed.data_ptr(), w_scale.data_ptr(), sd, _ptr(w_zero), N, K, group_size,
-                                pw.ptr(), nbytes, _stream(w_packed.device))
+    rc = _launch(w_packed.get_device(), L.w4a8_prepare_weights, w_packed.data_ptr(), w_scale.data_ptr(), sd,
+                 _ptr(w_zero), N, K, group_size, pw.ptr(), nbytes, _stream(w_packed.device))
     _lib.check(rc, "w4a8_prepare_weights")
     return pw
 
@@ -354,8 +369,8 @@ def linear_prepared(x: torch.Tensor, pw: PreparedWeight, out: Optional[torch.Ten
     ws, wsb = workspace(_ws_bytes(M, N, K, pw.group_size), x.device)
     L = _lib.lib()
     fn = L.w4a8_linear_prepared if act is None else L.w4a8_linear_prepared_swiglu
-    rc = fn(x2.data_ptr(), M, K, x2.stride(0), N, pw.group_size, pw.ptr(), pw.ws_dtype,
-            1 if pw.has_zero else 0, y.data_ptr(), y.stride(0), ws, wsb, _stream_of(x2))
+    rc = _launch(x2.get_device(), fn, x2.data_ptr(), M, K, x2.stride(0), N, pw.group_size, pw.ptr(), pw.ws_dtype,
+                 1 if pw.has_zero else 0, y.data_ptr(), y.stride(0), ws, wsb, _stream_of(x2))
     if rc != 0:
         _lib.check(rc, "w4a8_linear_prepared" if act is None else "w4a8_linear_prepared_swiglu")
     return y if x.dim() == 2 else y.reshape(*x.shape[:-1], N)
@@ -365,9 +380,8 @@ def linear_gemm_prepared(M: int, pw: PreparedWeight, y: torch.Tensor) -> None:
     """Second half of ``linear_prepared`` after ``linear_quant(x2, pw.N, pw.group_size)``."""
     L = _lib.lib()
     ws, wsb = workspace(_ws_bytes(M, pw.N, pw.K, pw.group_size), y.device)
-    rc = L.w4a8_linear_gemm_prepared(M, pw.K, pw.N, pw.group_size, pw.ptr(), pw.ws_dtype,
-                                     1 if pw.has_zero else 0, y.data_ptr(), y.stride(0), ws, wsb,
-                                     _stream(y.device))
+    rc = _launch(y.get_device(), L.w4a8_linear_gemm_prepared, M, pw.K, pw.N, pw.group_size, pw.ptr(), pw.ws_dtype,
+                 1 if pw.has_zero else 0, y.data_ptr(), y.stride(0), ws, wsb, _stream(y.device))
     _lib.check(rc, "w4a8_linear_gemm_prepared")
 
 
@@ -383,8 +397,8 @@ def group_partials(x: torch.Tensor, w_packed: torch.Tensor, w_zero: Optional[tor
     P = torch.empty((G, M, N), dtype=torch.int32, device=x.device)
     L = _lib.lib()
     ws, wsb = workspace(L.w4a8_linear_workspace_size(M, N, K, group_size), x.device)
-    rc = L.w4a8_group_partials(x.data_ptr(), M, K, K, N, group_size, w_packed.data_ptr(), _ptr(w_zero),
-                               P.data_ptr(), ws, wsb, _stream(x.device))
+    rc = _launch(x.get_device(), L.w4a8_group_partials, x.data_ptr(), M, K, K, N, group_size, w_packed.data_ptr(),
+                 _ptr(w_zero), P.data_ptr(), ws, wsb, _stream(x.device))
     _lib.check(rc, "w4a8_group_partials")
     return P
 
@@ -473,8 +487,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
         ldy = K
     else:
         y, ldy = _dense_rows(out, x.shape, K, x.device, "rms_norm", "out")
-    rc = _lib.lib().w4a8_rms_norm(x2.data_ptr(), M, K, ldx, rp, ldr, rop, ldro, weight.data_ptr(), wd, eps, y.data_ptr(),
-                                  ldy, _stream_of(x2))
+    rc = _launch(x2.get_device(), _lib.lib().w4a8_rms_norm, x2.data_ptr(), M, K, ldx, rp, ldr, rop, ldro,
+                 weight.data_ptr(), wd, eps, y.data_ptr(), ldy, _stream_of(x2))
     if rc != 0:
         _lib.check(rc, "w4a8_rms_norm")
     if x.dim() != 2:
@@ -498,10 +512,9 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, group_size: int, eps: 
     x2, M, K, ldx, wd, r2, rp, ldr, ro, rop, ldro = _norm_args(x, weight, residual, residual_out, "rms_norm_quant")
     q = torch.empty((M, K), dtype=torch.int8, device=x.device)
     s = torch.empty((num_groups(K, max(group_size, 1)), M), dtype=scale_dtype, device=x.device)
-    rc = _lib.lib().w4a8_rms_norm_quant(x2.data_ptr(), M, K, ldx, rp, ldr, rop, ldro, weight.data_ptr(), wd, eps,
-                                        group_size, q.data_ptr(), s.data_ptr(),
-                                        _lib.DTYPE_F32 if scale_dtype is torch.float32 else _lib.DTYPE_BF16,
-                                        _stream_of(x2))
+    rc = _launch(x2.get_device(), _lib.lib().w4a8_rms_norm_quant, x2.data_ptr(), M, K, ldx, rp, ldr, rop, ldro,
+                 weight.data_ptr(), wd, eps, group_size, q.data_ptr(), s.data_ptr(),
+                 _lib.DTYPE_F32 if scale_dtype is torch.float32 else _lib.DTYPE_BF16, _stream_of(x2))
     if rc != 0:
         _lib.check(rc, "w4a8_rms_norm_quant")
     return q, s, ro
@@ -525,10 +538,9 @@ def linear_prepared_rms_norm(x: torch.Tensor, weight: torch.Tensor, pw: Prepared
         y, ldy = _dense_rows(out, (M, N), N, x.device, what, f"out [{M}, {N}]")
     if M > 0:
         ws, wsb = workspace(_ws_bytes(M, N, K, pw.group_size), x.device)
-        rc = _lib.lib().w4a8_linear_prepared_rms_norm(x2.data_ptr(), M, K, ldx, rp, ldr, rop, ldro, weight.data_ptr(), wd,
-                                                      eps, N, pw.group_size, pw.ptr(), pw.ws_dtype,
-                                                      1 if pw.has_zero else 0, y.data_ptr(), ldy, ws, wsb,
-                                                      _stream_of(x2))
+        rc = _launch(x2.get_device(), _lib.lib().w4a8_linear_prepared_rms_norm, x2.data_ptr(), M, K, ldx, rp, ldr, rop,
+                     ldro, weight.data_ptr(), wd, eps, N, pw.group_size, pw.ptr(), pw.ws_dtype, 1 if pw.has_zero else 0,
+                     y.data_ptr(), ldy, ws, wsb, _stream_of(x2))
         if rc != 0:
             _lib.check(rc, "w4a8_linear_prepared_rms_norm")
     if x.dim() != 2:
