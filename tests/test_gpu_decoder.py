@@ -169,3 +169,26 @@ def test_captured_steps_equal_eager_ones():
         outs.append(got + [t for c in dec.caches for t in (c.k, c.v, c.k_scale, c.v_scale)])
     for x, y in zip(*outs):
         assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+def test_captured_step_keeps_its_decoder():
+    """The graph reads weights, caches and rotary table by address: they live as long as it does.  (Nothing is
+    replayed here.)"""
+    import gc
+    import weakref
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    dev = torch.device("cuda", 0)
+    dec, _ = _build(dev, 24)
+    s = dec.pages.add()
+    run = dec.capture(dec.pages.plan([s], [1], dev))
+    held = [weakref.ref(dec)] + [weakref.ref(t) for L in dec.layers for t in (L.qkv.buf, L.norm1, L.down.buf)]
+    held += [weakref.ref(t) for c in dec.caches for t in (c.k, c.v_scale)] + [weakref.ref(dec.cos_sin), weakref.ref(dec.final_norm)]
+    dec.layers = []                                # as a caller that goes on to other layers leaves it
+    del dec
+    gc.collect()
+    assert all(r() is not None for r in held)
+    del run
+    gc.collect()
+    assert all(r() is None for r in held)

@@ -181,6 +181,9 @@ class Captured:
     """``Decoder.step`` as a CUDA graph; calling it with a plan of the captured shape runs that step."""
 
     def __init__(self, dec: Decoder, plan: Plan):
+        # The graph holds addresses only: what it reads and writes outside its own pool stays alive here, the
+        # layers as they were captured too.
+        self._keep = (dec, [dataclasses.replace(L) for L in dec.layers], list(dec.caches), dec.final_norm, dec.cos_sin)
         self.plan = dataclasses.replace(plan, page_table=plan.page_table.clone(), kv_lens=plan.kv_lens.clone(),
                                         cu=plan.cu.clone())
         self.h = torch.zeros((plan.tokens, dec.cfg.hidden), dtype=torch.bfloat16, device=plan.kv_lens.device)
