@@ -283,7 +283,7 @@ W4A8_API int w4a8_linear_prepared_rms_norm(const void* x, int64_t M, int64_t K, 
  *   page_table  int32 [batch, ld_table], table_cols columns in use: the page that
  *               holds tokens [c * page_size, (c + 1) * page_size) of a sequence
  *   kv_lens     int32 [batch]: tokens of each sequence in the cache, the call's
- *               own included (at most table_cols * page_size count)
+ *               own included; tokens past table_cols * page_size have no page
  *   cu          int32 [batch + 1]: the call's tokens of sequence s are rows
  *               [cu[s], cu[s + 1]), its LAST cu[s + 1] - cu[s] tokens
  * They are read on the device, so a captured graph follows their contents.  A

@@ -283,3 +283,15 @@ def test_refusals():
         with pytest.raises(RuntimeError):
             f()
     assert kvcache.attention(q[:0], cache, table, kl, cu, 1).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("qs,over", [([1], 1), ([3], 2), ([20], 5), ([100], 40), ([2], 900)])
+def test_lengths_past_the_table(qs, over):
+    """Tokens past the table's last column are not there; the others stay at their positions."""
+    c = Case(5, 1, 128, 16, qs, [160], seed=14)
+    c.lens = [160 + over]
+    c.check(c.run())
+    if over >= qs[0]:                                    # every row sees all that is there, wherever it is itself
+        first = c.run()
+        c.lens = [2 ** 31 - 1]
+        assert torch.equal(c.run(), first)

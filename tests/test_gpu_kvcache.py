@@ -250,3 +250,18 @@ def test_refusals():
             f()
     assert kvcache.kv_write(cache, k[:0], k[:0], t, kl, cu) is None
     assert kvcache.kv_read(cache, t, kl, cu, 0)[0].shape == (0, 2, 64)
+
+
+@pytest.mark.parametrize("page,d", [(16, 64), (32, 128), (128, 128)])
+def test_lengths_past_the_table(page, d):
+    """Tokens past the table's last column have no page: they are not written (and what is there stays), their q is
+    turned by their own position, and they read back as zeros."""
+    cap = 2 * page
+    t = Twin(2, d, page, [cap, cap], seed=9)
+    t.write(t.rows(2 * cap - 3, 2), t.rows(2 * cap - 3, 2), [cap, cap - 3], [cap, cap - 3])
+    t.write(t.rows(18, 2), t.rows(18, 2), [cap + 7, cap + 5], [10, 8], q=t.rows(18, 3), table=_table(64, cap + 20))
+    t.write(t.rows(5, 2), t.rows(5, 2), [cap + 100, cap - 3], [4, 1], q=t.rows(5, 3), table=_table(64, cap + 200))
+    t.read([cap + 7, cap + 5], [20, 5])
+    big = 2 ** 31 - 1
+    t.write(t.rows(3, 2), t.rows(3, 2), [big, cap], [3, 0], q=t.rows(3, 3), table=_table(64, cap))
+    t.read([big, cap], [2, cap])

@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
                 for (int h = 0; h < 2; ++h) {
                     const int qr = cur.tile * C::R + nt * 8 + 2 * c + h;
                     // rows past the sequence's last are computed on zero queries and not stored
-                    limit[nt][h] = qr < cur.s.n * p.group ? cur.s.len - cur.s.n + row_token(p, qr) : 0x7FFFFFFF;
+                    limit[nt][h] = qr < cur.s.n * p.group ? cur.s.pos + row_token(p, qr) : 0x7FFFFFFF;
                     min_limit = min(min_limit, limit[nt][h]);
                     m[nt][h] = kNegInf;
                     negm[nt][h] = first_reference(kNegInf);

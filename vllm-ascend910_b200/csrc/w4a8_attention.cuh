@@ -88,10 +88,11 @@ __device__ __forceinline__ float ex2(float x)
 
 // ------------------------------------------------------------------ the batch
 
-// A sequence as the kernels see it, every value held within the tensors.
+// A sequence as the kernels see it, every value but `pos` held within the tensors.
 struct Seq {
     int q0, n;       // first query token and their number
-    int len;         // tokens in the cache
+    int len;         // tokens that the page table has columns for
+    int pos;         // the first query token's position (the sequence may be longer than the table)
 };
 
 __device__ __forceinline__ Seq load_seq(const CacheView& c, int s)
@@ -101,8 +102,9 @@ __device__ __forceinline__ Seq load_seq(const CacheView& c, int s)
     const int64_t b = min(static_cast<int64_t>(max(c.cu[s + 1], 0)), c.tokens);
     r.q0 = static_cast<int>(a);
     r.n = static_cast<int>(max(b - a, static_cast<int64_t>(0)));
-    r.len = static_cast<int>(min(static_cast<int64_t>(max(c.kv_lens[s], 0)),
-                                 static_cast<int64_t>(c.table_cols) << c.page_log2));
+    const int whole = max(c.kv_lens[s], 0);
+    r.len = min(whole, c.table_cols << c.page_log2);        // (the product fits: checked on the host)
+    r.pos = whole - r.n;
     return r;
 }
 

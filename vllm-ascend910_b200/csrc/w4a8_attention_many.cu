@@ -149,7 +149,7 @@ __device__ __forceinline__ long long quotient(long long a, long long b)
 __device__ __forceinline__ int many_blocks(const Seq& s, int group, int t)
 {
     const int last = min(s.n - 1, static_cast<int>((static_cast<uint32_t>(t + 1) * kRows - 1) / static_cast<uint32_t>(group)));
-    const int lim = s.len - s.n + last;
+    const int lim = min(s.pos + last, s.len - 1);
     return lim < 0 ? 1 : lim / kBlk + 1;
 }
 
@@ -535,7 +535,7 @@ __device__ __forceinline__ void softmax_role(const AttentionParams& p, ManyBars*
         // (RPI rows a turn, a lane per 16 bytes), then a lane is a row: its largest
         // element to [2^13, 2^14), fp16, in place ----
         float qs = 0.0f;                                        // what turns a raw score into log2 units
-        const int limit = valid ? a.s.len - a.s.n + row_token(p, pr) : 0x7FFFFFFF;   // last token the row sees
+        const int limit = valid ? a.s.pos + row_token(p, pr) : 0x7FFFFFFF;   // last token the row sees
         {
             // (a lane finds its own row's place; the lanes that copy the row are told)
             const int tok = valid ? row_token(p, pr) : 0;

@@ -58,14 +58,16 @@ __device__ __forceinline__ void rotate_pair(float& a, float& b, float c, float s
 }
 
 // Bounds of sequence s: its first token in the call, their number, its length
-// after the call (kept inside the tensors).
+// after the call.  The length may pass what the page table has columns for
+// (capacity): tokens there have a position and no page.
 __device__ __forceinline__ void seq_bounds(const CacheView& c, int s, int64_t& t0, int& n, int& len)
 {
     t0 = min(static_cast<int64_t>(max(c.cu[s], 0)), c.tokens);
     const int64_t t1 = min(static_cast<int64_t>(max(c.cu[s + 1], 0)), c.tokens);
     n = static_cast<int>(max(t1 - t0, static_cast<int64_t>(0)));
-    len = static_cast<int>(min(static_cast<int64_t>(max(c.kv_lens[s], 0)), static_cast<int64_t>(c.table_cols) << c.page_log2));
+    len = max(c.kv_lens[s], 0);
 }
+__device__ __forceinline__ int capacity(const CacheView& c) { return c.table_cols << c.page_log2; }     // (checked on the host)
 
 // The sequence that token t belongs to: the last s with cu[s] <= t.  The whole
 // warp searches for its first token t0 (32 probes a step, so two dependent loads
@@ -160,8 +162,9 @@ __device__ __forceinline__ int touched_pages(const CacheView& cv, int s)
     int64_t t0;
     int n, len;
     seq_bounds(cv, min(s, cv.batch - 1), t0, n, len);
-    const int lo = max(len - n, 0);          // tokens before position 0 are not written
-    return s < cv.batch && len > lo ? ((len - 1) >> cv.page_log2) - (lo >> cv.page_log2) + 1 : 0;
+    const int lo = max(len - n, 0);          // tokens before position 0 are not written, nor those past the table
+    const int hi = min(len, capacity(cv));
+    return s < cv.batch && hi > lo ? ((hi - 1) >> cv.page_log2) - (lo >> cv.page_log2) + 1 : 0;
 }
 
 // Query heads of kQTok tokens.
@@ -382,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, 4) kv_write_kernel(const KvWritePara
 constexpr int kRTok = 16;          // most tokens of one block
 
 // bf16(code * scale) of each sequence's last cu[s + 1] - cu[s] tokens.  A token
-// without a page (or before position 0) reads as zeros.
+// without a page (or before position 0, or past the table) reads as zeros.
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvReadParams p, const int per)
 {
     __shared__ int64_t sh_ph[kRTok];       // page * kv_heads, or -1
@@ -398,7 +401,7 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvReadParams p,
         seq_bounds(cv, s, first, n, len);
         const int64_t pos = static_cast<int64_t>(len) - n + (t0 + tid - first);
         int id = -1;
-        if (pos >= 0 && pos < len) id = cv.table[static_cast<int64_t>(s) * cv.ld_table + (pos >> cv.page_log2)];
+        if (pos >= 0 && pos < min(len, capacity(cv))) id = cv.table[static_cast<int64_t>(s) * cv.ld_table + (pos >> cv.page_log2)];
         sh_ph[tid] = id >= 0 && id < cv.pages ? static_cast<int64_t>(id) * cv.kv_heads : -1;
         sh_row[tid] = static_cast<int>(pos & (cv.page - 1));
     }

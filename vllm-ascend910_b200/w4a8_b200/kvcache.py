@@ -12,7 +12,8 @@ where the step's tokens of sequence ``s`` are rows ``cu_q[s] .. cu_q[s + 1]`` of
 q, k, v and are that sequence's last tokens: ``kv_lens[s]`` counts them.  The
 lengths, offsets and the page table are read on the device, so a captured
 CUDA graph follows their contents; a page id outside the cache means "no
-page" (not written, not attended to, read as zeros).
+page" (not written, not attended to, read as zeros), and so does a length past the
+table's columns for the tokens there.
 
 Argument checks raise ``RuntimeError``; kernels run on the current stream of
 the tensors' device, whichever device is current.  The reference has no counterpart (its serving stack keeps a
