@@ -192,3 +192,33 @@ def test_captured_step_keeps_its_decoder():
     del run
     gc.collect()
     assert all(r() is None for r in held)
+
+
+def test_pages_refuse_lengths_past_the_positions():
+    from w4a8_b200 import decoder
+    p = decoder.Pages(100, 16, positions=40)
+    a, b = p.add(), p.add()
+    p.plan([a, b], [39, 40], "cpu")
+    free = p.free_pages
+    with pytest.raises(RuntimeError, match="41 tokens.*40 positions"):
+        p.plan([a, b], [1, 1], "cpu")
+    assert (p.length(a), p.length(b), p.free_pages) == (39, 40, free)      # as before the refusal
+    assert p.plan([a], [1], "cpu").kv_lens.tolist() == [40]
+    c = p.add()
+    with pytest.raises(RuntimeError, match="positions"):
+        p.plan([c], [41], "cpu")
+    unbounded = decoder.Pages(9, 16)
+    assert unbounded.plan([unbounded.add()], [100], "cpu").tokens == 100
+
+
+@pytest.mark.gpu
+def test_decoder_refuses_positions_past_its_table():
+    """A token without a row in the rotary table is refused, not turned by the last row's angles."""
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    dev = torch.device("cuda", 0)
+    dec, _ = _build(dev, 40)
+    s = dec.pages.add()
+    dec.pages.plan([s], [dec.cfg.positions], dev)
+    with pytest.raises(RuntimeError, match="positions"):
+        dec.pages.plan([s], [1], dev)

@@ -90,10 +90,13 @@ class Plan:
 
 
 class Pages:
-    """The pages of one cache geometry: free ones, and those that each sequence holds in order."""
+    """The pages of one cache geometry: free ones, and those that each sequence holds in order.
 
-    def __init__(self, pages: int, page_size: int):
-        self.page_size = page_size
+    ``positions``: rows of the rotary table, which no sequence may outgrow (past its end the
+    kernels would turn every token by the last row's angles)."""
+
+    def __init__(self, pages: int, page_size: int, positions: Optional[int] = None):
+        self.page_size, self.positions = page_size, positions
         self._free: List[int] = list(range(pages))[::-1]
         self._held: Dict[int, List[int]] = {}
         self._len: Dict[int, int] = {}
@@ -118,11 +121,15 @@ class Pages:
         del self._len[seq]
 
     def plan(self, seqs: Sequence[int], counts: Sequence[int], device, columns: int = 0) -> Plan:
-        """Lengthens each sequence by its count and lays out the step; nothing changes when pages run out."""
+        """Lengthens each sequence by its count and lays out the step; nothing changes when pages run out
+        or a sequence would outgrow the positions."""
         _check(len(seqs) == len(counts) and len(seqs) > 0, "Pages: a step needs sequences, and a count for each")
         _check(len(set(seqs)) == len(seqs), "Pages: a sequence can be in a step once")
         _check(all(n > 0 for n in counts), "Pages: each sequence of a step brings at least one token")
         S = self.page_size
+        longest = max(self._len[s] + n for s, n in zip(seqs, counts))
+        if self.positions is not None and longest > self.positions:
+            raise RuntimeError(f"Pages: a sequence of {longest} tokens, the rotary table has {self.positions} positions")
         need = [-(-(self._len[s] + n) // S) - len(self._held[s]) for s, n in zip(seqs, counts)]
         if sum(need) > len(self._free):
             raise RuntimeError(f"Pages: {sum(need)} pages needed, {len(self._free)} free")
@@ -148,7 +155,7 @@ class Decoder:
         self.cfg, self.layers, self.final_norm = cfg, list(layers), final_norm
         self.caches = [kvcache.KVCache.empty(pages, cfg.kv_heads, cfg.page_size, cfg.head_dim, device) for _ in layers]
         self.cos_sin = kvcache.rotary_table(cfg.head_dim, cfg.positions, cfg.rope_base, cfg.rope_scaling, device)
-        self.pages = Pages(pages, cfg.page_size)
+        self.pages = Pages(pages, cfg.page_size, cfg.positions)
 
     def step(self, h: torch.Tensor, plan: Plan) -> torch.Tensor:
         """Embedded tokens bf16 [tokens, hidden], in the plan's order -> the stack's normed output."""
