@@ -39,6 +39,12 @@
 //     of one segment are joined in the CTA; parts of CTAs by the last of them to
 //     finish (a counter tells which), always in unit order, so the bits do not
 //     depend on who is last.  Nothing waits for another CTA.
+//   * The counters outlive the call, so what an earlier one left must not matter,
+//     not even calls that overlapped on one workspace against its rule.  A word of
+//     the workspace counts started CTAs modulo four calls' worth: its quotient by
+//     the grid is the call's number modulo 4, the same for all of its CTAs since calls
+//     follow one another.  A segment's parts are counted in that byte of its word,
+//     and the CTA that owns the word clears the other three for the calls to come.
 //
 // Measured (B200, 40 query heads on 8 of 128): 64 single tokens at 64 to 8,191 (566 MB
 // of codes) 109 us, 5.2 TB/s, 79 % of a plain copy's rate; for seconds on end 124 us, since
@@ -264,6 +270,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
     __shared__ float piece_m[2 * C::WARPS][C::R], piece_l[2 * C::WARPS][C::R];
     __shared__ long long warp_sum[C::WARPS];
     __shared__ long long running;
+    __shared__ uint32_t byte_shift;                   // 8 * (the call's number modulo 4): the counters' byte
     __shared__ bool is_last[2];
     __shared__ int seg_cta0[2], seg_parts[2];
     long long* prefix = reinterpret_cast<long long*>(smem + C::SMEM);   // [batch + 1] units before each sequence
@@ -273,6 +280,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
     if (tid < 2 * C::WARPS) pieces[tid].seg = -1;
     if (tid == 0) running = 0;
     pdl_wait();
+    const uint32_t started = tid == 0 ? atomicInc(p.calls, 4 * gridDim.x - 1) : 0;     // (in flight during the scan)
 
     // ---- units before each sequence ----
     __syncthreads();
@@ -297,6 +305,10 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
         __syncthreads();
         if (tid == C::THREADS - 1) running = before + x;
         __syncthreads();
+    }
+    if (tid == 0) {
+        byte_shift = 8 * (started / gridDim.x);
+        atomicAnd(p.tickets + blockIdx.x, 0xFFu << byte_shift);
     }
     const long long total = running;
     // equal contiguous shares, none below the least: a short list leaves the last
@@ -753,14 +765,11 @@ __global__ void __launch_bounds__(C::THREADS, 1) attend_few_kernel(const Attenti
         seg_cta0[warp] = cta0;
         seg_parts[warp] = n;
         uint32_t ticket;
-        asm volatile("fence.acq_rel.gpu;\n\tatom.relaxed.gpu.global.add.u32 %0, [%1], 1;\n\tfence.acq_rel.gpu;"
+        asm volatile("fence.acq_rel.gpu;\n\tatom.relaxed.gpu.global.add.u32 %0, [%1], %2;\n\tfence.acq_rel.gpu;"
                      : "=r"(ticket)
-                     : "l"(p.tickets + cta0)
+                     : "l"(p.tickets + cta0), "r"(1u << byte_shift)
                      : "memory");
-        if (ticket == static_cast<uint32_t>(n - 1)) {
-            is_last[warp] = true;
-            p.tickets[cta0] = 0;
-        }
+        is_last[warp] = ((ticket >> byte_shift) & 0xFFu) == static_cast<uint32_t>(n - 1);
     }
     __syncthreads();
     for (int sl = 0; sl < 2; ++sl) {

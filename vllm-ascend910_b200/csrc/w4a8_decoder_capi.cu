@@ -10,7 +10,8 @@ using namespace w4a8;
 namespace {
 
 constexpr size_t kStatusBytes = 1024;      // status word block at the start of a workspace
-constexpr int kTicketWord = 16;            // first ticket word within it
+constexpr int kCallsWord = 8;              // the count of started CTAs within it
+constexpr int kTicketWord = 16;            // first ticket word within it (a byte counts up to 255 parts)
 constexpr int64_t kMaxTokens = int64_t(1) << 30;
 
 bool aligned(const void* ptr, uintptr_t a) { return (reinterpret_cast<uintptr_t>(ptr) & (a - 1)) == 0; }
@@ -155,6 +156,7 @@ int w4a8_attention(const w4a8_kv_cache* cache, const int32_t* page_table, int64_
     p.max_q = max_q_len;
     p.scale_log2 = softmax_scale * 1.4426950408889634f;
     p.status = static_cast<int*>(workspace);
+    p.calls = static_cast<uint32_t*>(workspace) + kCallsWord;
     p.tickets = static_cast<uint32_t*>(workspace) + kTicketWord;
     if (sms > static_cast<int>(kStatusBytes / 4) - kTicketWord) return W4A8_ERR_DEVICE;
     p.ws = static_cast<uint8_t*>(workspace) + kStatusBytes;

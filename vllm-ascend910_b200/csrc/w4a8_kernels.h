@@ -223,7 +223,8 @@ struct AttentionParams {
     int segments;             // about how many row tiles there are, of all heads and sequences (host's estimate)
     int few_most;             // attend_few_kernel takes sequences of at most this many packed rows
     int* status;              // workspace: status word
-    uint32_t* tickets;        // workspace: zeroed counters beside it, one per CTA (attend_few_kernel leaves them zero)
+    uint32_t* calls;          // workspace: CTAs of attend_few_kernel that have started, modulo four calls' worth
+    uint32_t* tickets;        // workspace: counters beside it, a word per CTA, a byte of it per call (modulo four)
     uint8_t* ws;              // workspace past the status block
 };
 

@@ -261,7 +261,10 @@ def attention(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor, kv_lens
     """Causal attention of the step's query tokens q [tokens, q_heads, head_dim] over the cache
     (``kv_write`` comes first: ``kv_lens`` counts these tokens).  q_heads is a multiple of the
     cache's kv_heads; ``max_q_len`` is the longest cu_q[s + 1] - cu_q[s]; ``scale`` defaults to
-    head_dim ** -0.5.  A row that sees no token is zero."""
+    head_dim ** -0.5.  A row that sees no token is zero.
+
+    Scratch is the device's workspace (``ops.workspace``), shared with the linears: calls on one device run
+    in stream order."""
     N = _lib.native()
     if N is not None and out is None:
         # a workspace that is too small for the call is refused, and grown below
