@@ -211,3 +211,23 @@ def test_every_wrapper_switches_to_its_tensors_device(dev, monkeypatch):
     names = [n for n, _ in seen]
     assert len(set(names)) >= 14 and {"w4a8_rms_norm", "w4a8_kv_write", "w4a8_kv_read", "w4a8_attention"} <= set(names)
     assert [n for n, ok in seen if not ok] == []
+
+
+@pytest.mark.gpu
+def test_refused_both_ways(dev, monkeypatch):
+    """A table without rows or columns, and tokens of no sequence: refused by the short way's call as by the long one."""
+    from w4a8_b200 import kvcache as kv
+    cache = kv.KVCache.empty(4, 2, 16, 64, dev)
+    i = dict(dtype=torch.int32, device=dev)
+    t, kl, cu = torch.tensor([[0, 1]], **i), torch.tensor([5], **i), torch.tensor([0, 5], **i)
+    k = torch.zeros(5, 2, 64, dtype=torch.bfloat16, device=dev)
+    calls = [lambda: kv.kv_write(cache, k, k, t, kl, cu, q=k, cos_sin=torch.empty(0, 64, device=dev)),
+             lambda: kv.kv_write(cache, k, k, t, kl, cu, cos_sin=torch.empty(8, 0, device=dev)),
+             lambda: kv.kv_write(cache, k, k, t[:0], kl[:0], cu[:1], q=k),
+             lambda: kv.kv_write(cache, k, k, t[:0], kl[:0], cu[:1])]
+    for f in calls:
+        with pytest.raises(RuntimeError):
+            f()
+        with pytest.raises(RuntimeError):
+            _long(monkeypatch, f)
+    assert kv.kv_write(cache, k[:0], k[:0], t[:0], kl[:0], cu[:1], q=k[:0]).shape == (0, 2, 64)

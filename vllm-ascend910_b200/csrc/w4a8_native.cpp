@@ -199,7 +199,8 @@ PyObject* kv_write(PyObject*, PyObject* const* a, Py_ssize_t n)
     }
     if (a[8] != Py_None) {
         cs = tensor(a[8]);
-        if (!dense(cs, at::kFloat, b.dev, 2)) return later();
+        // (an empty table's null pointer would mean "no rotary" to the C call)
+        if (!dense(cs, at::kFloat, b.dev, 2) || cs->numel() == 0) return later();
     }
     const int interleaved = PyObject_IsTrue(a[9]);
     if (interleaved < 0) {

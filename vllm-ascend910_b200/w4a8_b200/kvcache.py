@@ -219,8 +219,10 @@ def kv_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, page_table: torch
         if not (0 < rot <= cache.head_dim and rot % 16 == 0 and rows > 0):
             raise RuntimeError("kv_write: rot must be a multiple of 16, at most head_dim")
         cs = cos_sin.data_ptr()
-    if T == 0 or B == 0:
+    if T == 0:
         return out
+    if B == 0:
+        raise RuntimeError("kv_write: tokens of no sequence")
     rc = _launch(cache._index, _lib.lib().w4a8_kv_write, cache._ref, tp, ld, cols, kv_lens.data_ptr(), cu_q.data_ptr(), B,
                  T, kp, ldk, vp, ldv, qp, ldq, hq, op, ldo, cs, rows, rot, 1 if interleaved else 0, _stream_of(k))
     if rc != 0:
