@@ -175,3 +175,61 @@ def test_refusals():
     for f in bad:
         with pytest.raises(RuntimeError):
             f()
+
+
+@pytest.mark.parametrize("M,K,gk", [(3, 640, 128), (3, 2120, 1024), (2, 5120, 64), (900, 5120, 1024), (700, 2120, 256),
+                                    (2, 27648, 128), (3, 20000, 1024)])
+def test_products_out_of_fp32_range(M, K, gk):
+    """Large weights: x * weight is near or past fp32's range while the result is not.  The scale is the result's."""
+    from w4a8_b200 import ops
+    dev = _dev()
+    x, r, _ = _inputs(M, K, 5 * M + K)
+    x, r = (x.float() * 2.0 ** 40).to(torch.bfloat16), (r.float() * 2.0 ** 40).to(torch.bfloat16)
+    w = 1 + 0.2 * torch.randn(K, generator=torch.Generator().manual_seed(1))
+    w[7], w[K // 2], w[K - 1] = 2.0 ** 100, -2.0 ** 60, 2.0 ** 90
+    q, s, _ = ops.rms_norm_quant(x.to(dev), w.to(dev), gk, 1e-6, residual=r.to(dev), scale_dtype=torch.float32)
+    y, _ = norm64(x, r, w.double().numpy(), 1e-6)
+    q, s = q.cpu().numpy().astype(np.float64), s.double().cpu().numpy()
+    assert np.isfinite(s).all()
+    for g in range(-(-K // gk)):
+        part = y[:, g * gk:(g + 1) * gk]
+        amax = np.abs(part).max(1)
+        assert (np.abs(s[g] - amax / 127) <= (2.0 ** -8 + 1e-5) * amax / 127).all()
+        back = q[:, g * gk:(g + 1) * gk] * s[g][:, None]
+        assert (np.abs(back - part) <= (0.5 + 127 * 2e-5) * s[g][:, None]).all()
+
+
+@pytest.mark.parametrize("K,gk", [(640, 128), (5120, 1024)])
+def test_rows_whose_squares_overflow(K, gk):
+    """Magnitudes past 2^64: the sum of squares is infinite and the row zero, with codes as without them."""
+    from w4a8_b200 import ops
+    dev = _dev()
+    x, _, w = _inputs(4, K, 6, False)
+    x[1] = (x[1].float() * 2.0 ** 70).to(torch.bfloat16)
+    x[2] = (x[2].float() * 2.0 ** 100).to(torch.bfloat16)
+    y = ops.rms_norm(x.to(dev), w.to(dev), 1e-6)
+    assert (y[1:3] == 0).all() and torch.isfinite(y).all()
+    q, s, _ = ops.rms_norm_quant(x.to(dev), w.to(dev), gk, 1e-6)
+    assert (q[1:3] == 0).all() and (s[:, 1:3].float() == torch.finfo(torch.bfloat16).tiny).all()
+    q0, s0, _ = ops.rms_norm_quant(x[[0, 3]].contiguous().to(dev), w.to(dev), gk, 1e-6)
+    assert torch.equal(q[[0, 3]], q0) and torch.equal(s[:, [0, 3]], s0)
+
+
+def test_linear_on_a_norm_out_of_fp32_range():
+    """The operand tiles take the same codes and scales."""
+    from w4a8_b200 import ops
+    dev = _dev()
+    M, N, K, gk = 20, 64, 1288, 1024
+    x, r, w = (t.to(dev) for t in _inputs(M, K, 21, True, torch.float32))
+    x, r = x * 2.0 ** 40, r * 2.0 ** 40
+    w[3], w[1100] = 2.0 ** 50, -2.0 ** 52
+    g = torch.Generator().manual_seed(2)
+    packed = ops.pack_int4_grouped(torch.randint(-8, 8, (N, K), generator=g, dtype=torch.int8), gk).to(dev)
+    ws = torch.ones(2, N, device=dev)
+    y, _ = ops.linear_prepared_rms_norm(x, w, ops.prepare_weights(packed, ws, None, K, gk), 1e-6, residual=r)
+    q, s, _ = ops.rms_norm_quant(x, w, gk, 1e-6, residual=r, scale_dtype=torch.float32)
+    assert torch.isfinite(s).all() and torch.isfinite(y).all()
+    codes = ops.unpack_int4_grouped(packed.cpu(), K, gk).double()
+    q, s = q.cpu().double(), s.cpu().double()
+    want = sum((q[:, a:a + gk] @ codes[:, a:a + gk].T) * s[i][:, None] for i, a in enumerate(range(0, K, gk)))
+    assert ((y.cpu().double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -20 * want.abs().max()).all()

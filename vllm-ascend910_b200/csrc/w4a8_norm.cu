@@ -8,7 +8,9 @@
 //   kNormBf16    y rounded once to bf16
 //   kNormCodes   int8 codes [M, K] and scales [G, M], the activation quantiser's
 //                rule (w4a8_common.cuh) applied to the fp32 y: one rounding
-//                where norm, store and quantise would make two
+//                where norm, store and quantise would make two.  A group's maximum
+//                is that of |h w|, times n, two fp32 roundings from max|y|: of bf16
+//                scales of random rows one in 100,000 is the next one for it
 //   kNormTiles   the same codes and scales in the GEMM's operand order, straight
 //                into a linear call's workspace (QuantParams' kOutKernel form)
 //
@@ -22,7 +24,7 @@
 // fp32 arithmetic runs in pairs, two elements an instruction; each rounds alone.
 //
 // Measured (B200, rows of 5120 with a residual): 4096 rows, bf16 out 27.5 us, 6.1 TB/s, 93 %
-// of a plain copy's rate; 8191 rows with codes 62 us in groups of 128 or 1024, 4.7 TB/s:
+// of a plain copy's rate; 8191 rows with codes 63 and 64 us in groups of 128 and 1024, 4.6 TB/s:
 // about 560 instructions for a thread's 16 elements bound it, not the memory (before the
 // pairs, the bodies without bounds tests and groups by vector order 75 and 96 us).  One
 // row: 1.9 us, launch and two load latencies.
@@ -106,6 +108,20 @@ __device__ __forceinline__ void load_weight8(const NormParams& p, int pos, uint6
     }
 }
 
+// The largest |h w| 2^-128 of 8 elements, as bits with the sign set.
+__device__ __forceinline__ uint32_t far_max(const uint64_t (&h)[4], const uint64_t (&w)[4])
+{
+    const uint64_t down = pair2(0x1p-64f, 0x1p-64f);
+    float a = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float lo, hi;
+        unpair2(f2_mul(f2_mul(h[i], down), f2_mul(w[i], down)), lo, hi);
+        a = max_abs_nan(a, lo, hi);
+    }
+    return __float_as_uint(a) | 0x80000000u;
+}
+
 template <int OUT, int VPT, bool WHOLE>
 __global__ void __launch_bounds__(VPT == 2 ? 512 : kMaxNormThreads, VPT == 2 ? 2 : 1) rms_norm_kernel(const NormParams p)
 {
@@ -174,8 +190,10 @@ __global__ void __launch_bounds__(VPT == 2 ? 512 : kMaxNormThreads, VPT == 2 ? 2
 
         // ---- sum of squares over the block; group maxima of |h w| on the way ----
         // max|y| is max|h w| * n up to fp32 rounding, so the maxima need not wait for
-        // the sum.  The 2^40 keeps tiny products normal; large ones are out of range
-        // only where the sum of squares is too.
+        // the sum.  The 2^40 keeps tiny products normal.  Products of 2^88 and more leave
+        // fp32's range so: a thread that meets one (or a NaN or infinity) takes its maximum
+        // times 2^-128 instead, where no finite product overflows, and says so by the sign
+        // bit, which also makes it the larger of any two as bits.
         uint32_t amax[VPT];
         const int tpg = p.gk >> 3;
         if (OUT != kNormBf16) {
@@ -191,6 +209,16 @@ __global__ void __launch_bounds__(VPT == 2 ? 512 : kMaxNormThreads, VPT == 2 ? 2
                 }
                 amax[j] = __float_as_uint(a);          // (as bits, a NaN is the largest)
             }
+            uint32_t far = amax[0];
+#pragma unroll
+            for (int j = 1; j < VPT; ++j) far = max(far, amax[j]);
+            if (far >= 0x7F800000u)
+#pragma unroll
+                for (int j = 0; j < VPT; ++j)
+                    if (amax[j] >= 0x7F800000u) {
+                        if (!kKeep) load_weight8(p, (j * T + tid) * 8, w[0]);
+                        amax[j] = far_max(h[j], w[kKeep ? j : 0]);
+                    }
             for (int o = (tpg < 32 ? tpg : 32) >> 1; o > 0; o >>= 1)
 #pragma unroll
                 for (int j = 0; j < VPT; ++j) amax[j] = max(amax[j], __shfl_xor_sync(0xffffffffu, amax[j], o));
@@ -234,12 +262,23 @@ __global__ void __launch_bounds__(VPT == 2 ? 512 : kMaxNormThreads, VPT == 2 ? 2
             }
         }
         const float n40 = n * 0x1p-40f;
+        float most[VPT];
+        uint32_t far = 0;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            most[j] = __uint_as_float(amax[j]) * n40;
+            far |= amax[j];
+        }
+        if (far >> 31)
+#pragma unroll
+            for (int j = 0; j < VPT; ++j)
+                if (amax[j] >> 31) most[j] = __uint_as_float(amax[j] & 0x7FFFFFFFu) * n * 0x1p64f * 0x1p64f;
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             const int pos = (j * T + tid) * 8;
             float y[8];
             unpair8(h[j], y);
-            const uint16_t sb = act_scale_bits(__uint_as_float(amax[j]) * n40);
+            const uint16_t sb = act_scale_bits(most[j]);
             const float s = bf16_bits_to_f32(sb);
             uint2 q;                                   // 8 codes, a byte each
             if (act_scale_fast(sb)) {
