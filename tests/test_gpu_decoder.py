@@ -222,3 +222,19 @@ def test_decoder_refuses_positions_past_its_table():
     dec.pages.plan([s], [dec.cfg.positions], dev)
     with pytest.raises(RuntimeError, match="positions"):
         dec.pages.plan([s], [1], dev)
+
+
+@pytest.mark.gpu
+def test_captured_step_refuses_what_the_step_refuses():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    dev = torch.device("cuda", 0)
+    dec, _ = _build(dev, 24)
+    seqs = [dec.pages.add() for _ in range(3)]
+    plan = dec.pages.plan(seqs, [1, 1, 1], dev)
+    run = dec.capture(plan)
+    for bad in (torch.zeros(1, 512, dtype=torch.bfloat16, device=dev), torch.zeros(512, dtype=torch.bfloat16, device=dev),
+                torch.zeros(3, 512, device=dev)):
+        for f in (run, dec.step):
+            with pytest.raises(RuntimeError):
+                f(bad, plan)

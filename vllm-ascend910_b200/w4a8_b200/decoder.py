@@ -208,6 +208,10 @@ class Captured:
 
     def __call__(self, h: torch.Tensor, plan: Plan) -> torch.Tensor:
         """The step's output; the next call overwrites it."""
+        # (copy_ would repeat a row for every token and convert types)
+        if h.shape != self.h.shape or h.dtype is not self.h.dtype:
+            raise RuntimeError(f"the captured step takes bfloat16 [{self.h.shape[0]}, {self.h.shape[1]}]; "
+                               f"got {h.dtype} {list(h.shape)}")
         self.h.copy_(h)
         self.plan.copy_(plan)
         self.graph.replay()
