@@ -145,3 +145,14 @@ def test_cpu_tensors_are_refused():
         ops.rms_norm(x, torch.ones(64, dtype=torch.bfloat16))
     with pytest.raises(RuntimeError):
         kvcache.KVCache.empty(2, 1, 16, 64, "cpu")
+
+
+def test_cache_table_past_64_bits_is_refused():
+    """Columns whose tokens do not fit 32 bits, however many: their product with the page size must not wrap."""
+    _lib, L = _lib_or_skip()
+    c = ctypes.byref(_lib.KvCacheDesc(A, 2 * A, 3 * A, 4 * A, 8, 2, 16, 64, 0))
+    for cols in (1 << 27, 1 << 30, 1 << 60, (1 << 60) + 4, (1 << 63) - 1):
+        assert L.w4a8_kv_read(c, 5 * A, cols, cols, 6 * A, 7 * A, 2, 0, None, None, None) == _lib.ERR_INVALID, cols
+        assert L.w4a8_attention(c, 5 * A, cols, cols, 6 * A, 7 * A, 2, 0, None, 256, 4, 3, 0.1, None, 256, None, 0,
+                                None) == _lib.ERR_INVALID, cols
+    assert L.w4a8_kv_read(c, 5 * A, 4, 4, 6 * A, 7 * A, 2, 0, None, None, None) == _lib.OK

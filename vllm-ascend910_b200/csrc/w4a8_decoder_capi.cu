@@ -25,7 +25,7 @@ int make_view(const w4a8_kv_cache* c, const int32_t* table, int64_t ld_table, in
     if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128) return W4A8_ERR_UNSUPPORTED;
     if (c->kv_heads <= 0 || c->kv_heads > 4096 || c->pages <= 0 || c->pages > 0x7FFFFFFF) return W4A8_ERR_INVALID;
     if (tokens > kMaxTokens || batch > kMaxTokens || table_cols < 0 || ld_table < table_cols) return W4A8_ERR_INVALID;
-    if (table_cols * c->page_size > 0x7FFFFFFF) return W4A8_ERR_INVALID;
+    if (table_cols > 0x7FFFFFFF / c->page_size) return W4A8_ERR_INVALID;
     if (batch == 0 || tokens == 0) {
         *out = CacheView{};
         return W4A8_OK;
