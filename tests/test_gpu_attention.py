@@ -321,3 +321,44 @@ def test_counters_left_by_a_spoiled_call(qs, lens):
         words[16:16 + sms] = stale
         for _ in range(6):
             assert torch.equal(c.run(cache), first)
+
+
+# one kv head and a long context: parts of tens of CTAs, shares of one unit and of several
+LONG = [
+    # hq, d, page, query tokens, lengths
+    (5, 128, 16, [1], [4000]),
+    (5, 128, 16, [1], [16000]),
+    (8, 64, 32, [1], [16000]),
+    (1, 64, 16, [1], [5003]),
+    (5, 128, 32, [3], [4000]),
+    (5, 128, 16, [3], [16000]),
+    (5, 128, 64, [5, 2], [9000, 16000]),
+    (4, 64, 16, [4], [12001]),
+    (5, 128, 16, [1] * 7, [1000, 3, 500, 16, 77, 2000, 15]),
+    (5, 128, 16, [5, 4], [700, 900]),
+]
+
+
+@pytest.mark.parametrize("hq,d,page,qs,lens", LONG)
+def test_long_contexts_against_64_bits(hq, d, page, qs, lens):
+    """Segments that many CTAs share: their join against 64 bits."""
+    c = Case(hq, 1, d, page, qs, lens, seed=15 + d)
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("hq,d,page,qs,lens", LONG[:8] + [(5, 128, 16, [40], [6000])])
+@pytest.mark.parametrize("falling", [False, True])
+def test_scores_that_grow_along_the_context(hq, d, page, qs, lens, falling):
+    """Scores whose deviation grows (or falls) twentyfold along the context: parts joined later outweigh earlier ones.
+
+    Deviations up to about 15: the products of one score have magnitudes that sum to about 0.64 sqrt(D) 15 = 110, so
+    their fp32 sum is off by D 2^-24 110 = 8.4e-4 at most, in numerator and denominator: 2e-3 of sum p |v| beside
+    the bound above."""
+    c = Case(hq, 1, d, page, qs, lens, seed=16 + d)
+    for s, n in enumerate(lens):
+        pages = -(-n // page)
+        ramp = torch.linspace(0.5, 10.0, pages)
+        c.scales[0][c.table[s][:pages], 0] = (ramp.flip(0) if falling else ramp) * 2.6 / 127
+    ref, mag = c.ref()
+    got = bf16_np(c.run())
+    assert (np.abs(got - ref) <= 2.0 ** -8 * np.abs(ref) + (2.0 ** -10 + 2e-3) * mag).all()
