@@ -47,11 +47,11 @@
 //     and the CTA that owns the word clears the other three for the calls to come.
 //
 // Measured (B200, 40 query heads on 8 of 128): 64 single tokens at 64 to 8,191 (566 MB
-// of codes) 109 us, 5.2 TB/s, 79 % of a plain copy's rate; for seconds on end 124 us, since
-// the board's power limit takes the SM clock from 1,965 to 1,730 MHz: bytes and
-// conversions cost power before they cost time.  One token at 4,000: 13.7 us, of which
+// of codes) 108 us, 5.3 TB/s, 80 % of a plain copy's rate; for three seconds on end 123 us, at
+// 996 W and an SM clock of 1,680 MHz instead of 1,965 (sampled, power cap active).  One
+// token at 4,000: 14 us, of which
 // the codes are 1.3: launch, the lists, a chain of loads and the join.  12 x 2-5 drafted
-// tokens at 3,000 to 16,000, one kv head: 29 us for 26 MB: a CTA's warps wait for few units
+// tokens at 3,000 to 16,000, one kv head: 28 us for 26 MB: a CTA's warps wait for few units
 // each, and 10 to 25 rows take up to four products of 8 rows a unit.
 #include <algorithm>
 

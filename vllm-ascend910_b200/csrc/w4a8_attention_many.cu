@@ -48,9 +48,10 @@
 // exponential unit (16 / clock / SM), about 1,500 cycles of shared memory (128 KB of
 // operands, 64 KB of codes and their conversion), about 1,200 issue slots per scheduler.
 // Measured (B200, 40 query heads on 8 of 128): 2,400 cycles a step, and 10,000 for a
-// tile's queries and output; three prompts of 1,364-1,668 tokens behind 179-791 184 us, 670
-// TFLOP/s; one prompt of 2,048, 4,096 and 8,192 tokens 77, 228 and 789 us, 556, 753 and 871
-// TFLOP/s, the last at 1,800 MHz: it reaches the board's power limit.
+// tile's queries and output; three prompts of 1,364-1,668 tokens behind 179-791 178 us, 692
+// TFLOP/s; one prompt of 2,048, 4,096 and 8,192 tokens 77, 215 and 721 us, 554, 798 and 954
+// TFLOP/s.  For three seconds on end 183, 76, 227 and 791 us, at 1,912, 1,965, 1,867 and 1,800 MHz:
+// all but the 2,048 reach the board's power limit.
 #include <algorithm>
 
 #include "w4a8_attention.cuh"

@@ -24,15 +24,16 @@
 // (kv head, K or V) items: a warp holds 4 rows of 128 elements in registers (a page
 // of 32 rows is eight warps), so k and v are read once -- rotated, their maximum found, and
 // written as codes.  All loads of a warp are in flight together, and four blocks an SM
-// (64 registers) hide more than three or five do: 7,543 tokens 53 us against 58 and 69.
+// (64 registers, for 56 bytes of spills) hide more than three or five do: 7,543 tokens
+// 53 us against 58 and 69.
 // A loop over several items a block was slower too (68 us).  Dividing by the scale is a
 // product with its reciprocal except next to half-integers, where the true division
 // decides (the activation quantiser's rule).
 //
-// Measured (B200): 7,543 tokens of 40 + 8 + 8 heads of 128, pages of 32: write 51 us, of
+// Measured (B200): 7,543 tokens of 40 + 8 + 8 heads of 128, pages of 32: write 50 us, of
 // which the queries' 155 MB alone take 24 at the memory's rate and the pages, by a chain of
 // dependent loads (lengths, rows and page id, scale) and some 650 instructions a warp in each
-// of 3,800 blocks, 28; read back 9 us (47 MB).  One token of 64 sequences written: 5.2 us; 530
+// of 3,800 blocks, 27; read back 9 us (47 MB).  One token of 64 sequences written: 5.2 us; 530
 // tokens read back: 2.9 us: launch and latency.
 #include <algorithm>
 

@@ -16,6 +16,8 @@
 //
 // A block holds one row in registers: a thread owns VPT vectors of 8 consecutive
 // elements (16-byte loads), so x and r are read once and y, r' are written once.
+// (At 64 registers a thread the compiler spills some: up to 56 bytes with two vectors,
+// 208 to 560 with four, which rows wider than 8,192 take, and whose weight is read for every row.)
 // Blocks stay for several rows when there are many: the weight is read once, and
 // the next row's loads are on their way while this one is reduced.  The sum of
 // squares takes one warp reduction and one barrier; the fp32 parts are added in a
@@ -25,9 +27,10 @@
 //
 // Measured (B200, rows of 5120 with a residual): 4096 rows, bf16 out 27.5 us, 6.1 TB/s, 93 %
 // of a plain copy's rate; 8191 rows with codes 63 and 64 us in groups of 128 and 1024, 4.6 TB/s:
-// about 560 instructions for a thread's 16 elements bound it, not the memory (before the
+// about 570 instructions for a thread's 16 elements bound it, not the memory (before the
 // pairs, the bodies without bounds tests and groups by vector order 75 and 96 us).  One
-// row: 1.9 us, launch and two load latencies.
+// row: 1.9 us, launch and two load latencies.  Rows of 27,648, whose spills and weights pass
+// through L1: 2,048 of them 105 us, 4.3 TB/s, and 147 with codes, 2.7 TB/s.
 #include <algorithm>
 
 #include "w4a8_common.cuh"

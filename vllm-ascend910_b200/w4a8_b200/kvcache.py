@@ -263,7 +263,7 @@ def attention(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor, kv_lens
     """Causal attention of the step's query tokens q [tokens, q_heads, head_dim] over the cache
     (``kv_write`` comes first: ``kv_lens`` counts these tokens).  q_heads is a multiple of the
     cache's kv_heads; ``max_q_len`` is the longest cu_q[s + 1] - cu_q[s]; ``scale`` defaults to
-    head_dim ** -0.5.  A row that sees no token is zero.
+    head_dim ** -0.5.  A row that sees no token is zero; a row that ``cu_q`` gives to no sequence is not written.
 
     Scratch is the device's workspace (``ops.workspace``), shared with the linears: calls on one device run
     in stream order."""
