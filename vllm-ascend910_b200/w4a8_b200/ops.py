@@ -74,7 +74,8 @@ def _stream_of(t: torch.Tensor) -> int:
     return _stream(t.device)
 
 
-_current_index = torch._C._cuda_getDevice      # (a tenth of torch.cuda.current_device()'s time)
+# (the raw lookup skips the initialisation check that current_device() makes per call)
+_current_index = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _launch(index: int, fn, *args) -> int:
