@@ -273,6 +273,42 @@ W4A8_API int w4a8_linear_prepared_rms_norm(const void* x, int64_t M, int64_t K, 
                                            const void* prepared, int32_t w_scale_dtype, int32_t has_zero, void* y,
                                            int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- linears in 8-bit integers ----
+ * One scale per token, one per output channel (the vendor's W8A8_DYNAMIC projections;
+ * the reference has such a linear as its comparison arm, npu_ops/python/vllm_engine_patch.py:107-158):
+ *   s[t] = max|h[t]| / 127,  q[t, k] = rint(h[t, k] / s[t])     (IEEE fp32, half-even)
+ *   y[t, n] = bf16(sum_k q[t, k] w[n, k] * s[t] * w_scale[n] + bias[n])
+ * with exact 32-bit integer sums, the sum's scales and bias applied in fp32 in this order.
+ * A token of zeros has scale 0; one with a value that is not finite has scale NaN, and its row of
+ * y is NaN.  h is x; bf16(silu(gate) * up) of x = [gate | up] with act = W4A8_ACT_SWIGLU
+ * (ldx >= 2 K); or the root-mean-square norm of x (+ residual) as w4a8_rms_norm, in fp32.
+ *   x          bf16 [M, ldx]
+ *   w          int8 [N, ldw], ldw >= K a multiple of 16, 16-byte aligned
+ *   w_scale    f32 [N];  bias f32 [N] or NULL
+ *   y          bf16 [M, ldy]
+ * 1 <= K <= W4A8_INT8_MAX_K (with a norm: W4A8_NORM_MAX_K); M, N <= 2^24.
+ * Workspace: w4a8_int8_workspace_size bytes, rules as for the linear calls, with which it
+ * may be shared in stream order. */
+#define W4A8_INT8_MAX_K 131071
+W4A8_API size_t w4a8_int8_workspace_size(int64_t M, int64_t K);
+/* The token quantiser alone: q int8 [M, ldq], scale f32 [M]. */
+W4A8_API int w4a8_int8_quant(const void* x, int64_t M, int64_t K, int64_t ldx, int32_t act, int8_t* q, int64_t ldq,
+                             float* scale, void* stream);
+/* The product alone, on codes q int8 [M, ldq] (16-byte aligned, ldq a multiple of 16) and their scales.
+ * Codes may be -128..127.  workspace: 1024 bytes for the status word. */
+W4A8_API int w4a8_int8_gemm(const int8_t* q, int64_t ldq, const float* scale, int64_t M, int64_t K, const int8_t* w,
+                            int64_t ldw, const float* w_scale, const float* bias, int64_t N, void* y, int64_t ldy,
+                            void* workspace, size_t workspace_bytes, void* stream);
+W4A8_API int w4a8_int8_linear(const void* x, int64_t M, int64_t K, int64_t ldx, int32_t act, const int8_t* w, int64_t ldw,
+                              const float* w_scale, const float* bias, int64_t N, void* y, int64_t ldy, void* workspace,
+                              size_t workspace_bytes, void* stream);
+/* Behind a norm: residual, residual_out, weight and eps as in w4a8_rms_norm. */
+W4A8_API int w4a8_int8_linear_rms_norm(const void* x, int64_t M, int64_t K, int64_t ldx, const void* residual, int64_t ldr,
+                                       void* residual_out, int64_t ldro, const void* weight, int32_t weight_dtype,
+                                       float eps, const int8_t* w, int64_t ldw, const float* w_scale, const float* bias,
+                                       int64_t N, void* y, int64_t ldy, void* workspace, size_t workspace_bytes,
+                                       void* stream);
+
 /* ---- paged 8-bit key / value cache ----
  * No counterpart in the reference (its serving stack keeps a bf16 cache).  One
  * layer's cache: int8 codes [pages, kv_heads, page_size, head_dim] and one fp32

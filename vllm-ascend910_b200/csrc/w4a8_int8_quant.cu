@@ -1,0 +1,228 @@
+// w4a8_int8_quant.cu -- activations for the 8-bit linears: int8 codes with one
+// scale per token.
+//
+//   s = max|h| / 127     q = rint(h / s), within +-127     (IEEE fp32, half-even)
+//
+// of a row h that is x itself, bf16(silu(gate) * up) of x = [gate | up], or the
+// root-mean-square norm of x (+ residual) in fp32:
+//
+//   h = (x + r) / sqrt(sum((x + r)^2) / K + eps) * weight     r' = bf16(x + r)
+//
+// A row of zeros has s = 0 and codes 0; a row with a value that is not finite has
+// s = NaN and codes 0, so that its outputs are NaN.
+//
+// A block holds one row in registers, 8 elements of 16 bytes a vector and up to four
+// vectors a thread (32,768 elements): x is read once.  Longer rows are read twice, the
+// second time out of L2.  The sum of squares and the maximum each take a
+// warp reduction and a barrier; partial sums are added in a fixed order.
+#include <algorithm>
+
+#include "w4a8_common.cuh"
+#include "w4a8_kernels.h"
+
+namespace w4a8 {
+
+namespace {
+
+constexpr int kMaxTokThreads = 1024;
+
+__device__ __forceinline__ void load8(const uint16_t* row, int pos, int K, bool vec, float (&v)[8])
+{
+    if (vec && pos + 8 <= K) {
+        unpack8_bf16(*reinterpret_cast<const uint4*>(row + pos), v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = pos + i < K ? bf16_bits_to_f32(row[pos + i]) : 0.0f;
+    }
+}
+
+__device__ __forceinline__ void store8(uint16_t* row, int pos, int K, bool vec, const float (&v)[8])
+{
+    if (vec && pos + 8 <= K) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+        *reinterpret_cast<uint4*>(row + pos) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (pos + i < K) row[pos + i] = f32_to_bf16_bits(v[i]);
+    }
+}
+
+__device__ __forceinline__ void load_weight8(const TokenQuantParams& p, int pos, float (&w)[8])
+{
+    if (p.weight_f32) {
+        const float* wf = static_cast<const float*>(p.weight);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = pos + i < p.K ? wf[pos + i] : 0.0f;
+    } else {
+        load8(static_cast<const uint16_t*>(p.weight), pos, p.K, p.vec_w, w);
+    }
+}
+
+// 8 elements of h before any norm.
+template <int SRC>
+__device__ __forceinline__ void row8(const TokenQuantParams& p, const uint16_t* x, const uint16_t* r, int pos, float (&v)[8])
+{
+    load8(x, pos, p.K, p.vec_x, v);
+    if (SRC == kTokSwiglu) {
+        float u[8];
+        load8(x + p.K, pos, p.K, p.vec_x && p.K % 8 == 0, u);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = swiglu_bf16(v[i], u[i]);
+    } else if (SRC == kTokNorm && r) {
+        float u[8];
+        load8(r, pos, p.K, p.vec_r, u);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = __fadd_rn(v[i], u[i]);
+    }
+}
+
+// 4 codes, a byte each, by the division alone: scales whose reciprocal fp32 cannot hold.
+__device__ __forceinline__ uint32_t codes4_div(const float* x, float s)
+{
+    uint32_t w = 0;
+    if (s > 0.0f)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float q = fminf(fmaxf(rintf(__fdiv_rn(x[i], s)), -127.0f), 127.0f);
+            w |= (static_cast<uint32_t>(static_cast<int>(q)) & 0xFFu) << (8 * i);
+        }
+    return w;
+}
+
+__device__ __forceinline__ void emit8(const TokenQuantParams& p, int8_t* q, int pos, const float (&v)[8], float s, float rcp,
+                                      bool fast)
+{
+    // (|h / s| < 127.5: s is the rounded quotient of the row's maximum and 127)
+    const uint32_t lo = fast ? codes4(v, s, rcp) : codes4_div(v, s), hi = fast ? codes4(v + 4, s, rcp) : codes4_div(v + 4, s);
+    if (p.vec_q && pos + 8 <= p.K) {
+        *reinterpret_cast<uint2*>(q + pos) = make_uint2(lo, hi);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (pos + i < p.K) q[pos + i] = static_cast<int8_t>((i < 4 ? lo : hi) >> (8 * (i & 3)));
+    }
+}
+
+// VPT vectors a thread in registers; 0: the row is read twice.
+template <int SRC, int VPT>
+__global__ void __launch_bounds__(kMaxTokThreads) token_quant_kernel(const TokenQuantParams p)
+{
+    __shared__ float red_sum[kMaxTokThreads / 32];
+    __shared__ uint32_t red_max[kMaxTokThreads / 32];
+    const int tid = threadIdx.x, T = blockDim.x, nw = T >> 5;
+    // The product that follows may start once everything before this kernel is done: it reads its weights
+    // without waiting for the codes.
+    pdl_wait();
+    pdl_launch_dependents();
+
+    const int64_t row = blockIdx.x;
+    const uint16_t* x = p.x + row * p.ldx;
+    const uint16_t* r = SRC == kTokNorm && p.res ? p.res + row * p.ldr : nullptr;
+    constexpr int HOLD = VPT ? VPT : 1;
+    const int vecs = VPT ? VPT : (p.K + 8 * T - 1) / (8 * T);
+    float h[HOLD][8];
+    float ss = 0.0f, big = 0.0f;
+#pragma unroll
+    for (int j = 0; j < vecs; ++j) {
+        const int pos = (j * T + tid) * 8;
+        float (&v)[8] = h[VPT ? j : 0];
+        if (pos < p.K) {
+            row8<SRC>(p, x, r, pos, v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+        }
+        if (SRC == kTokNorm) {
+            if (p.res_out && pos < p.K) store8(p.res_out + row * p.ldro, pos, p.K, p.vec_ro, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) big = max_abs_nan(big, v[i], v[i + 1]);
+        }
+    }
+    if (SRC == kTokNorm) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (lane_id() == 0) red_sum[warp_id()] = ss;
+        __syncthreads();
+        ss = static_cast<int>(lane_id()) < nw ? red_sum[lane_id()] : 0.0f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float n = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(ss, static_cast<float>(p.K)) + p.eps));
+#pragma unroll
+        for (int j = 0; j < HOLD; ++j) {
+            const int pos = (j * T + tid) * 8;
+            if (pos >= p.K) continue;
+            float w[8];
+            load_weight8(p, pos, w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h[j][i] = __fmul_rn(__fmul_rn(h[j][i], n), w[i]);
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) big = max_abs_nan(big, h[j][i], h[j][i + 1]);
+        }
+    }
+    uint32_t amax = __reduce_max_sync(0xffffffffu, __float_as_uint(big));     // (as bits, a NaN is the largest)
+    if (lane_id() == 0) red_max[warp_id()] = amax;
+    __syncthreads();
+    amax = __reduce_max_sync(0xffffffffu, static_cast<int>(lane_id()) < nw ? red_max[lane_id()] : 0u);
+    const bool finite = amax < 0x7F800000u;
+    const float s = finite ? __fdiv_rn(__uint_as_float(amax), 127.0f) : __uint_as_float(0x7FC00000u);
+    if (tid == 0) p.scale[row] = s;
+    const bool fast = finite && s >= 1.1754943508222875e-38f;
+    const float rcp = fast ? __frcp_rn(s) : 0.0f;
+    int8_t* q = p.q + row * p.ldq;
+#pragma unroll
+    for (int j = 0; j < vecs; ++j) {
+        const int pos = (j * T + tid) * 8;
+        if (pos >= p.K) continue;
+        if (!VPT) row8<SRC>(p, x, r, pos, h[0]);
+        emit8(p, q, pos, h[VPT ? j : 0], s, rcp, fast);
+    }
+}
+
+template <int SRC, int VPT>
+cudaError_t launch(const TokenQuantParams& p, int threads, cudaStream_t stream)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.M);
+    cfg.blockDim = dim3(threads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, token_quant_kernel<SRC, VPT>, p);
+}
+
+template <int SRC>
+cudaError_t launch_source(const TokenQuantParams& p, cudaStream_t stream)
+{
+    const int nvec = (p.K + 7) / 8;
+    const auto threads = [&](int vpt) { return ((nvec + vpt - 1) / vpt + 31) / 32 * 32; };
+    if (threads(1) <= kMaxTokThreads) return launch<SRC, 1>(p, threads(1), stream);
+    if (threads(2) <= kMaxTokThreads) return launch<SRC, 2>(p, threads(2), stream);
+    if (threads(4) <= kMaxTokThreads) return launch<SRC, 4>(p, threads(4), stream);
+    if (SRC == kTokNorm) return cudaErrorInvalidValue;
+    return launch<SRC == kTokNorm ? kTokPlain : SRC, 0>(p, kMaxTokThreads, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_token_quant(const TokenQuantParams& p, int source, cudaStream_t stream)
+{
+    switch (source) {
+        case kTokPlain: return launch_source<kTokPlain>(p, stream);
+        case kTokSwiglu: return launch_source<kTokSwiglu>(p, stream);
+        default: return launch_source<kTokNorm>(p, stream);
+    }
+}
+
+}  // namespace w4a8

@@ -234,9 +234,56 @@ cudaError_t launch_kv_read(const KvReadParams& p, cudaStream_t stream);
 size_t attention_ws_bytes(int batch, int64_t tokens, int q_heads, int kv_heads, int D, int max_q, int sms);
 cudaError_t launch_attention(const AttentionParams& p, int sms, cudaStream_t stream);
 
+// ---- linears in 8-bit integers: token quantiser (w4a8_int8_quant.cu), product (w4a8_int8_gemm.cu) ----
+enum TokenSource { kTokPlain = 0, kTokSwiglu = 1, kTokNorm = 2 };
+
+struct TokenQuantParams {
+    const uint16_t* x;        // bf16 [M, ldx]; kTokSwiglu: [gate | up], 2 K used
+    int64_t ldx;
+    int M, K;
+    int vec_x, vec_r, vec_ro, vec_w, vec_q;   // 16-byte (codes: 8-byte) accesses are legal
+    int8_t* q;                // [M, ldq]
+    int64_t ldq;
+    float* scale;             // [M]
+    // kTokNorm
+    const uint16_t* res;      // bf16 [M, ldr], or null
+    uint16_t* res_out;        // bf16 [M, ldro], or null
+    int64_t ldr, ldro;
+    const void* weight;       // [K] bf16 or fp32
+    int weight_f32;
+    float eps;
+};
+
+cudaError_t launch_token_quant(const TokenQuantParams& p, int source, cudaStream_t stream);
+
+struct alignas(64) Int8GemmParams {
+    CUtensorMap tm_w;         // int8 weights [N, K], boxes of 128 bytes x the kernel's rows, SW128
+    CUtensorMap tm_a;         // int8 codes [M, K], likewise
+    const float* a_scale;     // [M]
+    const float* w_scale;     // [N]
+    const float* bias;        // [N] or null
+    uint16_t* y;              // bf16 [M, ldy]
+    int64_t ldy;
+    int* status;              // device status word
+    int M, N, K;
+};
+
+// How a call runs: tiles of one CTA with 128 channels x tt tokens, K cut over a cluster of
+// `split` CTAs (few), or of a pair of CTAs with nt channels x 256 tokens (many).
+struct Int8Plan {
+    bool many;
+    int tt, split, nt;
+    int w_rows, a_rows;       // rows of the tensor maps' boxes
+};
+Int8Plan int8_plan(int64_t M, int64_t N, int64_t K, int sms);
+cudaError_t launch_int8_gemm(const Int8GemmParams& p, const Int8Plan& plan, int sms, cudaStream_t stream, bool pdl);
+
 // Host helpers of the C entry points (w4a8_capi.cu).
 int capi_device_sms(int* sms);
 int capi_fail_cuda(cudaError_t e);
+// Tensor map of bytes [rows, cols] with row_bytes from row to row, boxes of box_rows x 128 bytes,
+// 128-byte swizzled; zeros outside.
+int capi_bytes_map(CUtensorMap* m, const void* base, int64_t cols, int64_t rows, int64_t row_bytes, int box_rows);
 
 // The one-shot all-reduce's side of the fused row-parallel linear
 // (w4a8_allreduce.cu): where a GEMM must push a message of `bytes`, and the

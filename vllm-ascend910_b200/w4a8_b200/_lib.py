@@ -27,6 +27,7 @@ OPT_AR_PUSH = 2                  # W4A8_OPT_AR_PUSH
 ACT_NONE = 0                     # W4A8_ACT_NONE
 ACT_SWIGLU = 1                   # W4A8_ACT_SWIGLU
 NORM_MAX_K = 32768               # W4A8_NORM_MAX_K
+INT8_MAX_K = 131071              # W4A8_INT8_MAX_K
 ATTENTION_MAX_BATCH = 2048       # W4A8_ATTENTION_MAX_BATCH
 
 _L = None
@@ -86,6 +87,14 @@ SIGNATURES = [
      [_p, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _i32, _f32, _i32, _p, _p, _i32, _p]),
     ("w4a8_linear_prepared_rms_norm", ctypes.c_int,
      [_p, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _i32, _f32, _i64, _i32, _p, _i32, _i32, _p, _i64, _p, _sz, _p]),
+    ("w4a8_int8_workspace_size", _sz, [_i64, _i64]),
+    ("w4a8_int8_quant", ctypes.c_int, [_p, _i64, _i64, _i64, _i32, _p, _i64, _p, _p]),
+    ("w4a8_int8_gemm", ctypes.c_int,
+     [_p, _i64, _p, _i64, _i64, _p, _i64, _p, _p, _i64, _p, _i64, _p, _sz, _p]),
+    ("w4a8_int8_linear", ctypes.c_int,
+     [_p, _i64, _i64, _i64, _i32, _p, _i64, _p, _p, _i64, _p, _i64, _p, _sz, _p]),
+    ("w4a8_int8_linear_rms_norm", ctypes.c_int,
+     [_p, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _i32, _f32, _p, _i64, _p, _p, _i64, _p, _i64, _p, _sz, _p]),
     ("w4a8_kv_write", ctypes.c_int,
      [_p, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _i32, _p, _i64, _p, _i64, _i32, _i32,
       _p]),

@@ -550,6 +550,136 @@ def linear_prepared_rms_norm(x: torch.Tensor, weight: torch.Tensor, pw: Prepared
     return y if r2 is None else (y, ro)
 
 
+# ---------------------------------------------------------------- linears in 8-bit integers
+
+class Int8Weight:
+    """An 8-bit linear's layer: codes int8 [N, K] (rows of a multiple of 16 bytes), fp32 scales and bias [N]."""
+
+    __slots__ = ("w", "scale", "bias", "N", "K", "ldw", "device", "_args")
+
+    def __init__(self, w: torch.Tensor, scale: torch.Tensor, bias: Optional[torch.Tensor], K: int):
+        self.w, self.scale, self.bias = w, scale, bias
+        self.N, self.K, self.ldw, self.device = w.shape[0], K, w.stride(0), w.device
+        self._args = (w.data_ptr(), self.ldw, scale.data_ptr(), _ptr(bias), self.N)
+
+
+def prepare_int8(w: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None) -> Int8Weight:
+    """The layer of codes w int8 [N, K], scales [N] or [N, 1] and an optional bias [N] (bf16 or f32 each): kept in
+    fp32; w itself where its rows suit the kernels (K a multiple of 16), else a copy with longer rows."""
+    _check(w.dim() == 2 and w.dtype == torch.int8, "prepare_int8: w must be int8 [N, K]")
+    N, K = w.shape
+    _check(N > 0 and 0 < K <= _lib.INT8_MAX_K, f"prepare_int8: needs N > 0 and K in 1..{_lib.INT8_MAX_K}; got [{N}, {K}]")
+    _check_cuda(w, w_scale, bias)
+    for name, t in (("w_scale", w_scale), ("bias", bias)):
+        _check(t is None or (t.dtype in (torch.bfloat16, torch.float32) and (tuple(t.shape) == (N,) or tuple(t.shape) == (N, 1))),
+               f"prepare_int8: {name} must be bfloat16 or float32 [{N}]")
+    w = w.detach()
+    if not (w.is_contiguous() and K % 16 == 0 and w.data_ptr() % 16 == 0):
+        rows = torch.zeros((N, -(-K // 16) * 16), dtype=torch.int8, device=w.device)
+        rows[:, :K] = w
+        w = rows
+    own = lambda t: t.detach().reshape(N).to(torch.float32, copy=True)                    # noqa: E731
+    return Int8Weight(w, own(w_scale), None if bias is None else own(bias), K)
+
+
+def _int8_ws(M: int, K: int, device: torch.device) -> Tuple[int, int]:
+    """The device's workspace, large enough for an 8-bit linear's codes (w4a8_int8_workspace_size)."""
+    return workspace(2048 + (4 * M + 1023) // 1024 * 1024 + M * ((K + 15) // 16 * 16), device)
+
+
+def quant_token(x: torch.Tensor, act: Optional[str] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """x bf16 [M, K] -> (codes int8 [M, K], scale f32 [M]): scale = max|x| / 127 of each token,
+    codes = rint(x / scale).  act="swiglu": of bf16(silu(gate) * up), x = [gate | up]."""
+    _check(x.dim() == 2 and x.dtype == torch.bfloat16, "quant_token: x must be bfloat16 [M, K]")
+    _check_cuda(x)
+    K = _act_k(x, act)
+    _check(0 < K <= _lib.INT8_MAX_K, f"quant_token: K must be 1..{_lib.INT8_MAX_K}; got {K}")
+    x, M, ldx = _rows(x, x.shape[1])
+    q = torch.empty((M, K), dtype=torch.int8, device=x.device)
+    s = torch.empty((M,), dtype=torch.float32, device=x.device)
+    rc = _launch(x.get_device(), _lib.lib().w4a8_int8_quant, x.data_ptr(), M, K, ldx,
+                 _lib.ACT_NONE if act is None else _lib.ACT_SWIGLU, q.data_ptr(), K, s.data_ptr(), _stream_of(x))
+    _lib.check(rc, "w4a8_int8_quant")
+    return q, s
+
+
+def gemm_int8(q: torch.Tensor, scale: torch.Tensor, layer: Int8Weight, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """bf16 [M, N] of codes q int8 [M, K] with a scale f32 [M] per token (``quant_token``) and an 8-bit layer."""
+    what = "gemm_int8"
+    _check(q.dim() == 2 and q.dtype == torch.int8 and q.shape[1] == layer.K, f"{what}: q must be int8 [M, {layer.K}]")
+    M, N, K = q.shape[0], layer.N, layer.K
+    _check(q.device == layer.device and scale.device == layer.device, f"{what}: tensors must be on the layer's device")
+    _check(scale.dtype == torch.float32 and tuple(scale.shape) == (M,) and scale.is_contiguous(),
+           f"{what}: scale must be a dense float32 [{M}]")
+    ld = q.stride(0) if M > 1 else -(-K // 16) * 16
+    if q.stride(1) != 1 and K > 1 or ld % 16 or ld < K or q.data_ptr() % 16:
+        rows = torch.empty((M, -(-K // 16) * 16), dtype=torch.int8, device=q.device)
+        rows[:, :K] = q
+        q, ld = rows, rows.shape[1]
+    y, ldy = _int8_out(out, M, N, layer, what)
+    if M == 0:
+        return y
+    ws, wsb = workspace(1024, q.device)
+    rc = _launch(q.get_device(), _lib.lib().w4a8_int8_gemm, q.data_ptr(), ld, scale.data_ptr(), M, K, *layer._args,
+                 y.data_ptr(), ldy, ws, wsb, _stream_of(q))
+    _lib.check(rc, "w4a8_int8_gemm")
+    return y
+
+
+def _int8_out(out: Optional[torch.Tensor], M: int, N: int, layer: Int8Weight, what: str):
+    if out is None:
+        return torch.empty((M, N), dtype=_BF16, device=layer.device), N
+    return _dense_rows(out, (M, N), N, layer.device, what, f"out [{M}, {N}]")
+
+
+def linear_int8(x: torch.Tensor, layer: Int8Weight, act: Optional[str] = None,
+                out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """y = x @ W^T (+ bias) in 8-bit integers: x bf16 [..., K] quantised per token (``quant_token``), exact integer
+    sums, bf16 [..., N].  act="swiglu": x = [gate | up], [..., 2 K]; ``out``: bf16 [M, N] with dense rows."""
+    if x.dtype is not _BF16 or x.device != layer.device:
+        raise RuntimeError("linear_int8: x must be bfloat16 on the layer's device (there is no CPU implementation)")
+    K, N = layer.K, layer.N
+    wide = K if act is None else 2 * K
+    if x.dim() == 0 or x.shape[-1] != wide or act not in (None, "swiglu"):
+        _act_k(x, act)
+        raise RuntimeError(f"linear_int8: x has shape {list(x.shape)}, the layer takes [..., {wide}]")
+    x2, M, ldx = _rows(x, wide)
+    y, ldy = _int8_out(out, M, N, layer, "linear_int8")
+    if M > 0:
+        ws, wsb = _int8_ws(M, K, x.device)
+        rc = _launch(x2.get_device(), _lib.lib().w4a8_int8_linear, x2.data_ptr(), M, K, ldx,
+                     _lib.ACT_NONE if act is None else _lib.ACT_SWIGLU, *layer._args, y.data_ptr(), ldy, ws, wsb,
+                     _stream_of(x2))
+        if rc != 0:
+            _lib.check(rc, "w4a8_int8_linear")
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
+
+
+def linear_int8_rms_norm(x: torch.Tensor, weight: torch.Tensor, layer: Int8Weight, eps: float = 1e-6,
+                         residual: Optional[torch.Tensor] = None, residual_out: Optional[torch.Tensor] = None,
+                         out: Optional[torch.Tensor] = None):
+    """``linear_int8`` on the norm of x (+ residual), whose fp32 result is quantised per token as it is made.
+    Returns y, or (y, bf16(x + residual))."""
+    what = "linear_int8_rms_norm"
+    x2, M, K, ldx, wd, r2, rp, ldr, ro, rop, ldro = _norm_args(x, weight, residual, residual_out, what)
+    if x.device != layer.device:
+        raise RuntimeError(f"{what}: x must be on the layer's device")
+    if K != layer.K:
+        raise RuntimeError(f"{what}: x has last dimension {K}, the layer takes {layer.K}")
+    N = layer.N
+    y, ldy = _int8_out(out, M, N, layer, what)
+    if M > 0:
+        ws, wsb = _int8_ws(M, K, x.device)
+        rc = _launch(x2.get_device(), _lib.lib().w4a8_int8_linear_rms_norm, x2.data_ptr(), M, K, ldx, rp, ldr, rop, ldro,
+                     weight.data_ptr(), wd, eps, *layer._args, y.data_ptr(), ldy, ws, wsb, _stream_of(x2))
+        if rc != 0:
+            _lib.check(rc, "w4a8_int8_linear_rms_norm")
+    if x.dim() != 2:
+        y = y.view(*x.shape[:-1], N)
+        ro = None if ro is None else ro.view(x.shape)
+    return y if r2 is None else (y, ro)
+
+
 # ---------------------------------------------------------------- weight packing (device-agnostic torch)
 
 def pack_int4(v: torch.Tensor) -> torch.Tensor:
