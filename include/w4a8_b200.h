@@ -350,11 +350,85 @@ W4A8_API int w4a8_kv_write(const w4a8_kv_cache* cache, const int32_t* page_table
                            int64_t tokens, const void* k, int64_t ldk, const void* v, int64_t ldv, const void* q,
                            int64_t ldq, int32_t q_heads, void* q_out, int64_t ldqo, const float* cos_sin,
                            int64_t table_rows, int32_t rot, int32_t interleaved, void* stream);
+/* The same with rotary positions that are not the tokens' places in their sequences, on up to
+ * four axes (time, height, width of images and videos): pair i of a head turns by row
+ * positions[a, t] of cos_sin, a = axis_of_pair[i].  positions int32 [axes, ld_positions] on the
+ * device, read by the kernel (rows outside the table: its first or last one); axis_of_pair
+ * [rot / 2] in HOST memory, read during the call, NULL for one axis.  cos_sin must be given. */
+W4A8_API int w4a8_kv_write_axes(const w4a8_kv_cache* cache, const int32_t* page_table, int64_t ld_table,
+                                int64_t table_cols, const int32_t* kv_lens, const int32_t* cu_q, int64_t batch,
+                                int64_t tokens, const void* k, int64_t ldk, const void* v, int64_t ldv, const void* q,
+                                int64_t ldq, int32_t q_heads, void* q_out, int64_t ldqo, const float* cos_sin,
+                                int64_t table_rows, int32_t rot, int32_t interleaved, const int32_t* positions,
+                                int64_t ld_positions, int32_t axes, const uint8_t* axis_of_pair, void* stream);
+/* The rotation alone, without a cache: q and k (which may be NULL) bf16 [tokens, ld] of heads * head_dim into
+ * q_out and k_out, each of which may be its input.  head_dim a multiple of 8, at most
+ * W4A8_ROTARY_MAX_DIM; elements past rot are copied.  Rows 16-byte aligned, leading dimensions multiples of 8. */
+#define W4A8_ROTARY_MAX_DIM 256
+W4A8_API int w4a8_rotary(const void* q, int64_t ldq, int32_t q_heads, void* q_out, int64_t ldqo, const void* k, int64_t ldk,
+                         int32_t k_heads, void* k_out, int64_t ldko, int64_t tokens, int32_t head_dim,
+                         const float* cos_sin, int64_t table_rows, int32_t rot, int32_t interleaved,
+                         const int32_t* positions, int64_t ld_positions, int32_t axes, const uint8_t* axis_of_pair,
+                         void* stream);
 /* Reads each sequence's last cu_out[s + 1] - cu_out[s] tokens back:
  * k, v bf16 [tokens, kv_heads, head_dim] dense. */
 W4A8_API int w4a8_kv_read(const w4a8_kv_cache* cache, const int32_t* page_table, int64_t ld_table,
                           int64_t table_cols, const int32_t* kv_lens, const int32_t* cu_out, int64_t batch,
                           int64_t tokens, void* k, void* v, void* stream);
+
+/* ---- pages kept on the device ----
+ * Which pages a sequence holds and how long it is, as tensors that the calls below read and change on the
+ * device, so that a captured step plans itself.  No counterpart in the reference.
+ *   free_pages  int32 [pages]: a stack of page ids, its top at free_count[0] - 1
+ *   table       int32 [sequences, columns]: the ceil(len / page_size) pages of each sequence in order
+ *   lens        int32 [sequences]: tokens of each
+ *   control     int32 [4], zeroed once: the status word, a counter that is 0 between calls, two of no use
+ * sequences <= W4A8_PLAN_MAX_SEQUENCES, pages * page_size and columns * page_size < 2^31.  Calls on one state run
+ * in stream order.
+ *
+ * A call that cannot be done as a whole changes nothing but the status word (its first non-zero
+ * value stays until the caller clears it): W4A8_PLAN_ROW a row outside the state or twice in the call, _COUNT a
+ * negative count, or more kept than held, _TOKENS more tokens than `tokens`, _PAGES too few free pages,
+ * _COLUMNS a sequence past its columns, _STATE a state that contradicts itself. */
+#define W4A8_PLAN_MAX_BATCH 2048
+#define W4A8_PLAN_MAX_SEQUENCES 65536
+#define W4A8_PLAN_ROW 1
+#define W4A8_PLAN_COUNT 2
+#define W4A8_PLAN_TOKENS 4
+#define W4A8_PLAN_PAGES 8
+#define W4A8_PLAN_COLUMNS 16
+#define W4A8_PLAN_STATE 32
+typedef struct w4a8_page_state {
+    int32_t* free_pages;
+    int32_t* free_count;
+    int32_t* table;
+    int32_t* lens;
+    int32_t* control;
+    int64_t pages, columns;
+    int32_t sequences, page_size;
+} w4a8_page_state;
+
+/* Lengthens sequence rows[i] by counts[i] >= 0 tokens for i = 0 .. batch - 1, taking pages off the stack in this
+ * order, and writes what the cache and attention calls take:
+ *   page_table  int32 [batch, columns], -1 past a sequence's pages;  kv_lens [batch];  cu [batch + 1]
+ *   slots       int32 [tokens] or NULL: page * page_size + place in the page, of each token of the step;
+ *               -1 past the last one
+ *   positions   int32 [axes, tokens] or NULL: rotary positions, 0 past the last token.  Without images the
+ *               token's place in its sequence, on every axis.  With n_segs > 0 (axes = 3):
+ *               segs int32 [n_segs, 4] holds (start, t, h, w) of grids whose first token is number `start` of its
+ *               sequence, grids seg_cu[i] .. seg_cu[i + 1] (int32 [batch + 1]) being rows[i]'s in order; token r of a
+ *               grid at text position o has positions o + r / (h w), o + r / w % h, o + r % w, and the
+ *               text behind it goes on at o + max(t, h, w).  A grid with a side below 1 holds no tokens.
+ * A refused step has page_table and slots -1, kv_lens, cu and positions 0. */
+W4A8_API int w4a8_pages_plan(const w4a8_page_state* state, const int32_t* rows, const int32_t* counts, int64_t batch,
+                             int64_t tokens, int32_t axes, const int32_t* seg_cu, const int32_t* segs, int64_t n_segs,
+                             int32_t* page_table, int32_t* kv_lens, int32_t* cu, int32_t* slots, int32_t* positions,
+                             void* stream);
+/* Shortens sequence rows[i] to keep[i] tokens (NULL: 0) and gives its pages past them back, from the last page of the
+ * last sequence to the first: the inverse of a plan over the same rows.  For sequences that ended and drafted
+ * tokens that were not accepted. */
+W4A8_API int w4a8_pages_shrink(const w4a8_page_state* state, const int32_t* rows, const int32_t* keep, int64_t batch,
+                               void* stream);
 
 /* ---- causal attention over the cache ----
  * out[t, h] = sum_j softmax_j(softmax_scale * q[t, h] . k_j) v_j over the cached

@@ -194,6 +194,16 @@ struct CacheView {
     int table_cols, batch, kv_heads, page, page_log2, D;
 };
 
+// Rotary positions of their own on up to kMaxAxes axes: row positions[a * ld + t] of the table for
+// the pairs of axis a; pair i's axis is bits 2 (i % 32) of map[i / 32].
+constexpr int kMaxAxes = 4;
+struct AxesView {
+    const int32_t* positions;
+    int64_t ld;
+    int axes;                 // 0: by the token's place in its sequence
+    uint64_t map[4];
+};
+
 struct KvWriteParams {
     CacheView c;
     const uint16_t* q;        // bf16 [tokens, ldq] of q_heads * D, or null
@@ -203,6 +213,18 @@ struct KvWriteParams {
     const float* cos_sin;     // [table_rows, rot]: cos of rot / 2 angles, then sin; null: no rotation
     int64_t ldq, ldk, ldv, ldqo, table_rows;
     int q_heads, rot, interleaved;
+    AxesView axes;
+};
+
+struct RotaryParams {
+    const uint16_t* x[2];     // q and k: bf16 [tokens, ld] of heads * D; k may be null
+    uint16_t* out[2];
+    int64_t ld[2], ldo[2];
+    int heads[2];
+    const float* cos_sin;     // as in KvWriteParams
+    int64_t tokens, table_rows;
+    int D, rot, interleaved;
+    AxesView axes;
 };
 
 struct KvReadParams {
@@ -230,9 +252,41 @@ struct AttentionParams {
 
 cudaError_t launch_kv_write(const KvWriteParams& p, cudaStream_t stream);
 cudaError_t launch_kv_read(const KvReadParams& p, cudaStream_t stream);
+cudaError_t launch_rotary(const RotaryParams& p, cudaStream_t stream);
 // Bytes of p.ws that a call of these sizes needs.
 size_t attention_ws_bytes(int batch, int64_t tokens, int q_heads, int kv_heads, int D, int max_q, int sms);
 cudaError_t launch_attention(const AttentionParams& p, int sms, cudaStream_t stream);
+
+// ---- pages kept on the device (w4a8_pages.cu) ----
+constexpr int kMaxPlanBatch = 2048;        // sequences of a step
+constexpr int kMaxPlanRows = 65536;        // sequences of a state
+
+// Why a step was refused: bits of the state's status word (W4A8_PLAN_* of the C ABI).
+enum : int { kPlanRow = 1, kPlanCount = 2, kPlanTokens = 4, kPlanPages = 8, kPlanColumns = 16, kPlanState = 32 };
+
+struct PagesParams {
+    int32_t* free;            // stack of free pages [pages]
+    int32_t* free_count;      // its height
+    int32_t* table;           // pages held [sequences][columns]
+    int32_t* lens;            // tokens held [sequences]
+    int* status;
+    uint32_t* ticket;         // blocks of the running call that are done; 0 between calls
+    int pages, sequences, columns, page_log2;
+    const int32_t* rows;      // [batch] the step's sequences
+    const int32_t* counts;    // [batch] tokens that each brings; shrink: tokens it keeps, or null
+    int batch, axes, n_segs;
+    int64_t tokens;           // room of slots and positions
+    const int32_t* seg_cu;    // [batch + 1] grids of each sequence, or null
+    const int32_t* segs;      // [n_segs] of start, t, h, w
+    int32_t* page_table;      // [batch][columns]
+    int32_t* kv_lens;         // [batch]
+    int32_t* cu;              // [batch + 1]
+    int32_t* slots;           // [tokens], or null
+    int32_t* positions;       // [axes][tokens], or null
+};
+
+cudaError_t launch_pages_plan(const PagesParams& p, cudaStream_t stream);
+cudaError_t launch_pages_shrink(const PagesParams& p, cudaStream_t stream);
 
 // ---- linears in 8-bit integers: token quantiser (w4a8_int8_quant.cu), product (w4a8_int8_gemm.cu) ----
 enum TokenSource { kTokPlain = 0, kTokSwiglu = 1, kTokNorm = 2 };

@@ -39,6 +39,7 @@
 
 #include "w4a8_common.cuh"
 #include "w4a8_kernels.h"
+#include "w4a8_rotary.cuh"
 
 namespace w4a8 {
 
@@ -50,13 +51,6 @@ constexpr int kWarps = kThreads / 32;
 // 4,096 tokens of 40 + 8 + 8 heads of 128; four: 4.2, 5.6 and 30.
 constexpr int kQTok = 4;
 __host__ __device__ constexpr int chunk_rows(int D) { return 512 / D; }   // rows that a warp holds: 16 elements a lane
-
-__device__ __forceinline__ void rotate_pair(float& a, float& b, float c, float s)
-{
-    const float x = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
-    b = __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s));
-    a = x;
-}
 
 // Bounds of sequence s: its first token in the call, their number, its length
 // after the call.  The length may pass what the page table has columns for
@@ -87,62 +81,6 @@ __device__ __forceinline__ int seq_of(const int32_t* cu, int batch, int64_t t0, 
     return lo;
 }
 
-// A work item of a head's row: two vectors of 8 elements.  Items [0, rot / 16)
-// are rotated -- half layout: elements [8j, 8j + 8) and the same past rot / 2;
-// interleaved: elements [16j, 16j + 16) -- the rest are 16 plain elements.
-__device__ __forceinline__ void item_cols(int j, int rot, int interleaved, int& c0, int& c1)
-{
-    if (j < rot / 16 && !interleaved) {
-        c0 = 8 * j;
-        c1 = rot / 2 + 8 * j;
-    } else {
-        c0 = 16 * j;
-        c1 = 16 * j + 8;
-    }
-}
-
-// Cosines and sines of item j's 8 pairs, from a table row.
-__device__ __forceinline__ void load_angles(const float* row, int j, int rot, float4 (&cs)[4])
-{
-    const float4* cp = reinterpret_cast<const float4*>(row + 8 * j);
-    const float4* sp = reinterpret_cast<const float4*>(row + rot / 2 + 8 * j);
-    cs[0] = cp[0];
-    cs[1] = cp[1];
-    cs[2] = sp[0];
-    cs[3] = sp[1];
-}
-
-__device__ __forceinline__ void rotate_item(int interleaved, const float4 (&cs)[4], float (&a)[8], float (&b)[8])
-{
-    const float c[8] = {cs[0].x, cs[0].y, cs[0].z, cs[0].w, cs[1].x, cs[1].y, cs[1].z, cs[1].w};
-    const float s[8] = {cs[2].x, cs[2].y, cs[2].z, cs[2].w, cs[3].x, cs[3].y, cs[3].z, cs[3].w};
-    if (!interleaved) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) rotate_pair(a[i], b[i], c[i], s[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) rotate_pair(a[2 * i], a[2 * i + 1], c[i], s[i]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) rotate_pair(b[2 * i], b[2 * i + 1], c[4 + i], s[4 + i]);
-    }
-}
-
-__device__ __forceinline__ uint4 pack8(const float (&v)[8])
-{
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t*>(&b);
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-__device__ __forceinline__ int64_t clamp_row(int64_t pos, int64_t rows)
-{
-    return pos < 0 ? 0 : (pos >= rows ? rows - 1 : pos);
-}
-
 // codes4 by the division alone, within +-127, for scales whose reciprocal fp32
 // cannot hold; 0 for a zero or non-finite scale.
 __device__ __forceinline__ uint32_t codes4_slow(const float* x, float s)
@@ -169,14 +107,14 @@ __device__ __forceinline__ int touched_pages(const CacheView& cv, int s)
 }
 
 // Query heads of kQTok tokens.
-template <int D>
+template <int D, bool AXES>
 __device__ __forceinline__ void rotate_queries(const KvWriteParams& p, int64_t t0)
 {
     constexpr int LPH = D / 16;                          // threads of a head
     const CacheView& cv = p.c;
     const int j = threadIdx.x % LPH, slot = threadIdx.x / LPH;
     const int64_t t = t0 + slot % kQTok;
-    const int s = p.rot ? seq_of(cv.cu, cv.batch, t0, min(t, cv.tokens - 1)) : 0;
+    const int s = p.rot && !AXES ? seq_of(cv.cu, cv.batch, t0, min(t, cv.tokens - 1)) : 0;
     if (t >= cv.tokens) return;
     int c0, c1;
     item_cols(j, p.rot, p.interleaved, c0, c1);
@@ -194,7 +132,9 @@ __device__ __forceinline__ void rotate_queries(const KvWriteParams& p, int64_t t
             w[k][0] = *reinterpret_cast<const uint4*>(src + h * D + c0);
             w[k][1] = *reinterpret_cast<const uint4*>(src + h * D + c1);
         }
-        if (turn && h0 == slot / kQTok) {
+        if (AXES && turn && h0 == slot / kQTok) {
+            load_angles_axes(p.cos_sin, p.axes, axis_rows(p.axes, t, p.table_rows), j, p.rot, cs);
+        } else if (turn && h0 == slot / kQTok) {
             int64_t first;
             int n, len;
             seq_bounds(cv, s, first, n, len);
@@ -221,7 +161,7 @@ struct Job {
     int s, n, len, pg;
 };
 
-template <int D, bool ONE>
+template <int D, bool ONE, bool AXES>
 __global__ void __launch_bounds__(kThreads, 4) kv_write_kernel(const KvWriteParams p, const int q_blocks, const int groups)
 {
     __shared__ uint32_t sh_max[kWarps];
@@ -235,7 +175,7 @@ __global__ void __launch_bounds__(kThreads, 4) kv_write_kernel(const KvWritePara
     // proportion, so that both kinds are resident together.
     const int64_t qi = static_cast<int64_t>(blockIdx.x) * q_blocks / gridDim.x;
     if ((static_cast<int64_t>(blockIdx.x) + 1) * q_blocks / gridDim.x > qi) {
-        rotate_queries<D>(p, qi * kQTok);
+        rotate_queries<D, AXES>(p, qi * kQTok);
         return;
     }
 
@@ -312,7 +252,10 @@ __global__ void __launch_bounds__(kThreads, 4) kv_write_kernel(const KvWritePara
         const uint4 w0 = *reinterpret_cast<const uint4*>(src + from * ld + c0);
         const uint4 w1 = *reinterpret_cast<const uint4*>(src + from * ld + c1);
         float4 cs[4];
-        if (rot) load_angles(p.cos_sin + clamp_row(page_at + row, p.table_rows) * rot, min(j, rot / 16 - 1), rot, cs);
+        if (AXES && rot)
+            load_angles_axes(p.cos_sin, p.axes, axis_rows(p.axes, t0 - start + page_at + from, p.table_rows), min(j, rot / 16 - 1),
+                             rot, cs);
+        else if (rot) load_angles(p.cos_sin + clamp_row(page_at + row, p.table_rows) * rot, min(j, rot / 16 - 1), rot, cs);
         float a[8], b[8];
         unpack8_bf16(w0, a);
         unpack8_bf16(w1, b);
@@ -468,11 +411,16 @@ cudaError_t launch_kv_write(const KvWriteParams& p, cudaStream_t stream)
     // Pages that eight warps hold (up to 32 rows of 128 or 64 of 64) need no loop over
     // chunks: without it 7,543 tokens in pages of 32 take 53 us, with it 57.
     const bool one = p.c.page / chunk_rows(p.c.D) <= kWarps;
+    if (p.axes.axes)
+        return p.c.D == 128 ? one ? launch(kv_write_kernel<128, true, true>, blocks, stream, p, qb, groups)
+                                  : launch(kv_write_kernel<128, false, true>, blocks, stream, p, qb, groups)
+               : one        ? launch(kv_write_kernel<64, true, true>, blocks, stream, p, qb, groups)
+                            : launch(kv_write_kernel<64, false, true>, blocks, stream, p, qb, groups);
     if (p.c.D == 128)
-        return one ? launch(kv_write_kernel<128, true>, blocks, stream, p, qb, groups)
-                   : launch(kv_write_kernel<128, false>, blocks, stream, p, qb, groups);
-    return one ? launch(kv_write_kernel<64, true>, blocks, stream, p, qb, groups)
-               : launch(kv_write_kernel<64, false>, blocks, stream, p, qb, groups);
+        return one ? launch(kv_write_kernel<128, true, false>, blocks, stream, p, qb, groups)
+                   : launch(kv_write_kernel<128, false, false>, blocks, stream, p, qb, groups);
+    return one ? launch(kv_write_kernel<64, true, false>, blocks, stream, p, qb, groups)
+               : launch(kv_write_kernel<64, false, false>, blocks, stream, p, qb, groups);
 }
 
 cudaError_t launch_kv_read(const KvReadParams& p, cudaStream_t stream)

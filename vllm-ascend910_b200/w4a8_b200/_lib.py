@@ -28,6 +28,13 @@ ACT_NONE = 0                     # W4A8_ACT_NONE
 ACT_SWIGLU = 1                   # W4A8_ACT_SWIGLU
 NORM_MAX_K = 32768               # W4A8_NORM_MAX_K
 INT8_MAX_K = 131071              # W4A8_INT8_MAX_K
+ROTARY_MAX_DIM = 256             # W4A8_ROTARY_MAX_DIM
+MAX_AXES = 4
+PLAN_MAX_BATCH = 2048            # W4A8_PLAN_MAX_BATCH
+PLAN_MAX_SEQUENCES = 65536       # W4A8_PLAN_MAX_SEQUENCES
+PLAN_REASONS = {1: "a row outside the state or twice in the call", 2: "a negative count, or more kept than held",
+                4: "more tokens than the step has room for", 8: "too few free pages", 16: "a sequence past its columns",
+                32: "a state that contradicts itself"}      # W4A8_PLAN_*
 ATTENTION_MAX_BATCH = 2048       # W4A8_ATTENTION_MAX_BATCH
 
 _L = None
@@ -98,7 +105,15 @@ SIGNATURES = [
     ("w4a8_kv_write", ctypes.c_int,
      [_p, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _i32, _p, _i64, _p, _i64, _i32, _i32,
       _p]),
+    ("w4a8_kv_write_axes", ctypes.c_int,
+     [_p, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _i32, _p, _i64, _p, _i64, _i32, _i32,
+      _p, _i64, _i32, _p, _p]),
+    ("w4a8_rotary", ctypes.c_int,
+     [_p, _i64, _i32, _p, _i64, _p, _i64, _i32, _p, _i64, _i64, _i32, _p, _i64, _i32, _i32, _p, _i64, _i32, _p, _p]),
     ("w4a8_kv_read", ctypes.c_int, [_p, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _p]),
+    ("w4a8_pages_plan", ctypes.c_int,
+     [_p, _p, _p, _i64, _i64, _i32, _p, _p, _i64, _p, _p, _p, _p, _p, _p]),
+    ("w4a8_pages_shrink", ctypes.c_int, [_p, _p, _p, _i64, _p]),
     ("w4a8_attention_workspace_size", _sz, [_i64, _i64, _i32, _i32, _i32, _i32]),
     ("w4a8_attention", ctypes.c_int,
      [_p, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _i32, _i32, _f32, _p, _i64, _p, _sz, _p]),
@@ -114,6 +129,12 @@ class KvCacheDesc(ctypes.Structure):
     """w4a8_kv_cache."""
     _fields_ = [("k", _p), ("v", _p), ("k_scale", _p), ("v_scale", _p), ("pages", _i64), ("kv_heads", _i32),
                 ("page_size", _i32), ("head_dim", _i32), ("reserved", _i32)]
+
+
+class PageStateDesc(ctypes.Structure):
+    """w4a8_page_state."""
+    _fields_ = [("free_pages", _p), ("free_count", _p), ("table", _p), ("lens", _p), ("control", _p), ("pages", _i64),
+                ("columns", _i64), ("sequences", _i32), ("page_size", _i32)]
 
 
 def lib_path() -> str:
