@@ -13,9 +13,14 @@ and ``rms_norm(h, final, residual=r)`` at the end.  ``Pages`` is the host's side
 cache: which pages a sequence holds and how long it is.  A step's ``Plan`` carries the
 page table, lengths and offsets on the device; every kernel reads them there, so a step
 captured in a CUDA graph (``Decoder.capture``) serves later steps of the same shape by
-copying the new plan into the old one's tensors.
+copying the new plan into the old one's tensors.  ``DevicePages`` keeps the same on the GPU: a step
+captured with its plan inside (``Decoder.capture_steps``) is replayed without any of that.
 
-    python -m w4a8_b200.decoder --layers 4 --batch 16 --prompt 512 --steps 16
+A layer's linears may be 8-bit ones (``ops.Int8Weight``) each on its own, as checkpoints mix them:
+``linear_int8_rms_norm`` and ``linear_int8`` take the places above.  With ``Config.rope_sections`` the rotary
+positions have several axes (time, height, width) and come with the plan.
+
+    python -m w4a8_b200.decoder --layers 4 --batch 16 --prompt 512 --steps 16 [--gpu-pages] [--int8 o,down]
 
 runs random weights of QwQ-32B's shapes: prompts, then captured single-token steps.
 The reference leaves norms, rotary positions, cache and attention to its serving stack.
@@ -24,12 +29,14 @@ from __future__ import annotations
 
 import argparse
 import dataclasses
-from typing import Dict, List, Optional, Sequence, Tuple
+from typing import Dict, List, Optional, Sequence, Tuple, Union
 
 import torch
 
 from . import kvcache, ops
-from .ops import PreparedWeight, _check
+from .ops import Int8Weight, PreparedWeight, _check
+
+Weight = Union[PreparedWeight, Int8Weight]
 
 
 @dataclasses.dataclass(frozen=True)
@@ -46,6 +53,8 @@ class Config:
     rope_scaling: Optional[Dict] = None
     page_size: int = 16
     positions: int = 8192
+    rope_sections: Optional[Tuple[int, ...]] = None      # pairs of each axis (kvcache.RotaryAxes)
+    rope_mixed: bool = False
 
     @property
     def qkv(self) -> int:
@@ -60,11 +69,11 @@ class Config:
 @dataclasses.dataclass
 class Layer:
     norm1: torch.Tensor
-    qkv: PreparedWeight
-    o: PreparedWeight
+    qkv: Weight
+    o: Weight
     norm2: torch.Tensor
-    gate_up: PreparedWeight
-    down: PreparedWeight
+    gate_up: Weight
+    down: Weight
 
 
 @dataclasses.dataclass
@@ -75,11 +84,15 @@ class Plan:
     cu: torch.Tensor           # int32 [batch + 1]
     tokens: int
     max_q_len: int
+    positions: Optional[torch.Tensor] = None   # int32 [axes, tokens]: rotary positions of their own
 
     def copy_(self, other: "Plan") -> None:
         """Takes over another step of the same shape, for a captured step's replay."""
         if (other.tokens, other.max_q_len, other.kv_lens.shape) != (self.tokens, self.max_q_len, self.kv_lens.shape):
             raise RuntimeError("Plan: the captured step has another shape")
+        if (self.positions is None) != (other.positions is None) or \
+                self.positions is not None and self.positions.shape != other.positions.shape:
+            raise RuntimeError("Plan: the captured step has other rotary positions")
         cols = other.page_table.shape[1]
         if cols > self.page_table.shape[1]:
             raise RuntimeError(f"Plan: {cols} pages a sequence, the captured step has room for "
@@ -87,6 +100,8 @@ class Plan:
         self.page_table[:, :cols] = other.page_table
         self.kv_lens.copy_(other.kv_lens)
         self.cu.copy_(other.cu)
+        if self.positions is not None:
+            self.positions.copy_(other.positions)
 
 
 class Pages:
@@ -144,6 +159,49 @@ class Pages:
         return Plan(put(table), put([self._len[s] for s in seqs]), put(cu), cu[-1], max(counts))
 
 
+class DevicePages:
+    """``Pages`` on the GPU (``kvcache.PageState``): sequences are rows 0 .. sequences - 1, and their lengths and
+    pages never come to the host, so neither do a step's refusals; ``check`` raises for those.
+
+    ``positions``: rows of the rotary table; no sequence outgrows the whole pages that fit them."""
+
+    def __init__(self, pages: int, page_size: int, sequences: int, positions: int, device="cuda", axes: int = 1):
+        _check(positions >= page_size, "DevicePages: the rotary table is shorter than a page")
+        self.state = kvcache.PageState.empty(pages, sequences, min(positions // page_size, pages), page_size, device)
+        self.axes = axes
+
+    def _put(self, v) -> torch.Tensor:
+        return v if isinstance(v, torch.Tensor) else torch.tensor(v, dtype=torch.int32).to(self.state.device)
+
+    def plan(self, rows, counts, tokens: int, max_q_len: int, images=None) -> Plan:
+        """Lengthens sequence rows[i] by counts[i] tokens (lists, or int32 tensors on the GPU) and lays out the step, on the
+        device.  ``tokens``: rows of the step's input, at least the counts' sum; ``max_q_len``: the largest count;
+        ``images``: ``kvcache.pages_plan``'s.  A step that cannot be has no tokens and no pages."""
+        m = kvcache.pages_plan(self.state, self._put(rows), self._put(counts), tokens, self.axes, images)
+        return Plan(m.page_table, m.kv_lens, m.cu, tokens, max_q_len, m.positions if self.axes > 1 else None)
+
+    def shrink(self, rows, keep) -> None:
+        """Sequence rows[i] keeps its first keep[i] tokens: drafted ones past them were not accepted."""
+        kvcache.pages_shrink(self.state, self._put(rows), self._put(keep))
+
+    def release(self, rows) -> None:
+        """Ends sequences; their rows are empty and their pages free for the steps after."""
+        kvcache.pages_shrink(self.state, self._put(rows))
+
+    def check(self) -> None:
+        """Raises if a plan, shrink or release was refused since the last time (waits for the current stream)."""
+        self.state.check()
+
+
+def _norm_linear(x, norm, w: Weight, eps, residual=None):
+    f = ops.linear_int8_rms_norm if isinstance(w, Int8Weight) else ops.linear_prepared_rms_norm
+    return f(x, norm, w, eps, residual=residual)
+
+
+def _linear(x, w: Weight, act=None):
+    return (ops.linear_int8 if isinstance(w, Int8Weight) else ops.linear_prepared)(x, w, act=act)
+
+
 class Decoder:
     """Layers, their caches and a rotary table on one GPU."""
 
@@ -156,25 +214,38 @@ class Decoder:
         self.caches = [kvcache.KVCache.empty(pages, cfg.kv_heads, cfg.page_size, cfg.head_dim, device) for _ in layers]
         self.cos_sin = kvcache.rotary_table(cfg.head_dim, cfg.positions, cfg.rope_base, cfg.rope_scaling, device)
         self.pages = Pages(pages, cfg.page_size, cfg.positions)
+        self.axes = None if cfg.rope_sections is None else kvcache.RotaryAxes(cfg.rope_sections, cfg.rope_mixed)
+        _check(self.axes is None or 2 * self.axes.pairs == cfg.head_dim, "Decoder: rope_sections must add up to head_dim / 2")
+
+    def device_pages(self, sequences: int) -> DevicePages:
+        """Pages of the caches kept on the GPU, for up to ``sequences`` sequences at a time.  They are the same pages as
+        ``self.pages``'s: a decoder uses one of the two."""
+        c = self.caches[0] if self.caches else None
+        _check(c is not None, "Decoder: device_pages needs a layer")
+        return DevicePages(c.pages, self.cfg.page_size, sequences, self.cfg.positions, c.device,
+                           1 if self.axes is None else self.axes.axes)
 
     def step(self, h: torch.Tensor, plan: Plan) -> torch.Tensor:
         """Embedded tokens bf16 [tokens, hidden], in the plan's order -> the stack's normed output."""
         c = self.cfg
         _check(h.dim() == 2 and tuple(h.shape) == (plan.tokens, c.hidden), f"step: h must be [{plan.tokens}, {c.hidden}]")
         T, D, nq, nk = plan.tokens, c.head_dim, c.q_heads * c.head_dim, c.kv_heads * c.head_dim
+        _check((plan.positions is None) == (self.axes is None), "step: a plan has rotary positions of its own where, and only "
+               "where, the configuration has rope_sections")
         batch = (plan.page_table, plan.kv_lens, plan.cu)
+        rope = dict(cos_sin=self.cos_sin, positions=plan.positions, axes=self.axes)
         r = None
         for L, cache in zip(self.layers, self.caches):
             if r is None:
-                qkv, r = ops.linear_prepared_rms_norm(h, L.norm1, L.qkv, c.eps), h
+                qkv, r = _norm_linear(h, L.norm1, L.qkv, c.eps), h
             else:
-                qkv, r = ops.linear_prepared_rms_norm(h, L.norm1, L.qkv, c.eps, residual=r)
+                qkv, r = _norm_linear(h, L.norm1, L.qkv, c.eps, residual=r)
             q, k, v = (t.unflatten(1, (-1, D)) for t in qkv.split((nq, nk, nk), 1))
-            q = kvcache.kv_write(cache, k, v, *batch, q=q, cos_sin=self.cos_sin)
+            q = kvcache.kv_write(cache, k, v, *batch, q=q, **rope)
             a = kvcache.attention(q, cache, *batch, plan.max_q_len)
-            h = ops.linear_prepared(a.view(T, nq), L.o)
-            gu, r = ops.linear_prepared_rms_norm(h, L.norm2, L.gate_up, c.eps, residual=r)
-            h = ops.linear_prepared(gu, L.down, act="swiglu")
+            h = _linear(a.view(T, nq), L.o)
+            gu, r = _norm_linear(h, L.norm2, L.gate_up, c.eps, residual=r)
+            h = _linear(gu, L.down, act="swiglu")
         if r is None:
             return ops.rms_norm(h, self.final_norm, c.eps)
         return ops.rms_norm(h, self.final_norm, c.eps, residual=r)[0]
@@ -182,6 +253,12 @@ class Decoder:
     def capture(self, plan: Plan) -> "Captured":
         """A captured step of the plan's shape.  The plan's own step is not run: nothing is written."""
         return Captured(self, plan)
+
+    def capture_steps(self, pages: DevicePages, rows, counts=None, tokens: Optional[int] = None, max_q_len: int = 1,
+                      images=None) -> "CapturedSteps":
+        """Steps over the sequences ``rows`` of ``pages`` that plan themselves on the GPU: each call brings ``counts`` tokens
+        of each (one, unless given; the result's ``counts`` tensor may be changed between calls)."""
+        return CapturedSteps(self, pages, rows, counts, tokens, max_q_len, images)
 
 
 class Captured:
@@ -192,7 +269,8 @@ class Captured:
         # layers as they were captured too.
         self._keep = (dec, [dataclasses.replace(L) for L in dec.layers], list(dec.caches), dec.final_norm, dec.cos_sin)
         self.plan = dataclasses.replace(plan, page_table=plan.page_table.clone(), kv_lens=plan.kv_lens.clone(),
-                                        cu=plan.cu.clone())
+                                        cu=plan.cu.clone(),
+                                        positions=None if plan.positions is None else plan.positions.clone())
         self.h = torch.zeros((plan.tokens, dec.cfg.hidden), dtype=torch.bfloat16, device=plan.kv_lens.device)
         # The workspace has to exist before the capture: one step without any page, which writes
         # nothing and attends to nothing.
@@ -218,13 +296,57 @@ class Captured:
         return self.out
 
 
-def random_layers(cfg: Config, n: int, seed: int = 0, device="cuda") -> Tuple[List[Layer], torch.Tensor]:
-    """Layers of random 4-bit weights, scaled so that each linear keeps its input's size, and a final norm."""
+class CapturedSteps:
+    """``DevicePages.plan`` and ``Decoder.step`` as one CUDA graph: a call takes the tokens' rows and nothing else."""
+
+    def __init__(self, dec: Decoder, pages: DevicePages, rows, counts, tokens: Optional[int], max_q_len: int, images):
+        # as in Captured: the graph holds addresses only
+        self._keep = (dec, [dataclasses.replace(L) for L in dec.layers], list(dec.caches), dec.final_norm, dec.cos_sin, pages)
+        self.rows = pages._put(rows).clone()
+        self.counts = torch.ones_like(self.rows) if counts is None else pages._put(counts).clone()
+        self.images = None if images is None else tuple(t.clone() for t in images)
+        _check(counts is None or tokens is not None, "capture_steps: counts need the number of tokens that there is room for")
+        T = self.rows.shape[0] if tokens is None else tokens
+        _check(T > 0, "capture_steps: a step needs tokens")
+        dev, B = self.rows.device, self.rows.shape[0]
+        self.h = torch.zeros((T, dec.cfg.hidden), dtype=torch.bfloat16, device=dev)
+        # The workspace has to exist before the capture: one step without any page, and no plan.
+        i = dict(dtype=torch.int32, device=dev)
+        empty = Plan(torch.full((B, pages.state.columns), -1, **i), torch.zeros(B, **i), torch.zeros(B + 1, **i), T, max_q_len,
+                     torch.zeros(pages.axes, T, **i) if pages.axes > 1 else None)
+        side = torch.cuda.Stream(dev)
+        side.wait_stream(torch.cuda.current_stream(dev))
+        with torch.cuda.stream(side):
+            dec.step(self.h, empty)
+        torch.cuda.current_stream(dev).wait_stream(side)
+        self.graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(self.graph):
+            self.plan = pages.plan(self.rows, self.counts, T, max_q_len, self.images)
+            self.out = dec.step(self.h, self.plan)
+
+    def __call__(self, h: torch.Tensor) -> torch.Tensor:
+        """The next step's output; the call after overwrites it, and ``self.plan``, the step's plan."""
+        if h.shape != self.h.shape or h.dtype is not self.h.dtype:
+            raise RuntimeError(f"the captured step takes bfloat16 [{self.h.shape[0]}, {self.h.shape[1]}]; "
+                               f"got {h.dtype} {list(h.shape)}")
+        self.h.copy_(h)
+        self.graph.replay()
+        return self.out
+
+
+def random_layers(cfg: Config, n: int, seed: int = 0, device="cuda", int8: Sequence[str] = ()) -> Tuple[List[Layer], torch.Tensor]:
+    """Layers of random 4-bit weights (8-bit ones for the linears named in ``int8``), scaled so that each linear keeps its
+    input's size, and a final norm."""
     g = torch.Generator(device=device).manual_seed(seed)
     layers = []
     for _ in range(n):
         ws = {}
         for name, (N, K) in cfg.projections().items():
+            if name in int8:
+                codes = torch.randint(-127, 128, (N, K), generator=g, device=device, dtype=torch.int8)
+                scale = torch.exp(torch.randn(N, generator=g, device=device) * 0.2) / (73.6 * K ** 0.5)
+                ws[name] = ops.prepare_int8(codes, scale)
+                continue
             codes = torch.randint(-8, 8, (N, K), generator=g, device=device, dtype=torch.int8)
             scale = torch.exp(torch.randn(ops.num_groups(K, cfg.group_size), N, generator=g, device=device) * 0.2) / (
                 4.6 * K ** 0.5)
@@ -250,28 +372,43 @@ def main(argv: Optional[Sequence[str]] = None) -> int:
     ap.add_argument("--batch", type=int, default=16)
     ap.add_argument("--prompt", type=int, default=512)
     ap.add_argument("--steps", type=int, default=16)
+    ap.add_argument("--gpu-pages", action="store_true", help="decode steps that plan themselves on the GPU")
+    ap.add_argument("--int8", default="", metavar="NAMES", help="8-bit linears among qkv, o, gate_up, down, by commas")
     a = ap.parse_args(argv)
     cfg = Config()
+    int8 = [n for n in a.int8.split(",") if n]
+    _check(all(n in cfg.projections() for n in int8), f"decoder: --int8 takes names of {', '.join(cfg.projections())}")
     dev = torch.device("cuda", torch.cuda.current_device())
     total = a.prompt + a.steps + 8
     _check(min(a.layers, a.batch, a.prompt, a.steps) > 0 and total <= cfg.positions, "decoder: sizes out of range")
-    layers, final = random_layers(cfg, a.layers, device=dev)
+    layers, final = random_layers(cfg, a.layers, device=dev, int8=int8)
     cols = -(-total // cfg.page_size)
     dec = Decoder(cfg, layers, final, a.batch * cols, dev)
     x = torch.randn(a.prompt, cfg.hidden, device=dev).bfloat16()
-    seqs = [dec.pages.add() for _ in range(a.batch)]
-    plans = [dec.pages.plan([s], [a.prompt], dev) for s in seqs]
+    if a.gpu_pages:
+        pages, seqs = dec.device_pages(a.batch), list(range(a.batch))
+        plans = [pages.plan([s], [a.prompt], a.prompt, a.prompt) for s in seqs]
+    else:
+        seqs = [dec.pages.add() for _ in range(a.batch)]
+        plans = [dec.pages.plan([s], [a.prompt], dev) for s in seqs]
     dec.step(x, plans[0])                                   # warm-up: workspace, kernels; written again below
     prompt_ms = _ms(lambda: [dec.step(x, p) for p in plans], 1) / a.batch
     h = torch.randn(a.batch, cfg.hidden, device=dev).bfloat16()
-    plan = dec.pages.plan(seqs, [1] * a.batch, dev, cols)
-    run = dec.capture(plan)
-    for _ in range(3):
-        run(h, plan)
+    if a.gpu_pages:
+        run = dec.capture_steps(pages, seqs)
+        for _ in range(3):
+            run(h)
+        step_ms = _ms(lambda: run(h), a.steps)
+        pages.check()
+    else:
         plan = dec.pages.plan(seqs, [1] * a.batch, dev, cols)
-    plans = [plan] + [dec.pages.plan(seqs, [1] * a.batch, dev, cols) for _ in range(a.steps - 1)]
-    it = iter(plans)
-    step_ms = _ms(lambda: run(h, next(it)), a.steps)
+        run = dec.capture(plan)
+        for _ in range(3):
+            run(h, plan)
+            plan = dec.pages.plan(seqs, [1] * a.batch, dev, cols)
+        plans = [plan] + [dec.pages.plan(seqs, [1] * a.batch, dev, cols) for _ in range(a.steps - 1)]
+        it = iter(plans)
+        step_ms = _ms(lambda: run(h, next(it)), a.steps)
     out = run.out.float()
     print(f"{a.layers} layers, {a.batch} sequences: prompt of {a.prompt} tokens {prompt_ms:.3f} ms "
           f"({a.prompt / prompt_ms * 1e3:.0f} tokens/s), decode step {step_ms * 1e3:.0f} us "

@@ -131,5 +131,46 @@ def dequantize(conv: Dict[str, Optional[torch.Tensor]]) -> torch.Tensor:
     return (codes - z) * sc
 
 
-__all__ = ["SUFFIXES", "unpack_output_axis", "pack_output_axis", "convert_projection", "load_projection",
+# ---------------------------------------------------------------- W8A8_DYNAMIC projections
+
+def load_int8(get: Callable[[str], torch.Tensor], names: Sequence[str]) -> Dict[str, Optional[torch.Tensor]]:
+    """The named 8-bit projections (the members of one fused linear) of a checkpoint that mixes them with the 4-bit
+    ones: ``<proj>.weight`` int8 [N, K], ``weight_scale`` [N, 1] and ``weight_offset`` [N, 1], which has to be zero,
+    ``<proj>.bias`` [N] where there is one; joined along N."""
+    ws, scales, biases = [], [], []
+    for name in names:
+        w, s = get(f"{name}.weight"), get(f"{name}.weight_scale").float().reshape(-1)
+        if w.dtype != torch.int8 or w.dim() != 2:
+            raise ValueError("weight must be int8 [N, K]")
+        if s.shape[0] != w.shape[0]:
+            raise ValueError("weight_scale must be per channel [N, 1]")
+        optional = {}
+        for suffix in ("weight_offset", "bias"):
+            try:
+                optional[suffix] = get(f"{name}.{suffix}").float().reshape(-1)
+            except KeyError:
+                optional[suffix] = None
+        offset, b = optional["weight_offset"], optional["bias"]
+        if offset is not None and bool(torch.any(offset != 0)):
+            raise ValueError("a per-channel weight_offset has no place in the symmetric 8-bit product")
+        if b is not None and b.shape[0] != w.shape[0]:
+            raise ValueError("bias must be [N]")
+        biases.append(b)
+        ws.append(w)
+        scales.append(s)
+    if any(w.shape[1] != ws[0].shape[1] for w in ws):
+        raise ValueError("fused members must share K")
+    bias = None
+    if any(b is not None for b in biases):
+        bias = torch.cat([torch.zeros(w.shape[0]) if b is None else b for w, b in zip(ws, biases)])
+    return {"w": torch.cat(ws), "w_scale": torch.cat(scales), "bias": bias}
+
+
+def prepare_int8(conv: Dict[str, Optional[torch.Tensor]], device) -> "ops.Int8Weight":
+    """The loaded projection as ``ops.linear_int8``'s layer on ``device``."""
+    return ops.prepare_int8(conv["w"].to(device), conv["w_scale"].to(device),
+                            None if conv["bias"] is None else conv["bias"].to(device))
+
+
+__all__ = ["load_int8", "prepare_int8", "SUFFIXES", "unpack_output_axis", "pack_output_axis", "convert_projection", "load_projection",
            "prepare", "dequantize"]
