@@ -119,10 +119,10 @@ __device__ __forceinline__ void cluster_sync()
 {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ int32_t load_cluster(uint32_t addr)
+__device__ __forceinline__ uint32_t load_cluster(uint32_t addr)
 {
-    int32_t v;
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
     return v;
 }
 
@@ -145,9 +145,14 @@ __device__ __forceinline__ void settle32(uint32_t (&r)[32])
     for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i]));
 }
 
-__device__ __forceinline__ float scaled(int32_t sum, float s, float ws, float b)
+__device__ __forceinline__ float scaled(uint32_t sum, float s, float ws, float b)
 {
-    return __fadd_rn(__fmul_rn(__fmul_rn(static_cast<float>(sum), s), ws), b);
+    return __fadd_rn(__fmul_rn(__fmul_rn(static_cast<float>(static_cast<int32_t>(sum)), s), ws), b);
+}
+__device__ __forceinline__ uint32_t two(float lo, float hi)
+{
+    const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&b);
 }
 
 // ---------------------------------------------------------------- few tokens
@@ -283,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, 2) int8_few_kernel(const __grid_cons
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
                         if (in && c + i < p.M)
-                            y[(c + i) * p.ldy] = f32_to_bf16_bits(scaled(static_cast<int32_t>(r[i]), sh_scale[c + i], ws, b));
+                            y[(c + i) * p.ldy] = f32_to_bf16_bits(scaled(r[i], sh_scale[c + i], ws, b));
                 }
             }
             tc_fence_before();
@@ -301,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, 2) int8_few_kernel(const __grid_cons
                 const float ws = p.w_scale[n], b = p.bias ? p.bias[n] : 0.0f;
                 for (int c = rank; c < p.M; c += SPLIT) {
                     const uint32_t at = smem_u32(ring) + (c * 128 + ch) * 4;
-                    int32_t sum = 0;
+                    uint32_t sum = 0;
 #pragma unroll
                     for (int o = 0; o < SPLIT; ++o) sum += load_cluster(map_rank(at, o));
                     p.y[c * p.ldy + n] = f32_to_bf16_bits(scaled(sum, sh_scale[c], ws, b));
@@ -342,7 +347,7 @@ __device__ __forceinline__ void tile_of(int64_t i, int mt, int nt, int& m, int& 
 
 template <int NT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    int8_many_kernel(const __grid_constant__ Int8GemmParams p, const int wide)
+    int8_many_kernel(const __grid_constant__ Int8GemmParams p, const int align)
 {
     using C = Many<NT>;
     constexpr int S = C::STAGES;
@@ -351,6 +356,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     __shared__ uint64_t full[S], empty[S], acc_full[2], acc_empty[2];
     __shared__ uint32_t tmem_at;
     __shared__ int abort_flag;
+    __shared__ uint16_t turn[4][32][34];                     // a warp's 32 x 32 outputs on their way to rows
 
     const int warp = warp_id(), lane = lane_id();
     const uint32_t rank = cluster_rank();
@@ -460,32 +466,44 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     __syncwarp();
                     if (lane == 0) arrive_remote(map_rank(smem_u32(&acc_empty[a]), 0));
                 }
-                if (wide && n + 32 <= p.N) {
-                    uint32_t o[16];
+                uint32_t o[16];
+                const bool whole = n + 32 <= p.N;
+                if (whole && align >= 16) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
                         const float4 ws = *reinterpret_cast<const float4*>(p.w_scale + n + i);
                         const float4 b = p.bias ? *reinterpret_cast<const float4*>(p.bias + n + i) : make_float4(0, 0, 0, 0);
-                        const __nv_bfloat162 lo = __floats2bfloat162_rn(scaled(static_cast<int32_t>(r[i]), s, ws.x, b.x),
-                                                                        scaled(static_cast<int32_t>(r[i + 1]), s, ws.y, b.y));
-                        const __nv_bfloat162 hi = __floats2bfloat162_rn(scaled(static_cast<int32_t>(r[i + 2]), s, ws.z, b.z),
-                                                                        scaled(static_cast<int32_t>(r[i + 3]), s, ws.w, b.w));
-                        o[i / 2] = *reinterpret_cast<const uint32_t*>(&lo);
-                        o[i / 2 + 1] = *reinterpret_cast<const uint32_t*>(&hi);
+                        o[i / 2] = two(scaled(r[i], s, ws.x, b.x), scaled(r[i + 1], s, ws.y, b.y));
+                        o[i / 2 + 1] = two(scaled(r[i + 2], s, ws.z, b.z), scaled(r[i + 3], s, ws.w, b.w));
                     }
-                    if (in)
+                    if (!in) continue;
+                    if (align >= 32) {
 #pragma unroll
                         for (int i = 0; i < 16; i += 8)      // 32 bytes: a whole sector a thread
                             asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(y + n + 2 * i), "r"(o[i]),
                                          "r"(o[i + 1]), "r"(o[i + 2]), "r"(o[i + 3]), "r"(o[i + 4]), "r"(o[i + 5]),
                                          "r"(o[i + 6]), "r"(o[i + 7])
                                          : "memory");
-                } else if (in) {
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (n + i < p.N)
-                            y[n + i] = f32_to_bf16_bits(scaled(static_cast<int32_t>(r[i]), s, p.w_scale[n + i],
-                                                               p.bias ? p.bias[n + i] : 0.0f));
+                        for (int i = 0; i < 16; i += 4)
+                            *reinterpret_cast<uint4*>(y + n + 2 * i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    }
+                } else if (n < p.N) {
+                    // rows that suit no vector, or their end: a lane a channel, row by row
+                    const int col = min(n + lane, p.N - 1);
+                    const float mws = p.w_scale[col], mb = p.bias ? p.bias[col] : 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        const float ws0 = __shfl_sync(0xffffffffu, mws, i), ws1 = __shfl_sync(0xffffffffu, mws, i + 1);
+                        const float b0 = __shfl_sync(0xffffffffu, mb, i), b1 = __shfl_sync(0xffffffffu, mb, i + 1);
+                        *reinterpret_cast<uint32_t*>(&turn[quad][lane][i]) = two(scaled(r[i], s, ws0, b0), scaled(r[i + 1], s, ws1, b1));
+                    }
+                    __syncwarp();
+                    const int64_t row0 = row - lane;
+                    for (int i = 0; i < 32 && row0 + i < p.M; ++i)
+                        if (n + lane < p.N) p.y[(row0 + i) * p.ldy + n + lane] = turn[quad][i][lane];
+                    __syncwarp();
                 }
             }
         }
@@ -566,12 +584,13 @@ cudaError_t launch_int8_gemm(const Int8GemmParams& p, const Int8Plan& plan, int 
     if (plan.many) {
         const int64_t mt = (p.M + 255) / 256, nt = (p.N + plan.nt - 1) / plan.nt;
         const int pairs = static_cast<int>(std::min<int64_t>(mt * nt, sms / 2));
-        // 32-byte stores of a row's outputs, 16-byte loads of the channels' scales
-        const int wide = reinterpret_cast<uintptr_t>(p.y) % 32 == 0 && p.ldy % 16 == 0 &&
-                         reinterpret_cast<uintptr_t>(p.w_scale) % 16 == 0 && reinterpret_cast<uintptr_t>(p.bias) % 16 == 0;
+        // the widest store that each row's outputs suit, where 16-byte loads suit the channels' scales
+        const auto fits = [&](uintptr_t a) { return reinterpret_cast<uintptr_t>(p.y) % a == 0 && 2 * p.ldy % a == 0; };
+        const bool loads = reinterpret_cast<uintptr_t>(p.w_scale) % 16 == 0 && reinterpret_cast<uintptr_t>(p.bias) % 16 == 0;
+        const int align = !loads ? 2 : fits(32) ? 32 : fits(16) ? 16 : 2;
         // (the kernel names its cluster itself)
-        return plan.nt == 256 ? launch(int8_many_kernel<256>, 2 * pairs, 1, Many<256>::SMEM, stream, pdl, p, wide)
-                              : launch(int8_many_kernel<128>, 2 * pairs, 1, Many<128>::SMEM, stream, pdl, p, wide);
+        return plan.nt == 256 ? launch(int8_many_kernel<256>, 2 * pairs, 1, Many<256>::SMEM, stream, pdl, p, align)
+                              : launch(int8_many_kernel<128>, 2 * pairs, 1, Many<128>::SMEM, stream, pdl, p, align);
     }
     switch (plan.tt) {
         case 16: return launch_few<16>(p, plan.split, sms, stream, pdl);

@@ -11,10 +11,10 @@
 // A row of zeros has s = 0 and codes 0; a row with a value that is not finite has
 // s = NaN and codes 0, so that its outputs are NaN.
 //
-// A block holds one row in registers, 8 elements of 16 bytes a vector and up to four
-// vectors a thread (32,768 elements): x is read once.  Longer rows are read twice, the
-// second time out of L2.  The sum of squares and the maximum each take a
-// warp reduction and a barrier; partial sums are added in a fixed order.
+// A block holds its part of a row in registers, 8 elements of 16 bytes a vector (as bf16, or fp32
+// behind a norm): x is read once.  A wide row of few is cut over a cluster of eight blocks, whose sums and maxima
+// meet in distributed shared memory.  Rows past 65,536 elements are read twice, the second time out of L2.
+// Sums and maxima take a warp reduction and a barrier; partial sums are added in a fixed order.
 #include <algorithm>
 
 #include "w4a8_common.cuh"
@@ -64,21 +64,82 @@ __device__ __forceinline__ void load_weight8(const TokenQuantParams& p, int pos,
     }
 }
 
-// 8 elements of h before any norm.
-template <int SRC>
-__device__ __forceinline__ void row8(const TokenQuantParams& p, const uint16_t* x, const uint16_t* r, int pos, float (&v)[8])
+// e^-g / (1 + ...) by the base-2 exponential of the hardware: -g log2(e) as a rounded product and what the rounding
+// left, 2^-21 of the result.  Gates below -87 give 0 (their product is less than 10^-35 of up).
+__device__ __forceinline__ float silu_up(float g, float u)
 {
-    load8(x, pos, p.K, p.vec_x, v);
-    if (SRC == kTokSwiglu) {
-        float u[8];
-        load8(x + p.K, pos, p.K, p.vec_x && p.K % 8 == 0, u);
+    constexpr float kL = 1.44269502162933349609375f, kLow = 1.925963033500011e-08f;     // log2(e) = kL + kLow
+    const float c = fminf(fmaxf(g, -87.0f), 87.0f), t = __fmul_rn(c, -kL);
+    const float low = fmaf(c, -kLow, fmaf(c, -kL, -t));
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+    e = fmaf(e, low * 0.693147180559945f, e);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return g * (g < -87.0f ? 0.0f : r) * u;
+}
+
+__device__ __forceinline__ uint4 pack8(const float (&v)[8])
+{
+    uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = swiglu_bf16(v[i], u[i]);
-    } else if (SRC == kTokNorm && r) {
-        float u[8];
-        load8(r, pos, p.K, p.vec_r, u);
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ uint4 load8_raw(const uint16_t* row, int pos, int K, bool vec)
+{
+    if (vec && pos + 8 <= K) return *reinterpret_cast<const uint4*>(row + pos);
+    uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = __fadd_rn(v[i], u[i]);
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = pos + 2 * i < K ? row[pos + 2 * i] : 0u, hi = pos + 2 * i + 1 < K ? row[pos + 2 * i + 1] : 0u;
+        w[i] = lo | (hi << 16);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// What a thread holds of 8 elements: bf16 before the scale is known, fp32 behind a norm.
+template <int SRC>
+struct Held {
+    uint4 v;
+    __device__ __forceinline__ void get(float (&x)[8]) const { unpack8_bf16(v, x); }
+};
+template <>
+struct Held<kTokNorm> {
+    float v[8];
+    __device__ __forceinline__ void get(float (&x)[8]) const
+    {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = v[i];
+    }
+};
+
+// 8 elements of h; behind a norm, of x + residual.
+template <int SRC>
+__device__ __forceinline__ void row8(const TokenQuantParams& p, const uint16_t* x, const uint16_t* r, int pos, Held<SRC>& h)
+{
+    if constexpr (SRC == kTokNorm) {
+        load8(x, pos, p.K, p.vec_x, h.v);
+        if (r) {
+            float u[8];
+            load8(r, pos, p.K, p.vec_r, u);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h.v[i] = __fadd_rn(h.v[i], u[i]);
+        }
+    } else {
+        h.v = load8_raw(x, pos, p.K, p.vec_x);
+        if (SRC == kTokSwiglu) {
+            float g[8], u[8];
+            const uint4 w = load8_raw(x + p.K, pos, p.K, p.vec_x && p.K % 8 == 0);
+            unpack8_bf16(h.v, g);
+            unpack8_bf16(w, u);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) g[i] = silu_up(g[i], u[i]);
+            h.v = pack8(g);
+        }
     }
 }
 
@@ -109,37 +170,61 @@ __device__ __forceinline__ void emit8(const TokenQuantParams& p, int8_t* q, int 
     }
 }
 
-// VPT vectors a thread in registers; 0: the row is read twice.
-template <int SRC, int VPT>
+__device__ __forceinline__ uint32_t cluster_rank()
+{
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+// (all threads of all blocks of the cluster)
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// A word of this block's shared memory as the cluster's block `rank` has it.
+__device__ __forceinline__ uint32_t peer_word(const uint32_t* p, uint32_t rank)
+{
+    uint32_t at, v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+
+// VPT vectors a thread in registers (0: the row is read twice), a row over CL blocks.
+template <int SRC, int VPT, int CL>
 __global__ void __launch_bounds__(kMaxTokThreads) token_quant_kernel(const TokenQuantParams p)
 {
     __shared__ float red_sum[kMaxTokThreads / 32];
     __shared__ uint32_t red_max[kMaxTokThreads / 32];
+    __shared__ uint32_t mine[2];                              // the block's sum and maximum, for the cluster's others
     const int tid = threadIdx.x, T = blockDim.x, nw = T >> 5;
     // The product that follows may start once everything before this kernel is done: it reads its weights
     // without waiting for the codes.
     pdl_wait();
     pdl_launch_dependents();
 
-    const int64_t row = blockIdx.x;
+    const int64_t row = blockIdx.x / CL;
+    const int rank = CL > 1 ? static_cast<int>(cluster_rank()) : 0;
     const uint16_t* x = p.x + row * p.ldx;
     const uint16_t* r = SRC == kTokNorm && p.res ? p.res + row * p.ldr : nullptr;
     constexpr int HOLD = VPT ? VPT : 1;
     const int vecs = VPT ? VPT : (p.K + 8 * T - 1) / (8 * T);
-    float h[HOLD][8];
+    const auto at = [&](int j) { return ((j * CL + rank) * T + tid) * 8; };
+    Held<SRC> h[HOLD];
     float ss = 0.0f, big = 0.0f;
 #pragma unroll
-    for (int j = 0; j < vecs; ++j) {
-        const int pos = (j * T + tid) * 8;
-        float (&v)[8] = h[VPT ? j : 0];
-        if (pos < p.K) {
-            row8<SRC>(p, x, r, pos, v);
-        } else {
+    for (int j = 0; j < vecs; ++j)
+        if (VPT && at(j) < p.K) row8<SRC>(p, x, r, at(j), h[j]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-        }
+    for (int j = 0; j < vecs; ++j) {
+        const int pos = at(j);
+        if (pos >= p.K) continue;
+        Held<SRC>& e = h[VPT ? j : 0];
+        if (!VPT) row8<SRC>(p, x, r, pos, e);
+        float v[8];
+        e.get(v);
         if (SRC == kTokNorm) {
-            if (p.res_out && pos < p.K) store8(p.res_out + row * p.ldro, pos, p.K, p.vec_ro, v);
+            if (p.res_out) store8(p.res_out + row * p.ldro, pos, p.K, p.vec_ro, v);
 #pragma unroll
             for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
         } else {
@@ -147,7 +232,7 @@ __global__ void __launch_bounds__(kMaxTokThreads) token_quant_kernel(const Token
             for (int i = 0; i < 8; i += 2) big = max_abs_nan(big, v[i], v[i + 1]);
         }
     }
-    if (SRC == kTokNorm) {
+    if constexpr (SRC == kTokNorm) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         if (lane_id() == 0) red_sum[warp_id()] = ss;
@@ -155,63 +240,96 @@ __global__ void __launch_bounds__(kMaxTokThreads) token_quant_kernel(const Token
         ss = static_cast<int>(lane_id()) < nw ? red_sum[lane_id()] : 0.0f;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (CL > 1) {
+            if (tid == 0) mine[0] = __float_as_uint(ss);
+            cluster_sync();
+            ss = 0.0f;
+#pragma unroll
+            for (int c = 0; c < CL; ++c) ss += __uint_as_float(peer_word(&mine[0], c));
+        }
         const float n = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(ss, static_cast<float>(p.K)) + p.eps));
 #pragma unroll
         for (int j = 0; j < HOLD; ++j) {
-            const int pos = (j * T + tid) * 8;
-            if (pos >= p.K) continue;
+            if (at(j) >= p.K) continue;
             float w[8];
-            load_weight8(p, pos, w);
+            load_weight8(p, at(j), w);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) h[j][i] = __fmul_rn(__fmul_rn(h[j][i], n), w[i]);
+            for (int i = 0; i < 8; ++i) h[j].v[i] = __fmul_rn(__fmul_rn(h[j].v[i], n), w[i]);
 #pragma unroll
-            for (int i = 0; i < 8; i += 2) big = max_abs_nan(big, h[j][i], h[j][i + 1]);
+            for (int i = 0; i < 8; i += 2) big = max_abs_nan(big, h[j].v[i], h[j].v[i + 1]);
         }
     }
     uint32_t amax = __reduce_max_sync(0xffffffffu, __float_as_uint(big));     // (as bits, a NaN is the largest)
     if (lane_id() == 0) red_max[warp_id()] = amax;
     __syncthreads();
     amax = __reduce_max_sync(0xffffffffu, static_cast<int>(lane_id()) < nw ? red_max[lane_id()] : 0u);
+    if (CL > 1) {
+        if (tid == 0) mine[1] = amax;
+        cluster_sync();
+#pragma unroll
+        for (int c = 0; c < CL; ++c) amax = max(amax, peer_word(&mine[1], c));
+    }
     const bool finite = amax < 0x7F800000u;
     const float s = finite ? __fdiv_rn(__uint_as_float(amax), 127.0f) : __uint_as_float(0x7FC00000u);
-    if (tid == 0) p.scale[row] = s;
+    if (tid == 0 && rank == 0) p.scale[row] = s;
     const bool fast = finite && s >= 1.1754943508222875e-38f;
     const float rcp = fast ? __frcp_rn(s) : 0.0f;
     int8_t* q = p.q + row * p.ldq;
 #pragma unroll
     for (int j = 0; j < vecs; ++j) {
-        const int pos = (j * T + tid) * 8;
+        const int pos = at(j);
         if (pos >= p.K) continue;
-        if (!VPT) row8<SRC>(p, x, r, pos, h[0]);
-        emit8(p, q, pos, h[VPT ? j : 0], s, rcp, fast);
+        Held<SRC>& e = h[VPT ? j : 0];
+        if (!VPT) row8<SRC>(p, x, r, pos, e);
+        float v[8];
+        e.get(v);
+        emit8(p, q, pos, v, s, rcp, fast);
     }
+    if (CL > 1) cluster_sync();                               // (the others read this block's words until here)
 }
 
-template <int SRC, int VPT>
+template <int SRC, int VPT, int CL = 1>
 cudaError_t launch(const TokenQuantParams& p, int threads, cudaStream_t stream)
 {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.M);
+    cfg.gridDim = dim3(static_cast<unsigned>(p.M) * CL);
     cfg.blockDim = dim3(threads);
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = CL;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, token_quant_kernel<SRC, VPT>, p);
+    cfg.numAttrs = CL > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, token_quant_kernel<SRC, VPT, CL>, p);
 }
+
+constexpr int kFewRows = 64;               // rows that a cluster each is no loss for
+constexpr int kManyRows = 296;
 
 template <int SRC>
 cudaError_t launch_source(const TokenQuantParams& p, cudaStream_t stream)
 {
     const int nvec = (p.K + 7) / 8;
     const auto threads = [&](int vpt) { return ((nvec + vpt - 1) / vpt + 31) / 32 * 32; };
+    if (nvec > 1024 && nvec <= 8 * 1024 && p.M <= kFewRows) return launch<SRC, 1, 8>(p, threads(8), stream);
+    // Many rows: more vectors a thread keep more bytes in flight.
+    if (p.M > kManyRows) {
+        if (SRC != kTokNorm && threads(8) >= 256 && threads(8) <= kMaxTokThreads) return launch<SRC, 8>(p, threads(8), stream);
+        if (threads(4) >= 128 && threads(4) <= kMaxTokThreads) return launch<SRC, 4>(p, threads(4), stream);
+        if (threads(2) >= 128 && threads(2) <= kMaxTokThreads) return launch<SRC, 2>(p, threads(2), stream);
+    }
     if (threads(1) <= kMaxTokThreads) return launch<SRC, 1>(p, threads(1), stream);
     if (threads(2) <= kMaxTokThreads) return launch<SRC, 2>(p, threads(2), stream);
     if (threads(4) <= kMaxTokThreads) return launch<SRC, 4>(p, threads(4), stream);
-    if (SRC == kTokNorm) return cudaErrorInvalidValue;
-    return launch<SRC == kTokNorm ? kTokPlain : SRC, 0>(p, kMaxTokThreads, stream);
+    if constexpr (SRC == kTokNorm) {
+        return cudaErrorInvalidValue;
+    } else {
+        if (threads(8) <= kMaxTokThreads) return launch<SRC, 8>(p, threads(8), stream);
+        return launch<SRC, 0>(p, kMaxTokThreads, stream);
+    }
 }
 
 }  // namespace

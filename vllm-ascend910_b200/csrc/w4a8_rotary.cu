@@ -20,7 +20,7 @@ namespace {
 
 constexpr int kThreads = 256;
 
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p, const int items, const int toks)
+__global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const RotaryParams p, const int items, const int toks)
 {
     pdl_wait();
     const int slot = threadIdx.x / items, j = threadIdx.x - slot * items, slots = kThreads / items;
