@@ -197,6 +197,7 @@ struct CacheView {
 // Rotary positions of their own on up to kMaxAxes axes: row positions[a * ld + t] of the table for
 // the pairs of axis a; pair i's axis is bits 2 (i % 32) of map[i / 32].
 constexpr int kMaxAxes = 4;
+constexpr int kMaxRotaryDim = 256;
 struct AxesView {
     const int32_t* positions;
     int64_t ld;

@@ -6,10 +6,10 @@
 // caller's table holds for the pair in the row of the token's position on the pair's axis
 // (time, height, width of an image's or video's patches; one axis: ordinary positions).
 //
-// A thread owns 16 elements of a head (two vectors of 8 pairs' halves) for one token, so it reads
-// the token's positions and its pairs' angles once and turns its part of every
-// (threads / (items x tokens))-th head with them, four heads' loads in flight.  Elements past `rot`
-// are copied, or left alone in place.
+// A block takes a few tokens.  It finds their cosines and sines first, pair by pair, in shared memory; a
+// thread then stays with 16 elements of a head (two vectors of 8 pairs' halves) and one token, keeps their
+// angles in registers and turns every (threads / (items x tokens))-th head with them, with several heads' loads in
+// flight.  Elements past `rot` are copied, or left alone in place.
 #include <algorithm>
 
 #include "w4a8_rotary.cuh"
@@ -18,58 +18,76 @@ namespace w4a8 {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
+constexpr int kTokLog2 = 2, kTokens = 1 << kTokLog2;     // tokens of a block, where there are many
+constexpr int kAhead = 2;
+constexpr int kManyTokens = 592;
 
-__global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const RotaryParams p, const int items, const int toks)
+// MANY: kTokens tokens and all their heads; else one token and `heads_each` heads of q or, in a token's later blocks, of k.
+template <bool INTERLEAVED, bool MANY>
+__global__ void __launch_bounds__(kThreads, 8) rotary_kernel(const RotaryParams p, const int items, const int heads_each)
 {
+    __shared__ __align__(16) float angles[kTokens][kMaxRotaryDim];
     pdl_wait();
-    const int slot = threadIdx.x / items, j = threadIdx.x - slot * items, slots = kThreads / items;
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * toks + slot % toks;
-    const int step = slots / toks, h_first = slot / toks;
-    if (t >= p.tokens || h_first >= step) return;             // (threads past the last whole set of slots)
+    constexpr int tok_log2 = MANY ? kTokLog2 : 0, toks = 1 << tok_log2;
+    const int tid = threadIdx.x, half = p.rot / 2;
+    const int64_t t0 = static_cast<int64_t>(blockIdx.x) << tok_log2;
+    const int step = (kThreads / items) >> tok_log2, slot = tid / items, j = tid - slot * items;
+    const int k_tok = slot & (toks - 1), first = slot >> tok_log2;
+    const int64_t t = t0 + k_tok;
+    const bool on = first < step && t < p.tokens;             // (not the threads past the last whole set)
+
     const bool turn = j < p.rot / 16;
     int c0, c1;
     if (turn) {
-        item_cols(j, p.rot, p.interleaved, c0, c1);
+        item_cols(j, p.rot, INTERLEAVED, c0, c1);
     } else {
         c0 = p.rot + 16 * (j - p.rot / 16);
         c1 = c0 + 8 < p.D ? c0 + 8 : c0;                     // (the last vector of D = 8 mod 16 twice)
     }
+    const int q_parts = MANY ? 0 : (p.heads[0] + heads_each - 1) / heads_each;
+    const int w0 = !MANY && static_cast<int>(blockIdx.y) >= q_parts;
+    const int h0 = MANY ? first : (static_cast<int>(blockIdx.y) - (w0 ? q_parts : 0)) * heads_each + first;
+    const int end0 = !on ? 0 : MANY ? p.heads[0] : min(h0 - first + heads_each, p.heads[w0]);
+    uint4 v[kAhead][2];
+    const auto load = [&](const uint16_t* src, int h, int end) {
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k, h += step)
+            if (h < end) {
+                const uint16_t* at = src + static_cast<int64_t>(h) * p.D;
+                v[k][0] = *reinterpret_cast<const uint4*>(at + c0);
+                v[k][1] = *reinterpret_cast<const uint4*>(at + c1);
+            }
+    };
+    load(p.x[w0] + t * p.ld[w0], h0, end0);
+    for (int i = tid; i < half << tok_log2; i += kThreads) {
+        const int k = i / half, pair = i - k * half, a = static_cast<int>(p.axes.map[pair >> 5] >> (2 * (pair & 31))) & 3;
+        const int64_t at = min(t0 + k, p.tokens - 1);
+        const float* row = p.cos_sin + clamp_row(p.axes.positions[a * p.axes.ld + at], p.table_rows) * p.rot;
+        angles[k][pair] = row[pair];
+        angles[k][half + pair] = row[half + pair];
+    }
+    __syncthreads();
+    if (!on) return;
     float4 cs[4] = {};
-    constexpr int AHEAD = 4;
-    bool have = false;
+    if (turn) load_angles(angles[k_tok], j, p.rot, cs);
 #pragma unroll 1
-    for (int w = 0; w < 2; ++w) {
-        if (!p.x[w] || (!turn && p.x[w] == p.out[w] && p.ld[w] == p.ldo[w])) continue;
+    for (int w = w0; w < (MANY ? 2 : w0 + 1); ++w) {
+        const int end = w == w0 ? end0 : p.heads[1];
         const uint16_t* src = p.x[w] + t * p.ld[w];
         uint16_t* dst = p.out[w] + t * p.ldo[w];
-        for (int h0 = h_first; h0 < p.heads[w]; h0 += AHEAD * step) {
-            uint4 v[AHEAD][2];
+        if (!turn && src == dst) continue;
+        if (w != w0) load(src, h0, end);
+        for (int h = h0; h < end; h += kAhead * step) {
 #pragma unroll
-            for (int k = 0; k < AHEAD; ++k) {
-                const int64_t h = min(h0 + k * step, p.heads[w] - 1);
-                v[k][0] = *reinterpret_cast<const uint4*>(src + h * p.D + c0);
-                v[k][1] = *reinterpret_cast<const uint4*>(src + h * p.D + c1);
-            }
-            if (turn && !have) {
-                load_angles_axes(p.cos_sin, p.axes, axis_rows(p.axes, t, p.table_rows), j, p.rot, cs);
-                have = true;
-            }
-#pragma unroll
-            for (int k = 0; k < AHEAD; ++k) {
-                const int64_t h = h0 + k * step;
-                if (h >= p.heads[w]) break;
-                if (turn) {
-                    float a[8], b[8];
-                    unpack8_bf16(v[k][0], a);
-                    unpack8_bf16(v[k][1], b);
-                    rotate_item(p.interleaved, cs, a, b);
-                    v[k][0] = pack8(a);
-                    v[k][1] = pack8(b);
+            for (int k = 0, g = h; k < kAhead; ++k, g += step)
+                if (g < end) {
+                    if (turn) turn_item(INTERLEAVED, cs, v[k][0], v[k][1]);
+                    uint16_t* at = dst + static_cast<int64_t>(g) * p.D;
+                    *reinterpret_cast<uint4*>(at + c0) = v[k][0];
+                    *reinterpret_cast<uint4*>(at + c1) = v[k][1];
                 }
-                *reinterpret_cast<uint4*>(dst + h * p.D + c0) = v[k][0];
-                *reinterpret_cast<uint4*>(dst + h * p.D + c1) = v[k][1];
-            }
+            load(src, h + kAhead * step, end);
         }
     }
 }
@@ -79,11 +97,13 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const RotaryParams 
 cudaError_t launch_rotary(const RotaryParams& p, cudaStream_t stream)
 {
     const int items = p.rot / 16 + (p.D - p.rot + 15) / 16, slots = kThreads / items;
-    const int toks = p.tokens < 592 ? 1 : std::min(4, slots);
-    const int64_t blocks = (p.tokens + toks - 1) / toks;
-    if (blocks > 0x7FFFFFFF) return cudaErrorInvalidValue;
+    const bool many = p.tokens >= kManyTokens;
+    const int each = many ? 0 : slots;
+    const int64_t blocks = many ? (p.tokens + kTokens - 1) >> kTokLog2 : p.tokens;
+    const int parts = many ? 1 : (p.heads[0] + each - 1) / each + (p.heads[1] + each - 1) / each;
+    if (blocks > 0x7FFFFFFF || parts > 65535) return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+    cfg.gridDim = dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(parts));
     cfg.blockDim = dim3(kThreads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -91,7 +111,11 @@ cudaError_t launch_rotary(const RotaryParams& p, cudaStream_t stream)
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, rotary_kernel, p, items, toks);
+    if (many)
+        return p.interleaved ? cudaLaunchKernelEx(&cfg, rotary_kernel<true, true>, p, items, each)
+                             : cudaLaunchKernelEx(&cfg, rotary_kernel<false, true>, p, items, each);
+    return p.interleaved ? cudaLaunchKernelEx(&cfg, rotary_kernel<true, false>, p, items, each)
+                         : cudaLaunchKernelEx(&cfg, rotary_kernel<false, false>, p, items, each);
 }
 
 }  // namespace w4a8

@@ -71,16 +71,46 @@ __device__ __forceinline__ int64_t clamp_row(int64_t pos, int64_t rows)
 }
 
 
+// rotate_item on the 16 elements as they are stored, two products an instruction.  The sums stay single
+// ones: a packed sum of packed products may become a fused one, which rounds once.
+__device__ __forceinline__ void turn_item(int interleaved, const float4 (&cs)[4], uint4& v0, uint4& v1)
+{
+    const uint64_t c[4] = {pair2(cs[0].x, cs[0].y), pair2(cs[0].z, cs[0].w), pair2(cs[1].x, cs[1].y), pair2(cs[1].z, cs[1].w)};
+    const uint64_t s[4] = {pair2(cs[2].x, cs[2].y), pair2(cs[2].z, cs[2].w), pair2(cs[3].x, cs[3].y), pair2(cs[3].z, cs[3].w)};
+    uint32_t* w[2] = {&v0.x, &v1.x};
+    const auto low = [](uint32_t x) { return __uint_as_float(x << 16); };
+    const auto high = [](uint32_t x) { return __uint_as_float(x & 0xFFFF0000u); };
+    const auto pack = [](float lo, float hi) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&b);
+    };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        // pairs 2 i and 2 i + 1: a word of either half, or two words next to each other
+        uint32_t &x = interleaved ? w[i >> 1][(2 * i) & 3] : w[0][i], &y = interleaved ? w[i >> 1][(2 * i + 1) & 3] : w[1][i];
+        const uint64_t a = interleaved ? pair2(low(x), low(y)) : pair2(low(x), high(x));
+        const uint64_t b = interleaved ? pair2(high(x), high(y)) : pair2(low(y), high(y));
+        float ac0, ac1, bs0, bs1, bc0, bc1, as0, as1;
+        unpair2(f2_mul(a, c[i]), ac0, ac1);
+        unpair2(f2_mul(b, s[i]), bs0, bs1);
+        unpair2(f2_mul(b, c[i]), bc0, bc1);
+        unpair2(f2_mul(a, s[i]), as0, as1);
+        const float a0 = __fsub_rn(ac0, bs0), a1 = __fsub_rn(ac1, bs1), b0 = __fadd_rn(bc0, as0), b1 = __fadd_rn(bc1, as1);
+        x = interleaved ? pack(a0, b0) : pack(a0, a1);
+        y = interleaved ? pack(a1, b1) : pack(b0, b1);
+    }
+}
+
 // Rows of the table that a token's axes point at.
 struct AxisRows {
-    int64_t at[kMaxAxes];
+    int32_t at[kMaxAxes];
 };
 
 __device__ __forceinline__ AxisRows axis_rows(const AxesView& v, int64_t t, int64_t rows)
 {
     AxisRows r;
 #pragma unroll
-    for (int a = 0; a < kMaxAxes; ++a) r.at[a] = a < v.axes ? clamp_row(v.positions[a * v.ld + t], rows) : 0;
+    for (int a = 0; a < kMaxAxes; ++a) r.at[a] = a < v.axes ? static_cast<int32_t>(clamp_row(v.positions[a * v.ld + t], rows)) : 0;
     return r;
 }
 
@@ -91,10 +121,10 @@ __device__ __forceinline__ void load_angles_axes(const float* table, const AxesV
 {
     const uint32_t bits = static_cast<uint32_t>(v.map[j >> 2] >> (16 * (j & 3))) & 0xFFFFu;
     const int first = bits & 3;
-    int64_t row = r.at[0];
+    int32_t row = r.at[0];
 #pragma unroll
     for (int a = 1; a < kMaxAxes; ++a) row = first == a ? r.at[a] : row;
-    load_angles(table + row * rot, j, rot, cs);
+    load_angles(table + static_cast<int64_t>(row) * rot, j, rot, cs);
     if (bits == first * 0x5555u) return;
 #pragma unroll
     for (int a = 0; a < kMaxAxes; ++a) {
@@ -102,7 +132,7 @@ __device__ __forceinline__ void load_angles_axes(const float* table, const AxesV
         const uint32_t x = bits ^ (a * 0x5555u), mine = ~(x | (x >> 1)) & 0x5555u;
         if (a == first || mine == 0) continue;
         float4 o[4];
-        load_angles(table + r.at[a] * rot, j, rot, o);
+        load_angles(table + static_cast<int64_t>(r.at[a]) * rot, j, rot, o);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             float4 &c = cs[i], &s = cs[2 + i];
