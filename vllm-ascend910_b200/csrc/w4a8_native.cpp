@@ -1,5 +1,6 @@
 // w4a8_native.cpp -- a short way from Python to the C entry points of the operators
-// that decode steps call most: norm, cache write and read, attention.
+// that decode steps call most: norm, cache write and read, attention, 8-bit linears, rotary
+// positions, pages.
 //
 // The Python wrappers (ops.py, kvcache.py) read some thirty tensor attributes a call
 // to check their arguments, which costs more than such a call's kernels run.  These
@@ -25,6 +26,11 @@ struct Table {
     decltype(&w4a8_kv_write) kv_write;
     decltype(&w4a8_kv_read) kv_read;
     decltype(&w4a8_attention) attention;
+    decltype(&w4a8_int8_linear) int8_linear;
+    decltype(&w4a8_int8_linear_rms_norm) int8_linear_rms_norm;
+    decltype(&w4a8_rotary) rotary;
+    decltype(&w4a8_pages_plan) pages_plan;
+    decltype(&w4a8_pages_shrink) pages_shrink;
 } g{};
 
 PyObject* later()
@@ -254,6 +260,151 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n)
     return rc == W4A8_OK ? wrap(out) : later();
 }
 
+// An 8-bit layer (_lib.Int8LayerDesc).
+struct Layer {
+    const int8_t* w;
+    const float *scale, *bias;
+    int64_t N, K, ldw;
+};
+
+const Layer* layer_of(PyObject* o) { return PyLong_Check(o) ? static_cast<const Layer*>(PyLong_AsVoidPtr(o)) : nullptr; }
+
+at::Tensor outputs(const at::Tensor* x, int64_t N, int dev)
+{
+    if (x->dim() == 2) return make({x->size(0), N}, at::kBFloat16, dev);
+    std::vector<int64_t> size(x->sizes().begin(), x->sizes().end());
+    size.back() = N;
+    return make(size, at::kBFloat16, dev);
+}
+
+// linear_int8(layer, device, x, act, workspace, workspace bytes)
+PyObject* linear_int8(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    if (n != 6 || !g.int8_linear || !PyLong_Check(a[1]) || !PyLong_Check(a[3]) || !PyLong_Check(a[4]) || !PyLong_Check(a[5])) return later();
+    const Layer* L = layer_of(a[0]);
+    const int dev = static_cast<int>(PyLong_AsLong(a[1])), act = static_cast<int>(PyLong_AsLong(a[3]));
+    const at::Tensor* x = tensor(a[2]);
+    if (!L || !x || x->dim() < 1 || !dense(x, at::kBFloat16, dev, x->dim()) || !current(dev)) return later();
+    const int64_t wide = act == W4A8_ACT_SWIGLU ? 2 * L->K : L->K;
+    if (x->size(-1) != wide || x->numel() == 0) return later();
+    at::Tensor y = outputs(x, L->N, dev);
+    const int rc = g.int8_linear(ptr(x), x->numel() / wide, L->K, wide, act, L->w, L->ldw, L->scale, L->bias, L->N, y.data_ptr(), L->N,
+                                 PyLong_AsVoidPtr(a[4]), static_cast<size_t>(PyLong_AsUnsignedLongLong(a[5])), stream(dev));
+    return rc == W4A8_OK ? wrap(y) : later();
+}
+
+// linear_int8_rms_norm(x, weight, residual or None, eps, layer, workspace, workspace bytes)
+PyObject* linear_int8_rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    Rows t;
+    if (n != 7 || !PyFloat_Check(a[3]) || !PyLong_Check(a[5]) || !PyLong_Check(a[6]) || !g.int8_linear_rms_norm || !rows(a, t)) return later();
+    const Layer* L = layer_of(a[4]);
+    if (!L || L->K != t.K || t.M == 0) return later();
+    at::Tensor y = outputs(t.x, L->N, t.dev), ro;
+    if (t.r) ro = make(t.x->sizes(), at::kBFloat16, t.dev);
+    const int rc = g.int8_linear_rms_norm(ptr(t.x), t.M, t.K, t.K, ptr(t.r), t.r ? t.K : 0, t.r ? ro.data_ptr() : nullptr,
+                                          t.r ? t.K : 0, ptr(t.w), t.wd, static_cast<float>(PyFloat_AS_DOUBLE(a[3])), L->w, L->ldw,
+                                          L->scale, L->bias, L->N, y.data_ptr(), L->N, PyLong_AsVoidPtr(a[5]),
+                                          static_cast<size_t>(PyLong_AsUnsignedLongLong(a[6])), stream(t.dev));
+    if (rc != W4A8_OK) return later();
+    return t.r ? pair(wrap(y), wrap(ro)) : wrap(y);
+}
+
+// [tokens, heads, D] with dense heads and 16-byte rows; its row stride.
+bool plain_heads(const at::Tensor* t, int dev, int64_t D, int64_t& ld)
+{
+    if (!is(t, at::kBFloat16, dev, 3) || t->size(2) != D || t->size(0) == 0 || t->size(1) == 0) return false;
+    ld = t->stride(0);
+    return t->stride(2) == 1 && (t->stride(1) == D || t->size(1) == 1) && ld % 8 == 0 && ld >= t->size(1) * D &&
+           reinterpret_cast<uintptr_t>(t->const_data_ptr()) % 16 == 0;
+}
+
+// rotary(q, k or None, cos_sin, positions, axes, pairs, axis of each pair or 0, interleaved)
+PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    if (n != 8 || !g.rotary || !PyLong_Check(a[4]) || !PyLong_Check(a[5]) || !PyLong_Check(a[6])) return later();
+    const at::Tensor *q = tensor(a[0]), *k = nullptr, *cs = tensor(a[2]), *pos = tensor(a[3]);
+    if (!q || !q->is_cuda() || q->dim() != 3) return later();
+    const int dev = q->get_device(), axes = static_cast<int>(PyLong_AsLong(a[4]));
+    const int64_t D = q->size(2), T = q->size(0);
+    int64_t ldq = 0, ldk = 0;
+    if (!plain_heads(q, dev, D, ldq) || !current(dev)) return later();
+    if (a[1] != Py_None) {
+        k = tensor(a[1]);
+        if (!plain_heads(k, dev, D, ldk) || k->size(0) != T) return later();
+    }
+    if (!dense(cs, at::kFloat, dev, 2) || cs->numel() == 0 || cs->size(1) != 2 * PyLong_AsLong(a[5])) return later();
+    if (!dense(pos, at::kInt, dev, 2) || pos->size(0) != axes || pos->size(1) != T) return later();
+    const int interleaved = PyObject_IsTrue(a[7]);
+    if (interleaved < 0) {
+        PyErr_Clear();
+        return later();
+    }
+    at::Tensor qo = make(q->sizes(), at::kBFloat16, dev), ko;
+    if (k) ko = make(k->sizes(), at::kBFloat16, dev);
+    const int rc = g.rotary(ptr(q), ldq, static_cast<int32_t>(q->size(1)), qo.data_ptr(), q->size(1) * D, ptr(k), ldk,
+                            k ? static_cast<int32_t>(k->size(1)) : 0, k ? ko.data_ptr() : nullptr, k ? k->size(1) * D : 0, T,
+                            static_cast<int32_t>(D), static_cast<const float*>(ptr(cs)), cs->size(0),
+                            static_cast<int32_t>(cs->size(1)), interleaved, ints(pos), T, axes,
+                            static_cast<const uint8_t*>(PyLong_AsVoidPtr(a[6])), stream(dev));
+    if (rc != W4A8_OK) return later();
+    return pair(wrap(qo), k ? wrap(ko) : Py_NewRef(Py_None));
+}
+
+// pages_plan(state, device, rows, counts, tokens, axes, seg_cu or None, segs or None)
+PyObject* pages_plan(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    if (n != 8 || !g.pages_plan || !PyLong_Check(a[0]) || !PyLong_Check(a[1]) || !PyLong_Check(a[4]) || !PyLong_Check(a[5])) return later();
+    const w4a8_page_state* st = static_cast<const w4a8_page_state*>(PyLong_AsVoidPtr(a[0]));
+    const int dev = static_cast<int>(PyLong_AsLong(a[1]));
+    const int64_t tokens = PyLong_AsLongLong(a[4]), axes = PyLong_AsLongLong(a[5]);
+    const at::Tensor *rows = tensor(a[2]), *counts = tensor(a[3]), *cu = nullptr, *segs = nullptr;
+    if (!st || tokens < 0 || axes < 1 || axes > 4 || !dense(rows, at::kInt, dev, 1) || !dense(counts, at::kInt, dev, 1) || !current(dev)) {
+        PyErr_Clear();
+        return later();
+    }
+    const int64_t B = rows->size(0);
+    if (counts->size(0) != B || B > W4A8_PLAN_MAX_BATCH) return later();
+    if (a[6] != Py_None) {
+        cu = tensor(a[6]);
+        segs = tensor(a[7]);
+        if (!dense(cu, at::kInt, dev, 1) || !dense(segs, at::kInt, dev, 2) || cu->size(0) != B + 1 || segs->size(1) != 4) return later();
+    }
+    const at::Tensor out[5] = {make({B, st->columns}, at::kInt, dev), make({B}, at::kInt, dev), make({B + 1}, at::kInt, dev),
+                               make({tokens}, at::kInt, dev), make({axes, tokens}, at::kInt, dev)};
+    int32_t* p[5];
+    for (int i = 0; i < 5; ++i) p[i] = static_cast<int32_t*>(out[i].data_ptr());
+    const int rc = g.pages_plan(st, ints(rows), ints(counts), B, tokens, static_cast<int32_t>(axes), cu ? ints(cu) : nullptr,
+                                segs ? ints(segs) : nullptr, segs ? segs->size(0) : 0, p[0], p[1], p[2], p[3], p[4], stream(dev));
+    if (rc != W4A8_OK) return later();
+    PyObject* r = PyTuple_New(5);
+    for (int i = 0; r && i < 5; ++i) {
+        PyObject* o = wrap(out[i]);
+        if (!o) {
+            Py_DECREF(r);
+            return nullptr;
+        }
+        PyTuple_SET_ITEM(r, i, o);
+    }
+    return r;
+}
+
+// pages_shrink(state, device, rows, keep or None): True
+PyObject* pages_shrink(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    if (n != 4 || !g.pages_shrink || !PyLong_Check(a[0]) || !PyLong_Check(a[1])) return later();
+    const int dev = static_cast<int>(PyLong_AsLong(a[1]));
+    const at::Tensor *rows = tensor(a[2]), *keep = nullptr;
+    if (!dense(rows, at::kInt, dev, 1) || !current(dev)) return later();
+    if (a[3] != Py_None) {
+        keep = tensor(a[3]);
+        if (!dense(keep, at::kInt, dev, 1) || keep->size(0) != rows->size(0)) return later();
+    }
+    const int rc = g.pages_shrink(static_cast<const w4a8_page_state*>(PyLong_AsVoidPtr(a[0])), ints(rows), keep ? ints(keep) : nullptr,
+                                  rows->size(0), stream(dev));
+    return rc == W4A8_OK ? Py_NewRef(Py_True) : later();
+}
+
 // C++ exceptions (an allocation that fails) become Python ones.
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t n)
@@ -268,26 +419,46 @@ PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t n)
     }
 }
 
-// bind(addresses of the entry points, in Table's order)
-PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n)
+// Addresses of entry points, in order.
+bool addresses(PyObject* const* a, Py_ssize_t n, void* (&p)[5])
 {
     if (n != 5) {
         PyErr_SetString(PyExc_TypeError, "bind: five addresses");
-        return nullptr;
+        return false;
     }
-    void* p[5];
     for (int i = 0; i < 5; ++i) {
         p[i] = PyLong_AsVoidPtr(a[i]);
         if (!p[i]) {
             if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "bind: null address");
-            return nullptr;
+            return false;
         }
     }
+    return true;
+}
+
+// bind(rms_norm, rms_norm_quant, kv_write, kv_read, attention)
+PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    void* p[5];
+    if (!addresses(a, n, p)) return nullptr;
     g.rms_norm = reinterpret_cast<decltype(g.rms_norm)>(p[0]);
     g.rms_norm_quant = reinterpret_cast<decltype(g.rms_norm_quant)>(p[1]);
     g.kv_write = reinterpret_cast<decltype(g.kv_write)>(p[2]);
     g.kv_read = reinterpret_cast<decltype(g.kv_read)>(p[3]);
     g.attention = reinterpret_cast<decltype(g.attention)>(p[4]);
+    Py_RETURN_NONE;
+}
+
+// bind_more(int8_linear, int8_linear_rms_norm, rotary, pages_plan, pages_shrink)
+PyObject* bind_more(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    void* p[5];
+    if (!addresses(a, n, p)) return nullptr;
+    g.int8_linear = reinterpret_cast<decltype(g.int8_linear)>(p[0]);
+    g.int8_linear_rms_norm = reinterpret_cast<decltype(g.int8_linear_rms_norm)>(p[1]);
+    g.rotary = reinterpret_cast<decltype(g.rotary)>(p[2]);
+    g.pages_plan = reinterpret_cast<decltype(g.pages_plan)>(p[3]);
+    g.pages_shrink = reinterpret_cast<decltype(g.pages_shrink)>(p[4]);
     Py_RETURN_NONE;
 }
 
@@ -298,11 +469,17 @@ PyCFunction entry()
 }
 
 PyMethodDef methods[] = {{"bind", entry<bind>(), METH_FASTCALL, nullptr},
+                         {"bind_more", entry<bind_more>(), METH_FASTCALL, nullptr},
                          {"rms_norm", entry<rms_norm>(), METH_FASTCALL, nullptr},
                          {"rms_norm_quant", entry<rms_norm_quant>(), METH_FASTCALL, nullptr},
                          {"kv_write", entry<kv_write>(), METH_FASTCALL, nullptr},
                          {"kv_read", entry<kv_read>(), METH_FASTCALL, nullptr},
                          {"attention", entry<attention>(), METH_FASTCALL, nullptr},
+                         {"linear_int8", entry<linear_int8>(), METH_FASTCALL, nullptr},
+                         {"linear_int8_rms_norm", entry<linear_int8_rms_norm>(), METH_FASTCALL, nullptr},
+                         {"rotary", entry<rotary>(), METH_FASTCALL, nullptr},
+                         {"pages_plan", entry<pages_plan>(), METH_FASTCALL, nullptr},
+                         {"pages_shrink", entry<pages_shrink>(), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -131,6 +131,11 @@ class KvCacheDesc(ctypes.Structure):
                 ("page_size", _i32), ("head_dim", _i32), ("reserved", _i32)]
 
 
+class Int8LayerDesc(ctypes.Structure):
+    """An 8-bit layer as ``_native`` takes it."""
+    _fields_ = [("w", _p), ("scale", _p), ("bias", _p), ("N", _i64), ("K", _i64), ("ldw", _i64)]
+
+
 class PageStateDesc(ctypes.Structure):
     """w4a8_page_state."""
     _fields_ = [("free_pages", _p), ("free_count", _p), ("table", _p), ("lens", _p), ("control", _p), ("pages", _i64),
@@ -171,8 +176,9 @@ def native():
         except ImportError:
             N = None
         if N is not None:
-            N.bind(*(ctypes.cast(getattr(L, name), _p).value for name in
-                     ("w4a8_rms_norm", "w4a8_rms_norm_quant", "w4a8_kv_write", "w4a8_kv_read", "w4a8_attention")))
+            at = lambda *names: [ctypes.cast(getattr(L, "w4a8_" + n), _p).value for n in names]       # noqa: E731
+            N.bind(*at("rms_norm", "rms_norm_quant", "kv_write", "kv_read", "attention"))
+            N.bind_more(*at("int8_linear", "int8_linear_rms_norm", "rotary", "pages_plan", "pages_shrink"))
         _N = N
     return _N
 

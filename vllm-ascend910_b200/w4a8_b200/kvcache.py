@@ -136,7 +136,7 @@ class RotaryAxes:
     width, ...; up to four), one axis after another, or ``mixed``: 0 1 2 0 1 2 ..., an axis whose pairs are used
     up left out.  Twice their sum is the rotary table's width."""
 
-    __slots__ = ("axes", "pairs", "_map")
+    __slots__ = ("axes", "pairs", "_map", "_ref")
 
     def __init__(self, sections: Sequence[int], mixed: bool = False):
         left = [int(n) for n in sections]
@@ -154,6 +154,7 @@ class RotaryAxes:
                         left[a] -= 1
                         ids.append(a)
         self._map = (ctypes.c_uint8 * self.pairs)(*ids)
+        self._ref = ctypes.addressof(self._map)
 
     def axis_of_pair(self) -> List[int]:
         return list(self._map)
@@ -209,6 +210,11 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], cos_sin: torch.Tensor, po
 
     positions int32 [axes, tokens] are read on the device; rows outside the table are its first or last one.
     ``q_out`` and ``k_out`` may be q and k."""
+    nat = _lib.native()
+    if nat is not None and axes is not None and q_out is None and k_out is None:
+        got = nat.rotary(q, k, cos_sin, positions, axes.axes, axes.pairs, axes._ref, interleaved)
+        if got is not NotImplemented:
+            return got
     what = "rotary"
     if not q.is_cuda or q.dim() != 3:
         raise RuntimeError("rotary: q must be a CUDA tensor [tokens, heads, head_dim] (there is no CPU implementation)")
@@ -473,6 +479,11 @@ def pages_plan(state: PageState, rows: torch.Tensor, counts: torch.Tensor, token
 
     A step that cannot be done as a whole (a row twice, too few pages, ...) changes nothing, comes back without pages and
     tokens, and leaves its reason for ``state.check()``."""
+    nat = _lib.native()
+    if nat is not None:
+        got = nat.pages_plan(state._ref, state._index, rows, counts, tokens, axes, *((None, None) if images is None else images))
+        if got is not NotImplemented:
+            return StepMaps(*got)
     B = _rows_of("pages_plan", state, rows, counts, "counts")
     if tokens < 0 or not 1 <= axes <= _lib.MAX_AXES:
         raise RuntimeError(f"pages_plan: tokens must not be negative, axes 1 to {_lib.MAX_AXES}")
@@ -500,6 +511,9 @@ def pages_shrink(state: PageState, rows: torch.Tensor, keep: Optional[torch.Tens
     """Sequence ``rows[i]`` keeps its first ``keep[i]`` tokens (None: none) and gives back its pages past them, from the last
     page of the last sequence to the first: what ``pages_plan`` over the same rows took, in the places it took it from.
     For sequences that ended and drafted tokens that were not accepted.  Refused as a whole like a plan."""
+    nat = _lib.native()
+    if nat is not None and nat.pages_shrink(state._ref, state._index, rows, keep) is not NotImplemented:
+        return
     B = _rows_of("pages_shrink", state, rows, keep, "keep")
     rc = _launch(state._index, _lib.lib().w4a8_pages_shrink, state._ref, rows.data_ptr(), None if keep is None else keep.data_ptr(),
                  B, _stream_of(rows))

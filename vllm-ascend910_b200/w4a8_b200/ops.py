@@ -13,6 +13,7 @@ while it was current keeps writing to it on every replay.
 """
 from __future__ import annotations
 
+import ctypes
 from typing import Dict, List, Optional, Tuple
 
 import torch
@@ -555,12 +556,14 @@ def linear_prepared_rms_norm(x: torch.Tensor, weight: torch.Tensor, pw: Prepared
 class Int8Weight:
     """An 8-bit linear's layer: codes int8 [N, K] (rows of a multiple of 16 bytes), fp32 scales and bias [N]."""
 
-    __slots__ = ("w", "scale", "bias", "N", "K", "ldw", "device", "_args")
+    __slots__ = ("w", "scale", "bias", "N", "K", "ldw", "device", "_args", "_desc", "_ref", "_index")
 
     def __init__(self, w: torch.Tensor, scale: torch.Tensor, bias: Optional[torch.Tensor], K: int):
         self.w, self.scale, self.bias = w, scale, bias
         self.N, self.K, self.ldw, self.device = w.shape[0], K, w.stride(0), w.device
         self._args = (w.data_ptr(), self.ldw, scale.data_ptr(), _ptr(bias), self.N)
+        self._desc = _lib.Int8LayerDesc(w.data_ptr(), scale.data_ptr(), _ptr(bias), self.N, K, self.ldw)
+        self._ref, self._index = ctypes.addressof(self._desc), w.get_device()
 
 
 def prepare_int8(w: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None) -> Int8Weight:
@@ -636,6 +639,13 @@ def linear_int8(x: torch.Tensor, layer: Int8Weight, act: Optional[str] = None,
                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y = x @ W^T (+ bias) in 8-bit integers: x bf16 [..., K] quantised per token (``quant_token``), exact integer
     sums, bf16 [..., N].  act="swiglu": x = [gate | up], [..., 2 K]; ``out``: bf16 [M, N] with dense rows."""
+    nat = _lib.native()
+    if nat is not None and out is None and (act is None or act == "swiglu"):
+        # a workspace that is too small for the call is refused, and grown below
+        got = nat.linear_int8(layer._ref, layer._index, x, _lib.ACT_NONE if act is None else _lib.ACT_SWIGLU,
+                              *workspace(0, layer.device))
+        if got is not NotImplemented:
+            return got
     if x.dtype is not _BF16 or x.device != layer.device:
         raise RuntimeError("linear_int8: x must be bfloat16 on the layer's device (there is no CPU implementation)")
     K, N = layer.K, layer.N
@@ -660,6 +670,11 @@ def linear_int8_rms_norm(x: torch.Tensor, weight: torch.Tensor, layer: Int8Weigh
                          out: Optional[torch.Tensor] = None):
     """``linear_int8`` on the norm of x (+ residual), whose fp32 result is quantised per token as it is made.
     Returns y, or (y, bf16(x + residual))."""
+    nat = _lib.native()
+    if nat is not None and residual_out is None and out is None and x.device == layer.device:
+        got = nat.linear_int8_rms_norm(x, weight, residual, eps, layer._ref, *workspace(0, layer.device))
+        if got is not NotImplemented:
+            return got
     what = "linear_int8_rms_norm"
     x2, M, K, ldx, wd, r2, rp, ldr, ro, rop, ldro = _norm_args(x, weight, residual, residual_out, what)
     if x.device != layer.device:
@@ -668,12 +683,11 @@ def linear_int8_rms_norm(x: torch.Tensor, weight: torch.Tensor, layer: Int8Weigh
         raise RuntimeError(f"{what}: x has last dimension {K}, the layer takes {layer.K}")
     N = layer.N
     y, ldy = _int8_out(out, M, N, layer, what)
-    if M > 0:
-        ws, wsb = _int8_ws(M, K, x.device)
-        rc = _launch(x2.get_device(), _lib.lib().w4a8_int8_linear_rms_norm, x2.data_ptr(), M, K, ldx, rp, ldr, rop, ldro,
-                     weight.data_ptr(), wd, eps, *layer._args, y.data_ptr(), ldy, ws, wsb, _stream_of(x2))
-        if rc != 0:
-            _lib.check(rc, "w4a8_int8_linear_rms_norm")
+    ws, wsb = _int8_ws(M, K, x.device)
+    rc = _launch(x2.get_device(), _lib.lib().w4a8_int8_linear_rms_norm, x2.data_ptr(), M, K, ldx, rp, ldr, rop, ldro,
+                 weight.data_ptr(), wd, eps, *layer._args, y.data_ptr(), ldy, ws, wsb, _stream_of(x2))
+    if rc != 0:
+        _lib.check(rc, "w4a8_int8_linear_rms_norm")
     if x.dim() != 2:
         y = y.view(*x.shape[:-1], N)
         ro = None if ro is None else ro.view(x.shape)
