@@ -23,6 +23,7 @@
 // Each wait for a barrier is bounded; one that runs out ends the CTA's roles and leaves a code in
 // the workspace's status word.
 #include <algorithm>
+#include <atomic>
 
 #include "w4a8_common.cuh"
 #include "w4a8_kernels.h"
@@ -31,7 +32,8 @@ namespace w4a8 {
 
 namespace {
 
-constexpr int kThreads = 192;              // producer, issuer, four epilogue warps
+constexpr int kThreads = 192;              // few: producer, issuer, four epilogue warps
+constexpr int kManyThreads = 320;          // many: eight epilogue warps
 constexpr int kFewTokens = 128;
 
 // Ids of the waits in the status word (kDevTimeoutBase + id; the other kernels' are smaller).
@@ -78,12 +80,12 @@ __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint3
 }
 
 // Arrive on `bar` of both CTAs of the pair once the MMAs issued so far are done.
-__device__ __forceinline__ void commit_pair(uint64_t* bar)
+__device__ __forceinline__ void commit_pair(uint64_t* bar, uint32_t lead)
 {
     asm volatile(
         "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
             smem_u32(bar)),
-        "h"(static_cast<uint16_t>(3))
+        "h"(static_cast<uint16_t>(3u << lead))
         : "memory");
 }
 
@@ -155,18 +157,82 @@ __device__ __forceinline__ uint32_t two(float lo, float hi)
     return *reinterpret_cast<const uint32_t*>(&b);
 }
 
+// 32 sums of a lane's row (channels n .. n + 31) into y: scaled, rounded and stored by the widest access that
+// `align` allows.  All lanes of the warp call it; `turn` is the warp's.
+// `scale`, `bias`: the channels' in shared memory.
+__device__ __forceinline__ void put32(const Int8GemmParams& p, const uint32_t (&r)[32], int n, int64_t row, bool in, float s,
+                                      const float* scale, const float* bias, int align, uint16_t (*turn)[34])
+{
+    const int lane = lane_id();
+    uint16_t* y = p.y + row * p.ldy + n;
+    if (n + 32 <= p.N && align >= 16) {
+        uint32_t o[16];
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+            const float4 ws = *reinterpret_cast<const float4*>(scale + i), b = *reinterpret_cast<const float4*>(bias + i);
+            o[i / 2] = two(scaled(r[i], s, ws.x, b.x), scaled(r[i + 1], s, ws.y, b.y));
+            o[i / 2 + 1] = two(scaled(r[i + 2], s, ws.z, b.z), scaled(r[i + 3], s, ws.w, b.w));
+        }
+        if (!in) return;
+        if (align >= 32) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 8)                  // 32 bytes: a whole sector a thread
+                asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(y + 2 * i), "r"(o[i]), "r"(o[i + 1]),
+                             "r"(o[i + 2]), "r"(o[i + 3]), "r"(o[i + 4]), "r"(o[i + 5]), "r"(o[i + 6]), "r"(o[i + 7])
+                             : "memory");
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(y + 2 * i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        }
+    } else if (n < p.N) {
+        // rows that suit no vector, or their end: a lane a channel, row by row
+#pragma unroll
+        for (int i = 0; i < 32; i += 2)
+            *reinterpret_cast<uint32_t*>(&turn[lane][i]) = two(scaled(r[i], s, scale[i], bias[i]), scaled(r[i + 1], s, scale[i + 1], bias[i + 1]));
+        __syncwarp();
+        const int64_t row0 = row - lane;
+        for (int i = 0; i < 32 && row0 + i < p.M; ++i)
+            if (n + lane < p.N) p.y[(row0 + i) * p.ldy + n + lane] = turn[i][lane];
+        __syncwarp();
+    }
+}
+
+// G tokens from c on of a warp's 32 channels (n0 ..; a lane a channel) into y: rounded sums v, turned in `turn` so
+// that a lane stores 16 bytes of a token where rows suit that, else a lane its channel.
+template <int G>
+__device__ __forceinline__ void put_tokens(const Int8GemmParams& p, const float (&v)[G], int c, int n0, bool vec, uint16_t (*turn)[40])
+{
+    const int lane = lane_id();
+    if (vec && n0 + 32 <= p.N) {
+#pragma unroll
+        for (int i = 0; i < G; ++i) turn[i][lane] = f32_to_bf16_bits(v[i]);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < G; i += 8) {
+            const int t = i + (lane >> 2), at = (lane & 3) * 8;
+            if (t < G && c + t < p.M)
+                *reinterpret_cast<uint4*>(p.y + static_cast<int64_t>(c + t) * p.ldy + n0 + at) = *reinterpret_cast<const uint4*>(&turn[t][at]);
+        }
+        __syncwarp();
+    } else if (n0 + lane < p.N) {
+#pragma unroll
+        for (int i = 0; i < G; ++i)
+            if (c + i < p.M) p.y[static_cast<int64_t>(c + i) * p.ldy + n0 + lane] = f32_to_bf16_bits(v[i]);
+    }
+}
+
 // ---------------------------------------------------------------- few tokens
 
 template <int TT>
 struct Few {
     static constexpr int STAGE = 16384 + TT * 128;
-    static constexpr int STAGES = 96 * 1024 / STAGE > 6 ? 6 : 96 * 1024 / STAGE;
+    static constexpr int STAGES = 104 * 1024 / STAGE;
     static constexpr int COLUMNS = 2 * TT < 32 ? 32 : 2 * TT;
     static constexpr size_t SMEM = 1024 + static_cast<size_t>(STAGES) * STAGE;
 };
 
 template <int TT, int SPLIT>
-__global__ void __launch_bounds__(kThreads, 2) int8_few_kernel(const __grid_constant__ Int8GemmParams p)
+__global__ void __launch_bounds__(kThreads, 2) int8_few_kernel(const __grid_constant__ Int8GemmParams p, const int vec)
 {
     using C = Few<TT>;
     constexpr int S = C::STAGES;
@@ -177,6 +243,7 @@ __global__ void __launch_bounds__(kThreads, 2) int8_few_kernel(const __grid_cons
     __shared__ uint32_t tmem_at;
     __shared__ int abort_flag;
     __shared__ float sh_scale[TT];
+    __shared__ __align__(16) uint16_t turn[4][16][40];
 
     const int warp = warp_id(), lane = lane_id();
     const uint32_t rank = SPLIT > 1 ? cluster_rank() : 0;
@@ -275,20 +342,29 @@ __global__ void __launch_bounds__(kThreads, 2) int8_few_kernel(const __grid_cons
             const float ws = in ? p.w_scale[n] : 0.0f, b = in && p.bias ? p.bias[n] : 0.0f;
             if (!mbar_wait(&acc_full[a], (tile >> 1) & 1, quit, p.status, kWaitAccFull)) break;
             tc_fence_after();
-            uint16_t* y = p.y + n;
-            for (int c = 0; c < TT && c < p.M; c += 16) {
-                uint32_t r[16];
-                tc_ld16(tmem + a * TT + c + lanes, r);
-                tc_wait_ld();
-                reg_fence16(r);
+            // the next columns are on their way while these are stored
+            uint32_t r[2][16];
+            tc_ld16(tmem + a * TT + lanes, r[0]);
+            tc_wait_ld();
+            reg_fence16(r[0]);
+#pragma unroll
+            for (int c = 0; c < TT; c += 16) {
+                if (c >= p.M) break;
+                uint32_t(&now)[16] = r[(c / 16) & 1];
+                uint32_t(&next)[16] = r[(c / 16 + 1) & 1];
+                if (c + 16 < TT) tc_ld16(tmem + a * TT + c + 16 + lanes, next);
                 if (SPLIT > 1) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) reinterpret_cast<uint32_t*>(ring)[(c + i) * 128 + ch] = r[i];
+                    for (int i = 0; i < 16; ++i) reinterpret_cast<uint32_t*>(ring)[(c + i) * 128 + ch] = now[i];
                 } else {
+                    float v[16];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (in && c + i < p.M)
-                            y[(c + i) * p.ldy] = f32_to_bf16_bits(scaled(r[i], sh_scale[c + i], ws, b));
+                    for (int i = 0; i < 16; ++i) v[i] = scaled(now[i], sh_scale[c + i], ws, b);
+                    put_tokens<16>(p, v, c, t * 128 + quad * 32, vec, turn[quad]);
+                }
+                if (c + 16 < TT) {
+                    tc_wait_ld();
+                    reg_fence16(next);
                 }
             }
             tc_fence_before();
@@ -300,19 +376,28 @@ __global__ void __launch_bounds__(kThreads, 2) int8_few_kernel(const __grid_cons
     if (SPLIT > 1) {
         cluster_sync();
         if (warp >= 2) {
+            // a share of the tokens out of every CTA's sums, G at a time with all their loads in flight
+            constexpr int G = TT == 16 ? 4 : 8;
             const int ch = (warp & 3) * 32 + lane;
             const int64_t n = static_cast<int64_t>(t0) * 128 + ch;
-            if (n < p.N) {
-                const float ws = p.w_scale[n], b = p.bias ? p.bias[n] : 0.0f;
-                for (int c = rank; c < p.M; c += SPLIT) {
-                    const uint32_t at = smem_u32(ring) + (c * 128 + ch) * 4;
-                    uint32_t sum = 0;
+            const bool in = n < p.N;
+            const float ws = in ? p.w_scale[n] : 0.0f, b = in && p.bias ? p.bias[n] : 0.0f;
+            for (int c = static_cast<int>(rank) * G; c < p.M; c += SPLIT * G) {
+                const uint32_t at = smem_u32(ring) + (c * 128 + ch) * 4;
+                uint32_t sum[G] = {};
 #pragma unroll
-                    for (int o = 0; o < SPLIT; ++o) sum += load_cluster(map_rank(at, o));
-                    p.y[c * p.ldy + n] = f32_to_bf16_bits(scaled(sum, sh_scale[c], ws, b));
+                for (int o = 0; o < SPLIT; ++o) {
+                    const uint32_t from = map_rank(at, o);
+#pragma unroll
+                    for (int i = 0; i < G; ++i) sum[i] += load_cluster(from + i * 512);
                 }
+                float v[G];
+#pragma unroll
+                for (int i = 0; i < G; ++i) v[i] = scaled(sum[i], sh_scale[c + i], ws, b);
+                put_tokens<G>(p, v, c, t0 * 128 + (warp & 3) * 32, vec, turn[warp & 3]);
             }
         }
+        __syncwarp();
         cluster_sync();                    // (the others' sums are read until here)
     } else {
         __syncthreads();
@@ -345,21 +430,24 @@ __device__ __forceinline__ void tile_of(int64_t i, int mt, int nt, int& m, int& 
     m = g * kGroup + rest - n * rows;
 }
 
-template <int NT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    int8_many_kernel(const __grid_constant__ Int8GemmParams p, const int align)
+// SPLIT > 1: a cluster of that many pairs cuts the K of one tile.
+template <int NT, int SPLIT>
+__global__ void __launch_bounds__(kManyThreads, 1) int8_many_kernel(const __grid_constant__ Int8GemmParams p, const int align)
 {
     using C = Many<NT>;
     constexpr int S = C::STAGES;
+    static_assert(SPLIT == 1 || NT * 128 * 4 <= S * C::STAGE, "the sums of a split tile lie where the ring was");
     extern __shared__ uint8_t raw[];
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
     __shared__ uint64_t full[S], empty[S], acc_full[2], acc_empty[2];
     __shared__ uint32_t tmem_at;
     __shared__ int abort_flag;
-    __shared__ uint16_t turn[4][32][34];                     // a warp's 32 x 32 outputs on their way to rows
+    __shared__ __align__(16) float sh_ws[2][NT], sh_b[2][NT];
+    __shared__ uint16_t turn[8][32][34];                     // a warp's 32 x 32 outputs on their way to rows
 
     const int warp = warp_id(), lane = lane_id();
-    const uint32_t rank = cluster_rank();
+    const uint32_t cta = cluster_rank(), rank = cta & 1, lead = cta & ~1u;       // in the pair; its first CTA
+    const int part = static_cast<int>(cta >> 1);
     if (threadIdx.x == 0) {
         for (int i = 0; i < S; ++i) {
             mbar_init(&full[i], 1);
@@ -367,7 +455,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&acc_full[i], 1);
-            mbar_init(&acc_empty[i], 8);                     // four warps of each CTA
+            mbar_init(&acc_empty[i], 16);                    // eight warps of each CTA
         }
         abort_flag = 0;
         fence_mbar_init();
@@ -383,7 +471,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
     const int mt = (p.M + 255) / 256, nt = (p.N + NT - 1) / NT, KB = (p.K + 127) / 128;
     const int64_t tiles = static_cast<int64_t>(mt) * nt;
-    const int pairs = gridDim.x / 2, pair = blockIdx.x / 2;
+    const int pairs = gridDim.x / (2 * SPLIT), pair = blockIdx.x / (2 * SPLIT);
+    const int kb0 = part * KB / SPLIT, kb1 = (part + 1) * KB / SPLIT;
 
     if (warp == 0) {
         if (lane == 0) {
@@ -395,7 +484,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 int m, n;
                 tile_of(t, mt, nt, m, n);
                 const int a_row = m * 256 + static_cast<int>(rank) * 128, w_row = n * NT + static_cast<int>(rank) * (NT / 2);
-                for (int kb = 0; kb < KB; ++kb, ++it) {
+                for (int kb = kb0; kb < kb1; ++kb, ++it) {
                     const int s = static_cast<int>(it % S);
                     const int64_t round = it / S;
                     if (round > 0 && !mbar_wait(&empty[s], (round - 1) & 1, quit, p.status, kWaitEmpty)) {
@@ -404,7 +493,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     }
                     // the pair's first CTA counts the bytes of both
                     if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * C::STAGE);
-                    const uint32_t bar = map_rank(smem_u32(&full[s]), 0);
+                    const uint32_t bar = map_rank(smem_u32(&full[s]), lead);
                     load_pair(ring + s * C::STAGE, &p.tm_a, bar, kb * 128, a_row, stay);
                     load_pair(ring + s * C::STAGE + C::A, &p.tm_w, bar, kb * 128, w_row, stay);
                 }
@@ -424,7 +513,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const int a = tile & 1;
                 if (tile >= 2 && !mbar_wait(&acc_empty[a], ((tile >> 1) - 1) & 1, quit, p.status, kWaitAccEmpty)) break;
                 tc_fence_after();
-                for (int kb = 0; kb < KB; ++kb, ++it) {
+                for (int kb = kb0; kb < kb1; ++kb, ++it) {
                     const int s = static_cast<int>(it % S);
                     if (!mbar_wait(&full[s], (it / S) & 1, quit, p.status, kWaitFull)) {
                         ok = false;
@@ -433,10 +522,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     tc_fence_after();
                     const uint64_t ad = smem_desc_sw128(base + s * C::STAGE), wd = smem_desc_sw128(base + s * C::STAGE + C::A);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) mma_i8<2>(tmem + a * NT, ad + 2 * k, wd + 2 * k, idesc, kb > 0 || k > 0);
-                    commit_pair(&empty[s]);
+                    for (int k = 0; k < 4; ++k) mma_i8<2>(tmem + a * NT, ad + 2 * k, wd + 2 * k, idesc, kb > kb0 || k > 0);
+                    commit_pair(&empty[s], lead);
                 }
-                if (ok) commit_pair(&acc_full[a]);
+                if (ok) commit_pair(&acc_full[a], lead);
             }
         }
     } else {
@@ -451,65 +540,74 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const int64_t row = static_cast<int64_t>(m) * 256 + rank * 128 + quad * 32 + lane;
             const bool in = row < p.M;
             const float s = in ? p.a_scale[row] : 0.0f;
-            uint16_t* y = p.y + row * p.ldy;
+            // the channels' scales are there before the sums (the other tile's warps still read the other buffer)
+            if (const int c = threadIdx.x - 64; c < NT) {
+                const int64_t n = static_cast<int64_t>(nn) * NT + c;
+                sh_ws[a][c] = n < p.N ? p.w_scale[n] : 0.0f;
+                sh_b[a][c] = n < p.N && p.bias ? p.bias[n] : 0.0f;
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
             if (!mbar_wait(&acc_full[a], (tile >> 1) & 1, quit, p.status, kWaitAccFull)) break;
             tc_fence_after();
-#pragma unroll 1
-            for (int c = 0; c < NT; c += 32) {
-                const int n = nn * NT + c;
-                uint32_t r[32];
-                load_columns32(tmem + a * NT + c + lanes, r);
-                tc_wait_ld();
-                settle32(r);
-                if (c + 32 >= NT) {
+            // this warp's half of the channels, the next 32 on their way while these are stored
+            const int c0 = (warp - 2) / 4 * (NT / 2);
+            uint32_t r[2][32];
+            load_columns32(tmem + a * NT + c0 + lanes, r[0]);
+            tc_wait_ld();
+            settle32(r[0]);
+#pragma unroll
+            for (int k = 0; k < NT / 64; ++k) {
+                const int c = c0 + 32 * k;
+                uint32_t(&now)[32] = r[k & 1];
+                uint32_t(&next)[32] = r[(k + 1) & 1];
+                if (k + 1 < NT / 64) {
+                    load_columns32(tmem + a * NT + c + 32 + lanes, next);
+                } else {
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) arrive_remote(map_rank(smem_u32(&acc_empty[a]), 0));
+                    if (lane == 0) arrive_remote(map_rank(smem_u32(&acc_empty[a]), lead));
                 }
-                uint32_t o[16];
-                const bool whole = n + 32 <= p.N;
-                if (whole && align >= 16) {
+                if (SPLIT > 1) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        const float4 ws = *reinterpret_cast<const float4*>(p.w_scale + n + i);
-                        const float4 b = p.bias ? *reinterpret_cast<const float4*>(p.bias + n + i) : make_float4(0, 0, 0, 0);
-                        o[i / 2] = two(scaled(r[i], s, ws.x, b.x), scaled(r[i + 1], s, ws.y, b.y));
-                        o[i / 2 + 1] = two(scaled(r[i + 2], s, ws.z, b.z), scaled(r[i + 3], s, ws.w, b.w));
-                    }
-                    if (!in) continue;
-                    if (align >= 32) {
-#pragma unroll
-                        for (int i = 0; i < 16; i += 8)      // 32 bytes: a whole sector a thread
-                            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(y + n + 2 * i), "r"(o[i]),
-                                         "r"(o[i + 1]), "r"(o[i + 2]), "r"(o[i + 3]), "r"(o[i + 4]), "r"(o[i + 5]),
-                                         "r"(o[i + 6]), "r"(o[i + 7])
-                                         : "memory");
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 16; i += 4)
-                            *reinterpret_cast<uint4*>(y + n + 2 * i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                    }
-                } else if (n < p.N) {
-                    // rows that suit no vector, or their end: a lane a channel, row by row
-                    const int col = min(n + lane, p.N - 1);
-                    const float mws = p.w_scale[col], mb = p.bias ? p.bias[col] : 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        const float ws0 = __shfl_sync(0xffffffffu, mws, i), ws1 = __shfl_sync(0xffffffffu, mws, i + 1);
-                        const float b0 = __shfl_sync(0xffffffffu, mb, i), b1 = __shfl_sync(0xffffffffu, mb, i + 1);
-                        *reinterpret_cast<uint32_t*>(&turn[quad][lane][i]) = two(scaled(r[i], s, ws0, b0), scaled(r[i + 1], s, ws1, b1));
-                    }
-                    __syncwarp();
-                    const int64_t row0 = row - lane;
-                    for (int i = 0; i < 32 && row0 + i < p.M; ++i)
-                        if (n + lane < p.N) p.y[(row0 + i) * p.ldy + n + lane] = turn[quad][i][lane];
-                    __syncwarp();
+                    for (int i = 0; i < 32; ++i) reinterpret_cast<uint32_t*>(ring)[(c + i) * 128 + quad * 32 + lane] = now[i];
+                } else {
+                    put32(p, now, nn * NT + c, row, in, s, sh_ws[a] + c, sh_b[a] + c, align, turn[warp - 2]);
+                }
+                if (k + 1 < NT / 64) {
+                    tc_wait_ld();
+                    settle32(next);
                 }
             }
         }
     }
     __syncwarp();
     cluster_sync();
+    if (SPLIT > 1) {
+        // a share of the channels out of every pair's sums
+        if (warp >= 2) {
+            int m, nn;
+            tile_of(pair, mt, nt, m, nn);
+            const int quad = warp & 3;
+            const int64_t row = static_cast<int64_t>(m) * 256 + rank * 128 + quad * 32 + lane;
+            const bool in = row < p.M;
+            const float s = in ? p.a_scale[row] : 0.0f;
+#pragma unroll 1
+            for (int k = part * (NT / 32) / SPLIT + (warp - 2) / 4; k < (part + 1) * (NT / 32) / SPLIT; k += 2) {
+                const int c = 32 * k;
+                uint32_t r[32] = {};
+                const uint32_t at = smem_u32(ring) + (c * 128 + quad * 32 + lane) * 4;
+#pragma unroll
+                for (int o = 0; o < SPLIT; ++o) {
+                    const uint32_t from = map_rank(at, 2 * o + rank);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) r[i] += load_cluster(from + i * 512);
+                }
+                put32(p, r, nn * NT + c, row, in, s, sh_ws[0] + c, sh_b[0] + c, align, turn[warp - 2]);
+            }
+        }
+        __syncwarp();
+        cluster_sync();                    // (the others' sums are read until here)
+    }
     if (warp == 1) {
         tc_fence_after();
         free_columns<2>(tmem, C::COLUMNS);
@@ -519,13 +617,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // ---------------------------------------------------------------- launch
 
 template <typename Kern, typename... Args>
-cudaError_t launch(Kern kern, int grid, int cluster, size_t smem, cudaStream_t stream, bool pdl, const Args&... args)
+cudaError_t launch(Kern kern, int grid, int threads, int cluster, size_t smem, cudaStream_t stream, bool pdl, const Args&... args)
 {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -550,11 +648,93 @@ cudaError_t launch_few(const Int8GemmParams& p, int split, int sms, cudaStream_t
 {
     const int tiles = (p.N + 127) / 128;
     constexpr size_t smem = Few<TT>::SMEM;
+    const int vec = reinterpret_cast<uintptr_t>(p.y) % 16 == 0 && p.ldy % 8 == 0;
     switch (split) {
-        case 8: return launch(int8_few_kernel<TT, 8>, tiles * 8, 8, smem, stream, pdl, p);
-        case 4: return launch(int8_few_kernel<TT, 4>, tiles * 4, 4, smem, stream, pdl, p);
-        case 2: return launch(int8_few_kernel<TT, 2>, tiles * 2, 2, smem, stream, pdl, p);
-        default: return launch(int8_few_kernel<TT, 1>, std::min(tiles, 2 * sms), 1, smem, stream, pdl, p);
+        case 8: return launch(int8_few_kernel<TT, 8>, tiles * 8, kThreads, 8, smem, stream, pdl, p, vec);
+        case 6: return launch(int8_few_kernel<TT, 6>, tiles * 6, kThreads, 6, smem, stream, pdl, p, vec);
+        case 3: return launch(int8_few_kernel<TT, 3>, tiles * 3, kThreads, 3, smem, stream, pdl, p, vec);
+        case 4: return launch(int8_few_kernel<TT, 4>, tiles * 4, kThreads, 4, smem, stream, pdl, p, vec);
+        case 2: return launch(int8_few_kernel<TT, 2>, tiles * 2, kThreads, 2, smem, stream, pdl, p, vec);
+        default: return launch(int8_few_kernel<TT, 1>, std::min(tiles, 2 * sms), kThreads, 1, smem, stream, pdl, p, vec);
+    }
+}
+
+template <int NT>
+cudaError_t launch_many(const Int8GemmParams& p, int split, int64_t tiles, int align, int sms, cudaStream_t stream, bool pdl)
+{
+    constexpr size_t smem = Many<NT>::SMEM;
+    const int n = static_cast<int>(std::min<int64_t>(tiles, split > 1 ? tiles : sms / 2));
+    switch (split) {
+        case 4: return launch(int8_many_kernel<NT, 4>, 8 * n, kManyThreads, 8, smem, stream, pdl, p, align);
+        case 3: return launch(int8_many_kernel<NT, 3>, 6 * n, kManyThreads, 6, smem, stream, pdl, p, align);
+        case 2: return launch(int8_many_kernel<NT, 2>, 4 * n, kManyThreads, 4, smem, stream, pdl, p, align);
+        default: return launch(int8_many_kernel<NT, 1>, 2 * n, kManyThreads, 2, smem, stream, pdl, p, align);
+    }
+}
+
+// Clusters of KERN that the current device holds at a time with `per_sm` CTAs an SM; 0 where that cannot be told.  (For
+// kernels with tensor memory the runtime counts one CTA an SM.  Two of the few-token kernel run: 40 clusters of six
+// take one wave, 24.5 us, 40 of eight do not, 29.4.)
+template <auto KERN>
+int resident(int cluster, int threads, size_t smem, int per_sm)
+{
+    constexpr int kDevices = 64;
+    static std::atomic<int> known[kDevices];                  // plus one
+    int dev = 0, n = 0, counted = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kDevices) return 0;
+    if ((n = known[dev].load(std::memory_order_relaxed)) > 0) return n - 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(cluster);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, KERN, &cfg) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&counted, KERN, threads, smem) != cudaSuccess || counted < 1) {
+        cudaGetLastError();
+        return 0;
+    }
+    n = n / counted * per_sm;
+    known[dev].store(n + 1, std::memory_order_relaxed);
+    return n;
+}
+
+template <int TT, int SPLIT>
+bool few_fits(int64_t tiles)
+{
+    return tiles <= resident<int8_few_kernel<TT, SPLIT>>(SPLIT, kThreads, Few<TT>::SMEM, 2);
+}
+
+// How many CTAs cut a tile's K: as many as are resident with the tiles there are, while each keeps enough blocks of 128
+// to be worth its share of the join -- two where the cut still leaves SMs idle, ten where SMs would hold two CTAs (with
+// fewer, 12000 x 2048 of one token 8.5 us uncut, 8.2 in two, 11.1 in three; 5120 x 27648 61.5 uncut, 24.8 in four,
+// 24.5 in six; 1280 x 5120 13.6 uncut, 5.4 in eight).
+template <int TT>
+int few_split(int64_t tiles, int64_t kb, int sms)
+{
+    const auto worth = [&](int s) { return kb >= (tiles * s <= sms ? 2 : 10) * s; };
+    if (kb < 8) return 1;
+    if (worth(8) && few_fits<TT, 8>(tiles)) return 8;
+    if (worth(6) && few_fits<TT, 6>(tiles)) return 6;
+    if (worth(4) && few_fits<TT, 4>(tiles)) return 4;
+    if (worth(3) && few_fits<TT, 3>(tiles)) return 3;
+    if (worth(2) && few_fits<TT, 2>(tiles)) return 2;
+    return 1;
+}
+
+template <int NT>
+bool many_fits(int64_t tiles, int split)
+{
+    switch (split) {
+        case 1: return true;
+        case 2: return tiles <= resident<int8_many_kernel<NT, 2>>(4, kManyThreads, Many<NT>::SMEM, 1);
+        case 3: return tiles <= resident<int8_many_kernel<NT, 3>>(6, kManyThreads, Many<NT>::SMEM, 1);
+        default: return tiles <= resident<int8_many_kernel<NT, 4>>(8, kManyThreads, Many<NT>::SMEM, 1);
     }
 }
 
@@ -563,19 +743,40 @@ cudaError_t launch_few(const Int8GemmParams& p, int split, int sms, cudaStream_t
 Int8Plan int8_plan(int64_t M, int64_t N, int64_t K, int sms)
 {
     Int8Plan r{};
+    const int64_t kb = (K + 127) / 128;
     r.many = M > kFewTokens;
-    if (r.many) {
-        r.nt = 256;
-        r.w_rows = r.nt / 2;
-        r.a_rows = 128;
+    if (!r.many) {
+        const int64_t tiles = (N + 127) / 128;
+        r.tt = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+        r.split = r.tt == 16   ? few_split<16>(tiles, kb, sms)
+                  : r.tt == 32 ? few_split<32>(tiles, kb, sms)
+                  : r.tt == 64 ? few_split<64>(tiles, kb, sms)
+                               : few_split<128>(tiles, kb, sms);
+        r.w_rows = 128;
+        r.a_rows = r.tt;
         return r;
     }
-    r.tt = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-    const int64_t tiles = (N + 127) / 128, kb = (K + 127) / 128;
-    r.split = 1;
-    while (r.split < 8 && tiles * r.split * 2 <= 2 * sms && kb >= 4 * r.split) r.split *= 2;
-    r.w_rows = 128;
-    r.a_rows = r.tt;
+    // The quickest by what each costs (microseconds measured on B200, 9 shapes of weights x 200 to 1024 tokens):
+    // starting and storing a tile, 0.26 or 0.31 a block of 128 of K in every wave of tiles, and a cut tile's join.
+    constexpr float kStart[2] = {5.7f, 6.7f}, kBlock[2] = {0.26f, 0.31f};
+    constexpr float kJoin[2][4] = {{0.0f, 0.9f, 1.8f, 2.0f}, {0.0f, 3.7f, 6.0f, 7.0f}};
+    const int64_t mt = (M + 255) / 256;
+    float best = 0.0f;
+    for (int wide = 1; wide >= 0; --wide)
+        for (int split = 1; split <= 4; ++split) {
+            const int nt = wide ? 256 : 128;
+            const int64_t tiles = mt * ((N + nt - 1) / nt), waves = (tiles * split + sms / 2 - 1) / (sms / 2);
+            if (split > 1 && (waves > 1 || kb < 2 * split || !(wide ? many_fits<256>(tiles, split) : many_fits<128>(tiles, split))))
+                continue;
+            const float cost = kStart[wide] + kBlock[wide] * static_cast<float>(waves * ((kb + split - 1) / split)) + kJoin[wide][split - 1];
+            if (r.nt == 0 || cost < best) {
+                best = cost;
+                r.nt = nt;
+                r.split = split;
+            }
+        }
+    r.w_rows = r.nt / 2;
+    r.a_rows = 128;
     return r;
 }
 
@@ -583,14 +784,11 @@ cudaError_t launch_int8_gemm(const Int8GemmParams& p, const Int8Plan& plan, int 
 {
     if (plan.many) {
         const int64_t mt = (p.M + 255) / 256, nt = (p.N + plan.nt - 1) / plan.nt;
-        const int pairs = static_cast<int>(std::min<int64_t>(mt * nt, sms / 2));
-        // the widest store that each row's outputs suit, where 16-byte loads suit the channels' scales
+        // the widest store that each row's outputs suit
         const auto fits = [&](uintptr_t a) { return reinterpret_cast<uintptr_t>(p.y) % a == 0 && 2 * p.ldy % a == 0; };
-        const bool loads = reinterpret_cast<uintptr_t>(p.w_scale) % 16 == 0 && reinterpret_cast<uintptr_t>(p.bias) % 16 == 0;
-        const int align = !loads ? 2 : fits(32) ? 32 : fits(16) ? 16 : 2;
-        // (the kernel names its cluster itself)
-        return plan.nt == 256 ? launch(int8_many_kernel<256>, 2 * pairs, 1, Many<256>::SMEM, stream, pdl, p, align)
-                              : launch(int8_many_kernel<128>, 2 * pairs, 1, Many<128>::SMEM, stream, pdl, p, align);
+        const int align = fits(32) ? 32 : fits(16) ? 16 : 2;
+        if (plan.nt == 256) return launch_many<256>(p, plan.split, mt * nt, align, sms, stream, pdl);
+        return launch_many<128>(p, plan.split, mt * nt, align, sms, stream, pdl);
     }
     switch (plan.tt) {
         case 16: return launch_few<16>(p, plan.split, sms, stream, pdl);
