@@ -370,10 +370,23 @@ PyObject* pages_plan(PyObject*, PyObject* const* a, Py_ssize_t n)
         segs = tensor(a[7]);
         if (!dense(cu, at::kInt, dev, 1) || !dense(segs, at::kInt, dev, 2) || cu->size(0) != B + 1 || segs->size(1) != 4) return later();
     }
-    const at::Tensor out[5] = {make({B, st->columns}, at::kInt, dev), make({B}, at::kInt, dev), make({B + 1}, at::kInt, dev),
-                               make({tokens}, at::kInt, dev), make({axes, tokens}, at::kInt, dev)};
+    // the outputs are parts of one allocation, each from a multiple of 16 bytes on
+    const int64_t wide[5] = {B * st->columns, B, B + 1, tokens, axes * tokens};
+    int64_t at_[5], total = 0;
+    for (int i = 0; i < 5; ++i) {
+        at_[i] = total;
+        total += (wide[i] + 3) / 4 * 4;
+    }
+    const at::Tensor whole = make({total}, at::kInt, dev);
+    const auto part = [&](int i, at::IntArrayRef size) {
+        auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), whole.dtype());
+        impl->set_storage_offset(at_[i]);
+        impl->set_sizes_contiguous(size);
+        return at::Tensor(std::move(impl));
+    };
+    const at::Tensor out[5] = {part(0, {B, st->columns}), part(1, {B}), part(2, {B + 1}), part(3, {tokens}), part(4, {axes, tokens})};
     int32_t* p[5];
-    for (int i = 0; i < 5; ++i) p[i] = static_cast<int32_t*>(out[i].data_ptr());
+    for (int i = 0; i < 5; ++i) p[i] = static_cast<int32_t*>(whole.data_ptr()) + at_[i];
     const int rc = g.pages_plan(st, ints(rows), ints(counts), B, tokens, static_cast<int32_t>(axes), cu ? ints(cu) : nullptr,
                                 segs ? ints(segs) : nullptr, segs ? segs->size(0) : 0, p[0], p[1], p[2], p[3], p[4], stream(dev));
     if (rc != W4A8_OK) return later();

@@ -15,8 +15,8 @@
 // `start` of its sequence begins at that token's text position o and counts (o + r / (h w), o + r / w % h, o + r % w);
 // what follows goes on at o + max(t, h, w).
 //
-// One launch.  Every block finds all sums itself (up to 2048 sequences: eight a thread, a scan over the block), so no block
-// waits for another, and does its share of table rows and tokens.  The lengths and the stack's height, which all blocks
+// One launch.  Every block finds all sums itself (up to 2048 sequences: eight or two a thread, a scan over the block), so no
+// block waits for another, and does its share of table rows and tokens.  The lengths and the stack's height, which all blocks
 // read first, are set by the block that finishes last.  A step that cannot be (a row twice or outside, too few pages, ...)
 // changes nothing: its tables say "no page" and "no tokens", and the status word says why.
 #include <algorithm>
@@ -28,9 +28,7 @@ namespace w4a8 {
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
-constexpr int kPer = kMaxPlanBatch / kThreads;
+constexpr int kSmall = 256, kLarge = 1024;                     // threads of a block
 
 struct Sums {
     int64_t tokens, pages;
@@ -50,51 +48,56 @@ struct Step {
     int row[kMaxPlanBatch];
     int len[kMaxPlanBatch];
     uint32_t seen[kMaxPlanRows / 32];
-    Sums warp_sums[kWarps];
+    Sums warp_sums[kLarge / 32];
     int bad, last;
 };
 
 __device__ __forceinline__ int pages_of(int64_t len, int log2) { return static_cast<int>((len + (int64_t(1) << log2) - 1) >> log2); }
 
 // Fills `st`; 0, or why the step cannot be.  SHRINK: counts are the lengths to keep (null: 0), pages those given back.
-template <bool SHRINK>
+template <int T, bool SHRINK>
 __device__ int gather(const PagesParams& p, Step& st, int& height)
 {
-    const int tid = threadIdx.x, B = p.batch, per = (B + kThreads - 1) / kThreads;
-    for (int i = tid; i < (p.sequences + 31) / 32; i += kThreads) st.seen[i] = 0;
+    constexpr int PER = kMaxPlanBatch / T, WARPS = T / 32;
+    const int tid = threadIdx.x, B = p.batch, per = (B + T - 1) / T;
+    int row[PER], count[PER], len[PER], need[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int i = tid * per + j;
+        const bool on = j < per && i < B;
+        row[j] = on ? p.rows[i] : -1;
+        count[j] = on && p.counts ? p.counts[i] : 0;
+    }
+    for (int i = tid; i < (p.sequences + 31) / 32; i += T) st.seen[i] = 0;
     if (tid == 0) st.bad = 0;
-    __syncthreads();
     height = *p.free_count;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) len[j] = row[j] >= 0 && row[j] < p.sequences ? p.lens[row[j]] : 0;
+    __syncthreads();
     int bad = height < 0 || height > p.pages ? kPlanState : 0;
     Sums mine{0, 0};
-    int count[kPer], need[kPer];
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-        const int i = tid * per + j;
-        count[j] = need[j] = 0;
+    for (int j = 0; j < PER; ++j) {
+        const int i = tid * per + j, n = count[j];
+        need[j] = 0;
         if (j >= per || i >= B) continue;
-        const int row = p.rows[i], n = SHRINK ? (p.counts ? p.counts[i] : 0) : p.counts[i];
-        int len = 0;
-        if (row < 0 || row >= p.sequences || (atomicOr(&st.seen[row >> 5], 1u << (row & 31)) >> (row & 31) & 1u)) {
+        const int held = pages_of(len[j], p.page_log2);
+        if (row[j] < 0 || row[j] >= p.sequences || (atomicOr(&st.seen[row[j] >> 5], 1u << (row[j] & 31)) >> (row[j] & 31) & 1u)) {
             bad |= kPlanRow;
+        } else if (len[j] < 0 || held > p.columns) {
+            bad |= kPlanState;
+        } else if (SHRINK) {
+            if (n < 0 || n > len[j]) bad |= kPlanCount;
+            else need[j] = held - pages_of(n, p.page_log2);
+        } else if (n < 0 || n > p.tokens) {
+            bad |= n < 0 ? kPlanCount : kPlanTokens;
+        } else if (const int all = pages_of(static_cast<int64_t>(len[j]) + n, p.page_log2); all > p.columns) {
+            bad |= kPlanColumns;
         } else {
-            len = p.lens[row];
-            if (len < 0 || pages_of(len, p.page_log2) > p.columns) {
-                bad |= kPlanState;
-            } else if (SHRINK) {
-                if (n < 0 || n > len) bad |= kPlanCount;
-                else need[j] = pages_of(len, p.page_log2) - pages_of(n, p.page_log2);
-            } else if (n < 0 || n > p.tokens) {
-                bad |= n < 0 ? kPlanCount : kPlanTokens;
-            } else if (pages_of(static_cast<int64_t>(len) + n, p.page_log2) > p.columns) {
-                bad |= kPlanColumns;
-            } else {
-                need[j] = pages_of(static_cast<int64_t>(len) + n, p.page_log2) - pages_of(len, p.page_log2);
-            }
+            need[j] = all - held;
         }
-        count[j] = n;
-        st.row[i] = row;
-        st.len[i] = len;
+        st.row[i] = row[j];
+        st.len[i] = len[j];
         mine = add(mine, {SHRINK ? 0 : n, need[j]});
     }
     Sums x = mine;
@@ -108,7 +111,7 @@ __device__ int gather(const PagesParams& p, Step& st, int& height)
     __syncthreads();
     Sums at{x.tokens - mine.tokens, x.pages - mine.pages}, total{0, 0};
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < WARPS; ++w) {
         if (w < static_cast<int>(warp_id())) at = add(at, st.warp_sums[w]);
         total = add(total, st.warp_sums[w]);
     }
@@ -118,7 +121,7 @@ __device__ int gather(const PagesParams& p, Step& st, int& height)
     if (SHRINK ? height + total.pages > p.pages : total.pages > height) bad |= SHRINK ? kPlanState : kPlanPages;
     if (bad) return bad;                                      // (sums past here fit 32 bits)
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
+    for (int j = 0; j < PER; ++j) {
         const int i = tid * per + j;
         if (j >= per || i >= B) continue;
         st.cu[i] = static_cast<int>(SHRINK ? count[j] : at.tokens);      // SHRINK: the length to keep
@@ -167,22 +170,25 @@ __device__ __forceinline__ void place(const PagesParams& p, int g0, int g1, int 
     out[0] = out[1] = out[2] = pos + shift;
 }
 
-__global__ void __launch_bounds__(kThreads) pages_plan_kernel(const PagesParams p)
+template <int T>
+__global__ void __launch_bounds__(T) pages_plan_kernel(const PagesParams p)
 {
     __shared__ Step st;
     pdl_wait();
     int height;
-    const int bad = gather<false>(p, st, height), B = p.batch;
-    const int tid = blockIdx.x * kThreads + threadIdx.x, all = gridDim.x * kThreads, S = 1 << p.page_log2;
+    const int bad = gather<T, false>(p, st, height), B = p.batch;
+    const int tid = blockIdx.x * T + threadIdx.x, all = gridDim.x * T, S = 1 << p.page_log2;
 
     for (int i = tid; i <= B; i += all) {
         p.cu[i] = bad ? 0 : st.cu[i];
         if (i < B) p.kv_lens[i] = bad ? 0 : st.len[i] + st.cu[i + 1] - st.cu[i];
     }
-    // Table rows, 128 columns a warp at a time: the pages held, the new ones, none.
-    const int chunks = (p.columns + 127) / 128;
+    // Table rows, 512 columns a warp at a time: the pages held, the new ones, none.  Four columns an access where
+    // rows suit that.
+    const bool vec = p.columns % 4 == 0 && (reinterpret_cast<uintptr_t>(p.table) | reinterpret_cast<uintptr_t>(p.page_table)) % 16 == 0;
+    const int span = vec ? 512 : 128, chunks = (p.columns + span - 1) / span;
     for (int64_t c = tid >> 5; c < static_cast<int64_t>(B) * chunks; c += all >> 5) {
-        const int i = static_cast<int>(c / chunks), c0 = static_cast<int>(c - static_cast<int64_t>(i) * chunks) * 128;
+        const int i = static_cast<int>(c / chunks), c0 = static_cast<int>(c - static_cast<int64_t>(i) * chunks) * span;
         int before = 0, after = 0, row = 0, taken = 0;
         if (!bad) {
             row = st.row[i];
@@ -191,18 +197,40 @@ __global__ void __launch_bounds__(kThreads) pages_plan_kernel(const PagesParams 
             after = before + st.pages[i + 1] - taken;
         }
         int32_t* held = p.table + static_cast<int64_t>(row) * p.columns;
+        int32_t* out = p.page_table + static_cast<int64_t>(i) * p.columns;
+        const auto fresh = [&](int col) {                     // a new page, or none
+            if (col >= after) return -1;
+            const int id = p.free[height - 1 - (taken + col - before)];
+            held[col] = id;
+            return id;
+        };
+        if (vec) {
+            int4 v[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int col = c0 + k * 32 + lane_id();
-            if (col >= p.columns) break;
-            int id = -1;
-            if (col < before) {
-                id = held[col];
-            } else if (col < after) {
-                id = p.free[height - 1 - (taken + col - before)];
-                held[col] = id;
+            for (int k = 0; k < 4; ++k) {
+                const int col = c0 + k * 128 + static_cast<int>(lane_id()) * 4;
+                v[k] = make_int4(-1, -1, -1, -1);
+                if (col < before) v[k] = *reinterpret_cast<const int4*>(held + col);
             }
-            p.page_table[static_cast<int64_t>(i) * p.columns + col] = id;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int col = c0 + k * 128 + static_cast<int>(lane_id()) * 4;
+                if (col >= p.columns) break;
+                if (col + 4 > before) {                       // (what a row holds past its pages is no page)
+                    v[k].x = col < before ? v[k].x : fresh(col);
+                    v[k].y = col + 1 < before ? v[k].y : fresh(col + 1);
+                    v[k].z = col + 2 < before ? v[k].z : fresh(col + 2);
+                    v[k].w = fresh(col + 3);
+                }
+                *reinterpret_cast<int4*>(out + col) = v[k];
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int col = c0 + k * 32 + lane_id();
+                if (col >= p.columns) break;
+                out[col] = col < before ? held[col] : fresh(col);
+            }
         }
     }
     if (p.slots || p.positions) {
@@ -241,17 +269,18 @@ __global__ void __launch_bounds__(kThreads) pages_plan_kernel(const PagesParams 
         if (threadIdx.x == 0) atomicCAS(p.status, 0, bad);
         return;
     }
-    for (int i = threadIdx.x; i < B; i += kThreads) p.lens[st.row[i]] = st.len[i] + st.cu[i + 1] - st.cu[i];
+    for (int i = threadIdx.x; i < B; i += T) p.lens[st.row[i]] = st.len[i] + st.cu[i + 1] - st.cu[i];
     if (threadIdx.x == 0) *p.free_count = height - st.pages[B];
 }
 
-__global__ void __launch_bounds__(kThreads) pages_shrink_kernel(const PagesParams p)
+template <int T>
+__global__ void __launch_bounds__(T) pages_shrink_kernel(const PagesParams p)
 {
     __shared__ Step st;
     pdl_wait();
     int height;
-    const int bad = gather<true>(p, st, height), B = p.batch;
-    const int tid = blockIdx.x * kThreads + threadIdx.x, all = gridDim.x * kThreads;
+    const int bad = gather<T, true>(p, st, height), B = p.batch;
+    const int tid = blockIdx.x * T + threadIdx.x, all = gridDim.x * T;
     if (!bad)
         for (int i = tid >> 5; i < B; i += all >> 5) {
             const int held = pages_of(st.len[i], p.page_log2), n = st.pages[i + 1] - st.pages[i];
@@ -267,34 +296,40 @@ __global__ void __launch_bounds__(kThreads) pages_shrink_kernel(const PagesParam
         if (threadIdx.x == 0) atomicCAS(p.status, 0, bad);
         return;
     }
-    for (int i = threadIdx.x; i < B; i += kThreads) p.lens[st.row[i]] = st.cu[i];
+    for (int i = threadIdx.x; i < B; i += T) p.lens[st.row[i]] = st.cu[i];
     if (threadIdx.x == 0) *p.free_count = height + st.pages[B];
 }
 
-cudaError_t launch(void (*kern)(PagesParams), const PagesParams& p, int64_t work, cudaStream_t stream)
+// Blocks of 1024 threads for large batches, whose sums take a block of 256 several rounds (2048 sequences of 1024
+// columns: plan 20 us by 256, 9.5 by 1024), of 256 for the others (256 of 512: 5.4 and 7.8), as many as there is work for.
+template <typename Kern>
+cudaError_t launch(Kern small, Kern large, const PagesParams& p, int64_t work, cudaStream_t stream)
 {
+    const bool many = p.batch > 2 * kSmall;
+    const int threads = many ? kLarge : kSmall;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(148, work / (4 * kThreads)))));
-    cfg.blockDim = dim3(kThreads);
+    cfg.gridDim = dim3(static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(148, work / threads))));
+    cfg.blockDim = dim3(threads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kern, p);
+    return cudaLaunchKernelEx(&cfg, many ? large : small, p);
 }
 
 }  // namespace
 
 cudaError_t launch_pages_plan(const PagesParams& p, cudaStream_t stream)
 {
-    return launch(pages_plan_kernel, p, static_cast<int64_t>(p.batch) * p.columns + 4 * p.tokens, stream);
+    return launch(pages_plan_kernel<kSmall>, pages_plan_kernel<kLarge>, p, static_cast<int64_t>(p.batch) * p.columns / 4 + 2 * p.tokens,
+                  stream);
 }
 
 cudaError_t launch_pages_shrink(const PagesParams& p, cudaStream_t stream)
 {
-    return launch(pages_shrink_kernel, p, static_cast<int64_t>(p.batch) * 32, stream);
+    return launch(pages_shrink_kernel<kSmall>, pages_shrink_kernel<kLarge>, p, static_cast<int64_t>(p.batch) * 16, stream);
 }
 
 }  // namespace w4a8
