@@ -26,9 +26,11 @@ namespace {
 
 constexpr int kMaxTokThreads = 1024;
 
+// WHOLE: rows are 16-byte aligned and K is a multiple of 8.
+template <bool WHOLE>
 __device__ __forceinline__ void load8(const uint16_t* row, int pos, int K, bool vec, float (&v)[8])
 {
-    if (vec && pos + 8 <= K) {
+    if (WHOLE || (vec && pos + 8 <= K)) {
         unpack8_bf16(*reinterpret_cast<const uint4*>(row + pos), v);
     } else {
 #pragma unroll
@@ -36,9 +38,10 @@ __device__ __forceinline__ void load8(const uint16_t* row, int pos, int K, bool 
     }
 }
 
+template <bool WHOLE>
 __device__ __forceinline__ void store8(uint16_t* row, int pos, int K, bool vec, const float (&v)[8])
 {
-    if (vec && pos + 8 <= K) {
+    if (WHOLE || (vec && pos + 8 <= K)) {
         uint32_t w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -60,22 +63,37 @@ __device__ __forceinline__ void load_weight8(const TokenQuantParams& p, int pos,
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i] = pos + i < p.K ? wf[pos + i] : 0.0f;
     } else {
-        load8(static_cast<const uint16_t*>(p.weight), pos, p.K, p.vec_w, w);
+        load8<false>(static_cast<const uint16_t*>(p.weight), pos, p.K, p.vec_w, w);
     }
 }
 
-// e^-g / (1 + ...) by the base-2 exponential of the hardware: -g log2(e) as a rounded product and what the rounding
-// left, 2^-21 of the result.  Gates below -87 give 0 (their product is less than 10^-35 of up).
-__device__ __forceinline__ float silu_up(float g, float u)
+// silu(g) u = g / (1 + e^-g) u of two elements.  The exponential is the hardware's base-2 one, of -g log2(e) as a
+// rounded product and what the rounding left: within 2^-21 of the result.  Past 88 the exponent stays: 1 + e^-88 is 1, and
+// the reciprocal of 1 + e^88, below fp32's normal numbers, is 0.
+__device__ __forceinline__ void silu_up2(float g0, float g1, float u0, float u1, float& y0, float& y1)
 {
     constexpr float kL = 1.44269502162933349609375f, kLow = 1.925963033500011e-08f;     // log2(e) = kL + kLow
-    const float c = fminf(fmaxf(g, -87.0f), 87.0f), t = __fmul_rn(c, -kL);
-    const float low = fmaf(c, -kLow, fmaf(c, -kL, -t));
-    float e, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-    e = fmaf(e, low * 0.693147180559945f, e);
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-    return g * (g < -87.0f ? 0.0f : r) * u;
+    const uint64_t c = pair2(fminf(fmaxf(g0, -88.0f), 88.0f), fminf(fmaxf(g1, -88.0f), 88.0f));
+    const uint64_t t = f2_mul(c, pair2(-kL, -kL)), minus_t = f2_mul(c, pair2(kL, kL));
+    const uint64_t low = f2_fma(c, pair2(-kLow, -kLow), f2_fma(c, pair2(-kL, -kL), minus_t));
+    float t0, t1, e0, e1, r0, r1;
+    unpair2(t, t0, t1);
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(t0));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(t1));
+    const uint64_t e = pair2(e0, e1);
+    constexpr float kLn2 = 0.693147180559945f;
+    unpair2(f2_add(f2_fma(e, f2_mul(low, pair2(kLn2, kLn2)), e), pair2(1.0f, 1.0f)), e0, e1);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r0) : "f"(e0));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r1) : "f"(e1));
+    unpair2(f2_mul(f2_mul(pair2(g0, g1), pair2(r0, r1)), pair2(u0, u1)), y0, y1);
+}
+
+// The larger of the magnitudes in m and of two bf16 values, each half its own; a NaN wins.
+__device__ __forceinline__ uint32_t max_abs2(uint32_t m, uint32_t w)
+{
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(m), "r"(w & 0x7FFF7FFFu));
+    return r;
 }
 
 __device__ __forceinline__ uint4 pack8(const float (&v)[8])
@@ -89,9 +107,10 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8])
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+template <bool WHOLE>
 __device__ __forceinline__ uint4 load8_raw(const uint16_t* row, int pos, int K, bool vec)
 {
-    if (vec && pos + 8 <= K) return *reinterpret_cast<const uint4*>(row + pos);
+    if (WHOLE || (vec && pos + 8 <= K)) return *reinterpret_cast<const uint4*>(row + pos);
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -118,26 +137,26 @@ struct Held<kTokNorm> {
 };
 
 // 8 elements of h; behind a norm, of x + residual.
-template <int SRC>
+template <int SRC, bool WHOLE>
 __device__ __forceinline__ void row8(const TokenQuantParams& p, const uint16_t* x, const uint16_t* r, int pos, Held<SRC>& h)
 {
     if constexpr (SRC == kTokNorm) {
-        load8(x, pos, p.K, p.vec_x, h.v);
+        load8<WHOLE>(x, pos, p.K, p.vec_x, h.v);
         if (r) {
             float u[8];
-            load8(r, pos, p.K, p.vec_r, u);
+            load8<WHOLE>(r, pos, p.K, p.vec_r, u);
 #pragma unroll
             for (int i = 0; i < 8; ++i) h.v[i] = __fadd_rn(h.v[i], u[i]);
         }
     } else {
-        h.v = load8_raw(x, pos, p.K, p.vec_x);
+        h.v = load8_raw<WHOLE>(x, pos, p.K, p.vec_x);
         if (SRC == kTokSwiglu) {
             float g[8], u[8];
-            const uint4 w = load8_raw(x + p.K, pos, p.K, p.vec_x && p.K % 8 == 0);
+            const uint4 w = load8_raw<WHOLE>(x + p.K, pos, p.K, p.vec_x && p.K % 8 == 0);
             unpack8_bf16(h.v, g);
             unpack8_bf16(w, u);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) g[i] = silu_up(g[i], u[i]);
+            for (int i = 0; i < 8; i += 2) silu_up2(g[i], g[i + 1], u[i], u[i + 1], g[i], g[i + 1]);
             h.v = pack8(g);
         }
     }
@@ -156,12 +175,13 @@ __device__ __forceinline__ uint32_t codes4_div(const float* x, float s)
     return w;
 }
 
+template <bool WHOLE>
 __device__ __forceinline__ void emit8(const TokenQuantParams& p, int8_t* q, int pos, const float (&v)[8], float s, float rcp,
                                       bool fast)
 {
     // (|h / s| < 127.5: s is the rounded quotient of the row's maximum and 127)
     const uint32_t lo = fast ? codes4(v, s, rcp) : codes4_div(v, s), hi = fast ? codes4(v + 4, s, rcp) : codes4_div(v + 4, s);
-    if (p.vec_q && pos + 8 <= p.K) {
+    if (WHOLE || (p.vec_q && pos + 8 <= p.K)) {
         *reinterpret_cast<uint2*>(q + pos) = make_uint2(lo, hi);
     } else {
 #pragma unroll
@@ -191,7 +211,7 @@ __device__ __forceinline__ uint32_t peer_word(const uint32_t* p, uint32_t rank)
 }
 
 // VPT vectors a thread in registers (0: the row is read twice), a row over CL blocks.
-template <int SRC, int VPT, int CL>
+template <int SRC, int VPT, int CL, bool WHOLE>
 __global__ void __launch_bounds__(kMaxTokThreads) token_quant_kernel(const TokenQuantParams p)
 {
     __shared__ float red_sum[kMaxTokThreads / 32];
@@ -212,26 +232,25 @@ __global__ void __launch_bounds__(kMaxTokThreads) token_quant_kernel(const Token
     const auto at = [&](int j) { return ((j * CL + rank) * T + tid) * 8; };
     Held<SRC> h[HOLD];
     float ss = 0.0f, big = 0.0f;
+    uint32_t big2 = 0;
 #pragma unroll
     for (int j = 0; j < vecs; ++j)
-        if (VPT && at(j) < p.K) row8<SRC>(p, x, r, at(j), h[j]);
+        if (VPT && at(j) < p.K) row8<SRC, WHOLE>(p, x, r, at(j), h[j]);
 #pragma unroll
     for (int j = 0; j < vecs; ++j) {
         const int pos = at(j);
         if (pos >= p.K) continue;
         Held<SRC>& e = h[VPT ? j : 0];
-        if (!VPT) row8<SRC>(p, x, r, pos, e);
-        float v[8];
-        e.get(v);
-        if (SRC == kTokNorm) {
-            if (p.res_out) store8(p.res_out + row * p.ldro, pos, p.K, p.vec_ro, v);
+        if (!VPT) row8<SRC, WHOLE>(p, x, r, pos, e);
+        if constexpr (SRC == kTokNorm) {
+            if (p.res_out) store8<WHOLE>(p.res_out + row * p.ldro, pos, p.K, p.vec_ro, e.v);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
+            for (int i = 0; i < 8; ++i) ss = fmaf(e.v[i], e.v[i], ss);
         } else {
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) big = max_abs_nan(big, v[i], v[i + 1]);
+            big2 = max_abs2(max_abs2(max_abs2(max_abs2(big2, e.v.x), e.v.y), e.v.z), e.v.w);
         }
     }
+    if (SRC != kTokNorm) big = max_abs_nan(0.0f, __uint_as_float(big2 << 16), __uint_as_float(big2 & 0xFFFF0000u));
     if constexpr (SRC == kTokNorm) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
@@ -280,10 +299,10 @@ __global__ void __launch_bounds__(kMaxTokThreads) token_quant_kernel(const Token
         const int pos = at(j);
         if (pos >= p.K) continue;
         Held<SRC>& e = h[VPT ? j : 0];
-        if (!VPT) row8<SRC>(p, x, r, pos, e);
+        if (!VPT) row8<SRC, WHOLE>(p, x, r, pos, e);
         float v[8];
         e.get(v);
-        emit8(p, q, pos, v, s, rcp, fast);
+        emit8<WHOLE>(p, q, pos, v, s, rcp, fast);
     }
     if (CL > 1) cluster_sync();                               // (the others read this block's words until here)
 }
@@ -291,6 +310,7 @@ __global__ void __launch_bounds__(kMaxTokThreads) token_quant_kernel(const Token
 template <int SRC, int VPT, int CL = 1>
 cudaError_t launch(const TokenQuantParams& p, int threads, cudaStream_t stream)
 {
+    const bool whole = p.K % 8 == 0 && p.vec_x && p.vec_q && (SRC != kTokNorm || ((!p.res || p.vec_r) && (!p.res_out || p.vec_ro)));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(p.M) * CL);
     cfg.blockDim = dim3(threads);
@@ -303,7 +323,8 @@ cudaError_t launch(const TokenQuantParams& p, int threads, cudaStream_t stream)
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = CL > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, token_quant_kernel<SRC, VPT, CL>, p);
+    return whole ? cudaLaunchKernelEx(&cfg, token_quant_kernel<SRC, VPT, CL, true>, p)
+                 : cudaLaunchKernelEx(&cfg, token_quant_kernel<SRC, VPT, CL, false>, p);
 }
 
 constexpr int kFewRows = 64;               // rows that a cluster each is no loss for
