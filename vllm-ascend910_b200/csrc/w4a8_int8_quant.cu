@@ -25,6 +25,8 @@ namespace w4a8 {
 namespace {
 
 constexpr int kMaxTokThreads = 1024;
+constexpr int kMaxRowThreads = 512;
+constexpr int kRowBytes = 112 * 1024;      // of a row in shared memory: two blocks an SM at least
 
 // WHOLE: rows are 16-byte aligned and K is a multiple of 8.
 template <bool WHOLE>
@@ -307,10 +309,121 @@ __global__ void __launch_bounds__(kMaxTokThreads) token_quant_kernel(const Token
     if (CL > 1) cluster_sync();                               // (the others read this block's words until here)
 }
 
+// Many rows that suit vectors: the row waits for its scale in shared memory (bf16; fp32 behind a norm), which leaves room
+// for 48 warps an SM where registers held 28.
+template <int SRC>
+__global__ void __launch_bounds__(kMaxRowThreads, 1536 / kMaxRowThreads) token_quant_rows_kernel(const TokenQuantParams p)
+{
+    extern __shared__ __align__(16) uint8_t staged[];
+    __shared__ float red_sum[kMaxRowThreads / 32];
+    __shared__ uint32_t red_max[kMaxRowThreads / 32];
+    const int tid = threadIdx.x, T = blockDim.x, nw = T >> 5, nvec = p.K / 8;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int64_t row = blockIdx.x;
+    const uint16_t* x = p.x + row * p.ldx;
+    const uint16_t* r = SRC == kTokNorm && p.res ? p.res + row * p.ldr : nullptr;
+    Held<SRC>* hold = reinterpret_cast<Held<SRC>*>(staged);
+    float big = 0.0f;
+    if constexpr (SRC == kTokNorm) {
+        // (halves of the 32 bytes a vector apart, so that a warp's accesses are to 16 bytes next to each other)
+        float4 *lo = reinterpret_cast<float4*>(staged), *hi = lo + nvec;
+        float ss = 0.0f;
+#pragma unroll 2
+        for (int v = tid; v < nvec; v += T) {
+            Held<SRC> h;
+            row8<SRC, true>(p, x, r, 8 * v, h);
+            if (p.res_out) store8<true>(p.res_out + row * p.ldro, 8 * v, p.K, true, h.v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss = fmaf(h.v[i], h.v[i], ss);
+            lo[v] = make_float4(h.v[0], h.v[1], h.v[2], h.v[3]);
+            hi[v] = make_float4(h.v[4], h.v[5], h.v[6], h.v[7]);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (lane_id() == 0) red_sum[warp_id()] = ss;
+        __syncthreads();
+        ss = static_cast<int>(lane_id()) < nw ? red_sum[lane_id()] : 0.0f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float n = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(ss, static_cast<float>(p.K)) + p.eps));
+#pragma unroll 2
+        for (int v = tid; v < nvec; v += T) {
+            float w[8], h[8];
+            load_weight8(p, 8 * v, w);
+            *reinterpret_cast<float4*>(h) = lo[v];
+            *reinterpret_cast<float4*>(h + 4) = hi[v];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h[i] = __fmul_rn(__fmul_rn(h[i], n), w[i]);
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) big = max_abs_nan(big, h[i], h[i + 1]);
+            lo[v] = make_float4(h[0], h[1], h[2], h[3]);
+            hi[v] = make_float4(h[4], h[5], h[6], h[7]);
+        }
+    } else {
+        uint32_t big2 = 0;
+#pragma unroll 2
+        for (int v = tid; v < nvec; v += T) {
+            Held<SRC> h;
+            row8<SRC, true>(p, x, r, 8 * v, h);
+            big2 = max_abs2(max_abs2(max_abs2(max_abs2(big2, h.v.x), h.v.y), h.v.z), h.v.w);
+            hold[v] = h;
+        }
+        big = max_abs_nan(0.0f, __uint_as_float(big2 << 16), __uint_as_float(big2 & 0xFFFF0000u));
+    }
+    uint32_t amax = __reduce_max_sync(0xffffffffu, __float_as_uint(big));     // (as bits, a NaN is the largest)
+    if (lane_id() == 0) red_max[warp_id()] = amax;
+    __syncthreads();
+    amax = __reduce_max_sync(0xffffffffu, static_cast<int>(lane_id()) < nw ? red_max[lane_id()] : 0u);
+    const bool finite = amax < 0x7F800000u;
+    const float s = finite ? __fdiv_rn(__uint_as_float(amax), 127.0f) : __uint_as_float(0x7FC00000u);
+    if (tid == 0) p.scale[row] = s;
+    const bool fast = finite && s >= 1.1754943508222875e-38f;
+    const float rcp = fast ? __frcp_rn(s) : 0.0f;
+    int8_t* q = p.q + row * p.ldq;
+#pragma unroll 2
+    for (int v = tid; v < nvec; v += T) {                     // (a thread's own vectors: no barrier since)
+        float h[8];
+        if constexpr (SRC == kTokNorm) {
+            const float4 *lo = reinterpret_cast<const float4*>(staged), *hi = lo + nvec;
+            *reinterpret_cast<float4*>(h) = lo[v];
+            *reinterpret_cast<float4*>(h + 4) = hi[v];
+        } else {
+            hold[v].get(h);
+        }
+        emit8<true>(p, q, 8 * v, h, s, rcp, fast);
+    }
+}
+
+bool whole_rows(const TokenQuantParams& p, int src)
+{
+    return p.K % 8 == 0 && p.vec_x && p.vec_q && (src != kTokNorm || ((!p.res || p.vec_r) && (!p.res_out || p.vec_ro)));
+}
+
+template <int SRC>
+cudaError_t launch_rows(const TokenQuantParams& p, cudaStream_t stream)
+{
+    const int threads = p.K <= 2048 * 8 ? 256 : 512;
+    const size_t smem = static_cast<size_t>(p.K) * (SRC == kTokNorm ? 4 : 2);
+    const cudaError_t e = cudaFuncSetAttribute(token_quant_rows_kernel<SRC>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowBytes);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(p.M));
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, token_quant_rows_kernel<SRC>, p);
+}
+
 template <int SRC, int VPT, int CL = 1>
 cudaError_t launch(const TokenQuantParams& p, int threads, cudaStream_t stream)
 {
-    const bool whole = p.K % 8 == 0 && p.vec_x && p.vec_q && (SRC != kTokNorm || ((!p.res || p.vec_r) && (!p.res_out || p.vec_ro)));
+    const bool whole = whole_rows(p, SRC);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(p.M) * CL);
     cfg.blockDim = dim3(threads);
@@ -336,6 +449,10 @@ cudaError_t launch_source(const TokenQuantParams& p, cudaStream_t stream)
     const int nvec = (p.K + 7) / 8;
     const auto threads = [&](int vpt) { return ((nvec + vpt - 1) / vpt + 31) / 32 * 32; };
     if (nvec > 1024 && nvec <= 8 * 1024 && p.M <= kFewRows) return launch<SRC, 1, 8>(p, threads(8), stream);
+    // Many wide rows through shared memory (2,048 of 27,648: plain 43 us, SwiGLU 60, norm 124; in registers 49, 79 and 128),
+    // narrower ones in registers (2,048 of 5120: plain 7.5 us, through shared memory 8.7).
+    if (p.M > kManyRows && whole_rows(p, SRC) && static_cast<int64_t>(p.K) * (SRC == kTokNorm ? 4 : 2) <= kRowBytes && nvec > 1024)
+        return launch_rows<SRC>(p, stream);
     // Many rows: more vectors a thread keep more bytes in flight.
     if (p.M > kManyRows) {
         if (SRC != kTokNorm && threads(8) >= 256 && threads(8) <= kMaxTokThreads) return launch<SRC, 8>(p, threads(8), stream);
