@@ -301,11 +301,11 @@ __global__ void __launch_bounds__(T) pages_shrink_kernel(const PagesParams p)
 }
 
 // Blocks of 1024 threads for large batches, whose sums take a block of 256 several rounds (2048 sequences of 1024
-// columns: plan 20 us by 256, 9.5 by 1024), of 256 for the others (256 of 512: 5.4 and 7.8), as many as there is work for.
+// columns: plan 20 us by 256, 9.5 by 1024), of 256 for the others (1,000 of 512: 6.6 and 9.4), as many as there is work for.
 template <typename Kern>
 cudaError_t launch(Kern small, Kern large, const PagesParams& p, int64_t work, cudaStream_t stream)
 {
-    const bool many = p.batch > 2 * kSmall;
+    const bool many = p.batch > 4 * kSmall;
     const int threads = many ? kLarge : kSmall;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(148, work / threads))));
