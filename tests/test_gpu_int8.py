@@ -294,3 +294,60 @@ def test_refusals():
     assert ops.linear_int8(x[:0], layer).shape == (0, 8) and ops.gemm_int8(q[:0], s[:0], layer).shape == (0, 8)
     assert [t.shape for t in ops.linear_int8_rms_norm(x[:0], norm, layer, residual=x[:0])] == [(0, 8), (0, 32)]
     assert ops.quant_token(x[:0])[0].shape == (0, 32)
+
+
+_FIRST = """
+import sys, torch
+sys.path.insert(0, sys.argv[1])
+from w4a8_b200 import ops
+dev = torch.device("cuda", 0)
+ops.workspace(32 << 20, dev)
+g = torch.Generator().manual_seed(3)
+for M, N, K in ((3, 640, 4096), (40, 1280, 5120), (300, 512, 2048), (20, 64, 20000)):
+    layer = ops.prepare_int8(torch.randint(-128, 128, (N, K), generator=g, dtype=torch.int8).to(dev), torch.rand(N, generator=g).to(dev))
+    x = torch.randn(M, K, generator=g).bfloat16().to(dev)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ops.linear_int8(x, layer)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, ops.linear_int8(x, layer)), (M, N, K)
+assert ops.workspace_status(dev) == 0
+print("same")
+"""
+
+
+def test_captured_before_any_other_call():
+    """The first call of a process inside a capture: kernels are loaded and their residency asked for there."""
+    import os
+    import subprocess
+    import sys
+    _dev()
+    root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "vllm-ascend910_b200")
+    r = subprocess.run([sys.executable, "-c", _FIRST, root], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
+
+
+def test_two_threads():
+    """Calls of two threads: each in stream order on one workspace under the other's lock, as the rule asks."""
+    import threading
+    from w4a8_b200 import ops
+    dev = _dev()
+    g = torch.Generator().manual_seed(4)
+    layers = [_layer(N, 512, g, dev=dev)[3] for N in (300, 700)]
+    xs = [torch.randn(M, 512, generator=g).to(BF).to(dev) for M in (5, 200)]
+    want = [ops.linear_int8(x, L) for x, L in zip(xs, layers)]
+    lock, bad = threading.Lock(), []
+
+    def work(i):
+        for _ in range(50):
+            with lock:
+                y = ops.linear_int8(xs[i], layers[i])
+            if not torch.equal(y, want[i]):
+                bad.append(i)
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert not bad

@@ -157,6 +157,13 @@ __device__ __forceinline__ uint32_t two(float lo, float hi)
     return *reinterpret_cast<const uint32_t*>(&b);
 }
 
+// After a wait that ran out: gives what is on its way to a barrier until `deadline` to arrive.
+__device__ __forceinline__ void settle(uint64_t* bar, uint32_t parity, uint64_t deadline)
+{
+    while (!mbar_try_wait(bar, parity) && global_timer_ns() < deadline) {
+    }
+}
+
 // 32 sums of a lane's row (channels n .. n + 31) into y: scaled, rounded and stored by the widest access that
 // `align` allows.  All lanes of the warp call it; `turn` is the warp's.
 // `scale`, `bias`: the channels' in shared memory.
@@ -239,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, 2) int8_few_kernel(const __grid_cons
     static_assert(TT * 128 * 4 <= S * C::STAGE, "the sums of a split tile lie where the ring was");
     extern __shared__ uint8_t raw[];
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    __shared__ uint64_t full[S], empty[S], acc_full[2], acc_empty[2];
+    __shared__ uint64_t full[S], empty[S], acc_full[2], acc_empty[2], done;
     __shared__ uint32_t tmem_at;
     __shared__ int abort_flag;
     __shared__ float sh_scale[TT];
@@ -256,6 +263,7 @@ __global__ void __launch_bounds__(kThreads, 2) int8_few_kernel(const __grid_cons
             mbar_init(&acc_full[i], 1);
             mbar_init(&acc_empty[i], 4);
         }
+        mbar_init(&done, 1);
         abort_flag = 0;
         fence_mbar_init();
         tma_prefetch_desc(&p.tm_w);
@@ -301,6 +309,10 @@ __global__ void __launch_bounds__(kThreads, 2) int8_few_kernel(const __grid_cons
             // no copy may be on its way when the CTA ends: the last round of each stage has been read
             for (int i = max(it - S, 0); i < it; ++i)
                 mbar_wait(&empty[i % S], (i / S) & 1, quit, p.status, kWaitDrain);
+            if (*quit) {
+                const uint64_t deadline = global_timer_ns() + kWaitLimitNs;
+                for (int i = max(it - S, 0); i < it; ++i) settle(&full[i % S], (i / S) & 1, deadline);
+            }
         }
     } else if (warp == 1) {
         if (elect_one()) {
@@ -326,6 +338,10 @@ __global__ void __launch_bounds__(kThreads, 2) int8_few_kernel(const __grid_cons
                     tc_commit(&empty[s]);
                 }
                 if (ok) tc_commit(&acc_full[a]);
+            }
+            if (*quit) {                   // (tensor memory is given back below)
+                tc_commit(&done);
+                settle(&done, 0, global_timer_ns() + kWaitLimitNs);
             }
         }
     } else {
@@ -439,7 +455,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) int8_many_kernel(const __grid
     static_assert(SPLIT == 1 || NT * 128 * 4 <= S * C::STAGE, "the sums of a split tile lie where the ring was");
     extern __shared__ uint8_t raw[];
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    __shared__ uint64_t full[S], empty[S], acc_full[2], acc_empty[2];
+    __shared__ uint64_t full[S], empty[S], acc_full[2], acc_empty[2], done;
     __shared__ uint32_t tmem_at;
     __shared__ int abort_flag;
     __shared__ __align__(16) float sh_ws[2][NT], sh_b[2][NT];
@@ -457,6 +473,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) int8_many_kernel(const __grid
             mbar_init(&acc_full[i], 1);
             mbar_init(&acc_empty[i], 16);                    // eight warps of each CTA
         }
+        mbar_init(&done, 1);
         abort_flag = 0;
         fence_mbar_init();
         tma_prefetch_desc(&p.tm_w);
@@ -502,6 +519,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) int8_many_kernel(const __grid
             // every copy and every arrival at this CTA's barriers is in before it ends
             for (int64_t i = it > S ? it - S : 0; i < it; ++i)
                 mbar_wait(&empty[i % S], (i / S) & 1, quit, p.status, kWaitDrain);
+            if (*quit && rank == 0) {      // (the first CTA's barriers count both CTAs' copies)
+                const uint64_t deadline = global_timer_ns() + kWaitLimitNs;
+                for (int64_t i = it > S ? it - S : 0; i < it; ++i) settle(&full[i % S], (i / S) & 1, deadline);
+            }
         }
     } else if (warp == 1) {
         if (rank == 0 && elect_one()) {
@@ -527,12 +548,18 @@ __global__ void __launch_bounds__(kManyThreads, 1) int8_many_kernel(const __grid
                 }
                 if (ok) commit_pair(&acc_full[a], lead);
             }
+            if (*quit) {                   // (tensor memory is given back below)
+                asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&done))
+                             : "memory");
+                settle(&done, 0, global_timer_ns() + kWaitLimitNs);
+            }
         }
     } else {
         const int quad = warp & 3;
         const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
         pdl_wait();
         int64_t tile = 0;
+        bool ok = true;                    // (a warp whose wait ran out still comes to the others' barrier)
         for (int64_t t = pair; t < tiles; t += pairs, ++tile) {
             int m, nn;
             tile_of(t, mt, nt, m, nn);
@@ -547,7 +574,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) int8_many_kernel(const __grid
                 sh_b[a][c] = n < p.N && p.bias ? p.bias[n] : 0.0f;
             }
             asm volatile("bar.sync 1, 256;" ::: "memory");
-            if (!mbar_wait(&acc_full[a], (tile >> 1) & 1, quit, p.status, kWaitAccFull)) break;
+            ok = ok && mbar_wait(&acc_full[a], (tile >> 1) & 1, quit, p.status, kWaitAccFull);
+            if (!ok) continue;
             tc_fence_after();
             // this warp's half of the channels, the next 32 on their way while these are stored
             const int c0 = (warp - 2) / 4 * (NT / 2);
