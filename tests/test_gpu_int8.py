@@ -328,8 +328,27 @@ def test_captured_before_any_other_call():
     assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
 
 
-def test_two_threads():
-    """Calls of two threads: each in stream order on one workspace under the other's lock, as the rule asks."""
+def _threads(*works):
+    """Each work in a thread of its own; what any of them raised is raised here."""
+    import threading
+    wrong = []
+
+    def run(f):
+        try:
+            f()
+        except BaseException as e:                           # noqa: BLE001
+            wrong.append(e)
+    ts = [threading.Thread(target=run, args=(f,)) for f in works]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    if wrong:
+        raise wrong[0]
+
+
+def test_threads():
+    """Calls of two threads, each in stream order on one workspace under the other's lock, as the rule asks."""
     import threading
     from w4a8_b200 import ops
     dev = _dev()
@@ -337,17 +356,27 @@ def test_two_threads():
     layers = [_layer(N, 512, g, dev=dev)[3] for N in (300, 700)]
     xs = [torch.randn(M, 512, generator=g).to(BF).to(dev) for M in (5, 200)]
     want = [ops.linear_int8(x, L) for x, L in zip(xs, layers)]
-    lock, bad = threading.Lock(), []
+    lock = threading.Lock()
 
     def work(i):
         for _ in range(50):
             with lock:
                 y = ops.linear_int8(xs[i], layers[i])
-            if not torch.equal(y, want[i]):
-                bad.append(i)
-    ts = [threading.Thread(target=work, args=(i,)) for i in range(2)]
-    for t in ts:
-        t.start()
-    for t in ts:
-        t.join()
-    assert not bad
+            assert torch.equal(y, want[i])
+    _threads(lambda: work(0), lambda: work(1))
+
+
+@pytest.mark.parametrize("M", [5, 200])
+def test_a_threads_first_call(M):
+    """The product alone as the first CUDA call of a thread, which has no context yet."""
+    from w4a8_b200 import ops
+    dev = _dev()
+    g = torch.Generator().manual_seed(5)
+    w, ws, b, layer = _layer(300, 512, g, dev=dev)
+    q = torch.randint(-127, 128, (M, 512), generator=g, dtype=torch.int8).to(dev)
+    s = torch.rand(M, generator=g).to(dev)
+    out = torch.empty(M, 300, dtype=BF, device=dev)
+    torch.cuda.synchronize()
+    _threads(lambda: ops.gemm_int8(q, s, layer, out=out))
+    torch.cuda.synchronize()
+    assert torch.equal(out, product32(sums64(q, w), s, ws, b))

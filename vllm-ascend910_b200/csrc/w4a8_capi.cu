@@ -579,10 +579,17 @@ int capi_fail_cuda(cudaError_t e) { return fail_cuda(e); }
 int capi_bytes_map(CUtensorMap* m, const void* base, int64_t cols, int64_t rows, int64_t row_bytes, int box_rows)
 {
     if (get_encoder() != W4A8_OK) return fail_cuda(cudaErrorNotSupported);
-    return encode_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, static_cast<uint64_t>(cols), static_cast<uint64_t>(rows),
-                     static_cast<uint64_t>(row_bytes), 128, static_cast<uint32_t>(box_rows), CU_TENSOR_MAP_SWIZZLE_128B)
-               ? W4A8_OK
-               : W4A8_ERR_INVALID;
+    const auto encode = [&] {
+        return encode_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, static_cast<uint64_t>(cols), static_cast<uint64_t>(rows),
+                         static_cast<uint64_t>(row_bytes), 128, static_cast<uint32_t>(box_rows), CU_TENSOR_MAP_SWIZZLE_128B);
+    };
+    if (encode()) return W4A8_OK;
+    // A thread whose first call this is has no context yet, which the driver's encoder, unlike a launch, does not make current.
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaSetDevice(dev);
+    if (e != cudaSuccess) return fail_cuda(e);
+    return encode() ? W4A8_OK : W4A8_ERR_INVALID;
 }
 
 }  // namespace w4a8
