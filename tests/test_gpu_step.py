@@ -209,6 +209,12 @@ def test_refusals():
         dec.capture_steps(pages, [0, 1], [2, 1])
     with pytest.raises(RuntimeError, match="tokens"):
         dec.capture_steps(pages, [])
+    for rows, counts in (([0, 1], [1]), (torch.zeros(2, device=dev), [1, 1])):
+        with pytest.raises(RuntimeError):
+            dec.capture_steps(pages, rows, counts, tokens=2)
+    with pytest.raises(RuntimeError, match="images"):
+        dec.capture_steps(pages, [0, 1], images=(torch.zeros(2, dtype=torch.int32, device=dev), torch.zeros(0, 4, dtype=torch.int32, device=dev)))
+    assert pages.state.status() == 0
     a, b = pages.plan([0], [2], 2, 2), pages.plan([0, 1], [1, 1], 2, 2)
     with pytest.raises(RuntimeError):
         a.copy_(b)

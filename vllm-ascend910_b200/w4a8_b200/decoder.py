@@ -310,7 +310,9 @@ class CapturedSteps:
         _check(T > 0, "capture_steps: a step needs tokens")
         dev, B = self.rows.device, self.rows.shape[0]
         self.h = torch.zeros((T, dec.cfg.hidden), dtype=torch.bfloat16, device=dev)
-        # The workspace has to exist before the capture: one step without any page, and no plan.
+        # The workspace has to exist before the capture: one step without any page, and a plan of no tokens, which
+        # changes nothing and refuses what the captured one would.
+        pages.plan(self.rows, torch.zeros_like(self.counts), T, max_q_len, self.images)
         i = dict(dtype=torch.int32, device=dev)
         empty = Plan(torch.full((B, pages.state.columns), -1, **i), torch.zeros(B, **i), torch.zeros(B + 1, **i), T, max_q_len,
                      torch.zeros(pages.axes, T, **i) if pages.axes > 1 else None)
