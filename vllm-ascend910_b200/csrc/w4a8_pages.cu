@@ -301,14 +301,15 @@ __global__ void __launch_bounds__(T) pages_shrink_kernel(const PagesParams p)
 }
 
 // Blocks of 1024 threads for large batches, whose sums take a block of 256 several rounds (2048 sequences of 1024
-// columns: plan 20 us by 256, 9.5 by 1024), of 256 for the others (1,000 of 512: 6.6 and 9.4), as many as there is work for.
+// columns: plan 20 us by 256, 9.5 by 1024), of 256 for the others (1,000 of 512: 6.6 and 9.4), as many as there is work
+// for: `warps` pieces that a warp does in one go, two of them each.
 template <typename Kern>
-cudaError_t launch(Kern small, Kern large, const PagesParams& p, int64_t work, cudaStream_t stream)
+cudaError_t launch(Kern small, Kern large, const PagesParams& p, int64_t warps, cudaStream_t stream)
 {
     const bool many = p.batch > 4 * kSmall;
     const int threads = many ? kLarge : kSmall;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(148, work / threads))));
+    cfg.gridDim = dim3(static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(148, warps * 16 / threads))));
     cfg.blockDim = dim3(threads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -323,13 +324,14 @@ cudaError_t launch(Kern small, Kern large, const PagesParams& p, int64_t work, c
 
 cudaError_t launch_pages_plan(const PagesParams& p, cudaStream_t stream)
 {
-    return launch(pages_plan_kernel<kSmall>, pages_plan_kernel<kLarge>, p, static_cast<int64_t>(p.batch) * p.columns / 4 + 2 * p.tokens,
-                  stream);
+    const int span = p.columns % 4 == 0 ? 512 : 128;
+    const int64_t rows = static_cast<int64_t>(p.batch) * ((p.columns + span - 1) / span);
+    return launch(pages_plan_kernel<kSmall>, pages_plan_kernel<kLarge>, p, std::max(rows, (p.tokens + 31) / 32), stream);
 }
 
 cudaError_t launch_pages_shrink(const PagesParams& p, cudaStream_t stream)
 {
-    return launch(pages_shrink_kernel<kSmall>, pages_shrink_kernel<kLarge>, p, static_cast<int64_t>(p.batch) * 16, stream);
+    return launch(pages_shrink_kernel<kSmall>, pages_shrink_kernel<kLarge>, p, p.batch, stream);
 }
 
 }  // namespace w4a8
