@@ -55,7 +55,8 @@ def _layer(N, K, g, bias=True, dev=None):
 
 
 @pytest.mark.parametrize("M,K", [(1, 1), (3, 7), (5, 1057), (2, 5120), (300, 256), (4, 8200), (3, 20000), (2, 40001),
-                                 (300, 9000), (400, 27648), (1000, 8192), (300, 65536), (70, 70000), (297, 20001)])
+                                 (300, 9000), (400, 27648), (1000, 8192), (300, 65536), (70, 70000), (297, 20001),
+                                 (300, 1029), (310, 9004), (2, 8)])
 def test_codes(M, K):
     from w4a8_b200 import ops
     dev = _dev()
@@ -174,7 +175,7 @@ def _near(y, h, w, ws, b, tied=None):
 
 
 @pytest.mark.parametrize("M,N,K", [(1, 512, 5120), (33, 130, 1057), (200, 640, 768), (16, 300, 27648), (2, 64, 40000), (300, 40, 9600),
-                                   (310, 24, 5120), (2, 8, 70000)])
+                                   (310, 24, 5120), (2, 8, 70000), (300, 16, 9001), (310, 8, 1029), (40, 8, 9004), (7, 8, 9)])
 def test_swiglu(M, N, K):
     from w4a8_b200 import ops
     dev = _dev()
@@ -193,7 +194,9 @@ def test_swiglu(M, N, K):
 
 @pytest.mark.parametrize("M,N,K,res,f32", [(1, 512, 5120, True, False), (64, 300, 1057, True, True), (200, 256, 8192, False, False),
                                            (5, 640, 64, True, False), (3, 16, 32768, True, False), (300, 24, 9600, True, True),
-                                           (320, 16, 27648, False, False), (297, 8, 32768, True, False), (400, 40, 768, True, False)])
+                                           (320, 16, 27648, False, False), (297, 8, 32768, True, False), (400, 40, 768, True, False),
+                                           (300, 16, 9001, True, False), (40, 16, 9003, True, True), (300, 8, 1029, True, False),
+                                           (5, 8, 20006, True, False), (700, 8, 13, True, False)])
 def test_behind_a_norm(M, N, K, res, f32):
     from w4a8_b200 import ops
     dev = _dev()

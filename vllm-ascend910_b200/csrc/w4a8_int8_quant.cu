@@ -28,40 +28,109 @@ constexpr int kMaxTokThreads = 1024;
 constexpr int kMaxRowThreads = 512;
 constexpr int kRowBytes = 112 * 1024;      // of a row in shared memory: two blocks an SM at least
 
-// WHOLE: rows are 16-byte aligned and K is a multiple of 8.
-template <bool WHOLE>
-__device__ __forceinline__ void load8(const uint16_t* row, int pos, int K, bool vec, float (&v)[8])
+// Elements first .. first + 7 of the sixteen in lo, hi (first 0 to 8, the same in the whole warp).
+__device__ __forceinline__ uint4 middle8(uint4 lo, uint4 hi, int first)
 {
-    if (WHOLE || (vec && pos + 8 <= K)) {
-        unpack8_bf16(*reinterpret_cast<const uint4*>(row + pos), v);
-    } else {
+    const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    if (first == 8) return hi;
+    uint32_t t[6], u[5];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = pos + i < K ? bf16_bits_to_f32(row[pos + i]) : 0.0f;
+    for (int i = 0; i < 6; ++i) t[i] = first & 4 ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) u[i] = first & 2 ? t[i + 1] : t[i];
+    const int odd = (first & 1) * 16;
+    return make_uint4(__funnelshift_r(u[0], u[1], odd), __funnelshift_r(u[1], u[2], odd), __funnelshift_r(u[2], u[3], odd),
+                      __funnelshift_r(u[3], u[4], odd));
+}
+
+// 8 bf16 elements from position pos < K of a row, zeros past K.  WHOLE: rows are 16-byte aligned and K is a multiple of
+// 8.  Otherwise they come out of the two aligned vectors that hold them, each of which is only read where it holds
+// an element of the row; by single elements they took eight times the accesses (2,026 rows of 6023
+// behind a norm, their product included, 63 us, so 44).
+template <bool WHOLE>
+__device__ __forceinline__ uint4 load8_raw(const uint16_t* row, int pos, int K, bool vec)
+{
+    if (WHOLE || (vec && pos + 8 <= K)) return *reinterpret_cast<const uint4*>(row + pos);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(row + pos);
+    const int mis = static_cast<int>(at & 15) >> 1, left = K - pos;
+    const uint4* v = reinterpret_cast<const uint4*>(at & ~static_cast<uintptr_t>(15));
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    uint4 r = v[0];
+    if (mis) r = middle8(r, left > 8 - mis ? v[1] : zero, mis);
+    if (left < 8) {
+        uint32_t* w = &r.x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (2 * i >= left) w[i] = 0;
+            else if (2 * i + 1 >= left) w[i] &= 0xFFFFu;
+        }
     }
+    return r;
 }
 
 template <bool WHOLE>
-__device__ __forceinline__ void store8(uint16_t* row, int pos, int K, bool vec, const float (&v)[8])
+__device__ __forceinline__ void load8(const uint16_t* row, int pos, int K, bool vec, float (&v)[8])
 {
-    if (WHOLE || (vec && pos + 8 <= K)) {
-        uint32_t w[4];
+    unpack8_bf16(load8_raw<WHOLE>(row, pos, K, vec), v);
+}
+
+__device__ __forceinline__ uint4 pack8(const float (&v)[8])
+{
+    uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-            w[i] = *reinterpret_cast<const uint32_t*>(&b);
-        }
-        *reinterpret_cast<uint4*>(row + pos) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (pos + i < K) row[pos + i] = f32_to_bf16_bits(v[i]);
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&b);
     }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ void store_some(uint16_t* p, uint4 v, int from, int to)
+{
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (i >= from && i < to) p[i] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+}
+
+// 8 elements at position pos, if below K.  Called by whole warps whose lanes hold neighbouring vectors: where rows suit no
+// vectors, a lane stores the aligned one that ends in its own elements and begins in those of the lane before.
+template <bool WHOLE>
+__device__ __forceinline__ void store8(uint16_t* row, int pos, int K, bool vec, const float (&h)[8])
+{
+    const uint4 mine = pack8(h);
+    const int n = min(K - pos, 8);                            // elements of this lane, maybe none
+    if (WHOLE || vec) {
+        if (WHOLE ? n > 0 : n == 8) *reinterpret_cast<uint4*>(row + pos) = mine;
+        else if (n > 0) store_some(row + pos, mine, 0, n);
+        return;
+    }
+    const int mis = static_cast<int>(reinterpret_cast<uintptr_t>(row + pos) & 15) >> 1, lane = lane_id();
+    uint4 prev;
+    prev.x = __shfl_up_sync(0xffffffffu, mine.x, 1);
+    prev.y = __shfl_up_sync(0xffffffffu, mine.y, 1);
+    prev.z = __shfl_up_sync(0xffffffffu, mine.z, 1);
+    prev.w = __shfl_up_sync(0xffffffffu, mine.w, 1);
+    if (n <= 0) return;
+    const int own = 8 - mis;                                  // elements of the vector that are this lane's
+    if (lane > 0 && n >= own) {
+        *reinterpret_cast<uint4*>(row + pos - mis) = middle8(prev, mine, own);
+    } else {
+        if (lane > 0 && mis) store_some(row + pos - 8, prev, own, 8);
+        store_some(row + pos, mine, 0, min(n, own));
+    }
+    if (mis && (lane == 31 || pos + 8 >= K)) store_some(row + pos, mine, own, n);
 }
 
 __device__ __forceinline__ void load_weight8(const TokenQuantParams& p, int pos, float (&w)[8])
 {
     if (p.weight_f32) {
         const float* wf = static_cast<const float*>(p.weight);
+        if (p.vec_w && pos + 8 <= p.K) {
+            *reinterpret_cast<float4*>(w) = *reinterpret_cast<const float4*>(wf + pos);
+            *reinterpret_cast<float4*>(w + 4) = *reinterpret_cast<const float4*>(wf + pos + 4);
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i] = pos + i < p.K ? wf[pos + i] : 0.0f;
     } else {
@@ -96,30 +165,6 @@ __device__ __forceinline__ uint32_t max_abs2(uint32_t m, uint32_t w)
     uint32_t r;
     asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(m), "r"(w & 0x7FFF7FFFu));
     return r;
-}
-
-__device__ __forceinline__ uint4 pack8(const float (&v)[8])
-{
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t*>(&b);
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-template <bool WHOLE>
-__device__ __forceinline__ uint4 load8_raw(const uint16_t* row, int pos, int K, bool vec)
-{
-    if (WHOLE || (vec && pos + 8 <= K)) return *reinterpret_cast<const uint4*>(row + pos);
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t lo = pos + 2 * i < K ? row[pos + 2 * i] : 0u, hi = pos + 2 * i + 1 < K ? row[pos + 2 * i + 1] : 0u;
-        w[i] = lo | (hi << 16);
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // What a thread holds of 8 elements: bf16 before the scale is known, fp32 behind a norm.
@@ -232,7 +277,7 @@ __global__ void __launch_bounds__(kMaxTokThreads) token_quant_kernel(const Token
     constexpr int HOLD = VPT ? VPT : 1;
     const int vecs = VPT ? VPT : (p.K + 8 * T - 1) / (8 * T);
     const auto at = [&](int j) { return ((j * CL + rank) * T + tid) * 8; };
-    Held<SRC> h[HOLD];
+    Held<SRC> h[HOLD] = {};
     float ss = 0.0f, big = 0.0f;
     uint32_t big2 = 0;
 #pragma unroll
@@ -241,14 +286,15 @@ __global__ void __launch_bounds__(kMaxTokThreads) token_quant_kernel(const Token
 #pragma unroll
     for (int j = 0; j < vecs; ++j) {
         const int pos = at(j);
-        if (pos >= p.K) continue;
         Held<SRC>& e = h[VPT ? j : 0];
-        if (!VPT) row8<SRC, WHOLE>(p, x, r, pos, e);
         if constexpr (SRC == kTokNorm) {
-            if (p.res_out) store8<WHOLE>(p.res_out + row * p.ldro, pos, p.K, p.vec_ro, e.v);
+            if (p.res_out) store8<WHOLE>(p.res_out + row * p.ldro, pos, p.K, p.vec_ro, e.v);     // (whole warps)
+            if (pos >= p.K) continue;
 #pragma unroll
             for (int i = 0; i < 8; ++i) ss = fmaf(e.v[i], e.v[i], ss);
         } else {
+            if (pos >= p.K) continue;
+            if (!VPT) row8<SRC, WHOLE>(p, x, r, pos, e);
             big2 = max_abs2(max_abs2(max_abs2(max_abs2(big2, e.v.x), e.v.y), e.v.z), e.v.w);
         }
     }
@@ -309,15 +355,15 @@ __global__ void __launch_bounds__(kMaxTokThreads) token_quant_kernel(const Token
     if (CL > 1) cluster_sync();                               // (the others read this block's words until here)
 }
 
-// Many rows that suit vectors: the row waits for its scale in shared memory (bf16; fp32 behind a norm), which leaves room
+// Many rows: the row waits for its scale in shared memory (bf16; fp32 behind a norm), which leaves room
 // for 48 warps an SM where registers held 28.
-template <int SRC>
+template <int SRC, bool WHOLE>
 __global__ void __launch_bounds__(kMaxRowThreads, 1536 / kMaxRowThreads) token_quant_rows_kernel(const TokenQuantParams p)
 {
     extern __shared__ __align__(16) uint8_t staged[];
     __shared__ float red_sum[kMaxRowThreads / 32];
     __shared__ uint32_t red_max[kMaxRowThreads / 32];
-    const int tid = threadIdx.x, T = blockDim.x, nw = T >> 5, nvec = p.K / 8;
+    const int tid = threadIdx.x, T = blockDim.x, nw = T >> 5, nvec = (p.K + 7) / 8, lane = lane_id();
     pdl_wait();
     pdl_launch_dependents();
     const int64_t row = blockIdx.x;
@@ -330,10 +376,11 @@ __global__ void __launch_bounds__(kMaxRowThreads, 1536 / kMaxRowThreads) token_q
         float4 *lo = reinterpret_cast<float4*>(staged), *hi = lo + nvec;
         float ss = 0.0f;
 #pragma unroll 2
-        for (int v = tid; v < nvec; v += T) {
-            Held<SRC> h;
-            row8<SRC, true>(p, x, r, 8 * v, h);
-            if (p.res_out) store8<true>(p.res_out + row * p.ldro, 8 * v, p.K, true, h.v);
+        for (int v = tid; WHOLE ? v < nvec : v - lane < nvec; v += T) {      // (whole warps for store8)
+            Held<SRC> h = {};
+            if (WHOLE || v < nvec) row8<SRC, WHOLE>(p, x, r, 8 * v, h);
+            if (p.res_out) store8<WHOLE>(p.res_out + row * p.ldro, 8 * v, p.K, p.vec_ro, h.v);
+            if (!WHOLE && v >= nvec) break;
 #pragma unroll
             for (int i = 0; i < 8; ++i) ss = fmaf(h.v[i], h.v[i], ss);
             lo[v] = make_float4(h.v[0], h.v[1], h.v[2], h.v[3]);
@@ -365,7 +412,7 @@ __global__ void __launch_bounds__(kMaxRowThreads, 1536 / kMaxRowThreads) token_q
 #pragma unroll 2
         for (int v = tid; v < nvec; v += T) {
             Held<SRC> h;
-            row8<SRC, true>(p, x, r, 8 * v, h);
+            row8<SRC, WHOLE>(p, x, r, 8 * v, h);
             big2 = max_abs2(max_abs2(max_abs2(max_abs2(big2, h.v.x), h.v.y), h.v.z), h.v.w);
             hold[v] = h;
         }
@@ -391,7 +438,7 @@ __global__ void __launch_bounds__(kMaxRowThreads, 1536 / kMaxRowThreads) token_q
         } else {
             hold[v].get(h);
         }
-        emit8<true>(p, q, 8 * v, h, s, rcp, fast);
+        emit8<WHOLE>(p, q, 8 * v, h, s, rcp, fast);
     }
 }
 
@@ -404,8 +451,9 @@ template <int SRC>
 cudaError_t launch_rows(const TokenQuantParams& p, cudaStream_t stream)
 {
     const int threads = p.K <= 2048 * 8 ? 256 : 512;
-    const size_t smem = static_cast<size_t>(p.K) * (SRC == kTokNorm ? 4 : 2);
-    const cudaError_t e = cudaFuncSetAttribute(token_quant_rows_kernel<SRC>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowBytes);
+    const size_t smem = static_cast<size_t>((p.K + 7) / 8) * (SRC == kTokNorm ? 32 : 16);
+    const auto kern = whole_rows(p, SRC) ? token_quant_rows_kernel<SRC, true> : token_quant_rows_kernel<SRC, false>;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowBytes);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(p.M));
@@ -417,7 +465,7 @@ cudaError_t launch_rows(const TokenQuantParams& p, cudaStream_t stream)
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, token_quant_rows_kernel<SRC>, p);
+    return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
 template <int SRC, int VPT, int CL = 1>
@@ -451,7 +499,7 @@ cudaError_t launch_source(const TokenQuantParams& p, cudaStream_t stream)
     if (nvec > 1024 && nvec <= 8 * 1024 && p.M <= kFewRows) return launch<SRC, 1, 8>(p, threads(8), stream);
     // Many wide rows through shared memory (2,048 of 27,648: plain 43 us, SwiGLU 60, norm 124; in registers 49, 79 and 128),
     // narrower ones in registers (2,048 of 5120: plain 7.5 us, through shared memory 8.7).
-    if (p.M > kManyRows && whole_rows(p, SRC) && static_cast<int64_t>(p.K) * (SRC == kTokNorm ? 4 : 2) <= kRowBytes && nvec > 1024)
+    if (p.M > kManyRows && nvec * (SRC == kTokNorm ? 32 : 16) <= kRowBytes && nvec > 1024)
         return launch_rows<SRC>(p, stream);
     // Many rows: more vectors a thread keep more bytes in flight.
     if (p.M > kManyRows) {
