@@ -112,9 +112,11 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank)
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
+// (What the arrival orders is tensor memory, by the fence before it.  A release for the whole cluster would also wait for
+// the tile's stores: 4,096 x 8192 of K 128 30.5 us, without FIG.)
 __device__ __forceinline__ void arrive_remote(uint32_t bar)
 {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // All threads of the cluster (each CTA gets here whatever its waits gave).
 __device__ __forceinline__ void cluster_sync()
@@ -164,44 +166,62 @@ __device__ __forceinline__ void settle(uint64_t* bar, uint32_t parity, uint64_t 
     }
 }
 
+// A warp's 32 rows of 32 outputs from `turn` into y, BYTES an access: 64 / BYTES lanes a row.
+template <int BYTES>
+__device__ __forceinline__ void put_rows(const Int8GemmParams& p, int n, int64_t row0, const uint16_t (*turn)[40])
+{
+    constexpr int LANES = 64 / BYTES, ROWS = 32 / LANES, EACH = BYTES / 2;
+    const int lane = lane_id(), c = lane % LANES * EACH, first = lane / LANES;
+    const int rows = static_cast<int>(min(static_cast<int64_t>(32), p.M - row0));
+    uint16_t* y = p.y + (row0 + first) * p.ldy + n + c;
+    const int64_t step = ROWS * p.ldy;
+    if (n + c + EACH <= p.N) {
+#pragma unroll 8
+        for (int i = first; i < rows; i += ROWS, y += step) {
+            if (BYTES == 16) *reinterpret_cast<uint4*>(y) = *reinterpret_cast<const uint4*>(&turn[i][c]);
+            else if (BYTES == 8) *reinterpret_cast<uint2*>(y) = *reinterpret_cast<const uint2*>(&turn[i][c]);
+            else if (BYTES == 4) *reinterpret_cast<uint32_t*>(y) = *reinterpret_cast<const uint32_t*>(&turn[i][c]);
+            else *y = turn[i][c];
+        }
+    } else {
+        for (int i = first; i < rows; i += ROWS, y += step)
+            for (int e = 0; e < EACH && n + c + e < p.N; ++e) y[e] = turn[i][c + e];
+    }
+}
+
 // 32 sums of a lane's row (channels n .. n + 31) into y: scaled, rounded and stored by the widest access that
-// `align` allows.  All lanes of the warp call it; `turn` is the warp's.
-// `scale`, `bias`: the channels' in shared memory.
+// `align` allows, 32 bytes of a row a thread or, turned in shared memory, whole rows of 64.  All lanes of the warp call
+// it; `turn` is the warp's; `scale`, `bias`: the channels' in shared memory.
 __device__ __forceinline__ void put32(const Int8GemmParams& p, const uint32_t (&r)[32], int n, int64_t row, bool in, float s,
-                                      const float* scale, const float* bias, int align, uint16_t (*turn)[34])
+                                      const float* scale, const float* bias, int align, uint16_t (*turn)[40])
 {
     const int lane = lane_id();
-    uint16_t* y = p.y + row * p.ldy + n;
-    if (n + 32 <= p.N && align >= 16) {
-        uint32_t o[16];
+    if (n >= p.N) return;
+    uint32_t o[16];
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-            const float4 ws = *reinterpret_cast<const float4*>(scale + i), b = *reinterpret_cast<const float4*>(bias + i);
-            o[i / 2] = two(scaled(r[i], s, ws.x, b.x), scaled(r[i + 1], s, ws.y, b.y));
-            o[i / 2 + 1] = two(scaled(r[i + 2], s, ws.z, b.z), scaled(r[i + 3], s, ws.w, b.w));
-        }
-        if (!in) return;
-        if (align >= 32) {
+    for (int i = 0; i < 32; i += 4) {
+        const float4 ws = *reinterpret_cast<const float4*>(scale + i), b = *reinterpret_cast<const float4*>(bias + i);
+        o[i / 2] = two(scaled(r[i], s, ws.x, b.x), scaled(r[i + 1], s, ws.y, b.y));
+        o[i / 2 + 1] = two(scaled(r[i + 2], s, ws.z, b.z), scaled(r[i + 3], s, ws.w, b.w));
+    }
+    if (n + 32 <= p.N && align >= 32) {
+        uint16_t* y = p.y + row * p.ldy + n;
+        if (in)
 #pragma unroll
             for (int i = 0; i < 16; i += 8)                  // 32 bytes: a whole sector a thread
                 asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(y + 2 * i), "r"(o[i]), "r"(o[i + 1]),
                              "r"(o[i + 2]), "r"(o[i + 3]), "r"(o[i + 4]), "r"(o[i + 5]), "r"(o[i + 6]), "r"(o[i + 7])
                              : "memory");
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(y + 2 * i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-        }
-    } else if (n < p.N) {
-        // rows that suit no vector, or their end: a lane a channel, row by row
-#pragma unroll
-        for (int i = 0; i < 32; i += 2)
-            *reinterpret_cast<uint32_t*>(&turn[lane][i]) = two(scaled(r[i], s, scale[i], bias[i]), scaled(r[i + 1], s, scale[i + 1], bias[i + 1]));
-        __syncwarp();
-        const int64_t row0 = row - lane;
-        for (int i = 0; i < 32 && row0 + i < p.M; ++i)
-            if (n + lane < p.N) p.y[(row0 + i) * p.ldy + n + lane] = turn[i][lane];
-        __syncwarp();
+        return;
     }
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(&turn[lane][2 * i]) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+    __syncwarp();
+    if (align >= 16) put_rows<16>(p, n, row - lane, turn);
+    else if (align == 8) put_rows<8>(p, n, row - lane, turn);
+    else if (align == 4) put_rows<4>(p, n, row - lane, turn);
+    else put_rows<2>(p, n, row - lane, turn);
+    __syncwarp();
 }
 
 // G tokens from c on of a warp's 32 channels (n0 ..; a lane a channel) into y: rounded sums v, turned in `turn` so
@@ -459,7 +479,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) int8_many_kernel(const __grid
     __shared__ uint32_t tmem_at;
     __shared__ int abort_flag;
     __shared__ __align__(16) float sh_ws[2][NT], sh_b[2][NT];
-    __shared__ uint16_t turn[8][32][34];                     // a warp's 32 x 32 outputs on their way to rows
+    __shared__ __align__(16) uint16_t turn[8][32][40];       // a warp's 32 x 32 outputs on their way to rows
 
     const int warp = warp_id(), lane = lane_id();
     const uint32_t cta = cluster_rank(), rank = cta & 1, lead = cta & ~1u;       // in the pair; its first CTA
@@ -560,20 +580,34 @@ __global__ void __launch_bounds__(kManyThreads, 1) int8_many_kernel(const __grid
         pdl_wait();
         int64_t tile = 0;
         bool ok = true;                    // (a warp whose wait ran out still comes to the others' barrier)
+        // the row's scale and, one channel a thread, the channels', loaded a tile ahead
+        float row_scale, ws, b;
+        const auto load = [&](int64_t t) {
+            int m, nn;
+            tile_of(t, mt, nt, m, nn);
+            const int64_t row = static_cast<int64_t>(m) * 256 + rank * 128 + quad * 32 + lane;
+            const int c = threadIdx.x - 64;
+            const int64_t n = static_cast<int64_t>(nn) * NT + c;
+            const bool there = c < NT && n < p.N;
+            row_scale = row < p.M ? p.a_scale[row] : 0.0f;
+            ws = there ? p.w_scale[n] : 0.0f;
+            b = there && p.bias ? p.bias[n] : 0.0f;
+        };
+        if (pair < tiles) load(pair);
         for (int64_t t = pair; t < tiles; t += pairs, ++tile) {
             int m, nn;
             tile_of(t, mt, nt, m, nn);
             const int a = tile & 1;
             const int64_t row = static_cast<int64_t>(m) * 256 + rank * 128 + quad * 32 + lane;
             const bool in = row < p.M;
-            const float s = in ? p.a_scale[row] : 0.0f;
-            // the channels' scales are there before the sums (the other tile's warps still read the other buffer)
+            const float s = row_scale;
+            // (the other tile's warps still read the other buffer)
             if (const int c = threadIdx.x - 64; c < NT) {
-                const int64_t n = static_cast<int64_t>(nn) * NT + c;
-                sh_ws[a][c] = n < p.N ? p.w_scale[n] : 0.0f;
-                sh_b[a][c] = n < p.N && p.bias ? p.bias[n] : 0.0f;
+                sh_ws[a][c] = ws;
+                sh_b[a][c] = b;
             }
             asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (t + pairs < tiles) load(t + pairs);
             ok = ok && mbar_wait(&acc_full[a], (tile >> 1) & 1, quit, p.status, kWaitAccFull);
             if (!ok) continue;
             tc_fence_after();
@@ -814,7 +848,7 @@ cudaError_t launch_int8_gemm(const Int8GemmParams& p, const Int8Plan& plan, int 
         const int64_t mt = (p.M + 255) / 256, nt = (p.N + plan.nt - 1) / plan.nt;
         // the widest store that each row's outputs suit
         const auto fits = [&](uintptr_t a) { return reinterpret_cast<uintptr_t>(p.y) % a == 0 && 2 * p.ldy % a == 0; };
-        const int align = fits(32) ? 32 : fits(16) ? 16 : 2;
+        const int align = fits(32) ? 32 : fits(16) ? 16 : fits(8) ? 8 : fits(4) ? 4 : 2;
         if (plan.nt == 256) return launch_many<256>(p, plan.split, mt * nt, align, sms, stream, pdl);
         return launch_many<128>(p, plan.split, mt * nt, align, sms, stream, pdl);
     }
