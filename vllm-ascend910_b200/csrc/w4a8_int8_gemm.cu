@@ -113,7 +113,7 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank)
     return r;
 }
 // (What the arrival orders is tensor memory, by the fence before it.  A release for the whole cluster would also wait for
-// the tile's stores: 4,096 x 8192 of K 128 30.5 us, without FIG.)
+// the tile's stores.)
 __device__ __forceinline__ void arrive_remote(uint32_t bar)
 {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -818,9 +818,10 @@ Int8Plan int8_plan(int64_t M, int64_t N, int64_t K, int sms)
         r.a_rows = r.tt;
         return r;
     }
-    // The quickest by what each costs (microseconds measured on B200, 9 shapes of weights x 200 to 1024 tokens):
-    // starting and storing a tile, 0.26 or 0.31 a block of 128 of K in every wave of tiles, and a cut tile's join.
-    constexpr float kStart[2] = {5.7f, 6.7f}, kBlock[2] = {0.26f, 0.31f};
+    // The quickest by what each costs (microseconds measured on B200, 9 shapes of weights x 200 to 1024 tokens, and K 128
+    // to 2048 of 4,096 x 8192): starting and storing a tile, 0.26 or 0.31 a block of 128 of K, in every further wave of tiles
+    // that or storing the tile before, and a cut tile's join.
+    constexpr float kStart[2] = {5.7f, 6.7f}, kBlock[2] = {0.26f, 0.31f}, kStore[2] = {1.7f, 3.2f};
     constexpr float kJoin[2][4] = {{0.0f, 0.9f, 1.8f, 2.0f}, {0.0f, 3.7f, 6.0f, 7.0f}};
     const int64_t mt = (M + 255) / 256;
     float best = 0.0f;
@@ -830,7 +831,8 @@ Int8Plan int8_plan(int64_t M, int64_t N, int64_t K, int sms)
             const int64_t tiles = mt * ((N + nt - 1) / nt), waves = (tiles * split + sms / 2 - 1) / (sms / 2);
             if (split > 1 && (waves > 1 || kb < 2 * split || !(wide ? many_fits<256>(tiles, split) : many_fits<128>(tiles, split))))
                 continue;
-            const float cost = kStart[wide] + kBlock[wide] * static_cast<float>(waves * ((kb + split - 1) / split)) + kJoin[wide][split - 1];
+            const float blocks = kBlock[wide] * static_cast<float>((kb + split - 1) / split);
+            const float cost = kStart[wide] + blocks + static_cast<float>(waves - 1) * std::max(blocks, kStore[wide]) + kJoin[wide][split - 1];
             if (r.nt == 0 || cost < best) {
                 best = cost;
                 r.nt = nt;
