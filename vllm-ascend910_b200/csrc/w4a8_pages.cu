@@ -302,14 +302,14 @@ __global__ void __launch_bounds__(T) pages_shrink_kernel(const PagesParams p)
 
 // Blocks of 1024 threads for large batches, whose sums take a block of 256 several rounds (2048 sequences of 1024
 // columns: plan 20 us by 256, 9.5 by 1024), of 256 for the others (1,000 of 512: 6.6 and 9.4), as many as there is work
-// for: `warps` pieces that a warp does in one go, two of them each.
+// for: two of `pieces` to a warp.
 template <typename Kern>
-cudaError_t launch(Kern small, Kern large, const PagesParams& p, int64_t warps, cudaStream_t stream)
+cudaError_t launch(Kern small, Kern large, const PagesParams& p, int64_t pieces, cudaStream_t stream)
 {
     const bool many = p.batch > 4 * kSmall;
     const int threads = many ? kLarge : kSmall;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(148, warps * 16 / threads))));
+    cfg.gridDim = dim3(static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(148, pieces * 16 / threads))));
     cfg.blockDim = dim3(threads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -326,7 +326,10 @@ cudaError_t launch_pages_plan(const PagesParams& p, cudaStream_t stream)
 {
     const int span = p.columns % 4 == 0 ? 512 : 128;
     const int64_t rows = static_cast<int64_t>(p.batch) * ((p.columns + span - 1) / span);
-    return launch(pages_plan_kernel<kSmall>, pages_plan_kernel<kLarge>, p, std::max(rows, (p.tokens + 31) / 32), stream);
+    // A warp for each row's span (plan and shrink: 256 rows of 512 columns 9.5 us so, 10.4 by half the warps; 2048 of 1024
+    // 15.6 and 17.1; 1,162 of 13 columns 12.9 and 13.5, by the columns alone 16.8), a piece for eight tokens: finding one
+    // among grids is a chain (12 prompts of 2,000 with four grids each 11.5 us so, 14.3 by a quarter of the blocks).
+    return launch(pages_plan_kernel<kSmall>, pages_plan_kernel<kLarge>, p, std::max(2 * rows, (p.tokens + 7) / 8), stream);
 }
 
 cudaError_t launch_pages_shrink(const PagesParams& p, cudaStream_t stream)
