@@ -10,6 +10,9 @@
 // thread then stays with 16 elements of a head (two vectors of 8 pairs' halves) and one token, keeps their
 // angles in registers and turns every (threads / (items x tokens))-th head with them, with several heads' loads in
 // flight.  Elements past `rot` are copied, or left alone in place.
+//
+// Many tokens: memory bounds it (8,191 tokens of 40 + 8 heads of 128 36.0 us, 5.6 TB/s).  Fewer: the chain of position, table
+// row, rotation and store (one token 1.9 us; 5,041 of 16 + 16 heads of 80 13.5, a wave of 1,184 blocks and the rest of a second).
 #include <algorithm>
 
 #include "w4a8_rotary.cuh"
@@ -19,21 +22,22 @@ namespace w4a8 {
 namespace {
 
 constexpr int kThreads = 128;
-constexpr int kTokens = 16;                 // most tokens of a block
 constexpr int kAhead = 2;
 constexpr int kManyTokens = 592;
 
-// MANY: 2^tok_log2 tokens and all their heads; else one token and `heads_each` heads of q or, in a token's later blocks, of k.
-template <bool INTERLEAVED, bool MANY>
-__global__ void __launch_bounds__(kThreads, 8) rotary_kernel(const RotaryParams p, const int items, const int heads_each, const int many_log2)
+// LOG2 > 0: 2^LOG2 tokens and all their heads; 0: one token and `heads_each` heads of q or, in a token's later blocks, of k.
+// (The number is a constant and shared memory sized by it: 8,191 tokens of 40 + 8 heads 36.0 us, 36.9 with room for 16.)
+template <bool INTERLEAVED, int LOG2>
+__global__ void __launch_bounds__(kThreads, 8) rotary_kernel(const RotaryParams p, const int items, const int heads_each)
 {
-    __shared__ __align__(16) float angles[kTokens][kMaxRotaryDim];
+    constexpr bool MANY = LOG2 > 0;
+    constexpr int toks = 1 << LOG2;
+    __shared__ __align__(16) float angles[toks][kMaxRotaryDim];
     pdl_wait();
-    const int tok_log2 = MANY ? many_log2 : 0, toks = 1 << tok_log2;
     const int tid = threadIdx.x, half = p.rot / 2;
-    const int64_t t0 = static_cast<int64_t>(blockIdx.x) << tok_log2;
-    const int step = (kThreads / items) >> tok_log2, slot = tid / items, j = tid - slot * items;
-    const int k_tok = slot & (toks - 1), first = slot >> tok_log2;
+    const int64_t t0 = static_cast<int64_t>(blockIdx.x) << LOG2;
+    const int step = (kThreads / items) >> LOG2, slot = tid / items, j = tid - slot * items;
+    const int k_tok = slot & (toks - 1), first = slot >> LOG2;
     const int64_t t = t0 + k_tok;
     const bool on = first < step && t < p.tokens;             // (not the threads past the last whole set)
 
@@ -60,7 +64,7 @@ __global__ void __launch_bounds__(kThreads, 8) rotary_kernel(const RotaryParams 
             }
     };
     load(p.x[w0] + t * p.ld[w0], h0, end0);
-    for (int i = tid; i < half << tok_log2; i += kThreads) {
+    for (int i = tid; i < half << LOG2; i += kThreads) {
         const int k = i / half, pair = i - k * half, a = static_cast<int>(p.axes.map[pair >> 5] >> (2 * (pair & 31))) & 3;
         const int64_t at = min(t0 + k, p.tokens - 1);
         const float* row = p.cos_sin + clamp_row(p.axes.positions[a * p.axes.ld + at], p.table_rows) * p.rot;
@@ -92,19 +96,10 @@ __global__ void __launch_bounds__(kThreads, 8) rotary_kernel(const RotaryParams 
     }
 }
 
-}  // namespace
-
-cudaError_t launch_rotary(const RotaryParams& p, cudaStream_t stream)
+template <int LOG2>
+cudaError_t launch(const RotaryParams& p, int items, int heads_each, int parts, cudaStream_t stream)
 {
-    const int items = p.rot / 16 + (p.D - p.rot + 15) / 16, slots = kThreads / items;
-    // Many tokens: four a block with all their heads, and more where a block has threads for more heads than there are
-    // (62,909 tokens of 1 + 1 heads of 96: 45 us by four, 22 by sixteen).  Few: one, its heads spread over blocks.
-    const bool many = p.tokens >= kManyTokens;
-    int tok_log2 = 2;
-    while ((1 << tok_log2) < kTokens && (slots >> tok_log2) > std::max(p.heads[0], p.heads[1])) ++tok_log2;
-    const int each = many ? 0 : slots;
-    const int64_t blocks = many ? (p.tokens + (1 << tok_log2) - 1) >> tok_log2 : p.tokens;
-    const int parts = many ? 1 : (p.heads[0] + each - 1) / each + (p.heads[1] + each - 1) / each;
+    const int64_t blocks = (p.tokens + (1 << LOG2) - 1) >> LOG2;
     if (blocks > 0x7FFFFFFF || parts > 65535) return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(parts));
@@ -115,11 +110,25 @@ cudaError_t launch_rotary(const RotaryParams& p, cudaStream_t stream)
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (many)
-        return p.interleaved ? cudaLaunchKernelEx(&cfg, rotary_kernel<true, true>, p, items, each, tok_log2)
-                             : cudaLaunchKernelEx(&cfg, rotary_kernel<false, true>, p, items, each, tok_log2);
-    return p.interleaved ? cudaLaunchKernelEx(&cfg, rotary_kernel<true, false>, p, items, each, tok_log2)
-                         : cudaLaunchKernelEx(&cfg, rotary_kernel<false, false>, p, items, each, tok_log2);
+    return p.interleaved ? cudaLaunchKernelEx(&cfg, rotary_kernel<true, LOG2>, p, items, heads_each)
+                         : cudaLaunchKernelEx(&cfg, rotary_kernel<false, LOG2>, p, items, heads_each);
+}
+
+}  // namespace
+
+cudaError_t launch_rotary(const RotaryParams& p, cudaStream_t stream)
+{
+    const int items = p.rot / 16 + (p.D - p.rot + 15) / 16, slots = kThreads / items;
+    // Few tokens: one a block, its heads spread over blocks.  (40 + 8 heads of 128, one and four tokens a
+    // block: 256 tokens 3.5 and 5.6 us, 512 5.6 and 5.7, 1,024 9.5 and 6.8.)
+    if (p.tokens < kManyTokens)
+        return launch<0>(p, items, slots, (p.heads[0] + slots - 1) / slots + (p.heads[1] + slots - 1) / slots, stream);
+    // Many: four a block with all their heads, and more where a block has threads for more heads than there are (62,909
+    // tokens of 1 + 1 heads of 96: 44 us by four, 21 by sixteen).
+    const int heads = std::max(p.heads[0], p.heads[1]);
+    if ((slots >> 3) > heads) return launch<4>(p, items, 0, 1, stream);
+    if ((slots >> 2) > heads) return launch<3>(p, items, 0, 1, stream);
+    return launch<2>(p, items, 0, 1, stream);
 }
 
 }  // namespace w4a8
