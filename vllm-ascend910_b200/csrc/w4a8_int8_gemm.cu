@@ -11,14 +11,15 @@
 // 128-byte swizzle that the MMA's descriptors name; what lies past K, M or N arrives as
 // zeros.  tcgen05.mma kind::i8 multiplies 32 bytes of K an instruction.
 //
-// few (up to kFewTokens tokens): the weights' bytes bound it.  A tile is 128 channels (the
-//   MMA's rows) by 16, 32, 64 or 128 tokens (its columns), so that few tokens waste little.
-//   Two CTAs an SM, each with a ring of 96 KB in flight.  With fewer tiles than CTAs, a
-//   cluster cuts a tile's K: each CTA leaves its sums in shared memory and adds up
-//   a share of the tokens out of all of them over distributed shared memory.
-// many: the tensor pipe bounds it.  A pair of CTAs (cta_group::2) owns 256 tokens x 256 (or
-//   128) channels: each brings 128 tokens and half of the channels, one of them issues for
-//   both.  Two accumulators fill tensor memory, one in work while the other is stored.
+// few (up to kFewTokens tokens): the weights' bytes bound it (64 tokens of 55296 x 5120 45.7 us, 6.2 TB/s; one of
+//   7168 x 5120 9.6, 3.8 TB/s, where launch and join weigh).  A tile is 128 channels (the MMA's rows) by 16, 32, 64 or 128
+//   tokens (its columns), so that few tokens waste little.  Two CTAs an SM, each with a ring of up to 104 KB in flight.
+//   With fewer tiles than CTAs, a cluster cuts a tile's K: each CTA leaves its sums in shared memory and adds up a
+//   share of the tokens out of all of them over distributed shared memory.  128 tokens still belong here: 55296 x 5120
+//   51.4 us, 57.4 by the other kernel; 7168 x 5120 14.2 and 16.6.
+// many: the tensor pipe bounds it (2,048 tokens of 55296 x 5120 370 to 400 us, 2.9 to 3.1 POP/s by the clock that the power
+//   limit leaves).  A pair of CTAs (cta_group::2) owns 256 tokens x 256 (or 128) channels: each brings 128 tokens and half of
+//   the channels, one of them issues for both.  Two accumulators fill tensor memory, one in work while the other is stored.
 //
 // Each wait for a barrier is bounded; one that runs out ends the CTA's roles and leaves a code in
 // the workspace's status word.

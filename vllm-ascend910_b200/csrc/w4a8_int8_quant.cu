@@ -13,7 +13,12 @@
 //
 // A block holds its part of a row in registers, 8 elements of 16 bytes a vector (as bf16, or fp32
 // behind a norm): x is read once.  A wide row of few is cut over a cluster of eight blocks, whose sums and maxima
-// meet in distributed shared memory.  Rows past 65,536 elements are read twice, the second time out of L2.
+// meet in distributed shared memory.  Many wide rows wait for their scale in shared memory.  Rows past 65,536 elements are read twice, the second time out of L2.
+//
+// Few rows are bound by their chain of loads, sums and a barrier (one row of 5120 1.6 us, 16 of 27,648 3.2, SwiGLU 3.6), many
+// by the bytes in flight: 2,048 rows of 5120 7.6 us (4.1 TB/s), 8,192 28, with SwiGLU 12.3 and 49, behind a norm about 15
+// (24.4 with a product that takes 9.9 alone); 2,048 of 27,648 43, SwiGLU 60.
+//
 // Sums and maxima take a warp reduction and a barrier; partial sums are added in a fixed order.
 #include <algorithm>
 
@@ -503,7 +508,8 @@ cudaError_t launch_source(const TokenQuantParams& p, cudaStream_t stream)
         return launch_rows<SRC>(p, stream);
     // Many rows: more vectors a thread keep more bytes in flight.
     if (p.M > kManyRows) {
-        if (SRC != kTokNorm && threads(8) >= 256 && threads(8) <= kMaxTokThreads) return launch<SRC, 8>(p, threads(8), stream);
+        if constexpr (SRC != kTokNorm)
+            if (threads(8) >= 256 && threads(8) <= kMaxTokThreads) return launch<SRC, 8>(p, threads(8), stream);
         if (threads(4) >= 128 && threads(4) <= kMaxTokThreads) return launch<SRC, 4>(p, threads(4), stream);
         if (threads(2) >= 128 && threads(2) <= kMaxTokThreads) return launch<SRC, 2>(p, threads(2), stream);
     }

@@ -106,7 +106,10 @@ __device__ __forceinline__ int touched_pages(const CacheView& cv, int s)
     return s < cv.batch && hi > lo ? ((hi - 1) >> cv.page_log2) - (lo >> cv.page_log2) + 1 : 0;
 }
 
-// Query heads of kQTok tokens.
+// Query heads of kQTok tokens.  AXES: at the caller's positions, a row of the table for each axis.  Those are a load more in
+// the chain before the angles and take registers that spill (7,600 tokens of 40 + 8 + 8 heads of 128: 47 us at the token's own
+// place, 61 by axes, 66 with axes mixed; one token 3.4, 4.3 and 4.4); two or three blocks an SM with more registers are
+// no quicker (62 to 77).
 template <int D, bool AXES>
 __device__ __forceinline__ void rotate_queries(const KvWriteParams& p, int64_t t0)
 {
