@@ -135,3 +135,19 @@ def test_cpu_tensors_are_refused():
               lambda: kvcache.PageState.empty(4, 2, 2, 16, "cpu")):
         with pytest.raises(RuntimeError):
             f()
+
+
+def test_members_without_a_bias_take_the_others_type():
+    """A fused linear of which one member has a bias: zeros for the other, in fp32 and where the scales are."""
+    from w4a8_b200 import vendor
+    ckpt = {"a.weight": torch.ones(4, 8, dtype=torch.int8), "a.weight_scale": torch.ones(4, 1), "a.bias": torch.arange(4.0),
+            "b.weight": torch.ones(2, 8, dtype=torch.int8), "b.weight_scale": torch.ones(2, 1)}
+    old = torch.get_default_dtype()
+    torch.set_default_dtype(torch.float64)
+    try:
+        got = vendor.load_int8(ckpt.__getitem__, ["b", "a"])
+    finally:
+        torch.set_default_dtype(old)
+    assert got["bias"].dtype == torch.float32 and got["bias"].tolist() == [0, 0, 0, 1, 2, 3]
+    meta = {k: t.to("meta") for k, t in ckpt.items()}
+    assert vendor.load_int8(meta.__getitem__, ["a", "b"])["bias"].device.type == "meta"

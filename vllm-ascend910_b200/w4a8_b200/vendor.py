@@ -162,7 +162,7 @@ def load_int8(get: Callable[[str], torch.Tensor], names: Sequence[str]) -> Dict[
         raise ValueError("fused members must share K")
     bias = None
     if any(b is not None for b in biases):
-        bias = torch.cat([torch.zeros(w.shape[0]) if b is None else b for w, b in zip(ws, biases)])
+        bias = torch.cat([torch.zeros_like(s) if b is None else b for s, b in zip(scales, biases)])
     return {"w": torch.cat(ws), "w_scale": torch.cat(scales), "bias": bias}
 
 
