@@ -129,3 +129,18 @@ def test_another_gpu_current(dev, monkeypatch):
         kvcache.pages_plan(st, r, r + 1, 1)
         kvcache.pages_shrink(st, r)
     assert seen == [0] * 7 and st.status() == 0
+
+
+@pytest.mark.gpu
+def test_images_need_three_axes_even_without_a_grid(dev, monkeypatch):
+    from w4a8_b200 import kvcache
+    _N()
+    st = kvcache.PageState.empty(8, 2, 4, 16, dev)
+    rows, counts = torch.arange(2, dtype=I, device=dev), torch.ones(2, dtype=I, device=dev)
+    none = (torch.zeros(3, dtype=I, device=dev), torch.zeros(0, 4, dtype=I, device=dev))
+    f = lambda: kvcache.pages_plan(st, rows, counts, 2, axes=1, images=none)              # noqa: E731
+    for call in (lambda: _long(monkeypatch, f), f):
+        with pytest.raises(RuntimeError, match="3 axes"):
+            call()
+    assert not st.lens.any() and st.status() == 0
+    assert kvcache.pages_plan(st, rows, counts, 2, axes=3, images=none).positions.tolist() == [[0, 0]] * 3

@@ -368,7 +368,8 @@ PyObject* pages_plan(PyObject*, PyObject* const* a, Py_ssize_t n)
     if (a[6] != Py_None) {
         cu = tensor(a[6]);
         segs = tensor(a[7]);
-        if (!dense(cu, at::kInt, dev, 1) || !dense(segs, at::kInt, dev, 2) || cu->size(0) != B + 1 || segs->size(1) != 4) return later();
+        if (axes != 3 || !dense(cu, at::kInt, dev, 1) || !dense(segs, at::kInt, dev, 2) || cu->size(0) != B + 1 || segs->size(1) != 4)
+            return later();
     }
     // the outputs are parts of one allocation, each from a multiple of 16 bytes on
     const int64_t wide[5] = {B * st->columns, B, B + 1, tokens, axes * tokens};
