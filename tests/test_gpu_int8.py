@@ -383,3 +383,34 @@ def test_a_threads_first_call(M):
     _threads(lambda: ops.gemm_int8(q, s, layer, out=out))
     torch.cuda.synchronize()
     assert torch.equal(out, product32(sums64(q, w), s, ws, b))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", [(70_000, 32_768, 40), (128, 96, 72), (300, 96, 72)])
+def test_offsets_past_32_bits(M, N, K):
+    """More than 2^31 output elements, and rows of x, the residual and the output whose offsets pass 2^31 elements: rows are
+    those of a call on them alone."""
+    from w4a8_b200 import ops
+    dev = torch.device("cuda", 0)
+    if torch.cuda.mem_get_info(dev)[0] < 48 << 30:
+        pytest.skip("needs 48 GB")
+    g = torch.Generator(device=dev).manual_seed(M)
+    layer = ops.prepare_int8(torch.randint(-128, 128, (N, K), generator=g, device=dev, dtype=torch.int8),
+                             torch.rand(N, generator=g, device=dev), torch.rand(N, generator=g, device=dev))
+    x, r = (torch.randn(M, K, generator=g, device=dev).to(BF) for _ in range(2))
+    w = torch.rand(K, generator=g, device=dev).to(BF)
+    if M == 70_000:
+        y = ops.linear_int8(x, layer)
+        for at in (0, 35_000, M - 200):
+            assert torch.equal(y[at:at + 200], ops.linear_int8(x[at:at + 200], layer))
+        return
+    far = 2 ** 31 // (M - 1) // 8 * 8 + 1024                    # elements from row to row
+    assert (M - 1) * far > 2 ** 31
+    wide = [torch.empty(M * far, dtype=BF, device=dev).as_strided((M, n), (far, 1)) for n in (K, K, N)]
+    wide[0].copy_(x), wide[1].copy_(r)
+    want, sums = ops.linear_int8_rms_norm(x, w, layer, 1e-6, residual=r)
+    got, ro = ops.linear_int8_rms_norm(wide[0], w, layer, 1e-6, residual=wide[1], out=wide[2])
+    assert torch.equal(got, want) and torch.equal(ro, sums)
+    assert torch.equal(ops.linear_int8(wide[0], layer, out=wide[2]), ops.linear_int8(x, layer))
+    for one, two in zip(ops.quant_token(wide[0]), ops.quant_token(x)):
+        assert torch.equal(one, two)

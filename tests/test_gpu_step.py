@@ -192,6 +192,29 @@ def test_sequences_that_rest_and_steps_that_cannot_be():
 
 
 @pytest.mark.gpu
+def test_counts_past_the_longest_that_was_named():
+    """A captured step whose counts grow past its max_q_len runs another kernel than the plan of their length would, and
+    is as near the plain model."""
+    dev = _dev()
+    dec, plain = _build(dev, 24)
+    for c in dec.caches:
+        for t in (c.k, c.v, c.k_scale, c.v_scale):
+            t.zero_()
+    pages = dec.device_pages(2)
+    g = torch.Generator().manual_seed(9)
+    xs = [torch.randn(n, 512, generator=g).bfloat16() for n in (20, 17, 30, 2)]
+    dec.step(torch.cat(xs[:2]).to(dev), pages.plan([0, 1], [20, 17], 37, 20))
+    run = dec.capture_steps(pages, [0, 1], [1, 1], tokens=32, max_q_len=1)
+    run.counts.copy_(torch.tensor([30, 2]))
+    y = run(torch.cat(xs[2:]).to(dev)).cpu().double()
+    pages.check()
+    for before, new, got in ((xs[0], xs[2], y[:30]), (xs[1], xs[3], y[30:])):
+        x = torch.cat([before, new]).double()
+        want = plain.run_at(x, places(x.shape[0], []))[len(before):]
+        assert ((got - want).norm() / want.norm()).item() < BOUND
+
+
+@pytest.mark.gpu
 def test_refusals():
     from w4a8_b200 import decoder
     dev = _dev()
