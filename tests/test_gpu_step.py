@@ -279,3 +279,29 @@ def test_loading_8_bit_projections():
                       ("k.weight", t["k.weight"][:, :9]), ("k.bias", torch.zeros(2)), ("k.weight", t["k.weight"][0])):
         with pytest.raises(ValueError):
             vendor.load_int8({**t, name: bad}.__getitem__, ["q", "k"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mixed", [False, True])
+def test_one_section_is_the_ordinary_rotation(mixed):
+    """A configuration with a single axis on pages of the GPU, eager and captured: its positions are the tokens' places, so
+    the stack gives the bits of one without sections."""
+    from w4a8_b200 import ops
+    dev = _dev()
+    outs = []
+    for sections in (None, (32,)):
+        dec, _ = _build(dev, 24, ("o",), sections, mixed)
+        for c in dec.caches:
+            for t in (c.k, c.v, c.k_scale, c.v_scale):
+                t.zero_()
+        g = torch.Generator().manual_seed(12)
+        pages = dec.device_pages(3)
+        plan = pages.plan([2, 0, 1], [15, 30, 15], 60, 30)
+        assert (plan.positions is None) == (sections is None)
+        got = [dec.step(torch.randn(60, 512, generator=g).bfloat16().to(dev), plan)]
+        run = dec.capture_steps(pages, [0, 1, 2])
+        for _ in range(3):
+            got.append(run(torch.randn(3, 512, generator=g).bfloat16().to(dev)).clone())
+        pages.check()
+        outs.append(got + [t for c in dec.caches for t in (c.k, c.v, c.k_scale, c.v_scale)])
+    assert all(torch.equal(a, b) for a, b in zip(*outs)) and ops.workspace_status(dev) == 0

@@ -163,12 +163,15 @@ class DevicePages:
     """``Pages`` on the GPU (``kvcache.PageState``): sequences are rows 0 .. sequences - 1, and their lengths and
     pages never come to the host, so neither do a step's refusals; ``check`` raises for those.
 
-    ``positions``: rows of the rotary table; no sequence outgrows the whole pages that fit them."""
+    ``positions``: rows of the rotary table; no sequence outgrows the whole pages that fit them.  ``rotary``: whether plans
+    carry rotary positions of their own, on ``axes`` axes, as a decoder with ``rope_sections`` takes them (None: with
+    more than one axis)."""
 
-    def __init__(self, pages: int, page_size: int, sequences: int, positions: int, device="cuda", axes: int = 1):
+    def __init__(self, pages: int, page_size: int, sequences: int, positions: int, device="cuda", axes: int = 1,
+                 rotary: Optional[bool] = None):
         _check(positions >= page_size, "DevicePages: the rotary table is shorter than a page")
         self.state = kvcache.PageState.empty(pages, sequences, min(positions // page_size, pages), page_size, device)
-        self.axes = axes
+        self.axes, self.rotary = axes, axes > 1 if rotary is None else rotary
 
     def _put(self, v) -> torch.Tensor:
         return v if isinstance(v, torch.Tensor) else torch.tensor(v, dtype=torch.int32).to(self.state.device)
@@ -178,7 +181,7 @@ class DevicePages:
         device.  ``tokens``: rows of the step's input, at least the counts' sum; ``max_q_len``: the largest count;
         ``images``: ``kvcache.pages_plan``'s.  A step that cannot be has no tokens and no pages."""
         m = kvcache.pages_plan(self.state, self._put(rows), self._put(counts), tokens, self.axes, images)
-        return Plan(m.page_table, m.kv_lens, m.cu, tokens, max_q_len, m.positions if self.axes > 1 else None)
+        return Plan(m.page_table, m.kv_lens, m.cu, tokens, max_q_len, m.positions if self.rotary else None)
 
     def shrink(self, rows, keep) -> None:
         """Sequence rows[i] keeps its first keep[i] tokens: drafted ones past them were not accepted."""
@@ -223,7 +226,7 @@ class Decoder:
         c = self.caches[0] if self.caches else None
         _check(c is not None, "Decoder: device_pages needs a layer")
         return DevicePages(c.pages, self.cfg.page_size, sequences, self.cfg.positions, c.device,
-                           1 if self.axes is None else self.axes.axes)
+                           1 if self.axes is None else self.axes.axes, self.axes is not None)
 
     def step(self, h: torch.Tensor, plan: Plan) -> torch.Tensor:
         """Embedded tokens bf16 [tokens, hidden], in the plan's order -> the stack's normed output."""
@@ -315,7 +318,7 @@ class CapturedSteps:
         pages.plan(self.rows, torch.zeros_like(self.counts), T, max_q_len, self.images)
         i = dict(dtype=torch.int32, device=dev)
         empty = Plan(torch.full((B, pages.state.columns), -1, **i), torch.zeros(B, **i), torch.zeros(B + 1, **i), T, max_q_len,
-                     torch.zeros(pages.axes, T, **i) if pages.axes > 1 else None)
+                     torch.zeros(pages.axes, T, **i) if pages.rotary else None)
         side = torch.cuda.Stream(dev)
         side.wait_stream(torch.cuda.current_stream(dev))
         with torch.cuda.stream(side):
