@@ -414,3 +414,20 @@ def test_offsets_past_32_bits(M, N, K):
     assert torch.equal(ops.linear_int8(wide[0], layer, out=wide[2]), ops.linear_int8(x, layer))
     for one, two in zip(ops.quant_token(wide[0]), ops.quant_token(x)):
         assert torch.equal(one, two)
+
+
+@pytest.mark.parametrize("M", [1, 5, 200])
+def test_layers_of_one_channel(M):
+    """Weights [1, K] whose row stride is not K: torch calls them contiguous whatever it is."""
+    from w4a8_b200 import ops
+    dev = _dev()
+    g = torch.Generator().manual_seed(M)
+    big = torch.randint(-128, 128, (8, 40), generator=g, dtype=torch.int8).to(dev)
+    col = torch.randint(-128, 128, (32, 1), generator=g, dtype=torch.int8).to(dev)
+    ws, b = torch.rand(1, generator=g).to(dev), torch.rand(1, generator=g).to(dev)
+    x = torch.randn(M, 32, generator=g).to(BF).to(dev)
+    q, s = codes32(x.float())
+    for w in (big[2:3, :32], big[1:2, :32], col.T, big[0].as_strided((1, 32), (1 << 41, 1))):
+        layer = ops.prepare_int8(w, ws, b)
+        want = product32(sums64(q, w), s, ws, b)
+        assert torch.equal(ops.linear_int8(x, layer), want) and torch.equal(ops.gemm_int8(q, s, layer), want)

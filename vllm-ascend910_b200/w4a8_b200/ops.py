@@ -560,7 +560,8 @@ class Int8Weight:
 
     def __init__(self, w: torch.Tensor, scale: torch.Tensor, bias: Optional[torch.Tensor], K: int):
         self.w, self.scale, self.bias = w, scale, bias
-        self.N, self.K, self.ldw, self.device = w.shape[0], K, w.stride(0), w.device
+        self.N, self.K, self.device = w.shape[0], K, w.device
+        self.ldw = w.stride(0) if self.N > 1 else w.shape[1]          # (one row's stride may be anything)
         self._args = (w.data_ptr(), self.ldw, scale.data_ptr(), _ptr(bias), self.N)
         self._desc = _lib.Int8LayerDesc(w.data_ptr(), scale.data_ptr(), _ptr(bias), self.N, K, self.ldw)
         self._ref, self._index = ctypes.addressof(self._desc), w.get_device()
