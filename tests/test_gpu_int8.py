@@ -431,3 +431,64 @@ def test_layers_of_one_channel(M):
         layer = ops.prepare_int8(w, ws, b)
         want = product32(sums64(q, w), s, ws, b)
         assert torch.equal(ops.linear_int8(x, layer), want) and torch.equal(ops.gemm_int8(q, s, layer), want)
+
+
+# gates of a row, about: from where sigma(g) leaves fp32's normal numbers (-87.3) and e^-g all of them (-88.7), to where no up
+# brings the product back into bf16's range
+FAR = [-60, -80, -86, -87, -88, -90, -100, -120, -150, -165, -170, -300]
+
+
+@pytest.mark.parametrize("M,K", [(12, 64), (12, 1057), (12, 27648), (320, 2048), (300, 9000), (300, 5003), (12, 70000)])
+def test_gates_far_below_zero(M, K):
+    """silu(g) up where sigma(g) is tiny and up large: the element is the product's, not the sigmoid's, to lose.
+
+    A row's scale is exact: its largest element is 2^e out of a gate of 64, whose sigmoid rounds to 1.  The others lie
+    within [2^e / 8, 0.9 2^e].  fp32 gives them within 2^-18 (four equal factors of two units in the last place each,
+    four products), so that their bf16 value is the 64-bit one except within 2^-18 of a tie, where it may be its neighbour,
+    2^-7 of the value or at most one code away; the codes of equal values are equal."""
+    from w4a8_b200 import ops
+    dev = _dev()
+    g = torch.Generator().manual_seed(M + K)
+    base = torch.tensor(FAR, dtype=torch.float64).repeat(-(-M // len(FAR)))[:M, None]
+    gate = (base + 6 * torch.rand(M, K, generator=g, dtype=torch.float64) - 3).to(BF).double()
+    silu = gate * torch.sigmoid(gate)
+    e = ((base * torch.sigmoid(base)).abs().log2().floor() + 118).clamp(max=0)
+    e = torch.where(base < -200, torch.zeros_like(e), e)
+    target = 2.0 ** e * (0.125 + 0.775 * torch.rand(M, K, generator=g, dtype=torch.float64)) * torch.sign(torch.randn(M, K, generator=g))
+    up = torch.where(base < -200, torch.full_like(target, 3e38), target / torch.where(silu == 0, torch.ones_like(silu), silu)).to(BF)
+    at = K // 3
+    gate[:, at] = 64.0
+    up[:, at] = (2.0 ** (e[:, 0] - 6)).to(BF)
+    assert torch.isfinite(up).all()
+    a = gate * torch.sigmoid(gate) * up.double()
+    assert torch.equal(a[:, at].to(BF).double(), 2.0 ** e[:, 0])
+    r = a.to(BF)
+    lo, hi = (a * (1 - 2.0 ** -18)).to(BF), (a * (1 + 2.0 ** -18)).to(BF)
+    x = torch.cat([gate.to(BF), up], 1).to(dev)
+    q, s = ops.quant_token(x, act="swiglu")
+    q2, s2 = codes32(r.float())
+    assert torch.equal(s.cpu(), s2)
+    far = (q.cpu().int() - q2.int()).abs()
+    assert (far[lo == hi] == 0).all() and far.max() <= 1 and (q2[base[:, 0] > -200] != 0).all()
+    layer = _layer(8, K, g, dev=dev)[3]
+    assert torch.equal(ops.linear_int8(x, layer, act="swiglu"), ops.gemm_int8(q, s, layer))
+
+
+@pytest.mark.parametrize("gate,up", [(float("nan"), 1.0), (-90.0, float("nan")), (-90.0, float("inf")), (-float("inf"), 1.0),
+                                     (-float("inf"), 0.0), (float("inf"), 1.0), (-1e30, float("inf"))])
+def test_gates_that_are_not_finite(gate, up):
+    """A gate or up without a value leaves its row without one and the others as they are; -inf's is the formula's
+    -inf / (1 + e^inf), 0 times infinity."""
+    from w4a8_b200 import ops
+    dev = _dev()
+    x = torch.randn(3, 80, generator=torch.Generator().manual_seed(3)).to(BF)
+    want = ops.quant_token(x.to(dev), act="swiglu")
+    x[1, 7], x[1, 47] = gate, up
+    q, s = ops.quant_token(x.to(dev), act="swiglu")
+    assert torch.isnan(s[1]) and (q[1] == 0).all()
+    assert torch.equal(q[[0, 2]], want[0][[0, 2]]) and torch.equal(s[[0, 2]], want[1][[0, 2]])
+    x[1, 7], x[1, 47] = -1e30, 3e38                             # finite and nothing left: as a zero
+    q, s = ops.quant_token(x.to(dev), act="swiglu")
+    x[1, 7], x[1, 47] = 0.0, 0.0
+    q2, s2 = ops.quant_token(x.to(dev), act="swiglu")
+    assert torch.equal(q, q2) and torch.equal(s, s2)

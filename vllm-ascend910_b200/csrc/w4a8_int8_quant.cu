@@ -17,7 +17,7 @@
 //
 // Few rows are bound by their chain of loads, sums and a barrier (one row of 5120 1.6 us, 16 of 27,648 3.2, SwiGLU 3.6), many
 // by the bytes in flight: 2,048 rows of 5120 7.6 us (4.1 TB/s), 8,192 28, with SwiGLU 12.3 and 49, behind a norm about 15
-// (24.4 with a product that takes 9.9 alone); 2,048 of 27,648 43, SwiGLU 60.
+// (24.4 with a product that takes 9.9 alone); 2,048 of 27,648 43, SwiGLU 61.
 //
 // Sums and maxima take a warp reduction and a barrier; partial sums are added in a fixed order.
 #include <algorithm>
@@ -143,13 +143,14 @@ __device__ __forceinline__ void load_weight8(const TokenQuantParams& p, int pos,
     }
 }
 
-// silu(g) u = g / (1 + e^-g) u of two elements.  The exponential is the hardware's base-2 one, of -g log2(e) as a
-// rounded product and what the rounding left: within 2^-21 of the result.  Past 88 the exponent stays: 1 + e^-88 is 1, and
-// the reciprocal of 1 + e^88, below fp32's normal numbers, is 0.
+// silu(g) u = g / (1 + e^-g) u of two elements, g >= kFarGate (below, nothing of use).  The exponential is the
+// hardware's base-2 one, of -g log2(e) as a rounded product and what the rounding left (log2(e) in two parts, after
+// Cody and Waite): within 2^-21 of the result.  Above 88 the exponent stays: 1 + e^-88 is 1.
+constexpr float kFarGate = -87.0f;         // from about -87.3 on 1 / (1 + e^-g) is below fp32's normal numbers
 __device__ __forceinline__ void silu_up2(float g0, float g1, float u0, float u1, float& y0, float& y1)
 {
     constexpr float kL = 1.44269502162933349609375f, kLow = 1.925963033500011e-08f;     // log2(e) = kL + kLow
-    const uint64_t c = pair2(fminf(fmaxf(g0, -88.0f), 88.0f), fminf(fmaxf(g1, -88.0f), 88.0f));
+    const uint64_t c = pair2(fminf(g0, 88.0f), fminf(g1, 88.0f));
     const uint64_t t = f2_mul(c, pair2(-kL, -kL)), minus_t = f2_mul(c, pair2(kL, kL));
     const uint64_t low = f2_fma(c, pair2(-kLow, -kLow), f2_fma(c, pair2(-kL, -kL), minus_t));
     float t0, t1, e0, e1, r0, r1;
@@ -162,6 +163,23 @@ __device__ __forceinline__ void silu_up2(float g0, float g1, float u0, float u1,
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r0) : "f"(e0));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r1) : "f"(e1));
     unpair2(f2_mul(f2_mul(pair2(g0, g1), pair2(r0, r1)), pair2(u0, u1)), y0, y1);
+}
+
+// The same of one element, g < kFarGate, where 1 / (1 + e^-g) is e^g (1 - e^g) = e^g: its four factors e^(g / 4) one by one
+// after u, whose size keeps each product in fp32's range while the last one is in it.
+__device__ __forceinline__ float silu_up_far(float g, float u)
+{
+    const float e = expf(0.25f * g);
+    return __fmul_rn(__fmul_rn(__fmul_rn(__fmul_rn(__fmul_rn(g, e), u), e), e), e);
+}
+
+// The largest of `most` and of 8 values' bits: above kFarBits where one is below kFarGate (or a NaN of negative sign).
+constexpr uint32_t kFarBits = 0xC2AE0000u;
+__device__ __forceinline__ uint32_t most_bits(uint32_t most, const float (&g)[8])
+{
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(g[i]));
+    return most;
 }
 
 // The larger of the magnitudes in m and of two bf16 values, each half its own; a NaN wins.
@@ -188,9 +206,13 @@ struct Held<kTokNorm> {
     }
 };
 
-// 8 elements of h; behind a norm, of x + residual.
-template <int SRC, bool WHOLE>
-__device__ __forceinline__ void row8(const TokenQuantParams& p, const uint16_t* x, const uint16_t* r, int pos, Held<SRC>& h)
+// 8 elements of h; behind a norm, of x + residual.  Gates below kFarGate take a branch of their own (FAR), or are left wrong
+// and gathered in `most`, for a thread that met one to take its vectors again: in a loop that waits for its loads the branch
+// holds up the next ones (2,048 rows of 27,648 64 to 66 us with it, 60 to 61 without), rows in registers have all theirs
+// on the way (8,192 of 5120 48.5 with it, 52.4 the other way).
+template <int SRC, bool WHOLE, bool FAR>
+__device__ __forceinline__ void row8(const TokenQuantParams& p, const uint16_t* x, const uint16_t* r, int pos, Held<SRC>& h,
+                                     uint32_t& most)
 {
     if constexpr (SRC == kTokNorm) {
         load8<WHOLE>(x, pos, p.K, p.vec_x, h.v);
@@ -203,13 +225,20 @@ __device__ __forceinline__ void row8(const TokenQuantParams& p, const uint16_t* 
     } else {
         h.v = load8_raw<WHOLE>(x, pos, p.K, p.vec_x);
         if (SRC == kTokSwiglu) {
-            float g[8], u[8];
+            float g[8], u[8], y[8];
             const uint4 w = load8_raw<WHOLE>(x + p.K, pos, p.K, p.vec_x && p.K % 8 == 0);
             unpack8_bf16(h.v, g);
             unpack8_bf16(w, u);
 #pragma unroll
-            for (int i = 0; i < 8; i += 2) silu_up2(g[i], g[i + 1], u[i], u[i + 1], g[i], g[i + 1]);
-            h.v = pack8(g);
+            for (int i = 0; i < 8; i += 2) silu_up2(g[i], g[i + 1], u[i], u[i + 1], y[i], y[i + 1]);
+            if constexpr (!FAR) {
+                most = most_bits(most, g);
+            } else if (most_bits(0, g) > kFarBits) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (g[i] < kFarGate) y[i] = silu_up_far(g[i], u[i]);
+            }
+            h.v = pack8(y);
         }
     }
 }
@@ -284,10 +313,10 @@ __global__ void __launch_bounds__(kMaxTokThreads) token_quant_kernel(const Token
     const auto at = [&](int j) { return ((j * CL + rank) * T + tid) * 8; };
     Held<SRC> h[HOLD] = {};
     float ss = 0.0f, big = 0.0f;
-    uint32_t big2 = 0;
+    uint32_t big2 = 0, most = 0;
 #pragma unroll
     for (int j = 0; j < vecs; ++j)
-        if (VPT && at(j) < p.K) row8<SRC, WHOLE>(p, x, r, at(j), h[j]);
+        if (VPT && at(j) < p.K) row8<SRC, WHOLE, true>(p, x, r, at(j), h[j], most);
 #pragma unroll
     for (int j = 0; j < vecs; ++j) {
         const int pos = at(j);
@@ -299,7 +328,7 @@ __global__ void __launch_bounds__(kMaxTokThreads) token_quant_kernel(const Token
             for (int i = 0; i < 8; ++i) ss = fmaf(e.v[i], e.v[i], ss);
         } else {
             if (pos >= p.K) continue;
-            if (!VPT) row8<SRC, WHOLE>(p, x, r, pos, e);
+            if (!VPT) row8<SRC, WHOLE, true>(p, x, r, pos, e, most);
             big2 = max_abs2(max_abs2(max_abs2(max_abs2(big2, e.v.x), e.v.y), e.v.z), e.v.w);
         }
     }
@@ -352,7 +381,7 @@ __global__ void __launch_bounds__(kMaxTokThreads) token_quant_kernel(const Token
         const int pos = at(j);
         if (pos >= p.K) continue;
         Held<SRC>& e = h[VPT ? j : 0];
-        if (!VPT) row8<SRC, WHOLE>(p, x, r, pos, e);
+        if (!VPT) row8<SRC, WHOLE, true>(p, x, r, pos, e, most);
         float v[8];
         e.get(v);
         emit8<WHOLE>(p, q, pos, v, s, rcp, fast);
@@ -383,7 +412,8 @@ __global__ void __launch_bounds__(kMaxRowThreads, 1536 / kMaxRowThreads) token_q
 #pragma unroll 2
         for (int v = tid; WHOLE ? v < nvec : v - lane < nvec; v += T) {      // (whole warps for store8)
             Held<SRC> h = {};
-            if (WHOLE || v < nvec) row8<SRC, WHOLE>(p, x, r, 8 * v, h);
+            uint32_t none = 0;
+            if (WHOLE || v < nvec) row8<SRC, WHOLE, false>(p, x, r, 8 * v, h, none);
             if (p.res_out) store8<WHOLE>(p.res_out + row * p.ldro, 8 * v, p.K, p.vec_ro, h.v);
             if (!WHOLE && v >= nvec) break;
 #pragma unroll
@@ -413,13 +443,23 @@ __global__ void __launch_bounds__(kMaxRowThreads, 1536 / kMaxRowThreads) token_q
             hi[v] = make_float4(h[4], h[5], h[6], h[7]);
         }
     } else {
-        uint32_t big2 = 0;
+        uint32_t big2 = 0, most = 0;
 #pragma unroll 2
         for (int v = tid; v < nvec; v += T) {
             Held<SRC> h;
-            row8<SRC, WHOLE>(p, x, r, 8 * v, h);
+            row8<SRC, WHOLE, false>(p, x, r, 8 * v, h, most);
             big2 = max_abs2(max_abs2(max_abs2(max_abs2(big2, h.v.x), h.v.y), h.v.z), h.v.w);
             hold[v] = h;
+        }
+        if (SRC == kTokSwiglu && most > kFarBits) {
+            big2 = 0;
+#pragma unroll 1
+            for (int v = tid; v < nvec; v += T) {
+                Held<SRC> h;
+                row8<SRC, WHOLE, true>(p, x, r, 8 * v, h, most);
+                big2 = max_abs2(max_abs2(max_abs2(max_abs2(big2, h.v.x), h.v.y), h.v.z), h.v.w);
+                hold[v] = h;
+            }
         }
         big = max_abs_nan(0.0f, __uint_as_float(big2 << 16), __uint_as_float(big2 & 0xFFFF0000u));
     }
@@ -502,7 +542,7 @@ cudaError_t launch_source(const TokenQuantParams& p, cudaStream_t stream)
     const int nvec = (p.K + 7) / 8;
     const auto threads = [&](int vpt) { return ((nvec + vpt - 1) / vpt + 31) / 32 * 32; };
     if (nvec > 1024 && nvec <= 8 * 1024 && p.M <= kFewRows) return launch<SRC, 1, 8>(p, threads(8), stream);
-    // Many wide rows through shared memory (2,048 of 27,648: plain 43 us, SwiGLU 60, norm 124; in registers 49, 79 and 128),
+    // Many wide rows through shared memory (2,048 of 27,648: plain 43 us, SwiGLU 61, norm 124; in registers 49, 79 and 128),
     // narrower ones in registers (2,048 of 5120: plain 7.5 us, through shared memory 8.7).
     if (p.M > kManyRows && nvec * (SRC == kTokNorm ? 32 : 16) <= kRowBytes && nvec > 1024)
         return launch_rows<SRC>(p, stream);
