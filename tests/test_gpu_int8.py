@@ -492,3 +492,54 @@ def test_gates_that_are_not_finite(gate, up):
     x[1, 7], x[1, 47] = 0.0, 0.0
     q2, s2 = ops.quant_token(x.to(dev), act="swiglu")
     assert torch.equal(q, q2) and torch.equal(s, s2)
+
+
+# Shapes that take every form of the product on a GPU of 148 SMs, ragged in every direction: the kernel, its tile of
+# tokens (few) or channels (many), and how many CTAs, or pairs of them, cut a tile's K.
+FORMS = [(("few", tt, split), (M, N, K)) for M, tt in ((5, 16), (20, 32), (50, 64), (100, 128))
+         for split, N, K in ((1, 301, 500), (2, 8001, 1100), (3, 6001, 1101), (4, 4002, 1100), (6, 2501, 1700), (8, 2003, 2100))] + [
+    (("many", 128, 1), (131, 101, 201)), (("many", 128, 2), (140, 103, 1101)), (("many", 128, 3), (131, 2401, 3001)),
+    (("many", 128, 4), (257, 102, 3001)), (("many", 256, 1), (300, 5001, 201)), (("many", 256, 2), (131, 6401, 10001)),
+    (("many", 256, 3), (200, 4803, 6007)), (("many", 256, 4), (140, 3201, 27650))]
+
+
+@pytest.mark.parametrize("form,shape", FORMS)
+def test_every_form_of_the_product(form, shape):
+    from w4a8_b200 import ops
+    dev = _dev()
+    M, N, K = shape
+    g = torch.Generator().manual_seed(M + N + K)
+    w, ws, b, layer = _layer(N, K, g, bias=M % 2 == 0, dev=dev)
+    q = torch.randint(-128, 128, (M, K), generator=g, dtype=torch.int8).to(dev)
+    s = (torch.rand(M, generator=g) * 0.02).to(dev)
+    want = product32(sums64(q, w), s, ws, b)
+    assert torch.equal(ops.gemm_int8(q, s, layer), want)
+    # rows that suit the widest stores, and what lies beside the output
+    wide = torch.full((M + 2, -(-N // 16) * 16 + 16), 7.0, dtype=BF, device=dev)
+    ops.gemm_int8(q, s, layer, out=wide[1:M + 1, :N])
+    assert torch.equal(wide[1:M + 1, :N], want) and (wide[[0, -1]] == 7).all() and (wide[:, N:] == 7).all()
+    assert ops.workspace_status(dev) == 0
+
+
+def test_the_shapes_take_every_form():
+    """The plans of the list above, by the names of the kernels that ran."""
+    import re
+    from torch.profiler import ProfilerActivity, profile
+    from w4a8_b200 import ops
+    dev = _dev()
+    if torch.cuda.get_device_properties(dev).multi_processor_count != 148:
+        pytest.skip("the list is for 148 SMs")
+    taken = []
+    for _, (M, N, K) in FORMS:
+        layer = ops.prepare_int8(torch.zeros(N, K, dtype=torch.int8, device=dev), torch.ones(N, device=dev))
+        q, s = torch.zeros(M, K, dtype=torch.int8, device=dev), torch.ones(M, device=dev)
+        torch.cuda.synchronize()
+        with profile(activities=[ProfilerActivity.CUDA]) as p:
+            ops.gemm_int8(q, s, layer)
+            torch.cuda.synchronize()
+        names = [re.search(r"int8_(few|many)_kernel<(\d+), (\d+)>", e.name) for e in p.events()]
+        taken.append([(m[1], int(m[2]), int(m[3])) for m in names if m])
+    if not any(taken):
+        pytest.skip("no kernel names on this machine")
+    # (the last needs 13 clusters of eight at a time, which not every set of 148 SMs may hold)
+    assert taken[:-1] == [[form] for form, _ in FORMS[:-1]] and taken[-1] in ([("many", 256, 4)], [("many", 128, 2)])
