@@ -212,3 +212,45 @@ def test_captured_positions_and_refusals():
         with pytest.raises(RuntimeError):
             f()
     assert kvcache.rotary(q[:0], k[:0], table, pos[:, :0], axes)[1].shape == (0, 2, 128)
+
+
+MANY = [
+    # tokens, q heads, k heads, head_dim, sections, mixed, interleaved: four, eight or sixteen tokens a block, the last block partly full
+    (661, 16, 16, 80, [20, 20], False, True),
+    (602, 5, 4, 128, [24, 20, 20], True, True),
+    (601, 3, 2, 128, [16, 24, 24], False, False),
+    (607, 2, 3, 128, [16, 24, 24], True, True),
+    (611, 1, 1, 96, [5, 3, 4, 4], False, True),
+    (650, 1, 0, 64, [8, 12, 12], True, False),
+    # elements behind the turned ones, copied or left alone
+    (599, 7, 2, 72, [11, 13, 8], True, False),
+    (605, 4, 3, 72, [32], False, True),
+    (613, 2, 1, 72, [10, 22], False, False),
+    (597, 9, 1, 256, [4, 4], True, True),
+    (1191, 1, 2, 40, [8, 8], False, False),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,hq,hk,d,sections,mixed,inter", MANY)
+def test_rotary_of_many_tokens(T, hq, hk, d, sections, mixed, inter):
+    if hk:
+        test_rotary(T, hq, hk, d, sections, mixed, inter)
+    from w4a8_b200 import kvcache
+    dev = _dev()
+    g = torch.Generator().manual_seed(T)
+    axes = kvcache.RotaryAxes(sections, mixed=mixed)
+    table = kvcache.rotary_table(2 * axes.pairs, 33, base=1e4, device="cpu")
+    pos = torch.randint(-3, 40, (axes.axes, T), generator=g, dtype=torch.int32)
+    # in rows longer than the heads, into others: what lies beside both stays
+    x = torch.randn(T, hq * d + 8, generator=g).to(BF).to(dev)
+    out = torch.full((T + 2, hq * d + 24), 7.0, dtype=BF, device=dev)
+    q = x[:, 8:].unflatten(1, (hq, d))
+    want = turn32(q.float().cpu(), pos, axes.axis_of_pair(), table, inter).to(BF)
+    view = out[1:T + 1, 8:hq * d + 8].unflatten(1, (hq, d))
+    kvcache.rotary(q, None, table.to(dev), pos.to(dev), axes, interleaved=inter, q_out=view)
+    assert torch.equal(view.cpu(), want)
+    assert (out[[0, -1]] == 7).all() and (out[:, :8] == 7).all() and (out[:, hq * d + 8:] == 7).all()
+    before = x[:, :8].clone()
+    kvcache.rotary(q, None, table.to(dev), pos.to(dev), axes, interleaved=inter, q_out=q)
+    assert torch.equal(q.cpu(), want) and torch.equal(x[:, :8], before)
