@@ -17,9 +17,10 @@
 //   With fewer tiles than CTAs, a cluster cuts a tile's K: each CTA leaves its sums in shared memory and adds up a
 //   share of the tokens out of all of them over distributed shared memory.  128 tokens still belong here: 55296 x 5120
 //   51.4 us, 57.4 by the other kernel; 7168 x 5120 14.2 and 16.6.
-// many: the tensor pipe bounds it (2,048 tokens of 55296 x 5120 370 to 400 us, 2.9 to 3.1 POP/s by the clock that the power
-//   limit leaves).  A pair of CTAs (cta_group::2) owns 256 tokens x 256 (or 128) channels: each brings 128 tokens and half of
-//   the channels, one of them issues for both.  Two accumulators fill tensor memory, one in work while the other is stored.
+// many: the tensor pipe bounds it (2,048 tokens of 55296 x 5120 349 us for one launch, 3.3 POP/s; 370 in a loop of some, 3.1;
+//   438 with the norm in front in a loop of seconds, 2.6 by the clock that the power limit leaves).  A pair of CTAs
+//   (cta_group::2) owns 256 tokens x 256 (or 128) channels: each brings 128 tokens and half of the channels, one of them issues
+//   for both.  Two accumulators fill tensor memory, one in work while the other is stored.
 //
 // Each wait for a barrier is bounded; one that runs out ends the CTA's roles and leaves a code in
 // the workspace's status word.
