@@ -305,3 +305,31 @@ def test_one_section_is_the_ordinary_rotation(mixed):
         pages.check()
         outs.append(got + [t for c in dec.caches for t in (c.k, c.v, c.k_scale, c.v_scale)])
     assert all(torch.equal(a, b) for a, b in zip(*outs)) and ops.workspace_status(dev) == 0
+
+
+@pytest.mark.gpu
+def test_captures_are_made_on_the_decoders_device(monkeypatch):
+    """A capture's stream is one of the decoder's GPU, which is made current for it, whichever was: on another's stream
+    nothing of the step would be captured.  (One GPU here: what the capture is told is looked at.)"""
+    dev = _dev()
+    dec, _ = _build(dev, 8)
+    inside, seen, real_graph = [], [], torch.cuda.graph
+
+    class Device(torch.cuda.device):
+        def __enter__(self):
+            inside.append(self.idx)
+            return super().__enter__()
+
+        def __exit__(self, *a):
+            inside.pop()
+            return super().__exit__(*a)
+
+    def graph(g, *a, stream=None, **k):
+        seen.append((stream is not None and stream.device == dev, 0 in inside))
+        return real_graph(g, *a, stream=stream, **k)
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "graph", graph)
+    dec.capture(dec.pages.plan([dec.pages.add()], [1], dev))
+    dec.capture_steps(dec.device_pages(2), [0, 1])
+    assert seen == [(True, True)] * 2

@@ -28,6 +28,7 @@ The reference leaves norms, rotary positions, cache and attention to its serving
 from __future__ import annotations
 
 import argparse
+import contextlib
 import dataclasses
 from typing import Dict, List, Optional, Sequence, Tuple, Union
 
@@ -264,6 +265,20 @@ class Decoder:
         return CapturedSteps(self, pages, rows, counts, tokens, max_q_len, images)
 
 
+@contextlib.contextmanager
+def _capture(graph: torch.cuda.CUDAGraph, device: torch.device, warm_up):
+    """A capture on a stream of ``device``, after ``warm_up`` has run there: the kernels go to their tensors' GPU and its
+    current stream, and on the stream of another that is current nothing would be captured."""
+    with torch.cuda.device(device):
+        side = torch.cuda.Stream(device)
+        side.wait_stream(torch.cuda.current_stream(device))
+        with torch.cuda.stream(side):
+            warm_up()
+        torch.cuda.current_stream(device).wait_stream(side)
+        with torch.cuda.graph(graph, stream=side):
+            yield
+
+
 class Captured:
     """``Decoder.step`` as a CUDA graph; calling it with a plan of the captured shape runs that step."""
 
@@ -278,13 +293,8 @@ class Captured:
         # The workspace has to exist before the capture: one step without any page, which writes
         # nothing and attends to nothing.
         self.plan.page_table.fill_(-1)
-        side = torch.cuda.Stream(self.h.device)
-        side.wait_stream(torch.cuda.current_stream(self.h.device))
-        with torch.cuda.stream(side):
-            dec.step(self.h, self.plan)
-        torch.cuda.current_stream(self.h.device).wait_stream(side)
         self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
+        with _capture(self.graph, self.h.device, lambda: dec.step(self.h, self.plan)):
             self.out = dec.step(self.h, self.plan)
 
     def __call__(self, h: torch.Tensor, plan: Plan) -> torch.Tensor:
@@ -319,13 +329,8 @@ class CapturedSteps:
         i = dict(dtype=torch.int32, device=dev)
         empty = Plan(torch.full((B, pages.state.columns), -1, **i), torch.zeros(B, **i), torch.zeros(B + 1, **i), T, max_q_len,
                      torch.zeros(pages.axes, T, **i) if pages.rotary else None)
-        side = torch.cuda.Stream(dev)
-        side.wait_stream(torch.cuda.current_stream(dev))
-        with torch.cuda.stream(side):
-            dec.step(self.h, empty)
-        torch.cuda.current_stream(dev).wait_stream(side)
         self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
+        with _capture(self.graph, dev, lambda: dec.step(self.h, empty)):
             self.plan = pages.plan(self.rows, self.counts, T, max_q_len, self.images)
             self.out = dec.step(self.h, self.plan)
 
